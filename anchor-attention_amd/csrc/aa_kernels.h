@@ -134,4 +134,48 @@ bool select_scores_sums(int batch, int n_q_heads, int n_kv_heads, int n_ctx, int
 hipError_t launch_select_compact(const SelectArgs& a, hipStream_t stream);
 hipError_t launch_ratio(const int32_t* counts, int64_t n, float inverse, float* ratio, hipStream_t stream);
 
+// ---- key/value cache in pages (include/anchor_attn_hip.h) ----
+struct PagedAppendArgs {
+  const uint16_t* q; int64_t q_st, q_sh;
+  uint16_t* q_out; int64_t qo_st, qo_sh;
+  const uint16_t* k; int64_t k_st, k_sh;
+  const uint16_t* v; int64_t v_st, v_sh;
+  const float* cos; const float* sin; int64_t cs_sn; int n_positions;  // (both or neither)
+  uint16_t* keys; int64_t kp_sp, kp_sh, kp_sn;
+  uint16_t* values; int64_t vp_sp, vp_sh, vp_sn;
+  uint16_t* bounds;  // optional
+  const int32_t* table; int64_t t_sb;
+  const int32_t* lengths; const int32_t* starts;  // starts: optional
+  int batch, n_tokens, n_q_heads, n_kv_heads, head_dim, n_pages, page_log, max_pages;  // n_q_heads 0: no queries
+  int dtype;
+};
+hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t stream);
+
+struct PagedDecodeArgs {
+  const uint16_t* q; int64_t q_sb, q_sh;
+  uint16_t* out; int64_t o_sb, o_sh;
+  const uint16_t* keys; int64_t kp_sp, kp_sh, kp_sn;
+  const uint16_t* values; int64_t vp_sp, vp_sh, vp_sn;
+  const int32_t* table; int64_t t_sb, t_sh;  // the pages that are read; t_sh 0: the same for all KV heads
+  const int32_t* lengths;
+  int batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_log, max_pages;
+  int n_chosen;  // sparse: entries of a (sequence, KV head) in `table`, which hold the chosen pages; 0: all pages
+  float sm_scale;
+  int dtype;
+};
+hipError_t launch_paged_decode(const PagedDecodeArgs& a, hipStream_t stream);
+
+struct PagedSelectArgs {
+  const uint16_t* q; int64_t q_sb, q_sh;
+  const uint16_t* bounds;
+  const int32_t* table; int64_t t_sb;
+  const int32_t* lengths;
+  float* scores;    // [batch, n_kv_heads, max_pages]
+  int32_t* pages;   // [batch, n_kv_heads, n_chosen]: places in the sequence
+  int32_t* chosen;  // the same, as pages of the pool
+  int batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_log, max_pages, n_chosen, n_first, n_last;
+  int dtype;
+};
+hipError_t launch_paged_select(const PagedSelectArgs& a, hipStream_t stream);
+
 }  // namespace aa

@@ -1,0 +1,600 @@
+"""Appending to a key/value cache in pages and decode steps that read it, whole or sparsely, against plain float64 implementations, at the
+lengths, pages and layouts where tiles, pages and shares of the work end.
+
+Tolerances.  u is half a step of the 16-bit type relative to a value (2^-8 for bf16, 2^-11 for fp16).
+Rotation: two products and a sum in float32 are off by at most 2^-23 of the products' magnitudes, the rounding by u of the result
+(half a step of the subnormals, 2^-25, for fp16).  Bounds are those of the stored keys and have no error.
+Attention: a score is a float32 sum of D exact products, off by at most D * 2^-24 * sum |q_d k_d| and twice in a quotient; with its scaling and exp2
+(arguments up to 2^8, 2^-24 of them, and an ulp of exp2 or two) a probability is off by 2 * D * 2^-24 * sum |q_d k_d| * scale + 2^-14 of it.  It is kept as two 16-bit numbers,
+off by u^2 (fp16: its grid of 2^-39 too, covered by 2^-14); sums over n keys in float32 add n * 2^-24.  All of that is relative to sum p |v| / sum p; the
+result is rounded once, u of it.  The chosen pages have to be the same."""
+import ctypes
+import types
+
+import pytest
+import torch
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def _ops():
+    from anchor_attn.src.ops import paged_cache
+    return paged_cache
+
+
+def _tables(n, d, base=1e4):
+    angle = torch.arange(n, dtype=torch.float64)[:, None] * base ** (-torch.arange(0, d, 2, dtype=torch.float64) / d)
+    return angle.cos().float().cuda(), angle.sin().float().cuda()
+
+
+def _pool(n_pages, hkv, page, d, dtype, g, layout):
+    """Pool memory in one of three layouts, the rows of its pages contiguous in each."""
+    if layout == "heads":  # [pages, KV heads, rows, D]
+        return torch.randn(n_pages, hkv, page, d, generator=g, device="cuda").to(dtype)
+    if layout == "rows":  # [pages, rows, KV heads, D]
+        return torch.randn(n_pages, page, hkv, d, generator=g, device="cuda").to(dtype).transpose(1, 2)
+    wide = torch.randn(n_pages, hkv + 1, page + 3, d + 8, generator=g, device="cuda").to(dtype)  # a part of something larger
+    return wide[:, 1:, 2:2 + page, 8:]
+
+
+class _Setup:
+    """A cache with keys of ``lengths`` in pages in random order; NaN where no sequence has a key; bounds of what is there."""
+
+    def __init__(self, lengths, hkv, d, page, dtype, seed, layout="heads", room=0, extra=0):
+        self.g = g = torch.Generator(device="cuda").manual_seed(seed)
+        self.page, self.d, self.hkv, self.dtype, self.host = page, d, hkv, dtype, list(lengths)
+        counts = [(n + room + page - 1) // page for n in lengths]
+        total = sum(counts) + 3
+        keys, values = (_pool(total, hkv, page, d, dtype, g, layout) for _ in range(2))
+        order = torch.randperm(total, generator=g, device="cuda").int()
+        self.table = torch.full((len(lengths), max(1, max(counts, default=1)) + extra), -1, dtype=torch.int32, device="cuda")
+        self.table[:, 1::2] = 2 ** 31 - 1  # (what is behind a sequence's pages does not matter)
+        used = torch.zeros(total, dtype=torch.int64, device="cuda")
+        begin = 0
+        for b, (n, c) in enumerate(zip(lengths, counts)):
+            mine = order[begin:begin + c]
+            self.table[b, :c] = mine
+            used[mine.long()] = (n - page * torch.arange(c, device="cuda")).clamp(0, page)
+            begin += c
+        there = (torch.arange(page, device="cuda") < used[:, None])[:, None, :, None]
+        keys.masked_fill_(~there, float("nan"))
+        values.masked_fill_(~there, float("nan"))
+        lo = torch.where(there, keys, float("inf")).amin(2)
+        hi = torch.where(there, keys, float("-inf")).amax(2)
+        bounds = torch.stack((lo, hi), 2).masked_fill((used == 0)[:, None, None, None], float("nan")).contiguous()
+        self.cache = _ops().PagedCache(keys, values, bounds)
+        self.lengths = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+
+    def rows(self, pool, b, h, pages=None):
+        """Keys or values of a sequence and KV head in order, float64 (of some pages, counted in the sequence)."""
+        n = self.host[b]
+        there = (n + self.page - 1) // self.page
+        pages = torch.arange(there, device="cuda") if pages is None else pages
+        last = there - 1
+        x = pool[self.table[b, pages].long(), h].reshape(-1, self.d)
+        return x[:x.shape[0] - (there * self.page - n)].double() if last >= 0 else x[:0].double()
+
+    def queries(self, hq, spread=3.0):
+        return (spread * torch.randn(len(self.host), hq, self.d, generator=self.g, device="cuda")).to(self.dtype)
+
+
+def _close(out, q, s, scale, pages=None):
+    dtype, d = out.dtype, s.d
+    group = q.shape[1] // s.hkv
+    for b in range(q.shape[0]):
+        for h in range(s.hkv):
+            got = out[b, h * group:(h + 1) * group].double()
+            if s.host[b] == 0:
+                assert bool((got == 0).all())
+                continue
+            mine = None if pages is None else pages[b, h][pages[b, h] >= 0].long()
+            k, v = s.rows(s.cache.keys, b, h, mine), s.rows(s.cache.values, b, h, mine)
+            x = q[b, h * group:(h + 1) * group].double()
+            p = (x @ k.T * scale).softmax(-1)
+            want = p @ v
+            magnitude = (x.abs() @ k.abs().T).amax(-1, keepdim=True) * scale
+            relative = 2.0 * d * 2.0 ** -24 * magnitude + 2.0 ** -14 + U[dtype] ** 2 + k.shape[0] * 2.0 ** -24
+            bound = U[dtype] * want.abs() * 1.001 + relative * (p @ v.abs()) + 2.0 ** -25
+            err = (got - want).abs()
+            assert bool((err <= bound).all()), (b, h, float((err - bound).max()), float(err.max()))
+
+
+def _chosen(q, s, n_pages, n_first, n_last):
+    """The pages by their definition: scores in float64, rounded to float32, sorted on the host."""
+    group = q.shape[1] // s.hkv
+    got = torch.full((q.shape[0], s.hkv, n_pages), -1, dtype=torch.int32)
+    for b in range(q.shape[0]):
+        there = (s.host[b] + s.page - 1) // s.page
+        at = s.table[b, :there].long()
+        for h in range(s.hkv):
+            if there <= n_pages:
+                got[b, h, :there] = torch.arange(there, dtype=torch.int32)
+                continue
+            lo, hi = s.cache.bounds[at, h].double().unbind(1)
+            x = q[b, h * group:(h + 1) * group, None].double()
+            score = torch.where(x >= 0, x * hi, x * lo).sum(-1).amax(0).float().tolist()
+            score = [float("inf") if x != x else x for x in score]
+            ends = set(range(n_first)) | set(range(there - n_last, there))
+            rank = sorted((i for i in range(there) if i not in ends), key=lambda i: (-score[i], i))
+            got[b, h] = torch.tensor(sorted(ends | set(rank[:n_pages - len(ends)])), dtype=torch.int32)
+    return got.cuda()
+
+
+def _rotated(x, cos, sin):
+    """Float64 rotation of ``[tokens, heads, D]`` by rows of the tables, and the magnitude that errors are relative to."""
+    half = x.shape[-1] // 2
+    a, b, c, s = x[..., :half].double(), x[..., half:].double(), cos.double()[:, None], sin.double()[:, None]
+    return torch.cat((a * c - b * s, b * c + a * s), -1), torch.cat(((a * c).abs() + (b * s).abs(), (b * c).abs() + (a * s).abs()), -1)
+
+
+def _rounded(got, want, magnitude):
+    err = (got.double() - want).abs()
+    bound = U[got.dtype] * want.abs() * 1.001 + 2.0 ** -23 * magnitude + 2.0 ** -25
+    assert bool((err <= bound).all()), float((err - bound).max())
+
+
+# ---- appending -----------------------------------------------------------------------------------------------------
+
+def _append_and_check(before, new, hq, hkv, d, page, dtype, layout, steps=False, padding=0, seed=0, bounds=True):
+    ops = _ops()
+    s = _Setup(before, hkv, d, page, dtype, seed, layout, room=max(new))
+    n = sum(new)
+    parts = (torch.randn(n + padding, hq + 2 * hkv, d, generator=s.g, device="cuda") * 2).to(dtype)
+    q, k, v = parts.split((hq, hkv, hkv), 1)
+    lengths = [a + b for a, b in zip(before, new)]
+    cos, sin = _tables(max(lengths) + 1, d)
+    starts = [sum(new[:b]) for b in range(len(new) + 1)]
+    cache = s.cache if bounds else ops.PagedCache(s.cache.keys, s.cache.values)
+    keys, values, old = s.cache.keys.clone(), s.cache.values.clone(), s.cache.bounds.clone()
+    out = torch.full((n + padding, hq, d), 7.0, dtype=dtype, device="cuda")
+    got = ops.append_to_pages(cache, q, k, v, cos, sin, s.table, torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+                              None if steps else torch.tensor(starts, dtype=torch.int32, device="cuda"), out=out)
+    assert got is out and bool((out[n:] == 7.0).all())
+    positions = torch.tensor([p for a, b in zip(before, new) for p in range(a, a + b)], device="cuda")
+    sequence = torch.tensor([i for i, b in enumerate(new) for _ in range(b)], device="cuda")
+    if n:
+        _rounded(out[:n], *_rotated(q[:n], cos[positions], sin[positions]))
+        at, slot = s.table[sequence, positions // page].long(), positions % page
+        stored = s.cache.keys[at, :, slot]
+        _rounded(stored, *_rotated(k[:n], cos[positions], sin[positions]))
+        assert torch.equal(s.cache.values[at, :, slot], v[:n])
+        keys[at, :, slot], values[at, :, slot] = stored, v[:n]
+    # nothing else has changed
+    for x, y in ((s.cache.keys, keys), (s.cache.values, values)):
+        assert torch.equal(x.isnan(), y.isnan()) and torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0))
+    if bounds:
+        for b, (a, c) in enumerate(zip(before, new)):
+            for i in range(a // page, (a + c + page - 1) // page if c else 0):
+                page_keys = s.cache.keys[int(s.table[b, i]), :, :min(page, a + c - i * page)]
+                old[int(s.table[b, i])] = torch.stack((page_keys.amin(1), page_keys.amax(1)), 1)
+    assert torch.equal(s.cache.bounds.nan_to_num(9.0), old.nan_to_num(9.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("before,new,hq,hkv,d,page,layout,padding", [
+    ([0], [1], 32, 8, 128, 64, "heads", 0),
+    ([0, 63, 64, 17], [130, 1, 64, 0], 28, 4, 128, 64, "rows", 5),
+    ([5, 0, 31, 100], [1, 33, 2, 300], 14, 2, 64, 16, "heads", 0),
+    ([0, 1, 255, 256], [257, 600, 1, 255], 8, 8, 128, 256, "part", 0),
+    ([0] * 70, [3] * 69 + [40], 4, 1, 64, 32, "heads", 70),
+    ([7, 128], [0, 0], 4, 2, 128, 128, "heads", 3),
+    ([300] * 3, [517, 1, 90], 71, 1, 64, 128, "part", 1),
+])
+def test_append(before, new, hq, hkv, d, page, layout, padding, dtype):
+    _append_and_check(before, new, hq, hkv, d, page, dtype, layout, padding=padding, seed=len(before))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,hq,hkv,d,page,bounds", [(1, 32, 8, 128, 64, True), (97, 28, 4, 128, 16, True), (33, 32, 8, 64, 256, False), (300, 14, 2, 64, 32, True)])
+def test_append_one_token_each(batch, hq, hkv, d, page, bounds):
+    _append_and_check([(37 * b) % 211 for b in range(batch)], [1] * batch, hq, hkv, d, page, BF16, "heads", steps=True, seed=batch, bounds=bounds)
+
+
+@pytest.mark.gpu
+def test_append_without_rotation_and_in_place():
+    ops = _ops()
+    s = _Setup([3, 40], 2, 64, 16, BF16, 4, room=9)
+    k, v, q = (torch.randn(18, h, 64, generator=s.g, device="cuda").to(BF16) for h in (2, 2, 6))
+    starts, lengths = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 9, 18], [12, 49]))
+    assert ops.append_to_pages(s.cache, None, k, v, None, None, s.table, lengths, starts) is None
+    s.host = [12, 49]
+    for b in range(2):
+        for h in range(2):
+            assert torch.equal(s.rows(s.cache.keys, b, h)[-9:], k[9 * b:9 * b + 9, h].double())
+            assert torch.equal(s.rows(s.cache.values, b, h)[-9:], v[9 * b:9 * b + 9, h].double())
+    cos, sin = _tables(64, 64)
+    want = ops.append_to_pages(s.cache, q, k, v, cos, sin, s.table, lengths, starts)
+    keys = s.cache.keys.clone()
+    assert ops.append_to_pages(s.cache, q, k, v, cos, sin, s.table, lengths, starts, out=q) is q
+    assert torch.equal(q, want) and torch.equal(keys.nan_to_num(9.0), s.cache.keys.nan_to_num(9.0))
+
+
+@pytest.mark.gpu
+def test_tokens_without_a_place_are_left_out():
+    """A length of 0, positions below 0 and behind the angles, the table or the pool's pages, starts beyond the tokens."""
+    ops = _ops()
+    s = _Setup([0] * 6, 2, 64, 16, BF16, 5, room=40)
+    keys, values, bounds = s.cache.keys.clone(), s.cache.values.clone(), s.cache.bounds.clone()
+    q, k, v = (torch.randn(6, h, 64, generator=s.g, device="cuda").to(BF16) for h in (4, 2, 2))
+    cos, sin = _tables(40, 64)
+    s.table[3, 0], s.table[4, 0] = -1, s.cache.n_pages
+    lengths = torch.tensor([0, 41, 1000, 5, 5, -7], dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 7.0)
+    ops.append_to_pages(s.cache, q, k, v, cos, sin, s.table, lengths, out=out)
+    assert bool((out == 7.0).all())
+    # one sequence of six tokens whose length is 2: the first four have positions below 0; and one whose tokens end behind the last
+    for begins, n, placed in (([0, 6, 6, 6, 6, 6, 6], 2, [4, 5]), ([6, 6, 6, 6, 6, 6, 6], 2, []), ([0, 3, 2 ** 31 - 1, 6, 6, 6, 6], 3, [0, 1, 2])):
+        for x, y in ((s.cache.keys, keys), (s.cache.values, values), (s.cache.bounds, bounds)):
+            x.copy_(y)
+        lengths = torch.tensor([n] + [0] * 5, dtype=torch.int32, device="cuda")
+        out = ops.append_to_pages(s.cache, q, k, v, cos, sin, s.table, lengths, torch.tensor(begins, dtype=torch.int32, device="cuda"), out=torch.full_like(q, 7.0))
+        assert [i for i in range(6) if bool((out[i] != 7.0).any())] == placed
+        assert int((~s.cache.keys.isnan()).sum()) == len(placed) * 2 * 64 == int((~s.cache.values.isnan()).sum())
+
+
+@pytest.mark.gpu
+def test_bounds_of_infinite_and_nan_keys():
+    ops = _ops()
+    s = _Setup([0], 1, 64, 16, F16, 6, room=32)
+    k = torch.randn(20, 1, 64, generator=s.g, device="cuda").to(F16)
+    k[3, 0, 5], k[4, 0, 6], k[5, 0, 7], k[17, 0, 8], k[18, 0, 9] = float("nan"), float("inf"), float("-inf"), float("nan"), 65504.0
+    starts = torch.tensor([0, 17], dtype=torch.int32, device="cuda")
+    for lo, hi, length in ((0, 17, 17), (17, 20, 20)):
+        ops.append_to_pages(s.cache, None, k[lo:hi], k[lo:hi], None, None, s.table, torch.tensor([length], dtype=torch.int32, device="cuda"),
+                            torch.tensor([0, hi - lo], dtype=torch.int32, device="cuda"))
+    del starts
+    for i, rows in enumerate((k[:16, 0], k[16:, 0])):
+        got = s.cache.bounds[int(s.table[0, i]), 0]
+        want = torch.stack((rows.amin(0), rows.amax(0)))  # (the framework's minimum of NaN is NaN)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(9.0), want.nan_to_num(9.0))
+
+
+# ---- reading -------------------------------------------------------------------------------------------------------
+
+LENGTHS = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129, 255, 257, 500, 1023]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lengths,hq,hkv,d,page,layout", [
+    (LENGTHS, 32, 8, 128, 64, "heads"), (LENGTHS, 28, 4, 128, 16, "rows"), (LENGTHS, 14, 2, 64, 16, "heads"), (LENGTHS, 32, 8, 64, 32, "part"),
+    (LENGTHS, 3, 3, 128, 256, "heads"), ([700, 1, 33], 16, 1, 64, 128, "heads"), ([700, 1, 33], 17, 1, 128, 128, "rows"), ([900, 0], 71, 1, 64, 64, "heads"),
+    ([20001], 32, 8, 128, 64, "heads"), ([9000, 40, 12345], 28, 4, 64, 16, "heads"), ([5], 14, 2, 64, 16, "heads"), ([0], 4, 2, 128, 16, "heads"),
+    ([70001], 8, 1, 128, 256, "rows"), ([1] * 300, 14, 2, 64, 16, "heads"), ([33, 7] * 500, 4, 1, 128, 32, "heads"), ([4097] + [3] * 63, 8, 2, 128, 64, "heads"),
+])
+def test_decode(lengths, hq, hkv, d, page, layout, dtype):
+    s = _Setup(lengths, hkv, d, page, dtype, hq + page, layout, extra=hq % 3)
+    q = s.queries(hq)
+    wide = torch.full((len(lengths), hq + 1, d + 8), 7.0, dtype=dtype, device="cuda")
+    out = wide[:, 1:, 8:]
+    assert _ops().paged_decode_attention(s.cache, q, s.table, s.lengths, out=out) is out
+    assert bool((wide[:, 0] == 7.0).all()) and bool((wide[:, :, :8] == 7.0).all())
+    _close(out, q, s, d ** -0.5)
+    again = _ops().paged_decode_attention(s.cache, q.transpose(0, 1).contiguous().transpose(0, 1), s.table, s.lengths, sm_scale=d ** -0.5)
+    assert torch.equal(out, again)  # the same bits
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_decode_with_an_attention_sink_and_a_scale(dtype):
+    """One key far above the others, whose probabilities lie on the 16-bit types' lowest grid."""
+    s = _Setup([6000, 300], 2, 128, 64, dtype, 3)
+    q = s.queries(8, 1.0)
+    q[:, :, 0] = 8.0
+    for b in range(2):
+        s.cache.keys[s.table[b, 0].long(), :, 0, 0] = 16.0
+    for scale in (0.088, 0.01, 1.0):
+        _close(_ops().paged_decode_attention(s.cache, q, s.table, s.lengths, sm_scale=scale), q, s, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("length,d", [(40, 128), (5000, 64)])
+def test_decode_with_infinite_and_nan_values_that_are_seen(length, d, dtype):
+    """An infinite value gives an infinity in its channel, NaN gives NaN, and the other channels stay as they are."""
+    s = _Setup([length], 2, d, 16, dtype, 8)
+    q = s.queries(8, 0.3)
+    want = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
+    at = s.table[0, 1].long()
+    s.cache.values[at, 0, 3, 5], s.cache.values[at, 0, 4, 6], s.cache.values[at, 0, 9, 7] = float("inf"), float("-inf"), float("nan")
+    s.cache.values[at, 0, 3, 8], s.cache.values[at, 0, 4, 8] = float("inf"), float("-inf")
+    got = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
+    assert bool((got[0, :4, 5] == float("inf")).all()) and bool((got[0, :4, 6] == float("-inf")).all()) and bool(got[0, :4, 7:9].isnan().all())
+    assert torch.equal(got[0, 4:], want[0, 4:])
+    rest = torch.ones(d, dtype=torch.bool, device="cuda")
+    rest[5:9] = False
+    assert bool(((got[0, :4, rest] - want[0, :4, rest]).abs() <= 2 * U[dtype] * want[0, :4, rest].abs() + 2.0 ** -13).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["nan", "inf"])
+def test_decode_with_nan_and_infinite_keys(what):
+    """A NaN score, or one of plus infinity, makes its heads NaN, as a soft-max in float32 has it, and no others; minus infinity leaves the key out."""
+    s = _Setup([100, 100], 2, 64, 16, BF16, 9)
+    q = s.queries(4, 0.5)
+    q[:, :, 0] = 1.0
+    want = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
+    s.cache.keys[s.table[0, 2].long(), 0, 1, 0] = float(what)
+    got = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
+    assert bool(got[0, :2].isnan().all()) and torch.equal(got[0, 2:], want[0, 2:]) and torch.equal(got[1], want[1])
+    s.cache.keys[s.table[0, 2].long(), 0, 1, 0] = float("-inf")
+    got = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
+    assert bool(got.isfinite().all()) and torch.equal(got[0, 2:], want[0, 2:])
+
+
+@pytest.mark.gpu
+def test_lengths_and_pages_that_do_not_fit_are_clamped():
+    """Lengths above the table are its size, pages outside the pool the nearest one; nothing else is read."""
+    s = _Setup([64, 64, 64], 2, 64, 16, BF16, 10)
+    q = s.queries(4)
+    want = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
+    lengths = torch.tensor([1000, 64, -3], dtype=torch.int32, device="cuda")
+    got = _ops().paged_decode_attention(s.cache, q, s.table, lengths)
+    assert torch.equal(got[:2], want[:2]) and bool((got[2] == 0).all())
+    table = s.table.clone()
+    s.cache.keys.nan_to_num_(0.5), s.cache.values.nan_to_num_(0.5), s.cache.bounds.nan_to_num_(0.5)
+    table[1, 2], table[1, 3] = -5, 2 ** 31 - 1
+    s.table[1, 2], s.table[1, 3] = 0, s.cache.n_pages - 1
+    assert torch.equal(_ops().paged_decode_attention(s.cache, q, table, lengths), _ops().paged_decode_attention(s.cache, q, s.table, lengths))
+    for a, b in zip(*(_ops().paged_sparse_decode_attention(s.cache, q, t, lengths, 3) for t in (table, s.table))):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_pools_beyond_four_gib(dtype):
+    ops = _ops()
+    n_pages = (9 << 30) // (8 * 64 * 128 * 2)
+    s = _Setup([200, 129], 8, 128, 64, dtype, 11)
+    small, table = s.cache, s.table.clone()
+    big = ops.PagedCache.empty(n_pages, 8, 64, 128, dtype)
+    place = n_pages - 1 - 7 * torch.arange(small.n_pages, device="cuda")
+    for a, b in ((big.keys, small.keys), (big.values, small.values), (big.bounds, small.bounds)):
+        a[place] = b
+    q = s.queries(32)
+    big_table = torch.where((table >= 0) & (table < small.n_pages), place[table.clamp(0, small.n_pages - 1).long()].int(), -1)
+    assert torch.equal(ops.paged_decode_attention(small, q, table, s.lengths), ops.paged_decode_attention(big, q, big_table, s.lengths))
+    for a, b in zip(ops.paged_sparse_decode_attention(small, q, table, s.lengths, 2), ops.paged_sparse_decode_attention(big, q, big_table, s.lengths, 2)):
+        assert torch.equal(a, b)
+    cos, sin = _tables(256, 128)
+    k, v = (torch.randn(2, 8, 128, device="cuda").to(dtype) for _ in range(2))
+    s.lengths.sub_(1)
+    for cache, t in ((small, table), (big, big_table)):
+        ops.append_to_pages(cache, q, k, v, cos, sin, t, s.lengths)
+    for a, b in ((big.keys, small.keys), (big.values, small.values), (big.bounds, small.bounds)):
+        assert torch.equal(a[place].nan_to_num(9.0), b.nan_to_num(9.0))
+
+
+# ---- sparse reading ------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lengths,hq,hkv,d,page,n_pages,n_first,n_last", [
+    (LENGTHS, 32, 8, 128, 16, 5, 1, 1), (LENGTHS, 28, 4, 64, 16, 8, 0, 3), ([1000, 999, 17], 14, 2, 64, 32, 6, 2, 4), ([1000, 0], 3, 3, 128, 256, 1, 0, 1),
+    ([20001], 32, 8, 128, 64, 33, 1, 2), ([60000, 3000], 8, 1, 64, 16, 200, 1, 2), ([2100], 14, 2, 64, 16, 32, 1, 2), ([800] * 40, 4, 2, 64, 16, 9, 1, 1),
+    ([5000, 70], 71, 1, 128, 32, 20, 1, 1), ([300, 40], 16, 1, 64, 64, 100, 1, 1), ([1 << 17], 4, 1, 64, 16, 500, 3, 3),
+])
+def test_sparse_decode(lengths, hq, hkv, d, page, n_pages, n_first, n_last, dtype):
+    s = _Setup(lengths, hkv, d, page, dtype, hq + n_pages, extra=1)
+    q = s.queries(hq)
+    out, pages = _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, n_pages, n_first, n_last)
+    assert torch.equal(pages, _chosen(q, s, n_pages, n_first, n_last))
+    _close(out, q, s, d ** -0.5, pages)
+
+
+@pytest.mark.gpu
+def test_equal_scores_go_to_the_lower_page():
+    for d, dtype, hkv, group in ((64, BF16, 2, 2), (128, F16, 1, 7)):
+        s = _Setup([16 * 100, 16 * 700], hkv, d, 16, dtype, 12)
+        s.cache.keys.copy_(torch.randn(d, generator=s.g, device="cuda").to(dtype).expand_as(s.cache.keys))
+        s.cache.bounds.copy_(s.cache.keys[:, :, :2])
+        # a few pages stand out, two of them alike
+        for i, f in ((50, 3.0), (20, 2.0), (70, 2.0), (30, 1.5)):
+            s.cache.bounds[s.table[:, i].long(), :, 1] = f * s.cache.bounds[0, 0, 1].abs().max() + 1
+        q = s.queries(hkv * group).abs()
+        for n in (3, 4, 5, 6, 7, 40):
+            got = _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, n, 1, 1)[1]
+            assert torch.equal(got, _chosen(q, s, n, 1, 1))
+
+
+@pytest.mark.gpu
+def test_scores_that_are_nan_or_infinite_come_first():
+    s = _Setup([16 * 60], 1, 64, 16, BF16, 13)
+    q = s.queries(2)
+    q[0, :, 1:4] = 1.0
+    at = s.table[0].long()
+    s.cache.bounds[at[40], 0, 1, 1], s.cache.bounds[at[30], 0, 0, 2], s.cache.bounds[at[20], 0, :, 3] = float("inf"), float("nan"), float("nan")
+    s.cache.bounds[at[10], 0, 1, 3] = float("-inf")
+    q[0, 1, 4] = -0.0
+    s.cache.bounds[at[:], 0, 0, 4] = float("-inf")  # (-0 is not below 0: the larger bound counts)
+    q[0, 0, 4] = 0.0
+    for n in (3, 4, 5, 30, 58, 59):
+        assert torch.equal(_ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, n, 1, 1)[1], _chosen(q, s, n, 1, 1))
+
+
+# ---- together ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+def test_a_prompt_and_decode_steps_together():
+    """A prompt through the prefill operator and into pages, then steps that append and attend; the same steps once more as one captured graph, with a
+    second graph in between that another cache's step was captured into.  Every step against float64 attention over what the cache holds."""
+    from anchor_attn.src.ops.anchor_attn_v4 import anchor_attn
+    ops = _ops()
+    n, hq, hkv, d, page, steps = 2048, 8, 2, 128, 64, 4
+    g = torch.Generator(device="cuda").manual_seed(21)
+    q, k, v = (torch.randn(1, n, h, d, generator=g, device="cuda").to(BF16) for h in (hq, hkv, hkv))
+    assert anchor_attn(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), return_computational_ratio=False).shape == (1, hq, n, d)
+    cos, sin = _tables(4096, d)
+
+    def begin():
+        s = _Setup([0, 0], hkv, d, page, BF16, 22, room=n + 200)
+        s.table[1, :20] = s.table[1, :20].flip(0)
+        prompt = torch.tensor([n, 129], dtype=torch.int32, device="cuda")
+        ops.append_to_pages(s.cache, None, torch.cat((k[0], k[0, :129])), torch.cat((v[0], v[0, :129])), None, None, s.table, prompt,
+                            torch.tensor([0, n, n + 129], dtype=torch.int32, device="cuda"))
+        s.lengths = prompt
+        return s
+
+    new = [tuple(torch.randn(2, h, d, generator=g, device="cuda").to(BF16) for h in (hq, hkv, hkv)) for _ in range(steps)]
+
+    def step(s, x):
+        s.lengths += 1
+        rotated = ops.append_to_pages(s.cache, *x, cos, sin, s.table, s.lengths)
+        return (rotated, ops.paged_decode_attention(s.cache, rotated, s.table, s.lengths), *ops.paged_sparse_decode_attention(s.cache, rotated, s.table, s.lengths, 8, 1, 2))
+
+    s, eager = begin(), []
+    for i, x in enumerate(new):
+        rotated, out, sparse, pages = step(s, x)
+        s.host = [n + i + 1, 129 + i + 1]
+        _close(out, rotated, s, d ** -0.5)
+        assert torch.equal(pages, _chosen(rotated, s, 8, 1, 2))
+        _close(sparse, rotated, s, d ** -0.5, pages)
+        eager.append([t.clone() for t in (rotated, out, sparse, pages)])
+
+    graphs = []
+    for _ in range(2):
+        s, x = begin(), tuple(t.clone() for t in new[0])
+        graph = torch.cuda.CUDAGraph()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(s, x)  # (warm-up; the lengths are set back)
+        torch.cuda.current_stream().wait_stream(side)
+        s.lengths -= 1
+        with torch.cuda.graph(graph):
+            outs = step(s, x)
+        graphs.append((s, x, graph, outs))
+    for i in range(steps):
+        for s, x, graph, outs in graphs:
+            for a, b in zip(x, new[i]):
+                a.copy_(b)
+            graph.replay()
+        step(begin(), new[0])  # (eager work between the replays)
+        torch.cuda.synchronize()
+        for _, _, _, outs in graphs:
+            for a, b in zip(outs, eager[i]):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    ops = _ops()
+    s = _Setup([3000, 5000, 100], 4, 128, 64, BF16, 31)
+    q = [s.queries(16) for _ in range(2)]
+    want = [(ops.paged_decode_attention(s.cache, x, s.table, s.lengths), *ops.paged_sparse_decode_attention(s.cache, x, s.table, s.lengths, 9)) for x in q]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append((ops.paged_decode_attention(s.cache, q[i], s.table, s.lengths), *ops.paged_sparse_decode_attention(s.cache, q[i], s.table, s.lengths, 9)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
+
+
+# ---- refusals ------------------------------------------------------------------------------------------------------
+
+APPEND = {"q": 4096, "q_st": 1024, "q_sh": 128, "q_out": 4096, "qo_st": 1024, "qo_sh": 128, "k": 4096, "k_st": 256, "k_sh": 128, "v": 4096, "v_st": 256, "v_sh": 128,
+          "cos": 4096, "sin": 4096, "cs_sn": 64, "n_positions": 100, "keys": 4096, "kp_sp": 4096, "kp_sh": 2048, "kp_sn": 128, "values": 4096, "vp_sp": 4096, "vp_sh": 2048,
+          "vp_sn": 128, "bounds": 4096, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "starts": 4096, "batch": 2, "n_tokens": 5, "n_q_heads": 8, "n_kv_heads": 2,
+          "head_dim": 128, "n_pages": 9, "page_size": 16, "max_pages": 8, "dtype": 0, "stream": None}
+DECODE = {"q": 4096, "q_sb": 1024, "q_sh": 128, "out": 4096, "o_sb": 1024, "o_sh": 128, "keys": 4096, "kp_sp": 4096, "kp_sh": 2048, "kp_sn": 128, "values": 4096, "vp_sp": 4096,
+          "vp_sh": 2048, "vp_sn": 128, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "workspace": 4096, "workspace_bytes": 1 << 40, "batch": 2, "n_q_heads": 8,
+          "n_kv_heads": 2, "head_dim": 128, "n_pages": 9, "page_size": 16, "max_pages": 8, "sm_scale": 0.1, "dtype": 0, "stream": None}
+SPARSE = {**{k: DECODE[k] for k in list(DECODE)[:14]}, "bounds": 4096, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "pages": 4096, "workspace": 4096,
+          "workspace_bytes": 1 << 40, **{k: DECODE[k] for k in list(DECODE)[19:26]}, "n_chosen": 4, "n_first": 1, "n_last": 1, "sm_scale": 0.1, "dtype": 0, "stream": None}
+CACHE = [({"batch": 0}, "must be positive"), ({"batch": 65536}, "not supported"), ({"n_kv_heads": 3}, "must divide"), ({"n_kv_heads": 0}, "must be positive"),
+         ({"head_dim": 96}, "head_dim 96"), ({"page_size": 48}, "page_size 48"), ({"page_size": 8}, "page_size 8"), ({"n_pages": 0}, "must be positive"),
+         ({"max_pages": 0}, "must be positive"), ({"max_pages": 65537}, "not supported"), ({"dtype": 2}, "dtype"), ({"keys": 0}, "keys is NULL"),
+         ({"keys": 4104}, "keys must be 16-byte aligned"), ({"kp_sh": 2052}, "keys must be 16-byte aligned"), ({"vp_sn": 120}, "smaller than head_dim"),
+         ({"vp_sn": 16392}, "larger than 16384"), ({"values": 0}, "values is NULL"), ({"page_table": 0}, "page_table is NULL"), ({"lengths": 0}, "lengths is NULL"),
+         ({"lengths": 4098}, "lengths must be 4-byte aligned"), ({"q": 4104}, "q must be 16-byte aligned"), ({"q_sh": 60}, "q must have strides")]
+READ = [({"q": 0}, "q is NULL"), ({"out": 0}, "out is NULL"), ({"out": 8}, "out must be 16-byte"), ({"sm_scale": 0.0}, "sm_scale"), ({"sm_scale": float("nan")}, "sm_scale"),
+        ({"sm_scale": float("inf")}, "sm_scale"), ({"n_q_heads": 0}, "query heads")]
+
+
+@pytest.mark.parametrize("fn,change,message", [
+    *[("append", c, m) for c, m in CACHE], *[("decode", c, m) for c, m in CACHE + READ], *[("sparse", c, m) for c, m in CACHE + READ],
+    ("append", {"n_tokens": 0}, "0 tokens"), ("append", {"n_tokens": 1 << 24}, "not supported"), ("append", {"starts": 0}, "5 tokens of 2 sequences"),
+    ("append", {"cos": 0}, "come together"), ("append", {"q": 0}, "come together"), ("append", {"q_out": 0}, "come together"), ("append", {"cos": 0, "sin": 0}, "come together"),
+    ("append", {"n_q_heads": 0}, "come together"), ("append", {"cs_sn": 63}, "cos and sin"), ("append", {"cs_sn": 60}, "cos and sin"), ("append", {"n_positions": 0}, "cos and sin"),
+    ("append", {"sin": 4100}, "sin must be 16-byte"), ("append", {"k": 0}, "k is NULL"), ("append", {"v": 4}, "v must be 16-byte"), ("append", {"v_st": 4}, "v must have strides"),
+    ("append", {"bounds": 8}, "bounds must be 16-byte"), ("append", {"starts": 6}, "starts must be 4-byte"),
+    ("sparse", {"n_last": 0}, "at least the last one"), ("sparse", {"n_first": -1}, "not supported"), ("sparse", {"n_first": 4}, "not supported"),
+    ("sparse", {"n_chosen": 65537}, "not supported"), ("sparse", {"n_chosen": 1}, "not supported"), ("sparse", {"bounds": 0}, "bounds is NULL"),
+    ("sparse", {"pages": 0}, "pages is NULL"), ("sparse", {"workspace_bytes": 100}, "workspace has 100 bytes"), ("sparse", {"workspace": 0}, "workspace is NULL"),
+])
+def test_what_the_c_interface_refuses(fn, change, message):
+    """Before anything is launched: the addresses are never read."""
+    from anchor_attn.src.ops import _hip
+    args, f = {"append": (APPEND, _hip.lib().aa_paged_append), "decode": (DECODE, _hip.lib().aa_paged_decode_fwd), "sparse": (SPARSE, _hip.lib().aa_paged_sparse_decode_fwd)}[fn]
+    assert len(args) == len(f.argtypes) and set(change) <= set(args)
+    with pytest.raises(_hip.AnchorAttnHipError, match=message):
+        _hip.check(f(*{**args, **change}.values()))
+
+
+def test_caches_that_are_refused():
+    from anchor_attn.src.ops import _hip
+    x = torch.zeros(3, 2, 16, 64, dtype=BF16)
+    with pytest.raises(_hip.AnchorAttnHipError, match="one GPU"):
+        _ops().PagedCache(x, x)
+    with pytest.raises(_hip.AnchorAttnHipError, match="must be a PagedCache"):
+        _ops().paged_decode_attention(types.SimpleNamespace(), x, x, x)
+
+
+@pytest.mark.gpu
+def test_what_the_entry_points_refuse():
+    from anchor_attn.src.ops import _hip
+    ops = _ops()
+    z = lambda *shape, dtype=BF16: torch.zeros(shape, dtype=dtype, device="cuda")  # noqa: E731
+    for keys, values, bounds in ((z(3, 2, 16, 64), z(3, 2, 16, 128), None), (z(3, 2, 24, 64), z(3, 2, 24, 64), None), (z(3, 2, 16, 96), z(3, 2, 16, 96), None),
+                                 (z(3, 2, 16, 64, dtype=torch.float32),) * 2 + (None,), (z(3, 2, 16, 64), z(3, 2, 16, 64, dtype=F16), None),
+                                 (z(3, 2, 16, 64), z(3, 2, 16, 64), z(3, 2, 2, 128)), (z(3, 2, 16, 64), z(3, 2, 16, 64), z(2, 3, 2, 64).transpose(0, 1)),
+                                 (z(3, 2, 16, 128)[..., ::2], z(3, 2, 16, 64), None), (z(3, 2, 16, 68)[..., 4:], z(3, 2, 16, 64), None), (z(0, 2, 16, 64),) * 2 + (None,),
+                                 (z(3, 2, 16, 64).requires_grad_(), z(3, 2, 16, 64), None), (z(1, 2, 1, 64).expand(3, 2, 16, 64), z(3, 2, 16, 64), None)):
+        with pytest.raises(_hip.AnchorAttnHipError):
+            ops.PagedCache(keys, values, bounds)
+    cache = ops.PagedCache.empty(5, 2, 16, 64)
+    table, lengths, starts = z(2, 3, dtype=torch.int32), z(2, dtype=torch.int32), z(3, dtype=torch.int32)
+    q, k, v, cos = z(2, 4, 64), z(2, 2, 64), z(2, 2, 64), z(50, 32, dtype=torch.float32)
+    good = {"cache": cache, "q": q, "page_table": table, "lengths": lengths}
+    more = {**good, "k": k, "v": v, "cos": cos, "sin": cos, "starts": starts}
+    reads = [{"q": z(2, 3, 64)}, {"q": z(3, 4, 64)}, {"q": z(2, 4, 128)}, {"q": z(2, 4, 64, dtype=F16)}, {"q": z(2, 64)}, {"q": z(2, 4, 128)[..., ::2]}, {"q": q.cpu()},
+             {"q": z(2, 4, 64).requires_grad_()}, {"page_table": table.long()}, {"page_table": table[0]}, {"page_table": z(3, 3, dtype=torch.int32)},
+             {"page_table": z(3, 2, dtype=torch.int32).T}, {"page_table": z(2, 0, dtype=torch.int32)}, {"page_table": z(2, 65537, dtype=torch.int32)}, {"lengths": lengths.long()},
+             {"lengths": z(4, dtype=torch.int32)[::2]}, {"lengths": lengths.cpu()}, {"out": z(2, 4, 128)}, {"out": z(2, 4, 64, dtype=F16)}, {"out": z(2, 4, 128)[..., ::2]}]
+    appends = [{"k": z(2, 4, 64)}, {"k": z(3, 2, 64)}, {"v": z(3, 2, 64)}, {"v": z(2, 1, 64)}, {"starts": z(2, dtype=torch.int32)}, {"starts": starts.long()}, {"cos": None},
+               {"cos": None, "sin": None}, {"cos": cos.double()}, {"cos": z(50, 64, dtype=torch.float32), "sin": z(50, 64, dtype=torch.float32)}, {"sin": z(49, 32, dtype=torch.float32)},
+               {"starts": None, "page_table": z(1, 3, dtype=torch.int32), "lengths": z(1, dtype=torch.int32)}, {"q": None, "out": z(2, 4, 64)}, {"k": k.clone().requires_grad_()}]
+    for fn, base, changes in ((ops.paged_decode_attention, good, reads + [{"sm_scale": -1.0}, {"sm_scale": float("inf")}]),
+                              (ops.paged_sparse_decode_attention, {**good, "n_pages": 2}, reads + [{"n_pages": 1}, {"n_last": 0}, {"n_first": -1}, {"n_pages": 65537}]),
+                              (ops.append_to_pages, more, reads + appends)):
+        fn(**base)
+        for change in changes:
+            with pytest.raises(_hip.AnchorAttnHipError):
+                fn(**{**base, **change})
+        with torch.no_grad():
+            fn(**{**base, "q": z(2, 4, 64).requires_grad_()})
+    with pytest.raises(_hip.AnchorAttnHipError, match="with bounds"):
+        ops.paged_sparse_decode_attention(ops.PagedCache(cache.keys, cache.values), q, table, lengths, 2)
+    with pytest.raises(_hip.AnchorAttnHipError, match="traced"):
+        torch.func.vmap(lambda x: ops.paged_decode_attention(cache, x, table, lengths))(q[None])
+    # nothing to do is no error
+    none = z(0, dtype=torch.int32)
+    assert ops.paged_decode_attention(cache, q[:0], table[:0], none).shape == (0, 4, 64)
+    assert ops.paged_sparse_decode_attention(cache, q[:0], table[:0], none, 2)[1].shape == (0, 2, 2)
+    assert ops.append_to_pages(cache, q[:0], k[:0], v[:0], cos, cos, table, lengths, starts).shape == (0, 4, 64)
+    torch.cuda.synchronize()
+
+
+def test_scratch_sizes():
+    from anchor_attn.src.ops import _hip
+    lib = _hip.lib()
+    assert lib.aa_paged_sparse_workspace_bytes(0, 8, 2, 128, 16, 8, 4) == 0
+    assert lib.aa_paged_sparse_workspace_bytes(2, 8, 2, 128, 16, 8, 4) >= 2 * 2 * (8 + 4) * 4
+    assert isinstance(lib.aa_paged_decode_workspace_bytes(2, 8, 2, 128, 16, 8), int) and ctypes.sizeof(ctypes.c_size_t) == 8
