@@ -944,7 +944,16 @@ int aa_paged_append(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int6
 }
 
 size_t aa_paged_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
-  return 0;
+  if (check_paged("aa_paged_decode_workspace_bytes", batch, n_q_heads, n_kv_heads, head_dim, 1, page_size, max_pages, AA_DTYPE_BF16)) return 0;
+  return paged_decode_scratch(head_dim, log2_of(page_size), max_pages).total;
+}
+// ... laid out at `workspace`
+static void give_scratch(PagedDecodeArgs& a, char* workspace, int max_pages) {
+  const PagedScratch s = paged_decode_scratch(a.head_dim, a.page_log, max_pages);
+  if (s.total == 0) return;
+  a.headers = (int32_t*)(workspace + s.headers);
+  a.part_stats = (float*)(workspace + s.stats);
+  a.parts = (float*)(workspace + s.parts);
 }
 
 static int paged_decode_args(const char* who, PagedDecodeArgs& a, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
@@ -968,7 +977,7 @@ static int paged_decode_args(const char* who, PagedDecodeArgs& a, const void* q,
     return AA_EBADARG;
   }
   a = {(const uint16_t*)q, q_sb, q_sh, (uint16_t*)out, o_sb, o_sh, (const uint16_t*)keys, kp_sp, kp_sh, kp_sn, (const uint16_t*)values, vp_sp, vp_sh, vp_sn,
-       page_table, pt_sb, 0, lengths, batch, n_q_heads, n_kv_heads, head_dim, n_pages, log2_of(page_size), max_pages, 0, sm_scale, dtype};
+       page_table, pt_sb, 0, lengths, batch, n_q_heads, n_kv_heads, head_dim, n_pages, log2_of(page_size), max_pages, 0, sm_scale, nullptr, nullptr, nullptr, dtype};
   return AA_OK;
 }
 
@@ -983,6 +992,7 @@ int aa_paged_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, void* out, in
   if (int rc = paged_decode_args(who, a, q, q_sb, q_sh, out, o_sb, o_sh, keys, kp_sp, kp_sh, kp_sn, values, vp_sp, vp_sh, vp_sn, page_table, pt_sb, lengths,
                                  workspace, workspace_bytes, needed, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, max_pages, sm_scale, dtype))
     return rc;
+  give_scratch(a, static_cast<char*>(workspace), max_pages);
   return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
 }
 
@@ -1031,6 +1041,7 @@ int aa_paged_sparse_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, void* 
   a.t_sb = (int64_t)n_kv_heads * n_chosen;
   a.t_sh = n_chosen;
   a.n_chosen = n_chosen;
+  give_scratch(a, ws + w.decode, n_chosen < max_pages ? n_chosen : max_pages);
   return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
 }
 

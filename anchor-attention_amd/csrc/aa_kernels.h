@@ -161,8 +161,14 @@ struct PagedDecodeArgs {
   int batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_log, max_pages;
   int n_chosen;  // sparse: entries of a (sequence, KV head) in `table`, which hold the chosen pages; 0: all pages
   float sm_scale;
+  // scratch (paged_decode_scratch), all or none: what the parts of cut units are, their maxima and sums, their accumulators
+  int32_t* headers; float* part_stats; float* parts;
   int dtype;
 };
+struct PagedScratch {
+  size_t headers, stats, parts, total;  // offsets in bytes
+};
+PagedScratch paged_decode_scratch(int head_dim, int page_log, int max_pages);
 hipError_t launch_paged_decode(const PagedDecodeArgs& a, hipStream_t stream);
 
 struct PagedSelectArgs {

@@ -1,81 +1,496 @@
 // Attention of one new token per sequence over a key/value cache in pages, on gfx950.
 //
-// Bound by reading keys and values once.  A work-group has one (sequence, query head) and takes 256 keys at a time: a thread's score each, then
-// a channel of the output each.
+// Bound by reading keys and values once.  A unit is a (sequence, KV head) with up to 16 heads of its group as the columns of 16 x 16 x 32 MFMAs; its
+// keys come in tiles of 32.  Lengths are known on the device only and may differ a lot, so the tiles of all units, one after the other, are cut into equal
+// shares, one for each of a fixed number of work-groups: every work-group sums the lengths and finds its share by itself.  A share that begins or ends
+// inside a unit leaves the state of its part (maximum, sum, accumulator) in the workspace, at most two of them, and paged_combine_kernel joins
+// the parts in order, so that results do not depend on timing.  Units of few tiles are never cut.
+//
+// The four waves of a work-group take a unit's tiles in turn and nothing passes through LDS until they are merged:
+//   S^T = K Q^T: a lane holds 8 channels of one key, the MFMA's own layout, straight from memory;
+//   O^T = V^T P^T: the order of keys inside a product is free, so P^T is S^T's registers as they lie (lane 16 g + c has keys 4 g + r and
+//   16 + 4 g + r of column c), and V^T wants 8 keys of one channel in a lane: a lane loads D / 16 channels of its 8 keys, whole rows
+//   by 16 lanes, and v_perm turns the block, one instruction per two elements.
+// P enters as two 16-bit numbers, its rounding and the rest, as in the other decode kernel.  The next tile's loads are in flight during a tile.
 #include "aa_kernels.h"
+#include "aa_nonfinite.h"
 #include "aa_paged.h"
 
 namespace aa {
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_decode_kernel(const PagedDecodeArgs p) {
-  constexpr int kParts = 256 / D;
-  __shared__ float q[D], prob[256], red[2][4], part[kParts][D];
-  const int tid = threadIdx.x, h = blockIdx.x, b = blockIdx.y;
-  const int kvh = h / (p.n_q_heads / p.n_kv_heads);
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(4))) const int32_t const_i32;
+
+constexpr int kCols = 16;       // columns of a unit: heads of the group
+constexpr int kTile = 32;       // keys of a tile
+constexpr int kWhole = 20;      // a unit of at most that many tiles is not cut
+constexpr int kShares = 512;    // work-groups
+constexpr int kSharesLog = 9;
+constexpr int kLeast = 4;       // tiles of a share
+
+template <typename T> __device__ __forceinline__ floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c);
+template <> __device__ __forceinline__ floatx4 mfma16<Bf16>(u32x4 a, u32x4 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&a), *reinterpret_cast<const bf16x8*>(&b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ floatx4 mfma16<F16>(u32x4 a, u32x4 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const f16x8*>(&a), *reinterpret_cast<const f16x8*>(&b), c, 0, 0, 0);
+}
+
+// max and sum over the lanes 16, 32 and 48 away, which hold the other keys of a column
+__device__ __forceinline__ float max_over_quarters(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return max_with_other_half(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_over_quarters(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// Rows of a page behind a wave-uniform address: a lane's loads then have an offset of 32 bits, and the address is scalar arithmetic.
+typedef __amdgpu_buffer_rsrc_t Rows;
+__device__ __forceinline__ Rows rows_at(const uint16_t* base, const bool there) {
+  const uint64_t u = (uint64_t)base;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)hi << 32 | lo), 0, there ? 0x7fffffff : 0, 0x00020000);
+}
+
+struct PagedPlace {  // of a tile, among all
+  int b, unit, tile, n_tiles;  // sequence, unit of it, tile of the unit, its tiles
+};
+
+__device__ __forceinline__ int tiles_of(const PagedDecodeArgs& p, const int b) {
   int length = clamped_length(p.lengths, b, p.max_pages, p.page_log);
-  const int left_out = p.n_chosen ? max(0, pages_of(length, p.page_log) - p.n_chosen) : 0;
-  length -= left_out << p.page_log;
-  const int32_t* table = p.table + b * p.t_sb + kvh * p.t_sh;
-  if (tid < D) q[tid] = T::from16(p.q[b * p.q_sb + h * p.q_sh + tid]);
-  __syncthreads();
-  const float scale = p.sm_scale * kLog2e;
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  const int d = tid % D, g = tid / D;
-  for (int base = 0; base < length; base += 256) {
-    const int key = base + tid;
-    float s = -INFINITY;
-    if (key < length) {
-      const uint16_t* k = p.keys + clamped_page(table[key >> p.page_log], p.n_pages) * p.kp_sp + kvh * p.kp_sh + (key & ((1 << p.page_log) - 1)) * p.kp_sn;
-      s = 0.f;
-      for (int i = 0; i < D; i += 8) {
-        float x[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(k + i), x);
+  if (p.n_chosen) length -= max(0, pages_of(length, p.page_log) - p.n_chosen) << p.page_log;
+  return max(1, (length + kTile - 1) / kTile);  // (one of no keys has to be written too)
+}
+
+template <typename T, int D, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const PagedDecodeArgs p) {
+  constexpr int kKS = D / 32;      // MFMAs of a score
+  constexpr int kDV = D / 16;      // channels of V that a lane loads
+  constexpr int kVW = kDV / 2;     // ... in words
+  constexpr int kPitch = D + 4;
+  __shared__ __attribute__((aligned(16))) float accs[WAVES][kCols][kPitch];
+  __shared__ float stats[2][WAVES][kCols];
+
+  const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = p.n_q_heads / p.n_kv_heads, col_blocks = (group + kCols - 1) / kCols, units = p.n_kv_heads * col_blocks;
+
+  // ---- this work-group's share -------------------------------------------------------------------
+  int64_t total = 0;
+  for (int i = 0; i < p.batch; i += 64) {
+    int n = i + lane < p.batch ? tiles_of(p, i + lane) : 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s = __builtin_fmaf(q[i + j], x[j], s);
+    for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d, 64);
+    total += __builtin_amdgcn_readfirstlane(n);
+  }
+  total *= units;
+  int64_t share = (total + kShares - 1) >> kSharesLog;
+  share = share < kLeast ? kLeast : share;
+  int64_t at = share * blockIdx.x, end = min(at + share, total);
+  // a place among all tiles; one inside a unit that is not cut is its beginning
+  auto find = [&](const int64_t x, int64_t& snapped) {
+    PagedPlace f = {p.batch, 0, 0, 1};
+    int64_t before = 0;
+    snapped = total;
+    for (int i = 0; i < p.batch; i += 64) {
+      const int n = i + lane < p.batch ? tiles_of(p, i + lane) : 0;
+      int sum = n;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(sum, d, 64);
+        if (lane >= d) sum += y;
+      }
+      const int in = __popcll(__ballot((before + sum) * units <= x));  // sequences of these 64 that end at or before x
+      if (in < 64 && i + in < p.batch) {
+        f.b = i + in;
+        f.n_tiles = __builtin_amdgcn_readlane(n, in);
+        const uint32_t rest = (uint32_t)(x - (before + __builtin_amdgcn_readlane(sum - n, in)) * units);
+        f.unit = rest / (uint32_t)f.n_tiles;
+        f.tile = rest - f.unit * f.n_tiles;
+        snapped = x;
+        if (f.n_tiles <= kWhole) {
+          snapped -= f.tile;
+          f.tile = 0;
+        }
+        break;
+      }
+      before += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return f;
+  };
+  int32_t* header = p.headers + 4 * blockIdx.x;
+  bool cut = false;
+  PagedPlace f = {0, 0, 0, 1};
+  if (at < total) {
+    if (end < total) find(end, end);
+    f = find(at, at);
+  }
+
+  const float scale = p.sm_scale * kLog2e;
+  const uint32_t k_lane = (2u * (c16 * (uint32_t)p.kp_sn + 8 * g)) & 0xfffffu, v_lane = (2u * (4 * g * (uint32_t)p.vp_sn + kDV * c16)) & 0xfffffu;
+  // what finds the tiles of a unit
+  struct Unit {
+    const_i32* table;
+    int64_t k_head, v_head;
+    int length, last_page, kvh, head0, n_cols;
+  };
+  auto unit_of = [&](const PagedPlace& f) __attribute__((always_inline)) {
+    Unit u;
+    u.kvh = f.unit / col_blocks;
+    u.head0 = u.kvh * group + (f.unit - u.kvh * col_blocks) * kCols;
+    u.n_cols = min(kCols, (u.kvh + 1) * group - u.head0);
+    u.length = __builtin_amdgcn_readfirstlane(clamped_length(p.lengths, f.b, p.max_pages, p.page_log));
+    if (p.n_chosen) u.length -= max(0, pages_of(u.length, p.page_log) - p.n_chosen) << p.page_log;
+    u.last_page = max(0, (u.length - 1) >> p.page_log);
+    u.table = (const_i32*)(p.table + f.b * p.t_sb + u.kvh * p.t_sh);
+    u.k_head = u.kvh * p.kp_sh;
+    u.v_head = u.kvh * p.vp_sh;
+    return u;
+  };
+  struct Tile {
+    u32x4 k[2][kKS];
+    uint32_t v[8][kVW];
+  };
+  // Where a tile lies: the first rows of its two halves.  (16 keys lie in one page; those behind the last page repeat its rows; of a tile
+  // that is not there nothing is read)
+  struct Spot {
+    int64_t k[2], v[2];
+    bool there;
+  };
+  auto spot = [&](const Unit& u, const int t, const bool there) __attribute__((always_inline)) {
+    Spot o;
+    o.there = there;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int key = kTile * t + 16 * half, row = key & ((1 << p.page_log) - 1);
+      const int64_t page = clamped_page(u.table[min(key >> p.page_log, u.last_page)], p.n_pages);
+      o.k[half] = page * p.kp_sp + row * p.kp_sn + u.k_head;
+      o.v[half] = page * p.vp_sp + row * p.vp_sn + u.v_head;
+    }
+    return o;
+  };
+  auto load_k = [&](Tile& x, const Spot& o) __attribute__((always_inline)) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const Rows kr = rows_at(p.keys + o.k[half], o.there);
+#pragma unroll
+      for (int s = 0; s < kKS; ++s) x.k[half][s] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_lane + 64 * s, 0, 0);
+    }
+  };
+  auto load_v = [&](Tile& x, const Spot& o) __attribute__((always_inline)) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const Rows vr = rows_at(p.values + o.v[half], o.there);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (kVW == 4) *reinterpret_cast<u32x4*>(x.v[4 * half + r]) = __builtin_amdgcn_raw_buffer_load_b128(vr, v_lane, 2 * r * (uint32_t)p.vp_sn, 0);
+        else *reinterpret_cast<u32x2*>(x.v[4 * half + r]) = __builtin_amdgcn_raw_buffer_load_b64(vr, v_lane, 2 * r * (uint32_t)p.vp_sn, 0);
       }
     }
-    float mx = s;
+  };
+  u32x4 q[kKS], q2[kKS];
+  auto load_q = [&](u32x4 (&q)[kKS], const PagedPlace& f, const Unit& u) __attribute__((always_inline)) {
+    const uint16_t* qp = p.q + f.b * p.q_sb + (int64_t)(u.head0 + min(c16, u.n_cols - 1)) * p.q_sh + 8 * g;
 #pragma unroll
-    for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
-    if ((tid & 63) == 0) red[0][tid >> 6] = mx;
-    __syncthreads();
-    const float m_new = fmaxf(m, fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])));
-    const float m_base = m_new == -INFINITY ? 0.f : m_new;
-    const float e = key < length ? fast_exp2((s - m_base) * scale) : 0.f;
-    prob[tid] = e;
-    float sum = e;
+    for (int s = 0; s < kKS; ++s) q[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s);
+  };
+
+  Tile x;
+  Unit u = {};
+  if (at < end) {
+    u = unit_of(f);
+    load_q(q2, f, u);
+    __builtin_amdgcn_sched_barrier(0);
+    const int t = f.tile + wave;
+    const Spot o = spot(u, t, t < min((int64_t)f.n_tiles, f.tile + (end - at)));
+    load_k(x, o);
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(x, o);
+  }
+  while (at < end) {
+    // ---- a unit's tiles [f.tile, last), and what comes after it -------------------------------------
+    const int last = (int)min((int64_t)f.n_tiles, f.tile + (end - at));
+    const int64_t at2 = at + (last - f.tile);
+    PagedPlace f2 = f;
+    Unit u2 = u;
+    int last2 = 0;
+    if (at2 < end) {
+      f2.tile = 0;
+      if (++f2.unit == units) {
+        f2.unit = 0;
+        ++f2.b;
+        f2.n_tiles = __builtin_amdgcn_readfirstlane(tiles_of(p, f2.b));
+      }
+      u2 = unit_of(f2);
+      last2 = (int)min((int64_t)f2.n_tiles, end - at2);
+    }
 #pragma unroll
-    for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
-    if ((tid & 63) == 0) red[1][tid >> 6] = sum;
-    __syncthreads();
-    const float alpha = fast_exp2((m - m_base) * scale);
-    l = l * alpha + ((red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
-    acc *= alpha;
-    m = m_new;
-    for (int i = g; i < min(256, length - base); i += kParts) {
-      const int k = base + i;
-      const uint16_t* v = p.values + clamped_page(table[k >> p.page_log], p.n_pages) * p.vp_sp + kvh * p.vp_sh + (k & ((1 << p.page_log) - 1)) * p.vp_sn;
-      acc = __builtin_fmaf(prob[i], T::from16(v[d]), acc);
+    for (int s = 0; s < kKS; ++s) q[s] = q2[s];
+    load_q(q2, f2, u2);  // (the last unit's once more)
+    __builtin_amdgcn_sched_barrier(0);
+    const int length = u.length, head0 = u.head0, n_cols = u.n_cols;
+    float m_run = -INFINITY, l_run = 0.f;
+    floatx4 acc[kDV];
+#pragma unroll
+    for (int j = 0; j < kDV; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+    auto scores = [&](const Tile& x, floatx4 (&s)[2]) __attribute__((always_inline)) {
+      s[0] = s[1] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kKS; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) s[half] = mfma16<T>(x.k[half][i], q[i], s[half]);
+    };
+    // rows behind the last key hold anything: their scores and values go
+    auto seen = [&](const int t, const int i) __attribute__((always_inline)) { return kTile * t + 16 * (i >> 2) + 4 * g + (i & 3) < length; };
+    auto probabilities = [&](floatx4 (&s)[2], const int t, u32x4& prob, u32x4& rest, const bool exact) __attribute__((always_inline)) {
+      if (kTile * (t + 1) > length) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = seen(t, i) ? s[i >> 2][i & 3] : -INFINITY;
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
+      const float m_new = fmaxf(m_run, max_over_quarters(mx));
+      const float m_base = m_new == -INFINITY ? 0.f : m_new;  // (no key of this column's so far)
+      if (__any(m_new > m_run)) {
+        const float alpha = fast_exp2((m_run - m_base) * scale);
+        l_run *= alpha;
+#pragma unroll
+        for (int j = 0; j < kDV; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[j][r] *= alpha;
+        m_run = m_new;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e0 = prob_exp2<T>(s[i >> 1][2 * (i & 1)] - m_base, scale), e1 = prob_exp2<T>(s[i >> 1][2 * (i & 1) + 1] - m_base, scale);
+        l_run += e0 + e1;
+        uint32_t w = T::pack(e0, e1);
+        if (exact) {
+          if (e0 > 0.f && (w & 0xffffu) == 0u) w |= 1u;
+          if (e1 > 0.f && (w >> 16) == 0u) w |= 0x10000u;
+        }
+        prob[i] = w;
+        rest[i] = T::pack_rest(e0, e1, w);
+      }
+    };
+    auto add_values = [&](Tile& x, const int t, const u32x4 prob, const u32x4 rest, const bool exact) __attribute__((always_inline)) {
+      if (kTile * (t + 1) > length) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int w = 0; w < kVW; ++w) x.v[i][w] = seen(t, i) ? x.v[i][w] : 0u;
+      }
+#pragma unroll
+      for (int w = 0; w < kVW; ++w)
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {
+          u32x4 v;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_perm(x.v[2 * i + 1][w], x.v[2 * i][w], odd ? 0x07060302u : 0x05040100u);
+          acc[2 * w + odd] = mfma16<T>(v, prob, acc[2 * w + odd]);
+          if (exact) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if ((v[i] & T::kExponent) == T::kExponent) v[i] &= 0xffff0000u;
+              if (((v[i] >> 16) & T::kExponent) == T::kExponent) v[i] &= 0xffffu;
+            }
+          }
+          acc[2 * w + odd] = mfma16<T>(v, rest, acc[2 * w + odd]);
+        }
+    };
+
+    // A tile's keys are read before its soft-max and its values after it, and each at once gives its registers to the next tile's, which is the
+    // next unit's first where this one has no more.
+    for (int t = f.tile + wave; t < last; t += WAVES) {
+      const bool here = t + WAVES < last;
+      Unit n;
+      n.table = here ? u.table : u2.table;
+      n.last_page = here ? u.last_page : u2.last_page;
+      n.k_head = here ? u.k_head : u2.k_head;
+      n.v_head = here ? u.v_head : u2.v_head;
+      const Spot o = spot(n, here ? t + WAVES : wave, here || wave < last2);
+      floatx4 s[2];
+      scores(x, s);
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(x, o);
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 prob, rest;
+      probabilities(s, t, prob, rest, false);
+      add_values(x, t, prob, rest, false);
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(x, o);
+    }
+    if (f.tile + wave >= last) {  // (a wave without a tile has loaded nothing for the next unit)
+      const Spot o = spot(u2, wave, wave < last2);
+      load_k(x, o);
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(x, o);
+    }
+    l_run = sum_over_quarters(l_run);
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < kDV; ++j) sum += (acc[j][0] + acc[j][1]) + (acc[j][2] + acc[j][3]);
+    if (__builtin_expect(__any(is_nan(sum) && !is_nan(l_run)), 0)) {
+      // Infinite values: with two products per key they give NaN.  The wave's sums once more, relative to the maximum: the rest meets the
+      // finite values only and a positive probability does not round to 0.
+      l_run = 0.f;
+#pragma unroll
+      for (int j = 0; j < kDV; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int t = f.tile + wave; t < last; t += WAVES) {
+        Tile y;
+        const Spot o = spot(u, t, true);
+        load_k(y, o);
+        load_v(y, o);
+        floatx4 s[2];
+        u32x4 prob, rest;
+        scores(y, s);
+        probabilities(s, t, prob, rest, true);
+        add_values(y, t, prob, rest, true);
+      }
+      l_run = sum_over_quarters(l_run);
+    }
+
+    // ---- the waves' states -> one ----------------------------------------------------------------
+    if (g == 0) {
+      stats[0][wave][c16] = m_run;
+      stats[1][wave][c16] = l_run;
+    }
+    if (c16 < n_cols) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < kDV; j += 4)
+          *reinterpret_cast<floatx4*>(&accs[wave][c16][kDV * (4 * g + r) + j]) = floatx4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
     }
     __syncthreads();
+    const bool from_start = f.tile == 0, to_end = last == f.n_tiles;
+    const int part = 2 * blockIdx.x + (from_start ? 1 : 0);
+    for (int i = tid; i < n_cols * (D / 4); i += 64 * WAVES) {
+      const int col = i / (D / 4), d = 4 * (i % (D / 4));
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stats[0][w][col]);
+      float l = 0.f;
+      floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float mw = stats[0][w][col];
+        const float weight = mw == -INFINITY ? 0.f : fast_exp2((mw - m) * scale);
+        l += weight * stats[1][w][col];
+        const floatx4 y = *reinterpret_cast<const floatx4*>(&accs[w][col][d]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += weight * y[e];
+      }
+      if (from_start && to_end) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint16_t* op = p.out + f.b * p.o_sb + (int64_t)(head0 + col) * p.o_sh + d;
+        *reinterpret_cast<u32x2*>(op) = u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
+      } else {
+        const int64_t to = (int64_t)part * kCols + col;
+        *reinterpret_cast<floatx4*>(p.parts + to * D + d) = x;
+        if (d == 0) {
+          p.part_stats[2 * to] = m;
+          p.part_stats[2 * to + 1] = l;
+        }
+      }
+    }
+    if (from_start && !to_end) {  // the others of this unit's parts are the next work-groups'
+      cut = true;
+      const int parts = (int)((at - f.tile + f.n_tiles - 1) / share) - (int)blockIdx.x + 1;
+      if (tid == 0) *reinterpret_cast<int4*>(header) = int4{parts, f.b, head0, n_cols};
+    }
+    at = at2;
+    f = f2;
+    u = u2;
+    __syncthreads();  // (the accumulators have been read)
   }
-  part[g][d] = acc;
+  if (!cut && tid == 0 && p.headers != nullptr) header[0] = 0;
+}
+
+// Joins the parts of a column whose unit begins in share blockIdx.x and ends in another: the weights first, then groups of D / 4 lanes add up
+// every so many parts.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArgs p) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  __shared__ float weight[kShares], red[2][4];
+  __shared__ floatx4 sums[kGroups][kLanes];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = blockIdx.y;
+  const int4 header = *reinterpret_cast<const int4*>(p.headers + 4 * blockIdx.x);
+  const int parts = header.x;
+  if (parts == 0 || col >= header.w) return;
+  const float scale = p.sm_scale * kLog2e;
+  // the first part is the second of its share, the others the first of theirs
+  auto part = [&](const int i) { return ((int64_t)2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kCols + col; };
+  float m = -INFINITY, l = 0.f;
+  for (int i = tid; i < parts; i += 256) m = fmaxf(m, p.part_stats[2 * part(i)]);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+  if (lane == 0) red[0][wave] = m;
   __syncthreads();
-  if (tid < D) {
-    for (int i = 1; i < kParts; ++i) acc += part[i][d];
-    p.out[b * p.o_sb + h * p.o_sh + d] = (uint16_t)T::pack(l == 0.f ? 0.f : acc / l, 0.f);
+  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  for (int i = tid; i < parts; i += 256) {
+    const float mi = p.part_stats[2 * part(i)];
+    const float w = mi == -INFINITY ? 0.f : fast_exp2((mi - m) * scale);
+    weight[i] = w;
+    l += w * p.part_stats[2 * part(i) + 1];
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
+  if (lane == 0) red[1][wave] = l;
+  __syncthreads();
+  const int gr = tid / kLanes, d4 = tid % kLanes;
+  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = gr; i < parts; i += kGroups) {
+    const floatx4 x = *reinterpret_cast<const floatx4*>(p.parts + part(i) * D + 4 * d4);
+    const float w = weight[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += w * x[e];
+  }
+  sums[gr][d4] = sum;
+  __syncthreads();
+  if (tid < kLanes) {
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += sums[i][tid][e];
+    l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* op = p.out + header.y * p.o_sb + (int64_t)(header.z + col) * p.o_sh + 4 * tid;
+    *reinterpret_cast<u32x2*>(op) = u32x2{T::pack(sum[0] * inv, sum[1] * inv), T::pack(sum[2] * inv, sum[3] * inv)};
   }
 }
 
+// Scratch of a step: a header, and two parts of 16 columns, for each share.  None where no unit is cut.
+PagedScratch paged_decode_scratch(int head_dim, int page_log, int max_pages) {
+  PagedScratch s = {0, 0, 0, 0};
+  if (max_pages << page_log <= kWhole * kTile) return s;
+  s.stats = (size_t)kShares * 16;
+  s.parts = s.stats + (size_t)kShares * 2 * kCols * 8;
+  s.total = s.parts + (size_t)kShares * 2 * kCols * head_dim * 4;
+  return s;
+}
+
+template <typename T, int D>
+static void launch_paged_decode_for(const PagedDecodeArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_decode_kernel<T, D, 4>), dim3(kShares), dim3(256), 0, stream, a);
+  const int group = a.n_q_heads / a.n_kv_heads;
+  if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3(kShares, group < kCols ? group : kCols), dim3(256), 0, stream, a);
+}
+
 hipError_t launch_paged_decode(const PagedDecodeArgs& a, hipStream_t stream) {
-  const dim3 grid(a.n_q_heads, a.batch), block(256);
   if (a.head_dim == 128) {
-    if (a.dtype == 0) hipLaunchKernelGGL((paged_decode_kernel<Bf16, 128>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((paged_decode_kernel<F16, 128>), grid, block, 0, stream, a);
+    if (a.dtype == 0) launch_paged_decode_for<Bf16, 128>(a, stream);
+    else launch_paged_decode_for<F16, 128>(a, stream);
   } else {
-    if (a.dtype == 0) hipLaunchKernelGGL((paged_decode_kernel<Bf16, 64>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((paged_decode_kernel<F16, 64>), grid, block, 0, stream, a);
+    if (a.dtype == 0) launch_paged_decode_for<Bf16, 64>(a, stream);
+    else launch_paged_decode_for<F16, 64>(a, stream);
   }
   return hipGetLastError();
 }
