@@ -915,8 +915,8 @@ int aa_paged_append(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int6
   const char* who = "aa_paged_append";
   int rc;
   if ((rc = check_paged(who, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, max_pages, dtype))) return rc;
-  if (n_tokens <= 0 || n_tokens >= 1 << 24 || (starts == nullptr && n_tokens != batch)) {
-    set_error("%s: %d tokens of %d sequences are not supported (1 to 2^24 - 1, without starts one of each sequence)", who, n_tokens, batch);
+  if (n_tokens <= 0 || n_tokens >= 1 << 24 || (int64_t)n_tokens * n_kv_heads >= 1 << 26 || (starts == nullptr && n_tokens != batch)) {
+    set_error("%s: %d tokens of %d sequences are not supported (1 to 2^24 - 1, fewer than 2^26 with their KV heads, without starts one of each sequence)", who, n_tokens, batch);
     return n_tokens <= 0 ? AA_EBADARG : AA_EUNSUPPORTED;
   }
   if ((cos == nullptr) != (sin == nullptr) || (q == nullptr) != (n_q_heads == 0) || (q == nullptr) != (q_out == nullptr) || (q != nullptr && cos == nullptr)) {
@@ -939,7 +939,7 @@ int aa_paged_append(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int6
   }
   PagedAppendArgs a = {(const uint16_t*)q, q_st, q_sh, (uint16_t*)q_out, qo_st, qo_sh, (const uint16_t*)k, k_st, k_sh, (const uint16_t*)v, v_st, v_sh,
                        cos, sin, cs_sn, n_positions, (uint16_t*)keys, kp_sp, kp_sh, kp_sn, (uint16_t*)values, vp_sp, vp_sh, vp_sn, (uint16_t*)bounds,
-                       page_table, pt_sb, lengths, starts, batch, n_tokens, n_q_heads, n_kv_heads, head_dim, n_pages, log2_of(page_size), max_pages, dtype};
+                       page_table, pt_sb, lengths, starts, batch, n_tokens, n_q_heads, n_kv_heads, head_dim, n_pages, log2_of(page_size), max_pages, dtype, 0};
   return check_launch(launch_paged_append(a, (hipStream_t)stream), who);
 }
 

@@ -4,6 +4,9 @@
 
 namespace aa {
 
+// Tables and lengths that no kernel that reads them writes: scalar loads where the index is wave-uniform.
+typedef __attribute__((address_space(4))) const int32_t const_i32;
+
 __device__ __forceinline__ int clamped_length(const int32_t* lengths, const int b, const int max_pages, const int page_log) {
   return min(max(lengths[b], 0), max_pages << page_log);
 }
