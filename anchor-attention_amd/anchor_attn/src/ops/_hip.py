@@ -19,6 +19,13 @@ AA_DTYPE_F16 = 1
 AA_STATIC_SCRATCH_BYTES = 40 * 1024 * 1024  # capacity of the library's static stage-2 scratch (aa_stage2_select_static)
 
 
+class PagedCacheStruct(ctypes.Structure):
+    """``aa_paged_cache``."""
+    _fields_ = [("keys", c_void_p), ("kp_sp", c_int64), ("kp_sh", c_int64), ("kp_sn", c_int64),
+                ("values", c_void_p), ("vp_sp", c_int64), ("vp_sh", c_int64), ("vp_sn", c_int64), ("bounds", c_void_p),
+                ("n_pages", c_int), ("n_kv_heads", c_int), ("page_size", c_int), ("head_dim", c_int), ("dtype", c_int)]
+
+
 class AnchorAttnHipError(RuntimeError):
     pass
 
@@ -57,13 +64,12 @@ _SIGNATURES = {
     "aa_rope": (c_int, _T3 * 4 + [c_void_p, c_void_p, c_int64] + _DIMS5 + [c_int, c_void_p]),
     "aa_silu_mul": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_void_p]),
     "aa_dense_rows_fwd": (c_int, _T3 * 4 + [c_void_p, c_int64, c_int64] + [c_void_p, c_size_t] + [c_int] * 7 + [c_float, c_int, c_void_p]),
-    # (pages: keys and values as [n_pages, n_kv_heads, page_size, head_dim]; batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, max_pages)
-    "aa_paged_append": (c_int, _T2 * 4 + [c_void_p, c_void_p, c_int64, c_int] + _T3 * 2 + [c_void_p, c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 9 + [c_void_p]),
+    # (the first argument: the address of a PagedCacheStruct)
+    "aa_paged_append": (c_int, [c_void_p] + _T2 * 4 + [c_void_p, c_void_p, c_int64, c_int] + [c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p]),
     "aa_paged_decode_workspace_bytes": (c_size_t, [c_int] * 6),
-    "aa_paged_decode_fwd": (c_int, _T2 * 2 + _T3 * 2 + [c_void_p, c_int64, c_void_p, c_void_p, c_size_t] + [c_int] * 7 + [c_float, c_int, c_void_p]),
+    "aa_paged_decode_fwd": (c_int, [c_void_p] + _T2 * 2 + [c_void_p, c_int64, c_void_p, c_void_p, c_size_t] + [c_int] * 3 + [c_float, c_void_p]),
     "aa_paged_sparse_workspace_bytes": (c_size_t, [c_int] * 7),
-    "aa_paged_sparse_decode_fwd": (c_int, _T2 * 2 + _T3 * 2 + [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_size_t] + [c_int] * 10
-                                   + [c_float, c_int, c_void_p]),
+    "aa_paged_sparse_decode_fwd": (c_int, [c_void_p] + _T2 * 2 + [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_size_t] + [c_int] * 6 + [c_float, c_void_p]),
     # the operator's sizes, then n_rows, n_keys, causal_offset
     "aa_anchor_attn_rows_workspace_bytes": (c_size_t, [c_int] * 10),
     "aa_anchor_attn_rows_fwd": (c_int, _T3 * 8 + [c_int] * 3 + [c_float] + [c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_double] + _DIMS5

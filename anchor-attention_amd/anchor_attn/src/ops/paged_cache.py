@@ -14,6 +14,7 @@ never accessed (``include/anchor_attn_hip.h`` says what is done instead).  Nothi
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -25,6 +26,7 @@ from .anchor_step_1_2_v2 import _stream
 PAGE_SIZES = (16, 32, 64, 128, 256)
 _TYPES = (torch.Tensor, torch.nn.Parameter)
 _HALF = (torch.bfloat16, torch.float16)
+_INT32, _FLOAT32 = torch.int32, torch.float32
 
 
 def _refuse(what: str):
@@ -32,28 +34,22 @@ def _refuse(what: str):
 
 
 def _rows(t, name, cache, heads):
-    """``(data_ptr, token stride, head stride)`` of a tensor ``[tokens, heads, head dimension]``."""
-    if type(t) not in _TYPES or t.dim() != 3 or t.dtype != cache.dtype or t.device != cache.device:
+    """``(data_ptr, token stride, head stride)`` of a tensor ``[tokens, heads, head dimension]`` and its shape."""
+    if type(t) not in _TYPES or t.dtype != cache.dtype or t.get_device() != cache.index or t.dim() != 3:
         _refuse(f"{name} must be a tensor [tokens, heads, head dimension] of the cache's type and device")
-    _, h, d = t.shape
+    _, h, d = shape = t.shape
     st, sh, sd = t.stride()
-    if d != cache.head_dim or (heads is not None and h != heads) or h % cache.n_kv_heads or not h:
+    ptr = t.data_ptr()
+    if d != cache.head_dim or (h != heads if heads else not h or h % cache.n_kv_heads):
         _refuse(f"{name} has {h} heads of {d}, the cache {cache.n_kv_heads} of {cache.head_dim}")
-    if sd != 1 or (st | sh) & 7 or t.data_ptr() & 15:
+    if sd != 1 or (st | sh) & 7 or ptr & 15:
         _refuse(f"the rows of {name} must be contiguous and begin on 16-byte boundaries")
-    return t.data_ptr(), st, sh
-
-
-def _like(out, q, name, cache):
-    if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if type(out) not in _TYPES or out.shape != q.shape:
-        _refuse(f"{name} must have the shape of q")
-    return out
+    return (ptr, st, sh), shape
 
 
 def _indices(t, name, cache, dim, rows=None):
-    if type(t) not in _TYPES or t.dim() != dim or t.dtype != torch.int32 or t.device != cache.device or (t.shape[-1] > 1 and t.stride(-1) != 1):
+    """``data_ptr`` of a tensor of whole numbers."""
+    if type(t) not in _TYPES or t.dtype != _INT32 or t.get_device() != cache.index or t.dim() != dim or (t.stride(-1) != 1 and t.shape[-1] > 1):
         _refuse(f"{name} must be an int32 tensor of {dim} dimension{'s' if dim > 1 else ''} on the cache's device, its rows contiguous")
     if rows is not None and t.shape[0] != rows:
         _refuse(f"{name} has {t.shape[0]} entries where {rows} are expected")
@@ -63,9 +59,10 @@ def _indices(t, name, cache, dim, rows=None):
 class PagedCache:
     """Keys and values in pages: ``keys``, ``values`` ``[n_pages, n_kv_heads, page_size, head_dim]`` (bf16 or fp16 on one GPU, rows contiguous on
     16-byte boundaries, the other strides free) and, for sparse steps, ``bounds`` ``[n_pages, n_kv_heads, 2, head_dim]`` (contiguous): the
-    smallest and the largest value of each channel over a page's keys, which :func:`append_to_pages` keeps.  The contents of pages that no table names do not matter."""
+    smallest and the largest value of each channel over a page's keys, which :func:`append_to_pages` keeps.  The contents of pages that no table names
+    do not matter.  The tensors stay the cache's own for as long as it is used: their contents may change, their memory may not."""
 
-    __slots__ = ("keys", "values", "bounds", "dtype", "device", "n_pages", "n_kv_heads", "page_size", "head_dim", "_dtype_code")
+    __slots__ = ("keys", "values", "bounds", "dtype", "device", "index", "n_pages", "n_kv_heads", "page_size", "head_dim", "_struct", "_address")
 
     def __init__(self, keys: torch.Tensor, values: torch.Tensor, bounds: Optional[torch.Tensor] = None):
         tensors = (keys, values) if bounds is None else (keys, values, bounds)
@@ -79,13 +76,16 @@ class PagedCache:
                     f"not {tuple(keys.shape)} and {tuple(values.shape)}")
         for t in (keys, values):
             sp, sh, sn, sd = t.stride()
-            if sd != 1 or (sp | sh | sn) & 7 or t.data_ptr() & 15 or not d <= sn <= 1 << 14:
-                _refuse("the rows of keys and values must be contiguous, begin on 16-byte boundaries and lie at most 16384 elements apart")
+            if sd != 1 or (sp | sh | sn) & 7 or t.data_ptr() & 15 or not d <= sn <= 1 << 14 or (not sp and n_pages > 1) or (not sh and kv_heads > 1):
+                _refuse("the rows of keys and values must be contiguous, begin on 16-byte boundaries and lie at most 16384 elements apart, and no two share memory")
         if bounds is not None and (bounds.shape != (n_pages, kv_heads, 2, d) or not bounds.is_contiguous() or bounds.data_ptr() & 15):
             _refuse(f"bounds must be a contiguous tensor {(n_pages, kv_heads, 2, d)}, not {tuple(bounds.shape)}")
-        self.keys, self.values, self.bounds, self.dtype, self.device = keys, values, bounds, keys.dtype, keys.device
+        self.keys, self.values, self.bounds, self.dtype, self.device, self.index = keys, values, bounds, keys.dtype, keys.device, keys.get_device()
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n_pages, kv_heads, page_size, d
-        self._dtype_code = _hip.dtype_code(keys)
+        # (what the C interface is told of the cache, once: 13 arguments fewer in each call)
+        self._struct = _hip.PagedCacheStruct(*_hip.t3(keys), *_hip.t3(values), None if bounds is None else bounds.data_ptr(), n_pages, kv_heads, page_size, d,
+                                             _hip.dtype_code(keys))
+        self._address = ctypes.addressof(self._struct)
 
     @classmethod
     def empty(cls, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, dtype=torch.bfloat16, device="cuda", bounds: bool = True):
@@ -96,18 +96,21 @@ class PagedCache:
     def _tables(self, page_table, lengths):
         """Arguments of a page table and lengths, and the sequences and most pages they are for."""
         lengths_ptr = _indices(lengths, "lengths", self, 1)
-        table = _indices(page_table, "page_table", self, 2, lengths.shape[0])
-        batch, most = page_table.shape
+        batch = lengths.shape[0]
+        table = _indices(page_table, "page_table", self, 2, batch)
+        most = page_table.shape[1]
         if batch > 65535 or not most or most * self.page_size > 1 << 20:
             _refuse(f"{batch} sequences of up to {most} pages of {self.page_size} are not supported (at most 65535 sequences, 1048576 keys, at least one page)")
         return (table, page_table.stride(0), lengths_ptr), batch, most
 
     def _launch(self, fn, *args):
-        if self.device.index == torch.cuda.current_device():
-            _hip.check(fn(*args, self._dtype_code, _stream()))
+        if self.index == torch.cuda.current_device():
+            rc = fn(self._address, *args, _stream())
         else:
             with torch.cuda.device(self.device):
-                _hip.check(fn(*args, self._dtype_code, _stream()))
+                rc = fn(self._address, *args, _stream())
+        if rc:
+            _hip.check(rc)
 
 
 def _plain(cache, *tensors):
@@ -115,8 +118,10 @@ def _plain(cache, *tensors):
         _refuse("the first argument must be a PagedCache")
     if not _called_plainly():
         _refuse("these operators cannot be traced, compiled, vmapped or watched by a mode")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        _refuse("these operators have no gradients: detach their inputs or call them under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _refuse("these operators have no gradients: detach their inputs or call them under torch.no_grad()")
 
 
 def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tensor],
@@ -133,64 +138,78 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
     Tokens without a place are left out - rows behind the last sequence, a length of 0, a position that ``cos`` or the table does not reach, a page
     outside the pool: their rows of ``out`` stay as they are (undefined in a new one).  Two sequences must not append to one page: the result is then one's or a mixture."""
     _plain(cache, q, k, v, cos, sin, out)
-    n = k.shape[0] if type(k) in _TYPES and k.dim() == 3 else -1
-    k_args = _rows(k, "k", cache, cache.n_kv_heads)
-    v_args = _rows(v, "v", cache, cache.n_kv_heads)
+    k_args, (n, _, _) = _rows(k, "k", cache, cache.n_kv_heads)
+    v_args, (n_values, _, _) = _rows(v, "v", cache, cache.n_kv_heads)
     tables, batch, most = cache._tables(page_table, lengths)
     starts_ptr = None if starts is None else _indices(starts, "starts", cache, 1, batch + 1)
-    if v.shape[0] != n or (starts is None and n != batch) or n >= 1 << 24:
-        _refuse(f"{n} keys, {v.shape[0]} values and {batch} sequences{' without starts' if starts is None else ''} do not go together (at most 2^24 - 1 tokens)")
-    if (cos is None) != (sin is None) or (q is not None and cos is None) or (q is None and out is not None):
-        _refuse("cos and sin come together, and queries need them")
-    angles = (None, None, 0, 0)
-    if cos is not None:
+    if n_values != n or (starts is None and n != batch) or n * cache.n_kv_heads >= 1 << 24:
+        _refuse(f"{n} keys, {n_values} values and {batch} sequences{' without starts' if starts is None else ''} do not go together (and fewer than 2^24 rows of keys)")
+    if cos is None:
+        if sin is not None or q is not None or out is not None:
+            _refuse("cos and sin come together, and queries need them")
+        angles, q_args, heads = (None, None, 0, 0), (None, 0, 0, None, 0, 0), 0
+    else:
+        strides = cos.stride()
         for t in (cos, sin):
-            if type(t) not in _TYPES or t.dim() != 2 or t.dtype != torch.float32 or t.device != cache.device or t.shape != cos.shape or t.stride() != cos.stride():
+            if type(t) not in _TYPES or t.dtype != _FLOAT32 or t.get_device() != cache.index or t.dim() != 2 or t.shape != cos.shape or t.stride() != strides:
                 _refuse("cos and sin must be float32 tensors [positions, D / 2] on the cache's device, laid out alike")
-            if t.shape[1] != cache.head_dim // 2 or not t.shape[0] or t.stride(1) != 1 or t.stride(0) & 3 or t.stride(0) < t.shape[1] or t.data_ptr() & 15:
-                _refuse("the rows of cos and sin must hold D / 2 elements, contiguous on 16-byte boundaries")
-        angles = (cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0])
-    q_args, out_args, heads = (None, 0, 0), (None, 0, 0), 0
-    if q is not None:
-        q_args, heads = _rows(q, "q", cache, None), q.shape[1]
-        if q.shape[0] != n:
-            _refuse(f"q has {q.shape[0]} tokens, k {n}")
-        out = _like(out, q, "out", cache)
-        out_args = _rows(out, "out", cache, heads)
-    if n == 0 or batch == 0:
-        return out
-    bounds = None if cache.bounds is None else cache.bounds.data_ptr()
-    cache._launch(_hip.lib().aa_paged_append, *q_args, *out_args, *k_args, *v_args, *angles, *_hip.t3(cache.keys), *_hip.t3(cache.values), bounds, *tables, starts_ptr,
-                  batch, n, heads, cache.n_kv_heads, cache.head_dim, cache.n_pages, cache.page_size, most)
+        n_positions, half = cos.shape
+        angles = (cos.data_ptr(), sin.data_ptr(), strides[0], n_positions)
+        if half * 2 != cache.head_dim or not n_positions or strides[1] != 1 or strides[0] & 3 or strides[0] < half or (angles[0] | angles[1]) & 15:
+            _refuse("the rows of cos and sin must hold D / 2 elements, contiguous on 16-byte boundaries")
+        if q is None:
+            if out is not None:
+                _refuse("an output needs queries")
+            q_args, heads = (None, 0, 0, None, 0, 0), 0
+        else:
+            q_rows, shape = _rows(q, "q", cache, 0)
+            heads = shape[1]
+            if shape[0] != n:
+                _refuse(f"q has {shape[0]} tokens, k {n}")
+            q_args = (*q_rows, *_out_rows(q, out, shape, cache)) if out is not None else (*q_rows, *_new_rows(out := torch.empty_like(q)))
+    if n and batch:
+        cache._launch(_hip.lib().aa_paged_append, *q_args, *k_args, *v_args, *angles, *tables, starts_ptr, batch, n, heads, most)
     return out
+
+
+def _new_rows(t):
+    st, sh, _ = t.stride()
+    return t.data_ptr(), st, sh
+
+
+def _out_rows(q, out, shape, cache):
+    rows, out_shape = _rows(out, "out", cache, shape[1])
+    if out_shape != shape:
+        _refuse("out must have the shape of q")
+    return rows
 
 
 def _decode_args(cache, q, page_table, lengths, sm_scale, out):
     _plain(cache, q, out)
-    q_args = _rows(q, "q", cache, None)
+    q_rows, shape = _rows(q, "q", cache, 0)
     tables, batch, most = cache._tables(page_table, lengths)
-    if q.shape[0] != batch:
-        _refuse(f"q has {q.shape[0]} tokens, the table {batch} sequences: a decode step has one of each")
-    out = _like(out, q, "out", cache)
+    if shape[0] != batch:
+        _refuse(f"q has {shape[0]} tokens, the table {batch} sequences: a decode step has one of each")
     scale = float(sm_scale) if sm_scale else cache.head_dim ** -0.5
     if not 1e-30 < scale < 1e30:
         _refuse(f"sm_scale must be positive and finite, not {sm_scale}")
-    sizes = (batch, q.shape[1], cache.n_kv_heads, cache.head_dim)
-    return out, (*q_args, *_rows(out, "out", cache, q.shape[1])), tables, sizes, most, scale
+    if out is not None:
+        out_rows = _out_rows(q, out, shape, cache)
+    else:
+        out_rows = _new_rows(out := torch.empty_like(q))
+    return out, (*q_rows, *out_rows, *tables), (batch, shape[1]), most, scale
 
 
 def paged_decode_attention(cache: PagedCache, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, sm_scale: Optional[float] = None,
                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one new token per sequence, ``q`` ``[batch, query heads, D]``, over the first ``lengths[b]`` keys of each: ``softmax(q K^T
     sm_scale) V``, zeros for a sequence of none.  ``sm_scale`` defaults to ``D ** -0.5``."""
-    out, tensors, tables, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
-    if sizes[0] == 0:
-        return out
-    lib = _hip.lib()
-    nbytes = lib.aa_paged_decode_workspace_bytes(*sizes, cache.page_size, most)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=cache.device) if nbytes else None
-    cache._launch(lib.aa_paged_decode_fwd, *tensors, *_hip.t3(cache.keys), *_hip.t3(cache.values), *tables, ws.data_ptr() if nbytes else None, nbytes,
-                  *sizes, cache.n_pages, cache.page_size, most, scale)
+    out, tensors, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
+    if sizes[0]:
+        lib = _hip.lib()
+        nbytes = lib.aa_paged_decode_workspace_bytes(*sizes, cache.n_kv_heads, cache.head_dim, cache.page_size, most)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=cache.device) if nbytes else None
+        cache._launch(lib.aa_paged_decode_fwd, *tensors, ws.data_ptr() if nbytes else None, nbytes, *sizes, most, scale)
     return out
 
 
@@ -202,18 +221,16 @@ def paged_sparse_decode_attention(cache: PagedCache, q: torch.Tensor, page_table
     over the heads of the group of ``sum_d max over the page's bounds of q_d * x_d``: no key of the page has a larger product with the query.
     It is summed in float64 and rounded to float32; NaN counts as infinity.  Returns the output and the chosen pages, int32 ``[batch, KV heads,
     n_pages]``: places in the sequence's row of the table, ascending, then -1.  The cache needs ``bounds``."""
-    out, tensors, tables, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
+    out, tensors, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
     n_pages, n_first, n_last = int(n_pages), int(n_first), int(n_last)
     if cache.bounds is None:
         _refuse("sparse steps need a cache with bounds")
     if n_first < 0 or n_last < 1 or n_first + n_last > n_pages or n_pages > 1 << 16:
         _refuse(f"{n_pages} pages, the first {n_first} and the last {n_last} among them, are not supported (at most 65536, at least the last one)")
-    pages = torch.empty((sizes[0], cache.n_kv_heads, n_pages), dtype=torch.int32, device=cache.device)
-    if sizes[0] == 0:
-        return out, pages
-    lib = _hip.lib()
-    nbytes = lib.aa_paged_sparse_workspace_bytes(*sizes, cache.page_size, most, n_pages)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=cache.device)
-    cache._launch(lib.aa_paged_sparse_decode_fwd, *tensors, *_hip.t3(cache.keys), *_hip.t3(cache.values), cache.bounds.data_ptr(), *tables, pages.data_ptr(),
-                  ws.data_ptr(), nbytes, *sizes, cache.n_pages, cache.page_size, most, n_pages, n_first, n_last, scale)
+    pages = torch.empty((sizes[0], cache.n_kv_heads, n_pages), dtype=_INT32, device=cache.device)
+    if sizes[0]:
+        lib = _hip.lib()
+        nbytes = lib.aa_paged_sparse_workspace_bytes(*sizes, cache.n_kv_heads, cache.head_dim, cache.page_size, most, n_pages)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=cache.device)
+        cache._launch(lib.aa_paged_sparse_decode_fwd, *tensors, pages.data_ptr(), ws.data_ptr(), nbytes, *sizes, most, n_pages, n_first, n_last, scale)
     return out, pages

@@ -855,11 +855,9 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
 }
 
 // ---- key/value cache in pages ----
-static int check_paged(const char* who, int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size, int max_pages, int dtype) {
-  int rc;
-  if ((rc = check_dtype(dtype, who))) return rc;
-  if (batch <= 0 || n_q_heads < 0 || n_kv_heads <= 0 || n_pages <= 0 || max_pages <= 0) {
-    set_error("%s: batch, head counts and page counts must be positive (got %d, %d, %d, %d, %d)", who, batch, n_q_heads, n_kv_heads, n_pages, max_pages);
+static int check_paged(const char* who, int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
+  if (batch <= 0 || n_q_heads < 0 || n_kv_heads <= 0 || max_pages <= 0) {
+    set_error("%s: batch, head counts and max_pages must be positive (got %d, %d, %d, %d)", who, batch, n_q_heads, n_kv_heads, max_pages);
     return AA_EBADARG;
   }
   if (n_q_heads % n_kv_heads != 0) {
@@ -903,48 +901,65 @@ static int check_words(const void* ptr, const char* who, const char* name) {
   return AA_OK;
 }
 
+// the cache itself, with the sizes of a call
+static int check_cache(const char* who, const aa_paged_cache* c, int batch, int n_q_heads, int max_pages, const int32_t* page_table, const int32_t* lengths) {
+  int rc;
+  if (c == nullptr) {
+    set_error("%s: cache is NULL", who);
+    return AA_EBADARG;
+  }
+  if ((rc = check_dtype(c->dtype, who)) || (rc = check_paged(who, batch, n_q_heads, c->n_kv_heads, c->head_dim, c->page_size, max_pages))) return rc;
+  if (c->n_pages <= 0) {
+    set_error("%s: n_pages must be positive (got %d)", who, c->n_pages);
+    return AA_EBADARG;
+  }
+  if ((rc = check_tensor(c->keys, c->kp_sp, c->kp_sh, c->kp_sn, c->page_size, c->head_dim, who, "keys")) ||
+      (rc = check_tensor(c->values, c->vp_sp, c->vp_sh, c->vp_sn, c->page_size, c->head_dim, who, "values")) ||
+      (c->bounds != nullptr && (rc = check_ptr(c->bounds, who, "bounds"))) || (rc = check_words(page_table, who, "page_table")) ||
+      (rc = check_words(lengths, who, "lengths")))
+    return rc;
+  return AA_OK;
+}
+
 static int log2_of(int power) { return 31 - __builtin_clz((unsigned)power); }
 
-int aa_paged_append(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+int aa_paged_append(const aa_paged_cache* cache, const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
                     const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
                     const float* cos, const float* sin, int64_t cs_sn, int n_positions,
-                    void* keys, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn, void* values, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn, void* bounds,
                     const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, const int32_t* starts,
-                    int batch, int n_tokens, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size, int max_pages,
-                    int dtype, void* stream) {
+                    int batch, int n_tokens, int n_q_heads, int max_pages, void* stream) {
   const char* who = "aa_paged_append";
   int rc;
-  if ((rc = check_paged(who, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, max_pages, dtype))) return rc;
-  if (n_tokens <= 0 || n_tokens >= 1 << 24 || (int64_t)n_tokens * n_kv_heads >= 1 << 26 || (starts == nullptr && n_tokens != batch)) {
-    set_error("%s: %d tokens of %d sequences are not supported (1 to 2^24 - 1, fewer than 2^26 with their KV heads, without starts one of each sequence)", who, n_tokens, batch);
+  if ((rc = check_cache(who, cache, batch, n_q_heads, max_pages, page_table, lengths))) return rc;
+  if (n_tokens <= 0 || n_tokens >= 1 << 24 || (int64_t)n_tokens * cache->n_kv_heads >= 1 << 24 || (starts == nullptr && n_tokens != batch)) {
+    set_error("%s: %d tokens of %d sequences are not supported (at least 1, fewer than 2^24 with their KV heads, without starts one of each sequence)",
+              who, n_tokens, batch);
     return n_tokens <= 0 ? AA_EBADARG : AA_EUNSUPPORTED;
   }
   if ((cos == nullptr) != (sin == nullptr) || (q == nullptr) != (n_q_heads == 0) || (q == nullptr) != (q_out == nullptr) || (q != nullptr && cos == nullptr)) {
     set_error("%s: cos and sin come together, and so do q, q_out and query heads, which need them", who);
     return AA_EBADARG;
   }
-  if (q != nullptr && ((rc = check_rows(q, q_st, q_sh, who, "q")) || (rc = check_rows(q_out, qo_st, qo_sh, who, "q_out")))) return rc;
-  if ((rc = check_rows(k, k_st, k_sh, who, "k")) || (rc = check_rows(v, v_st, v_sh, who, "v")) ||
-      (rc = check_tensor(keys, kp_sp, kp_sh, kp_sn, page_size, head_dim, who, "keys")) ||
-      (rc = check_tensor(values, vp_sp, vp_sh, vp_sn, page_size, head_dim, who, "values")) ||
-      (bounds != nullptr && (rc = check_ptr(bounds, who, "bounds"))) || (rc = check_words(page_table, who, "page_table")) ||
-      (rc = check_words(lengths, who, "lengths")) || (starts != nullptr && (rc = check_words(starts, who, "starts"))))
+  if ((q != nullptr && ((rc = check_rows(q, q_st, q_sh, who, "q")) || (rc = check_rows(q_out, qo_st, qo_sh, who, "q_out")))) ||
+      (rc = check_rows(k, k_st, k_sh, who, "k")) || (rc = check_rows(v, v_st, v_sh, who, "v")) ||
+      (starts != nullptr && (rc = check_words(starts, who, "starts"))))
     return rc;
   if (cos != nullptr) {
     if ((rc = check_ptr(cos, who, "cos")) || (rc = check_ptr(sin, who, "sin"))) return rc;
-    if (n_positions <= 0 || cs_sn < head_dim / 2 || cs_sn % 4 != 0) {
+    if (n_positions <= 0 || cs_sn < cache->head_dim / 2 || cs_sn % 4 != 0) {
       set_error("%s: cos and sin must have rows of head_dim / 2 elements on 16-byte boundaries (got %d, %lld elements apart)", who, n_positions, (long long)cs_sn);
       return AA_EBADARG;
     }
   }
-  PagedAppendArgs a = {(const uint16_t*)q, q_st, q_sh, (uint16_t*)q_out, qo_st, qo_sh, (const uint16_t*)k, k_st, k_sh, (const uint16_t*)v, v_st, v_sh,
-                       cos, sin, cs_sn, n_positions, (uint16_t*)keys, kp_sp, kp_sh, kp_sn, (uint16_t*)values, vp_sp, vp_sh, vp_sn, (uint16_t*)bounds,
-                       page_table, pt_sb, lengths, starts, batch, n_tokens, n_q_heads, n_kv_heads, head_dim, n_pages, log2_of(page_size), max_pages, dtype, 0};
+  const PagedAppendArgs a = {(const uint16_t*)q, q_st, q_sh, (uint16_t*)q_out, qo_st, qo_sh, (const uint16_t*)k, k_st, k_sh, (const uint16_t*)v, v_st, v_sh,
+                             cos, sin, cs_sn, n_positions, (uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn, (uint16_t*)cache->values,
+                             cache->vp_sp, cache->vp_sh, cache->vp_sn, (uint16_t*)cache->bounds, page_table, pt_sb, lengths, starts, batch, n_tokens, n_q_heads,
+                             cache->n_kv_heads, cache->head_dim, cache->n_pages, log2_of(cache->page_size), max_pages, cache->dtype, 0};
   return check_launch(launch_paged_append(a, (hipStream_t)stream), who);
 }
 
 size_t aa_paged_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
-  if (check_paged("aa_paged_decode_workspace_bytes", batch, n_q_heads, n_kv_heads, head_dim, 1, page_size, max_pages, AA_DTYPE_BF16)) return 0;
+  if (check_paged("aa_paged_decode_workspace_bytes", batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages)) return 0;
   return paged_decode_scratch(head_dim, log2_of(page_size), max_pages).total;
 }
 // ... laid out at `workspace`
@@ -956,41 +971,36 @@ static void give_scratch(PagedDecodeArgs& a, char* workspace, int max_pages) {
   a.parts = (float*)(workspace + s.parts);
 }
 
-static int paged_decode_args(const char* who, PagedDecodeArgs& a, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
-                             const void* keys, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn, const void* values, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn,
-                             const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, void* workspace, size_t workspace_bytes, size_t needed,
-                             int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size, int max_pages, float sm_scale, int dtype) {
+static int paged_decode_args(const char* who, PagedDecodeArgs& a, const aa_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, void* out,
+                             int64_t o_sb, int64_t o_sh, const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, void* workspace,
+                             size_t workspace_bytes, size_t needed, int batch, int n_q_heads, int max_pages, float sm_scale) {
   int rc;
-  if ((rc = check_paged(who, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, max_pages, dtype))) return rc;
   if (n_q_heads == 0 || !(sm_scale > 0.f) || sm_scale > 3.4e38f) {
     set_error("%s: %d query heads and sm_scale %g: both must be positive and finite", who, n_q_heads, (double)sm_scale);
     return AA_EBADARG;
   }
-  if ((rc = check_rows(q, q_sb, q_sh, who, "q")) || (rc = check_rows(out, o_sb, o_sh, who, "out")) ||
-      (rc = check_tensor(keys, kp_sp, kp_sh, kp_sn, page_size, head_dim, who, "keys")) ||
-      (rc = check_tensor(values, vp_sp, vp_sh, vp_sn, page_size, head_dim, who, "values")) ||
-      (rc = check_words(page_table, who, "page_table")) || (rc = check_words(lengths, who, "lengths")) ||
-      (needed > 0 && (rc = check_ptr(workspace, who, "workspace"))))
+  if ((rc = check_rows(q, q_sb, q_sh, who, "q")) || (rc = check_rows(out, o_sb, o_sh, who, "out")) || (needed > 0 && (rc = check_ptr(workspace, who, "workspace"))))
     return rc;
   if (workspace_bytes < needed) {
     set_error("%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, needed);
     return AA_EBADARG;
   }
-  a = {(const uint16_t*)q, q_sb, q_sh, (uint16_t*)out, o_sb, o_sh, (const uint16_t*)keys, kp_sp, kp_sh, kp_sn, (const uint16_t*)values, vp_sp, vp_sh, vp_sn,
-       page_table, pt_sb, 0, lengths, batch, n_q_heads, n_kv_heads, head_dim, n_pages, log2_of(page_size), max_pages, 0, sm_scale, nullptr, nullptr, nullptr, dtype};
+  a = {(const uint16_t*)q, q_sb, q_sh, (uint16_t*)out, o_sb, o_sh, (const uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn,
+       (const uint16_t*)cache->values, cache->vp_sp, cache->vp_sh, cache->vp_sn, page_table, pt_sb, 0, lengths, batch, n_q_heads, cache->n_kv_heads,
+       cache->head_dim, cache->n_pages, log2_of(cache->page_size), max_pages, 0, sm_scale, nullptr, nullptr, nullptr, cache->dtype};
   return AA_OK;
 }
 
-int aa_paged_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
-                        const void* keys, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn, const void* values, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn,
+int aa_paged_decode_fwd(const aa_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
                         const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, void* workspace, size_t workspace_bytes,
-                        int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size, int max_pages,
-                        float sm_scale, int dtype, void* stream) {
+                        int batch, int n_q_heads, int max_pages, float sm_scale, void* stream) {
   const char* who = "aa_paged_decode_fwd";
   PagedDecodeArgs a;
-  const size_t needed = aa_paged_decode_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages);
-  if (int rc = paged_decode_args(who, a, q, q_sb, q_sh, out, o_sb, o_sh, keys, kp_sp, kp_sh, kp_sn, values, vp_sp, vp_sh, vp_sn, page_table, pt_sb, lengths,
-                                 workspace, workspace_bytes, needed, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, max_pages, sm_scale, dtype))
+  int rc;
+  if ((rc = check_cache(who, cache, batch, n_q_heads, max_pages, page_table, lengths))) return rc;
+  const size_t needed = paged_decode_scratch(cache->head_dim, log2_of(cache->page_size), max_pages).total;
+  if ((rc = paged_decode_args(who, a, cache, q, q_sb, q_sh, out, o_sb, o_sh, page_table, pt_sb, lengths, workspace, workspace_bytes, needed, batch, n_q_heads,
+                              max_pages, sm_scale)))
     return rc;
   give_scratch(a, static_cast<char*>(workspace), max_pages);
   return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
@@ -999,27 +1009,24 @@ int aa_paged_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, void* out, in
 struct SparseScratch {
   size_t scores, chosen, decode, total;
 };
-static SparseScratch carve_sparse(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_chosen) {
+static SparseScratch carve_sparse(int batch, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_chosen) {
   SparseScratch w;
   const size_t units = (size_t)batch * n_kv_heads;
   w.scores = 0;
   w.chosen = align256(units * max_pages * 4);
   w.decode = w.chosen + align256(units * n_chosen * 4);
-  w.total = w.decode + aa_paged_decode_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim, page_size, n_chosen < max_pages ? n_chosen : max_pages);
+  w.total = w.decode + paged_decode_scratch(head_dim, log2_of(page_size), std::min(n_chosen, max_pages)).total;
   return w;
 }
 
 size_t aa_paged_sparse_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_chosen) {
-  if (batch <= 0 || n_kv_heads <= 0 || max_pages <= 0 || n_chosen <= 0) return 0;
-  return carve_sparse(batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages, n_chosen).total;
+  if (n_chosen <= 0 || check_paged("aa_paged_sparse_workspace_bytes", batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages)) return 0;
+  return carve_sparse(batch, n_kv_heads, head_dim, page_size, max_pages, n_chosen).total;
 }
 
-int aa_paged_sparse_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
-                               const void* keys, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn,
-                               const void* values, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn, const void* bounds,
+int aa_paged_sparse_decode_fwd(const aa_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
                                const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, int32_t* pages, void* workspace, size_t workspace_bytes,
-                               int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size, int max_pages,
-                               int n_chosen, int n_first, int n_last, float sm_scale, int dtype, void* stream) {
+                               int batch, int n_q_heads, int max_pages, int n_chosen, int n_first, int n_last, float sm_scale, void* stream) {
   const char* who = "aa_paged_sparse_decode_fwd";
   PagedDecodeArgs a;
   int rc;
@@ -1027,21 +1034,23 @@ int aa_paged_sparse_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, void* 
     set_error("%s: %d pages, the first %d and the last %d among them, are not supported (at most 65536, at least the last one)", who, n_chosen, n_first, n_last);
     return AA_EBADARG;
   }
-  if ((rc = check_paged(who, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, max_pages, dtype))) return rc;
-  const SparseScratch w = carve_sparse(batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages, n_chosen);
-  if ((rc = paged_decode_args(who, a, q, q_sb, q_sh, out, o_sb, o_sh, keys, kp_sp, kp_sh, kp_sn, values, vp_sp, vp_sh, vp_sn, page_table, pt_sb, lengths,
-                              workspace, workspace_bytes, w.total, batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, max_pages, sm_scale, dtype)) ||
-      (rc = check_ptr(bounds, who, "bounds")) || (rc = check_words(pages, who, "pages")))
+  if ((rc = check_cache(who, cache, batch, n_q_heads, max_pages, page_table, lengths)) || (rc = check_ptr(cache->bounds, who, "bounds")) ||
+      (rc = check_words(pages, who, "pages")))
+    return rc;
+  const SparseScratch w = carve_sparse(batch, cache->n_kv_heads, cache->head_dim, cache->page_size, max_pages, n_chosen);
+  if ((rc = paged_decode_args(who, a, cache, q, q_sb, q_sh, out, o_sb, o_sh, page_table, pt_sb, lengths, workspace, workspace_bytes, w.total, batch, n_q_heads,
+                              max_pages, sm_scale)))
     return rc;
   char* ws = static_cast<char*>(workspace);
-  const PagedSelectArgs s = {a.q, q_sb, q_sh, (const uint16_t*)bounds, page_table, pt_sb, lengths, (float*)(ws + w.scores), pages, (int32_t*)(ws + w.chosen),
-                             batch, n_q_heads, n_kv_heads, head_dim, n_pages, a.page_log, max_pages, n_chosen, n_first, n_last, dtype};
+  const PagedSelectArgs s = {a.q, q_sb, q_sh, (const uint16_t*)cache->bounds, page_table, pt_sb, lengths, (float*)(ws + w.scores), pages,
+                             (int32_t*)(ws + w.chosen), batch, n_q_heads, cache->n_kv_heads, cache->head_dim, cache->n_pages, a.page_log, max_pages, n_chosen,
+                             n_first, n_last, cache->dtype};
   if ((rc = check_launch(launch_paged_select(s, (hipStream_t)stream), who))) return rc;
   a.table = s.chosen;
-  a.t_sb = (int64_t)n_kv_heads * n_chosen;
+  a.t_sb = (int64_t)cache->n_kv_heads * n_chosen;
   a.t_sh = n_chosen;
   a.n_chosen = n_chosen;
-  give_scratch(a, ws + w.decode, n_chosen < max_pages ? n_chosen : max_pages);
+  give_scratch(a, ws + w.decode, std::min(n_chosen, max_pages));
   return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
 }
 

@@ -257,49 +257,55 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
 
 /* ---- key/value cache in pages -----------------------------------------------------------------
  * What a serving program does after the prompt: a cache that grows by a token per sequence and step, and decode steps that read it.
- * keys, values [n_pages, n_kv_heads, page_size, head_dim] with element strides of page, head and row (_sp, _sh, _sn); page_size 16, 32, 64, 128
- * or 256, head_dim 128 or 64.  page_table int32 [batch, max_pages] (pt_sb elements from one row to the next): the pages of a sequence in
- * order.  lengths int32 [batch]: its keys, those that the step appends included.  max_pages * page_size is at most 2^20, batch at most 65535.
- * Tables and lengths are read as they are found in device memory: a length below 0 or above max_pages * page_size is clamped to it, and a page
- * outside [0, n_pages) is never accessed (a reading step takes the nearest one, an appending one leaves the token out).
+ *
+ * aa_paged_cache (host memory, read during the call only): keys, values [n_pages, n_kv_heads, page_size, head_dim] with element strides of page, head and
+ * row (_sp, _sh, _sn); page_size 16, 32, 64, 128 or 256, head_dim 128 or 64.  bounds [n_pages, n_kv_heads, 2, head_dim], contiguous: the smallest
+ * and the largest value of each channel over a page's keys (NaN where one is NaN), kept by aa_paged_append, read by sparse steps; may be NULL for others.
+ *
+ * page_table int32 [batch, max_pages] (pt_sb elements from one row to the next): the pages of a sequence in order.  lengths int32 [batch]: its
+ * keys, those that the step appends included.  max_pages * page_size is at most 2^20, batch at most 65535.  Both are read as they are found in device
+ * memory.  What reads the cache clamps a length to [0, max_pages * page_size] and a page to the nearest one there is; what
+ * appends leaves out tokens without a place.
  *
  * aa_paged_append: token t of sequence b, starts[b] <= t < starts[b + 1] (int32 [batch + 1], ascending; NULL: one token of each sequence), becomes key
  * lengths[b] - (starts[b + 1] - starts[b]) + t - starts[b] of the sequence, which is its position: k and (if not NULL) q are rotated by row
- * `position` of cos and sin (float32 [n_positions, head_dim / 2], cs_sn elements from row to row; first half' = first * cos - second * sin, second' = second * cos +
- * first * sin, in float32 with one rounding), k and v stored in the sequence's pages, q to q_out, which may be q.  cos and sin NULL: k is stored as
- * it is, and q must be NULL.  bounds (may be NULL): [n_pages, n_kv_heads, 2, head_dim], the smallest and the largest value of each channel over a
- * page's keys (NaN where one is NaN), set by a page's first key and widened by the others.  A token that has no place - behind the last sequence, at a position below 0, in no row
- * of cos and sin or in no page - is left out: nothing is read or written for it.  q, k, v, q_out: [n_tokens, heads, head_dim] with strides of token and
- * head (_st, _sh).  Two tokens for one place, or of two sequences for one page, give one or a mixture of both.
+ * `position` of cos and sin (float32 [n_positions, head_dim / 2], cs_sn elements from row to row; first half' = first * cos - second * sin, second' = second *
+ * cos + first * sin, in float32 with one rounding), k and v stored in the sequence's pages, q to q_out, which may be q.  cos and sin NULL: k is stored as it is, and
+ * q must be NULL and n_q_heads 0.  A page's bounds are set by its first key and widened by the others.  A token that has no place - behind the last
+ * sequence, at a position below 0, in no row of cos and sin, behind the table or in no page of the pool - is left out: nothing is written for it.
+ * q, k, v, q_out: [n_tokens, heads, head_dim] with strides of token and head (_st, _sh).  Two tokens for one place, or of two sequences for one page, give one or a
+ * mixture of both.
  *
  * aa_paged_decode_fwd: out[b, h] = softmax(q[b, h] . keys * sm_scale) values over the keys 0 .. lengths[b] - 1 of sequence b; a sequence of none gives 0.
  * q, out: [batch, n_q_heads, head_dim] with strides of sequence and head.  workspace: aa_paged_decode_workspace_bytes() bytes of device scratch, which
  * may be none (contents undefined afterwards).
  *
- * aa_paged_sparse_decode_fwd: the same over n_chosen pages for each sequence and KV head, or all where the sequence has no more: its first n_first, its last n_last (at
- * least 1) and those of the others whose score is largest, the lower page first among equal ones.  The score is the largest over the heads of the
+ * aa_paged_sparse_decode_fwd: the same over n_chosen pages for each sequence and KV head, or all where the sequence has no more: its first n_first, its last
+ * n_last (at least 1) and those of the others whose score is largest, the lower page first among equal ones.  The score is the largest over the heads of the
  * group of sum_d q_d * (q_d >= 0 ? largest_d : smallest_d), which no product of the query with a key of the page exceeds: a sum in float64, rounded to
  * float32; NaN counts as infinity.  pages int32 [batch, n_kv_heads, n_chosen], contiguous: the chosen ones (places in the sequence), ascending, then -1. */
-int aa_paged_append(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+typedef struct {
+  void* keys;
+  int64_t kp_sp, kp_sh, kp_sn;
+  void* values;
+  int64_t vp_sp, vp_sh, vp_sn;
+  void* bounds;
+  int n_pages, n_kv_heads, page_size, head_dim, dtype;
+} aa_paged_cache;
+
+int aa_paged_append(const aa_paged_cache* cache, const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
                     const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
                     const float* cos, const float* sin, int64_t cs_sn, int n_positions,
-                    void* keys, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn, void* values, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn, void* bounds,
                     const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, const int32_t* starts,
-                    int batch, int n_tokens, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size, int max_pages,
-                    int dtype, void* stream);
+                    int batch, int n_tokens, int n_q_heads, int max_pages, void* stream);
 size_t aa_paged_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages);
-int aa_paged_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
-                        const void* keys, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn, const void* values, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn,
+int aa_paged_decode_fwd(const aa_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
                         const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, void* workspace, size_t workspace_bytes,
-                        int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size, int max_pages,
-                        float sm_scale, int dtype, void* stream);
+                        int batch, int n_q_heads, int max_pages, float sm_scale, void* stream);
 size_t aa_paged_sparse_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_chosen);
-int aa_paged_sparse_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
-                               const void* keys, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn,
-                               const void* values, int64_t vp_sp, int64_t vp_sh, int64_t vp_sn, const void* bounds,
+int aa_paged_sparse_decode_fwd(const aa_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
                                const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, int32_t* pages, void* workspace, size_t workspace_bytes,
-                               int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_pages, int page_size, int max_pages,
-                               int n_chosen, int n_first, int n_last, float sm_scale, int dtype, void* stream);
+                               int batch, int n_q_heads, int max_pages, int n_chosen, int n_first, int n_last, float sm_scale, void* stream);
 
 #ifdef __cplusplus
 }

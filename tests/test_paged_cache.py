@@ -499,32 +499,33 @@ def test_two_streams_at_once():
 
 # ---- refusals ------------------------------------------------------------------------------------------------------
 
-APPEND = {"q": 4096, "q_st": 1024, "q_sh": 128, "q_out": 4096, "qo_st": 1024, "qo_sh": 128, "k": 4096, "k_st": 256, "k_sh": 128, "v": 4096, "v_st": 256, "v_sh": 128,
-          "cos": 4096, "sin": 4096, "cs_sn": 64, "n_positions": 100, "keys": 4096, "kp_sp": 4096, "kp_sh": 2048, "kp_sn": 128, "values": 4096, "vp_sp": 4096, "vp_sh": 2048,
-          "vp_sn": 128, "bounds": 4096, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "starts": 4096, "batch": 2, "n_tokens": 5, "n_q_heads": 8, "n_kv_heads": 2,
-          "head_dim": 128, "n_pages": 9, "page_size": 16, "max_pages": 8, "dtype": 0, "stream": None}
-DECODE = {"q": 4096, "q_sb": 1024, "q_sh": 128, "out": 4096, "o_sb": 1024, "o_sh": 128, "keys": 4096, "kp_sp": 4096, "kp_sh": 2048, "kp_sn": 128, "values": 4096, "vp_sp": 4096,
-          "vp_sh": 2048, "vp_sn": 128, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "workspace": 4096, "workspace_bytes": 1 << 40, "batch": 2, "n_q_heads": 8,
-          "n_kv_heads": 2, "head_dim": 128, "n_pages": 9, "page_size": 16, "max_pages": 8, "sm_scale": 0.1, "dtype": 0, "stream": None}
-SPARSE = {**{k: DECODE[k] for k in list(DECODE)[:14]}, "bounds": 4096, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "pages": 4096, "workspace": 4096,
-          "workspace_bytes": 1 << 40, **{k: DECODE[k] for k in list(DECODE)[19:26]}, "n_chosen": 4, "n_first": 1, "n_last": 1, "sm_scale": 0.1, "dtype": 0, "stream": None}
-CACHE = [({"batch": 0}, "must be positive"), ({"batch": 65536}, "not supported"), ({"n_kv_heads": 3}, "must divide"), ({"n_kv_heads": 0}, "must be positive"),
+CACHE = {"keys": 4096, "kp_sp": 4096, "kp_sh": 2048, "kp_sn": 128, "values": 4096, "vp_sp": 4096, "vp_sh": 2048, "vp_sn": 128, "bounds": 4096,
+         "n_pages": 9, "n_kv_heads": 2, "page_size": 16, "head_dim": 128, "dtype": 0}
+APPEND = {"cache": CACHE, "q": 4096, "q_st": 1024, "q_sh": 128, "q_out": 4096, "qo_st": 1024, "qo_sh": 128, "k": 4096, "k_st": 256, "k_sh": 128, "v": 4096, "v_st": 256,
+          "v_sh": 128, "cos": 4096, "sin": 4096, "cs_sn": 64, "n_positions": 100, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "starts": 4096, "batch": 2, "n_tokens": 5,
+          "n_q_heads": 8, "max_pages": 8, "stream": None}
+DECODE = {"cache": CACHE, "q": 4096, "q_sb": 1024, "q_sh": 128, "out": 4096, "o_sb": 1024, "o_sh": 128, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "workspace": 4096,
+          "workspace_bytes": 1 << 40, "batch": 2, "n_q_heads": 8, "max_pages": 100, "sm_scale": 0.1, "stream": None}
+SPARSE = {**{k: DECODE[k] for k in list(DECODE)[:10]}, "pages": 4096, **{k: DECODE[k] for k in list(DECODE)[10:15]}, "n_chosen": 4, "n_first": 1, "n_last": 1, "sm_scale": 0.1,
+          "stream": None}
+EVERY = [({"batch": 0}, "must be positive"), ({"batch": 65536}, "not supported"), ({"n_kv_heads": 3}, "must divide"), ({"n_kv_heads": 0}, "must be positive"),
          ({"head_dim": 96}, "head_dim 96"), ({"page_size": 48}, "page_size 48"), ({"page_size": 8}, "page_size 8"), ({"n_pages": 0}, "must be positive"),
          ({"max_pages": 0}, "must be positive"), ({"max_pages": 65537}, "not supported"), ({"dtype": 2}, "dtype"), ({"keys": 0}, "keys is NULL"),
          ({"keys": 4104}, "keys must be 16-byte aligned"), ({"kp_sh": 2052}, "keys must be 16-byte aligned"), ({"vp_sn": 120}, "smaller than head_dim"),
          ({"vp_sn": 16392}, "larger than 16384"), ({"values": 0}, "values is NULL"), ({"page_table": 0}, "page_table is NULL"), ({"lengths": 0}, "lengths is NULL"),
-         ({"lengths": 4098}, "lengths must be 4-byte aligned"), ({"q": 4104}, "q must be 16-byte aligned"), ({"q_sh": 60}, "q must have strides")]
+         ({"lengths": 4098}, "lengths must be 4-byte aligned"), ({"q": 4104}, "q must be 16-byte aligned"), ({"q_sh": 60}, "q must have strides"),
+         ({"bounds": 8}, "bounds must be 16-byte"), ({"cache": None}, "cache is NULL")]
 READ = [({"q": 0}, "q is NULL"), ({"out": 0}, "out is NULL"), ({"out": 8}, "out must be 16-byte"), ({"sm_scale": 0.0}, "sm_scale"), ({"sm_scale": float("nan")}, "sm_scale"),
         ({"sm_scale": float("inf")}, "sm_scale"), ({"n_q_heads": 0}, "query heads")]
 
 
 @pytest.mark.parametrize("fn,change,message", [
-    *[("append", c, m) for c, m in CACHE], *[("decode", c, m) for c, m in CACHE + READ], *[("sparse", c, m) for c, m in CACHE + READ],
-    ("append", {"n_tokens": 0}, "0 tokens"), ("append", {"n_tokens": 1 << 24}, "not supported"), ("append", {"starts": 0}, "5 tokens of 2 sequences"),
+    *[("append", c, m) for c, m in EVERY], *[("decode", c, m) for c, m in EVERY + READ], *[("sparse", c, m) for c, m in EVERY + READ],
+    ("append", {"n_tokens": 0}, "0 tokens"), ("append", {"n_tokens": 1 << 24}, "not supported"), ("append", {"n_tokens": 1 << 23}, "not supported"), ("decode", {"workspace_bytes": 100}, "workspace has 100 bytes"), ("decode", {"workspace": 0}, "workspace is NULL"), ("append", {"starts": 0}, "5 tokens of 2 sequences"),
     ("append", {"cos": 0}, "come together"), ("append", {"q": 0}, "come together"), ("append", {"q_out": 0}, "come together"), ("append", {"cos": 0, "sin": 0}, "come together"),
     ("append", {"n_q_heads": 0}, "come together"), ("append", {"cs_sn": 63}, "cos and sin"), ("append", {"cs_sn": 60}, "cos and sin"), ("append", {"n_positions": 0}, "cos and sin"),
     ("append", {"sin": 4100}, "sin must be 16-byte"), ("append", {"k": 0}, "k is NULL"), ("append", {"v": 4}, "v must be 16-byte"), ("append", {"v_st": 4}, "v must have strides"),
-    ("append", {"bounds": 8}, "bounds must be 16-byte"), ("append", {"starts": 6}, "starts must be 4-byte"),
+    ("append", {"starts": 6}, "starts must be 4-byte"),
     ("sparse", {"n_last": 0}, "at least the last one"), ("sparse", {"n_first": -1}, "not supported"), ("sparse", {"n_first": 4}, "not supported"),
     ("sparse", {"n_chosen": 65537}, "not supported"), ("sparse", {"n_chosen": 1}, "not supported"), ("sparse", {"bounds": 0}, "bounds is NULL"),
     ("sparse", {"pages": 0}, "pages is NULL"), ("sparse", {"workspace_bytes": 100}, "workspace has 100 bytes"), ("sparse", {"workspace": 0}, "workspace is NULL"),
@@ -533,9 +534,13 @@ def test_what_the_c_interface_refuses(fn, change, message):
     """Before anything is launched: the addresses are never read."""
     from anchor_attn.src.ops import _hip
     args, f = {"append": (APPEND, _hip.lib().aa_paged_append), "decode": (DECODE, _hip.lib().aa_paged_decode_fwd), "sparse": (SPARSE, _hip.lib().aa_paged_sparse_decode_fwd)}[fn]
-    assert len(args) == len(f.argtypes) and set(change) <= set(args)
+    assert len(args) == len(f.argtypes) and set(change) <= set(args) | set(CACHE)
+    args = {**args, **{k: v for k, v in change.items() if k in args}}
+    if args["cache"] is not None:
+        struct = _hip.PagedCacheStruct(*{**CACHE, **{k: v for k, v in change.items() if k in CACHE}}.values())
+        args["cache"] = ctypes.addressof(struct)
     with pytest.raises(_hip.AnchorAttnHipError, match=message):
-        _hip.check(f(*{**args, **change}.values()))
+        _hip.check(f(*args.values()))
 
 
 def test_caches_that_are_refused():
