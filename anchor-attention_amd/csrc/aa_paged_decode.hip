@@ -23,7 +23,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kCols = 16;       // columns of a unit: heads of the group
 constexpr int kTile = 32;       // keys of a tile
-constexpr int kWhole = 20;      // a unit of at most that many tiles is not cut
+constexpr int kOver = 2;        // what a unit costs beside its tiles, in tiles
+constexpr int kWhole = 20;      // a unit of at most that many tiles is not cut between work-groups
 constexpr int kShares = 512;    // work-groups
 constexpr int kSharesLog = 9;
 constexpr int kLeast = 4;       // tiles of a share
@@ -71,63 +72,79 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
   constexpr int kDV = D / 16;      // channels of V that a lane loads
   constexpr int kVW = kDV / 2;     // ... in words
   constexpr int kPitch = D + 4;
-  __shared__ __attribute__((aligned(16))) float accs[WAVES][kCols][kPitch];
-  __shared__ float stats[2][WAVES][kCols];
+  // States of units that a wave has a part of only: [wave][0: the first of its units, which began before; 1: its last, which goes on][column]
+  extern __shared__ __attribute__((aligned(16))) float states[];
+  __shared__ float stats[WAVES][2][2][kCols];
+  __shared__ int4 parts_of[WAVES][2];  // whether there is one, whether the unit ends in it; sequence, unit
 
   const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = p.n_q_heads / p.n_kv_heads, col_blocks = (group + kCols - 1) / kCols, units = p.n_kv_heads * col_blocks;
+  const int most_cols = min(group, kCols);
 
-  // ---- this work-group's share -------------------------------------------------------------------
+  // ---- this wave's share -------------------------------------------------------------------------
+  // All units one after the other, each as long as its tiles and kOver.  (Up to 64 sequences: one lane each, and their sums stay)
+  int n0 = 0, sum0 = 0;
+  auto scan = [&](const int i, int& n, int& sum) __attribute__((always_inline)) {  // of sequences i .. i + 63: lengths, and sums up to each
+    n = i + lane < p.batch ? tiles_of(p, i + lane) + kOver : 0;
+    sum = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += y;
+    }
+  };
   int64_t total = 0;
   for (int i = 0; i < p.batch; i += 64) {
-    int n = i + lane < p.batch ? tiles_of(p, i + lane) : 0;
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d, 64);
-    total += __builtin_amdgcn_readfirstlane(n);
+    scan(i, n0, sum0);
+    total += __builtin_amdgcn_readlane(sum0, 63);
   }
   total *= units;
-  int64_t share = (total + kShares - 1) >> kSharesLog;
-  share = share < kLeast ? kLeast : share;
-  int64_t at = share * blockIdx.x, end = min(at + share, total);
-  // a place among all tiles; one inside a unit that is not cut is its beginning
-  auto find = [&](const int64_t x, int64_t& snapped) {
+  // the unit of place x, the tile that is due there, and the place itself, which is the unit's beginning if that is near or `whole` and the unit is short
+  auto find = [&](int64_t& x, const bool whole) {
     PagedPlace f = {p.batch, 0, 0, 1};
     int64_t before = 0;
-    snapped = total;
     for (int i = 0; i < p.batch; i += 64) {
-      const int n = i + lane < p.batch ? tiles_of(p, i + lane) : 0;
-      int sum = n;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(sum, d, 64);
-        if (lane >= d) sum += y;
-      }
+      int n = n0, sum = sum0;
+      if (p.batch > 64) scan(i, n, sum);
       const int in = __popcll(__ballot((before + sum) * units <= x));  // sequences of these 64 that end at or before x
       if (in < 64 && i + in < p.batch) {
+        const uint32_t length = __builtin_amdgcn_readlane(n, in);
+        const uint32_t rest = (uint32_t)(x - (before + __builtin_amdgcn_readlane(sum, in) - length) * units);
         f.b = i + in;
-        f.n_tiles = __builtin_amdgcn_readlane(n, in);
-        const uint32_t rest = (uint32_t)(x - (before + __builtin_amdgcn_readlane(sum - n, in)) * units);
-        f.unit = rest / (uint32_t)f.n_tiles;
-        f.tile = rest - f.unit * f.n_tiles;
-        snapped = x;
-        if (f.n_tiles <= kWhole) {
-          snapped -= f.tile;
+        f.unit = rest / length;
+        f.n_tiles = length - kOver;
+        f.tile = rest - f.unit * length;
+        if (f.tile <= kOver || (whole && f.n_tiles <= kWhole)) {
+          x -= f.tile;
           f.tile = 0;
+        } else {
+          f.tile -= kOver;
         }
-        break;
+        return f;
       }
       before += __builtin_amdgcn_readlane(sum, 63);
     }
+    x = total;
     return f;
   };
-  int32_t* header = p.headers + 4 * blockIdx.x;
-  bool cut = false;
+  int64_t share = (total + kShares - 1) >> kSharesLog;
+  share = share < kLeast ? kLeast : share;
+  int64_t at = min(share * blockIdx.x, total), end = min(share * blockIdx.x + share, total);
   PagedPlace f = {0, 0, 0, 1};
-  if (at < total) {
-    if (end < total) find(end, end);
-    f = find(at, at);
+  if (at < end) {
+    if (end < total) find(end, true);
+    find(at, true);
+    // the waves' parts of it
+    const int64_t all = end - at, from = at + all * wave / WAVES, to = at + all * (wave + 1) / WAVES;
+    at = from;
+    if (wave + 1 < WAVES) {
+      end = to;
+      find(end, false);
+    }
+    f = find(at, false);
   }
+  if (lane < 2) parts_of[wave][lane] = int4{0, 0, 0, 0};
 
   const float scale = p.sm_scale * kLog2e;
   const uint32_t k_lane = (2u * (c16 * (uint32_t)p.kp_sn + 8 * g)) & 0xfffffu, v_lane = (2u * (4 * g * (uint32_t)p.vp_sn + kDV * c16)) & 0xfffffu;
@@ -204,20 +221,20 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     u = unit_of(f);
     load_q(q2, f, u);
     __builtin_amdgcn_sched_barrier(0);
-    const int t = f.tile + wave;
-    const Spot o = spot(u, t, t < min((int64_t)f.n_tiles, f.tile + (end - at)));
+    const Spot o = spot(u, f.tile, true);
     load_k(x, o);
     __builtin_amdgcn_sched_barrier(0);
     load_v(x, o);
   }
   while (at < end) {
     // ---- a unit's tiles [f.tile, last), and what comes after it -------------------------------------
-    const int last = (int)min((int64_t)f.n_tiles, f.tile + (end - at));
-    const int64_t at2 = at + (last - f.tile);
+    const int64_t unit_at = at - (f.tile ? f.tile + kOver : 0);
+    const int last = (int)min((int64_t)f.n_tiles, end - unit_at - kOver);
+    const int64_t at2 = last == f.n_tiles ? unit_at + f.n_tiles + kOver : end;
     PagedPlace f2 = f;
     Unit u2 = u;
-    int last2 = 0;
-    if (at2 < end) {
+    const bool more = at2 < end;
+    if (more) {
       f2.tile = 0;
       if (++f2.unit == units) {
         f2.unit = 0;
@@ -225,7 +242,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
         f2.n_tiles = __builtin_amdgcn_readfirstlane(tiles_of(p, f2.b));
       }
       u2 = unit_of(f2);
-      last2 = (int)min((int64_t)f2.n_tiles, end - at2);
     }
 #pragma unroll
     for (int s = 0; s < kKS; ++s) q[s] = q2[s];
@@ -306,14 +322,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
 
     // A tile's keys are read before its soft-max and its values after it, and each at once gives its registers to the next tile's, which is the
     // next unit's first where this one has no more.
-    for (int t = f.tile + wave; t < last; t += WAVES) {
-      const bool here = t + WAVES < last;
+    for (int t = f.tile; t < last; ++t) {
+      const bool here = t + 1 < last;
       Unit n;
       n.table = here ? u.table : u2.table;
       n.last_page = here ? u.last_page : u2.last_page;
       n.k_head = here ? u.k_head : u2.k_head;
       n.v_head = here ? u.v_head : u2.v_head;
-      const Spot o = spot(n, here ? t + WAVES : wave, here || wave < last2);
+      const Spot o = spot(n, here ? t + 1 : 0, here || more);
       floatx4 s[2];
       scores(x, s);
       __builtin_amdgcn_sched_barrier(0);
@@ -322,12 +338,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       u32x4 prob, rest;
       probabilities(s, t, prob, rest, false);
       add_values(x, t, prob, rest, false);
-      __builtin_amdgcn_sched_barrier(0);
-      load_v(x, o);
-    }
-    if (f.tile + wave >= last) {  // (a wave without a tile has loaded nothing for the next unit)
-      const Spot o = spot(u2, wave, wave < last2);
-      load_k(x, o);
       __builtin_amdgcn_sched_barrier(0);
       load_v(x, o);
     }
@@ -341,7 +351,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       l_run = 0.f;
 #pragma unroll
       for (int j = 0; j < kDV; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
-      for (int t = f.tile + wave; t < last; t += WAVES) {
+      for (int t = f.tile; t < last; ++t) {
         Tile y;
         const Spot o = spot(u, t, true);
         load_k(y, o);
@@ -355,43 +365,82 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       l_run = sum_over_quarters(l_run);
     }
 
-    // ---- the waves' states -> one ----------------------------------------------------------------
-    if (g == 0) {
-      stats[0][wave][c16] = m_run;
-      stats[1][wave][c16] = l_run;
-    }
-    if (c16 < n_cols) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < kDV; j += 4)
-          *reinterpret_cast<floatx4*>(&accs[wave][c16][kDV * (4 * g + r) + j]) = floatx4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
-    }
-    __syncthreads();
     const bool from_start = f.tile == 0, to_end = last == f.n_tiles;
-    const int part = 2 * blockIdx.x + (from_start ? 1 : 0);
+    if (from_start && to_end) {
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+      if (c16 < n_cols) {
+        uint16_t* op = p.out + f.b * p.o_sb + (int64_t)(head0 + c16) * p.o_sh + kDV * 4 * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < kDV; j += 4)
+            *reinterpret_cast<u32x2*>(op + kDV * r + j) = u32x2{T::pack(acc[j][r] * inv, acc[j + 1][r] * inv), T::pack(acc[j + 2][r] * inv, acc[j + 3][r] * inv)};
+      }
+    } else {
+      const int which = from_start ? 1 : 0;
+      if (g == 0) {
+        stats[wave][which][0][c16] = m_run;
+        stats[wave][which][1][c16] = l_run;
+      }
+      if (c16 < n_cols) {
+        float* to = states + ((2 * wave + which) * most_cols + c16) * kPitch + kDV * 4 * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < kDV; j += 4) *reinterpret_cast<floatx4*>(to + kDV * r + j) = floatx4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
+      }
+      // (where its last part lies, of work-groups)
+      if (lane == 0) parts_of[wave][which] = int4{1 + (int)to_end, f.b, f.unit, (int)((unit_at + f.n_tiles + kOver - 1) / share)};
+    }
+    at = at2;
+    f = f2;
+    u = u2;
+  }
+
+  // ---- the waves' parts of a unit -> one ------------------------------------------------------------
+  __syncthreads();
+  int4* header = reinterpret_cast<int4*>(p.headers) + blockIdx.x;
+  bool goes_on = false;
+  // the unit that began before this work-group, then those that begin in a wave and do not end there
+  for (int e = 0; e < 2 * WAVES;) {  // (entry 2 w + which of parts_of; waves without a share have none)
+    const int4 info = parts_of[e >> 1][e & 1];
+    const int first = e++;
+    if (info.x == 0) continue;
+    const bool begins = first & 1;
+    bool ends = info.x == 2;
+    uint32_t entries = 1u << first;  // of this unit
+    for (; e < 2 * WAVES && !ends; ++e) {
+      const int x = parts_of[e >> 1][e & 1].x;
+      if (x == 0) continue;
+      if (e & 1) break;
+      entries |= 1u << e;
+      ends = x == 2;
+    }
+    const int kvh = info.z / col_blocks, head0 = kvh * group + (info.z - kvh * col_blocks) * kCols, n_cols = min(kCols, (kvh + 1) * group - head0);
     for (int i = tid; i < n_cols * (D / 4); i += 64 * WAVES) {
       const int col = i / (D / 4), d = 4 * (i % (D / 4));
       float m = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stats[0][w][col]);
+      for (uint32_t left = entries; left; left &= left - 1) {
+        const int of = __builtin_ctz(left);
+        m = fmaxf(m, stats[of >> 1][of & 1][0][col]);
+      }
       float l = 0.f;
       floatx4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        const float mw = stats[0][w][col];
+      for (uint32_t left = entries; left; left &= left - 1) {
+        const int of = __builtin_ctz(left);
+        const float mw = stats[of >> 1][of & 1][0][col];
         const float weight = mw == -INFINITY ? 0.f : fast_exp2((mw - m) * scale);
-        l += weight * stats[1][w][col];
-        const floatx4 y = *reinterpret_cast<const floatx4*>(&accs[w][col][d]);
+        l += weight * stats[of >> 1][of & 1][1][col];
+        const floatx4 y = *reinterpret_cast<const floatx4*>(states + (of * most_cols + col) * kPitch + d);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] += weight * y[e];
       }
-      if (from_start && to_end) {
+      if (begins && ends) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint16_t* op = p.out + f.b * p.o_sb + (int64_t)(head0 + col) * p.o_sh + d;
+        uint16_t* op = p.out + info.y * p.o_sb + (int64_t)(head0 + col) * p.o_sh + d;
         *reinterpret_cast<u32x2*>(op) = u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
       } else {
-        const int64_t to = (int64_t)part * kCols + col;
+        const int64_t to = (int64_t)(2 * blockIdx.x + (begins ? 1 : 0)) * kCols + col;
         *reinterpret_cast<floatx4*>(p.parts + to * D + d) = x;
         if (d == 0) {
           p.part_stats[2 * to] = m;
@@ -399,17 +448,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
         }
       }
     }
-    if (from_start && !to_end) {  // the others of this unit's parts are the next work-groups'
-      cut = true;
-      const int parts = (int)((at - f.tile + f.n_tiles - 1) / share) - (int)blockIdx.x + 1;
-      if (tid == 0) *reinterpret_cast<int4*>(header) = int4{parts, f.b, head0, n_cols};
+    if (begins && !ends) {  // the unit's other parts are the next work-groups'
+      goes_on = true;
+      if (tid == 0) *header = int4{info.w - (int)blockIdx.x + 1, info.y, head0, n_cols};
     }
-    at = at2;
-    f = f2;
-    u = u2;
-    __syncthreads();  // (the accumulators have been read)
   }
-  if (!cut && tid == 0 && p.headers != nullptr) header[0] = 0;
+  if (!goes_on && tid == 0 && p.headers != nullptr) header->x = 0;
 }
 
 // Joins the parts of a column whose unit begins in share blockIdx.x and ends in another: the weights first, then groups of D / 4 lanes add up
@@ -478,9 +522,9 @@ PagedScratch paged_decode_scratch(int head_dim, int page_log, int max_pages) {
 
 template <typename T, int D>
 static void launch_paged_decode_for(const PagedDecodeArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_decode_kernel<T, D, 4>), dim3(kShares), dim3(256), 0, stream, a);
-  const int group = a.n_q_heads / a.n_kv_heads;
-  if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3(kShares, group < kCols ? group : kCols), dim3(256), 0, stream, a);
+  const int group = a.n_q_heads / a.n_kv_heads, cols = group < kCols ? group : kCols;
+  hipLaunchKernelGGL((paged_decode_kernel<T, D, 4>), dim3(kShares), dim3(256), (size_t)8 * cols * (D + 4) * 4, stream, a);
+  if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3(kShares, cols), dim3(256), 0, stream, a);
 }
 
 hipError_t launch_paged_decode(const PagedDecodeArgs& a, hipStream_t stream) {
