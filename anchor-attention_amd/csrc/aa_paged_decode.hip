@@ -23,11 +23,11 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kCols = 16;       // columns of a unit: heads of the group
 constexpr int kTile = 32;       // keys of a tile
-constexpr int kOver = 2;        // what a unit costs beside its tiles, in tiles
+constexpr int kOver = 3;        // what a unit costs beside its tiles, in tiles
 constexpr int kWhole = 20;      // a unit of at most that many tiles is not cut between work-groups
-constexpr int kShares = 512;    // work-groups
-constexpr int kSharesLog = 9;
-constexpr int kLeast = 4;       // tiles of a share
+constexpr int kShares = 256;    // work-groups
+constexpr int kSharesLog = 8;
+constexpr int kLeast = 8;       // tiles of a share
 
 template <typename T> __device__ __forceinline__ floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c);
 template <> __device__ __forceinline__ floatx4 mfma16<Bf16>(u32x4 a, u32x4 b, floatx4 c) {
@@ -57,13 +57,26 @@ __device__ __forceinline__ Rows rows_at(const uint16_t* base, const bool there) 
 }
 
 struct PagedPlace {  // of a tile, among all
-  int b, unit, tile, n_tiles;  // sequence, unit of it, tile of the unit, its tiles
+  int b, unit, tile;       // sequence, unit of it, tile of the unit
+  int n_tiles, length;     // of the sequence
+  int64_t start;           // the unit's beginning
 };
 
-__device__ __forceinline__ int tiles_of(const PagedDecodeArgs& p, const int b) {
-  int length = clamped_length(p.lengths, b, p.max_pages, p.page_log);
-  if (p.n_chosen) length -= max(0, pages_of(length, p.page_log) - p.n_chosen) << p.page_log;
-  return max(1, (length + kTile - 1) / kTile);  // (one of no keys has to be written too)
+// keys that are read of a sequence
+__device__ __forceinline__ int keys_of(const PagedDecodeArgs& p, const int length) {
+  const int n = min(max(length, 0), p.max_pages << p.page_log);
+  return p.n_chosen ? n - (max(0, pages_of(n, p.page_log) - p.n_chosen) << p.page_log) : n;
+}
+__device__ __forceinline__ int tiles_of(const int keys) { return max(1, (keys + kTile - 1) / kTile); }  // (a sequence of none has to be written too)
+
+// n / d where the quotient is below 2^16
+__device__ __forceinline__ uint32_t small_quotient(const uint32_t n, const uint32_t d) {
+  uint32_t q = (uint32_t)((float)n * __builtin_amdgcn_rcpf((float)d));
+  q = __builtin_amdgcn_readfirstlane(q);
+  // (off by one at most: three roundings of 2^-23 of a quotient below 2^16)
+  if (q * d > n) --q;
+  else if (n - q * d >= d) ++q;
+  return q;
 }
 
 template <typename T, int D, int WAVES>
@@ -84,65 +97,71 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
 
   // ---- this wave's share -------------------------------------------------------------------------
   // All units one after the other, each as long as its tiles and kOver.  (Up to 64 sequences: one lane each, and their sums stay)
-  int n0 = 0, sum0 = 0;
-  auto scan = [&](const int i, int& n, int& sum) __attribute__((always_inline)) {  // of sequences i .. i + 63: lengths, and sums up to each
-    n = i + lane < p.batch ? tiles_of(p, i + lane) + kOver : 0;
-    sum = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int y = __shfl_up(sum, d, 64);
-      if (lane >= d) sum += y;
-    }
+  int keys0 = 0, sum0 = 0;
+  auto scan = [&](const int i, int& keys, int& sum) __attribute__((always_inline)) {  // of sequences i .. i + 63: their keys, and the sums up to each
+    keys = i + lane < p.batch ? keys_of(p, p.lengths[i + lane]) : 0;
+    sum = sums_up_to(i + lane < p.batch ? tiles_of(keys) + kOver : 0);
   };
   int64_t total = 0;
   for (int i = 0; i < p.batch; i += 64) {
-    scan(i, n0, sum0);
+    scan(i, keys0, sum0);
     total += __builtin_amdgcn_readlane(sum0, 63);
   }
   total *= units;
-  // the unit of place x, the tile that is due there, and the place itself, which is the unit's beginning if that is near or `whole` and the unit is short
+  // x becomes the beginning of its unit if that is near or the unit is short and `whole`
+  auto settle = [&](PagedPlace& f, int64_t& x, const bool whole) __attribute__((always_inline)) {
+    f.tile = (int)(x - f.start) - kOver;
+    if (f.tile <= 0 || (whole && f.n_tiles <= kWhole)) {
+      f.tile = 0;
+      x = f.start;
+    }
+  };
+  // the place x < total
   auto find = [&](int64_t& x, const bool whole) {
-    PagedPlace f = {p.batch, 0, 0, 1};
+    PagedPlace f = {};
     int64_t before = 0;
-    for (int i = 0; i < p.batch; i += 64) {
-      int n = n0, sum = sum0;
-      if (p.batch > 64) scan(i, n, sum);
+    for (int i = 0;; i += 64) {
+      int keys = keys0, sum = sum0;
+      if (p.batch > 64) scan(i, keys, sum);
       const int in = __popcll(__ballot((before + sum) * units <= x));  // sequences of these 64 that end at or before x
-      if (in < 64 && i + in < p.batch) {
-        const uint32_t length = __builtin_amdgcn_readlane(n, in);
-        const uint32_t rest = (uint32_t)(x - (before + __builtin_amdgcn_readlane(sum, in) - length) * units);
+      if (in < 64 || i + 64 >= p.batch) {
         f.b = i + in;
-        f.unit = rest / length;
-        f.n_tiles = length - kOver;
-        f.tile = rest - f.unit * length;
-        if (f.tile <= kOver || (whole && f.n_tiles <= kWhole)) {
-          x -= f.tile;
-          f.tile = 0;
-        } else {
-          f.tile -= kOver;
-        }
+        f.length = __builtin_amdgcn_readlane(keys, in);
+        f.n_tiles = tiles_of(f.length);
+        const uint32_t extent = f.n_tiles + kOver;
+        const int64_t start = (before + __builtin_amdgcn_readlane(sum, in) - extent) * units;
+        f.unit = small_quotient((uint32_t)(x - start), extent);
+        f.start = start + (int64_t)f.unit * extent;
+        settle(f, x, whole);
         return f;
       }
       before += __builtin_amdgcn_readlane(sum, 63);
     }
-    x = total;
-    return f;
+  };
+  // the same for a place that is not before f's
+  auto find_from = [&](const PagedPlace& f, int64_t& x, const bool whole) {
+    if (x >= f.start + f.n_tiles + kOver) return find(x, whole);
+    PagedPlace r = f;
+    settle(r, x, whole);
+    return r;
   };
   int64_t share = (total + kShares - 1) >> kSharesLog;
   share = share < kLeast ? kLeast : share;
   int64_t at = min(share * blockIdx.x, total), end = min(share * blockIdx.x + share, total);
-  PagedPlace f = {0, 0, 0, 1};
+  PagedPlace f = {};
   if (at < end) {
-    if (end < total) find(end, true);
-    find(at, true);
+    f = find(at, true);
+    if (end < total) find_from(f, end, true);
     // the waves' parts of it
-    const int64_t all = end - at, from = at + all * wave / WAVES, to = at + all * (wave + 1) / WAVES;
-    at = from;
-    if (wave + 1 < WAVES) {
-      end = to;
-      find(end, false);
+    const int64_t all = end - at, to = at + all * (wave + 1) / WAVES;
+    at += all * wave / WAVES;
+    if (at < end) {
+      f = find_from(f, at, false);
+      if (wave + 1 < WAVES) {
+        end = to;
+        if (end < total) find_from(f, end, false);
+      }
     }
-    f = find(at, false);
   }
   if (lane < 2) parts_of[wave][lane] = int4{0, 0, 0, 0};
 
@@ -159,8 +178,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     u.kvh = f.unit / col_blocks;
     u.head0 = u.kvh * group + (f.unit - u.kvh * col_blocks) * kCols;
     u.n_cols = min(kCols, (u.kvh + 1) * group - u.head0);
-    u.length = __builtin_amdgcn_readfirstlane(clamped_length(p.lengths, f.b, p.max_pages, p.page_log));
-    if (p.n_chosen) u.length -= max(0, pages_of(u.length, p.page_log) - p.n_chosen) << p.page_log;
+    u.length = f.length;
     u.last_page = max(0, (u.length - 1) >> p.page_log);
     u.table = (const_i32*)(p.table + f.b * p.t_sb + u.kvh * p.t_sh);
     u.k_head = u.kvh * p.kp_sh;
@@ -228,18 +246,20 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
   }
   while (at < end) {
     // ---- a unit's tiles [f.tile, last), and what comes after it -------------------------------------
-    const int64_t unit_at = at - (f.tile ? f.tile + kOver : 0);
-    const int last = (int)min((int64_t)f.n_tiles, end - unit_at - kOver);
-    const int64_t at2 = last == f.n_tiles ? unit_at + f.n_tiles + kOver : end;
+    const int64_t unit_end = f.start + f.n_tiles + kOver;
+    const int last = (int)min((int64_t)f.n_tiles, end - f.start - kOver);
+    const int64_t at2 = min(unit_end, end);
     PagedPlace f2 = f;
     Unit u2 = u;
     const bool more = at2 < end;
     if (more) {
       f2.tile = 0;
+      f2.start = unit_end;
       if (++f2.unit == units) {
         f2.unit = 0;
         ++f2.b;
-        f2.n_tiles = __builtin_amdgcn_readfirstlane(tiles_of(p, f2.b));
+        f2.length = p.batch <= 64 ? __builtin_amdgcn_readlane(keys0, f2.b) : keys_of(p, ((const_i32*)p.lengths)[f2.b]);
+        f2.n_tiles = tiles_of(f2.length);
       }
       u2 = unit_of(f2);
     }
@@ -390,7 +410,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
           for (int j = 0; j < kDV; j += 4) *reinterpret_cast<floatx4*>(to + kDV * r + j) = floatx4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
       }
       // (where its last part lies, of work-groups)
-      if (lane == 0) parts_of[wave][which] = int4{1 + (int)to_end, f.b, f.unit, (int)((unit_at + f.n_tiles + kOver - 1) / share)};
+      if (lane == 0) parts_of[wave][which] = int4{1 + (int)to_end, f.b, f.unit, (int)((unit_end - 1) / share)};
     }
     at = at2;
     f = f2;
