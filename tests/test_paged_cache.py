@@ -603,3 +603,39 @@ def test_scratch_sizes():
     assert lib.aa_paged_sparse_workspace_bytes(0, 8, 2, 128, 16, 8, 4) == 0
     assert lib.aa_paged_sparse_workspace_bytes(2, 8, 2, 128, 16, 8, 4) >= 2 * 2 * (8 + 4) * 4
     assert isinstance(lib.aa_paged_decode_workspace_bytes(2, 8, 2, 128, 16, 8), int) and ctypes.sizeof(ctypes.c_size_t) == 8
+
+
+# ---- choices that a float32 sum leaves open --------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d,page,n_there,n_pages", [(64, 16, 300, 40), (128, 16, 700, 65), (128, 64, 1500, 100), (64, 16, 9000, 333)])
+def test_scores_that_differ_by_less_than_a_float32_sum_shows(d, page, n_there, n_pages, dtype):
+    """Large products of both signs that cancel and small ones that decide: neighbouring ranks differ by 2^-20 of the magnitudes and less; some are equal."""
+    s = _Setup([page * n_there - 3, page * 9], 2, d, page, dtype, n_there)
+    g = torch.Generator(device="cuda").manual_seed(n_there + d)
+    q = s.queries(6)
+    q[:, :, 0], q[:, :, 1], q[:, :, 2:] = 64.0, 64.0, q[:, :, 2:] * 2.0 ** -9
+    big = (torch.randint(0, 64, s.cache.bounds[:, :, :, 0].shape, generator=g, device="cuda").float() + 64.0)[:, :, :1]
+    s.cache.bounds[..., 0], s.cache.bounds[..., 1] = big.to(dtype), -big.to(dtype)
+    few = torch.randint(0, 40, (s.cache.n_pages, 1), generator=g, device="cuda").expand(-1, 2)  # (40 kinds of pages)
+    kinds = torch.randn(40, 2, d - 2, generator=g, device="cuda").to(dtype)
+    if n_there > 500:
+        s.cache.bounds[..., 2:] = s.cache.bounds[..., 2:].nan_to_num(0.25)
+    else:
+        s.cache.bounds[..., 2:] = kinds[few[:, :1]].expand(-1, 2, -1, -1)
+    for n in (3, n_pages, n_pages + 1, 270):
+        if n <= n_there:
+            assert torch.equal(_ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, n, 1, 1)[1], _chosen(q, s, n, 1, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,size", [(BF16, 1e-38), (F16, 1e-7), (F16, 2e-5), (BF16, 1e30), (F16, 3e4)])
+def test_scores_of_very_small_and_very_large_bounds(dtype, size):
+    s = _Setup([16 * 400], 2, 64, 16, dtype, 5)
+    s.cache.bounds.copy_((torch.randn(s.cache.bounds.shape, generator=s.g, device="cuda") * size).clamp(-6e4 if dtype == F16 else -3e38, 6e4 if dtype == F16 else 3e38).to(dtype))
+    s.cache.bounds[::3] = 0
+    for scale in (1.0, 1e-4, 1e4):
+        q = (s.queries(4).float() * scale).to(dtype)
+        for n in (3, 60, 350):
+            assert torch.equal(_ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, n, 1, 1)[1], _chosen(q, s, n, 1, 1))
