@@ -13,10 +13,14 @@
 
 namespace aa {
 
-constexpr int kAbreast = 4;        // pages of a lane
+// Pages of a lane: several share a head's queries and their sums' exchange, one leaves a wave soonest.
+constexpr int kAbreast = 4, kAbreastFused = 1;
+constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
 constexpr int kFused = 1024;       // a table of at most that many pages is scored and chosen from by one launch
 constexpr int kInLds = 8192;       // the scores of at most that many pages are kept in LDS
 constexpr int kMostPages = 1 << 16;
+constexpr int kListed = 1024;      // the chosen pages up to that many pass through LDS
+constexpr int kQueryWords = 4096;  // of LDS for a group's queries; those of more heads are read from memory
 
 // A score as an unsigned number of the same order, from 1 on; NaN as infinity, -0 as 0.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -25,40 +29,48 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
-// The scores of kPages consecutive pages of a sequence by one wave.
-template <typename T, int D>
+// The scores of kPages consecutive pages of a sequence by one wave, N by each lane.
+template <typename T, int D, int N>
 struct Scores {
-  static constexpr int kLanes = D / 8, kSide = 64 / kLanes, kPages = kSide * kAbreast;
+  static constexpr int kLanes = D / 8, kSide = 64 / kLanes, kPages = kSide * N;
+  static_assert(N == 4 || N == 2 || N == 1, "what the exchange is written for");
   struct Pages {  // of the pool
-    int at[kAbreast];
+    int at[N];
   };
   static __device__ __forceinline__ Pages find(const PagedSelectArgs& p, const int b, const int first) {
     const int32_t* table = p.table + b * p.t_sb;
     Pages x;
 #pragma unroll
-    for (int i = 0; i < kAbreast; ++i) x.at[i] = table[min(first + kSide * i + (int)(threadIdx.x & 63) / kLanes, p.max_pages - 1)];
+    for (int i = 0; i < N; ++i) x.at[i] = table[min(first + kSide * i + (int)(threadIdx.x & 63) / kLanes, p.max_pages - 1)];
     return x;
   }
-  // store(k, score) is called by one lane for each page, 0 <= k < kPages
-  template <typename Store>
-  static __device__ __forceinline__ void form(const PagedSelectArgs& p, const int b, const int kvh, const Pages& x, Store store) {
-    const int lane = threadIdx.x & 63, c = lane % kLanes, group = p.n_q_heads / p.n_kv_heads;
-    float bounds[kAbreast][2][8];
-    {
-      uint4 raw[kAbreast][2];
+  struct Bounds {
+    uint4 raw[N][2];
+  };
+  static __device__ __forceinline__ Bounds load(const PagedSelectArgs& p, const int kvh, const Pages& x) {
+    Bounds y;
 #pragma unroll
-      for (int i = 0; i < kAbreast; ++i) {  // (behind the last page the table holds anything)
-        const uint16_t* lo = p.bounds + ((int64_t)clamped_page(x.at[i], p.n_pages) * p.n_kv_heads + kvh) * 2 * D + 8 * c;
-        raw[i][0] = *reinterpret_cast<const uint4*>(lo);
-        raw[i][1] = *reinterpret_cast<const uint4*>(lo + D);
-      }
-#pragma unroll
-      for (int i = 0; i < kAbreast; ++i)
-#pragma unroll
-        for (int w = 0; w < 2; ++w) unpack8<T>(raw[i][w], bounds[i][w]);
+    for (int i = 0; i < N; ++i) {  // (behind the last page the table holds anything)
+      const uint16_t* lo = p.bounds + ((int64_t)clamped_page(x.at[i], p.n_pages) * p.n_kv_heads + kvh) * 2 * D + 8 * (threadIdx.x % kLanes);
+      y.raw[i][0] = *reinterpret_cast<const uint4*>(lo);
+      y.raw[i][1] = *reinterpret_cast<const uint4*>(lo + D);
     }
+    return y;
+  }
+  // `staged`: the group's queries one after the other (as many as stage() has room for).  store(k, score) is called by one lane for each page, 0 <= k < kPages
+  template <typename Store>
+  static __device__ __forceinline__ void form(const PagedSelectArgs& p, const int b, const int kvh, const Bounds& y, const uint32_t* staged, const int room, Store store) {
+    const int lane = threadIdx.x & 63, c = lane % kLanes, group = p.n_q_heads / p.n_kv_heads;
+    float bounds[N][2][8];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) unpack8<T>(y.raw[i][w], bounds[i][w]);
     const uint16_t* qp = p.q + b * p.q_sb + (int64_t)kvh * group * p.q_sh + 8 * c;
-    uint4 next = *reinterpret_cast<const uint4*>(qp);
+    auto query = [&](const int h) {
+      return h < room ? *reinterpret_cast<const uint4*>(staged + h * (D / 2) + 4 * c) : *reinterpret_cast<const uint4*>(qp + h * p.q_sh);
+    };
+    uint4 next = query(0);
     const bool odd = lane & 1, odd2 = lane & 2;
     float best = -INFINITY;
     bool nan = false;
@@ -66,26 +78,31 @@ struct Scores {
     for (int h = 1; h <= group; ++h) {
       float q[8];
       unpack8<T>(next, q);
-      next = *reinterpret_cast<const uint4*>(qp + min(h, group - 1) * p.q_sh);
-      double sum[kAbreast];
+      next = query(min(h, group - 1));
+      double sum[N];
 #pragma unroll
-      for (int i = 0; i < kAbreast; ++i) sum[i] = 0.0;
+      for (int i = 0; i < N; ++i) sum[i] = 0.0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const bool larger = q[j] >= 0.f;
 #pragma unroll
-        for (int i = 0; i < kAbreast; ++i) sum[i] += (double)(q[j] * (larger ? bounds[i][1][j] : bounds[i][0][j]));
+        for (int i = 0; i < N; ++i) sum[i] += (double)(q[j] * (larger ? bounds[i][1][j] : bounds[i][0][j]));
       }
       if (kLanes == 8) {  // (a lane and the one mirrored in their 8 then hold the same, and 4 neighbours all parts)
 #pragma unroll
-        for (int i = 0; i < kAbreast; ++i) sum[i] += dpp<kDppHalfMirror>(sum[i]);
+        for (int i = 0; i < N; ++i) sum[i] += dpp<kDppHalfMirror>(sum[i]);
       }
-      // a lane keeps the half of the sums that its bit names and gives the other half away
-      double a = odd ? sum[2] : sum[0], a2 = odd ? sum[3] : sum[1];
-      a += dpp<kDppXor1>(odd ? sum[0] : sum[2]);
-      a2 += dpp<kDppXor1>(odd ? sum[1] : sum[3]);
-      double s = odd2 ? a2 : a;
-      s += dpp<kDppXor2>(odd2 ? a : a2);
+      // while a lane has several it keeps the half that its bit names and gives the other half away
+      double half[2], s;
+      if (N == 4) {
+        half[0] = (odd ? sum[N / 2] : sum[0]) + dpp<kDppXor1>(odd ? sum[0] : sum[N / 2]);
+        half[1] = (odd ? sum[N - 1] : sum[N > 1 ? 1 : 0]) + dpp<kDppXor1>(odd ? sum[N > 1 ? 1 : 0] : sum[N - 1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) half[i] = sum[i] + dpp<kDppXor1>(sum[i]);
+      }
+      if (N > 1) s = (odd2 ? half[1] : half[0]) + dpp<kDppXor2>(odd2 ? half[0] : half[1]);
+      else s = half[0] + dpp<kDppXor2>(half[0]);
       if (kLanes == 16) {
         s += dpp<kDppRor8>(s);
         s += dpp<kDppRor4>(s);
@@ -93,36 +110,52 @@ struct Scores {
       nan = nan || s != s;
       best = fmaxf(best, (float)s);
     }
-    if (c < 4) store(kSide * ((odd ? 2 : 0) + (odd2 ? 1 : 0)) + lane / kLanes, nan ? INFINITY : best);
+    if (c < 4 && (N == 4 || !odd) && (N > 1 || !odd2)) store(kSide * ((odd ? 2 : 0) + (odd2 ? 1 : 0)) + lane / kLanes, nan ? INFINITY : best);
   }
 };
+
+// A group's queries to LDS by some threads, so that no head waits for memory; for how many heads there is room.
+template <int D>
+__device__ __forceinline__ int stage_queries(const PagedSelectArgs& p, const int b, const int kvh, uint32_t* staged, const int words, const int thread, const int threads) {
+  const int group = p.n_q_heads / p.n_kv_heads, room = min(group, words / (D / 2));
+  for (int i = thread; i < room * (D / 8); i += threads)
+    reinterpret_cast<uint4*>(staged)[i] =
+        *reinterpret_cast<const uint4*>(p.q + b * p.q_sb + (int64_t)(kvh * group + i / (D / 8)) * p.q_sh + 8 * (i % (D / 8)));
+  return room;
+}
 
 // A work-group's waves have neighbouring KV heads, whose bounds lie side by side, of the same pages of a sequence.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_scores_kernel(const PagedSelectArgs p) {
-  typedef Scores<T, D> S;
-  const int b = blockIdx.z, step = gridDim.x * S::kPages;
-  const int kvh = 4 * blockIdx.y + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  typedef Scores<T, D, kAbreast> S;
+  __shared__ __attribute__((aligned(16))) uint32_t staged[4][kQueryWords / 4];
+  const int b = blockIdx.z, step = gridDim.x * S::kPages, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kvh = min((int)(4 * blockIdx.y) + wave, p.n_kv_heads - 1);  // (a wave without one does the last one's once more)
   int first = blockIdx.x * S::kPages;
   typename S::Pages at = S::find(p, b, first);
   const int there = pages_of(clamped_length(p.lengths, b, p.max_pages, p.page_log), p.page_log);
-  if (there <= p.n_chosen || kvh >= p.n_kv_heads) return;
+  if (there <= p.n_chosen || first >= there) return;
+  typename S::Bounds y = S::load(p, kvh, at);
+  const int room = stage_queries<D>(p, b, kvh, staged[wave], kQueryWords / 4, threadIdx.x & 63, 64);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (read by the same wave only)
+  __builtin_amdgcn_wave_barrier();
+  at = S::find(p, b, first + step);
   float* scores = p.scores + ((int64_t)b * p.n_kv_heads + kvh) * p.max_pages;
-  for (; first < there; first += step) {
-    const typename S::Pages now = at;
-    at = S::find(p, b, first + step);
-    S::form(p, b, kvh, now, [&](const int k, const float x) {
+  for (;;) {
+    S::form(p, b, kvh, y, staged[wave], room, [&](const int k, const float x) {
       if (first + k < there) scores[first + k] = x;
     });
+    first += step;
+    if (first >= there) return;
+    y = S::load(p, kvh, at);
+    at = S::find(p, b, first + step);
   }
 }
 
 // FROM: 0 the scores are formed here, 1 they are read once, 2 as often as they are needed (more than LDS is to hold)
-constexpr int choose_threads(const int from) { return from == 0 ? 512 : 1024; }
 template <typename T, int D, int FROM>
-__global__ void __launch_bounds__(choose_threads(FROM)) paged_choose_kernel(const PagedSelectArgs p) {
-  typedef Scores<T, D> S;
-  constexpr int kChooseThreads = choose_threads(FROM), kChooseWaves = kChooseThreads / 64;
+__global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const PagedSelectArgs p) {
+  typedef Scores<T, D, kAbreastFused> S;
   constexpr int kMostItems = (FROM == 0 ? kFused : FROM == 1 ? kInLds : kMostPages) / kChooseThreads;
   __shared__ uint32_t kept[FROM == 0 ? kFused : FROM == 1 ? kInLds : 1];
   __shared__ uint32_t bins[4][256], ranges[2][kChooseWaves], counts[kMostItems * kChooseWaves], before[kMostItems * kChooseWaves];
@@ -133,6 +166,19 @@ __global__ void __launch_bounds__(choose_threads(FROM)) paged_choose_kernel(cons
   int32_t* pages = p.pages + unit * p.n_chosen;
   int32_t* chosen = p.chosen + unit * p.n_chosen;
   const int32_t* table = p.table + b * p.t_sb;
+  __shared__ __attribute__((aligned(16))) uint32_t staged[FROM == 0 ? kQueryWords : 1];
+  __shared__ int list[kListed];
+  // (what does not depend on the length is requested before it is known)
+  float early[2] = {0.f, 0.f};
+  typename S::Pages at;
+  int room = 0;
+  if (FROM == 0) {
+    at = S::find(p, b, wave * S::kPages);
+    room = stage_queries<D>(p, b, kvh, staged, kQueryWords, tid, kChooseThreads);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) early[j] = kChooseThreads * j + tid < p.max_pages ? scores[kChooseThreads * j + tid] : 0.f;
+  }
   const int there = pages_of(clamped_length(p.lengths, b, p.max_pages, p.page_log), p.page_log);
   if (there <= p.n_chosen) {
     for (int i = tid; i < p.n_chosen; i += kChooseThreads) {
@@ -143,14 +189,22 @@ __global__ void __launch_bounds__(choose_threads(FROM)) paged_choose_kernel(cons
   }
   const int first = p.n_first, last = there - p.n_last;  // the pages to choose from
   if (FROM == 0) {
+    typename S::Bounds y = S::load(p, kvh, at);
+    __syncthreads();
 #pragma nounroll
-    for (int i = wave * S::kPages; i < there; i += kChooseWaves * S::kPages)
-      S::form(p, b, kvh, S::find(p, b, i), [&](const int k, const float x) {
+    for (int i = wave * S::kPages; i < there;) {
+      S::form(p, b, kvh, y, staged, room, [&](const int k, const float x) {
         if (i + k < there) kept[i + k] = ordered(x);
       });
+      i += kChooseWaves * S::kPages;
+      if (i < there) y = S::load(p, kvh, S::find(p, b, i));
+    }
   }
   if (FROM == 1) {
-    for (int i = tid; i < there; i += kChooseThreads) kept[i] = ordered(scores[i]);
+    for (int j = 0; kChooseThreads * j < there; ++j) {
+      const int i = kChooseThreads * j + tid;
+      if (i < there) kept[i] = ordered(j == 0 ? early[0] : j == 1 ? early[1] : scores[i]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4 * 256; i += kChooseThreads) bins[0][i + tid] = 0u;
@@ -246,26 +300,34 @@ __global__ void __launch_bounds__(choose_threads(FROM)) paged_choose_kernel(cons
     const uint64_t below = (1ull << lane) - 1, equals = __ballot(x >= lo && x <= hi);
     const bool mine = x > hi || is_end(j) || (x >= lo && equal_before + __popcll(equals & below) < wanted);
     const uint64_t takes = __ballot(mine);
-    if (mine) pages[(packed & 0xffffu) + min(equal_before, wanted) + __popcll(takes & below)] = place(j);
+    if (mine) {
+      const int to = (packed & 0xffffu) + min(equal_before, wanted) + __popcll(takes & below);
+      if (to < kListed) list[to] = place(j);
+      else pages[to] = place(j);
+    }
   });
   __syncthreads();  // (the list is complete: its pages of the pool are read side by side)
-  for (int i = tid; i < p.n_chosen; i += kChooseThreads) chosen[i] = table[pages[i]];
+  for (int i = tid; i < p.n_chosen; i += kChooseThreads) {
+    const int page = i < kListed ? list[i] : pages[i];
+    if (i < kListed) pages[i] = page;
+    chosen[i] = table[page];
+  }
 }
 
 template <typename T, int D>
 static void launch_paged_select_for(const PagedSelectArgs& a, hipStream_t stream) {
   const dim3 units(a.n_kv_heads, a.batch);
   if (a.max_pages <= kFused) {
-    hipLaunchKernelGGL((paged_choose_kernel<T, D, 0>), units, dim3(choose_threads(0)), 0, stream, a);
+    hipLaunchKernelGGL((paged_choose_kernel<T, D, 0>), units, dim3(kChooseThreads), 0, stream, a);
     return;
   }
   // (some four thousand work-groups, however long the table is and however short the sequences)
-  const int chunks = (a.max_pages + Scores<T, D>::kPages - 1) / Scores<T, D>::kPages, fours = (a.n_kv_heads + 3) / 4;
+  const int chunks = (a.max_pages + Scores<T, D, kAbreast>::kPages - 1) / Scores<T, D, kAbreast>::kPages, fours = (a.n_kv_heads + 3) / 4;
   const int64_t n = (int64_t)fours * a.batch;
   const int side = (int)((4096 + n - 1) / n);
   hipLaunchKernelGGL((paged_scores_kernel<T, D>), dim3(chunks < side ? chunks : side, fours, a.batch), dim3(256), 0, stream, a);
-  if (a.max_pages <= kInLds) hipLaunchKernelGGL((paged_choose_kernel<T, D, 1>), units, dim3(choose_threads(1)), 0, stream, a);
-  else hipLaunchKernelGGL((paged_choose_kernel<T, D, 2>), units, dim3(choose_threads(2)), 0, stream, a);
+  if (a.max_pages <= kInLds) hipLaunchKernelGGL((paged_choose_kernel<T, D, 1>), units, dim3(kChooseThreads), 0, stream, a);
+  else hipLaunchKernelGGL((paged_choose_kernel<T, D, 2>), units, dim3(kChooseThreads), 0, stream, a);
 }
 
 hipError_t launch_paged_select(const PagedSelectArgs& a, hipStream_t stream) {
