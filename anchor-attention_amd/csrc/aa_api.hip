@@ -979,6 +979,10 @@ static int paged_decode_args(const char* who, PagedDecodeArgs& a, const aa_paged
     set_error("%s: %d query heads and sm_scale %g: both must be positive and finite", who, n_q_heads, (double)sm_scale);
     return AA_EBADARG;
   }
+  if ((int64_t)batch * n_q_heads >= 1 << 24) {
+    set_error("%s: %d sequences of %d query heads are not supported (fewer than 2^24 together)", who, batch, n_q_heads);
+    return AA_EUNSUPPORTED;
+  }
   if ((rc = check_rows(q, q_sb, q_sh, who, "q")) || (rc = check_rows(out, o_sb, o_sh, who, "out")) || (needed > 0 && (rc = check_ptr(workspace, who, "workspace"))))
     return rc;
   if (workspace_bytes < needed) {

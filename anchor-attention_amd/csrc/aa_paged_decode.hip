@@ -27,6 +27,7 @@ constexpr int kOver = 3;        // what a unit costs beside its tiles, in tiles
 constexpr int kWhole = 20;      // a unit of at most that many tiles is not cut between work-groups
 constexpr int kShares = 256;    // work-groups
 constexpr int kSharesLog = 8;
+constexpr int kPerLane = 4;     // sequences that a lane counts
 constexpr int kLeast = 8;       // tiles of a share
 
 template <typename T> __device__ __forceinline__ floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c);
@@ -56,10 +57,12 @@ __device__ __forceinline__ Rows rows_at(const uint16_t* base, const bool there) 
   return __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)hi << 32 | lo), 0, there ? 0x7fffffff : 0, 0x00020000);
 }
 
-struct PagedPlace {  // of a tile, among all
-  int b, unit, tile;       // sequence, unit of it, tile of the unit
-  int n_tiles, length;     // of the sequence
-  int64_t start;           // the unit's beginning
+// Place: an integer that counts the tiles of all units
+template <typename Place>
+struct PagedPlace {       // of a tile, among all
+  int b, unit, tile;      // sequence, unit of it, tile of the unit
+  int n_tiles, length;    // of the sequence
+  Place start;            // the unit's beginning
 };
 
 // keys that are read of a sequence
@@ -79,7 +82,7 @@ __device__ __forceinline__ uint32_t small_quotient(const uint32_t n, const uint3
   return q;
 }
 
-template <typename T, int D, int WAVES>
+template <typename T, int D, int WAVES, typename Place>
 __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const PagedDecodeArgs p) {
   constexpr int kKS = D / 32;      // MFMAs of a score
   constexpr int kDV = D / 16;      // channels of V that a lane loads
@@ -88,7 +91,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
   // States of units that a wave has a part of only: [wave][0: the first of its units, which began before; 1: its last, which goes on][column]
   extern __shared__ __attribute__((aligned(16))) float states[];
   __shared__ float stats[WAVES][2][2][kCols];
-  __shared__ int4 parts_of[WAVES][2];  // whether there is one, whether the unit ends in it; sequence, unit
+  __shared__ int4 parts_of[WAVES][2];  // 0 if there is none, 2 if the unit ends in it; sequence; first head, and columns in the upper half; parts of work-groups
 
   const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -96,20 +99,37 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
   const int most_cols = min(group, kCols);
 
   // ---- this wave's share -------------------------------------------------------------------------
-  // All units one after the other, each as long as its tiles and kOver.  (Up to 64 sequences: one lane each, and their sums stay)
-  int keys0 = 0, sum0 = 0;
-  auto scan = [&](const int i, int& keys, int& sum) __attribute__((always_inline)) {  // of sequences i .. i + 63: their keys, and the sums up to each
-    keys = i + lane < p.batch ? keys_of(p, p.lengths[i + lane]) : 0;
-    sum = sums_up_to(i + lane < p.batch ? tiles_of(keys) + kOver : 0);
+  // All units one after the other, each as long as its tiles and kOver.  A lane has kPerLane sequences in a row, a scan 64 lanes' (whose numbers stay if
+  // there are no more)
+  int keys0[kPerLane], sum0 = 0;
+  auto scan = [&](const int i, int (&keys)[kPerLane], int& sum) __attribute__((always_inline)) {  // of the sequences from i on: their keys, and the sums up to each lane's last
+    int own = 0;
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+      const int b = i + kPerLane * lane + j;
+      keys[j] = b < p.batch ? keys_of(p, p.lengths[b]) : 0;
+      own += b < p.batch ? tiles_of(keys[j]) + kOver : 0;
+    }
+    sum = sums_up_to(own);
   };
-  int64_t total = 0;
-  for (int i = 0; i < p.batch; i += 64) {
+  auto keys_at = [&](const int (&keys)[kPerLane], const int at) {  // of the at-th sequence of a scan
+    int x = __builtin_amdgcn_readlane(keys[0], at / kPerLane);
+#pragma unroll
+    for (int j = 1; j < kPerLane; ++j) {
+      const int y = __builtin_amdgcn_readlane(keys[j], at / kPerLane);
+      x = at % kPerLane == j ? y : x;
+    }
+    return x;
+  };
+  constexpr int kScan = 64 * kPerLane;
+  Place total = 0;
+  for (int i = 0; i < p.batch; i += kScan) {
     scan(i, keys0, sum0);
     total += __builtin_amdgcn_readlane(sum0, 63);
   }
   total *= units;
   // x becomes the beginning of its unit if that is near or the unit is short and `whole`
-  auto settle = [&](PagedPlace& f, int64_t& x, const bool whole) __attribute__((always_inline)) {
+  auto settle = [&](PagedPlace<Place>& f, Place& x, const bool whole) __attribute__((always_inline)) {
     f.tile = (int)(x - f.start) - kOver;
     if (f.tile <= 0 || (whole && f.n_tiles <= kWhole)) {
       f.tile = 0;
@@ -117,21 +137,32 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     }
   };
   // the place x < total
-  auto find = [&](int64_t& x, const bool whole) {
-    PagedPlace f = {};
-    int64_t before = 0;
-    for (int i = 0;; i += 64) {
-      int keys = keys0, sum = sum0;
-      if (p.batch > 64) scan(i, keys, sum);
-      const int in = __popcll(__ballot((before + sum) * units <= x));  // sequences of these 64 that end at or before x
-      if (in < 64 || i + 64 >= p.batch) {
-        f.b = i + in;
-        f.length = __builtin_amdgcn_readlane(keys, in);
-        f.n_tiles = tiles_of(f.length);
-        const uint32_t extent = f.n_tiles + kOver;
-        const int64_t start = (before + __builtin_amdgcn_readlane(sum, in) - extent) * units;
-        f.unit = small_quotient((uint32_t)(x - start), extent);
-        f.start = start + (int64_t)f.unit * extent;
+  auto find = [&](Place& x, const bool whole) {
+    PagedPlace<Place> f = {};
+    Place before = 0;
+    for (int i = 0;; i += kScan) {
+      int keys[kPerLane], sum = sum0;
+#pragma unroll
+      for (int j = 0; j < kPerLane; ++j) keys[j] = keys0[j];
+      if (p.batch > kScan) scan(i, keys, sum);
+      const int in = __popcll(__ballot((before + sum) * units <= x));  // lanes whose sequences end at or before x
+      if (in < 64 || i + kScan >= p.batch) {
+        f.start = in > 0 ? (before + __builtin_amdgcn_readlane(sum, in - 1)) * units : before * units;
+        uint32_t extent = 1;
+#pragma unroll
+        for (int j = 0; j < kPerLane; ++j) {  // (its last sequence that begins at or before x)
+          const int length = __builtin_amdgcn_readlane(keys[j], in), tiles = tiles_of(length);
+          const Place next = f.start + (Place)extent * units;
+          if (j == 0 || (next <= x && i + kPerLane * in + j < p.batch)) {
+            if (j > 0) f.start = next;
+            f.b = i + kPerLane * in + j;
+            f.length = length;
+            f.n_tiles = tiles;
+            extent = tiles + kOver;
+          }
+        }
+        f.unit = small_quotient((uint32_t)(x - f.start), extent);
+        f.start += (Place)f.unit * (Place)extent;
         settle(f, x, whole);
         return f;
       }
@@ -139,21 +170,20 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     }
   };
   // the same for a place that is not before f's
-  auto find_from = [&](const PagedPlace& f, int64_t& x, const bool whole) {
+  auto find_from = [&](const PagedPlace<Place>& f, Place& x, const bool whole) {
     if (x >= f.start + f.n_tiles + kOver) return find(x, whole);
-    PagedPlace r = f;
+    PagedPlace<Place> r = f;
     settle(r, x, whole);
     return r;
   };
-  int64_t share = (total + kShares - 1) >> kSharesLog;
-  share = share < kLeast ? kLeast : share;
-  int64_t at = min(share * blockIdx.x, total), end = min(share * blockIdx.x + share, total);
-  PagedPlace f = {};
+  const Place share = max((total + (kShares - 1)) >> kSharesLog, (Place)kLeast), raw = share * (Place)blockIdx.x;
+  Place at = min(raw, total), end = min(raw + share, total);
+  PagedPlace<Place> f = {};
   if (at < end) {
     f = find(at, true);
     if (end < total) find_from(f, end, true);
     // the waves' parts of it
-    const int64_t all = end - at, to = at + all * (wave + 1) / WAVES;
+    const Place all = end - at, to = at + all * (wave + 1) / WAVES;
     at += all * wave / WAVES;
     if (at < end) {
       f = find_from(f, at, false);
@@ -173,9 +203,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     int64_t k_head, v_head;
     int length, last_page, kvh, head0, n_cols;
   };
-  auto unit_of = [&](const PagedPlace& f) __attribute__((always_inline)) {
+  auto unit_of = [&](const PagedPlace<Place>& f) __attribute__((always_inline)) {
     Unit u;
-    u.kvh = f.unit / col_blocks;
+    u.kvh = col_blocks == 1 ? f.unit : f.unit / col_blocks;
     u.head0 = u.kvh * group + (f.unit - u.kvh * col_blocks) * kCols;
     u.n_cols = min(kCols, (u.kvh + 1) * group - u.head0);
     u.length = f.length;
@@ -227,7 +257,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     }
   };
   u32x4 q[kKS], q2[kKS];
-  auto load_q = [&](u32x4 (&q)[kKS], const PagedPlace& f, const Unit& u) __attribute__((always_inline)) {
+  auto load_q = [&](u32x4 (&q)[kKS], const PagedPlace<Place>& f, const Unit& u) __attribute__((always_inline)) {
     const uint16_t* qp = p.q + f.b * p.q_sb + (int64_t)(u.head0 + min(c16, u.n_cols - 1)) * p.q_sh + 8 * g;
 #pragma unroll
     for (int s = 0; s < kKS; ++s) q[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s);
@@ -246,10 +276,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
   }
   while (at < end) {
     // ---- a unit's tiles [f.tile, last), and what comes after it -------------------------------------
-    const int64_t unit_end = f.start + f.n_tiles + kOver;
-    const int last = (int)min((int64_t)f.n_tiles, end - f.start - kOver);
-    const int64_t at2 = min(unit_end, end);
-    PagedPlace f2 = f;
+    const Place unit_end = f.start + f.n_tiles + kOver;
+    const int last = (int)min((Place)f.n_tiles, end - f.start - kOver);
+    const Place at2 = min(unit_end, end);
+    PagedPlace<Place> f2 = f;
     Unit u2 = u;
     const bool more = at2 < end;
     if (more) {
@@ -258,7 +288,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       if (++f2.unit == units) {
         f2.unit = 0;
         ++f2.b;
-        f2.length = p.batch <= 64 ? __builtin_amdgcn_readlane(keys0, f2.b) : keys_of(p, ((const_i32*)p.lengths)[f2.b]);
+        f2.length = p.batch <= kScan ? keys_at(keys0, f2.b) : keys_of(p, ((const_i32*)p.lengths)[f2.b]);
         f2.n_tiles = tiles_of(f2.length);
       }
       u2 = unit_of(f2);
@@ -409,8 +439,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
 #pragma unroll
           for (int j = 0; j < kDV; j += 4) *reinterpret_cast<floatx4*>(to + kDV * r + j) = floatx4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
       }
-      // (where its last part lies, of work-groups)
-      if (lane == 0) parts_of[wave][which] = int4{1 + (int)to_end, f.b, f.unit, (int)((unit_end - 1) / share)};
+      // (how many shares its places from this one's beginning on are)
+      if (lane == 0) {
+        const uint32_t left = (uint32_t)(unit_end - 1 - raw);
+        parts_of[wave][which] = int4{1 + (int)to_end, f.b, n_cols << 16 | head0, share > (Place)left ? 1 : 1 + (int)(left / (uint32_t)share)};
+      }
     }
     at = at2;
     f = f2;
@@ -436,22 +469,24 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       entries |= 1u << e;
       ends = x == 2;
     }
-    const int kvh = info.z / col_blocks, head0 = kvh * group + (info.z - kvh * col_blocks) * kCols, n_cols = min(kCols, (kvh + 1) * group - head0);
+    const int head0 = info.z & 0xffff, n_cols = info.z >> 16;
     for (int i = tid; i < n_cols * (D / 4); i += 64 * WAVES) {
       const int col = i / (D / 4), d = 4 * (i % (D / 4));
-      float m = -INFINITY;
-      for (uint32_t left = entries; left; left &= left - 1) {
-        const int of = __builtin_ctz(left);
-        m = fmaxf(m, stats[of >> 1][of & 1][0][col]);
+      float m = -INFINITY, ms[WAVES];
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {  // (one entry a wave: the second of the one that the unit begins in, the first of others)
+        ms[w] = entries >> (2 * w) & 3u ? stats[w][2 * w + 1 == first][0][col] : -INFINITY;
+        m = fmaxf(m, ms[w]);
       }
       float l = 0.f;
       floatx4 x = {0.f, 0.f, 0.f, 0.f};
-      for (uint32_t left = entries; left; left &= left - 1) {
-        const int of = __builtin_ctz(left);
-        const float mw = stats[of >> 1][of & 1][0][col];
-        const float weight = mw == -INFINITY ? 0.f : fast_exp2((mw - m) * scale);
-        l += weight * stats[of >> 1][of & 1][1][col];
-        const floatx4 y = *reinterpret_cast<const floatx4*>(states + (of * most_cols + col) * kPitch + d);
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        if (!(entries >> (2 * w) & 3u)) continue;
+        const int k = 2 * w + 1 == first;
+        const float weight = ms[w] == -INFINITY ? 0.f : fast_exp2((ms[w] - m) * scale);
+        l += weight * stats[w][k][1][col];
+        const floatx4 y = *reinterpret_cast<const floatx4*>(states + ((2 * w + k) * most_cols + col) * kPitch + d);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] += weight * y[e];
       }
@@ -470,7 +505,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     }
     if (begins && !ends) {  // the unit's other parts are the next work-groups'
       goes_on = true;
-      if (tid == 0) *header = int4{info.w - (int)blockIdx.x + 1, info.y, head0, n_cols};
+      if (tid == 0) *header = int4{info.w, info.y, head0, n_cols};
     }
   }
   if (!goes_on && tid == 0 && p.headers != nullptr) header->x = 0;
@@ -481,7 +516,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArgs p) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
-  __shared__ float weight[kShares], red[2][4];
+  __shared__ float weight[256], red[2][4];
   __shared__ floatx4 sums[kGroups][kLanes];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = blockIdx.y;
   const int4 header = *reinterpret_cast<const int4*>(p.headers + 4 * blockIdx.x);
@@ -490,27 +525,36 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArg
   const float scale = p.sm_scale * kLog2e;
   // the first part is the second of its share, the others the first of theirs
   auto part = [&](const int i) { return ((int64_t)2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kCols + col; };
-  float m = -INFINITY, l = 0.f;
-  for (int i = tid; i < parts; i += 256) m = fmaxf(m, p.part_stats[2 * part(i)]);
+  static_assert(kShares <= 256, "a thread has a part's maximum and sum");
+  const int gr = tid / kLanes, d4 = tid % kLanes;
+  floatx4 early[4];  // (requested with the maxima)
+#pragma unroll
+  for (int j = 0; j < 4; ++j) early[j] = *reinterpret_cast<const floatx4*>(p.parts + part(min(gr + j * kGroups, parts - 1)) * D + 4 * d4);
+  const float mine = tid < parts ? p.part_stats[2 * part(tid)] : -INFINITY;
+  float l = tid < parts ? p.part_stats[2 * part(tid) + 1] : 0.f;
+  float m = mine;
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
   if (lane == 0) red[0][wave] = m;
   __syncthreads();
   m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  for (int i = tid; i < parts; i += 256) {
-    const float mi = p.part_stats[2 * part(i)];
-    const float w = mi == -INFINITY ? 0.f : fast_exp2((mi - m) * scale);
-    weight[i] = w;
-    l += w * p.part_stats[2 * part(i) + 1];
-  }
+  const float w = mine == -INFINITY ? 0.f : fast_exp2((mine - m) * scale);
+  weight[tid] = w;
+  l *= w;
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
   if (lane == 0) red[1][wave] = l;
   __syncthreads();
-  const int gr = tid / kLanes, d4 = tid % kLanes;
   floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (gr + j * kGroups < parts) {
+      const float w = weight[gr + j * kGroups];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += w * early[j][e];
+    }
 #pragma unroll 4
-  for (int i = gr; i < parts; i += kGroups) {
+  for (int i = gr + 4 * kGroups; i < parts; i += kGroups) {
     const floatx4 x = *reinterpret_cast<const floatx4*>(p.parts + part(i) * D + 4 * d4);
     const float w = weight[i];
 #pragma unroll
@@ -542,8 +586,12 @@ PagedScratch paged_decode_scratch(int head_dim, int page_log, int max_pages) {
 
 template <typename T, int D>
 static void launch_paged_decode_for(const PagedDecodeArgs& a, hipStream_t stream) {
-  const int group = a.n_q_heads / a.n_kv_heads, cols = group < kCols ? group : kCols;
-  hipLaunchKernelGGL((paged_decode_kernel<T, D, 4>), dim3(kShares), dim3(256), (size_t)8 * cols * (D + 4) * 4, stream, a);
+  const int group = a.n_q_heads / a.n_kv_heads, cols = group < kCols ? group : kCols, units = a.n_kv_heads * ((group + kCols - 1) / kCols);
+  const size_t lds = (size_t)8 * cols * (D + 4) * 4;
+  // (places fit 32 bits unless thousands of sequences have tables for a million keys)
+  const int64_t most = (int64_t)a.batch * units * (((int64_t)a.max_pages << a.page_log) / kTile + 1 + kOver);
+  if (most < 1ll << 30) hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int>), dim3(kShares), dim3(256), lds, stream, a);
+  else hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int64_t>), dim3(kShares), dim3(256), lds, stream, a);
   if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3(kShares, cols), dim3(256), 0, stream, a);
 }
 

@@ -262,7 +262,7 @@ LENGTHS = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129, 255, 257, 500,
     (LENGTHS, 32, 8, 128, 64, "heads"), (LENGTHS, 28, 4, 128, 16, "rows"), (LENGTHS, 14, 2, 64, 16, "heads"), (LENGTHS, 32, 8, 64, 32, "part"),
     (LENGTHS, 3, 3, 128, 256, "heads"), ([700, 1, 33], 16, 1, 64, 128, "heads"), ([700, 1, 33], 17, 1, 128, 128, "rows"), ([900, 0], 71, 1, 64, 64, "heads"),
     ([20001], 32, 8, 128, 64, "heads"), ([9000, 40, 12345], 28, 4, 64, 16, "heads"), ([5], 14, 2, 64, 16, "heads"), ([0], 4, 2, 128, 16, "heads"),
-    ([70001], 8, 1, 128, 256, "rows"), ([1] * 300, 14, 2, 64, 16, "heads"), ([33, 7] * 500, 4, 1, 128, 32, "heads"), ([4097] + [3] * 63, 8, 2, 128, 64, "heads"),
+    ([70001], 8, 1, 128, 256, "rows"), ([700] * 130 + [5000], 8, 2, 64, 64, "heads"), ([2500, 0, 0, 1] * 30, 4, 1, 64, 32, "heads"), ([700, 650, 641, 640, 639] * 60, 2, 2, 64, 32, "heads"), ([1] * 300, 14, 2, 64, 16, "heads"), ([33, 7] * 500, 4, 1, 128, 32, "heads"), ([4097] + [3] * 63, 8, 2, 128, 64, "heads"),
 ])
 def test_decode(lengths, hq, hkv, d, page, layout, dtype):
     s = _Setup(lengths, hkv, d, page, dtype, hq + page, layout, extra=hq % 3)
@@ -516,7 +516,7 @@ EVERY = [({"batch": 0}, "must be positive"), ({"batch": 65536}, "not supported")
          ({"lengths": 4098}, "lengths must be 4-byte aligned"), ({"q": 4104}, "q must be 16-byte aligned"), ({"q_sh": 60}, "q must have strides"),
          ({"bounds": 8}, "bounds must be 16-byte"), ({"cache": None}, "cache is NULL")]
 READ = [({"q": 0}, "q is NULL"), ({"out": 0}, "out is NULL"), ({"out": 8}, "out must be 16-byte"), ({"sm_scale": 0.0}, "sm_scale"), ({"sm_scale": float("nan")}, "sm_scale"),
-        ({"sm_scale": float("inf")}, "sm_scale"), ({"n_q_heads": 0}, "query heads")]
+        ({"sm_scale": float("inf")}, "sm_scale"), ({"n_q_heads": 0}, "query heads"), ({"batch": 4096, "n_q_heads": 4096}, "together")]
 
 
 @pytest.mark.parametrize("fn,change,message", [
@@ -639,3 +639,17 @@ def test_scores_of_very_small_and_very_large_bounds(dtype, size):
         q = (s.queries(4).float() * scale).to(dtype)
         for n in (3, 60, 350):
             assert torch.equal(_ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, n, 1, 1)[1], _chosen(q, s, n, 1, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_tables_so_wide_that_places_need_64_bits(d):
+    """2100 sequences, 16 KV heads, tables for a million keys: the same bits as with tables that are as wide as they need be."""
+    g = torch.Generator().manual_seed(d)
+    s = _Setup([int(x) for x in torch.randint(0, 40, (2098,), generator=g)] + [3001, 900], 16, d, 256, BF16, 7)
+    q = s.queries(16)
+    wide = torch.full((2100, 4096), -1, dtype=torch.int32, device="cuda")
+    wide[:, :s.table.shape[1]] = s.table
+    assert torch.equal(_ops().paged_decode_attention(s.cache, q, wide, s.lengths), _ops().paged_decode_attention(s.cache, q, s.table, s.lengths))
+    for a, b in zip(_ops().paged_sparse_decode_attention(s.cache, q, wide, s.lengths, 3), _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 3)):
+        assert torch.equal(a, b)
