@@ -15,10 +15,6 @@ __device__ __forceinline__ int pages_of(const int length, const int page_log) { 
 // the nearest page there is
 __device__ __forceinline__ int clamped_page(const int page, const int n_pages) { return min(max(page, 0), n_pages - 1); }
 
-// The smaller (larger) of two numbers; NaN where one is NaN (the hardware's minimum drops it).
-__device__ __forceinline__ float min_or_nan(const float a, const float b) { return b < a || b != b ? b : a; }
-__device__ __forceinline__ float max_or_nan(const float a, const float b) { return b > a || b != b ? b : a; }
-
 // One instruction's exchange inside rows of 16 lanes (the lanes are all active); those that receive nothing get `none`.
 constexpr int kDppXor1 = 0xb1, kDppXor2 = 0x4e, kDppHalfMirror = 0x141, kDppRor4 = 0x124, kDppRor8 = 0x128;
 template <int CONTROL, int ROWS = 0xf>

@@ -40,12 +40,82 @@ __device__ __forceinline__ Rows8 rotated(const Rows8& raw, const Angles& a) {
   return {pack8<T>(x), pack8<T>(y)};
 }
 
+// Bounds are kept as pairs of 16-bit whole numbers of the same order (-0 below 0, NaN of either sign beyond the infinities), two to an
+// instruction.  There and back:
+__device__ __forceinline__ uint32_t in_order(const uint32_t x) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  const i16x2 signs = *reinterpret_cast<const i16x2*>(&x) >> 15;
+  return x ^ (*reinterpret_cast<const uint32_t*>(&signs) & 0x7fff7fffu);
+}
+__device__ __forceinline__ uint32_t least(const uint32_t a, const uint32_t b) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  const i16x2 m = __builtin_elementwise_min(*reinterpret_cast<const i16x2*>(&a), *reinterpret_cast<const i16x2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t most(const uint32_t a, const uint32_t b) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  const i16x2 m = __builtin_elementwise_max(*reinterpret_cast<const i16x2*>(&a), *reinterpret_cast<const i16x2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+struct Bounds8 {  // of 8 channels of each half
+  uint32_t lo[8], hi[8];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      lo[j] = 0x7fff7fffu;
+      hi[j] = 0x80008000u;
+    }
+  }
+  __device__ __forceinline__ void widen(const uint32_t (&low)[8], const uint32_t (&high)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      lo[j] = least(lo[j], low[j]);
+      hi[j] = most(hi[j], high[j]);
+    }
+  }
+};
+__device__ __forceinline__ void words(const Rows8& x, uint32_t (&w)[8]) {
+  const uint32_t raw[8] = {x.first.x, x.first.y, x.first.z, x.first.w, x.second.x, x.second.y, x.second.z, x.second.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = in_order(raw[j]);
+}
+// Back, where both bounds become NaN if a key was.
+template <typename T>
+__device__ __forceinline__ void bounds_of(const Bounds8& b, Rows8& lo, Rows8& hi) {
+  uint32_t l[8], h[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    l[j] = in_order(b.lo[j]);
+    h[j] = in_order(b.hi[j]);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t mask = 0x7fffu << (16 * half), most_finite = (uint32_t)T::kExponent << (16 * half);
+      if ((l[j] & mask) > most_finite || (h[j] & mask) > most_finite) {
+        l[j] |= mask;
+        h[j] |= mask;
+      }
+    }
+  }
+  lo = {uint4{l[0], l[1], l[2], l[3]}, uint4{l[4], l[5], l[6], l[7]}};
+  hi = {uint4{h[0], h[1], h[2], h[3]}, uint4{h[4], h[5], h[6], h[7]}};
+}
+// f over the lanes of a wave that have the same piece (lane % PIECES), one instruction or two each
+template <int PIECES, typename F>
+__device__ __forceinline__ uint32_t over_tokens(uint32_t x, F f) {
+  if (PIECES == 4) x = f(x, dpp<kDppRor4>(x));
+  x = f(x, dpp<kDppRor8>(x));
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = f(r[0], r[1]);
+  const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return f(s[0], s[1]);
+}
+
 template <typename T, int D, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) paged_append_kernel(const PagedAppendArgs p) {
   constexpr int kPieces = D / 16;                  // lanes of a token
   constexpr int kInWave = 64 / kPieces;            // tokens of a wave
   constexpr int kTokens = WAVES * kInWave;         // ... and of the work-group, side by side
-  __shared__ float red[WAVES > 1 ? WAVES - 1 : 1][kPieces][32];
+  __shared__ uint32_t red[WAVES > 1 ? WAVES - 1 : 1][kPieces][16];
   const int tid = threadIdx.x, lane = tid & 63, c = tid % kPieces, row = tid / kPieces;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % p.n_kv_heads, group = p.n_q_heads / p.n_kv_heads, page_size = 1 << p.page_log;
@@ -85,18 +155,14 @@ __global__ void __launch_bounds__(64 * WAVES) paged_append_kernel(const PagedApp
       old[0] = load8(bounds, D / 2);
       old[1] = load8(bounds + D, D / 2);
     }
-    float lo[16], hi[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      lo[j] = INFINITY;
-      hi[j] = -INFINITY;
-    }
+    Bounds8 own;
+    own.clear();
     for (int i = row; i < n; i += kTokens) {
       const int64_t tok = t0 + i;
       Rows8 k = load8(p.k + tok * p.k_st + kvh * p.k_sh + 8 * c, D / 2);
       const Rows8 v = load8(p.v + tok * p.v_st + kvh * p.v_sh + 8 * c, D / 2);
-      Angles a;
       if (p.cos != nullptr) {
+        Angles a;
         const float *cos = p.cos + (position + i) * p.cs_sn + 8 * c, *sin = p.sin + (position + i) * p.cs_sn + 8 * c;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -119,69 +185,53 @@ __global__ void __launch_bounds__(64 * WAVES) paged_append_kernel(const PagedApp
       store8(p.keys + at * p.kp_sp + kvh * p.kp_sh + (slot + i) * p.kp_sn + 8 * c, D / 2, k);
       store8(p.values + at * p.vp_sp + kvh * p.vp_sh + (slot + i) * p.vp_sn + 8 * c, D / 2, v);
       if (p.bounds != nullptr) {  // (those of the keys as stored)
-        float x[2][8];
-        unpack8<T>(k.first, x[0]);
-        unpack8<T>(k.second, x[1]);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          lo[j] = min_or_nan(lo[j], x[j >> 3][j & 7]);
-          hi[j] = max_or_nan(hi[j], x[j >> 3][j & 7]);
-        }
+        uint32_t w[8];
+        words(k, w);
+        own.widen(w, w);
       }
     }
     if (p.bounds == nullptr) continue;
+    if (n > 1) {  // over the tokens of a wave
 #pragma unroll
-    for (int d = kPieces; d < 64; d <<= 1) {  // over the tokens of a wave
-      if (n * kPieces > d) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          lo[j] = min_or_nan(lo[j], __shfl_xor(lo[j], d, 64));
-          hi[j] = max_or_nan(hi[j], __shfl_xor(hi[j], d, 64));
-        }
+      for (int j = 0; j < 8; ++j) {
+        own.lo[j] = over_tokens<kPieces>(own.lo[j], least);
+        own.hi[j] = over_tokens<kPieces>(own.hi[j], most);
       }
     }
     if (WAVES > 1 && n > kInWave) {  // over the waves
       if (wave > 0 && lane < kPieces) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          red[wave - 1][c][j] = lo[j];
-          red[wave - 1][c][16 + j] = hi[j];
+        for (int j = 0; j < 8; ++j) {
+          red[wave - 1][c][j] = own.lo[j];
+          red[wave - 1][c][8 + j] = own.hi[j];
         }
       }
       __syncthreads();
-      if (row == 0)
+      if (row == 0) {
 #pragma unroll
-        for (int w = 0; w < WAVES - 1; ++w)
+        for (int w = 0; w < WAVES - 1; ++w) {
+          uint32_t low[8], high[8];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            lo[j] = min_or_nan(lo[j], red[w][c][j]);
-            hi[j] = max_or_nan(hi[j], red[w][c][16 + j]);
+          for (int j = 0; j < 8; ++j) {
+            low[j] = red[w][c][j];
+            high[j] = red[w][c][8 + j];
           }
+          own.widen(low, high);
+        }
+      }
       __syncthreads();
     }
     if (writes) {
       if (slot != 0) {
-        float x[4][8];
-        unpack8<T>(old[0].first, x[0]);
-        unpack8<T>(old[0].second, x[1]);
-        unpack8<T>(old[1].first, x[2]);
-        unpack8<T>(old[1].second, x[3]);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          lo[j] = min_or_nan(lo[j], x[j >> 3][j & 7]);
-          hi[j] = max_or_nan(hi[j], x[2 + (j >> 3)][j & 7]);
-        }
+        uint32_t low[8], high[8];
+        words(old[0], low);
+        words(old[1], high);
+        own.widen(low, high);
       }
-      float y[4][8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        y[0][j] = lo[j];
-        y[1][j] = lo[8 + j];
-        y[2][j] = hi[j];
-        y[3][j] = hi[8 + j];
-      }
-      store8(bounds, D / 2, {pack8<T>(y[0]), pack8<T>(y[1])});
-      store8(bounds + D, D / 2, {pack8<T>(y[2]), pack8<T>(y[3])});
+      Rows8 lo, hi;
+      bounds_of<T>(own, lo, hi);
+      store8(bounds, D / 2, lo);
+      store8(bounds + D, D / 2, hi);
     }
   }
 }
