@@ -142,8 +142,8 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
     v_args, (n_values, _, _) = _rows(v, "v", cache, cache.n_kv_heads)
     tables, batch, most = cache._tables(page_table, lengths)
     starts_ptr = None if starts is None else _indices(starts, "starts", cache, 1, batch + 1)
-    if n_values != n or (starts is None and n != batch) or n * cache.n_kv_heads >= 1 << 24:
-        _refuse(f"{n} keys, {n_values} values and {batch} sequences{' without starts' if starts is None else ''} do not go together (and fewer than 2^24 rows of keys)")
+    if n_values != n or (starts is None and n != batch) or n * cache.n_kv_heads >= 1 << 23:
+        _refuse(f"{n} keys, {n_values} values and {batch} sequences{' without starts' if starts is None else ''} do not go together (and fewer than 2^23 rows of keys)")
     if cos is None:
         if sin is not None or q is not None or out is not None:
             _refuse("cos and sin come together, and queries need them")

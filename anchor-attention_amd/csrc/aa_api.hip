@@ -931,8 +931,8 @@ int aa_paged_append(const aa_paged_cache* cache, const void* q, int64_t q_st, in
   const char* who = "aa_paged_append";
   int rc;
   if ((rc = check_cache(who, cache, batch, n_q_heads, max_pages, page_table, lengths))) return rc;
-  if (n_tokens <= 0 || n_tokens >= 1 << 24 || (int64_t)n_tokens * cache->n_kv_heads >= 1 << 24 || (starts == nullptr && n_tokens != batch)) {
-    set_error("%s: %d tokens of %d sequences are not supported (at least 1, fewer than 2^24 with their KV heads, without starts one of each sequence)",
+  if (n_tokens <= 0 || n_tokens >= 1 << 24 || (int64_t)n_tokens * cache->n_kv_heads >= 1 << 23 || (starts == nullptr && n_tokens != batch)) {
+    set_error("%s: %d tokens of %d sequences are not supported (at least 1, fewer than 2^23 with their KV heads, without starts one of each sequence)",
               who, n_tokens, batch);
     return n_tokens <= 0 ? AA_EBADARG : AA_EUNSUPPORTED;
   }
@@ -954,7 +954,7 @@ int aa_paged_append(const aa_paged_cache* cache, const void* q, int64_t q_st, in
   const PagedAppendArgs a = {(const uint16_t*)q, q_st, q_sh, (uint16_t*)q_out, qo_st, qo_sh, (const uint16_t*)k, k_st, k_sh, (const uint16_t*)v, v_st, v_sh,
                              cos, sin, cs_sn, n_positions, (uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn, (uint16_t*)cache->values,
                              cache->vp_sp, cache->vp_sh, cache->vp_sn, (uint16_t*)cache->bounds, page_table, pt_sb, lengths, starts, batch, n_tokens, n_q_heads,
-                             cache->n_kv_heads, cache->head_dim, cache->n_pages, log2_of(cache->page_size), max_pages, cache->dtype, 0};
+                             cache->n_kv_heads, cache->head_dim, cache->n_pages, log2_of(cache->page_size), max_pages, cache->dtype, 0, 0};
   return check_launch(launch_paged_append(a, (hipStream_t)stream), who);
 }
 

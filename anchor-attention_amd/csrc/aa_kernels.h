@@ -148,7 +148,7 @@ struct PagedAppendArgs {
   const int32_t* lengths; const int32_t* starts;  // starts: optional
   int batch, n_tokens, n_q_heads, n_kv_heads, head_dim, n_pages, page_log, max_pages;  // n_q_heads 0: no queries
   int dtype;
-  int chunk;  // set by the launcher: tokens of a work-group
+  int chunk, key_chunks;  // set by the launcher: tokens of a work-group of keys, and how many of these a KV head has
 };
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t stream);
 

@@ -1,10 +1,11 @@
 // New tokens of a paged key/value cache on gfx950: the rotary embedding of queries and keys, keys and values into their pages, and the bounds
 // of the pages' keys.
 //
-// Bound by reading and writing each element once.  A run is what a page receives: the tokens of one sequence that go to one page.  A work-group
-// has the runs that begin among its few tokens, for one KV head and its group of queries, so that a page's bounds are one work-group's and need
-// no atomics.  A lane takes 8 channels of each half of all rows of a token (D / 16 lanes a token), whose cosines and sines it loads once.
-// A step of one token each is latency: what does not depend on the token's place is requested before that is known.
+// Bound by reading and writing each element once.  A lane takes 8 channels of each half of rows (D / 16 lanes a row).  Two kinds of work-groups
+// share the launch.  One has a few tokens and a KV head: queries of its group and the value, any token apart from the others, with the token's cosines and
+// sines in registers.  The other has the keys that pages receive: a run is the tokens of one sequence that go to one page, and a work-group takes the runs
+// that begin among its few tokens, so that a page's bounds are one work-group's and need no atomics.  (With queries and values in the runs, too, prompts
+// of few KV heads or large pages had too few work-groups: 6001 tokens, 14/2 heads of 64, pages of 64 48 us, of 256 47; 21 and 18 so.)
 #include "aa_kernels.h"
 #include "aa_paged.h"
 
@@ -110,85 +111,123 @@ __device__ __forceinline__ uint32_t over_tokens(uint32_t x, F f) {
   return f(s[0], s[1]);
 }
 
+// Where a token goes: its position, the page of the pool and the row in it; not ok: nowhere.
+struct Place {
+  int64_t position;
+  int at, slot;
+  bool ok;
+};
+// token t of sequence b, whose tokens are those from begin to end; TABLE, a pointer to tables and lengths
+template <typename Words>
+__device__ __forceinline__ Place place_of(const PagedAppendArgs& p, const Words* lengths, const Words* table, const int b, const int begin, const int end, const int t) {
+  Place x = {(int64_t)lengths[b] - end + t, 0, 0, false};
+  if (t < begin || t >= end || x.position < 0 || x.position >> p.page_log >= p.max_pages || (p.cos != nullptr && x.position >= p.n_positions)) return x;
+  x.at = table[b * p.t_sb + (x.position >> p.page_log)];
+  x.slot = (int)x.position & ((1 << p.page_log) - 1);
+  x.ok = (uint32_t)x.at < (uint32_t)p.n_pages;
+  return x;
+}
+// The sequences that end at or before t (wave-uniform), which is the one that t belongs to.
+__device__ __forceinline__ int sequence_of(const PagedAppendArgs& p, const int t) {
+  const int lane = threadIdx.x & 63;
+  int b = 0;
+  for (int i = 0; i < p.batch; i += 64) {
+    const int n = __popcll(__ballot(i + lane < p.batch && p.starts[min(i + lane, p.batch - 1) + 1] <= t));
+    b += n;
+    if (n < 64) break;
+  }
+  return b;
+}
+__device__ __forceinline__ Angles angles_of(const PagedAppendArgs& p, const int64_t position, const int c) {
+  Angles a;
+  const float *cos = p.cos + position * p.cs_sn + 8 * c, *sin = p.sin + position * p.cs_sn + 8 * c;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    a.cos[j] = reinterpret_cast<const float4*>(cos)[j];
+    a.sin[j] = reinterpret_cast<const float4*>(sin)[j];
+  }
+  return a;
+}
+
+// Queries and values of the tokens from `first` on, one of each kPieces lanes.
+template <typename T, int D>
+__device__ __forceinline__ void queries_and_values(const PagedAppendArgs& p, const int first, const int kvh) {
+  constexpr int kPieces = D / 16, kInWave = 64 / kPieces;
+  const int c = threadIdx.x % kPieces, group = p.n_q_heads / p.n_kv_heads;
+  const int t0 = first + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kInWave, t = t0 + (threadIdx.x & 63) / kPieces;
+  if (t0 >= p.n_tokens) return;
+  int b = t, begin = t, end = t + 1;
+  if (p.starts != nullptr) {
+    b = sequence_of(p, t0);  // (and from there on lane by lane)
+    while (b < p.batch && p.starts[b + 1] <= t) ++b;
+    if (b >= p.batch) return;
+    begin = p.starts[b];
+    end = p.starts[b + 1];
+  }
+  if (t >= p.n_tokens) return;
+  const Place x = place_of(p, p.lengths, p.table, b, begin, end, t);
+  if (!x.ok) return;
+  const Rows8 v = load8(p.v + t * p.v_st + kvh * p.v_sh + 8 * c, D / 2);
+  if (group > 0) {
+    const Angles a = angles_of(p, x.position, c);
+    for (int h = 0; h < group; h += 4) {
+      Rows8 q[4];
+      const uint16_t* src = p.q + t * p.q_st + (int64_t)(kvh * group + h) * p.q_sh + 8 * c;
+      uint16_t* dst = p.q_out + t * p.qo_st + (int64_t)(kvh * group + h) * p.qo_sh + 8 * c;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (h + j < group) q[j] = load8(src + j * p.q_sh, D / 2);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (h + j < group) store8(dst + j * p.qo_sh, D / 2, rotated<T>(q[j], a));
+    }
+  }
+  store8(p.values + x.at * p.vp_sp + kvh * p.vp_sh + x.slot * p.vp_sn + 8 * c, D / 2, v);
+}
+
+// Keys of the runs that begin among the `chunk` tokens from `first` on, and their pages' bounds.
 template <typename T, int D, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) paged_append_kernel(const PagedAppendArgs p) {
+__device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const int first, const int kvh, uint32_t (*red)[D / 16][16]) {
   constexpr int kPieces = D / 16;                  // lanes of a token
   constexpr int kInWave = 64 / kPieces;            // tokens of a wave
   constexpr int kTokens = WAVES * kInWave;         // ... and of the work-group, side by side
-  __shared__ uint32_t red[WAVES > 1 ? WAVES - 1 : 1][kPieces][16];
   const int tid = threadIdx.x, lane = tid & 63, c = tid % kPieces, row = tid / kPieces;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kvh = blockIdx.x % p.n_kv_heads, group = p.n_q_heads / p.n_kv_heads, page_size = 1 << p.page_log;
-  const int first = blockIdx.x / p.n_kv_heads * p.chunk;
-  const const_i32 *lengths = (const_i32*)p.lengths, *starts = (const_i32*)p.starts;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), page_size = 1 << p.page_log;
+  const const_i32 *lengths = (const_i32*)p.lengths, *starts = (const_i32*)p.starts, *table = (const_i32*)p.table;
 
   for (int t = first; t < min(first + p.chunk, p.n_tokens);) {
     int b = t, begin = t, end = t + 1;
     if (p.starts != nullptr) {
-      b = 0;
-      for (int i = 0; i < p.batch; i += 64) {  // the sequences that end at or before t
-        const int n = __popcll(__ballot(i + lane < p.batch && p.starts[min(i + lane, p.batch - 1) + 1] <= t));
-        b += n;
-        if (n < 64) break;
-      }
+      b = sequence_of(p, t);
       if (b >= p.batch) return;  // (behind the last sequence)
       begin = starts[b];
       end = starts[b + 1];
     }
-    const int64_t position = (int64_t)lengths[b] - end + t;
-    if (t < begin || t >= end || position < 0 || position >> p.page_log >= p.max_pages) {
-      ++t;
-      continue;
-    }
-    const int at = ((const_i32*)(p.table + b * p.t_sb))[position >> p.page_log], slot = (int)position & (page_size - 1);
-    int n = min(min(end, p.n_tokens) - t, page_size - slot);
+    const Place x = place_of(p, lengths, table, b, begin, end, t);
+    // the rest of the run; of tokens before the first position as many as there are
+    int n = 1;
+    if (t >= begin && t < end) n = x.position < 0 ? (int)min(-x.position, (int64_t)(end - t)) : min(min(end, p.n_tokens) - t, page_size - ((int)x.position & (page_size - 1)));
     const int t0 = t;
     t += n;
-    if (t0 != begin && slot != 0) continue;  // (the rest of a run that began among the tokens before)
-    if (p.cos != nullptr) n = (int)min((int64_t)n, p.n_positions - position);
-    if ((uint32_t)at >= (uint32_t)p.n_pages || n <= 0) continue;
+    if (!x.ok || (t0 != begin && x.slot != 0)) continue;  // (nowhere; the rest of a run that began among the tokens before)
+    if (p.cos != nullptr) n = (int)min((int64_t)n, p.n_positions - x.position);
 
-    uint16_t* bounds = p.bounds + ((int64_t)at * p.n_kv_heads + kvh) * 2 * D + 8 * c;
+    uint16_t* bounds = p.bounds + ((int64_t)x.at * p.n_kv_heads + kvh) * 2 * D + 8 * c;
     Rows8 old[2];
     const bool writes = p.bounds != nullptr && row == 0;  // the bounds, at the end
-    if (writes && slot != 0) {
+    if (writes && x.slot != 0) {
       old[0] = load8(bounds, D / 2);
       old[1] = load8(bounds + D, D / 2);
     }
     Bounds8 own;
     own.clear();
     for (int i = row; i < n; i += kTokens) {
-      const int64_t tok = t0 + i;
-      Rows8 k = load8(p.k + tok * p.k_st + kvh * p.k_sh + 8 * c, D / 2);
-      const Rows8 v = load8(p.v + tok * p.v_st + kvh * p.v_sh + 8 * c, D / 2);
-      if (p.cos != nullptr) {
-        Angles a;
-        const float *cos = p.cos + (position + i) * p.cs_sn + 8 * c, *sin = p.sin + (position + i) * p.cs_sn + 8 * c;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          a.cos[j] = reinterpret_cast<const float4*>(cos)[j];
-          a.sin[j] = reinterpret_cast<const float4*>(sin)[j];
-        }
-        for (int h = 0; h < group; h += 4) {
-          Rows8 q[4];
-          const uint16_t* src = p.q + tok * p.q_st + (int64_t)(kvh * group + h) * p.q_sh + 8 * c;
-          uint16_t* dst = p.q_out + tok * p.qo_st + (int64_t)(kvh * group + h) * p.qo_sh + 8 * c;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (h + j < group) q[j] = load8(src + j * p.q_sh, D / 2);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (h + j < group) store8(dst + j * p.qo_sh, D / 2, rotated<T>(q[j], a));
-        }
-        k = rotated<T>(k, a);
-      }
-      store8(p.keys + at * p.kp_sp + kvh * p.kp_sh + (slot + i) * p.kp_sn + 8 * c, D / 2, k);
-      store8(p.values + at * p.vp_sp + kvh * p.vp_sh + (slot + i) * p.vp_sn + 8 * c, D / 2, v);
-      if (p.bounds != nullptr) {  // (those of the keys as stored)
-        uint32_t w[8];
-        words(k, w);
-        own.widen(w, w);
-      }
+      Rows8 k = load8(p.k + (int64_t)(t0 + i) * p.k_st + kvh * p.k_sh + 8 * c, D / 2);
+      if (p.cos != nullptr) k = rotated<T>(k, angles_of(p, x.position + i, c));
+      store8(p.keys + x.at * p.kp_sp + kvh * p.kp_sh + (x.slot + i) * p.kp_sn + 8 * c, D / 2, k);
+      uint32_t w[8];  // (of the keys as stored)
+      words(k, w);
+      own.widen(w, w);
     }
     if (p.bounds == nullptr) continue;
     if (n > 1) {  // over the tokens of a wave
@@ -222,7 +261,7 @@ __global__ void __launch_bounds__(64 * WAVES) paged_append_kernel(const PagedApp
       __syncthreads();
     }
     if (writes) {
-      if (slot != 0) {
+      if (x.slot != 0) {
         uint32_t low[8], high[8];
         words(old[0], low);
         words(old[1], high);
@@ -236,15 +275,25 @@ __global__ void __launch_bounds__(64 * WAVES) paged_append_kernel(const PagedApp
   }
 }
 
+template <typename T, int D, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) paged_append_kernel(const PagedAppendArgs p) {
+  __shared__ uint32_t red[WAVES > 1 ? WAVES - 1 : 1][D / 16][16];
+  const int kvh = blockIdx.x % p.n_kv_heads, at = blockIdx.x / p.n_kv_heads;
+  if (at < p.key_chunks) keys_and_bounds<T, D, WAVES>(p, at * p.chunk, kvh, red);
+  else queries_and_values<T, D>(p, (at - p.key_chunks) * (WAVES * 1024 / D), kvh);
+}
+
 template <typename T, int D>
 static void launch_paged_append_for(PagedAppendArgs a, hipStream_t stream) {
-  // Tokens of a work-group: few, so that short runs do not queue up in one, but no fewer than make some thousand work-groups
+  // Tokens of a work-group of keys: few, so that short runs do not queue up in one, but no fewer than make some thousand work-groups
   const int64_t most = (int64_t)a.n_tokens * a.n_kv_heads / 4096, page_size = 1 << a.page_log;
   a.chunk = a.starts == nullptr || most < 1 ? 1 : (int)(most < page_size ? most : page_size);
-  const dim3 grid((uint32_t)((a.n_tokens + a.chunk - 1) / a.chunk) * (uint32_t)a.n_kv_heads);
-  const int waves = a.starts == nullptr ? 1 : (int)(page_size * (D / 16) / 64);
-  if (waves <= 1) hipLaunchKernelGGL((paged_append_kernel<T, D, 1>), grid, dim3(64), 0, stream, a);
-  else if (waves == 2) hipLaunchKernelGGL((paged_append_kernel<T, D, 2>), grid, dim3(128), 0, stream, a);
+  a.key_chunks = (a.n_tokens + a.chunk - 1) / a.chunk;
+  // waves of a work-group: as many as the tokens of a page fill
+  const int waves = a.starts == nullptr ? 1 : (int)(page_size * (D / 16) / 64), w = waves <= 1 ? 1 : waves == 2 ? 2 : 4;
+  const dim3 grid((uint32_t)(a.key_chunks + (a.n_tokens + w * 1024 / D - 1) / (w * 1024 / D)) * (uint32_t)a.n_kv_heads);
+  if (w == 1) hipLaunchKernelGGL((paged_append_kernel<T, D, 1>), grid, dim3(64), 0, stream, a);
+  else if (w == 2) hipLaunchKernelGGL((paged_append_kernel<T, D, 2>), grid, dim3(128), 0, stream, a);
   else hipLaunchKernelGGL((paged_append_kernel<T, D, 4>), grid, dim3(256), 0, stream, a);
 }
 

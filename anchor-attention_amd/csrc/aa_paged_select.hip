@@ -17,6 +17,10 @@ namespace aa {
 constexpr int kAbreast = 4, kAbreastFused = 1;
 constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
 constexpr int kFused = 1024;       // a table of at most that many pages is scored and chosen from by one launch
+// ... if its bounds have so few (channel, head) products that one work-group forms them sooner than a launch of its own starts: 32/8 heads of 128, one
+// sequence, 64 pages 17.6 us a step by one launch and 19.8 by two, 128 pages 19.7 and 19.6, 256 24.2 and 19.7; 14/2 heads of 64 128 pages 16.6 and 19.0,
+// 192 17.9 and 19.1, 256 20.7 and 19.0.
+constexpr int kFusedProducts = 72 * 1024;
 constexpr int kInLds = 8192;       // the scores of at most that many pages are kept in LDS
 constexpr int kMostPages = 1 << 16;
 constexpr int kListed = 1024;      // the chosen pages up to that many pass through LDS
@@ -317,7 +321,7 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
 template <typename T, int D>
 static void launch_paged_select_for(const PagedSelectArgs& a, hipStream_t stream) {
   const dim3 units(a.n_kv_heads, a.batch);
-  if (a.max_pages <= kFused) {
+  if (a.max_pages <= kFused && (int64_t)a.max_pages * (a.n_q_heads / a.n_kv_heads) * D <= kFusedProducts) {
     hipLaunchKernelGGL((paged_choose_kernel<T, D, 0>), units, dim3(kChooseThreads), 0, stream, a);
     return;
   }
