@@ -60,7 +60,7 @@ class PagedCache:
     """Keys and values in pages: ``keys``, ``values`` ``[n_pages, n_kv_heads, page_size, head_dim]`` (bf16 or fp16 on one GPU, rows contiguous on
     16-byte boundaries, the other strides free) and, for sparse steps, ``bounds`` ``[n_pages, n_kv_heads, 2, head_dim]`` (contiguous): the
     smallest and the largest value of each channel over a page's keys, which :func:`append_to_pages` keeps.  The contents of pages that no table names
-    do not matter.  The tensors stay the cache's own for as long as it is used: their contents may change, their memory may not."""
+    do not matter.  The tensors stay the cache's own for as long as it is used: their contents may change, their memory may not, and a cache gets no others."""
 
     __slots__ = ("keys", "values", "bounds", "dtype", "device", "index", "n_pages", "n_kv_heads", "page_size", "head_dim", "_struct", "_address")
 
@@ -80,12 +80,18 @@ class PagedCache:
                 _refuse("the rows of keys and values must be contiguous, begin on 16-byte boundaries and lie at most 16384 elements apart, and no two share memory")
         if bounds is not None and (bounds.shape != (n_pages, kv_heads, 2, d) or not bounds.is_contiguous() or bounds.data_ptr() & 15):
             _refuse(f"bounds must be a contiguous tensor {(n_pages, kv_heads, 2, d)}, not {tuple(bounds.shape)}")
-        self.keys, self.values, self.bounds, self.dtype, self.device, self.index = keys, values, bounds, keys.dtype, keys.device, keys.get_device()
-        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n_pages, kv_heads, page_size, d
         # (what the C interface is told of the cache, once: 13 arguments fewer in each call)
-        self._struct = _hip.PagedCacheStruct(*_hip.t3(keys), *_hip.t3(values), None if bounds is None else bounds.data_ptr(), n_pages, kv_heads, page_size, d,
-                                             _hip.dtype_code(keys))
-        self._address = ctypes.addressof(self._struct)
+        struct = _hip.PagedCacheStruct(*_hip.t3(keys), *_hip.t3(values), None if bounds is None else bounds.data_ptr(), n_pages, kv_heads, page_size, d,
+                                       _hip.dtype_code(keys))
+        for name, value in zip(self.__slots__, (keys, values, bounds, keys.dtype, keys.device, keys.get_device(), n_pages, kv_heads, page_size, d, struct,
+                                                ctypes.addressof(struct))):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"a PagedCache does not change: {name}")
+
+    def __reduce__(self):
+        return PagedCache, (self.keys, self.values, self.bounds)
 
     @classmethod
     def empty(cls, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, dtype=torch.bfloat16, device="cuda", bounds: bool = True):
@@ -127,7 +133,8 @@ def _plain(cache, *tensors):
 def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tensor],
                     sin: Optional[torch.Tensor], page_table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
-    """Appends new tokens to the cache and returns their rotated queries (in ``out``, which may be ``q``, if it is given).
+    """Appends new tokens to the cache and returns their rotated queries (in ``out``, if it is given; that may be ``q`` and otherwise shares no memory with
+    the inputs).
 
     ``q`` ``[tokens, query heads, D]``, ``k``, ``v`` ``[tokens, KV heads, D]``: the tokens of all sequences one after the other; sequence ``b`` has
     tokens ``starts[b]`` to ``starts[b + 1]`` (``[batch + 1]``; None: one token each).  ``lengths`` ``[batch]`` counts a sequence's keys
@@ -166,7 +173,7 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
             heads = shape[1]
             if shape[0] != n:
                 _refuse(f"q has {shape[0]} tokens, k {n}")
-            q_args = (*q_rows, *_out_rows(q, out, shape, cache)) if out is not None else (*q_rows, *_new_rows(out := torch.empty_like(q)))
+            q_args = (*q_rows, *_out_rows(out, shape, cache)) if out is not None else (*q_rows, *_new_rows(out := torch.empty_like(q)))
     if n and batch:
         cache._launch(_hip.lib().aa_paged_append, *q_args, *k_args, *v_args, *angles, *tables, starts_ptr, batch, n, heads, most)
     return out
@@ -177,10 +184,10 @@ def _new_rows(t):
     return t.data_ptr(), st, sh
 
 
-def _out_rows(q, out, shape, cache):
+def _out_rows(out, shape, cache):
     rows, out_shape = _rows(out, "out", cache, shape[1])
-    if out_shape != shape:
-        _refuse("out must have the shape of q")
+    if out_shape != shape or (not rows[1] and shape[0] > 1) or (not rows[2] and shape[1] > 1):
+        _refuse("out must have the shape of q, and no two of its rows the same memory")
     return rows
 
 
@@ -194,7 +201,7 @@ def _decode_args(cache, q, page_table, lengths, sm_scale, out):
     if not 1e-30 < scale < 1e30:
         _refuse(f"sm_scale must be positive and finite, not {sm_scale}")
     if out is not None:
-        out_rows = _out_rows(q, out, shape, cache)
+        out_rows = _out_rows(out, shape, cache)
     else:
         out_rows = _new_rows(out := torch.empty_like(q))
     return out, (*q_rows, *out_rows, *tables), (batch, shape[1]), most, scale
@@ -203,7 +210,7 @@ def _decode_args(cache, q, page_table, lengths, sm_scale, out):
 def paged_decode_attention(cache: PagedCache, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, sm_scale: Optional[float] = None,
                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one new token per sequence, ``q`` ``[batch, query heads, D]``, over the first ``lengths[b]`` keys of each: ``softmax(q K^T
-    sm_scale) V``, zeros for a sequence of none.  ``sm_scale`` defaults to ``D ** -0.5``."""
+    sm_scale) V``, zeros for a sequence of none.  ``sm_scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``."""
     out, tensors, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
     if sizes[0]:
         lib = _hip.lib()

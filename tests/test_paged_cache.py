@@ -8,7 +8,9 @@ Attention: a score is a float32 sum of D exact products, off by at most D * 2^-2
 (arguments up to 2^8, 2^-24 of them, and an ulp of exp2 or two) a probability is off by 2 * D * 2^-24 * sum |q_d k_d| * scale + 2^-14 of it.  It is kept as two 16-bit numbers,
 off by u^2 (fp16: its grid of 2^-39 too, covered by 2^-14); sums over n keys in float32 add n * 2^-24.  All of that is relative to sum p |v| / sum p; the
 result is rounded once, u of it.  The chosen pages have to be the same."""
+import copy
 import ctypes
+import pickle
 import types
 
 import pytest
@@ -204,8 +206,9 @@ def test_append_without_rotation_and_in_place():
         for h in range(2):
             assert torch.equal(s.rows(s.cache.keys, b, h)[-9:], k[9 * b:9 * b + 9, h].double())
             assert torch.equal(s.rows(s.cache.values, b, h)[-9:], v[9 * b:9 * b + 9, h].double())
-    cos, sin = _tables(64, 64)
+    cos, sin = torch.cat(_tables(64, 64), 1).split(32, 1)  # (parts of one table)
     want = ops.append_to_pages(s.cache, q, k, v, cos, sin, s.table, lengths, starts)
+    assert torch.equal(want, ops.append_to_pages(s.cache, q, k, v, cos.contiguous(), sin.contiguous(), s.table, lengths, starts))
     keys = s.cache.keys.clone()
     assert ops.append_to_pages(s.cache, q, k, v, cos, sin, s.table, lengths, starts, out=q) is q
     assert torch.equal(q, want) and torch.equal(keys.nan_to_num(9.0), s.cache.keys.nan_to_num(9.0))
@@ -239,12 +242,10 @@ def test_bounds_of_infinite_and_nan_keys():
     ops = _ops()
     s = _Setup([0], 1, 64, 16, F16, 6, room=32)
     k = torch.randn(20, 1, 64, generator=s.g, device="cuda").to(F16)
-    k[3, 0, 5], k[4, 0, 6], k[5, 0, 7], k[17, 0, 8], k[18, 0, 9] = float("nan"), float("inf"), float("-inf"), float("nan"), 65504.0
-    starts = torch.tensor([0, 17], dtype=torch.int32, device="cuda")
+    k[3, 0, 5], k[4, 0, 6], k[5, 0, 7], k[17, 0, 8], k[18, 0, 9], k[19, 0, 10], k[6, 0, 11] = float("nan"), float("inf"), float("-inf"), float("nan"), 65504.0, -float("nan"), -0.0
     for lo, hi, length in ((0, 17, 17), (17, 20, 20)):
         ops.append_to_pages(s.cache, None, k[lo:hi], k[lo:hi], None, None, s.table, torch.tensor([length], dtype=torch.int32, device="cuda"),
                             torch.tensor([0, hi - lo], dtype=torch.int32, device="cuda"))
-    del starts
     for i, rows in enumerate((k[:16, 0], k[16:, 0])):
         got = s.cache.bounds[int(s.table[0, i]), 0]
         want = torch.stack((rows.amin(0), rows.amax(0)))  # (the framework's minimum of NaN is NaN)
@@ -274,6 +275,7 @@ def test_decode(lengths, hq, hkv, d, page, layout, dtype):
     _close(out, q, s, d ** -0.5)
     again = _ops().paged_decode_attention(s.cache, q.transpose(0, 1).contiguous().transpose(0, 1), s.table, s.lengths, sm_scale=d ** -0.5)
     assert torch.equal(out, again)  # the same bits
+    assert _ops().paged_decode_attention(s.cache, q, s.table, s.lengths, out=q) is q and torch.equal(q, again)
 
 
 @pytest.mark.gpu
@@ -587,6 +589,13 @@ def test_what_the_entry_points_refuse():
             fn(**{**base, "q": z(2, 4, 64).requires_grad_()})
     with pytest.raises(_hip.AnchorAttnHipError, match="with bounds"):
         ops.paged_sparse_decode_attention(ops.PagedCache(cache.keys, cache.values), q, table, lengths, 2)
+    with pytest.raises(_hip.AnchorAttnHipError, match="same memory"):
+        ops.paged_decode_attention(cache, q, table, lengths, out=z(1, 4, 64).expand(2, 4, 64))
+    with pytest.raises(AttributeError, match="does not change"):
+        cache.keys = cache.values
+    for other in (copy.copy(cache), copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+        assert type(other) is ops.PagedCache and torch.equal(ops.paged_decode_attention(other, q, table, lengths), ops.paged_decode_attention(cache, q, table, lengths))
+    assert copy.deepcopy(cache).keys.data_ptr() != cache.keys.data_ptr()
     with pytest.raises(_hip.AnchorAttnHipError, match="traced"):
         torch.func.vmap(lambda x: ops.paged_decode_attention(cache, x, table, lengths))(q[None])
     # nothing to do is no error
