@@ -127,16 +127,18 @@ __device__ __forceinline__ Place place_of(const PagedAppendArgs& p, const Words*
   x.ok = (uint32_t)x.at < (uint32_t)p.n_pages;
   return x;
 }
-// The sequences that end at or before t (wave-uniform), which is the one that t belongs to.
+// The sequences that end at or before t (wave-uniform), which is the one that t belongs to: every lane asks for the end of a 64th of those left, so that
+// a load does for 64 sequences, two for 4096 and three for all.
 __device__ __forceinline__ int sequence_of(const PagedAppendArgs& p, const int t) {
   const int lane = threadIdx.x & 63;
-  int b = 0;
-  for (int i = 0; i < p.batch; i += 64) {
-    const int n = __popcll(__ballot(i + lane < p.batch && p.starts[min(i + lane, p.batch - 1) + 1] <= t));
-    b += n;
-    if (n < 64) break;
+  int from = 0, left = p.batch;  // (those before `from` end at or before t, those from from + left on do not)
+  for (;;) {
+    const int step = (left + 63) >> 6, at = from + (lane + 1) * step - 1;
+    const int n = __popcll(__ballot(at < from + left && p.starts[min(at, p.batch - 1) + 1] <= t));
+    from += n * step;
+    left = min(left - n * step, step - 1);
+    if (left <= 0) return from;
   }
-  return b;
 }
 __device__ __forceinline__ Angles angles_of(const PagedAppendArgs& p, const int64_t position, const int c) {
   Angles a;
@@ -158,9 +160,18 @@ __device__ __forceinline__ void queries_and_values(const PagedAppendArgs& p, con
   if (t0 >= p.n_tokens) return;
   int b = t, begin = t, end = t + 1;
   if (p.starts != nullptr) {
-    b = sequence_of(p, t0);  // (and from there on lane by lane)
-    while (b < p.batch && p.starts[b + 1] <= t) ++b;
+    b = sequence_of(p, t0);
     if (b >= p.batch) return;
+    if (((const_i32*)p.starts)[b + 1] < t0 + kInWave) {  // several sequences' tokens: the next 64 are looked through for each
+      const int lane = threadIdx.x & 63, b0 = b, ends = p.starts[min(b0 + lane, p.batch - 1) + 1];
+#pragma nounroll
+      for (int j = 0; j < kInWave; ++j) {
+        int n = __popcll(__ballot(b0 + lane < p.batch && ends <= t0 + j));
+        if (n == 64) n = sequence_of(p, t0 + j) - b0;
+        b = lane / kPieces == j ? b0 + n : b;
+      }
+      if (b >= p.batch) return;
+    }
     begin = p.starts[b];
     end = p.starts[b + 1];
   }

@@ -182,6 +182,9 @@ def _append_and_check(before, new, hq, hkv, d, page, dtype, layout, steps=False,
     ([0, 1, 255, 256], [257, 600, 1, 255], 8, 8, 128, 256, "part", 0),
     ([0] * 70, [3] * 69 + [40], 4, 1, 64, 32, "heads", 70),
     ([7, 128], [0, 0], 4, 2, 128, 128, "heads", 3),
+    ([7] * 4, [9, 0, 1, 70], 4, 2, 128, 32, "heads", 3),
+    ([2, 5] + [0] * 200 + [9, 1], [1, 2] + [0] * 200 + [30, 1], 4, 1, 128, 16, "heads", 40),
+    ([3] * 300 + [0] * 4400, [i % 3 for i in range(300)] + [0] * 4000 + [1, 0, 0, 2] * 100, 2, 1, 64, 16, "heads", 11),
     ([300] * 3, [517, 1, 90], 71, 1, 64, 128, "part", 1),
 ])
 def test_append(before, new, hq, hkv, d, page, layout, padding, dtype):
