@@ -128,10 +128,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     total += __builtin_amdgcn_readlane(sum0, 63);
   }
   total *= units;
-  // x becomes the beginning of its unit if that is near or the unit is short and `whole`
+  // x becomes the beginning of its unit if that is near, or if units are not cut and `whole`
   auto settle = [&](PagedPlace<Place>& f, Place& x, const bool whole) __attribute__((always_inline)) {
     f.tile = (int)(x - f.start) - kOver;
-    if (f.tile <= 0 || (whole && f.n_tiles <= kWhole)) {
+    if (f.tile <= 0 || (whole && p.headers == nullptr)) {
       f.tile = 0;
       x = f.start;
     }
