@@ -6,6 +6,9 @@
 // sines in registers.  The other has the keys that pages receive: a run is the tokens of one sequence that go to one page, and a work-group takes the runs
 // that begin among its few tokens, so that a page's bounds are one work-group's and need no atomics.  (With queries and values in the runs, too, prompts
 // of few KV heads or large pages had too few work-groups: 6001 tokens, 14/2 heads of 64, pages of 64 48 us, of 256 47; 21 and 18 so.)
+//
+// Measured: a token of each of 96 sequences, 28/4 heads of 128, bf16 4.5 us, the launch and a chain of three loads; a prompt of 6001, 32/8 of 64, fp16 16.0 us, 4.8
+// TB/s; six prompts of 700 to 21000 tokens, 32/8 of 128, bf16 205 us, 5.1 TB/s, where a copy reaches 5.2.
 #include "aa_kernels.h"
 #include "aa_paged.h"
 
@@ -286,23 +289,30 @@ __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const 
   }
 }
 
+// Work-groups of the same tokens are one XCD's, one after the other, so that its L2 reads their cosines and sines once (a prompt of
+// 6001 tokens, 32/8 heads of 128 32.3 -> 29.7 us).  Turns are dealt out by a hash, since runs may begin every so many work-groups: 64 tokens of a sequence each and a
+// prompt of 2000 took 20.3 us in plain order, 15.8 so, 18.3 with the KV heads' work-groups spread over the XCDs.
+constexpr uint32_t kXcds = 8;
 template <typename T, int D, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) paged_append_kernel(const PagedAppendArgs p) {
   __shared__ uint32_t red[WAVES > 1 ? WAVES - 1 : 1][D / 16][16];
-  const int kvh = blockIdx.x % p.n_kv_heads, at = blockIdx.x / p.n_kv_heads;
+  const uint32_t xcd = blockIdx.x % kXcds, of_xcd = blockIdx.x / kXcds, turn = of_xcd / p.n_kv_heads;
+  const int kvh = of_xcd - turn * p.n_kv_heads, at = turn * kXcds + (xcd + (turn * 0x9e3779b1u >> 29)) % kXcds;
   if (at < p.key_chunks) keys_and_bounds<T, D, WAVES>(p, at * p.chunk, kvh, red);
   else queries_and_values<T, D>(p, (at - p.key_chunks) * (WAVES * 1024 / D), kvh);
 }
 
 template <typename T, int D>
 static void launch_paged_append_for(PagedAppendArgs a, hipStream_t stream) {
-  // Tokens of a work-group of keys: few, so that short runs do not queue up in one, but no fewer than make some thousand work-groups
+  // Tokens of a work-group of keys: few, so that short runs do not queue up in one, but no fewer than make some thousand work-groups (prompts of 700 to 21000 tokens,
+  // 32/8 heads of 128: 205 us, with 1 everywhere some 600; 200 sequences of a token, padded to 256: 14, with a page everywhere 109; 64 of a token and a prompt of 2000: 18, 122)
   const int64_t most = (int64_t)a.n_tokens * a.n_kv_heads / 4096, page_size = 1 << a.page_log;
   a.chunk = a.starts == nullptr || most < 1 ? 1 : (int)(most < page_size ? most : page_size);
   a.key_chunks = (a.n_tokens + a.chunk - 1) / a.chunk;
   // waves of a work-group: as many as the tokens of a page fill
   const int waves = a.starts == nullptr ? 1 : (int)(page_size * (D / 16) / 64), w = waves <= 1 ? 1 : waves == 2 ? 2 : 4;
-  const dim3 grid((uint32_t)(a.key_chunks + (a.n_tokens + w * 1024 / D - 1) / (w * 1024 / D)) * (uint32_t)a.n_kv_heads);
+  const uint32_t chunks = a.key_chunks + (a.n_tokens + w * 1024 / D - 1) / (w * 1024 / D);
+  const dim3 grid((chunks + kXcds - 1) / kXcds * kXcds * a.n_kv_heads);
   if (w == 1) hipLaunchKernelGGL((paged_append_kernel<T, D, 1>), grid, dim3(64), 0, stream, a);
   else if (w == 2) hipLaunchKernelGGL((paged_append_kernel<T, D, 2>), grid, dim3(128), 0, stream, a);
   else hipLaunchKernelGGL((paged_append_kernel<T, D, 4>), grid, dim3(256), 0, stream, a);

@@ -2,16 +2,24 @@
 //
 // Bound by reading keys and values once.  A unit is a (sequence, KV head) with up to 16 heads of its group as the columns of 16 x 16 x 32 MFMAs; its
 // keys come in tiles of 32.  Lengths are known on the device only and may differ a lot, so the tiles of all units, one after the other, are cut into equal
-// shares, one for each of a fixed number of work-groups: every work-group sums the lengths and finds its share by itself.  A share that begins or ends
-// inside a unit leaves the state of its part (maximum, sum, accumulator) in the workspace, at most two of them, and paged_combine_kernel joins
-// the parts in order, so that results do not depend on timing.  Units of few tiles are never cut.
+// shares, one for each of a fixed number of work-groups, and each share into equal parts of its four waves: every wave sums the lengths and finds its part
+// by itself.  A wave walks its part alone, from unit to unit, and nothing passes through LDS until the end, where the states (maximum, sum, accumulator) of units
+// that several waves have are joined.  A share that begins or ends inside a unit leaves that unit's state in the workspace, two states at most, and
+// paged_combine_kernel joins them in order, so that results do not depend on timing.  Where the table has room for few tiles only, no unit is cut between
+// work-groups, and there is no second launch.
 //
-// The four waves of a work-group take a unit's tiles in turn and nothing passes through LDS until they are merged:
+// Inside a wave:
 //   S^T = K Q^T: a lane holds 8 channels of one key, the MFMA's own layout, straight from memory;
 //   O^T = V^T P^T: the order of keys inside a product is free, so P^T is S^T's registers as they lie (lane 16 g + c has keys 4 g + r and
 //   16 + 4 g + r of column c), and V^T wants 8 keys of one channel in a lane: a lane loads D / 16 channels of its 8 keys, whole rows
 //   by 16 lanes, and v_perm turns the block, one instruction per two elements.
-// P enters as two 16-bit numbers, its rounding and the rest, as in the other decode kernel.  The next tile's loads are in flight during a tile.
+// P enters as two 16-bit numbers, its rounding and the rest, as in the other decode kernel: the MFMAs are idle most of the time, and one rounding of P
+// costs as much as that of the output.  There is one set of registers for a tile; its keys are requested anew as soon as the scores have read them, its values after
+// the last product, so that loads are always in flight.
+//
+// Measured (bf16 unless said): 32 sequences of 500 to 16000 keys, 32/8 heads of 128 111 us, of which 4.8 the join: 5.7 TB/s while it reads, where a copy of that
+// size reaches 5.2 to 5.4; 2 of 131071, 28/4 heads of 128, fp16 101 us, 5.6 TB/s; one of 33001, 32/8 of 128 32.4 us, of which about 4 pass before the first
+// tile has come (lengths, table, rows, one after the other), 1.7 at the end and 4 in the join; one of 300, 14/2 of 64 8 us, nothing but such chains.
 #include "aa_kernels.h"
 #include "aa_nonfinite.h"
 #include "aa_paged.h"
@@ -23,12 +31,21 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kCols = 16;       // columns of a unit: heads of the group
 constexpr int kTile = 32;       // keys of a tile
-constexpr int kOver = 3;        // what a unit costs beside its tiles, in tiles
-constexpr int kWhole = 20;      // a unit of at most that many tiles is not cut between work-groups
-constexpr int kShares = 256;    // work-groups
+// What a unit costs beside its tiles, in tiles.  (128 sequences of 20 to 1200 keys, 32/8 heads of 64: 0 30.1 us, 3 24.6, 6 24.9; 32 of 500 to 16000, 32/8 of 128:
+// 114, 110.8, 112.2.)
+constexpr int kOver = 3;
+// Where the table has room for that many tiles of a sequence at most, units are not cut between work-groups and nothing is joined: one of 300 keys, 14/2 heads of
+// 64, 10.3 us; with a limit of 8, cut and joined, 14.9.
+constexpr int kWhole = 20;
+// Work-groups, one to a CU.  (512: one sequence of 33001 keys 33.9 us instead of 32.3, 32 of 500 to 16000 113 instead of 110, 128 of 20 to 1200 45 instead of 25.)
+constexpr int kShares = 256;
 constexpr int kSharesLog = 8;
-constexpr int kPerLane = 4;     // sequences that a lane counts
-constexpr int kLeast = 8;       // tiles of a share
+// Sequences that a lane counts, so that 256 are one scan.  (1: 256 of 1 to 800 keys, 14/2 heads of 64, 17.4 us instead of 16.5; 1000 of 1 to 200, 32/8 of 64, 45.7
+// instead of 40.4; up to 128 the same.)
+constexpr int kPerLane = 4;
+// Tiles of a share at least: fewer work-groups leave fewer parts to join, and each has longer to go.  (64 pages of 64 of one sequence, 32/8 heads of 128, chosen and
+// read: 4 24.4 us, 8 24.4, 16 26.7.)
+constexpr int kLeast = 8;
 
 template <typename T> __device__ __forceinline__ floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c);
 template <> __device__ __forceinline__ floatx4 mfma16<Bf16>(u32x4 a, u32x4 b, floatx4 c) {
@@ -512,7 +529,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
 }
 
 // Joins the parts of a column whose unit begins in share blockIdx.x and ends in another: the weights first, then groups of D / 4 lanes add up
-// every so many parts.
+// every so many parts.  Few bytes; the launch and three loads one after the other take 3.2 to 5 us, which a step pays whether or not a unit was cut, since the
+// host does not know the lengths.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArgs p) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;

@@ -271,7 +271,8 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
  * lengths[b] - (starts[b + 1] - starts[b]) + t - starts[b] of the sequence, which is its position: k and (if not NULL) q are rotated by row
  * `position` of cos and sin (float32 [n_positions, head_dim / 2], cs_sn elements from row to row; first half' = first * cos - second * sin, second' = second *
  * cos + first * sin, in float32 with one rounding), k and v stored in the sequence's pages, q to q_out, which may be q.  cos and sin NULL: k is stored as it is, and
- * q must be NULL and n_q_heads 0.  A page's bounds are set by its first key and widened by the others.  A token that has no place - behind the last
+ * q must be NULL and n_q_heads 0.  A page's bounds are set by its first key and widened by the others; those of
+ * keys that were taken back (a smaller length) stay until the page's first key is stored again.  A token that has no place - behind the last
  * sequence, at a position below 0, in no row of cos and sin, behind the table or in no page of the pool - is left out: nothing is written for it.
  * q, k, v, q_out: [n_tokens, heads, head_dim] with strides of token and head (_st, _sh).  Two tokens for one place, or of two sequences for one page, give one or a
  * mixture of both.

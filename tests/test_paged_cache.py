@@ -665,3 +665,34 @@ def test_tables_so_wide_that_places_need_64_bits(d):
     assert torch.equal(_ops().paged_decode_attention(s.cache, q, wide, s.lengths), _ops().paged_decode_attention(s.cache, q, s.table, s.lengths))
     for a, b in zip(_ops().paged_sparse_decode_attention(s.cache, q, wide, s.lengths, 3), _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 3)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_the_longest_sequences():
+    """A million keys in pages of 16: some pages chosen, nearly all, all; and of equal scores the first."""
+    ops = _ops()
+    s = _Setup([1 << 20, (1 << 20) - 39], 1, 64, 16, F16, 12)
+    q = s.queries(3, 1.0)
+    _close(ops.paged_decode_attention(s.cache, q, s.table, s.lengths), q, s, 64 ** -0.5)
+    for n_pages in (100, 40000, 65535, 65536):
+        out, pages = ops.paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, n_pages, 1, 2)
+        assert torch.equal(pages, _chosen(q, s, n_pages, 1, 2))
+        _close(out, q, s, 64 ** -0.5, pages)
+    s.cache.bounds.fill_(1.0)
+    pages = ops.paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 50000, 1, 2)[1].cpu()
+    for b, there in enumerate((65536, 65534)):
+        assert pages[b, 0].tolist() == list(range(49998)) + [there - 2, there - 1]
+
+
+@pytest.mark.gpu
+def test_pages_that_sequences_share():
+    """One prefix in several rows of the table, and a page twice in one row."""
+    ops = _ops()
+    s = _Setup([300, 290, 100], 2, 128, 16, BF16, 13)
+    s.table[1, :12] = s.table[0, :12]
+    s.table[2, 3] = s.table[2, 1]
+    q = s.queries(8)
+    _close(ops.paged_decode_attention(s.cache, q, s.table, s.lengths), q, s, 128 ** -0.5)
+    out, pages = ops.paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 6, 1, 1)
+    assert torch.equal(pages, _chosen(q, s, 6, 1, 1))
+    _close(out, q, s, 128 ** -0.5, pages)
