@@ -37,7 +37,7 @@ constexpr int kOver = 3;
 // Where the table has room for that many tiles of a sequence at most, units are not cut between work-groups and nothing is joined: one of 300 keys, 14/2 heads of
 // 64, 10.3 us; with a limit of 8, cut and joined, 14.9.
 constexpr int kWhole = 20;
-// Work-groups, one to a CU.  (512: one sequence of 33001 keys 33.9 us instead of 32.3, 32 of 500 to 16000 113 instead of 110, 128 of 20 to 1200 45 instead of 25.)
+// Work-groups, one to a CU.  (512: 32 sequences of 500 to 16000 keys, 32/8 heads of 128 112 us instead of 110, 128 of 20 to 1200, 32/8 of 64 23.8 instead of 22.9.)
 constexpr int kShares = 256;
 constexpr int kSharesLog = 8;
 // Sequences that a lane counts, so that 256 are one scan.  (1: 256 of 1 to 800 keys, 14/2 heads of 64, 17.4 us instead of 16.5; 1000 of 1 to 200, 32/8 of 64, 45.7

@@ -3,12 +3,13 @@
 // A score is defined by a float64 sum, so that the chosen pages do not depend on its order: products of two 16-bit numbers are exact in float32, their
 // sum is formed in float64 and rounded once.  A lane has 8 channels of 4 pages, so a page is 8 or 16 lanes'; their sums are exchanged inside rows of
 // lanes so that each lane ends with one page's.  With many pages conversions and additions in float64 bound it: 16 sequences of 6000 to 60000 keys in pages of 16,
-// 32/8 heads of 64, fp16 18.5 us for 49 MB of bounds, which take 9.4 to read; one sequence of 131072 keys in pages of 64, 32/8 of 128 5.7 us, 8 MB.  (Choosing the head that
+// 32/8 heads of 64, fp16 16.9 us for 49 MB of bounds, which take 9.4 to read; one sequence of 131072 keys in pages of 64, 32/8 of 128 5.7 us, 8 MB.  (Choosing the head that
 // counts by sums in float32 and summing only that one's in float64 where no other is near was slower, 23 and 6.4 us: twice the exchanges between lanes, and a
-// wave nearly always has a page where two heads are near.)
+// wave nearly always has a page where two heads are near.  So were bounds kept in float64, two products with the positive and the negative part of a query, 21: 200
+// registers leave two waves to a SIMD.)
 //
-// Choosing is latency (6.4 us for 2048 pages of one sequence, 8.3 for up to 3750 of 16; 8.7 with the scores, for 132 pages): a work-group per (sequence, KV head) finds what the wanted number of scores reaches by histograms of 256 equal ranges of the
-// numbers' order, each inside the range of the last one that holds it; the first spans the smallest to the largest score, so that two or three do, whatever the
+// Choosing is latency (6.4 us for 2048 pages of one sequence, 8.3 for up to 3750 of 16; 8.7 with the scores, for 132 pages): a work-group per (sequence,
+// KV head) finds what the wanted number of scores reaches by histograms of 256 equal ranges of the numbers' order, each inside the range of the last one that holds it; the first spans the smallest to the largest score, so that two or three do, whatever the
 // scores' exponents (at most four).  Every wave reads the bins for itself, which leaves one barrier for each histogram.  Integer work: the order in which
 // counts are added does not matter.  The code is kept short, since most of it runs once and its first instructions come from memory.
 #include "aa_kernels.h"
@@ -17,6 +18,7 @@
 namespace aa {
 
 // Pages of a lane: several share a head's queries and their sums' exchange, one leaves a wave soonest.
+// (2 in the scores' launch: the 16 sequences above 53 us a step instead of 51.5.)
 constexpr int kAbreast = 4, kAbreastFused = 1;
 constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
 constexpr int kFused = 1024;       // a table of at most that many pages is scored and chosen from by one launch
@@ -36,6 +38,69 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Bounds of 8 channels of N pages, and sums of their products with queries: exact products in float32, sums in float64.
+template <typename T, int N>
+struct Products {
+  float bounds[N][2][8];
+  static __device__ __forceinline__ u32x4 query(const u32x4 q) { return q; }  // as it is staged
+  __device__ __forceinline__ explicit Products(const u32x4 (&raw)[N][2]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) unpack8<T>(*reinterpret_cast<const uint4*>(&raw[i][w]), bounds[i][w]);
+  }
+  __device__ __forceinline__ void add(double (&sum)[N], const u32x4 raw) const {
+    float q[8];
+    unpack8<T>(*reinterpret_cast<const uint4*>(&raw), q);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool larger = q[j] >= 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum[i] += (double)(q[j] * (larger ? bounds[i][1][j] : bounds[i][0][j]));
+    }
+  }
+};
+// fp16 has an instruction that multiplies two of them into a float32, and two bounds are chosen at once by their queries' signs, for which -0 becomes 0
+// (16 sequences of 6000 to 60000 keys in pages of 16: 16.9 us, with conversions as in bf16 18.5).
+template <int N>
+struct Products<F16, N> {
+  u32x4 bounds[N][2];
+  static __device__ __forceinline__ u32x4 query(u32x4 q) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if ((q[i] & 0xffffu) == 0x8000u) q[i] &= 0xffff0000u;
+      if (q[i] >> 16 == 0x8000u) q[i] &= 0xffffu;
+    }
+    return q;
+  }
+  __device__ __forceinline__ explicit Products(const u32x4 (&raw)[N][2]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) bounds[i][w] = raw[i][w];
+  }
+  __device__ __forceinline__ void add(double (&sum)[N], const u32x4 raw) const {
+    typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t both = raw[j];
+      const i16x2 signs = *reinterpret_cast<const i16x2*>(&both) >> 15;
+      const uint32_t smaller = *reinterpret_cast<const uint32_t*>(&signs);
+      const pair q = *reinterpret_cast<const pair*>(&both);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t chosen = (bounds[i][0][j] & smaller) | (bounds[i][1][j] & ~smaller);
+        const pair x = *reinterpret_cast<const pair*>(&chosen);
+        sum[i] += (double)__builtin_fmaf((float)q[0], (float)x[0], 0.f);
+        sum[i] += (double)__builtin_fmaf((float)q[1], (float)x[1], 0.f);
+      }
+    }
+  }
+};
+
 // The scores of kPages consecutive pages of a sequence by one wave, N by each lane.
 template <typename T, int D, int N>
 struct Scores {
@@ -52,15 +117,15 @@ struct Scores {
     return x;
   }
   struct Bounds {
-    uint4 raw[N][2];
+    u32x4 raw[N][2];
   };
   static __device__ __forceinline__ Bounds load(const PagedSelectArgs& p, const int kvh, const Pages& x) {
     Bounds y;
 #pragma unroll
     for (int i = 0; i < N; ++i) {  // (behind the last page the table holds anything)
       const uint16_t* lo = p.bounds + ((int64_t)clamped_page(x.at[i], p.n_pages) * p.n_kv_heads + kvh) * 2 * D + 8 * (threadIdx.x % kLanes);
-      y.raw[i][0] = *reinterpret_cast<const uint4*>(lo);
-      y.raw[i][1] = *reinterpret_cast<const uint4*>(lo + D);
+      y.raw[i][0] = *reinterpret_cast<const u32x4*>(lo);
+      y.raw[i][1] = *reinterpret_cast<const u32x4*>(lo + D);
     }
     return y;
   }
@@ -68,37 +133,23 @@ struct Scores {
   template <typename Store>
   static __device__ __forceinline__ void form(const PagedSelectArgs& p, const int b, const int kvh, const Bounds& y, const uint32_t* staged, const int room, Store store) {
     const int lane = threadIdx.x & 63, c = lane % kLanes, group = p.n_q_heads / p.n_kv_heads;
-    float bounds[N][2][8];
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int w = 0; w < 2; ++w) unpack8<T>(y.raw[i][w], bounds[i][w]);
     const uint16_t* qp = p.q + b * p.q_sb + (int64_t)kvh * group * p.q_sh + 8 * c;
     auto query = [&](const int h) {
-      return h < room ? *reinterpret_cast<const uint4*>(staged + h * (D / 2) + 4 * c) : *reinterpret_cast<const uint4*>(qp + h * p.q_sh);
+      if (h < room) return *reinterpret_cast<const u32x4*>(staged + h * (D / 2) + 4 * c);
+      return Products<T, N>::query(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(qp + h * p.q_sh)));
     };
-    uint4 next = query(0);
-    const bool odd = lane & 1, odd2 = lane & 2;
+    const Products<T, N> products(y.raw);
+    u32x4 next = query(0);
+    // bits of a lane that say which of its pages it ends with: the same in the lane that is mirrored in 8
+    const bool odd = (kLanes == 8 ? lane ^ lane >> 2 : lane) & 1, odd2 = (kLanes == 8 ? lane ^ lane >> 1 : lane) & 2;
     float best = -INFINITY;
     bool nan = false;
 #pragma nounroll
     for (int h = 1; h <= group; ++h) {
-      float q[8];
-      unpack8<T>(next, q);
+      const u32x4 q = next;
       next = query(min(h, group - 1));
-      double sum[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) sum[i] = 0.0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool larger = q[j] >= 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] += (double)(q[j] * (larger ? bounds[i][1][j] : bounds[i][0][j]));
-      }
-      if (kLanes == 8) {  // (a lane and the one mirrored in their 8 then hold the same, and 4 neighbours all parts)
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] += dpp<kDppHalfMirror>(sum[i]);
-      }
+      double sum[N] = {};
+      products.add(sum, q);
       // while a lane has several it keeps the half that its bit names and gives the other half away
       double half[2], s;
       if (N == 4) {
@@ -110,7 +161,9 @@ struct Scores {
       }
       if (N > 1) s = (odd2 ? half[1] : half[0]) + dpp<kDppXor2>(odd2 ? half[0] : half[1]);
       else s = half[0] + dpp<kDppXor2>(half[0]);
-      if (kLanes == 16) {
+      if (kLanes == 8) {
+        s += dpp<kDppHalfMirror>(s);
+      } else {
         s += dpp<kDppRor8>(s);
         s += dpp<kDppRor4>(s);
       }
@@ -122,12 +175,12 @@ struct Scores {
 };
 
 // A group's queries to LDS by some threads, so that no head waits for memory; for how many heads there is room.
-template <int D>
+template <typename T, int D>
 __device__ __forceinline__ int stage_queries(const PagedSelectArgs& p, const int b, const int kvh, uint32_t* staged, const int words, const int thread, const int threads) {
   const int group = p.n_q_heads / p.n_kv_heads, room = min(group, words / (D / 2));
   for (int i = thread; i < room * (D / 8); i += threads)
-    reinterpret_cast<uint4*>(staged)[i] =
-        *reinterpret_cast<const uint4*>(p.q + b * p.q_sb + (int64_t)(kvh * group + i / (D / 8)) * p.q_sh + 8 * (i % (D / 8)));
+    reinterpret_cast<u32x4*>(staged)[i] =
+        Products<T, 1>::query(*reinterpret_cast<const u32x4*>(p.q + b * p.q_sb + (int64_t)(kvh * group + i / (D / 8)) * p.q_sh + 8 * (i % (D / 8))));
   return room;
 }
 
@@ -143,7 +196,7 @@ __global__ void __launch_bounds__(256) paged_scores_kernel(const PagedSelectArgs
   const int there = pages_of(clamped_length(p.lengths, b, p.max_pages, p.page_log), p.page_log);
   if (there <= p.n_chosen || first >= there) return;
   typename S::Bounds y = S::load(p, kvh, at);
-  const int room = stage_queries<D>(p, b, kvh, staged[wave], kQueryWords / 4, threadIdx.x & 63, 64);
+  const int room = stage_queries<T, D>(p, b, kvh, staged[wave], kQueryWords / 4, threadIdx.x & 63, 64);
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (read by the same wave only)
   __builtin_amdgcn_wave_barrier();
   at = S::find(p, b, first + step);
@@ -181,7 +234,7 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
   int room = 0;
   if (FROM == 0) {
     at = S::find(p, b, wave * S::kPages);
-    room = stage_queries<D>(p, b, kvh, staged, kQueryWords, tid, kChooseThreads);
+    room = stage_queries<T, D>(p, b, kvh, staged, kQueryWords, tid, kChooseThreads);
   } else {
 #pragma unroll
     for (int j = 0; j < 2; ++j) early[j] = kChooseThreads * j + tid < p.max_pages ? scores[kChooseThreads * j + tid] : 0.f;
@@ -328,7 +381,7 @@ static void launch_paged_select_for(const PagedSelectArgs& a, hipStream_t stream
     hipLaunchKernelGGL((paged_choose_kernel<T, D, 0>), units, dim3(kChooseThreads), 0, stream, a);
     return;
   }
-  // (some four thousand work-groups, however long the table is and however short the sequences)
+  // (some four thousand work-groups, however long the table is and however short the sequences: the step above with 2560 52.8 us, with 1024 57.7)
   const int chunks = (a.max_pages + Scores<T, D, kAbreast>::kPages - 1) / Scores<T, D, kAbreast>::kPages, fours = (a.n_kv_heads + 3) / 4;
   const int64_t n = (int64_t)fours * a.batch;
   const int side = (int)((4096 + n - 1) / n);

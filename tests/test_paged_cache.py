@@ -696,3 +696,18 @@ def test_pages_that_sequences_share():
     out, pages = ops.paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 6, 1, 1)
     assert torch.equal(pages, _chosen(q, s, 6, 1, 1))
     _close(out, q, s, 128 ** -0.5, pages)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("there", [60, 1400])
+def test_scores_of_zero_queries_and_infinite_bounds(there, dtype):
+    """Either zero takes the larger bound, and only that one: an infinity or NaN in the other does not count."""
+    s = _Setup([16 * there], 2, 64, 16, dtype, 14)
+    q = s.queries(70)  # (more heads than LDS has room for, where there are many pages)
+    q[:, :, 3], q[:, ::2, 4], q[:, 1::2, 4], q[0, 5, 7] = 0.0, -0.0, 0.0, float("nan")
+    for pages, channel, lo, hi in ((3, 3, float("-inf"), 1.0), (5, 4, float("-inf"), 1.0), (7, 4, float("nan"), 1.0), (9, 4, -1.0, float("inf")), (11, 9, float("-inf"), float("inf"))):
+        at = s.table[0, pages::13].long()
+        s.cache.bounds[at, 1, 0, channel], s.cache.bounds[at, 1, 1, channel] = lo, hi
+    pages = _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 20, 1, 1)[1]
+    assert torch.equal(pages, _chosen(q, s, 20, 1, 1))
