@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 
 _LIB_NAME = "libanchor_attn_hip.so"
@@ -26,6 +27,11 @@ class PagedCacheStruct(ctypes.Structure):
                 ("n_pages", c_int), ("n_kv_heads", c_int), ("page_size", c_int), ("head_dim", c_int), ("dtype", c_int)]
 
 
+# ``aa_paged_tokens`` and ``aa_paged_step`` (packed: a call with 26 arguments costs 2.2 us of ctypes' conversions, one with a packed struct 0.5)
+PAGED_TOKENS = struct.Struct("@" + "Pqq" * 4 + "PPqPqPP" + "5i0q")
+PAGED_STEP = struct.Struct("@" + "Pqq" * 2 + "PqPPNP" + "6if0q")
+
+
 class AnchorAttnHipError(RuntimeError):
     pass
 
@@ -36,7 +42,6 @@ def library_path() -> str:
 
 
 _T3 = [c_void_p, c_int64, c_int64, c_int64]  # pointer + (batch, head, row) element strides
-_T2 = [c_void_p, c_int64, c_int64]  # pointer + (token, head) element strides
 _DIMS5 = [c_int, c_int, c_int, c_int, c_int]  # batch, n_q_heads, n_kv_heads, n_ctx, head_dim
 
 _SIGNATURES = {
@@ -64,12 +69,12 @@ _SIGNATURES = {
     "aa_rope": (c_int, _T3 * 4 + [c_void_p, c_void_p, c_int64] + _DIMS5 + [c_int, c_void_p]),
     "aa_silu_mul": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_void_p]),
     "aa_dense_rows_fwd": (c_int, _T3 * 4 + [c_void_p, c_int64, c_int64] + [c_void_p, c_size_t] + [c_int] * 7 + [c_float, c_int, c_void_p]),
-    # (the first argument: the address of a PagedCacheStruct)
-    "aa_paged_append": (c_int, [c_void_p] + _T2 * 4 + [c_void_p, c_void_p, c_int64, c_int] + [c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 4 + [c_void_p]),
+    # (the address of a PagedCacheStruct, and PAGED_TOKENS or PAGED_STEP)
+    "aa_paged_append": (c_int, [c_void_p, c_char_p, c_void_p]),
     "aa_paged_decode_workspace_bytes": (c_size_t, [c_int] * 6),
-    "aa_paged_decode_fwd": (c_int, [c_void_p] + _T2 * 2 + [c_void_p, c_int64, c_void_p, c_void_p, c_size_t] + [c_int] * 3 + [c_float, c_void_p]),
+    "aa_paged_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p]),
     "aa_paged_sparse_workspace_bytes": (c_size_t, [c_int] * 7),
-    "aa_paged_sparse_decode_fwd": (c_int, [c_void_p] + _T2 * 2 + [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_size_t] + [c_int] * 6 + [c_float, c_void_p]),
+    "aa_paged_sparse_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p]),
     # the operator's sizes, then n_rows, n_keys, causal_offset
     "aa_anchor_attn_rows_workspace_bytes": (c_size_t, [c_int] * 10),
     "aa_anchor_attn_rows_fwd": (c_int, _T3 * 8 + [c_int] * 3 + [c_float] + [c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_double] + _DIMS5

@@ -110,12 +110,12 @@ class PagedCache:
             _refuse(f"{batch} sequences of up to {most} pages of {self.page_size} are not supported (at most 65535 sequences, 1048576 keys, at least one page)")
         return (table, page_table.stride(0), lengths_ptr), batch, most
 
-    def _launch(self, fn, *args):
+    def _launch(self, fn, packed):
         if self.index == torch.cuda.current_device():
-            rc = fn(self._address, *args, _stream())
+            rc = fn(self._address, packed, _stream())
         else:
             with torch.cuda.device(self.device):
-                rc = fn(self._address, *args, _stream())
+                rc = fn(self._address, packed, _stream())
         if rc:
             _hip.check(rc)
 
@@ -149,26 +149,26 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
     k_args, (n, _, _) = _rows(k, "k", cache, cache.n_kv_heads)
     v_args, (n_values, _, _) = _rows(v, "v", cache, cache.n_kv_heads)
     tables, batch, most = cache._tables(page_table, lengths)
-    starts_ptr = None if starts is None else _indices(starts, "starts", cache, 1, batch + 1)
+    starts_ptr = 0 if starts is None else _indices(starts, "starts", cache, 1, batch + 1)
     if n_values != n or (starts is None and n != batch) or n * cache.n_kv_heads >= 1 << 23:
         _refuse(f"{n} keys, {n_values} values and {batch} sequences{' without starts' if starts is None else ''} do not go together (and fewer than 2^23 rows of keys)")
     if cos is None:
         if sin is not None or q is not None or out is not None:
             _refuse("cos and sin come together, and queries need them")
-        angles, q_args, heads = (None, None, 0, 0), (None, 0, 0, None, 0, 0), 0
+        angles, n_positions, q_args, heads = (0, 0, 0), 0, (0,) * 6, 0
     else:
         strides = cos.stride()
         for t in (cos, sin):
             if type(t) not in _TYPES or t.dtype != _FLOAT32 or t.get_device() != cache.index or t.dim() != 2 or t.shape != cos.shape or t.stride() != strides:
                 _refuse("cos and sin must be float32 tensors [positions, D / 2] on the cache's device, laid out alike")
         n_positions, half = cos.shape
-        angles = (cos.data_ptr(), sin.data_ptr(), strides[0], n_positions)
+        angles = (cos.data_ptr(), sin.data_ptr(), strides[0])
         if half * 2 != cache.head_dim or not n_positions or strides[1] != 1 or strides[0] & 3 or strides[0] < half or (angles[0] | angles[1]) & 15:
             _refuse("the rows of cos and sin must hold D / 2 elements, contiguous on 16-byte boundaries")
         if q is None:
             if out is not None:
                 _refuse("an output needs queries")
-            q_args, heads = (None, 0, 0, None, 0, 0), 0
+            q_args, heads = (0,) * 6, 0
         else:
             q_rows, shape = _rows(q, "q", cache, 0)
             heads = shape[1]
@@ -176,7 +176,7 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
                 _refuse(f"q has {shape[0]} tokens, k {n}")
             q_args = (*q_rows, *_out_rows(out, shape, cache)) if out is not None else (*q_rows, *_new_rows(out := torch.empty_like(q)))
     if n and batch:
-        cache._launch(_hip.lib().aa_paged_append, *q_args, *k_args, *v_args, *angles, *tables, starts_ptr, batch, n, heads, most)
+        cache._launch(_hip.lib().aa_paged_append, _hip.PAGED_TOKENS.pack(*q_args, *k_args, *v_args, *angles, *tables, starts_ptr, n_positions, batch, n, heads, most))
     return out
 
 
@@ -217,7 +217,7 @@ def paged_decode_attention(cache: PagedCache, q: torch.Tensor, page_table: torch
         lib = _hip.lib()
         nbytes = lib.aa_paged_decode_workspace_bytes(*sizes, cache.n_kv_heads, cache.head_dim, cache.page_size, most)
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=cache.device) if nbytes else None
-        cache._launch(lib.aa_paged_decode_fwd, *tensors, ws.data_ptr() if nbytes else None, nbytes, *sizes, most, scale)
+        cache._launch(lib.aa_paged_decode_fwd, _hip.PAGED_STEP.pack(*tensors, ws.data_ptr() if nbytes else 0, nbytes, 0, *sizes, most, 0, 0, 0, scale))
     return out
 
 
@@ -240,5 +240,6 @@ def paged_sparse_decode_attention(cache: PagedCache, q: torch.Tensor, page_table
         lib = _hip.lib()
         nbytes = lib.aa_paged_sparse_workspace_bytes(*sizes, cache.n_kv_heads, cache.head_dim, cache.page_size, most, n_pages)
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=cache.device)
-        cache._launch(lib.aa_paged_sparse_decode_fwd, *tensors, pages.data_ptr(), ws.data_ptr(), nbytes, *sizes, most, n_pages, n_first, n_last, scale)
+        cache._launch(lib.aa_paged_sparse_decode_fwd,
+                      _hip.PAGED_STEP.pack(*tensors, ws.data_ptr(), nbytes, pages.data_ptr(), *sizes, most, n_pages, n_first, n_last, scale))
     return out, pages

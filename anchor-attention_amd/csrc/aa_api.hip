@@ -889,6 +889,11 @@ static int check_rows(const void* ptr, int64_t st, int64_t sh, const char* who, 
   return AA_OK;
 }
 
+static int check_given(const void* ptr, const char* who, const char* name) {
+  if (ptr == nullptr) set_error("%s: %s is NULL", who, name);
+  return ptr == nullptr ? AA_EBADARG : AA_OK;
+}
+
 static int check_words(const void* ptr, const char* who, const char* name) {
   if (ptr == nullptr) {
     set_error("%s: %s is NULL", who, name);
@@ -923,38 +928,37 @@ static int check_cache(const char* who, const aa_paged_cache* c, int batch, int 
 
 static int log2_of(int power) { return 31 - __builtin_clz((unsigned)power); }
 
-int aa_paged_append(const aa_paged_cache* cache, const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
-                    const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
-                    const float* cos, const float* sin, int64_t cs_sn, int n_positions,
-                    const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, const int32_t* starts,
-                    int batch, int n_tokens, int n_q_heads, int max_pages, void* stream) {
+int aa_paged_append(const aa_paged_cache* cache, const aa_paged_tokens* t, void* stream) {
   const char* who = "aa_paged_append";
   int rc;
-  if ((rc = check_cache(who, cache, batch, n_q_heads, max_pages, page_table, lengths))) return rc;
-  if (n_tokens <= 0 || n_tokens >= 1 << 24 || (int64_t)n_tokens * cache->n_kv_heads >= 1 << 23 || (starts == nullptr && n_tokens != batch)) {
+  if ((rc = check_given(t, who, "tokens")) || (rc = check_cache(who, cache, t->batch, t->n_q_heads, t->max_pages, t->page_table, t->lengths))) return rc;
+  if (t->n_tokens <= 0 || t->n_tokens >= 1 << 24 || (int64_t)t->n_tokens * cache->n_kv_heads >= 1 << 23 || (t->starts == nullptr && t->n_tokens != t->batch)) {
     set_error("%s: %d tokens of %d sequences are not supported (at least 1, fewer than 2^23 with their KV heads, without starts one of each sequence)",
-              who, n_tokens, batch);
-    return n_tokens <= 0 ? AA_EBADARG : AA_EUNSUPPORTED;
+              who, t->n_tokens, t->batch);
+    return t->n_tokens <= 0 ? AA_EBADARG : AA_EUNSUPPORTED;
   }
-  if ((cos == nullptr) != (sin == nullptr) || (q == nullptr) != (n_q_heads == 0) || (q == nullptr) != (q_out == nullptr) || (q != nullptr && cos == nullptr)) {
+  if ((t->cos == nullptr) != (t->sin == nullptr) || (t->q == nullptr) != (t->n_q_heads == 0) || (t->q == nullptr) != (t->q_out == nullptr) ||
+      (t->q != nullptr && t->cos == nullptr)) {
     set_error("%s: cos and sin come together, and so do q, q_out and query heads, which need them", who);
     return AA_EBADARG;
   }
-  if ((q != nullptr && ((rc = check_rows(q, q_st, q_sh, who, "q")) || (rc = check_rows(q_out, qo_st, qo_sh, who, "q_out")))) ||
-      (rc = check_rows(k, k_st, k_sh, who, "k")) || (rc = check_rows(v, v_st, v_sh, who, "v")) ||
-      (starts != nullptr && (rc = check_words(starts, who, "starts"))))
+  if ((t->q != nullptr && ((rc = check_rows(t->q, t->q_st, t->q_sh, who, "q")) || (rc = check_rows(t->q_out, t->qo_st, t->qo_sh, who, "q_out")))) ||
+      (rc = check_rows(t->k, t->k_st, t->k_sh, who, "k")) || (rc = check_rows(t->v, t->v_st, t->v_sh, who, "v")) ||
+      (t->starts != nullptr && (rc = check_words(t->starts, who, "starts"))))
     return rc;
-  if (cos != nullptr) {
-    if ((rc = check_ptr(cos, who, "cos")) || (rc = check_ptr(sin, who, "sin"))) return rc;
-    if (n_positions <= 0 || cs_sn < cache->head_dim / 2 || cs_sn % 4 != 0) {
-      set_error("%s: cos and sin must have rows of head_dim / 2 elements on 16-byte boundaries (got %d, %lld elements apart)", who, n_positions, (long long)cs_sn);
+  if (t->cos != nullptr) {
+    if ((rc = check_ptr(t->cos, who, "cos")) || (rc = check_ptr(t->sin, who, "sin"))) return rc;
+    if (t->n_positions <= 0 || t->cs_sn < cache->head_dim / 2 || t->cs_sn % 4 != 0) {
+      set_error("%s: cos and sin must have rows of head_dim / 2 elements on 16-byte boundaries (got %d, %lld elements apart)", who, t->n_positions,
+                (long long)t->cs_sn);
       return AA_EBADARG;
     }
   }
-  const PagedAppendArgs a = {(const uint16_t*)q, q_st, q_sh, (uint16_t*)q_out, qo_st, qo_sh, (const uint16_t*)k, k_st, k_sh, (const uint16_t*)v, v_st, v_sh,
-                             cos, sin, cs_sn, n_positions, (uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn, (uint16_t*)cache->values,
-                             cache->vp_sp, cache->vp_sh, cache->vp_sn, (uint16_t*)cache->bounds, page_table, pt_sb, lengths, starts, batch, n_tokens, n_q_heads,
-                             cache->n_kv_heads, cache->head_dim, cache->n_pages, log2_of(cache->page_size), max_pages, cache->dtype, 0, 0};
+  const PagedAppendArgs a = {(const uint16_t*)t->q, t->q_st, t->q_sh, (uint16_t*)t->q_out, t->qo_st, t->qo_sh, (const uint16_t*)t->k, t->k_st, t->k_sh,
+                             (const uint16_t*)t->v, t->v_st, t->v_sh, t->cos, t->sin, t->cs_sn, t->n_positions, (uint16_t*)cache->keys, cache->kp_sp,
+                             cache->kp_sh, cache->kp_sn, (uint16_t*)cache->values, cache->vp_sp, cache->vp_sh, cache->vp_sn, (uint16_t*)cache->bounds,
+                             t->page_table, t->pt_sb, t->lengths, t->starts, t->batch, t->n_tokens, t->n_q_heads, cache->n_kv_heads, cache->head_dim,
+                             cache->n_pages, log2_of(cache->page_size), t->max_pages, cache->dtype, 0, 0};
   return check_launch(launch_paged_append(a, (hipStream_t)stream), who);
 }
 
@@ -971,42 +975,37 @@ static void give_scratch(PagedDecodeArgs& a, char* workspace, int max_pages) {
   a.parts = (float*)(workspace + s.parts);
 }
 
-static int paged_decode_args(const char* who, PagedDecodeArgs& a, const aa_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, void* out,
-                             int64_t o_sb, int64_t o_sh, const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, void* workspace,
-                             size_t workspace_bytes, size_t needed, int batch, int n_q_heads, int max_pages, float sm_scale) {
+static int paged_decode_args(const char* who, PagedDecodeArgs& a, const aa_paged_cache* cache, const aa_paged_step* t, size_t needed) {
   int rc;
-  if (n_q_heads == 0 || !(sm_scale > 0.f) || sm_scale > 3.4e38f) {
-    set_error("%s: %d query heads and sm_scale %g: both must be positive and finite", who, n_q_heads, (double)sm_scale);
+  if (t->n_q_heads == 0 || !(t->sm_scale > 0.f) || t->sm_scale > 3.4e38f) {
+    set_error("%s: %d query heads and sm_scale %g: both must be positive and finite", who, t->n_q_heads, (double)t->sm_scale);
     return AA_EBADARG;
   }
-  if ((int64_t)batch * n_q_heads >= 1 << 24) {
-    set_error("%s: %d sequences of %d query heads are not supported (fewer than 2^24 together)", who, batch, n_q_heads);
+  if ((int64_t)t->batch * t->n_q_heads >= 1 << 24) {
+    set_error("%s: %d sequences of %d query heads are not supported (fewer than 2^24 together)", who, t->batch, t->n_q_heads);
     return AA_EUNSUPPORTED;
   }
-  if ((rc = check_rows(q, q_sb, q_sh, who, "q")) || (rc = check_rows(out, o_sb, o_sh, who, "out")) || (needed > 0 && (rc = check_ptr(workspace, who, "workspace"))))
+  if ((rc = check_rows(t->q, t->q_sb, t->q_sh, who, "q")) || (rc = check_rows(t->out, t->o_sb, t->o_sh, who, "out")) ||
+      (needed > 0 && (rc = check_ptr(t->workspace, who, "workspace"))))
     return rc;
-  if (workspace_bytes < needed) {
-    set_error("%s: workspace has %zu bytes, %zu needed", who, workspace_bytes, needed);
+  if (t->workspace_bytes < needed) {
+    set_error("%s: workspace has %zu bytes, %zu needed", who, t->workspace_bytes, needed);
     return AA_EBADARG;
   }
-  a = {(const uint16_t*)q, q_sb, q_sh, (uint16_t*)out, o_sb, o_sh, (const uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn,
-       (const uint16_t*)cache->values, cache->vp_sp, cache->vp_sh, cache->vp_sn, page_table, pt_sb, 0, lengths, batch, n_q_heads, cache->n_kv_heads,
-       cache->head_dim, cache->n_pages, log2_of(cache->page_size), max_pages, 0, sm_scale, nullptr, nullptr, nullptr, cache->dtype};
+  a = {(const uint16_t*)t->q, t->q_sb, t->q_sh, (uint16_t*)t->out, t->o_sb, t->o_sh, (const uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn,
+       (const uint16_t*)cache->values, cache->vp_sp, cache->vp_sh, cache->vp_sn, t->page_table, t->pt_sb, 0, t->lengths, t->batch, t->n_q_heads,
+       cache->n_kv_heads, cache->head_dim, cache->n_pages, log2_of(cache->page_size), t->max_pages, 0, t->sm_scale, nullptr, nullptr, nullptr, cache->dtype};
   return AA_OK;
 }
 
-int aa_paged_decode_fwd(const aa_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
-                        const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, void* workspace, size_t workspace_bytes,
-                        int batch, int n_q_heads, int max_pages, float sm_scale, void* stream) {
+int aa_paged_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* t, void* stream) {
   const char* who = "aa_paged_decode_fwd";
   PagedDecodeArgs a;
   int rc;
-  if ((rc = check_cache(who, cache, batch, n_q_heads, max_pages, page_table, lengths))) return rc;
-  const size_t needed = paged_decode_scratch(cache->head_dim, log2_of(cache->page_size), max_pages).total;
-  if ((rc = paged_decode_args(who, a, cache, q, q_sb, q_sh, out, o_sb, o_sh, page_table, pt_sb, lengths, workspace, workspace_bytes, needed, batch, n_q_heads,
-                              max_pages, sm_scale)))
-    return rc;
-  give_scratch(a, static_cast<char*>(workspace), max_pages);
+  if ((rc = check_given(t, who, "step")) || (rc = check_cache(who, cache, t->batch, t->n_q_heads, t->max_pages, t->page_table, t->lengths))) return rc;
+  const size_t needed = paged_decode_scratch(cache->head_dim, log2_of(cache->page_size), t->max_pages).total;
+  if ((rc = paged_decode_args(who, a, cache, t, needed))) return rc;
+  give_scratch(a, static_cast<char*>(t->workspace), t->max_pages);
   return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
 }
 
@@ -1028,33 +1027,31 @@ size_t aa_paged_sparse_workspace_bytes(int batch, int n_q_heads, int n_kv_heads,
   return carve_sparse(batch, n_kv_heads, head_dim, page_size, max_pages, n_chosen).total;
 }
 
-int aa_paged_sparse_decode_fwd(const aa_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
-                               const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, int32_t* pages, void* workspace, size_t workspace_bytes,
-                               int batch, int n_q_heads, int max_pages, int n_chosen, int n_first, int n_last, float sm_scale, void* stream) {
+int aa_paged_sparse_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* t, void* stream) {
   const char* who = "aa_paged_sparse_decode_fwd";
   PagedDecodeArgs a;
   int rc;
-  if (n_first < 0 || n_last < 1 || n_chosen > 1 << 16 || (int64_t)n_first + n_last > n_chosen) {
-    set_error("%s: %d pages, the first %d and the last %d among them, are not supported (at most 65536, at least the last one)", who, n_chosen, n_first, n_last);
+  if ((rc = check_given(t, who, "step"))) return rc;
+  if (t->n_first < 0 || t->n_last < 1 || t->n_chosen > 1 << 16 || (int64_t)t->n_first + t->n_last > t->n_chosen) {
+    set_error("%s: %d pages, the first %d and the last %d among them, are not supported (at most 65536, at least the last one)", who, t->n_chosen, t->n_first,
+              t->n_last);
     return AA_EBADARG;
   }
-  if ((rc = check_cache(who, cache, batch, n_q_heads, max_pages, page_table, lengths)) || (rc = check_ptr(cache->bounds, who, "bounds")) ||
-      (rc = check_words(pages, who, "pages")))
+  if ((rc = check_cache(who, cache, t->batch, t->n_q_heads, t->max_pages, t->page_table, t->lengths)) || (rc = check_ptr(cache->bounds, who, "bounds")) ||
+      (rc = check_words(t->pages, who, "pages")))
     return rc;
-  const SparseScratch w = carve_sparse(batch, cache->n_kv_heads, cache->head_dim, cache->page_size, max_pages, n_chosen);
-  if ((rc = paged_decode_args(who, a, cache, q, q_sb, q_sh, out, o_sb, o_sh, page_table, pt_sb, lengths, workspace, workspace_bytes, w.total, batch, n_q_heads,
-                              max_pages, sm_scale)))
-    return rc;
-  char* ws = static_cast<char*>(workspace);
-  const PagedSelectArgs s = {a.q, q_sb, q_sh, (const uint16_t*)cache->bounds, page_table, pt_sb, lengths, (float*)(ws + w.scores), pages,
-                             (int32_t*)(ws + w.chosen), batch, n_q_heads, cache->n_kv_heads, cache->head_dim, cache->n_pages, a.page_log, max_pages, n_chosen,
-                             n_first, n_last, cache->dtype};
+  const SparseScratch w = carve_sparse(t->batch, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages, t->n_chosen);
+  if ((rc = paged_decode_args(who, a, cache, t, w.total))) return rc;
+  char* ws = static_cast<char*>(t->workspace);
+  const PagedSelectArgs s = {a.q, a.q_sb, a.q_sh, (const uint16_t*)cache->bounds, t->page_table, t->pt_sb, t->lengths, (float*)(ws + w.scores), t->pages,
+                             (int32_t*)(ws + w.chosen), a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim, a.n_pages, a.page_log, a.max_pages, t->n_chosen,
+                             t->n_first, t->n_last, cache->dtype};
   if ((rc = check_launch(launch_paged_select(s, (hipStream_t)stream), who))) return rc;
   a.table = s.chosen;
-  a.t_sb = (int64_t)cache->n_kv_heads * n_chosen;
-  a.t_sh = n_chosen;
-  a.n_chosen = n_chosen;
-  give_scratch(a, ws + w.decode, std::min(n_chosen, max_pages));
+  a.t_sb = (int64_t)a.n_kv_heads * t->n_chosen;
+  a.t_sh = t->n_chosen;
+  a.n_chosen = t->n_chosen;
+  give_scratch(a, ws + w.decode, std::min(t->n_chosen, t->max_pages));
   return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
 }
 

@@ -294,19 +294,38 @@ typedef struct {
   int n_pages, n_kv_heads, page_size, head_dim, dtype;
 } aa_paged_cache;
 
-int aa_paged_append(const aa_paged_cache* cache, const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
-                    const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
-                    const float* cos, const float* sin, int64_t cs_sn, int n_positions,
-                    const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, const int32_t* starts,
-                    int batch, int n_tokens, int n_q_heads, int max_pages, void* stream);
+/* What aa_paged_append is given (host memory, read during the call only). */
+typedef struct {
+  const void* q; int64_t q_st, q_sh;
+  void* q_out; int64_t qo_st, qo_sh;
+  const void* k; int64_t k_st, k_sh;
+  const void* v; int64_t v_st, v_sh;
+  const float* cos;
+  const float* sin; int64_t cs_sn;
+  const int32_t* page_table; int64_t pt_sb;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int n_positions, batch, n_tokens, n_q_heads, max_pages;
+} aa_paged_tokens;
+
+/* What a decode step is given (likewise). */
+typedef struct {
+  const void* q; int64_t q_sb, q_sh;
+  void* out; int64_t o_sb, o_sh;
+  const int32_t* page_table; int64_t pt_sb;
+  const int32_t* lengths;
+  void* workspace; size_t workspace_bytes;
+  int32_t* pages;                 /* sparse steps only */
+  int batch, n_q_heads, max_pages;
+  int n_chosen, n_first, n_last;  /* sparse steps only */
+  float sm_scale;
+} aa_paged_step;
+
+int aa_paged_append(const aa_paged_cache* cache, const aa_paged_tokens* tokens, void* stream);
 size_t aa_paged_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages);
-int aa_paged_decode_fwd(const aa_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
-                        const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, void* workspace, size_t workspace_bytes,
-                        int batch, int n_q_heads, int max_pages, float sm_scale, void* stream);
+int aa_paged_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, void* stream);
 size_t aa_paged_sparse_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_chosen);
-int aa_paged_sparse_decode_fwd(const aa_paged_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, void* out, int64_t o_sb, int64_t o_sh,
-                               const int32_t* page_table, int64_t pt_sb, const int32_t* lengths, int32_t* pages, void* workspace, size_t workspace_bytes,
-                               int batch, int n_q_heads, int max_pages, int n_chosen, int n_first, int n_last, float sm_scale, void* stream);
+int aa_paged_sparse_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, void* stream);
 
 #ifdef __cplusplus
 }

@@ -10,6 +10,7 @@ off by u^2 (fp16: its grid of 2^-39 too, covered by 2^-14); sums over n keys in 
 result is rounded once, u of it.  The chosen pages have to be the same."""
 import copy
 import ctypes
+import pathlib
 import pickle
 import types
 
@@ -506,20 +507,18 @@ def test_two_streams_at_once():
 
 CACHE = {"keys": 4096, "kp_sp": 4096, "kp_sh": 2048, "kp_sn": 128, "values": 4096, "vp_sp": 4096, "vp_sh": 2048, "vp_sn": 128, "bounds": 4096,
          "n_pages": 9, "n_kv_heads": 2, "page_size": 16, "head_dim": 128, "dtype": 0}
-APPEND = {"cache": CACHE, "q": 4096, "q_st": 1024, "q_sh": 128, "q_out": 4096, "qo_st": 1024, "qo_sh": 128, "k": 4096, "k_st": 256, "k_sh": 128, "v": 4096, "v_st": 256,
-          "v_sh": 128, "cos": 4096, "sin": 4096, "cs_sn": 64, "n_positions": 100, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "starts": 4096, "batch": 2, "n_tokens": 5,
-          "n_q_heads": 8, "max_pages": 8, "stream": None}
-DECODE = {"cache": CACHE, "q": 4096, "q_sb": 1024, "q_sh": 128, "out": 4096, "o_sb": 1024, "o_sh": 128, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "workspace": 4096,
-          "workspace_bytes": 1 << 40, "batch": 2, "n_q_heads": 8, "max_pages": 100, "sm_scale": 0.1, "stream": None}
-SPARSE = {**{k: DECODE[k] for k in list(DECODE)[:10]}, "pages": 4096, **{k: DECODE[k] for k in list(DECODE)[10:15]}, "n_chosen": 4, "n_first": 1, "n_last": 1, "sm_scale": 0.1,
-          "stream": None}
+TOKENS = {"q": 4096, "q_st": 1024, "q_sh": 128, "q_out": 4096, "qo_st": 1024, "qo_sh": 128, "k": 4096, "k_st": 256, "k_sh": 128, "v": 4096, "v_st": 256, "v_sh": 128,
+          "cos": 4096, "sin": 4096, "cs_sn": 64, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "starts": 4096, "n_positions": 100, "batch": 2, "n_tokens": 5, "n_q_heads": 8,
+          "max_pages": 8}
+STEP = {"q": 4096, "q_sb": 1024, "q_sh": 128, "out": 4096, "o_sb": 1024, "o_sh": 128, "page_table": 4096, "pt_sb": 8, "lengths": 4096, "workspace": 4096,
+        "workspace_bytes": 1 << 40, "pages": 4096, "batch": 2, "n_q_heads": 8, "max_pages": 100, "n_chosen": 4, "n_first": 1, "n_last": 1, "sm_scale": 0.1}
 EVERY = [({"batch": 0}, "must be positive"), ({"batch": 65536}, "not supported"), ({"n_kv_heads": 3}, "must divide"), ({"n_kv_heads": 0}, "must be positive"),
          ({"head_dim": 96}, "head_dim 96"), ({"page_size": 48}, "page_size 48"), ({"page_size": 8}, "page_size 8"), ({"n_pages": 0}, "must be positive"),
          ({"max_pages": 0}, "must be positive"), ({"max_pages": 65537}, "not supported"), ({"dtype": 2}, "dtype"), ({"keys": 0}, "keys is NULL"),
          ({"keys": 4104}, "keys must be 16-byte aligned"), ({"kp_sh": 2052}, "keys must be 16-byte aligned"), ({"vp_sn": 120}, "smaller than head_dim"),
          ({"vp_sn": 16392}, "larger than 16384"), ({"values": 0}, "values is NULL"), ({"page_table": 0}, "page_table is NULL"), ({"lengths": 0}, "lengths is NULL"),
          ({"lengths": 4098}, "lengths must be 4-byte aligned"), ({"q": 4104}, "q must be 16-byte aligned"), ({"q_sh": 60}, "q must have strides"),
-         ({"bounds": 8}, "bounds must be 16-byte"), ({"cache": None}, "cache is NULL")]
+         ({"bounds": 8}, "bounds must be 16-byte"), ({"cache": None}, "cache is NULL"), ({"given": None}, "is NULL")]
 READ = [({"q": 0}, "q is NULL"), ({"out": 0}, "out is NULL"), ({"out": 8}, "out must be 16-byte"), ({"sm_scale": 0.0}, "sm_scale"), ({"sm_scale": float("nan")}, "sm_scale"),
         ({"sm_scale": float("inf")}, "sm_scale"), ({"n_q_heads": 0}, "query heads"), ({"batch": 4096, "n_q_heads": 4096}, "together")]
 
@@ -538,14 +537,27 @@ READ = [({"q": 0}, "q is NULL"), ({"out": 0}, "out is NULL"), ({"out": 8}, "out 
 def test_what_the_c_interface_refuses(fn, change, message):
     """Before anything is launched: the addresses are never read."""
     from anchor_attn.src.ops import _hip
-    args, f = {"append": (APPEND, _hip.lib().aa_paged_append), "decode": (DECODE, _hip.lib().aa_paged_decode_fwd), "sparse": (SPARSE, _hip.lib().aa_paged_sparse_decode_fwd)}[fn]
-    assert len(args) == len(f.argtypes) and set(change) <= set(args) | set(CACHE)
-    args = {**args, **{k: v for k, v in change.items() if k in args}}
-    if args["cache"] is not None:
-        struct = _hip.PagedCacheStruct(*{**CACHE, **{k: v for k, v in change.items() if k in CACHE}}.values())
-        args["cache"] = ctypes.addressof(struct)
+    lib = _hip.lib()
+    given, packs, f = {"append": (TOKENS, _hip.PAGED_TOKENS, lib.aa_paged_append), "decode": (STEP, _hip.PAGED_STEP, lib.aa_paged_decode_fwd),
+                       "sparse": (STEP, _hip.PAGED_STEP, lib.aa_paged_sparse_decode_fwd)}[fn]
+    assert set(change) <= {*given, *CACHE, "cache", "given"}
+    struct = _hip.PagedCacheStruct(*{**CACHE, **{k: v for k, v in change.items() if k in CACHE}}.values())
     with pytest.raises(_hip.AnchorAttnHipError, match=message):
-        _hip.check(f(*args.values()))
+        _hip.check(f(None if "cache" in change else ctypes.addressof(struct),
+                     None if "given" in change else packs.pack(*{**given, **{k: v for k, v in change.items() if k in given}}.values()), None))
+
+
+def test_packed_structs_are_laid_out_as_in_c(tmp_path):
+    import subprocess
+    from anchor_attn.src.ops import _hip
+    source = tmp_path / "sizes.c"
+    source.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "anchor_attn_hip.h"\nint main(void) { printf("%zu %zu %zu %zu %zu", sizeof(aa_paged_cache), '
+                      'sizeof(aa_paged_tokens), sizeof(aa_paged_step), offsetof(aa_paged_tokens, n_positions), offsetof(aa_paged_step, sm_scale)); return 0; }\n')
+    include = pathlib.Path(__file__).resolve().parent.parent / "include"
+    subprocess.run(["gcc", f"-I{include}", "-o", tmp_path / "sizes", source], check=True)
+    sizes = [int(x) for x in subprocess.run([tmp_path / "sizes"], check=True, capture_output=True, text=True).stdout.split()]
+    assert sizes[:3] == [ctypes.sizeof(_hip.PagedCacheStruct), _hip.PAGED_TOKENS.size, _hip.PAGED_STEP.size]
+    assert _hip.PAGED_TOKENS.pack(*range(24))[sizes[3]] == 19 and _hip.PAGED_STEP.pack(*[0] * 18, 1.0)[sizes[4]:][:4] == b"\0\0\x80?"
 
 
 def test_caches_that_are_refused():
