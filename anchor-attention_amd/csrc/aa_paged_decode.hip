@@ -471,41 +471,48 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
   __syncthreads();
   int4* header = reinterpret_cast<int4*>(p.headers) + blockIdx.x;
   bool goes_on = false;
-  // the unit that began before this work-group, then those that begin in a wave and do not end there
-  for (int e = 0; e < 2 * WAVES;) {  // (entry 2 w + which of parts_of; waves without a share have none)
-    const int4 info = parts_of[e >> 1][e & 1];
-    const int first = e++;
-    if (info.x == 0) continue;
+  // the unit that began before this work-group, then those that begin in a wave and do not end there.  (Entry 2 w + which of parts_of is a lane's; waves without
+  // a share have none)
+  const int4 mine = parts_of[min(lane, 2 * WAVES - 1) >> 1][lane & 1];
+  uint32_t left = (uint32_t)__ballot(lane < 2 * WAVES && mine.x != 0);
+  const uint32_t last_ones = (uint32_t)__ballot(lane < 2 * WAVES && mine.x == 2);
+  while (left != 0) {
+    const int first = __builtin_ctz(left);
     const bool begins = first & 1;
-    bool ends = info.x == 2;
     uint32_t entries = 1u << first;  // of this unit
-    for (; e < 2 * WAVES && !ends; ++e) {
-      const int x = parts_of[e >> 1][e & 1].x;
-      if (x == 0) continue;
-      if (e & 1) break;
-      entries |= 1u << e;
-      ends = x == 2;
+    left &= left - 1;
+    bool ends = last_ones & entries;
+    while (!ends && left != 0 && !(__builtin_ctz(left) & 1)) {
+      const uint32_t next = left & -left;
+      entries |= next;
+      ends = last_ones & next;
+      left &= left - 1;
     }
+    const int4 info = {0, __builtin_amdgcn_readlane(mine.y, first), __builtin_amdgcn_readlane(mine.z, first), __builtin_amdgcn_readlane(mine.w, first)};
     const int head0 = info.z & 0xffff, n_cols = info.z >> 16;
     for (int i = tid; i < n_cols * (D / 4); i += 64 * WAVES) {
       const int col = i / (D / 4), d = 4 * (i % (D / 4));
-      float m = -INFINITY, ms[WAVES];
+      float m = -INFINITY, l = 0.f, ms[WAVES], ls[WAVES];
+      floatx4 x = {0.f, 0.f, 0.f, 0.f}, xs[WAVES];
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) {  // (one entry a wave: the second of the one that the unit begins in, the first of others)
-        ms[w] = entries >> (2 * w) & 3u ? stats[w][2 * w + 1 == first][0][col] : -INFINITY;
+      for (int w = 0; w < WAVES; ++w) {  // (one entry a wave: the second of the one that the unit begins in, the first of others; all are read at once)
+        const int k = 2 * w + 1 == first;
+        ms[w] = stats[w][k][0][col];
+        ls[w] = stats[w][k][1][col];
+        xs[w] = *reinterpret_cast<const floatx4*>(states + ((2 * w + k) * most_cols + col) * kPitch + d);
+      }
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        ms[w] = entries >> (2 * w) & 3u ? ms[w] : -INFINITY;
         m = fmaxf(m, ms[w]);
       }
-      float l = 0.f;
-      floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
         if (!(entries >> (2 * w) & 3u)) continue;
-        const int k = 2 * w + 1 == first;
         const float weight = ms[w] == -INFINITY ? 0.f : fast_exp2((ms[w] - m) * scale);
-        l += weight * stats[w][k][1][col];
-        const floatx4 y = *reinterpret_cast<const floatx4*>(states + ((2 * w + k) * most_cols + col) * kPitch + d);
+        l += weight * ls[w];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] += weight * y[e];
+        for (int e = 0; e < 4; ++e) x[e] += weight * xs[w][e];
       }
       if (begins && ends) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
