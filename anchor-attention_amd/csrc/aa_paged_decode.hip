@@ -40,9 +40,9 @@ constexpr int kWhole = 20;
 // Work-groups, one to a CU.  (512: 32 sequences of 500 to 16000 keys, 32/8 heads of 128 112 us instead of 110, 128 of 20 to 1200, 32/8 of 64 23.8 instead of 22.9.)
 constexpr int kShares = 256;
 constexpr int kSharesLog = 8;
-// Sequences that a lane counts, so that 256 are one scan.  (1: 256 of 1 to 800 keys, 14/2 heads of 64, 17.4 us instead of 16.5; 1000 of 1 to 200, 32/8 of 64, 45.7
+// Sequences that a lane counts where there are more than 64, so that 256 are one scan.  (1: 256 of 1 to 800 keys, 14/2 heads of 64, 17.4 us instead of 16.5; 1000 of 1 to 200, 32/8 of 64, 45.7
 // instead of 40.4; up to 128 the same.)
-constexpr int kPerLane = 4;
+constexpr int kPerLane = 4, kPerLaneLog = 2;
 // Tiles of a share at least: fewer work-groups leave fewer parts to join, and each has longer to go.  (64 pages of 64 of one sequence, 32/8 heads of 128, chosen and
 // read: 4 24.4 us, 8 24.4, 16 26.7.)
 constexpr int kLeast = 8;
@@ -118,22 +118,25 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
   // ---- this wave's share -------------------------------------------------------------------------
   // All units one after the other, each as long as its tiles and kOver.  A lane has kPerLane sequences in a row, a scan 64 lanes' (whose numbers stay if
   // there are no more)
-  int keys0[kPerLane], sum0 = 0;
+  const int per_log = p.batch <= 64 ? 0 : kPerLaneLog;
+  int keys0[kPerLane] = {}, sum0 = 0;
   auto scan = [&](const int i, int (&keys)[kPerLane], int& sum) __attribute__((always_inline)) {  // of the sequences from i on: their keys, and the sums up to each lane's last
     int own = 0;
 #pragma unroll
     for (int j = 0; j < kPerLane; ++j) {
-      const int b = i + kPerLane * lane + j;
+      if (j > 0 && per_log == 0) break;
+      const int b = i + (lane << per_log) + j;
       keys[j] = b < p.batch ? keys_of(p, p.lengths[b]) : 0;
       own += b < p.batch ? tiles_of(keys[j]) + kOver : 0;
     }
     sum = sums_up_to(own);
   };
   auto keys_at = [&](const int (&keys)[kPerLane], const int at) {  // of the at-th sequence of a scan
-    int x = __builtin_amdgcn_readlane(keys[0], at / kPerLane);
+    int x = __builtin_amdgcn_readlane(keys[0], at >> per_log);
 #pragma unroll
     for (int j = 1; j < kPerLane; ++j) {
-      const int y = __builtin_amdgcn_readlane(keys[j], at / kPerLane);
+      if (per_log == 0) break;
+      const int y = __builtin_amdgcn_readlane(keys[j], at >> per_log);
       x = at % kPerLane == j ? y : x;
     }
     return x;
@@ -168,11 +171,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
         uint32_t extent = 1;
 #pragma unroll
         for (int j = 0; j < kPerLane; ++j) {  // (its last sequence that begins at or before x)
+          if (j > 0 && per_log == 0) break;
           const int length = __builtin_amdgcn_readlane(keys[j], in), tiles = tiles_of(length);
           const Place next = f.start + (Place)extent * units;
-          if (j == 0 || (next <= x && i + kPerLane * in + j < p.batch)) {
+          if (j == 0 || (next <= x && i + (in << per_log) + j < p.batch)) {
             if (j > 0) f.start = next;
-            f.b = i + kPerLane * in + j;
+            f.b = i + (in << per_log) + j;
             f.length = length;
             f.n_tiles = tiles;
             extent = tiles + kOver;
