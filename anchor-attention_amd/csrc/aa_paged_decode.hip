@@ -17,9 +17,10 @@
 // costs as much as that of the output.  There is one set of registers for a tile; its keys are requested anew as soon as the scores have read them, its values after
 // the last product, so that loads are always in flight.
 //
-// Measured (bf16 unless said): 32 sequences of 500 to 16000 keys, 32/8 heads of 128 111 us, of which 4.8 the join: 5.7 TB/s while it reads, where a copy of that
-// size reaches 5.2 to 5.4; 2 of 131071, 28/4 heads of 128, fp16 101 us, 5.6 TB/s; one of 33001, 32/8 of 128 32.4 us, of which about 4 pass before the first
-// tile has come (lengths, table, rows, one after the other), 1.7 at the end and 4 in the join; one of 300, 14/2 of 64 8 us, nothing but such chains.
+// Measured (bf16 unless said): 32 sequences of 500 to 16000 keys, 32/8 heads of 128 109 us, of which 4.8 the join: 5.7 TB/s while it reads, where a copy of that
+// size reaches 5.2 to 5.4; 2 of 131071, 28/4 heads of 128, fp16 100 us, 5.6 TB/s; one of 33001, 32/8 of 128 31.7 us, of which about 4 pass before the first
+// tile has come (lengths, table, rows, one after the other), 1 at the end and 4 in the join; one of 300, 14/2 of 64 7.2 us, nothing but such chains.  What is
+// executed before the first load counts there: a place is looked for only where it is not in the unit of the one before.
 #include "aa_kernels.h"
 #include "aa_nonfinite.h"
 #include "aa_paged.h"

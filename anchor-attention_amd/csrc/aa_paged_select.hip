@@ -3,12 +3,12 @@
 // A score is defined by a float64 sum, so that the chosen pages do not depend on its order: products of two 16-bit numbers are exact in float32, their
 // sum is formed in float64 and rounded once.  A lane has 8 channels of 4 pages, so a page is 8 or 16 lanes'; their sums are exchanged inside rows of
 // lanes so that each lane ends with one page's.  With many pages conversions and additions in float64 bound it: 16 sequences of 6000 to 60000 keys in pages of 16,
-// 32/8 heads of 64, fp16 16.9 us for 49 MB of bounds, which take 9.4 to read; one sequence of 131072 keys in pages of 64, 32/8 of 128 5.7 us, 8 MB.  (Choosing the head that
+// 32/8 heads of 64, fp16 16.9 us for 49 MB of bounds, which take 9.4 to read; one sequence of 131072 keys in pages of 64, 32/8 of 128 5.8 us, 8 MB.  (Choosing the head that
 // counts by sums in float32 and summing only that one's in float64 where no other is near was slower, 23 and 6.4 us: twice the exchanges between lanes, and a
 // wave nearly always has a page where two heads are near.  So were bounds kept in float64, two products with the positive and the negative part of a query, 21: 200
 // registers leave two waves to a SIMD.)
 //
-// Choosing is latency (6.4 us for 2048 pages of one sequence, 8.3 for up to 3750 of 16; 8.7 with the scores, for 132 pages): a work-group per (sequence,
+// Choosing is latency (6.4 us for 2048 pages of one sequence, 8.3 for up to 3750 of 16; 8.9 with the scores, for 132 pages): a work-group per (sequence,
 // KV head) finds what the wanted number of scores reaches by histograms of 256 equal ranges of the numbers' order, each inside the range of the last one that holds it; the first spans the smallest to the largest score, so that two or three do, whatever the
 // scores' exponents (at most four).  Every wave reads the bins for itself, which leaves one barrier for each histogram.  Integer work: the order in which
 // counts are added does not matter.  The code is kept short, since most of it runs once and its first instructions come from memory.
