@@ -22,10 +22,6 @@ __device__ __forceinline__ uint32_t dpp(const uint32_t x, const uint32_t none = 
   return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)x, CONTROL, ROWS, 0xf, false);
 }
 template <int CONTROL>
-__device__ __forceinline__ float dpp(const float x) {
-  return __uint_as_float(dpp<CONTROL>(__float_as_uint(x)));
-}
-template <int CONTROL>
 __device__ __forceinline__ double dpp(const double x) {
   const uint64_t u = (uint64_t)__double_as_longlong(x);
   return __longlong_as_double((long long)((uint64_t)dpp<CONTROL>((uint32_t)(u >> 32)) << 32 | dpp<CONTROL>((uint32_t)u)));

@@ -62,9 +62,19 @@ __device__ __forceinline__ float max_over_quarters(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
   return max_with_other_half(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
-__device__ __forceinline__ float sum_over_quarters(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+__device__ __forceinline__ float sum_over_quarters(const float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t w = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+  const auto s = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+// f over all lanes of a wave
+template <typename F>
+__device__ __forceinline__ float over_wave(const float x, const float none, F f) {
+  const uint32_t all = up_to(__float_as_uint(x), __float_as_uint(none),
+                             [&](const uint32_t a, const uint32_t b) { return __float_as_uint(f(__uint_as_float(a), __uint_as_float(b))); });
+  return __uint_as_float(__builtin_amdgcn_readlane(all, 63));
 }
 
 // Rows of a page behind a wave-uniform address: a lane's loads then have an offset of 32 bits, and the address is scalar arithmetic.
@@ -562,17 +572,13 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArg
   for (int j = 0; j < 4; ++j) early[j] = *reinterpret_cast<const floatx4*>(p.parts + part(min(gr + j * kGroups, parts - 1)) * D + 4 * d4);
   const float mine = tid < parts ? p.part_stats[2 * part(tid)] : -INFINITY;
   float l = tid < parts ? p.part_stats[2 * part(tid) + 1] : 0.f;
-  float m = mine;
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+  float m = over_wave(mine, -INFINITY, [](const float a, const float b) { return fmaxf(a, b); });
   if (lane == 0) red[0][wave] = m;
   __syncthreads();
   m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   const float w = mine == -INFINITY ? 0.f : fast_exp2((mine - m) * scale);
   weight[tid] = w;
-  l *= w;
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
+  l = over_wave(l * w, 0.f, [](const float a, const float b) { return a + b; });
   if (lane == 0) red[1][wave] = l;
   __syncthreads();
   floatx4 sum = {0.f, 0.f, 0.f, 0.f};

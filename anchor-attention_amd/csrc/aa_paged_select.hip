@@ -105,7 +105,7 @@ struct Products<F16, N> {
 template <typename T, int D, int N>
 struct Scores {
   static constexpr int kLanes = D / 8, kSide = 64 / kLanes, kPages = kSide * N;
-  static_assert(N == 4 || N == 2 || N == 1, "what the exchange is written for");
+  static_assert(N == 4 || N == 1, "what the exchange is written for");
   struct Pages {  // of the pool
     int at[N];
   };
@@ -150,17 +150,15 @@ struct Scores {
       next = query(min(h, group - 1));
       double sum[N] = {};
       products.add(sum, q);
-      // while a lane has several it keeps the half that its bit names and gives the other half away
-      double half[2], s;
-      if (N == 4) {
-        half[0] = (odd ? sum[N / 2] : sum[0]) + dpp<kDppXor1>(odd ? sum[0] : sum[N / 2]);
-        half[1] = (odd ? sum[N - 1] : sum[N > 1 ? 1 : 0]) + dpp<kDppXor1>(odd ? sum[N > 1 ? 1 : 0] : sum[N - 1]);
+      double s;
+      if constexpr (N == 4) {  // twice a lane keeps the half of what it has that a bit of it names, and gives the other away
+        const double a = (odd ? sum[2] : sum[0]) + dpp<kDppXor1>(odd ? sum[0] : sum[2]);
+        const double b = (odd ? sum[3] : sum[1]) + dpp<kDppXor1>(odd ? sum[1] : sum[3]);
+        s = (odd2 ? b : a) + dpp<kDppXor2>(odd2 ? a : b);
       } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) half[i] = sum[i] + dpp<kDppXor1>(sum[i]);
+        s = sum[0] + dpp<kDppXor1>(sum[0]);
+        s += dpp<kDppXor2>(s);
       }
-      if (N > 1) s = (odd2 ? half[1] : half[0]) + dpp<kDppXor2>(odd2 ? half[0] : half[1]);
-      else s = half[0] + dpp<kDppXor2>(half[0]);
       if (kLanes == 8) {
         s += dpp<kDppHalfMirror>(s);
       } else {
@@ -170,7 +168,7 @@ struct Scores {
       nan = nan || s != s;
       best = fmaxf(best, (float)s);
     }
-    if (c < 4 && (N == 4 || !odd) && (N > 1 || !odd2)) store(kSide * ((odd ? 2 : 0) + (odd2 ? 1 : 0)) + lane / kLanes, nan ? INFINITY : best);
+    if (c < (N == 4 ? 4 : 1)) store(kSide * (N == 4 ? (odd ? 2 : 0) + (odd2 ? 1 : 0) : 0) + lane / kLanes, nan ? INFINITY : best);
   }
 };
 
