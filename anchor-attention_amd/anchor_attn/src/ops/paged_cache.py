@@ -21,7 +21,7 @@ import torch
 
 from . import _hip
 from .anchor_attn_v4 import _called_plainly
-from .anchor_step_1_2_v2 import _stream
+from .anchor_step_1_2_v2 import _raw_stream, _stream
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 _TYPES = (torch.Tensor, torch.nn.Parameter)
@@ -112,7 +112,7 @@ class PagedCache:
 
     def _launch(self, fn, packed):
         if self.index == torch.cuda.current_device():
-            rc = fn(self._address, packed, _stream())
+            rc = fn(self._address, packed, _raw_stream(self.index) if _raw_stream is not None else _stream())
         else:
             with torch.cuda.device(self.device):
                 rc = fn(self._address, packed, _stream())
@@ -216,7 +216,7 @@ def paged_decode_attention(cache: PagedCache, q: torch.Tensor, page_table: torch
     if sizes[0]:
         lib = _hip.lib()
         nbytes = lib.aa_paged_decode_workspace_bytes(*sizes, cache.n_kv_heads, cache.head_dim, cache.page_size, most)
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=cache.device) if nbytes else None
+        ws = lengths.new_empty((nbytes >> 2,)) if nbytes else None
         cache._launch(lib.aa_paged_decode_fwd, _hip.PAGED_STEP.pack(*tensors, ws.data_ptr() if nbytes else 0, nbytes, 0, *sizes, most, 0, 0, 0, scale))
     return out
 
@@ -235,11 +235,11 @@ def paged_sparse_decode_attention(cache: PagedCache, q: torch.Tensor, page_table
         _refuse("sparse steps need a cache with bounds")
     if n_first < 0 or n_last < 1 or n_first + n_last > n_pages or n_pages > 1 << 16:
         _refuse(f"{n_pages} pages, the first {n_first} and the last {n_last} among them, are not supported (at most 65536, at least the last one)")
-    pages = torch.empty((sizes[0], cache.n_kv_heads, n_pages), dtype=_INT32, device=cache.device)
+    pages = lengths.new_empty((sizes[0], cache.n_kv_heads, n_pages))
     if sizes[0]:
         lib = _hip.lib()
         nbytes = lib.aa_paged_sparse_workspace_bytes(*sizes, cache.n_kv_heads, cache.head_dim, cache.page_size, most, n_pages)
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=cache.device)
+        ws = lengths.new_empty((nbytes >> 2,))
         cache._launch(lib.aa_paged_sparse_decode_fwd,
                       _hip.PAGED_STEP.pack(*tensors, ws.data_ptr(), nbytes, pages.data_ptr(), *sizes, most, n_pages, n_first, n_last, scale))
     return out, pages
