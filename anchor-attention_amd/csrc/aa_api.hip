@@ -1016,7 +1016,7 @@ static SparseScratch carve_sparse(int batch, int n_kv_heads, int head_dim, int p
   SparseScratch w;
   const size_t units = (size_t)batch * n_kv_heads;
   w.scores = 0;
-  w.chosen = align256(units * max_pages * 4);
+  w.chosen = align256(units * paged_score_pitch(max_pages) * 4);
   w.decode = w.chosen + align256(units * n_chosen * 4);
   w.total = w.decode + paged_decode_scratch(head_dim, log2_of(page_size), std::min(n_chosen, max_pages)).total;
   return w;

@@ -172,12 +172,13 @@ struct PagedScratch {
 PagedScratch paged_decode_scratch(int head_dim, int page_log, int max_pages);
 hipError_t launch_paged_decode(const PagedDecodeArgs& a, hipStream_t stream);
 
+constexpr int paged_score_pitch(int max_pages) { return (max_pages + 3) & ~3; }
 struct PagedSelectArgs {
   const uint16_t* q; int64_t q_sb, q_sh;
   const uint16_t* bounds;
   const int32_t* table; int64_t t_sb;
   const int32_t* lengths;
-  float* scores;    // [batch, n_kv_heads, max_pages]
+  float* scores;    // [batch, n_kv_heads, paged_score_pitch(max_pages)]
   int32_t* pages;   // [batch, n_kv_heads, n_chosen]: places in the sequence
   int32_t* chosen;  // the same, as pages of the pool
   int batch, n_q_heads, n_kv_heads, head_dim, n_pages, page_log, max_pages, n_chosen, n_first, n_last;

@@ -26,7 +26,22 @@ constexpr int kFused = 1024;       // a table of at most that many pages is scor
 // sequence, 64 pages 17.6 us a step by one launch and 19.8 by two, 128 pages 19.7 and 19.6, 256 24.2 and 19.7; 14/2 heads of 64 128 pages 16.6 and 19.0,
 // 192 17.9 and 19.1, 256 20.7 and 19.0.
 constexpr int kFusedProducts = 72 * 1024;
-constexpr int kInLds = 8192;       // the scores of at most that many pages are kept in LDS
+constexpr int kInLds = 32768;      // the scores of at most that many pages are kept in LDS
+// Pages that a thread of the choosing work-group looks at together, side by side: 4, and 1 in tables of at most kOnes pages, where the other threads would have
+// nothing to do.  (One sequence, 32/8 heads of 128, 8192 pages: 1 36.0 us a step, 4 32.3; 1875 pages 21.7 and 21.8, 469 20.5 and 21.5.)
+constexpr int kItem = 4, kOnes = 2048;
+// ITEM numbers from p on
+template <int ITEM, typename X>
+__device__ __forceinline__ void load_item(const X* p, X (&x)[ITEM]) {
+  typedef X four __attribute__((ext_vector_type(4)));
+  if constexpr (ITEM == 4) {
+    const four y = *reinterpret_cast<const four*>(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = y[e];
+  } else {
+    x[0] = *p;
+  }
+}
 constexpr int kMostPages = 1 << 16;
 constexpr int kListed = 1024;      // the chosen pages up to that many pass through LDS
 constexpr int kQueryWords = 4096;  // of LDS for a group's queries; those of more heads are read from memory
@@ -198,7 +213,7 @@ __global__ void __launch_bounds__(256) paged_scores_kernel(const PagedSelectArgs
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (read by the same wave only)
   __builtin_amdgcn_wave_barrier();
   at = S::find(p, b, first + step);
-  float* scores = p.scores + ((int64_t)b * p.n_kv_heads + kvh) * p.max_pages;
+  float* scores = p.scores + ((int64_t)b * p.n_kv_heads + kvh) * paged_score_pitch(p.max_pages);
   for (;;) {
     S::form(p, b, kvh, y, staged[wave], room, [&](const int k, const float x) {
       if (first + k < there) scores[first + k] = x;
@@ -211,23 +226,23 @@ __global__ void __launch_bounds__(256) paged_scores_kernel(const PagedSelectArgs
 }
 
 // FROM: 0 the scores are formed here, 1 they are read once, 2 as often as they are needed (more than LDS is to hold)
-template <typename T, int D, int FROM>
+template <typename T, int D, int FROM, int ITEM>
 __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const PagedSelectArgs p) {
   typedef Scores<T, D, kAbreastFused> S;
-  constexpr int kMostItems = (FROM == 0 ? kFused : FROM == 1 ? kInLds : kMostPages) / kChooseThreads;
-  __shared__ uint32_t kept[FROM == 0 ? kFused : FROM == 1 ? kInLds : 1];
+  constexpr int kMostItems = (FROM == 0 ? kFused : FROM == 2 ? kMostPages : ITEM == 1 ? kOnes : kInLds) / (ITEM * kChooseThreads);
+  extern __shared__ __attribute__((aligned(16))) uint32_t kept[];  // (not where they stay in memory)
   __shared__ uint32_t bins[4][256], ranges[2][kChooseWaves], counts[kMostItems * kChooseWaves], before[kMostItems * kChooseWaves];
   const int kvh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t unit = (int64_t)b * p.n_kv_heads + kvh;
-  const float* scores = p.scores + unit * p.max_pages;
+  const float* scores = p.scores + unit * paged_score_pitch(p.max_pages);
   int32_t* pages = p.pages + unit * p.n_chosen;
   int32_t* chosen = p.chosen + unit * p.n_chosen;
   const int32_t* table = p.table + b * p.t_sb;
   __shared__ __attribute__((aligned(16))) uint32_t staged[FROM == 0 ? kQueryWords : 1];
   __shared__ int list[kListed];
   // (what does not depend on the length is requested before it is known)
-  float early[2] = {0.f, 0.f};
+  float early[2][ITEM] = {};
   typename S::Pages at;
   int room = 0;
   if (FROM == 0) {
@@ -235,7 +250,8 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
     room = stage_queries<T, D>(p, b, kvh, staged, kQueryWords, tid, kChooseThreads);
   } else {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) early[j] = kChooseThreads * j + tid < p.max_pages ? scores[kChooseThreads * j + tid] : 0.f;
+    for (int j = 0; j < 2; ++j)
+      if (ITEM * (kChooseThreads * j + tid) < p.max_pages) load_item(scores + ITEM * (kChooseThreads * j + tid), early[j]);
   }
   const int there = pages_of(clamped_length(p.lengths, b, p.max_pages, p.page_log), p.page_log);
   if (there <= p.n_chosen) {
@@ -258,37 +274,56 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
       if (i < there) y = S::load(p, kvh, S::find(p, b, i));
     }
   }
+  // item j of a thread is ITEM pages from place(j) on
+  const int items = (there + ITEM * kChooseThreads - 1) / (ITEM * kChooseThreads);
+  auto place = [&](const int j) { return ITEM * (kChooseThreads * j + tid); };
   if (FROM == 1) {
-    for (int j = 0; kChooseThreads * j < there; ++j) {
-      const int i = kChooseThreads * j + tid;
-      if (i < there) kept[i] = ordered(j == 0 ? early[0] : j == 1 ? early[1] : scores[i]);
+    for (int j = 0; j < items; ++j) {
+      const int i = place(j);
+      if (i >= there) break;
+      float x[ITEM];
+      if (j > 1) load_item(scores + i, x);
+#pragma unroll
+      for (int e = 0; e < ITEM; ++e) kept[i + e] = ordered(j == 0 ? early[0][e] : j == 1 ? early[1][e] : x[e]);
     }
   }
 #pragma unroll
   for (int i = 0; i < 4 * 256; i += kChooseThreads) bins[0][i + tid] = 0u;
   if (FROM == 0) __syncthreads();
 
-  // item j of a thread is page kChooseThreads * j + tid: a number from 1 on if it is one to choose from, else 0
-  const int items = (there + kChooseThreads - 1) / kChooseThreads;
-  auto place = [&](const int j) { return kChooseThreads * j + tid; };
-  auto each = [&](auto&& f) {  // f(j, number)
+  auto each = [&](auto&& f) {  // f(j, numbers): from 1 on for pages to choose from, else 0
 #pragma nounroll
     for (int j = 0; j < items; ++j) {
       const int i = place(j);
-      uint32_t x = 0u;
-      if (i >= first && i < last) x = FROM < 2 ? kept[i] : ordered(scores[i]);
+      uint32_t x[ITEM] = {};
+      if (i < there) {
+        uint32_t raw[ITEM];
+        if constexpr (FROM < 2) {
+          load_item(kept + i, raw);
+        } else {
+          float y[ITEM];
+          load_item(scores + i, y);
+#pragma unroll
+          for (int e = 0; e < ITEM; ++e) raw[e] = ordered(y[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < ITEM; ++e) x[e] = i + e >= first && i + e < last ? raw[e] : 0u;
+      }
       f(j, x);
     }
   };
-  auto is_end = [&](const int j) { return place(j) < there && (place(j) < first || place(j) >= last); };
+  auto is_end = [&](const int i) { return i < there && (i < first || i >= last); };
 
   uint32_t lo = 0xffffffffu, hi = 0xffffffffu;  // (no number reaches them)
   int wanted = p.n_chosen - p.n_first - p.n_last;
   if (wanted > 0) {
     hi = 0u;
-    each([&](const int j, const uint32_t x) {
-      lo = x ? min(lo, x) : lo;
-      hi = max(hi, x);
+    each([&](const int, const uint32_t (&x)[ITEM]) {
+#pragma unroll
+      for (int e = 0; e < ITEM; ++e) {
+        lo = min(lo, x[e] - 1u);  // (0 becomes the largest)
+        hi = max(hi, x[e]);
+      }
     });
     lo = up_to(lo, 0xffffffffu, [](const uint32_t a, const uint32_t b) { return min(a, b); });
     hi = up_to(hi, 0u, [](const uint32_t a, const uint32_t b) { return max(a, b); });
@@ -304,15 +339,17 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
       lo = min(lo, ranges[0][w]);
       hi = max(hi, ranges[1][w]);
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
+    lo = __builtin_amdgcn_readfirstlane(lo) + 1u;
     hi = __builtin_amdgcn_readfirstlane(hi);
     // The wanted-th largest score lies from lo to hi; all of those above are taken.  A range is 2^32 long at most and the next one a 256th, so four do.
 #pragma nounroll
     for (int round = 0;; ++round) {
       const uint32_t span = hi - lo;
       const int shift = span < 256u ? 0 : 24 - __builtin_clz(span);  // span >> shift < 256
-      each([&](const int j, const uint32_t x) {
-        if (x >= lo && x <= hi) atomicAdd(&bins[round][(x - lo) >> shift], 1u);
+      each([&](const int, const uint32_t (&x)[ITEM]) {
+#pragma unroll
+        for (int e = 0; e < ITEM; ++e)
+          if (x[e] >= lo && x[e] <= hi) atomicAdd(&bins[round][(x[e] - lo) >> shift], 1u);
       });
       __syncthreads();
       const uint4 bin4 = *reinterpret_cast<const uint4*>(&bins[round][4 * lane]);
@@ -338,9 +375,15 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
   }
 
   // Scores above hi are taken, and of those from lo to hi the first `wanted`: counted by item and wave, which is the pages' order.
-  each([&](const int j, const uint32_t x) {
-    const uint32_t equal = __popcll(__ballot(x >= lo && x <= hi)), sure = __popcll(__ballot(x > hi || is_end(j)));
-    if (lane == 0) counts[kChooseWaves * j + wave] = equal << 16 | sure;
+  auto counts_of = [&](const int j, const uint32_t (&x)[ITEM]) {  // of an item, in the upper and the lower half
+    uint32_t packed = 0;
+#pragma unroll
+    for (int e = 0; e < ITEM; ++e) packed += (x[e] >= lo && x[e] <= hi ? 0x10000u : 0u) + (x[e] > hi || is_end(place(j) + e) ? 1u : 0u);
+    return packed;
+  };
+  each([&](const int j, const uint32_t (&x)[ITEM]) {
+    const uint32_t all = sums_up_to(counts_of(j, x));
+    if (lane == 63) counts[kChooseWaves * j + wave] = all;
   });
   __syncthreads();
   uint32_t so_far_equal = 0, so_far_sure = 0;
@@ -352,16 +395,19 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
     so_far_equal += __builtin_amdgcn_readlane(equals, 63);
     so_far_sure += __builtin_amdgcn_readlane(sures, 63);
   }
-  each([&](const int j, const uint32_t x) {
-    const uint32_t packed = before[kChooseWaves * j + wave];
-    const int equal_before = packed >> 16;
-    const uint64_t below = (1ull << lane) - 1, equals = __ballot(x >= lo && x <= hi);
-    const bool mine = x > hi || is_end(j) || (x >= lo && equal_before + __popcll(equals & below) < wanted);
-    const uint64_t takes = __ballot(mine);
-    if (mine) {
-      const int to = (packed & 0xffffu) + min(equal_before, wanted) + __popcll(takes & below);
-      if (to < kListed) list[to] = place(j);
-      else pages[to] = place(j);
+  each([&](const int j, const uint32_t (&x)[ITEM]) {
+    const uint32_t packed = before[kChooseWaves * j + wave], own = counts_of(j, x), in_wave = sums_up_to(own) - own;
+    int equal_before = (packed >> 16) + (in_wave >> 16), sure_before = (packed & 0xffffu) + (in_wave & 0xffffu);
+#pragma unroll
+    for (int e = 0; e < ITEM; ++e) {
+      const bool equal = x[e] >= lo && x[e] <= hi, sure = x[e] > hi || is_end(place(j) + e);
+      if (sure || (equal && equal_before < wanted)) {
+        const int to = sure_before + min(equal_before, wanted);
+        if (to < kListed) list[to] = place(j) + e;
+        else pages[to] = place(j) + e;
+      }
+      equal_before += equal;
+      sure_before += sure;
     }
   });
   __syncthreads();  // (the list is complete: its pages of the pool are read side by side)
@@ -376,7 +422,7 @@ template <typename T, int D>
 static void launch_paged_select_for(const PagedSelectArgs& a, hipStream_t stream) {
   const dim3 units(a.n_kv_heads, a.batch);
   if (a.max_pages <= kFused && (int64_t)a.max_pages * (a.n_q_heads / a.n_kv_heads) * D <= kFusedProducts) {
-    hipLaunchKernelGGL((paged_choose_kernel<T, D, 0>), units, dim3(kChooseThreads), 0, stream, a);
+    hipLaunchKernelGGL((paged_choose_kernel<T, D, 0, 1>), units, dim3(kChooseThreads), 4 * paged_score_pitch(a.max_pages), stream, a);
     return;
   }
   // (some four thousand work-groups, however long the table is and however short the sequences: the step above with 2560 52.8 us, with 1024 57.7)
@@ -384,8 +430,10 @@ static void launch_paged_select_for(const PagedSelectArgs& a, hipStream_t stream
   const int64_t n = (int64_t)fours * a.batch;
   const int side = (int)((4096 + n - 1) / n);
   hipLaunchKernelGGL((paged_scores_kernel<T, D>), dim3(chunks < side ? chunks : side, fours, a.batch), dim3(256), 0, stream, a);
-  if (a.max_pages <= kInLds) hipLaunchKernelGGL((paged_choose_kernel<T, D, 1>), units, dim3(kChooseThreads), 0, stream, a);
-  else hipLaunchKernelGGL((paged_choose_kernel<T, D, 2>), units, dim3(kChooseThreads), 0, stream, a);
+  const size_t lds = 4 * paged_score_pitch(a.max_pages);
+  if (a.max_pages <= kOnes) hipLaunchKernelGGL((paged_choose_kernel<T, D, 1, 1>), units, dim3(kChooseThreads), lds, stream, a);
+  else if (a.max_pages <= kInLds) hipLaunchKernelGGL((paged_choose_kernel<T, D, 1, kItem>), units, dim3(kChooseThreads), lds, stream, a);
+  else hipLaunchKernelGGL((paged_choose_kernel<T, D, 2, kItem>), units, dim3(kChooseThreads), 0, stream, a);
 }
 
 hipError_t launch_paged_select(const PagedSelectArgs& a, hipStream_t stream) {
