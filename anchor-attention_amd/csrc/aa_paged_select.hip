@@ -8,7 +8,7 @@
 // wave nearly always has a page where two heads are near.  So were bounds kept in float64, two products with the positive and the negative part of a query, 21: 200
 // registers leave two waves to a SIMD.)
 //
-// Choosing is latency (6.4 us for 2048 pages of one sequence, 8.3 for up to 3750 of 16; 8.9 with the scores, for 132 pages): a work-group per (sequence,
+// Choosing is latency (6.0 us for 2048 pages of one sequence, 7.5 for 8192, 18 for 25000; 8.6 with the scores, for 132 pages): a work-group per (sequence,
 // KV head) finds what the wanted number of scores reaches by histograms of 256 equal ranges of the numbers' order, each inside the range of the last one that holds it; the first spans the smallest to the largest score, so that two or three do, whatever the
 // scores' exponents (at most four).  Every wave reads the bins for itself, which leaves one barrier for each histogram.  Integer work: the order in which
 // counts are added does not matter.  The code is kept short, since most of it runs once and its first instructions come from memory.
@@ -28,7 +28,7 @@ constexpr int kFused = 1024;       // a table of at most that many pages is scor
 constexpr int kFusedProducts = 72 * 1024;
 constexpr int kInLds = 32768;      // the scores of at most that many pages are kept in LDS
 // Pages that a thread of the choosing work-group looks at together, side by side: 4, and 1 in tables of at most kOnes pages, where the other threads would have
-// nothing to do.  (One sequence, 32/8 heads of 128, 8192 pages: 1 36.0 us a step, 4 32.3; 1875 pages 21.7 and 21.8, 469 20.5 and 21.5.)
+// nothing to do.  (Steps of one sequence, 32/8 heads of 128: 8192 pages one 36.0 us, four 32.0; 1875 pages 21.6 and 21.8, 469 20.5 and 21.5.)
 constexpr int kItem = 4, kOnes = 2048;
 // ITEM numbers from p on
 template <int ITEM, typename X>
@@ -46,7 +46,8 @@ constexpr int kMostPages = 1 << 16;
 constexpr int kListed = 1024;      // the chosen pages up to that many pass through LDS
 constexpr int kQueryWords = 4096;  // of LDS for a group's queries; those of more heads are read from memory
 
-// A score as an unsigned number of the same order, from 1 on; NaN as infinity, -0 as 0.
+// A score as an unsigned number of the same order, from 1 to below kEnd - 1; NaN as infinity, -0 as 0.
+constexpr uint32_t kEnd = 0xffffffffu;  // what stands for pages that are taken in any case; 0 stands for no page
 __device__ __forceinline__ uint32_t ordered(float x) {
   x = x != x ? INFINITY : x + 0.f;
   const uint32_t u = __float_as_uint(x);
@@ -262,13 +263,14 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
     return;
   }
   const int first = p.n_first, last = there - p.n_last;  // the pages to choose from
+  auto number = [&](const int i, const float score) { return i >= there ? 0u : i < first || i >= last ? kEnd : ordered(score); };
   if (FROM == 0) {
     typename S::Bounds y = S::load(p, kvh, at);
     __syncthreads();
 #pragma nounroll
     for (int i = wave * S::kPages; i < there;) {
       S::form(p, b, kvh, y, staged, room, [&](const int k, const float x) {
-        if (i + k < there) kept[i + k] = ordered(x);
+        if (i + k < there) kept[i + k] = number(i + k, x);
       });
       i += kChooseWaves * S::kPages;
       if (i < there) y = S::load(p, kvh, S::find(p, b, i));
@@ -284,45 +286,42 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
       float x[ITEM];
       if (j > 1) load_item(scores + i, x);
 #pragma unroll
-      for (int e = 0; e < ITEM; ++e) kept[i + e] = ordered(j == 0 ? early[0][e] : j == 1 ? early[1][e] : x[e]);
+      for (int e = 0; e < ITEM; ++e) kept[i + e] = number(i + e, j == 0 ? early[0][e] : j == 1 ? early[1][e] : x[e]);
     }
   }
 #pragma unroll
   for (int i = 0; i < 4 * 256; i += kChooseThreads) bins[0][i + tid] = 0u;
   if (FROM == 0) __syncthreads();
 
-  auto each = [&](auto&& f) {  // f(j, numbers): from 1 on for pages to choose from, else 0
+  auto each = [&](auto&& f) {  // f(j, numbers)
 #pragma nounroll
     for (int j = 0; j < items; ++j) {
       const int i = place(j);
       uint32_t x[ITEM] = {};
       if (i < there) {
-        uint32_t raw[ITEM];
         if constexpr (FROM < 2) {
-          load_item(kept + i, raw);
+          load_item(kept + i, x);
         } else {
           float y[ITEM];
           load_item(scores + i, y);
 #pragma unroll
-          for (int e = 0; e < ITEM; ++e) raw[e] = ordered(y[e]);
+          for (int e = 0; e < ITEM; ++e) x[e] = number(i + e, y[e]);
         }
-#pragma unroll
-        for (int e = 0; e < ITEM; ++e) x[e] = i + e >= first && i + e < last ? raw[e] : 0u;
       }
       f(j, x);
     }
   };
-  auto is_end = [&](const int i) { return i < there && (i < first || i >= last); };
 
-  uint32_t lo = 0xffffffffu, hi = 0xffffffffu;  // (no number reaches them)
+  uint32_t lo = kEnd - 1u, hi = kEnd - 1u;  // (no score has them)
   int wanted = p.n_chosen - p.n_first - p.n_last;
   if (wanted > 0) {
+    lo = kEnd;
     hi = 0u;
     each([&](const int, const uint32_t (&x)[ITEM]) {
 #pragma unroll
       for (int e = 0; e < ITEM; ++e) {
-        lo = min(lo, x[e] - 1u);  // (0 becomes the largest)
-        hi = max(hi, x[e]);
+        lo = min(lo, x[e] - 1u);  // (0 becomes the largest, kEnd the one below)
+        hi = max(hi, x[e] + 1u);  // (kEnd becomes 0)
       }
     });
     lo = up_to(lo, 0xffffffffu, [](const uint32_t a, const uint32_t b) { return min(a, b); });
@@ -340,7 +339,7 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
       hi = max(hi, ranges[1][w]);
     }
     lo = __builtin_amdgcn_readfirstlane(lo) + 1u;
-    hi = __builtin_amdgcn_readfirstlane(hi);
+    hi = __builtin_amdgcn_readfirstlane(hi) - 1u;
     // The wanted-th largest score lies from lo to hi; all of those above are taken.  A range is 2^32 long at most and the next one a 256th, so four do.
 #pragma nounroll
     for (int round = 0;; ++round) {
@@ -349,7 +348,7 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
       each([&](const int, const uint32_t (&x)[ITEM]) {
 #pragma unroll
         for (int e = 0; e < ITEM; ++e)
-          if (x[e] >= lo && x[e] <= hi) atomicAdd(&bins[round][(x[e] - lo) >> shift], 1u);
+          if (x[e] - lo <= span) atomicAdd(&bins[round][(x[e] - lo) >> shift], 1u);
       });
       __syncthreads();
       const uint4 bin4 = *reinterpret_cast<const uint4*>(&bins[round][4 * lane]);
@@ -375,14 +374,14 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
   }
 
   // Scores above hi are taken, and of those from lo to hi the first `wanted`: counted by item and wave, which is the pages' order.
-  auto counts_of = [&](const int j, const uint32_t (&x)[ITEM]) {  // of an item, in the upper and the lower half
+  auto counts_of = [&](const uint32_t (&x)[ITEM]) {  // of an item, in the upper and the lower half
     uint32_t packed = 0;
 #pragma unroll
-    for (int e = 0; e < ITEM; ++e) packed += (x[e] >= lo && x[e] <= hi ? 0x10000u : 0u) + (x[e] > hi || is_end(place(j) + e) ? 1u : 0u);
+    for (int e = 0; e < ITEM; ++e) packed += (x[e] - lo <= hi - lo ? 0x10000u : 0u) + (x[e] > hi ? 1u : 0u);
     return packed;
   };
   each([&](const int j, const uint32_t (&x)[ITEM]) {
-    const uint32_t all = sums_up_to(counts_of(j, x));
+    const uint32_t all = sums_up_to(counts_of(x));
     if (lane == 63) counts[kChooseWaves * j + wave] = all;
   });
   __syncthreads();
@@ -396,11 +395,11 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
     so_far_sure += __builtin_amdgcn_readlane(sures, 63);
   }
   each([&](const int j, const uint32_t (&x)[ITEM]) {
-    const uint32_t packed = before[kChooseWaves * j + wave], own = counts_of(j, x), in_wave = sums_up_to(own) - own;
+    const uint32_t packed = before[kChooseWaves * j + wave], own = counts_of(x), in_wave = sums_up_to(own) - own;
     int equal_before = (packed >> 16) + (in_wave >> 16), sure_before = (packed & 0xffffu) + (in_wave & 0xffffu);
 #pragma unroll
     for (int e = 0; e < ITEM; ++e) {
-      const bool equal = x[e] >= lo && x[e] <= hi, sure = x[e] > hi || is_end(place(j) + e);
+      const bool equal = x[e] - lo <= hi - lo, sure = x[e] > hi;
       if (sure || (equal && equal_before < wanted)) {
         const int to = sure_before + min(equal_before, wanted);
         if (to < kListed) list[to] = place(j) + e;
