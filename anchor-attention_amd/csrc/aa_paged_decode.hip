@@ -77,12 +77,13 @@ __device__ __forceinline__ float over_wave(const float x, const float none, F f)
   return __uint_as_float(__builtin_amdgcn_readlane(all, 63));
 }
 
-// Rows of a page behind a wave-uniform address: a lane's loads then have an offset of 32 bits, and the address is scalar arithmetic.
+// Rows of a page behind a wave-uniform address: a lane's loads then have an offset of 32 bits, and the address is scalar arithmetic.  Rows behind the last key are out
+// of range, so that nothing is fetched for them (1000 sequences of 1 to 200 keys, 32/8 heads of 128, 56.7 -> 47.2 us).
 typedef __amdgpu_buffer_rsrc_t Rows;
-__device__ __forceinline__ Rows rows_at(const uint16_t* base, const bool there) {
+__device__ __forceinline__ Rows rows_at(const uint16_t* base, const int bytes) {
   const uint64_t u = (uint64_t)base;
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
-  return __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)hi << 32 | lo), 0, there ? 0x7fffffff : 0, 0x00020000);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)hi << 32 | lo), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
 // Place: an integer that counts the tiles of all units
@@ -251,28 +252,27 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     u32x4 k[2][kKS];
     uint32_t v[8][kVW];
   };
-  // Where a tile lies: the first rows of its two halves.  (16 keys lie in one page; those behind the last page repeat its rows; of a tile
-  // that is not there nothing is read)
+  // Where a tile lies: the first rows of its two halves, and how many rows are read.  (16 keys lie in one page; of a tile that is not there, nothing)
   struct Spot {
     int64_t k[2], v[2];
-    bool there;
+    int rows[2];
   };
   auto spot = [&](const Unit& u, const int t, const bool there) __attribute__((always_inline)) {
     Spot o;
-    o.there = there;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int key = kTile * t + 16 * half, row = key & ((1 << p.page_log) - 1);
       const int64_t page = clamped_page(u.table[min(key >> p.page_log, u.last_page)], p.n_pages);
       o.k[half] = page * p.kp_sp + row * p.kp_sn + u.k_head;
       o.v[half] = page * p.vp_sp + row * p.vp_sn + u.v_head;
+      o.rows[half] = there ? min(max(u.length - key, 0), 16) : 0;
     }
     return o;
   };
   auto load_k = [&](Tile& x, const Spot& o) __attribute__((always_inline)) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const Rows kr = rows_at(p.keys + o.k[half], o.there);
+      const Rows kr = rows_at(p.keys + o.k[half], o.rows[half] * (2 * (int)p.kp_sn));
 #pragma unroll
       for (int s = 0; s < kKS; ++s) x.k[half][s] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_lane + 64 * s, 0, 0);
     }
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
   auto load_v = [&](Tile& x, const Spot& o) __attribute__((always_inline)) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const Rows vr = rows_at(p.values + o.v[half], o.there);
+      const Rows vr = rows_at(p.values + o.v[half], o.rows[half] * (2 * (int)p.vp_sn));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if constexpr (kVW == 4) *reinterpret_cast<u32x4*>(x.v[4 * half + r]) = __builtin_amdgcn_raw_buffer_load_b128(vr, v_lane, 2 * r * (uint32_t)p.vp_sn, 0);
@@ -409,6 +409,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       Unit n;
       n.table = here ? u.table : u2.table;
       n.last_page = here ? u.last_page : u2.last_page;
+      n.length = here ? u.length : u2.length;
       n.k_head = here ? u.k_head : u2.k_head;
       n.v_head = here ? u.v_head : u2.v_head;
       const Spot o = spot(n, here ? t + 1 : 0, here || more);
