@@ -381,6 +381,7 @@ def test_pools_beyond_four_gib(dtype):
     (LENGTHS, 32, 8, 128, 16, 5, 1, 1), (LENGTHS, 28, 4, 64, 16, 8, 0, 3), ([1000, 999, 17], 14, 2, 64, 32, 6, 2, 4), ([1000, 0], 3, 3, 128, 256, 1, 0, 1),
     ([20001], 32, 8, 128, 64, 33, 1, 2), ([60000, 3000], 8, 1, 64, 16, 200, 1, 2), ([2100], 14, 2, 64, 16, 32, 1, 2), ([800] * 40, 4, 2, 64, 16, 9, 1, 1),
     ([5000, 70], 71, 1, 128, 32, 20, 1, 1), ([300, 40], 16, 1, 64, 64, 100, 1, 1), ([1 << 17], 4, 1, 64, 16, 500, 3, 3),
+    ([1 << 19, 9], 2, 1, 64, 16, 300, 1, 1), ([16 * 2048], 4, 2, 64, 16, 70, 1, 2), ([16 * 2049 - 5, 3000], 4, 2, 64, 16, 1500, 0, 2), ([16 * 4099, 16 * 4096], 2, 2, 64, 16, 2000, 7, 5),
 ])
 def test_sparse_decode(lengths, hq, hkv, d, page, n_pages, n_first, n_last, dtype):
     s = _Setup(lengths, hkv, d, page, dtype, hq + n_pages, extra=1)
@@ -723,3 +724,24 @@ def test_scores_of_zero_queries_and_infinite_bounds(there, dtype):
         s.cache.bounds[at, 1, 0, channel], s.cache.bounds[at, 1, 1, channel] = lo, hi
     pages = _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 20, 1, 1)[1]
     assert torch.equal(pages, _chosen(q, s, 20, 1, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,hq,hkv,d,n_pages", [([3000, 40], 34, 2, 128, 20), ([16 * 25000, 7], 2, 1, 64, 300)])
+def test_captured_steps_that_take_much_lds(lengths, hq, hkv, d, n_pages):
+    """Sixteen columns of 128, and the scores of 25000 pages; replayed with other queries and lengths between eager steps."""
+    ops = _ops()
+    s = _Setup(lengths, hkv, d, 16, BF16, 15)
+    q = s.queries(hq)
+    step = lambda: (ops.paged_decode_attention(s.cache, q, s.table, s.lengths), *ops.paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, n_pages))  # noqa: E731
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for shorter in (0, 500, 1000, 0):
+        q.copy_(s.queries(hq))
+        s.lengths[0] = lengths[0] - shorter
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
