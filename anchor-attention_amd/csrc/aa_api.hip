@@ -964,11 +964,11 @@ int aa_paged_append(const aa_paged_cache* cache, const aa_paged_tokens* t, void*
 
 size_t aa_paged_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
   if (check_paged("aa_paged_decode_workspace_bytes", batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages)) return 0;
-  return paged_decode_scratch(head_dim, log2_of(page_size), max_pages).total;
+  return paged_decode_scratch(batch, n_q_heads, n_kv_heads, head_dim, log2_of(page_size), max_pages).total;
 }
 // ... laid out at `workspace`
 static void give_scratch(PagedDecodeArgs& a, char* workspace, int max_pages) {
-  const PagedScratch s = paged_decode_scratch(a.head_dim, a.page_log, max_pages);
+  const PagedScratch s = paged_decode_scratch(a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim, a.page_log, max_pages);
   if (s.total == 0) return;
   a.headers = (int32_t*)(workspace + s.headers);
   a.part_stats = (float*)(workspace + s.stats);
@@ -1003,7 +1003,7 @@ int aa_paged_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* t, voi
   PagedDecodeArgs a;
   int rc;
   if ((rc = check_given(t, who, "step")) || (rc = check_cache(who, cache, t->batch, t->n_q_heads, t->max_pages, t->page_table, t->lengths))) return rc;
-  const size_t needed = paged_decode_scratch(cache->head_dim, log2_of(cache->page_size), t->max_pages).total;
+  const size_t needed = paged_decode_scratch(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, log2_of(cache->page_size), t->max_pages).total;
   if ((rc = paged_decode_args(who, a, cache, t, needed))) return rc;
   give_scratch(a, static_cast<char*>(t->workspace), t->max_pages);
   return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
@@ -1012,19 +1012,19 @@ int aa_paged_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* t, voi
 struct SparseScratch {
   size_t scores, chosen, decode, total;
 };
-static SparseScratch carve_sparse(int batch, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_chosen) {
+static SparseScratch carve_sparse(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_chosen) {
   SparseScratch w;
   const size_t units = (size_t)batch * n_kv_heads;
   w.scores = 0;
   w.chosen = align256(units * paged_score_pitch(max_pages) * 4);
   w.decode = w.chosen + align256(units * n_chosen * 4);
-  w.total = w.decode + paged_decode_scratch(head_dim, log2_of(page_size), std::min(n_chosen, max_pages)).total;
+  w.total = w.decode + paged_decode_scratch(batch, n_q_heads, n_kv_heads, head_dim, log2_of(page_size), std::min(n_chosen, max_pages)).total;
   return w;
 }
 
 size_t aa_paged_sparse_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_chosen) {
   if (n_chosen <= 0 || check_paged("aa_paged_sparse_workspace_bytes", batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages)) return 0;
-  return carve_sparse(batch, n_kv_heads, head_dim, page_size, max_pages, n_chosen).total;
+  return carve_sparse(batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages, n_chosen).total;
 }
 
 int aa_paged_sparse_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* t, void* stream) {
@@ -1040,7 +1040,7 @@ int aa_paged_sparse_decode_fwd(const aa_paged_cache* cache, const aa_paged_step*
   if ((rc = check_cache(who, cache, t->batch, t->n_q_heads, t->max_pages, t->page_table, t->lengths)) || (rc = check_ptr(cache->bounds, who, "bounds")) ||
       (rc = check_words(t->pages, who, "pages")))
     return rc;
-  const SparseScratch w = carve_sparse(t->batch, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages, t->n_chosen);
+  const SparseScratch w = carve_sparse(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages, t->n_chosen);
   if ((rc = paged_decode_args(who, a, cache, t, w.total))) return rc;
   char* ws = static_cast<char*>(t->workspace);
   const PagedSelectArgs s = {a.q, a.q_sb, a.q_sh, (const uint16_t*)cache->bounds, t->page_table, t->pt_sb, t->lengths, (float*)(ws + w.scores), t->pages,

@@ -169,7 +169,7 @@ struct PagedDecodeArgs {
 struct PagedScratch {
   size_t headers, stats, parts, total;  // offsets in bytes
 };
-PagedScratch paged_decode_scratch(int head_dim, int page_log, int max_pages);
+PagedScratch paged_decode_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_log, int max_pages);
 hipError_t launch_paged_decode(const PagedDecodeArgs& a, hipStream_t stream);
 
 constexpr int paged_score_pitch(int max_pages) { return (max_pages + 3) & ~3; }

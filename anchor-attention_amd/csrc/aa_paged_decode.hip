@@ -35,9 +35,13 @@ constexpr int kTile = 32;       // keys of a tile
 // What a unit costs beside its tiles, in tiles.  (128 sequences of 20 to 1200 keys, 32/8 heads of 64: 0 30.1 us, 3 24.6, 6 24.9; 32 of 500 to 16000, 32/8 of 128:
 // 114, 110.8, 112.2.)
 constexpr int kOver = 3;
-// Where the table has room for that many tiles of a sequence at most, units are not cut between work-groups and nothing is joined: one of 300 keys, 14/2 heads of
-// 64, 10.3 us; with a limit of 8, cut and joined, 14.9.
-constexpr int kWhole = 20;
+// Where the table has room for that many tiles of a sequence at most, units are not cut between work-groups and nothing is joined.  (One sequence, cut and joined or not:
+// 300 keys, 14/2 heads of 64, 14.9 and 10.3 us, 1500 keys 13.6 and 12.4, 1780 13.4 and 13.8; 760 keys, 32/8 of 128, 13.8 and 11.8, 890 14.1 and 12.8, 1200 14.1 and 15.9;
+// 32 of 200 to 890 18.1 and 15.7.)  Many units keep all work-groups busy for longer than a join takes, and uncut ones of different lengths do so less evenly: 128
+// sequences of 1 to 1500 keys, 32/8 of 64, 19.3 and 21.0, of 1 to 890, 32/8 of 128, 20.8 and 21.9.
+template <int D> constexpr int kWhole = 28;
+template <> constexpr int kWhole<64> = 48;
+constexpr int kMany = 768, kWholeMany = 20;  // units, and what holds for more
 // Work-groups, one to a CU.  (512: 32 sequences of 500 to 16000 keys, 32/8 heads of 128 112 us instead of 110, 128 of 20 to 1200, 32/8 of 64 23.8 instead of 22.9.)
 constexpr int kShares = 256;
 constexpr int kSharesLog = 8;
@@ -612,9 +616,11 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArg
 }
 
 // Scratch of a step: a header, and two parts of 16 columns, for each share.  None where no unit is cut.
-PagedScratch paged_decode_scratch(int head_dim, int page_log, int max_pages) {
+PagedScratch paged_decode_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_log, int max_pages) {
   PagedScratch s = {0, 0, 0, 0};
-  if (max_pages << page_log <= kWhole * kTile) return s;
+  const int64_t units = (int64_t)batch * n_kv_heads * ((n_q_heads / n_kv_heads + kCols - 1) / kCols);
+  const int whole = units > kMany ? kWholeMany : head_dim == 64 ? kWhole<64> : kWhole<128>;
+  if (max_pages << page_log <= whole * kTile) return s;
   s.stats = (size_t)kShares * 16;
   s.parts = s.stats + (size_t)kShares * 2 * kCols * 8;
   s.total = s.parts + (size_t)kShares * 2 * kCols * head_dim * 4;
