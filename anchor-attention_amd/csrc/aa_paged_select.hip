@@ -8,10 +8,11 @@
 // wave nearly always has a page where two heads are near.  So were bounds kept in float64, two products with the positive and the negative part of a query, 21: 200
 // registers leave two waves to a SIMD.)
 //
-// Choosing is latency (6.0 us for 2048 pages of one sequence, 7.5 for 8192, 18 for 25000; 8.6 with the scores, for 132 pages): a work-group per (sequence,
-// KV head) finds what the wanted number of scores reaches by histograms of 256 equal ranges of the numbers' order, each inside the range of the last one that holds it; the first spans the smallest to the largest score, so that two or three do, whatever the
-// scores' exponents (at most four).  Every wave reads the bins for itself, which leaves one barrier for each histogram.  Integer work: the order in which
-// counts are added does not matter.  The code is kept short, since most of it runs once and its first instructions come from memory.
+// Choosing is latency (6.0 us for 2048 pages of one sequence, 7.5 for 8192, 18 for 25000; 8.4 with the scores, for 132 pages): a work-group per (sequence, KV head)
+// finds what the wanted number of scores reaches by histograms of 256 equal ranges of the numbers' order, each inside the range of the last one that holds it; the
+// first spans the smallest to the largest score, so that two or three do, whatever the scores' exponents (at most four).  Every wave reads the bins for itself,
+// which leaves one barrier for each histogram.  Integer work: the order in which counts are added does not matter.  The code is kept short, since most of it runs
+// once and its first instructions come from memory.
 #include "aa_kernels.h"
 #include "aa_paged.h"
 
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(256) paged_scores_kernel(const PagedSelectArgs
   }
 }
 
-// FROM: 0 the scores are formed here, 1 they are read once, 2 as often as they are needed (more than LDS is to hold)
+// FROM: 0 the scores are formed here, 1 they are read once, 2 as often as they are needed (more than LDS is to hold).  ITEM: pages of a thread, side by side
 template <typename T, int D, int FROM, int ITEM>
 __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const PagedSelectArgs p) {
   typedef Scores<T, D, kAbreastFused> S;
