@@ -138,7 +138,8 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
     the inputs).
 
     ``q`` ``[tokens, query heads, D]``, ``k``, ``v`` ``[tokens, KV heads, D]``: the tokens of all sequences one after the other; sequence ``b`` has
-    tokens ``starts[b]`` to ``starts[b + 1]`` (``[batch + 1]``; None: one token each).  ``lengths`` ``[batch]`` counts a sequence's keys
+    tokens ``starts[b]`` to ``starts[b + 1]`` (``[batch + 1]``, ascending; the first may lie below 0 and the last behind the
+    tokens that are given; None: one token each).  ``lengths`` ``[batch]`` counts a sequence's keys
     **with** its new ones, which are its last; a token's place in the sequence is its position.  ``cos``, ``sin`` float32 ``[positions, D / 2]`` are the angles of all
     positions: channels ``d`` and ``d + D / 2`` are turned by the angle of ``d``, in float32 with one rounding.  Without them (and without
     queries) keys are stored as they are: those of a prompt that the model has rotated itself.

@@ -223,7 +223,8 @@ __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const 
     if (t >= begin && t < end) n = x.position < 0 ? (int)min(-x.position, (int64_t)(end - t)) : min(min(end, p.n_tokens) - t, page_size - ((int)x.position & (page_size - 1)));
     const int t0 = t;
     t += n;
-    if (!x.ok || (t0 != begin && x.slot != 0)) continue;  // (nowhere; the rest of a run that began among the tokens before)
+    // (nowhere; the rest of a run that began among the tokens before, of which there are none before token 0, wherever the sequence begins)
+    if (!x.ok || (t0 != max(begin, 0) && x.slot != 0)) continue;
     if (p.cos != nullptr) n = (int)min((int64_t)n, p.n_positions - x.position);
 
     uint16_t* bounds = p.bounds + ((int64_t)x.at * p.n_kv_heads + kvh) * 2 * D + 8 * c;

@@ -274,6 +274,7 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
  * q must be NULL and n_q_heads 0.  A page's bounds are set by its first key and widened by the others; those of
  * keys that were taken back (a smaller length) stay until the page's first key is stored again.  A token that has no place - behind the last
  * sequence, at a position below 0, in no row of cos and sin, behind the table or in no page of the pool - is left out: nothing is written for it.
+ * starts[0] may lie below 0 and starts[batch] behind n_tokens: the tokens from 0 to n_tokens - 1 are appended, each where it belongs.
  * q, k, v, q_out: [n_tokens, heads, head_dim] with strides of token and head (_st, _sh).  Two tokens for one place, or of two sequences for one page, give one or a
  * mixture of both.
  *

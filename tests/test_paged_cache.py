@@ -745,3 +745,29 @@ def test_captured_steps_that_take_much_lds(lengths, hq, hkv, d, n_pages):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+# ---- the edges of what may be given ------------------------------------------------------------------------------------
+
+def _same(x, y):
+    """Equal, infinities among them, and NaN in the same places."""
+    return torch.equal(x.isnan(), y.isnan()) and torch.equal(x.masked_fill(x.isnan(), 9.0), y.masked_fill(y.isnan(), 9.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("before,new,hkv,d,page,missing", [([3, 16], [5, 4], 2, 64, 16, 3), ([7, 0], [70, 9], 1, 128, 32, 1), ([200], [3], 2, 128, 256, 40), ([5, 1], [300, 0], 3, 64, 64, 2000)])
+def test_starts_before_the_first_token(before, new, hkv, d, page, missing, dtype):
+    """The rows of a larger batch from its `missing`-th token on: tokens 0 onwards have the same places as if the first sequence began with them, keys and bounds as well as
+    queries and values."""
+    ops, results = _ops(), []
+    for first in (0, -missing):
+        s = _Setup(before, hkv, d, page, dtype, 41, room=max(new))
+        q, k, v = (torch.randn(sum(new), h, d, generator=s.g, device="cuda").to(dtype) for h in (2 * hkv, hkv, hkv))
+        starts = torch.tensor([first, *(sum(new[:b + 1]) for b in range(len(new)))], dtype=torch.int32, device="cuda")
+        lengths = torch.tensor([a + b for a, b in zip(before, new)], dtype=torch.int32, device="cuda")
+        out = ops.append_to_pages(s.cache, q, k, v, *_tables(max(before) + max(new), d), s.table, lengths, starts, out=torch.full_like(q, 7.0))
+        results.append((out, s.cache.keys, s.cache.values, s.cache.bounds))
+    assert all(_same(a, b) for a, b in zip(*results))
+    # (and they are stored: a key of every new token)
+    assert int((~results[1][1].isnan()).sum()) == (sum(before) + sum(new)) * hkv * d
