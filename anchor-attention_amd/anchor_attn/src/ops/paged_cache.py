@@ -228,7 +228,7 @@ def paged_sparse_decode_attention(cache: PagedCache, q: torch.Tensor, page_table
     """:func:`paged_decode_attention` over ``n_pages`` pages of each sequence and KV head (all where there are no more): the first ``n_first``, the last
     ``n_last`` and, of those between, the ones whose score is largest, the lower page first among equals.  The score of a page is the largest
     over the heads of the group of ``sum_d max over the page's bounds of q_d * x_d``: no key of the page has a larger product with the query.
-    It is summed in float64 and rounded to float32; NaN counts as infinity.  Returns the output and the chosen pages, int32 ``[batch, KV heads,
+    The products are exact, summed in float64 (in any order) and rounded to float32; NaN counts as infinity.  Returns the output and the chosen pages, int32 ``[batch, KV heads,
     n_pages]``: places in the sequence's row of the table, ascending, then -1.  The cache needs ``bounds``."""
     out, tensors, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
     n_pages, n_first, n_last = int(n_pages), int(n_first), int(n_last)

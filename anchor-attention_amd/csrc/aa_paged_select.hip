@@ -1,7 +1,7 @@
 // Which pages of a cache a sparse decode step reads, on gfx950: the scores of the pages' bounds and the largest of them.
 //
-// A score is defined by a float64 sum, so that the chosen pages do not depend on its order: products of two 16-bit numbers are exact in float32, their
-// sum is formed in float64 and rounded once.  A lane has 8 channels of 4 pages, so a page is 8 or 16 lanes'; their sums are exchanged inside rows of
+// A score is defined by a float64 sum, so that the chosen pages do not depend on its order: products of two 16-bit numbers are exact (in float32 those of fp16, in
+// float64 those of bf16), their sum is formed in float64 and rounded once.  A lane has 8 channels of 4 pages, so a page is 8 or 16 lanes'; their sums are exchanged inside rows of
 // lanes so that each lane ends with one page's.  With many pages conversions and additions in float64 bound it: 16 sequences of 6000 to 60000 keys in pages of 16,
 // 32/8 heads of 64, fp16 16.9 us for 49 MB of bounds, which take 9.4 to read; one sequence of 131072 keys in pages of 64, 32/8 of 128 5.8 us, 8 MB.  (Choosing the head that
 // counts by sums in float32 and summing only that one's in float64 where no other is near was slower, 23 and 6.4 us: twice the exchanges between lanes, and a
@@ -13,6 +13,8 @@
 // first spans the smallest to the largest score, so that two or three do, whatever the scores' exponents (at most four).  Every wave reads the bins for itself,
 // which leaves one barrier for each histogram.  Integer work: the order in which counts are added does not matter.  The code is kept short, since most of it runs
 // once and its first instructions come from memory.
+#include <type_traits>
+
 #include "aa_kernels.h"
 #include "aa_paged.h"
 
@@ -57,16 +59,26 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// Bounds of 8 channels of N pages, and sums of their products with queries: exact products in float32, sums in float64.
+// Bounds of 8 channels of N pages, and sums of their products with queries, both in float64: bf16 has the exponents of float32, so that a product of two may lie
+// beyond 2^128, or below 2^-126, and the sum still be a float32.  In float64 it is exact, and part of the addition.
 template <typename T, int N>
 struct Products {
-  float bounds[N][2][8];
+  typedef typename std::conditional<N == 1, double, float>::type Bound;  // (converted once where there is one page, with the queries where several share them)
+  Bound bounds[N][2][8];
   static __device__ __forceinline__ u32x4 query(const u32x4 q) { return q; }  // as it is staged
   __device__ __forceinline__ explicit Products(const u32x4 (&raw)[N][2]) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int w = 0; w < 2; ++w) unpack8<T>(*reinterpret_cast<const uint4*>(&raw[i][w]), bounds[i][w]);
+      for (int w = 0; w < 2; ++w) {
+        float x[8];
+        unpack8<T>(*reinterpret_cast<const uint4*>(&raw[i][w]), x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          bounds[i][w][j] = x[j];
+          if constexpr (N == 1) asm("" : "+v"(bounds[i][w][j]));  // (here and not once more for every head)
+        }
+      }
   }
   __device__ __forceinline__ void add(double (&sum)[N], const u32x4 raw) const {
     float q[8];
@@ -74,12 +86,13 @@ struct Products {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const bool larger = q[j] >= 0.f;
+      const double x = q[j];
 #pragma unroll
-      for (int i = 0; i < N; ++i) sum[i] += (double)(q[j] * (larger ? bounds[i][1][j] : bounds[i][0][j]));
+      for (int i = 0; i < N; ++i) sum[i] = __builtin_fma(x, (double)(larger ? bounds[i][1][j] : bounds[i][0][j]), sum[i]);
     }
   }
 };
-// fp16 has an instruction that multiplies two of them into a float32, and two bounds are chosen at once by their queries' signs, for which -0 becomes 0
+// A product of two fp16 numbers is exact in float32; an instruction multiplies two of them into one, and two bounds are chosen at once by their queries' signs, for which -0 becomes 0
 // (16 sequences of 6000 to 60000 keys in pages of 16: 16.9 us, with conversions as in bf16 18.5).
 template <int N>
 struct Products<F16, N> {

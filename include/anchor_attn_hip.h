@@ -284,8 +284,8 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
  *
  * aa_paged_sparse_decode_fwd: the same over n_chosen pages for each sequence and KV head, or all where the sequence has no more: its first n_first, its last
  * n_last (at least 1) and those of the others whose score is largest, the lower page first among equal ones.  The score is the largest over the heads of the
- * group of sum_d q_d * (q_d >= 0 ? largest_d : smallest_d), which no product of the query with a key of the page exceeds: a sum in float64, rounded to
- * float32; NaN counts as infinity.  pages int32 [batch, n_kv_heads, n_chosen], contiguous: the chosen ones (places in the sequence), ascending, then -1. */
+ * group of sum_d q_d * (q_d >= 0 ? largest_d : smallest_d), which no product of the query with a key of the page exceeds: exact products, a sum in float64
+ * (in any order), rounded to float32; NaN counts as infinity.  pages int32 [batch, n_kv_heads, n_chosen], contiguous: the chosen ones (places in the sequence), ascending, then -1. */
 typedef struct {
   void* keys;
   int64_t kp_sp, kp_sh, kp_sn;

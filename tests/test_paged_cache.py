@@ -771,3 +771,30 @@ def test_starts_before_the_first_token(before, new, hkv, d, page, missing, dtype
     assert all(_same(a, b) for a, b in zip(*results))
     # (and they are stored: a key of every new token)
     assert int((~results[1][1].isnan()).sum()) == (sum(before) + sum(new)) * hkv * d
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size,scale", [(1e30, 1e9), (1e19, 1e19), (2e37, 5.0), (3e38, 1e38), (1e-25, 1e-19), (1e-30, 1e-10), (1e-38, 1e-38), (1e-20, 1e-19)])
+@pytest.mark.parametrize("there,d", [(60, 64), (700, 64), (400, 128)])
+def test_scores_whose_products_leave_float32(there, d, size, scale):
+    """bf16 products beyond 2^128 or below 2^-126: the score is their float64 sum, rounded to float32 (often an infinity of its sign, or 0)."""
+    s = _Setup([16 * there], 2, d, 16, BF16, there + d)
+    s.cache.bounds.copy_((torch.randn(s.cache.bounds.shape, generator=s.g, device="cuda").double() * size).clamp(-3e38, 3e38).to(BF16))
+    s.cache.bounds[::5] *= 0.03125
+    q = (s.queries(6, 1.0).double() * scale).clamp(-3e38, 3e38).to(BF16)
+    for n in (3, 20, 50):
+        assert torch.equal(_ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, n, 1, 1)[1], _chosen(q, s, n, 1, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("there", [60, 3000])
+def test_a_score_whose_large_products_cancel(there):
+    """(2^64, 2^64, 1) . (2^64, -2^64, x) is x: what two large products leave is known, not infinite."""
+    s = _Setup([16 * there], 1, 64, 16, BF16, there)
+    q = torch.zeros(1, 3, 64, dtype=BF16, device="cuda")
+    q[..., :2], q[..., 2] = 2.0 ** 64, 1.0
+    s.cache.bounds.zero_()
+    s.cache.bounds[..., 0], s.cache.bounds[..., 1] = 2.0 ** 64, -2.0 ** 64
+    s.cache.bounds[:, :, :, 2] = torch.randn(s.cache.n_pages, 1, 2, generator=s.g, device="cuda").to(BF16)
+    s.cache.bounds[::2, :, :, :2] = 0
+    assert torch.equal(_ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 20, 1, 1)[1], _chosen(q, s, 20, 1, 1))
