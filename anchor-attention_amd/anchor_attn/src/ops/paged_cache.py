@@ -212,7 +212,7 @@ def _decode_args(cache, q, page_table, lengths, sm_scale, out):
 def paged_decode_attention(cache: PagedCache, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, sm_scale: Optional[float] = None,
                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one new token per sequence, ``q`` ``[batch, query heads, D]``, over the first ``lengths[b]`` keys of each: ``softmax(q K^T
-    sm_scale) V``, zeros for a sequence of none.  ``sm_scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``."""
+    sm_scale) V``, zeros for a sequence of none (NaN for one whose scores are all minus infinity).  ``sm_scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``."""
     out, tensors, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
     if sizes[0]:
         lib = _hip.lib()

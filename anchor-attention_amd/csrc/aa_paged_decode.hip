@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
 
     const bool from_start = f.tile == 0, to_end = last == f.n_tiles;
     if (from_start && to_end) {
-      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+      const float inv = length == 0 ? 0.f : 1.f / l_run;  // (no keys: 0; keys whose scores are all minus infinity: 0 / 0, as a soft-max has it)
       if (c16 < n_cols) {
         uint16_t* op = p.out + f.b * p.o_sb + (int64_t)(head0 + c16) * p.o_sh + kDV * 4 * g;
 #pragma unroll
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
         for (int e = 0; e < 4; ++e) x[e] += weight * xs[w][e];
       }
       if (begins && ends) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = 1.f / l;  // (a unit that is cut has keys)
         uint16_t* op = p.out + info.y * p.o_sb + (int64_t)(head0 + col) * p.o_sh + d;
         *reinterpret_cast<u32x2*>(op) = u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
       } else {
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArg
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[e] += sums[i][tid][e];
     l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = 1.f / l;
     uint16_t* op = p.out + header.y * p.o_sb + (int64_t)(header.z + col) * p.o_sh + 4 * tid;
     *reinterpret_cast<u32x2*>(op) = u32x2{T::pack(sum[0] * inv, sum[1] * inv), T::pack(sum[2] * inv, sum[3] * inv)};
   }

@@ -278,7 +278,8 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
  * q, k, v, q_out: [n_tokens, heads, head_dim] with strides of token and head (_st, _sh).  Two tokens for one place, or of two sequences for one page, give one or a
  * mixture of both.
  *
- * aa_paged_decode_fwd: out[b, h] = softmax(q[b, h] . keys * sm_scale) values over the keys 0 .. lengths[b] - 1 of sequence b; a sequence of none gives 0.
+ * aa_paged_decode_fwd: out[b, h] = softmax(q[b, h] . keys * sm_scale) values over the keys 0 .. lengths[b] - 1 of sequence b; a sequence of none gives 0,
+ * one whose scores are all minus infinity NaN, as the quotient has it.
  * q, out: [batch, n_q_heads, head_dim] with strides of sequence and head.  workspace: aa_paged_decode_workspace_bytes() bytes of device scratch, which
  * may be none (contents undefined afterwards).
  *

@@ -798,3 +798,30 @@ def test_a_score_whose_large_products_cancel(there):
     s.cache.bounds[:, :, :, 2] = torch.randn(s.cache.n_pages, 1, 2, generator=s.g, device="cuda").to(BF16)
     s.cache.bounds[::2, :, :, :2] = 0
     assert torch.equal(_ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 20, 1, 1)[1], _chosen(q, s, 20, 1, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lengths,d", [([1, 40, 0, 17], 64), ([700, 5000, 33, 0], 128), ([20001, 3], 64)])
+def test_decode_where_every_score_is_minus_infinity(lengths, d, dtype):
+    """The soft-max of such scores is NaN (0 / 0), in one tile, in several and where a unit's parts are joined; other heads stay as they are, and a sequence of no keys
+    gives zeros."""
+    s = _Setup(lengths, 2, d, 16, dtype, 17)
+    q = s.queries(4, 0.5)
+    q[:, :, 0] = 1.0
+    want = [_ops().paged_decode_attention(s.cache, q, s.table, s.lengths), _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 40)[0]]
+    s.cache.keys[:, 0, :, 0] = float("-inf")
+    s.cache.bounds[:, 0, :, 0] = float("-inf")
+    got = [_ops().paged_decode_attention(s.cache, q, s.table, s.lengths), _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 40)[0]]
+    for x, y in zip(got, want):
+        for b, n in enumerate(lengths):
+            assert bool(x[b, :2].isnan().all()) if n else bool((x[b] == 0).all())
+        assert torch.equal(x[:, 2:], y[:, 2:])
+    # one key that is seen is enough
+    for b, n in enumerate(lengths):
+        if n:
+            s.cache.keys[s.table[b, (n - 1) // 16].long(), 0, (n - 1) % 16, 0] = 0.0
+    got = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
+    for b, n in enumerate(lengths):
+        if n:
+            assert torch.equal(got[b, :2], s.cache.values[s.table[b, (n - 1) // 16].long(), 0, (n - 1) % 16].expand(2, d))
