@@ -199,9 +199,9 @@ def _decode_args(cache, q, page_table, lengths, sm_scale, out):
     tables, batch, most = cache._tables(page_table, lengths)
     if shape[0] != batch:
         _refuse(f"q has {shape[0]} tokens, the table {batch} sequences: a decode step has one of each")
-    scale = float(sm_scale) if sm_scale else cache.head_dim ** -0.5
+    scale = cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale)
     if not 1e-30 < scale < 1e30:
-        _refuse(f"sm_scale must be positive and finite, not {sm_scale}")
+        _refuse(f"sm_scale must be positive, from 1e-30 to 1e30, not {sm_scale}")
     if out is not None:
         out_rows = _out_rows(out, shape, cache)
     else:

@@ -825,3 +825,16 @@ def test_decode_where_every_score_is_minus_infinity(lengths, d, dtype):
     for b, n in enumerate(lengths):
         if n:
             assert torch.equal(got[b, :2], s.cache.values[s.table[b, (n - 1) // 16].long(), 0, (n - 1) % 16].expand(2, d))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, 0, False, -0.0, float("nan"), 1e31])
+def test_a_scale_that_is_given_is_not_the_default(scale):
+    from anchor_attn.src.ops import _hip
+    s = _Setup([40], 2, 64, 16, BF16, 18)
+    q = s.queries(4)
+    with pytest.raises(_hip.AnchorAttnHipError, match="sm_scale must be positive"):
+        _ops().paged_decode_attention(s.cache, q, s.table, s.lengths, sm_scale=scale)
+    with pytest.raises(_hip.AnchorAttnHipError, match="sm_scale must be positive"):
+        _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 2, sm_scale=scale)
+    assert torch.equal(_ops().paged_decode_attention(s.cache, q, s.table, s.lengths, sm_scale=None), _ops().paged_decode_attention(s.cache, q, s.table, s.lengths, sm_scale=0.125))
