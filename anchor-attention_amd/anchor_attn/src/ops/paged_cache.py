@@ -61,9 +61,11 @@ class PagedCache:
     16-byte boundaries, the other strides free) and, for sparse steps, ``bounds`` ``[n_pages, n_kv_heads, 2, head_dim]`` (contiguous): the
     smallest and the largest value of each channel over a page's keys, which :func:`append_to_pages` sets with a page's first key and widens with the
     others (keys that are taken back by a smaller length stay in them until the first is stored again; whoever copies pages copies their bounds).  The contents of pages that no table names
-    do not matter.  The tensors stay the cache's own for as long as it is used: their contents may change, their memory may not, and a cache gets no others."""
+    do not matter.  The tensors stay the cache's own for as long as it is used: their contents may change, their memory may not, and a cache gets no others.  After
+    ``cache.keys.data = ...`` or a ``resize_`` that moves them calls are refused."""
 
-    __slots__ = ("keys", "values", "bounds", "dtype", "device", "index", "n_pages", "n_kv_heads", "page_size", "head_dim", "_struct", "_address")
+    __slots__ = ("keys", "values", "bounds", "dtype", "device", "index", "n_pages", "n_kv_heads", "page_size", "head_dim", "_struct", "_address",
+                 "_addresses", "_pointers", "_memory")
 
     def __init__(self, keys: torch.Tensor, values: torch.Tensor, bounds: Optional[torch.Tensor] = None):
         tensors = (keys, values) if bounds is None else (keys, values, bounds)
@@ -84,8 +86,11 @@ class PagedCache:
         # (what the C interface is told of the cache, once: 13 arguments fewer in each call)
         struct = _hip.PagedCacheStruct(*_hip.t3(keys), *_hip.t3(values), None if bounds is None else bounds.data_ptr(), n_pages, kv_heads, page_size, d,
                                        _hip.dtype_code(keys))
+        addresses = (keys.data_ptr, values.data_ptr, int if bounds is None else bounds.data_ptr)
         for name, value in zip(self.__slots__, (keys, values, bounds, keys.dtype, keys.device, keys.get_device(), n_pages, kv_heads, page_size, d, struct,
-                                                ctypes.addressof(struct))):
+                                                ctypes.addressof(struct), addresses, tuple(f() for f in addresses),
+                                                # (what the struct points to lives as long as the cache, also if a tensor is given other memory)
+                                                tuple(t.detach() for t in tensors))):
             object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value):
@@ -111,6 +116,9 @@ class PagedCache:
         return (table, page_table.stride(0), lengths_ptr), batch, most
 
     def _launch(self, fn, packed):
+        keys, values, bounds = self._addresses
+        if (keys(), values(), bounds()) != self._pointers:
+            _refuse("a tensor of the cache has been given other memory, which a PagedCache does not follow: make a new one")
         if self.index == torch.cuda.current_device():
             rc = fn(self._address, packed, _raw_stream(self.index) if _raw_stream is not None else _stream())
         else:

@@ -838,3 +838,39 @@ def test_a_scale_that_is_given_is_not_the_default(scale):
     with pytest.raises(_hip.AnchorAttnHipError, match="sm_scale must be positive"):
         _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 2, sm_scale=scale)
     assert torch.equal(_ops().paged_decode_attention(s.cache, q, s.table, s.lengths, sm_scale=None), _ops().paged_decode_attention(s.cache, q, s.table, s.lengths, sm_scale=0.125))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["keys", "values", "bounds"])
+def test_a_cache_whose_tensors_get_other_memory_is_refused(name):
+    """... before anything is launched: its address is the old one's."""
+    from anchor_attn.src.ops import _hip
+    ops = _ops()
+    s = _Setup([40, 3], 2, 64, 16, BF16, 19, room=20)
+    q, k, v = (torch.randn(2, h, 64, generator=s.g, device="cuda").to(BF16) for h in (4, 2, 2))
+    cos, sin = _tables(100, 64)
+    calls = [lambda: ops.paged_decode_attention(s.cache, q, s.table, s.lengths), lambda: ops.paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 2)[0],
+             lambda: ops.append_to_pages(s.cache, q, k, v, cos, sin, s.table, s.lengths)]
+    calls[2]()  # (the same once more changes nothing)
+    want = [call().clone() for call in calls]
+    tensor = getattr(s.cache, name)
+    old, kept = tensor.data, [x.clone() for x in (s.cache.keys, s.cache.values, s.cache.bounds)]
+    for other in (torch.zeros_like(old), torch.zeros_like(old[:1])):
+        tensor.data = other
+        for call in calls:
+            with pytest.raises(_hip.AnchorAttnHipError, match="other memory"):
+                call()
+    tensor.data = old
+    # a resize_ that moves it (to a tensor of its own first, so that the others' memory is not one with it)
+    moved = [x.clone() for x in (s.cache.keys, s.cache.values, s.cache.bounds)]
+    cache = ops.PagedCache(*moved)
+    getattr(cache, name).resize_(4096, *old.shape[1:])
+    with pytest.raises(_hip.AnchorAttnHipError, match="other memory"):
+        ops.paged_decode_attention(cache, q, s.table, s.lengths)
+    torch.cuda.synchronize()
+    # the cache itself is as it was, and its contents may change
+    assert all(_same(x, y) for x, y in zip((s.cache.keys, s.cache.values, s.cache.bounds), kept))
+    for call, x in zip(calls, want):
+        assert torch.equal(call(), x)
+    s.cache.values.copy_(2 * s.cache.values)
+    assert torch.equal(calls[0](), 2 * want[0])
