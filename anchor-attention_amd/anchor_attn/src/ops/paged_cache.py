@@ -56,9 +56,34 @@ def _indices(t, name, cache, dim, rows=None):
     return t.data_ptr()
 
 
+def _dims(t):
+    """``(stride, size)`` of a tensor's dimensions of more than one entry, the largest stride first."""
+    return sorted(((s, n) for s, n in zip(t.stride(), t.shape) if n > 1), reverse=True)
+
+
+def _extent(dims):
+    """Elements from a tensor's first to its last."""
+    return 1 + sum(s * (n - 1) for s, n in dims)
+
+
+def _own_places(dims):
+    """Whether every stride reaches beyond what the smaller ones span, as in every part or transposition of a contiguous tensor: no two entries are one place."""
+    return all(s >= _extent(dims[i + 1:]) for i, (s, _) in enumerate(dims))
+
+
+def _apart(a, b, distance):
+    """Whether two such tensors, the second beginning ``distance`` elements behind the first, share no place (False where that cannot be told)."""
+    if distance >= _extent(a) or -distance >= _extent(b):
+        return True
+    if not a or not b or a[0][0] != b[0][0]:
+        return False
+    stride = a[0][0]  # (one of the other's entries begins less than a stride behind each entry, and one less than a stride before it)
+    return _apart(a[1:], b[1:], distance % stride) and _apart(a[1:], b[1:], distance % stride - stride)
+
+
 class PagedCache:
     """Keys and values in pages: ``keys``, ``values`` ``[n_pages, n_kv_heads, page_size, head_dim]`` (bf16 or fp16 on one GPU, rows contiguous on
-    16-byte boundaries, the other strides free) and, for sparse steps, ``bounds`` ``[n_pages, n_kv_heads, 2, head_dim]`` (contiguous): the
+    16-byte boundaries, the other strides those of any part or transposition of a tensor, no two places the same memory) and, for sparse steps, ``bounds`` ``[n_pages, n_kv_heads, 2, head_dim]`` (contiguous): the
     smallest and the largest value of each channel over a page's keys, which :func:`append_to_pages` sets with a page's first key and widens with the
     others (keys that are taken back by a smaller length stay in them until the first is stored again; whoever copies pages copies their bounds).  The contents of pages that no table names
     do not matter.  The tensors stay the cache's own for as long as it is used: their contents may change, their memory may not, and a cache gets no others.  After
@@ -79,10 +104,12 @@ class PagedCache:
                     f"not {tuple(keys.shape)} and {tuple(values.shape)}")
         for t in (keys, values):
             sp, sh, sn, sd = t.stride()
-            if sd != 1 or (sp | sh | sn) & 7 or t.data_ptr() & 15 or not d <= sn <= 1 << 14 or (not sp and n_pages > 1) or (not sh and kv_heads > 1):
+            if sd != 1 or (sp | sh | sn) & 7 or t.data_ptr() & 15 or not d <= sn <= 1 << 14 or not _own_places(_dims(t)):
                 _refuse("the rows of keys and values must be contiguous, begin on 16-byte boundaries and lie at most 16384 elements apart, and no two share memory")
         if bounds is not None and (bounds.shape != (n_pages, kv_heads, 2, d) or not bounds.is_contiguous() or bounds.data_ptr() & 15):
             _refuse(f"bounds must be a contiguous tensor {(n_pages, kv_heads, 2, d)}, not {tuple(bounds.shape)}")
+        if any(not _apart(_dims(x), _dims(y), (y.data_ptr() - x.data_ptr()) // 2) for i, x in enumerate(tensors) for y in tensors[i + 1:]):
+            _refuse("keys, values and bounds must not share memory (parts of one tensor that lie between each other need the same strides)")
         # (what the C interface is told of the cache, once: 13 arguments fewer in each call)
         struct = _hip.PagedCacheStruct(*_hip.t3(keys), *_hip.t3(values), None if bounds is None else bounds.data_ptr(), n_pages, kv_heads, page_size, d,
                                        _hip.dtype_code(keys))
@@ -153,7 +180,8 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
     queries) keys are stored as they are: those of a prompt that the model has rotated itself.
 
     Tokens without a place are left out - rows behind the last sequence, a length of 0, a position that ``cos`` or the table does not reach, a page
-    outside the pool: their rows of ``out`` stay as they are (undefined in a new one).  Two sequences must not append to one page: the result is then one's or a mixture."""
+    outside the pool: their rows of ``out`` stay as they are (undefined in a new one).  Two sequences must not append to one page: the result is then one's or a mixture.
+    ``k`` and ``v`` must not lie in the pages that are appended to."""
     _plain(cache, q, k, v, cos, sin, out)
     k_args, (n, _, _) = _rows(k, "k", cache, cache.n_kv_heads)
     v_args, (n_values, _, _) = _rows(v, "v", cache, cache.n_kv_heads)
@@ -196,7 +224,9 @@ def _new_rows(t):
 
 def _out_rows(out, shape, cache):
     rows, out_shape = _rows(out, "out", cache, shape[1])
-    if out_shape != shape or (not rows[1] and shape[0] > 1) or (not rows[2] and shape[1] > 1):
+    n, h, d = shape
+    _, st, sh = rows
+    if out_shape != shape or not (((h == 1 or sh >= d) and (n < 2 or st >= (h - 1) * sh + d)) or ((n < 2 or st >= d) and (h == 1 or sh >= (n - 1) * st + d))):
         _refuse("out must have the shape of q, and no two of its rows the same memory")
     return rows
 
@@ -220,7 +250,8 @@ def _decode_args(cache, q, page_table, lengths, sm_scale, out):
 def paged_decode_attention(cache: PagedCache, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, sm_scale: Optional[float] = None,
                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one new token per sequence, ``q`` ``[batch, query heads, D]``, over the first ``lengths[b]`` keys of each: ``softmax(q K^T
-    sm_scale) V``, zeros for a sequence of none (NaN for one whose scores are all minus infinity).  ``sm_scale`` defaults to ``D ** -0.5``; ``out`` may be ``q``."""
+    sm_scale) V``, zeros for a sequence of none (NaN for one whose scores are all minus infinity).  ``sm_scale`` defaults to ``D ** -0.5``; ``out`` may be ``q`` and
+    otherwise shares no memory with the inputs."""
     out, tensors, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
     if sizes[0]:
         lib = _hip.lib()

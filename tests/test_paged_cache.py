@@ -874,3 +874,82 @@ def test_a_cache_whose_tensors_get_other_memory_is_refused(name):
         assert torch.equal(call(), x)
     s.cache.values.copy_(2 * s.cache.values)
     assert torch.equal(calls[0](), 2 * want[0])
+
+
+@pytest.mark.gpu
+def test_memory_that_is_shared_is_refused():
+    """Rows of one tensor that overlap without a stride of 0, tensors that overlap each other, outputs whose rows do: nothing is launched."""
+    from anchor_attn.src.ops import _hip
+    ops = _ops()
+    z = lambda *shape: torch.zeros(shape, dtype=BF16, device="cuda")  # noqa: E731
+    pool, other = z(1 << 16), z(5, 2, 16, 64)
+    dense = (2 * 16 * 64, 16 * 64, 64, 1)
+    at = lambda begin, strides: pool.as_strided((5, 2, 16, 64), strides, begin)  # noqa: E731
+    for strides in ((1024, 1024, 64, 1), (2048, 512, 64, 1), (8, 1024, 64, 1), (2040, 1024, 64, 1), (1024, 64, 64, 1), (64, 1024, 64, 1)):
+        for keys, values in ((at(0, strides), other), (other, at(0, strides))):
+            with pytest.raises(_hip.AnchorAttnHipError, match="no two share memory"):
+                ops.PagedCache(keys, values)
+    for keys, values, bounds in ((other, other, None), (at(0, dense), at(0, dense), None), (at(0, dense), at(9 * 1024, dense), None), (at(9 * 1024, dense), at(0, dense), None),
+                                 (at(0, dense), at(10240 - 8, dense), None), (at(0, (4096, 1024, 64, 1)), at(2040, (4096, 1024, 64, 1)), None),
+                                 (at(0, (4096, 1024, 64, 1)), at(1024, (4096, 1024, 64, 1)), None), (at(0, (4096, 1024, 64, 1)), at(2048, (4096, 2048, 64, 1)), None),
+                                 (at(0, dense), other, pool[8192:8192 + 5 * 256].view(5, 2, 2, 64)), (other, at(512, dense), pool[:1280].view(5, 2, 2, 64))):
+        with pytest.raises(_hip.AnchorAttnHipError, match="must not share memory"):
+            ops.PagedCache(keys, values, bounds)
+    cache = ops.PagedCache(z(5, 2, 16, 64), z(5, 2, 16, 64))
+    table, lengths = torch.zeros(3, 2, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    for strides in ((64, 64, 1), (8, 256, 1), (256, 8, 1), (128, 64, 1), (248, 64, 1), (64, 128, 1), (64, 184, 1)):
+        with pytest.raises(_hip.AnchorAttnHipError, match="same memory"):
+            ops.paged_decode_attention(cache, z(3, 4, 64), table, lengths, out=pool.as_strided((3, 4, 64), strides))
+    for strides in ((256, 64, 1), (64, 192, 1), (1024, 72, 1), (72, 1024, 1)):
+        out = pool.as_strided((3, 4, 64), strides)
+        assert ops.paged_decode_attention(cache, z(3, 4, 64), table, lengths, out=out) is out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["pages of both", "rows of both", "heads of both", "one after the other", "heads and rows"])
+def test_keys_and_values_that_lie_between_each_other(layout):
+    """Parts of one tensor: the same bits as from two."""
+    ops, n, h, page, d = _ops(), 30, 2, 16, 64
+    if layout == "pages of both":
+        keys, values = torch.zeros(n, 2, h, page, d, dtype=BF16, device="cuda").unbind(1)
+    elif layout == "rows of both":
+        keys, values = torch.zeros(n, h, page, 2 * d, dtype=BF16, device="cuda").split(d, -1)
+    elif layout == "heads of both":
+        keys, values = (x.transpose(1, 2) for x in torch.zeros(n, page, 2 * h, d, dtype=BF16, device="cuda").split(h, 2))
+    elif layout == "one after the other":
+        keys, values = torch.zeros(2, n, h, page, d, dtype=BF16, device="cuda").unbind(0)
+    else:
+        both = torch.zeros(n, 2 * h * page * d, dtype=BF16, device="cuda")
+        keys, values = both[:, :h * page * d].view(n, h, page, d), both[:, h * page * d:].view(n, page, h, d).transpose(1, 2)
+    s = _Setup([0, 0], h, d, page, BF16, 23, room=200)
+    assert s.cache.n_pages <= n
+    lengths, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([200, 37], [0, 200, 237]))
+    q, k, v = (torch.randn(237, x, d, generator=s.g, device="cuda").to(BF16) for x in (4, h, h))
+    results = []
+    for cache in (s.cache, ops.PagedCache(keys, values, torch.zeros(n, h, 2, d, dtype=BF16, device="cuda"))):
+        rotated = ops.append_to_pages(cache, q, k, v, *_tables(200, d), s.table, lengths, starts)
+        results.append((rotated, ops.paged_decode_attention(cache, rotated[:2], s.table, lengths), *ops.paged_sparse_decode_attention(cache, rotated[:2], s.table, lengths, 5)))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_tensors_that_are_told_apart_share_no_place():
+    """... against all places of small tensors with strides of any kind."""
+    import itertools
+    import random
+    ops, r = _ops(), random.Random(3)
+    places = lambda dims, begin: [begin + sum(i * s for i, (s, _) in zip(at, dims)) for at in itertools.product(*(range(n) for _, n in dims))]  # noqa: E731
+    told, refused = 0, 0
+    for _ in range(20000):
+        a, b = (sorted(((r.choice([1, 2, 3, 4, 6, 8, 12, 24]), r.randint(2, 4)) for _ in range(r.randint(0, 3))), reverse=True) for _ in range(2))
+        b = r.choice([a, b])
+        of_a = set(places(a, 0))
+        alone = len(of_a) == len(places(a, 0))
+        assert alone or not ops._own_places(a)
+        if ops._own_places(a) and ops._own_places(b):
+            distance = r.randint(-30, 30)
+            if ops._apart(a, b, distance):
+                told += 1
+                assert not of_a & set(places(b, distance))
+            else:
+                refused += bool(of_a & set(places(b, distance)))
+    assert told > 1000 and refused > 1000
