@@ -162,7 +162,7 @@ def _plain(cache, *tensors):
         _refuse("these operators cannot be traced, compiled, vmapped or watched by a mode")
     if torch.is_grad_enabled():
         for t in tensors:
-            if t is not None and t.requires_grad:
+            if getattr(t, "requires_grad", False):  # (what is no tensor is refused where its type is looked at)
                 _refuse("these operators have no gradients: detach their inputs or call them under torch.no_grad()")
 
 
@@ -194,7 +194,7 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
             _refuse("cos and sin come together, and queries need them")
         angles, n_positions, q_args, heads = (0, 0, 0), 0, (0,) * 6, 0
     else:
-        strides = cos.stride()
+        strides = cos.stride() if type(cos) in _TYPES else None
         for t in (cos, sin):
             if type(t) not in _TYPES or t.dtype != _FLOAT32 or t.get_device() != cache.index or t.dim() != 2 or t.shape != cos.shape or t.stride() != strides:
                 _refuse("cos and sin must be float32 tensors [positions, D / 2] on the cache's device, laid out alike")
@@ -270,9 +270,15 @@ def paged_sparse_decode_attention(cache: PagedCache, q: torch.Tensor, page_table
     The products are exact, summed in float64 (in any order) and rounded to float32; NaN counts as infinity.  Returns the output and the chosen pages, int32 ``[batch, KV heads,
     n_pages]``: places in the sequence's row of the table, ascending, then -1.  The cache needs ``bounds``."""
     out, tensors, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
-    n_pages, n_first, n_last = int(n_pages), int(n_first), int(n_last)
     if cache.bounds is None:
         _refuse("sparse steps need a cache with bounds")
+    given = n_pages, n_first, n_last
+    try:
+        n_pages, n_first, n_last = whole = tuple(map(int, given))
+    except (TypeError, ValueError, OverflowError):
+        whole = None
+    if whole != given:
+        _refuse("n_pages, n_first and n_last must be whole numbers, not %s, %s and %s" % given)
     if n_first < 0 or n_last < 1 or n_first + n_last > n_pages or n_pages > 1 << 16:
         _refuse(f"{n_pages} pages, the first {n_first} and the last {n_last} among them, are not supported (at most 65536, at least the last one)")
     pages = lengths.new_empty((sizes[0], cache.n_kv_heads, n_pages))

@@ -953,3 +953,28 @@ def test_tensors_that_are_told_apart_share_no_place():
             else:
                 refused += bool(of_a & set(places(b, distance)))
     assert told > 1000 and refused > 1000
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [True, False])
+def test_what_is_no_tensor_or_whole_number_is_refused(grad):
+    """By the error that every refused call raises, with gradients recorded or not."""
+    import numpy as np
+    from anchor_attn.src.ops import _hip
+    ops = _ops()
+    s = _Setup([40, 3], 2, 64, 16, BF16, 24, room=20)
+    q, k = s.queries(4), torch.zeros(2, 2, 64, dtype=BF16, device="cuda")
+    cos, sin = _tables(100, 64)
+    steps = {"cache": s.cache, "q": q, "page_table": s.table, "lengths": s.lengths}
+    for fn, given, names in ((ops.paged_decode_attention, steps, ("q", "page_table", "lengths", "out")),
+                             (ops.paged_sparse_decode_attention, {**steps, "n_pages": 2}, ("q", "page_table", "lengths", "out")),
+                             (ops.append_to_pages, {**steps, "k": k, "v": k, "cos": cos, "sin": sin}, ("q", "k", "v", "cos", "sin", "page_table", "lengths", "starts", "out"))):
+        for name in names:
+            for other in ([1.0], "x", 3, np.zeros((2, 4, 64), np.float32)):
+                with torch.set_grad_enabled(grad), pytest.raises(_hip.AnchorAttnHipError):
+                    fn(**{**given, name: other})
+    for change in ({"n_pages": 2.5}, {"n_pages": "2"}, {"n_pages": float("inf")}, {"n_first": float("nan")}, {"n_pages": None}, {"n_first": 0.5}, {"n_last": 1.5}, {"n_last": None}):
+        with pytest.raises(_hip.AnchorAttnHipError, match="whole numbers"):
+            ops.paged_sparse_decode_attention(**{**steps, "n_pages": 3, **change})
+    want = ops.paged_sparse_decode_attention(**steps, n_pages=2)
+    assert all(torch.equal(a, b) for a, b in zip(want, ops.paged_sparse_decode_attention(**steps, n_pages=np.int64(2), n_first=torch.tensor(1), n_last=1.0)))
