@@ -977,8 +977,8 @@ static void give_scratch(PagedDecodeArgs& a, char* workspace, int max_pages) {
 
 static int paged_decode_args(const char* who, PagedDecodeArgs& a, const aa_paged_cache* cache, const aa_paged_step* t, size_t needed) {
   int rc;
-  if (t->n_q_heads == 0 || !(t->sm_scale > 0.f) || t->sm_scale > 3.4e38f) {
-    set_error("%s: %d query heads and sm_scale %g: both must be positive and finite", who, t->n_q_heads, (double)t->sm_scale);
+  if (t->n_q_heads == 0 || !(t->sm_scale > 0.f) || t->sm_scale * kLog2e > 3.4e38f) {  // (the kernels multiply by the product)
+    set_error("%s: %d query heads and sm_scale %g: both must be positive and below 2.3e38", who, t->n_q_heads, (double)t->sm_scale);
     return AA_EBADARG;
   }
   if ((int64_t)t->batch * t->n_q_heads >= 1 << 24) {

@@ -280,7 +280,7 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
  *
  * aa_paged_decode_fwd: out[b, h] = softmax(q[b, h] . keys * sm_scale) values over the keys 0 .. lengths[b] - 1 of sequence b; a sequence of none gives 0,
  * one whose scores are all minus infinity NaN, as the quotient has it.
- * q, out: [batch, n_q_heads, head_dim] with strides of sequence and head.  workspace: aa_paged_decode_workspace_bytes() bytes of device scratch, which
+ * q, out: [batch, n_q_heads, head_dim] with strides of sequence and head; out may be q.  sm_scale is positive and below 2.3e38.  workspace: aa_paged_decode_workspace_bytes() bytes of device scratch, which
  * may be none (contents undefined afterwards).
  *
  * aa_paged_sparse_decode_fwd: the same over n_chosen pages for each sequence and KV head, or all where the sequence has no more: its first n_first, its last

@@ -978,3 +978,13 @@ def test_what_is_no_tensor_or_whole_number_is_refused(grad):
             ops.paged_sparse_decode_attention(**{**steps, "n_pages": 3, **change})
     want = ops.paged_sparse_decode_attention(**steps, n_pages=2)
     assert all(torch.equal(a, b) for a, b in zip(want, ops.paged_sparse_decode_attention(**steps, n_pages=np.int64(2), n_first=torch.tensor(1), n_last=1.0)))
+
+
+@pytest.mark.parametrize("fn", ["aa_paged_decode_fwd", "aa_paged_sparse_decode_fwd"])
+@pytest.mark.parametrize("scale", [3e38, 2.5e38, -1.0, float("-inf")])
+def test_scales_that_leave_float32_are_refused(fn, scale):
+    """The kernels multiply scores by sm_scale * log2 e: an infinity there gives NaN for the largest score."""
+    from anchor_attn.src.ops import _hip
+    struct = _hip.PagedCacheStruct(*CACHE.values())
+    with pytest.raises(_hip.AnchorAttnHipError, match="sm_scale"):
+        _hip.check(getattr(_hip.lib(), fn)(ctypes.addressof(struct), _hip.PAGED_STEP.pack(*{**STEP, "sm_scale": scale}.values()), None))
