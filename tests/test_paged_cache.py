@@ -988,3 +988,179 @@ def test_scales_that_leave_float32_are_refused(fn, scale):
     struct = _hip.PagedCacheStruct(*CACHE.values())
     with pytest.raises(_hip.AnchorAttnHipError, match="sm_scale"):
         _hip.check(getattr(_hip.lib(), fn)(ctypes.addressof(struct), _hip.PAGED_STEP.pack(*{**STEP, "sm_scale": scale}.values()), None))
+
+
+# ---- what the documents allow -----------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_bounds_tell_infinities_from_the_largest_numbers(dtype):
+    """Infinite keys give infinite bounds, the largest finite ones finite bounds, in the page's first append and in one that widens them; NaN of either sign both."""
+    ops = _ops()
+    s = _Setup([0], 1, 64, 16, dtype, 25, room=40)
+    most = torch.finfo(dtype).max
+    k = torch.randn(40, 1, 64, generator=s.g, device="cuda").to(dtype)
+    for row in (2, 17, 30):
+        for channel, x in enumerate((float("inf"), float("-inf"), most, -most, float("nan"), -float("nan"), -0.0)):
+            k[row + channel % 3, 0, channel] = x
+            k[row + (channel + 1) % 3, 0, 32 + channel] = x
+        k[row, 0, 20], k[row + 1, 0, 20] = float("inf"), float("-inf")
+        k[row, 0, 21], k[row + 1, 0, 21] = float("inf"), float("nan")
+        k[row, 0, 22], k[row + 1, 0, 22] = most, float("inf")
+    for lo, hi in ((0, 3), (3, 16), (16, 19), (19, 40)):
+        ops.append_to_pages(s.cache, None, k[lo:hi], k[lo:hi], None, None, s.table, torch.tensor([hi], dtype=torch.int32, device="cuda"),
+                            torch.tensor([0, hi - lo], dtype=torch.int32, device="cuda"))
+        for i in range(0, hi, 16):
+            page, rows = int(s.table[0, i // 16]), k[i:min(hi, i + 16), 0]
+            assert _same(s.cache.keys[page, 0, :rows.shape[0]], rows) and _same(s.cache.values[page, 0, :rows.shape[0]], rows)
+            assert _same(s.cache.bounds[page, 0], torch.stack((rows.amin(0), rows.amax(0))))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,hq,hkv,d,page", [(1, 14, 2, 64, 16), (97, 32, 8, 128, 64), (300, 4, 1, 128, 256)])
+def test_append_one_token_each_in_fp16(batch, hq, hkv, d, page):
+    _append_and_check([(37 * b) % 211 for b in range(batch)], [1] * batch, hq, hkv, d, page, F16, "heads", steps=True, seed=batch)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_rows_that_lie_as_far_apart_as_they_may(dtype):
+    """Rows 16384 elements apart, appended to and read: the same bits as from dense pages."""
+    ops, n, h, page, d = _ops(), 11, 3, 32, 128
+    far = [torch.full((n, page, 16384), float("nan"), dtype=dtype, device="cuda")[:, :, 128:128 + h * 256].unflatten(2, (h, 256))[..., 64:64 + d].transpose(1, 2) for _ in range(2)]
+    s = _Setup([0, 0], h, d, page, dtype, 26, room=100)
+    assert s.cache.n_pages <= n and far[0].stride()[2] == 16384
+    lengths, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([97, 31], [0, 97, 128]))
+    q, k, v = (torch.randn(128, x, d, generator=s.g, device="cuda").to(dtype) for x in (2 * h, h, h))
+    results = []
+    for cache in (s.cache, ops.PagedCache(*far, torch.zeros(n, h, 2, d, dtype=dtype, device="cuda"))):
+        rotated = ops.append_to_pages(cache, q, k, v, *_tables(100, d), s.table, lengths, starts)
+        results.append((rotated, ops.paged_decode_attention(cache, rotated[:2], s.table, lengths), *ops.paged_sparse_decode_attention(cache, rotated[:2], s.table, lengths, 3)))
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and bool(results[1][1].isfinite().all())
+
+
+@pytest.mark.gpu
+def test_views_that_repeat_or_leave_out():
+    """Expanded queries, one row of a table for all sequences, a table that is part of a wider one, lengths from the middle of a tensor."""
+    ops = _ops()
+    s = _Setup([300, 270, 5], 2, 64, 16, BF16, 27)
+    q = s.queries(4)
+    run = lambda q, t, n: (ops.paged_decode_attention(s.cache, q, t, n), *ops.paged_sparse_decode_attention(s.cache, q, t, n, 6))  # noqa: E731
+    want = run(q, s.table, s.lengths)
+    wide, more = torch.full((3, 100), -1, dtype=torch.int32, device="cuda"), torch.tensor([9, 9, 300, 270, 5, 9], dtype=torch.int32, device="cuda")
+    wide[:, 3:3 + s.table.shape[1]] = s.table
+    assert all(torch.equal(a, b) for a, b in zip(run(q, wide[:, 3:3 + s.table.shape[1]], more[2:5]), want))
+    lengths = torch.tensor([300, 100, 0], dtype=torch.int32, device="cuda")
+    one = run(q[:1].expand(3, 4, 64).contiguous(), s.table[:1].repeat(3, 1), lengths)
+    assert all(torch.equal(a, b) for a, b in zip(run(q[:1].expand(3, 4, 64), s.table[:1].expand(3, -1), lengths), one))
+    one_head = run(q[:, :1].expand(3, 4, 64).contiguous(), s.table, s.lengths)
+    assert all(torch.equal(a, b) for a, b in zip(run(q[:, :1].expand(3, 4, 64), s.table, s.lengths), one_head))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(4096, 1, 64), (3000, 1500, 64), (9000, 9000, 64), (640, 20, 128)])
+def test_many_heads(hq, hkv, d):
+    s = _Setup([70, 33], hkv, d, 16, BF16, 28)
+    q = s.queries(hq, 1.0)
+    out, (sparse, pages) = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths), _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 4)
+    for b, n in enumerate(s.host):
+        there = (n + 15) // 16
+        at = s.table[b, :there].long()
+        k, v = (x[at].transpose(0, 1).flatten(1, 2)[:, :n].double() for x in (s.cache.keys, s.cache.values))
+        x = q[b].view(hkv, hq // hkv, d).double()
+        score = (x @ k.transpose(1, 2)) * d ** -0.5
+        lo, hi = (s.cache.bounds[at, :, i].transpose(0, 1).double() for i in (0, 1))
+        page_score = (x.clamp(min=0) @ hi.transpose(1, 2) + x.clamp(max=0) @ lo.transpose(1, 2)).amax(1).float()
+        chosen = torch.zeros(hkv, there, dtype=torch.bool, device="cuda")
+        if there <= 4:
+            chosen[:] = True
+        else:  # (five pages: the first, the last and two between are read)
+            page_score[:, 0] = page_score[:, -1] = float("inf")
+            chosen.scatter_(1, page_score.sort(dim=1, descending=True, stable=True).indices[:, :4], True)
+        assert torch.equal(chosen, torch.zeros(hkv, there + 1, dtype=torch.bool, device="cuda").scatter_(1, pages[b].long() % (there + 1), True)[:, :there])
+        hidden = ~chosen.repeat_interleave(16, 1)[:, None, :n]
+        for got, p in ((out, score.softmax(-1)), (sparse, score.masked_fill(hidden, float("-inf")).softmax(-1))):
+            want = (p @ v).reshape(hq, d)
+            relative = 2.0 * d * 2.0 ** -24 * float((x.abs() @ k.abs().transpose(1, 2)).amax()) * d ** -0.5 + 2.0 ** -14 + U[BF16] ** 2 + n * 2.0 ** -24
+            bound = U[BF16] * want.abs() * 1.001 + relative * (p @ v.abs()).reshape(hq, d) + 2.0 ** -25
+            assert bool(((got[b].double() - want).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+def test_the_most_sequences():
+    """65535 of them, of 0 to 16 keys: a sequence's output is the same as that of a batch of its own."""
+    ops, n = _ops(), 65535
+    g = torch.Generator(device="cuda").manual_seed(29)
+    cache = ops.PagedCache.empty(4096, 1, 16, 64)
+    cache.keys.normal_(generator=g), cache.values.normal_(generator=g)
+    table = torch.randint(0, 4096, (n, 1), generator=g, device="cuda", dtype=torch.int32)
+    lengths = torch.randint(0, 17, (n,), generator=g, device="cuda", dtype=torch.int32)
+    q = torch.randn(n, 2, 64, generator=g, device="cuda").to(BF16)
+    out = ops.paged_decode_attention(cache, q, table, lengths)
+    for b in (0, 1, 63, 64, 255, 256, 257, 32768, 65279, 65280, 65533, 65534):
+        assert torch.equal(out[b:b + 1], ops.paged_decode_attention(cache, q[b:b + 1], table[b:b + 1], lengths[b:b + 1]))
+    keys, values = cache.keys[table[:, 0].long(), 0], cache.values[table[:, 0].long(), 0]
+    score = (q.float() @ keys.float().transpose(1, 2)) / 8
+    p = score.masked_fill(torch.arange(16, device="cuda") >= lengths[:, None, None], float("-inf")).softmax(-1).nan_to_num(0.0)
+    # (besides the output's rounding 2 * 64 * 2^-24 * sum |q k| / 8, below 2^-13 here, 2^-14 of exp2, 2^-16 of the pairs: 2^-12 of sum p |v|)
+    assert bool(((out.float() - p @ values.float()).abs() <= 2.0 ** -8 * (p @ values.float()).abs() * 1.01 + 2.0 ** -12 * (p @ values.abs().float())).all())
+    # and appended to: every sequence's next token, to pages of their own
+    pool = ops.PagedCache.empty(n, 1, 16, 64)
+    own = torch.randperm(n, generator=g, device="cuda").int()[:, None]
+    k = torch.randn(n, 1, 64, generator=g, device="cuda").to(BF16)
+    pool.keys.zero_(), pool.values.zero_()
+    ops.append_to_pages(pool, None, k, q[:, :1], None, None, own, lengths)
+    there = lengths > 0
+    at, slot = own[there, 0].long(), lengths[there].long() - 1
+    assert torch.equal(pool.keys[at, 0, slot], k[there, 0]) and torch.equal(pool.values[at, 0, slot], q[there, 0])
+    assert int((pool.keys != 0).any(-1).sum()) == int(there.sum())
+
+
+@pytest.mark.gpu
+def test_a_prompt_of_a_million_tokens():
+    ops, n, page = _ops(), (1 << 20) - 37, 64
+    g = torch.Generator(device="cuda").manual_seed(30)
+    cache = ops.PagedCache.empty(n // page + 1, 1, page, 64, F16)
+    table = torch.randperm(cache.n_pages, generator=g, device="cuda").int()[None]
+    k, v = (torch.randn(n, 1, 64, generator=g, device="cuda").to(F16) for _ in range(2))
+    ops.append_to_pages(cache, None, k, v, None, None, table, torch.tensor([n], dtype=torch.int32, device="cuda"), torch.tensor([0, n], dtype=torch.int32, device="cuda"))
+    for pool, x in ((cache.keys, k), (cache.values, v)):
+        assert torch.equal(pool[table[0].long(), 0].flatten(0, 1)[:n], x[:, 0])
+    full = n // page
+    assert torch.equal(cache.bounds[table[0, :full].long(), 0, 0], k[:full * page, 0].view(full, page, 64).amin(1))
+    assert torch.equal(cache.bounds[table[0, :full].long(), 0, 1], k[:full * page, 0].view(full, page, 64).amax(1))
+    assert torch.equal(cache.bounds[table[0, full].long(), 0], torch.stack((k[full * page:, 0].amin(0), k[full * page:, 0].amax(0))))
+
+
+@pytest.mark.gpu
+def test_inference_mode_and_threads():
+    import threading
+    ops = _ops()
+    s = _Setup([3000, 5000, 100], 4, 128, 64, BF16, 31, room=64)
+    q = [s.queries(16) for _ in range(4)]
+    step = lambda x: (ops.paged_decode_attention(s.cache, x, s.table, s.lengths), *ops.paged_sparse_decode_attention(s.cache, x, s.table, s.lengths, 9))  # noqa: E731
+    want = [step(x) for x in q]
+    with torch.inference_mode():
+        cache = ops.PagedCache(s.cache.keys.clone(), s.cache.values.clone(), s.cache.bounds.clone())
+        assert torch.equal(ops.paged_decode_attention(cache, q[0], s.table, s.lengths), want[0][0])
+        k = torch.zeros(3, 4, 128, dtype=BF16, device="cuda")
+        ops.append_to_pages(cache, None, k, k, None, None, s.table, s.lengths + 1)
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                got[i] = [step(q[i]) for _ in range(10)]
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for outs, x in zip(got, want):
+        assert all(torch.equal(a, b) for one in outs for a, b in zip(one, x))
