@@ -13,8 +13,6 @@
 // first spans the smallest to the largest score, so that two or three do, whatever the scores' exponents (at most four).  Every wave reads the bins for itself,
 // which leaves one barrier for each histogram.  Integer work: the order in which counts are added does not matter.  The code is kept short, since most of it runs
 // once and its first instructions come from memory.
-#include <type_traits>
-
 #include "aa_kernels.h"
 #include "aa_paged.h"
 
@@ -59,26 +57,22 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// Bounds of 8 channels of N pages, and sums of their products with queries, both in float64: bf16 has the exponents of float32, so that a product of two may lie
-// beyond 2^128, or below 2^-126, and the sum still be a float32.  In float64 it is exact, and part of the addition.
-template <typename T, int N>
+// Bounds of 8 channels of N pages, and sums of their products with queries in float64.
+//
+// WIDE: products in float64 too.  bf16 has the exponents of float32, in which a product may overflow, or lose bits below 2^-126; those of fp16 do not.  bf16 products are
+// formed in float32 all the same, in a quarter less time (32/8 heads of 64, 256 pages scored and chosen from in one launch 17.5 us a step instead of 18.1), and once more
+// in float64 where the sum shows that this may have counted: one that overflowed leaves an infinity or NaN, and 128 that lost 2^-150 each are off by
+// 2^-143, less than a float64 sum's own rounding of what is 2^-80 or larger.
+template <typename T, int N, bool WIDE = false>
 struct Products {
-  typedef typename std::conditional<N == 1, double, float>::type Bound;  // (converted once where there is one page, with the queries where several share them)
-  Bound bounds[N][2][8];
+  static constexpr bool kMayLeave = !WIDE;  // float32
+  float bounds[N][2][8];
   static __device__ __forceinline__ u32x4 query(const u32x4 q) { return q; }  // as it is staged
   __device__ __forceinline__ explicit Products(const u32x4 (&raw)[N][2]) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        float x[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(&raw[i][w]), x);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          bounds[i][w][j] = x[j];
-          if constexpr (N == 1) asm("" : "+v"(bounds[i][w][j]));  // (here and not once more for every head)
-        }
-      }
+      for (int w = 0; w < 2; ++w) unpack8<T>(*reinterpret_cast<const uint4*>(&raw[i][w]), bounds[i][w]);
   }
   __device__ __forceinline__ void add(double (&sum)[N], const u32x4 raw) const {
     float q[8];
@@ -86,16 +80,20 @@ struct Products {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const bool larger = q[j] >= 0.f;
-      const double x = q[j];
 #pragma unroll
-      for (int i = 0; i < N; ++i) sum[i] = __builtin_fma(x, (double)(larger ? bounds[i][1][j] : bounds[i][0][j]), sum[i]);
+      for (int i = 0; i < N; ++i) {
+        const float x = larger ? bounds[i][1][j] : bounds[i][0][j];
+        if constexpr (WIDE) sum[i] = __builtin_fma((double)q[j], (double)x, sum[i]);
+        else sum[i] += (double)(q[j] * x);
+      }
     }
   }
 };
 // A product of two fp16 numbers is exact in float32; an instruction multiplies two of them into one, and two bounds are chosen at once by their queries' signs, for which -0 becomes 0
 // (16 sequences of 6000 to 60000 keys in pages of 16: 16.9 us, with conversions as in bf16 18.5).
 template <int N>
-struct Products<F16, N> {
+struct Products<F16, N, false> {
+  static constexpr bool kMayLeave = false;
   u32x4 bounds[N][2];
   static __device__ __forceinline__ u32x4 query(u32x4 q) {
 #pragma unroll
@@ -159,46 +157,59 @@ struct Scores {
     }
     return y;
   }
-  // `staged`: the group's queries one after the other (as many as stage() has room for).  store(k, score) is called by one lane for each page, 0 <= k < kPages
+  // `staged`: the group's queries one after the other (as many as stage() has room for); `count`: of the pages there are; store(k, score) is called by one lane for each page,
+  // 0 <= k < kPages
   template <typename Store>
-  static __device__ __forceinline__ void form(const PagedSelectArgs& p, const int b, const int kvh, const Bounds& y, const uint32_t* staged, const int room, Store store) {
+  static __device__ __forceinline__ void form(const PagedSelectArgs& p, const int b, const int kvh, const Bounds& y, const uint32_t* staged, const int room, const int count,
+                                              Store store) {
     const int lane = threadIdx.x & 63, c = lane % kLanes, group = p.n_q_heads / p.n_kv_heads;
     const uint16_t* qp = p.q + b * p.q_sb + (int64_t)kvh * group * p.q_sh + 8 * c;
     auto query = [&](const int h) {
       if (h < room) return *reinterpret_cast<const u32x4*>(staged + h * (D / 2) + 4 * c);
       return Products<T, N>::query(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(qp + h * p.q_sh)));
     };
-    const Products<T, N> products(y.raw);
-    u32x4 next = query(0);
     // bits of a lane that say which of its pages it ends with: the same in the lane that is mirrored in 8
     const bool odd = (kLanes == 8 ? lane ^ lane >> 2 : lane) & 1, odd2 = (kLanes == 8 ? lane ^ lane >> 1 : lane) & 2;
-    float best = -INFINITY;
-    bool nan = false;
+    const int mine = kSide * (N == 4 ? (odd ? 2 : 0) + (odd2 ? 1 : 0) : 0) + lane / kLanes;
+    float best;
+    bool nan, unsure;
+    auto over_heads = [&](const auto products) __attribute__((always_inline)) {
+      best = -INFINITY;
+      nan = unsure = false;
+      u32x4 next = query(0);
 #pragma nounroll
-    for (int h = 1; h <= group; ++h) {
-      const u32x4 q = next;
-      next = query(min(h, group - 1));
-      double sum[N] = {};
-      products.add(sum, q);
-      double s;
-      if constexpr (N == 4) {  // twice a lane keeps the half of what it has that a bit of it names, and gives the other away
-        const double a = (odd ? sum[2] : sum[0]) + dpp<kDppXor1>(odd ? sum[0] : sum[2]);
-        const double b = (odd ? sum[3] : sum[1]) + dpp<kDppXor1>(odd ? sum[1] : sum[3]);
-        s = (odd2 ? b : a) + dpp<kDppXor2>(odd2 ? a : b);
-      } else {
-        s = sum[0] + dpp<kDppXor1>(sum[0]);
-        s += dpp<kDppXor2>(s);
+      for (int h = 1; h <= group; ++h) {
+        const u32x4 q = next;
+        next = query(min(h, group - 1));
+        double sum[N] = {};
+        products.add(sum, q);
+        double s;
+        if constexpr (N == 4) {  // twice a lane keeps the half of what it has that a bit of it names, and gives the other away
+          const double a = (odd ? sum[2] : sum[0]) + dpp<kDppXor1>(odd ? sum[0] : sum[2]);
+          const double b = (odd ? sum[3] : sum[1]) + dpp<kDppXor1>(odd ? sum[1] : sum[3]);
+          s = (odd2 ? b : a) + dpp<kDppXor2>(odd2 ? a : b);
+        } else {
+          s = sum[0] + dpp<kDppXor1>(sum[0]);
+          s += dpp<kDppXor2>(s);
+        }
+        if (kLanes == 8) {
+          s += dpp<kDppHalfMirror>(s);
+        } else {
+          s += dpp<kDppRor8>(s);
+          s += dpp<kDppRor4>(s);
+        }
+        nan = nan || s != s;
+        best = fmaxf(best, (float)s);
+        if constexpr (products.kMayLeave) {  // (by its exponent: below -80, or that of infinities and NaN)
+          const uint32_t exponent = (uint32_t)__double2hiint(s) >> 20 & 0x7ffu;
+          unsure = unsure || exponent - (1023u - 80u) >= 2047u - (1023u - 80u);
+        }
       }
-      if (kLanes == 8) {
-        s += dpp<kDppHalfMirror>(s);
-      } else {
-        s += dpp<kDppRor8>(s);
-        s += dpp<kDppRor4>(s);
-      }
-      nan = nan || s != s;
-      best = fmaxf(best, (float)s);
-    }
-    if (c < (N == 4 ? 4 : 1)) store(kSide * (N == 4 ? (odd ? 2 : 0) + (odd2 ? 1 : 0) : 0) + lane / kLanes, nan ? INFINITY : best);
+    };
+    over_heads(Products<T, N>(y.raw));
+    if constexpr (Products<T, N>::kMayLeave)
+      if (__builtin_expect(__any(unsure && mine < count), 0)) over_heads(Products<T, N, true>(y.raw));
+    if (c < (N == 4 ? 4 : 1)) store(mine, nan ? INFINITY : best);
   }
 };
 
@@ -230,7 +241,7 @@ __global__ void __launch_bounds__(256) paged_scores_kernel(const PagedSelectArgs
   at = S::find(p, b, first + step);
   float* scores = p.scores + ((int64_t)b * p.n_kv_heads + kvh) * paged_score_pitch(p.max_pages);
   for (;;) {
-    S::form(p, b, kvh, y, staged[wave], room, [&](const int k, const float x) {
+    S::form(p, b, kvh, y, staged[wave], room, there - first, [&](const int k, const float x) {
       if (first + k < there) scores[first + k] = x;
     });
     first += step;
@@ -283,7 +294,7 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
     __syncthreads();
 #pragma nounroll
     for (int i = wave * S::kPages; i < there;) {
-      S::form(p, b, kvh, y, staged, room, [&](const int k, const float x) {
+      S::form(p, b, kvh, y, staged, room, there - i, [&](const int k, const float x) {
         if (i + k < there) kept[i + k] = number(i + k, x);
       });
       i += kChooseWaves * S::kPages;
