@@ -23,10 +23,12 @@ namespace aa {
 constexpr int kAbreast = 4, kAbreastFused = 1;
 constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
 constexpr int kFused = 1024;       // a table of at most that many pages is scored and chosen from by one launch
-// ... if its bounds have so few (channel, head) products that one work-group forms them sooner than a launch of its own starts: 32/8 heads of 128, one
-// sequence, 64 pages 17.6 us a step by one launch and 19.8 by two, 128 pages 19.7 and 19.6, 256 24.2 and 19.7; 14/2 heads of 64 128 pages 16.6 and 19.0,
-// 192 17.9 and 19.1, 256 20.7 and 19.0.
-constexpr int kFusedProducts = 72 * 1024;
+// ... if one work-group does that sooner than a launch of its own starts.  It takes pages * D * (heads of the group + kPerPage): a page's bounds cost as much to
+// fetch and convert as the products of twelve heads.  Steps of one sequence, bf16, pages of 16, by one launch and by two: 32/8 heads of 128, 96 pages 17.8 and 19.3 us, 128
+// 19.5 and 19.3; 28/4 of 128, 96 pages 19.0 and 19.5, 128 21.8 and 20.3; 32/8 of 64, 192 pages 16.6 and 18.4, 256 17.9 and 18.2; 14/2 of 64, 192 pages 17.6 and 18.6,
+// 256 20.1 and 18.9.  16 sequences, and fp16, the same within 5 %.  Where the units fill the CUs, scores by themselves are no more side by side than with the choosing: 64
+// sequences, 32/8 of 128, 192 pages 44.3 and 45.3, 256 48.5 and 48.4; 28/4 of 128, 192 pages 32.2 and 32.4, 256 36.0 and 35.1; 32/8 of 64, 384 pages 34.5 and 36.0.
+constexpr int kPerPage = 12, kFusedWork = 256 * 1024, kFusedWorkMany = 460 * 1024, kManyUnits = 256;
 constexpr int kInLds = 32768;      // the scores of at most that many pages are kept in LDS
 // Pages that a thread of the choosing work-group looks at together, side by side: 4, and 1 in tables of at most kOnes pages, where the other threads would have
 // nothing to do.  (Steps of one sequence, 32/8 heads of 128: 8192 pages one 36.0 us, four 32.0; 1875 pages 21.6 and 21.8, 469 20.5 and 21.5.)
@@ -445,7 +447,8 @@ __global__ void __launch_bounds__(kChooseThreads) paged_choose_kernel(const Page
 template <typename T, int D>
 static void launch_paged_select_for(const PagedSelectArgs& a, hipStream_t stream) {
   const dim3 units(a.n_kv_heads, a.batch);
-  if (a.max_pages <= kFused && (int64_t)a.max_pages * (a.n_q_heads / a.n_kv_heads) * D <= kFusedProducts) {
+  const int64_t work = (int64_t)a.max_pages * D * (a.n_q_heads / a.n_kv_heads + kPerPage);
+  if (a.max_pages <= kFused && work <= ((int64_t)a.batch * a.n_kv_heads < kManyUnits ? kFusedWork : kFusedWorkMany)) {
     hipLaunchKernelGGL((paged_choose_kernel<T, D, 0, 1>), units, dim3(kChooseThreads), 4 * paged_score_pitch(a.max_pages), stream, a);
     return;
   }

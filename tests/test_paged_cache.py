@@ -1164,3 +1164,19 @@ def test_inference_mode_and_threads():
     assert not errors
     for outs, x in zip(got, want):
         assert all(torch.equal(a, b) for one in outs for a, b in zip(one, x))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d,batch,width", [(32, 8, 128, 1, 128), (32, 8, 128, 1, 129), (32, 8, 128, 32, 230), (32, 8, 128, 32, 231), (14, 2, 64, 1, 215), (14, 2, 64, 1, 216),
+                                                  (71, 1, 128, 3, 24), (71, 1, 128, 3, 25), (2, 2, 64, 1, 315), (2, 2, 64, 2, 316), (256, 256, 64, 1, 566), (256, 256, 64, 1, 567)])
+def test_sparse_decode_on_both_sides_of_one_launch_or_two(hq, hkv, d, batch, width):
+    """Tables of widths where scoring and choosing become two launches, with the same sequences."""
+    lengths = [16 * (width if hkv < 99 else 60) - 3 - 16 * b for b in range(min(batch, 3))] + [100] * (batch - 3)
+    s = _Setup(lengths, hkv, d, 16, BF16, width)
+    if s.table.shape[1] < width:
+        s.table = torch.cat((s.table, torch.full((batch, width - s.table.shape[1]), -1, dtype=torch.int32, device="cuda")), 1)
+    assert s.table.shape[1] == width
+    q = s.queries(hq)
+    out, pages = _ops().paged_sparse_decode_attention(s.cache, q, s.table, s.lengths, 11, 1, 2)
+    assert torch.equal(pages, _chosen(q, s, 11, 1, 2))
+    _close(out, q, s, d ** -0.5, pages)
