@@ -83,14 +83,14 @@ def _apart(a, b, distance):
 
 class PagedCache:
     """Keys and values in pages: ``keys``, ``values`` ``[n_pages, n_kv_heads, page_size, head_dim]`` (bf16 or fp16 on one GPU, rows contiguous on
-    16-byte boundaries, the other strides those of any part or transposition of a tensor, no two places the same memory) and, for sparse steps, ``bounds`` ``[n_pages, n_kv_heads, 2, head_dim]`` (contiguous): the
-    smallest and the largest value of each channel over a page's keys, which :func:`append_to_pages` sets with a page's first key and widens with the
+    16-byte boundaries, the other strides free; to be appended to, those of any part or transposition of a tensor, no two places the same memory) and, for
+    sparse steps, ``bounds`` ``[n_pages, n_kv_heads, 2, head_dim]`` (contiguous): the smallest and the largest value of each channel over a page's keys, which :func:`append_to_pages` sets with a page's first key and widens with the
     others (keys that are taken back by a smaller length stay in them until the first is stored again; whoever copies pages copies their bounds).  The contents of pages that no table names
     do not matter.  The tensors stay the cache's own for as long as it is used: their contents may change, their memory may not, and a cache gets no others.  After
     ``cache.keys.data = ...`` or a ``resize_`` that moves them calls are refused."""
 
     __slots__ = ("keys", "values", "bounds", "dtype", "device", "index", "n_pages", "n_kv_heads", "page_size", "head_dim", "_struct", "_address",
-                 "_addresses", "_pointers", "_memory")
+                 "_addresses", "_pointers", "_apart", "_memory")
 
     def __init__(self, keys: torch.Tensor, values: torch.Tensor, bounds: Optional[torch.Tensor] = None):
         tensors = (keys, values) if bounds is None else (keys, values, bounds)
@@ -104,18 +104,20 @@ class PagedCache:
                     f"not {tuple(keys.shape)} and {tuple(values.shape)}")
         for t in (keys, values):
             sp, sh, sn, sd = t.stride()
-            if sd != 1 or (sp | sh | sn) & 7 or t.data_ptr() & 15 or not d <= sn <= 1 << 14 or not _own_places(_dims(t)):
+            if sd != 1 or (sp | sh | sn) & 7 or t.data_ptr() & 15 or not d <= sn <= 1 << 14 or (not sp and n_pages > 1) or (not sh and kv_heads > 1):
                 _refuse("the rows of keys and values must be contiguous, begin on 16-byte boundaries and lie at most 16384 elements apart, and no two share memory")
         if bounds is not None and (bounds.shape != (n_pages, kv_heads, 2, d) or not bounds.is_contiguous() or bounds.data_ptr() & 15):
             _refuse(f"bounds must be a contiguous tensor {(n_pages, kv_heads, 2, d)}, not {tuple(bounds.shape)}")
-        if any(not _apart(_dims(x), _dims(y), (y.data_ptr() - x.data_ptr()) // 2) for i, x in enumerate(tensors) for y in tensors[i + 1:]):
-            _refuse("keys, values and bounds must not share memory (parts of one tensor that lie between each other need the same strides)")
+        # (reading does not mind; what is written twice at once would be anything)
+        dims = [_dims(t) for t in tensors]
+        apart = all(map(_own_places, dims)) and all(_apart(dims[i], dims[j], (tensors[j].data_ptr() - tensors[i].data_ptr()) // 2)
+                                                    for i in range(len(dims)) for j in range(i + 1, len(dims)))
         # (what the C interface is told of the cache, once: 13 arguments fewer in each call)
         struct = _hip.PagedCacheStruct(*_hip.t3(keys), *_hip.t3(values), None if bounds is None else bounds.data_ptr(), n_pages, kv_heads, page_size, d,
                                        _hip.dtype_code(keys))
         addresses = (keys.data_ptr, values.data_ptr, int if bounds is None else bounds.data_ptr)
         for name, value in zip(self.__slots__, (keys, values, bounds, keys.dtype, keys.device, keys.get_device(), n_pages, kv_heads, page_size, d, struct,
-                                                ctypes.addressof(struct), addresses, tuple(f() for f in addresses),
+                                                ctypes.addressof(struct), addresses, tuple(f() for f in addresses), apart,
                                                 # (what the struct points to lives as long as the cache, also if a tensor is given other memory)
                                                 tuple(t.detach() for t in tensors))):
             object.__setattr__(self, name, value)
@@ -161,9 +163,12 @@ def _plain(cache, *tensors):
     if not _called_plainly():
         _refuse("these operators cannot be traced, compiled, vmapped or watched by a mode")
     if torch.is_grad_enabled():
-        for t in tensors:
-            if getattr(t, "requires_grad", False):  # (what is no tensor is refused where its type is looked at)
-                _refuse("these operators have no gradients: detach their inputs or call them under torch.no_grad()")
+        try:
+            for t in tensors:
+                if t is not None and t.requires_grad:
+                    _refuse("these operators have no gradients: detach their inputs or call them under torch.no_grad()")
+        except AttributeError:
+            pass  # (what is no tensor is refused where its type is looked at)
 
 
 def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tensor],
@@ -183,6 +188,8 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
     outside the pool: their rows of ``out`` stay as they are (undefined in a new one).  Two sequences must not append to one page: the result is then one's or a mixture.
     ``k`` and ``v`` must not lie in the pages that are appended to."""
     _plain(cache, q, k, v, cos, sin, out)
+    if not cache._apart:
+        _refuse("keys, values and bounds that share memory cannot be appended to (parts of one tensor that lie between each other need the same strides)")
     k_args, (n, _, _) = _rows(k, "k", cache, cache.n_kv_heads)
     v_args, (n_values, _, _) = _rows(v, "v", cache, cache.n_kv_heads)
     tables, batch, most = cache._tables(page_table, lengths)
@@ -194,7 +201,10 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
             _refuse("cos and sin come together, and queries need them")
         angles, n_positions, q_args, heads = (0, 0, 0), 0, (0,) * 6, 0
     else:
-        strides = cos.stride() if type(cos) in _TYPES else None
+        try:
+            strides = cos.stride()
+        except AttributeError:
+            strides = None
         for t in (cos, sin):
             if type(t) not in _TYPES or t.dtype != _FLOAT32 or t.get_device() != cache.index or t.dim() != 2 or t.shape != cos.shape or t.stride() != strides:
                 _refuse("cos and sin must be float32 tensors [positions, D / 2] on the cache's device, laid out alike")

@@ -877,32 +877,40 @@ def test_a_cache_whose_tensors_get_other_memory_is_refused(name):
 
 
 @pytest.mark.gpu
-def test_memory_that_is_shared_is_refused():
-    """Rows of one tensor that overlap without a stride of 0, tensors that overlap each other, outputs whose rows do: nothing is launched."""
+def test_memory_that_is_shared_is_not_written():
+    """A cache whose rows overlap without a stride of 0, or whose tensors do, is read and not appended to; outputs whose rows overlap are refused."""
     from anchor_attn.src.ops import _hip
     ops = _ops()
     z = lambda *shape: torch.zeros(shape, dtype=BF16, device="cuda")  # noqa: E731
-    pool, other = z(1 << 16), z(5, 2, 16, 64)
+    pool, other = torch.randn(1 << 16, device="cuda").to(BF16), torch.randn(5, 2, 16, 64, device="cuda").to(BF16)
     dense = (2 * 16 * 64, 16 * 64, 64, 1)
     at = lambda begin, strides: pool.as_strided((5, 2, 16, 64), strides, begin)  # noqa: E731
+    table, lengths = torch.tensor([[3, 1], [0, 2], [4, 4]], dtype=torch.int32, device="cuda"), torch.tensor([20, 32, 17], dtype=torch.int32, device="cuda")
+    q, k, starts = torch.randn(3, 4, 64, device="cuda").to(BF16), z(3, 2, 64), torch.arange(4, dtype=torch.int32, device="cuda")
+    caches = []
     for strides in ((1024, 1024, 64, 1), (2048, 512, 64, 1), (8, 1024, 64, 1), (2040, 1024, 64, 1), (1024, 64, 64, 1), (64, 1024, 64, 1)):
-        for keys, values in ((at(0, strides), other), (other, at(0, strides))):
-            with pytest.raises(_hip.AnchorAttnHipError, match="no two share memory"):
-                ops.PagedCache(keys, values)
-    for keys, values, bounds in ((other, other, None), (at(0, dense), at(0, dense), None), (at(0, dense), at(9 * 1024, dense), None), (at(9 * 1024, dense), at(0, dense), None),
-                                 (at(0, dense), at(10240 - 8, dense), None), (at(0, (4096, 1024, 64, 1)), at(2040, (4096, 1024, 64, 1)), None),
-                                 (at(0, (4096, 1024, 64, 1)), at(1024, (4096, 1024, 64, 1)), None), (at(0, (4096, 1024, 64, 1)), at(2048, (4096, 2048, 64, 1)), None),
-                                 (at(0, dense), other, pool[8192:8192 + 5 * 256].view(5, 2, 2, 64)), (other, at(512, dense), pool[:1280].view(5, 2, 2, 64))):
-        with pytest.raises(_hip.AnchorAttnHipError, match="must not share memory"):
-            ops.PagedCache(keys, values, bounds)
+        caches += [(at(0, strides), other, None), (other, at(0, strides), None)]
+    caches += [(other, other, None), (at(0, dense), at(0, dense), None), (at(0, dense), at(9 * 1024, dense), None), (at(9 * 1024, dense), at(0, dense), None),
+               (at(0, dense), at(10240 - 8, dense), None), (at(0, (4096, 1024, 64, 1)), at(2040, (4096, 1024, 64, 1)), None),
+               (at(0, (4096, 1024, 64, 1)), at(1024, (4096, 1024, 64, 1)), None), (at(0, (4096, 1024, 64, 1)), at(2048, (4096, 2048, 64, 1)), None),
+               (at(0, dense), other, pool[8192:8192 + 5 * 256].view(5, 2, 2, 64)), (other, at(512, dense), pool[:1280].view(5, 2, 2, 64))]
+    for keys, values, bounds in caches:
+        cache = ops.PagedCache(keys, values, bounds)
+        before = pool.clone()
+        for given in (starts, None):
+            with pytest.raises(_hip.AnchorAttnHipError, match="cannot be appended to"):
+                ops.append_to_pages(cache, None, k, k, None, None, table, lengths, given)
+        apart = ops.PagedCache(keys.clone().contiguous(), values.clone().contiguous(), None if bounds is None else bounds.clone())
+        assert torch.equal(ops.paged_decode_attention(cache, q, table, lengths), ops.paged_decode_attention(apart, q, table, lengths))
+        assert torch.equal(pool, before)
     cache = ops.PagedCache(z(5, 2, 16, 64), z(5, 2, 16, 64))
-    table, lengths = torch.zeros(3, 2, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    ops.append_to_pages(cache, None, k, k, None, None, table, lengths, starts)
     for strides in ((64, 64, 1), (8, 256, 1), (256, 8, 1), (128, 64, 1), (248, 64, 1), (64, 128, 1), (64, 184, 1)):
         with pytest.raises(_hip.AnchorAttnHipError, match="same memory"):
-            ops.paged_decode_attention(cache, z(3, 4, 64), table, lengths, out=pool.as_strided((3, 4, 64), strides))
+            ops.paged_decode_attention(cache, q, table, lengths, out=pool.as_strided((3, 4, 64), strides))
     for strides in ((256, 64, 1), (64, 192, 1), (1024, 72, 1), (72, 1024, 1)):
         out = pool.as_strided((3, 4, 64), strides)
-        assert ops.paged_decode_attention(cache, z(3, 4, 64), table, lengths, out=out) is out
+        assert ops.paged_decode_attention(cache, q, table, lengths, out=out) is out
 
 
 @pytest.mark.gpu
