@@ -186,7 +186,7 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
 
     Tokens without a place are left out - rows behind the last sequence, a length of 0, a position that ``cos`` or the table does not reach, a page
     outside the pool: their rows of ``out`` stay as they are (undefined in a new one).  Two sequences must not append to one page: the result is then one's or a mixture.
-    ``k`` and ``v`` must not lie in the pages that are appended to."""
+    ``k`` and ``v`` must not lie in the pages that are appended to.  A call has fewer than 2^23 rows of keys (tokens times KV heads)."""
     _plain(cache, q, k, v, cos, sin, out)
     if not cache._apart:
         _refuse("keys, values and bounds that share memory cannot be appended to (parts of one tensor that lie between each other need the same strides)")

@@ -17,9 +17,9 @@
 // costs as much as that of the output.  There is one set of registers for a tile; its keys are requested anew as soon as the scores have read them, its values after
 // the last product, so that loads are always in flight.
 //
-// Measured (bf16 unless said): 32 sequences of 500 to 16000 keys, 32/8 heads of 128 109 us, of which 4.8 the join: 5.7 TB/s while it reads, where a copy of that
-// size reaches 5.2 to 5.4; 2 of 131071, 28/4 heads of 128, fp16 100 us, 5.6 TB/s; one of 33001, 32/8 of 128 31.7 us, of which about 4 pass before the first
-// tile has come (lengths, table, rows, one after the other), 1 at the end and 4 in the join; one of 300, 14/2 of 64 7.2 us, nothing but such chains.  What is
+// Measured (bf16 unless said): 32 sequences of 500 to 16000 keys, 32/8 heads of 128 108 us, of which 4.8 the join: 5.7 TB/s while it reads, where a copy of that
+// size reaches 5.2 to 5.4; 2 of 131071, 28/4 heads of 128, fp16 99 us, 5.6 TB/s; one of 33001, 32/8 of 128 31.2 us, of which about 4 pass before the first
+// tile has come (lengths, table, rows, one after the other), 1 at the end and 4 in the join; one of 300, 14/2 of 64 7.4 us, nothing but such chains.  What is
 // executed before the first load counts there: a place is looked for only where it is not in the unit of the one before.
 #include "aa_kernels.h"
 #include "aa_nonfinite.h"
@@ -32,24 +32,26 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kCols = 16;       // columns of a unit: heads of the group
 constexpr int kTile = 32;       // keys of a tile
-// What a unit costs beside its tiles, in tiles.  (128 sequences of 20 to 1200 keys, 32/8 heads of 64: 0 30.1 us, 3 24.6, 6 24.9; 32 of 500 to 16000, 32/8 of 128:
-// 114, 110.8, 112.2.)
+// What a unit costs beside its tiles, in tiles.  (128 sequences of 20 to 1200 keys, 32/8 heads of 64: 0 28.5 us, 3 21.7, 6 23.1; 32 of 500 to 16000, 32/8 of 128:
+// 111, 107.7, 110.)
 constexpr int kOver = 3;
-// Where the table has room for that many tiles of a sequence at most, units are not cut between work-groups and nothing is joined.  (One sequence, cut and joined or not:
-// 300 keys, 14/2 heads of 64, 14.9 and 10.3 us, 1500 keys 13.6 and 12.4, 1780 13.4 and 13.8; 760 keys, 32/8 of 128, 13.8 and 11.8, 890 14.1 and 12.8, 1200 14.1 and 15.9;
-// 32 of 200 to 890 18.1 and 15.7.)  Many units keep all work-groups busy for longer than a join takes, and uncut ones of different lengths do so less evenly: 128
-// sequences of 1 to 1500 keys, 32/8 of 64, 19.3 and 21.0, of 1 to 890, 32/8 of 128, 20.8 and 21.9.
+// Where the table has room for that many tiles of a sequence at most, units are not cut between work-groups and nothing is joined.  (By the table's room, since the host knows
+// no lengths: the same 300 keys cost a step with a join in a table for more.  One sequence, cut and joined or not: 300 keys, 14/2 heads of 64, 14.0 and 10.1 us, 1500 keys 14.4
+// and 12.8, 1780 14.6 and 14.1; 760 keys, 32/8 of 128, 14.4 and 11.9, 890 14.5 and 12.7, 1200 14.2 and 15.8; 32 of 200 to 890 17.5 and 15.9.)  Many units keep all
+// work-groups busy for longer than a join takes, and uncut ones of different lengths do so less evenly: 128 sequences of 1 to 1500 keys, 32/8 of 64, 19.2 and 20.8, of 1 to
+// 890, 32/8 of 128, 20.8 and 22.2.
 template <int D> constexpr int kWhole = 28;
 template <> constexpr int kWhole<64> = 48;
 constexpr int kMany = 768, kWholeMany = 20;  // units, and what holds for more
-// Work-groups, one to a CU.  (512: 32 sequences of 500 to 16000 keys, 32/8 heads of 128 112 us instead of 110, 128 of 20 to 1200, 32/8 of 64 23.8 instead of 22.9.)
+// Work-groups, one to a CU.  (128: 32 sequences of 500 to 16000 keys, 32/8 heads of 128 124 us instead of 108, 128 of 20 to 1200, 32/8 of 64 27.9 instead of 21.7; 512, when these
+// were 110 and 22.9, 112 and 23.8.)
 constexpr int kShares = 256;
 constexpr int kSharesLog = 8;
-// Sequences that a lane counts where there are more than 64, so that 256 are one scan.  (1: 256 of 1 to 800 keys, 14/2 heads of 64, 17.4 us instead of 16.5; 1000 of 1 to 200, 32/8 of 64, 45.7
-// instead of 40.4; up to 128 the same.)
+// Sequences that a lane counts where there are more than 64, so that 256 are one scan.  (1: 256 of 1 to 800 keys, 14/2 heads of 64, 14.6 us instead of 12.2; 1000 of 1 to 200, 32/8 of 64, 49.4
+// instead of 39.8; 128 of 20 to 1200 23.0 instead of 21.7.)
 constexpr int kPerLane = 4, kPerLaneLog = 2;
 // Tiles of a share at least: fewer work-groups leave fewer parts to join, and each has longer to go.  (64 pages of 64 of one sequence, 32/8 heads of 128, chosen and
-// read: 4 24.4 us, 8 24.4, 16 26.7.)
+// read: 4 22.2 us, 8 22.2, 16 24.4.)
 constexpr int kLeast = 8;
 
 template <typename T> __device__ __forceinline__ floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c);
@@ -556,7 +558,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
 }
 
 // Joins the parts of a column whose unit begins in share blockIdx.x and ends in another: the weights first, then groups of D / 4 lanes add up
-// every so many parts.  Few bytes; the launch and three loads one after the other take 3.2 to 5 us, which a step pays whether or not a unit was cut, since the
+// every so many parts.  Few bytes; the launch and three loads one after the other take 3 to 5 us, which a step pays whether or not a unit was cut, since the
 // host does not know the lengths.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArgs p) {

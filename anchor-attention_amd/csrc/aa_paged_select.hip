@@ -1,14 +1,14 @@
 // Which pages of a cache a sparse decode step reads, on gfx950: the scores of the pages' bounds and the largest of them.
 //
-// A score is defined by a float64 sum, so that the chosen pages do not depend on its order: products of two 16-bit numbers are exact (in float32 those of fp16, in
-// float64 those of bf16), their sum is formed in float64 and rounded once.  A lane has 8 channels of 4 pages, so a page is 8 or 16 lanes'; their sums are exchanged inside rows of
+// A score is defined by a float64 sum, so that the chosen pages do not depend on its order: products of two 16-bit numbers are exact (in float32 those of fp16 and nearly all of
+// bf16), their sum is formed in float64 and rounded once.  A lane has 8 channels of 4 pages, so a page is 8 or 16 lanes'; their sums are exchanged inside rows of
 // lanes so that each lane ends with one page's.  With many pages conversions and additions in float64 bound it: 16 sequences of 6000 to 60000 keys in pages of 16,
-// 32/8 heads of 64, fp16 16.9 us for 49 MB of bounds, which take 9.4 to read; one sequence of 131072 keys in pages of 64, 32/8 of 128 5.8 us, 8 MB.  (Choosing the head that
-// counts by sums in float32 and summing only that one's in float64 where no other is near was slower, 23 and 6.4 us: twice the exchanges between lanes, and a
+// 32/8 heads of 64, fp16 17.5 us for 49 MB of bounds, which take 9.4 to read; one sequence of 131072 keys in pages of 64, 32/8 of 128 5.8 us, 8 MB.  (Choosing the head that
+// counts by sums in float32 and summing only that one's in float64 where no other is near was slower, 23 and 6.4 us against 18.5 and 5.7: twice the exchanges between lanes, and a
 // wave nearly always has a page where two heads are near.  So were bounds kept in float64, two products with the positive and the negative part of a query, 21: 200
 // registers leave two waves to a SIMD.)
 //
-// Choosing is latency (6.0 us for 2048 pages of one sequence, 7.5 for 8192, 18 for 25000; 8.4 with the scores, for 132 pages): a work-group per (sequence, KV head)
+// Choosing is latency (6.0 us for 2048 pages of one sequence, 7.5 for 8192, 18 for 25000; 8.5 with the scores, for 132 pages): a work-group per (sequence, KV head)
 // finds what the wanted number of scores reaches by histograms of 256 equal ranges of the numbers' order, each inside the range of the last one that holds it; the
 // first spans the smallest to the largest score, so that two or three do, whatever the scores' exponents (at most four).  Every wave reads the bins for itself,
 // which leaves one barrier for each histogram.  Integer work: the order in which counts are added does not matter.  The code is kept short, since most of it runs
@@ -19,7 +19,7 @@
 namespace aa {
 
 // Pages of a lane: several share a head's queries and their sums' exchange, one leaves a wave soonest.
-// (2 in the scores' launch: the 16 sequences above 53 us a step instead of 51.5.)
+// (1 in the scores' launch: the 16 sequences above 46.2 us a step instead of 43.1.)
 constexpr int kAbreast = 4, kAbreastFused = 1;
 constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
 constexpr int kFused = 1024;       // a table of at most that many pages is scored and chosen from by one launch
@@ -31,7 +31,7 @@ constexpr int kFused = 1024;       // a table of at most that many pages is scor
 constexpr int kPerPage = 12, kFusedWork = 256 * 1024, kFusedWorkMany = 460 * 1024, kManyUnits = 256;
 constexpr int kInLds = 32768;      // the scores of at most that many pages are kept in LDS
 // Pages that a thread of the choosing work-group looks at together, side by side: 4, and 1 in tables of at most kOnes pages, where the other threads would have
-// nothing to do.  (Steps of one sequence, 32/8 heads of 128: 8192 pages one 36.0 us, four 32.0; 1875 pages 21.6 and 21.8, 469 20.5 and 21.5.)
+// nothing to do.  (Steps of one sequence, 32/8 heads of 128: 8192 pages one 34.6 us, four 29.8; 1875 pages the same, 469 20.5 and 21.5.)
 constexpr int kItem = 4, kOnes = 2048;
 // ITEM numbers from p on
 template <int ITEM, typename X>
@@ -92,7 +92,7 @@ struct Products {
   }
 };
 // A product of two fp16 numbers is exact in float32; an instruction multiplies two of them into one, and two bounds are chosen at once by their queries' signs, for which -0 becomes 0
-// (16 sequences of 6000 to 60000 keys in pages of 16: 16.9 us, with conversions as in bf16 18.5).
+// (16 sequences of 6000 to 60000 keys in pages of 16: 43.0 us a step, with conversions as in bf16 44.7).
 template <int N>
 struct Products<F16, N, false> {
   static constexpr bool kMayLeave = false;
@@ -452,7 +452,7 @@ static void launch_paged_select_for(const PagedSelectArgs& a, hipStream_t stream
     hipLaunchKernelGGL((paged_choose_kernel<T, D, 0, 1>), units, dim3(kChooseThreads), 4 * paged_score_pitch(a.max_pages), stream, a);
     return;
   }
-  // (some four thousand work-groups, however long the table is and however short the sequences: the step above with 2560 52.8 us, with 1024 57.7)
+  // (some four thousand work-groups, however long the table is and however short the sequences: the step above 43.1 us, with 2560 43.6, with 1024 46.5)
   const int chunks = (a.max_pages + Scores<T, D, kAbreast>::kPages - 1) / Scores<T, D, kAbreast>::kPages, fours = (a.n_kv_heads + 3) / 4;
   const int64_t n = (int64_t)fours * a.batch;
   const int side = (int)((4096 + n - 1) / n);

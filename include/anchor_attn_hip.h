@@ -274,14 +274,15 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
  * q must be NULL and n_q_heads 0.  A page's bounds are set by its first key and widened by the others; those of
  * keys that were taken back (a smaller length) stay until the page's first key is stored again.  A token that has no place - behind the last
  * sequence, at a position below 0, in no row of cos and sin, behind the table or in no page of the pool - is left out: nothing is written for it.
+ * n_tokens * n_kv_heads is below 2^23.
  * starts[0] may lie below 0 and starts[batch] behind n_tokens: the tokens from 0 to n_tokens - 1 are appended, each where it belongs.
  * q, k, v, q_out: [n_tokens, heads, head_dim] with strides of token and head (_st, _sh).  Two tokens for one place, or of two sequences for one page, give one or a
  * mixture of both.
  *
  * aa_paged_decode_fwd: out[b, h] = softmax(q[b, h] . keys * sm_scale) values over the keys 0 .. lengths[b] - 1 of sequence b; a sequence of none gives 0,
  * one whose scores are all minus infinity NaN, as the quotient has it.
- * q, out: [batch, n_q_heads, head_dim] with strides of sequence and head; out may be q.  sm_scale is positive and below 2.3e38.  workspace: aa_paged_decode_workspace_bytes() bytes of device scratch, which
- * may be none (contents undefined afterwards).
+ * q, out: [batch, n_q_heads, head_dim] with strides of sequence and head; out may be q.  sm_scale is positive and below 2.3e38.
+ * workspace: aa_paged_decode_workspace_bytes() bytes of device scratch, which may be none (contents undefined afterwards).
  *
  * aa_paged_sparse_decode_fwd: the same over n_chosen pages for each sequence and KV head, or all where the sequence has no more: its first n_first, its last
  * n_last (at least 1) and those of the others whose score is largest, the lower page first among equal ones.  The score is the largest over the heads of the
