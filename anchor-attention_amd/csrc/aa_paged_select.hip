@@ -62,7 +62,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // Bounds of 8 channels of N pages, and sums of their products with queries in float64.
 //
 // WIDE: products in float64 too.  bf16 has the exponents of float32, in which a product may overflow, or lose bits below 2^-126; those of fp16 do not.  bf16 products are
-// formed in float32 all the same, in a quarter less time (32/8 heads of 64, 256 pages scored and chosen from in one launch 17.5 us a step instead of 18.1), and once more
+// formed in float32 all the same, which is sooner (32/8 heads of 64, 256 pages scored and chosen from in one launch 17.5 us a step instead of 18.1), and once more
 // in float64 where the sum shows that this may have counted: one that overflowed leaves an infinity or NaN, and 128 that lost 2^-150 each are off by
 // 2^-143, less than a float64 sum's own rounding of what is 2^-80 or larger.
 template <typename T, int N, bool WIDE = false>
