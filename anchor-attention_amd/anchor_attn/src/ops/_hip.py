@@ -30,6 +30,7 @@ class PagedCacheStruct(ctypes.Structure):
 # ``aa_paged_tokens`` and ``aa_paged_step`` (packed: a call with 26 arguments costs 2.2 us of ctypes' conversions, one with a packed struct 0.5)
 PAGED_TOKENS = struct.Struct("@" + "Pqq" * 4 + "PPqPqPP" + "5i0q")
 PAGED_STEP = struct.Struct("@" + "Pqq" * 2 + "PqPPNP" + "6if0q")
+PAGED_MORE = struct.Struct("@PPPqqPPf0q")  # aa_paged_more
 
 
 class AnchorAttnHipError(RuntimeError):
@@ -71,6 +72,7 @@ _SIGNATURES = {
     "aa_dense_rows_fwd": (c_int, _T3 * 4 + [c_void_p, c_int64, c_int64] + [c_void_p, c_size_t] + [c_int] * 7 + [c_float, c_int, c_void_p]),
     # (the address of a PagedCacheStruct, and PAGED_TOKENS or PAGED_STEP)
     "aa_paged_append": (c_int, [c_void_p, c_char_p, c_void_p]),
+    "aa_paged_append_more": (c_int, [c_void_p, c_char_p, c_char_p, c_void_p]),
     "aa_paged_decode_workspace_bytes": (c_size_t, [c_int] * 6),
     "aa_paged_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p]),
     "aa_paged_sparse_workspace_bytes": (c_size_t, [c_int] * 7),

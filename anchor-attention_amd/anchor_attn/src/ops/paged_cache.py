@@ -87,12 +87,13 @@ class PagedCache:
     sparse steps, ``bounds`` ``[n_pages, n_kv_heads, 2, head_dim]`` (contiguous): the smallest and the largest value of each channel over a page's keys, which :func:`append_to_pages` sets with a page's first key and widens with the
     others (keys that are taken back by a smaller length stay in them until the first is stored again; whoever copies pages copies their bounds).  The contents of pages that no table names
     do not matter.  The tensors stay the cache's own for as long as it is used: their contents may change, their memory may not, and a cache gets no others.  After
-    ``cache.keys.data = ...`` or a ``resize_`` that moves them calls are refused."""
+    ``cache.keys.data = ...`` or a ``resize_`` that moves them calls are refused.  ``weights``, optional, float32 ``[n_pages, n_kv_heads, page_size]`` (contiguous): how
+    much attention each key has had, 0 when it is appended, counted by :func:`paged_weighing_decode_attention`, read by :func:`evict_from_pages`."""
 
-    __slots__ = ("keys", "values", "bounds", "dtype", "device", "index", "n_pages", "n_kv_heads", "page_size", "head_dim", "_struct", "_address",
-                 "_addresses", "_pointers", "_apart", "_memory")
+    __slots__ = ("keys", "values", "bounds", "weights", "dtype", "device", "index", "n_pages", "n_kv_heads", "page_size", "head_dim", "_struct", "_address",
+                 "_addresses", "_pointers", "_apart", "_memory", "_weights")
 
-    def __init__(self, keys: torch.Tensor, values: torch.Tensor, bounds: Optional[torch.Tensor] = None):
+    def __init__(self, keys: torch.Tensor, values: torch.Tensor, bounds: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None):
         tensors = (keys, values) if bounds is None else (keys, values, bounds)
         if any(type(t) not in _TYPES or t.dim() != 4 or t.dtype != keys.dtype or t.device != keys.device or not t.is_cuda for t in tensors):
             _refuse("keys, values and bounds must be tensors of four dimensions, one type and one GPU")
@@ -108,6 +109,14 @@ class PagedCache:
                 _refuse("the rows of keys and values must be contiguous, begin on 16-byte boundaries and lie at most 16384 elements apart, and no two share memory")
         if bounds is not None and (bounds.shape != (n_pages, kv_heads, 2, d) or not bounds.is_contiguous() or bounds.data_ptr() & 15):
             _refuse(f"bounds must be a contiguous tensor {(n_pages, kv_heads, 2, d)}, not {tuple(bounds.shape)}")
+        if weights is not None:
+            if type(weights) not in _TYPES or weights.dtype != _FLOAT32 or weights.device != keys.device or weights.shape != (n_pages, kv_heads, page_size):
+                _refuse(f"weights must be a float32 tensor {(n_pages, kv_heads, page_size)} on the cache's device")
+            if not weights.is_contiguous() or weights.data_ptr() & 15 or weights.requires_grad:
+                _refuse("weights must be contiguous on a 16-byte boundary and need no gradients")
+            begin, end = weights.data_ptr(), weights.data_ptr() + 4 * weights.numel()
+            if any(begin < t.data_ptr() + 2 * _extent(_dims(t)) and t.data_ptr() < end for t in tensors):
+                _refuse("weights must lie apart from keys, values and bounds")
         # (reading does not mind; what is written twice at once would be anything)
         dims = [_dims(t) for t in tensors]
         apart = all(map(_own_places, dims)) and all(_apart(dims[i], dims[j], (tensors[j].data_ptr() - tensors[i].data_ptr()) // 2)
@@ -116,23 +125,25 @@ class PagedCache:
         struct = _hip.PagedCacheStruct(*_hip.t3(keys), *_hip.t3(values), None if bounds is None else bounds.data_ptr(), n_pages, kv_heads, page_size, d,
                                        _hip.dtype_code(keys))
         addresses = (keys.data_ptr, values.data_ptr, int if bounds is None else bounds.data_ptr)
-        for name, value in zip(self.__slots__, (keys, values, bounds, keys.dtype, keys.device, keys.get_device(), n_pages, kv_heads, page_size, d, struct,
+        for name, value in zip(self.__slots__, (keys, values, bounds, weights, keys.dtype, keys.device, keys.get_device(), n_pages, kv_heads, page_size, d, struct,
                                                 ctypes.addressof(struct), addresses, tuple(f() for f in addresses), apart,
                                                 # (what the struct points to lives as long as the cache, also if a tensor is given other memory)
-                                                tuple(t.detach() for t in tensors))):
+                                                tuple(t.detach() for t in (*tensors, *(() if weights is None else (weights,)))),
+                                                0 if weights is None else weights.data_ptr())):
             object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value):
         raise AttributeError(f"a PagedCache does not change: {name}")
 
     def __reduce__(self):
-        return PagedCache, (self.keys, self.values, self.bounds)
+        return PagedCache, (self.keys, self.values, self.bounds, self.weights)
 
     @classmethod
-    def empty(cls, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, dtype=torch.bfloat16, device="cuda", bounds: bool = True):
+    def empty(cls, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, dtype=torch.bfloat16, device="cuda", bounds: bool = True, weights: bool = False):
         """A cache with new memory, whose contents are undefined until they are appended."""
         keys, values = (torch.empty(n_pages, n_kv_heads, page_size, head_dim, dtype=dtype, device=device) for _ in range(2))
-        return cls(keys, values, torch.empty(n_pages, n_kv_heads, 2, head_dim, dtype=dtype, device=device) if bounds else None)
+        return cls(keys, values, torch.empty(n_pages, n_kv_heads, 2, head_dim, dtype=dtype, device=device) if bounds else None,
+                   torch.empty(n_pages, n_kv_heads, page_size, dtype=torch.float32, device=device) if weights else None)
 
     def _tables(self, page_table, lengths):
         """Arguments of a page table and lengths, and the sequences and most pages they are for."""
@@ -144,15 +155,21 @@ class PagedCache:
             _refuse(f"{batch} sequences of up to {most} pages of {self.page_size} are not supported (at most 65535 sequences, 1048576 keys, at least one page)")
         return (table, page_table.stride(0), lengths_ptr), batch, most
 
-    def _launch(self, fn, packed):
+    def _weighed(self):
+        """``data_ptr`` of the weights; 0 without."""
+        if self.weights is not None and self.weights.data_ptr() != self._weights:
+            _refuse("a tensor of the cache has been given other memory, which a PagedCache does not follow: make a new one")
+        return self._weights
+
+    def _launch(self, fn, *packed):
         keys, values, bounds = self._addresses
         if (keys(), values(), bounds()) != self._pointers:
             _refuse("a tensor of the cache has been given other memory, which a PagedCache does not follow: make a new one")
         if self.index == torch.cuda.current_device():
-            rc = fn(self._address, packed, _raw_stream(self.index) if _raw_stream is not None else _stream())
+            rc = fn(self._address, *packed, _raw_stream(self.index) if _raw_stream is not None else _stream())
         else:
             with torch.cuda.device(self.device):
-                rc = fn(self._address, packed, _stream())
+                rc = fn(self._address, *packed, _stream())
         if rc:
             _hip.check(rc)
 
@@ -173,7 +190,8 @@ def _plain(cache, *tensors):
 
 def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tensor],
                     sin: Optional[torch.Tensor], page_table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None,
-                    out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                    out: Optional[torch.Tensor] = None, *, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, norm_eps: float = 1e-6,
+                    positions: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Appends new tokens to the cache and returns their rotated queries (in ``out``, if it is given; that may be ``q`` and otherwise shares no memory with
     the inputs).
 
@@ -186,8 +204,13 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
 
     Tokens without a place are left out - rows behind the last sequence, a length of 0, a position that ``cos`` or the table does not reach, a page
     outside the pool: their rows of ``out`` stay as they are (undefined in a new one).  Two sequences must not append to one page: the result is then one's or a mixture.
-    ``k`` and ``v`` must not lie in the pages that are appended to.  A call has fewer than 2^23 rows of keys (tokens times KV heads)."""
-    _plain(cache, q, k, v, cos, sin, out)
+    ``k`` and ``v`` must not lie in the pages that are appended to.  A call has fewer than 2^23 rows of keys (tokens times KV heads).
+
+    ``q_norm``, ``k_norm`` ``[D]`` of the cache's type (both, or ``k_norm`` where there are no queries): before it is rotated, each head ``x`` becomes
+    ``x / sqrt(mean(x^2) + norm_eps) * weight``, in float32 with one rounding after both.  ``positions`` int32 ``[batch]``: how many positions a sequence has had, where
+    that is more than its keys (:func:`evict_from_pages`): its last token is rotated by ``positions[b] - 1``; a sequence of fewer positions than keys is left out.
+    ``k_out`` ``[tokens, KV heads, D]``, which may be ``k``: the keys as they are stored, for the prompt's own attention.  The weights of new keys, in a cache that keeps them, become 0."""
+    _plain(cache, q, k, v, cos, sin, out, q_norm, k_norm, k_out)
     if not cache._apart:
         _refuse("keys, values and bounds that share memory cannot be appended to (parts of one tensor that lie between each other need the same strides)")
     k_args, (n, _, _) = _rows(k, "k", cache, cache.n_kv_heads)
@@ -222,7 +245,25 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
             if shape[0] != n:
                 _refuse(f"q has {shape[0]} tokens, k {n}")
             q_args = (*q_rows, *_out_rows(out, shape, cache)) if out is not None else (*q_rows, *_new_rows(out := torch.empty_like(q)))
-    if n and batch:
+    weights = cache._weighed()
+    more = None
+    if weights or not (q_norm is k_norm is positions is k_out is None):
+        if cos is None and not (k_norm is positions is k_out is None):
+            _refuse("norms, positions and rotated keys need cos and sin")
+        if (q_norm is None) != (k_norm is None or q is None):
+            _refuse("norms of queries and keys come together, that of keys alone where there are no queries")
+        norms = tuple(0 if t is None else _channels(t, name, cache) for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")))
+        try:
+            eps = float(norm_eps)
+        except (TypeError, ValueError):
+            eps = -1.0
+        if not 0 <= eps <= 1:
+            _refuse(f"norm_eps must be from 0 to 1, not {norm_eps}")
+        more = _hip.PAGED_MORE.pack(*norms, *((0, 0, 0) if k_out is None else _out_rows(k_out, k.shape, cache, "k_out")),
+                                    0 if positions is None else _indices(positions, "positions", cache, 1, batch), weights, eps)
+    if n and batch and more is not None:
+        cache._launch(_hip.lib().aa_paged_append_more, _hip.PAGED_TOKENS.pack(*q_args, *k_args, *v_args, *angles, *tables, starts_ptr, n_positions, batch, n, heads, most), more)
+    elif n and batch:
         cache._launch(_hip.lib().aa_paged_append, _hip.PAGED_TOKENS.pack(*q_args, *k_args, *v_args, *angles, *tables, starts_ptr, n_positions, batch, n, heads, most))
     return out
 
@@ -232,12 +273,19 @@ def _new_rows(t):
     return t.data_ptr(), st, sh
 
 
-def _out_rows(out, shape, cache):
-    rows, out_shape = _rows(out, "out", cache, shape[1])
+def _channels(t, name, cache):
+    """``data_ptr`` of a tensor ``[D]``."""
+    if type(t) not in _TYPES or t.dtype != cache.dtype or t.get_device() != cache.index or t.shape != (cache.head_dim,) or t.stride() != (1,) or t.data_ptr() & 15:
+        _refuse(f"{name} must be a contiguous tensor [head dimension] of the cache's type and device, on a 16-byte boundary")
+    return t.data_ptr()
+
+
+def _out_rows(out, shape, cache, name="out"):
+    rows, out_shape = _rows(out, name, cache, shape[1])
     n, h, d = shape
     _, st, sh = rows
     if out_shape != shape or not (((h == 1 or sh >= d) and (n < 2 or st >= (h - 1) * sh + d)) or ((n < 2 or st >= d) and (h == 1 or sh >= (n - 1) * st + d))):
-        _refuse("out must have the shape of q, and no two of its rows the same memory")
+        _refuse(f"{name} must have the shape of {'q' if name == 'out' else 'k'}, and no two of its rows the same memory")
     return rows
 
 

@@ -928,8 +928,7 @@ static int check_cache(const char* who, const aa_paged_cache* c, int batch, int 
 
 static int log2_of(int power) { return 31 - __builtin_clz((unsigned)power); }
 
-int aa_paged_append(const aa_paged_cache* cache, const aa_paged_tokens* t, void* stream) {
-  const char* who = "aa_paged_append";
+static int paged_append(const char* who, const aa_paged_cache* cache, const aa_paged_tokens* t, const aa_paged_more* more, void* stream) {
   int rc;
   if ((rc = check_given(t, who, "tokens")) || (rc = check_cache(who, cache, t->batch, t->n_q_heads, t->max_pages, t->page_table, t->lengths))) return rc;
   if (t->n_tokens <= 0 || t->n_tokens >= 1 << 24 || (int64_t)t->n_tokens * cache->n_kv_heads >= 1 << 23 || (t->starts == nullptr && t->n_tokens != t->batch)) {
@@ -958,8 +957,34 @@ int aa_paged_append(const aa_paged_cache* cache, const aa_paged_tokens* t, void*
                              (const uint16_t*)t->v, t->v_st, t->v_sh, t->cos, t->sin, t->cs_sn, t->n_positions, (uint16_t*)cache->keys, cache->kp_sp,
                              cache->kp_sh, cache->kp_sn, (uint16_t*)cache->values, cache->vp_sp, cache->vp_sh, cache->vp_sn, (uint16_t*)cache->bounds,
                              t->page_table, t->pt_sb, t->lengths, t->starts, t->batch, t->n_tokens, t->n_q_heads, cache->n_kv_heads, cache->head_dim,
-                             cache->n_pages, log2_of(cache->page_size), t->max_pages, cache->dtype, 0, 0};
+                             cache->n_pages, log2_of(cache->page_size), t->max_pages, cache->dtype, 0, 0, (const uint16_t*)more->q_norm,
+                             (const uint16_t*)more->k_norm, more->norm_eps, (uint16_t*)more->k_out, more->ko_st, more->ko_sh, more->positions, more->weights};
   return check_launch(launch_paged_append(a, (hipStream_t)stream), who);
+}
+
+int aa_paged_append(const aa_paged_cache* cache, const aa_paged_tokens* t, void* stream) {
+  const aa_paged_more none = {};
+  return paged_append("aa_paged_append", cache, t, &none, stream);
+}
+
+int aa_paged_append_more(const aa_paged_cache* cache, const aa_paged_tokens* t, const aa_paged_more* m, void* stream) {
+  const char* who = "aa_paged_append_more";
+  int rc;
+  if ((rc = check_given(t, who, "tokens")) || (rc = check_given(m, who, "more"))) return rc;
+  if ((t->cos == nullptr && (m->k_norm != nullptr || m->k_out != nullptr || m->positions != nullptr)) ||
+      (m->q_norm != nullptr) != (m->k_norm != nullptr && t->q != nullptr)) {
+    set_error("%s: norms, rotated keys and positions need cos and sin, and norms of queries and keys come together (without queries that of keys alone)", who);
+    return AA_EBADARG;
+  }
+  if (m->k_norm != nullptr && !(m->norm_eps >= 0.f && m->norm_eps <= 1.f)) {
+    set_error("%s: norm_eps %g must be from 0 to 1", who, (double)m->norm_eps);
+    return AA_EBADARG;
+  }
+  if ((m->q_norm != nullptr && (rc = check_ptr(m->q_norm, who, "q_norm"))) || (m->k_norm != nullptr && (rc = check_ptr(m->k_norm, who, "k_norm"))) ||
+      (m->k_out != nullptr && (rc = check_rows(m->k_out, m->ko_st, m->ko_sh, who, "k_out"))) ||
+      (m->positions != nullptr && (rc = check_words(m->positions, who, "positions"))) || (m->weights != nullptr && (rc = check_words(m->weights, who, "weights"))))
+    return rc;
+  return paged_append(who, cache, t, m, stream);
 }
 
 size_t aa_paged_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {

@@ -149,6 +149,11 @@ struct PagedAppendArgs {
   int batch, n_tokens, n_q_heads, n_kv_heads, head_dim, n_pages, page_log, max_pages;  // n_q_heads 0: no queries
   int dtype;
   int chunk, key_chunks;  // set by the launcher: tokens of a work-group of keys, and how many of these a KV head has
+  // optional: norms of queries and keys before they are rotated, the rotated keys once more, positions apart from lengths, weights of the keys, which begin at 0
+  const uint16_t* q_norm; const uint16_t* k_norm; float norm_eps;
+  uint16_t* k_out; int64_t ko_st, ko_sh;
+  const int32_t* positions;
+  float* weights;  // [n_pages, n_kv_heads, page size]
 };
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t stream);
 

@@ -27,12 +27,41 @@ __device__ __forceinline__ void store8(uint16_t* p, const int half, const Rows8&
 struct Angles {
   float4 cos[2], sin[2];
 };
-// turned by their angles: float32, one rounding
+// A norm's weights of these channels, and the norm: x * w / sqrt(mean of the head's x^2 + eps), float32.  A head is D / 16 neighbouring lanes', all of them active.
+struct Norm8 {
+  float first[8], second[8];
+};
 template <typename T>
-__device__ __forceinline__ Rows8 rotated(const Rows8& raw, const Angles& a) {
+__device__ __forceinline__ Norm8 norm_of(const uint16_t* weight, const int c, const int half) {
+  const Rows8 raw = load8(weight + 8 * c, half);
+  Norm8 w;
+  unpack8<T>(raw.first, w.first);
+  unpack8<T>(raw.second, w.second);
+  return w;
+}
+template <int PIECES>
+__device__ __forceinline__ void normalise(float (&x)[8], float (&y)[8], const Norm8& w, const float eps) {
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum += x[j] * x[j] + y[j] * y[j];
+  sum += __uint_as_float(dpp<kDppXor1>(__float_as_uint(sum)));
+  sum += __uint_as_float(dpp<kDppXor2>(__float_as_uint(sum)));
+  if (PIECES == 8) sum += __uint_as_float(dpp<kDppHalfMirror>(__float_as_uint(sum)));  // (the four lanes of either half have the same sum)
+  const float scale = rsqrtf(sum * (1.f / (16 * PIECES)) + eps);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    x[j] *= scale * w.first[j];
+    y[j] *= scale * w.second[j];
+  }
+}
+
+// turned by their angles, after a norm if there is one: float32, one rounding
+template <typename T, int PIECES>
+__device__ __forceinline__ Rows8 rotated(const Rows8& raw, const Angles& a, const Norm8* norm = nullptr, const float eps = 0.f) {
   float x[8], y[8];
   unpack8<T>(raw.first, x);
   unpack8<T>(raw.second, y);
+  if (norm != nullptr) normalise<PIECES>(x, y, *norm, eps);
   const float c[8] = {a.cos[0].x, a.cos[0].y, a.cos[0].z, a.cos[0].w, a.cos[1].x, a.cos[1].y, a.cos[1].z, a.cos[1].w};
   const float s[8] = {a.sin[0].x, a.sin[0].y, a.sin[0].z, a.sin[0].w, a.sin[1].x, a.sin[1].y, a.sin[1].z, a.sin[1].w};
 #pragma unroll
@@ -114,17 +143,21 @@ __device__ __forceinline__ uint32_t over_tokens(uint32_t x, F f) {
   return f(s[0], s[1]);
 }
 
-// Where a token goes: its position, the page of the pool and the row in it; not ok: nowhere.
+// Where a token goes: its place in the sequence, what its position is more than that, the page of the pool and the row in it; not ok: nowhere.
 struct Place {
   int64_t position;
+  int64_t shift;
   int at, slot;
   bool ok;
 };
 // token t of sequence b, whose tokens are those from begin to end; TABLE, a pointer to tables and lengths
-template <typename Words>
+template <bool MORE, typename Words>
 __device__ __forceinline__ Place place_of(const PagedAppendArgs& p, const Words* lengths, const Words* table, const int b, const int begin, const int end, const int t) {
-  Place x = {(int64_t)lengths[b] - end + t, 0, 0, false};
-  if (t < begin || t >= end || x.position < 0 || x.position >> p.page_log >= p.max_pages || (p.cos != nullptr && x.position >= p.n_positions)) return x;
+  Place x = {(int64_t)lengths[b] - end + t, 0, 0, 0, false};
+  if (MORE && p.positions != nullptr) x.shift = (int64_t)((const Words*)p.positions)[b] - lengths[b];
+  if (t < begin || t >= end || x.position < 0 || x.shift < 0 || x.position >> p.page_log >= p.max_pages ||
+      (p.cos != nullptr && x.position + x.shift >= p.n_positions))
+    return x;
   x.at = table[b * p.t_sb + (x.position >> p.page_log)];
   x.slot = (int)x.position & ((1 << p.page_log) - 1);
   x.ok = (uint32_t)x.at < (uint32_t)p.n_pages;
@@ -155,7 +188,7 @@ __device__ __forceinline__ Angles angles_of(const PagedAppendArgs& p, const int6
 }
 
 // Queries and values of the tokens from `first` on, one of each kPieces lanes.
-template <typename T, int D>
+template <typename T, int D, bool MORE>
 __device__ __forceinline__ void queries_and_values(const PagedAppendArgs& p, const int first, const int kvh) {
   constexpr int kPieces = D / 16, kInWave = 64 / kPieces;
   const int c = threadIdx.x % kPieces, group = p.n_q_heads / p.n_kv_heads;
@@ -179,11 +212,14 @@ __device__ __forceinline__ void queries_and_values(const PagedAppendArgs& p, con
     end = p.starts[b + 1];
   }
   if (t >= p.n_tokens) return;
-  const Place x = place_of(p, p.lengths, p.table, b, begin, end, t);
+  const Place x = place_of<MORE>(p, p.lengths, p.table, b, begin, end, t);
   if (!x.ok) return;
   const Rows8 v = load8(p.v + t * p.v_st + kvh * p.v_sh + 8 * c, D / 2);
   if (group > 0) {
-    const Angles a = angles_of(p, x.position, c);
+    const Angles a = angles_of(p, x.position + x.shift, c);
+    const bool normed = MORE && p.q_norm != nullptr;
+    Norm8 norm;
+    if (normed) norm = norm_of<T>(p.q_norm, c, D / 2);
     for (int h = 0; h < group; h += 4) {
       Rows8 q[4];
       const uint16_t* src = p.q + t * p.q_st + (int64_t)(kvh * group + h) * p.q_sh + 8 * c;
@@ -193,14 +229,14 @@ __device__ __forceinline__ void queries_and_values(const PagedAppendArgs& p, con
         if (h + j < group) q[j] = load8(src + j * p.q_sh, D / 2);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (h + j < group) store8(dst + j * p.qo_sh, D / 2, rotated<T>(q[j], a));
+        if (h + j < group) store8(dst + j * p.qo_sh, D / 2, normed ? rotated<T, kPieces>(q[j], a, &norm, p.norm_eps) : rotated<T, kPieces>(q[j], a));
     }
   }
   store8(p.values + x.at * p.vp_sp + kvh * p.vp_sh + x.slot * p.vp_sn + 8 * c, D / 2, v);
 }
 
 // Keys of the runs that begin among the `chunk` tokens from `first` on, and their pages' bounds.
-template <typename T, int D, int WAVES>
+template <typename T, int D, int WAVES, bool MORE>
 __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const int first, const int kvh, uint32_t (*red)[D / 16][16]) {
   constexpr int kPieces = D / 16;                  // lanes of a token
   constexpr int kInWave = 64 / kPieces;            // tokens of a wave
@@ -208,6 +244,9 @@ __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const 
   const int tid = threadIdx.x, lane = tid & 63, c = tid % kPieces, row = tid / kPieces;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), page_size = 1 << p.page_log;
   const const_i32 *lengths = (const_i32*)p.lengths, *starts = (const_i32*)p.starts, *table = (const_i32*)p.table;
+  const bool normed = MORE && p.k_norm != nullptr;
+  Norm8 norm;
+  if (normed) norm = norm_of<T>(p.k_norm, c, D / 2);
 
   for (int t = first; t < min(first + p.chunk, p.n_tokens);) {
     int b = t, begin = t, end = t + 1;
@@ -217,7 +256,7 @@ __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const 
       begin = starts[b];
       end = starts[b + 1];
     }
-    const Place x = place_of(p, lengths, table, b, begin, end, t);
+    const Place x = place_of<MORE>(p, lengths, table, b, begin, end, t);
     // the rest of the run; of tokens before the first position as many as there are
     int n = 1;
     if (t >= begin && t < end) n = x.position < 0 ? (int)min(-x.position, (int64_t)(end - t)) : min(min(end, p.n_tokens) - t, page_size - ((int)x.position & (page_size - 1)));
@@ -225,7 +264,7 @@ __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const 
     t += n;
     // (nowhere; the rest of a run that began among the tokens before, of which there are none before token 0, wherever the sequence begins)
     if (!x.ok || (t0 != max(begin, 0) && x.slot != 0)) continue;
-    if (p.cos != nullptr) n = (int)min((int64_t)n, p.n_positions - x.position);
+    if (p.cos != nullptr) n = (int)min((int64_t)n, p.n_positions - x.position - x.shift);
 
     uint16_t* bounds = p.bounds + ((int64_t)x.at * p.n_kv_heads + kvh) * 2 * D + 8 * c;
     Rows8 old[2];
@@ -238,7 +277,12 @@ __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const 
     own.clear();
     for (int i = row; i < n; i += kTokens) {
       Rows8 k = load8(p.k + (int64_t)(t0 + i) * p.k_st + kvh * p.k_sh + 8 * c, D / 2);
-      if (p.cos != nullptr) k = rotated<T>(k, angles_of(p, x.position + i, c));
+      if (p.cos != nullptr) {
+        const Angles a = angles_of(p, x.position + x.shift + i, c);
+        k = normed ? rotated<T, kPieces>(k, a, &norm, p.norm_eps) : rotated<T, kPieces>(k, a);
+      }
+      if (MORE && p.k_out != nullptr) store8(p.k_out + (int64_t)(t0 + i) * p.ko_st + kvh * p.ko_sh + 8 * c, D / 2, k);
+      if (MORE && p.weights != nullptr && c == 0) p.weights[(((int64_t)x.at * p.n_kv_heads + kvh) << p.page_log) + x.slot + i] = 0.f;
       store8(p.keys + x.at * p.kp_sp + kvh * p.kp_sh + (x.slot + i) * p.kp_sn + 8 * c, D / 2, k);
       uint32_t w[8];  // (of the keys as stored)
       words(k, w);
@@ -294,16 +338,16 @@ __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const 
 // 6001 tokens, 32/8 heads of 128 32.3 -> 29.7 us).  Turns are dealt out by a hash, since runs may begin every so many work-groups: 64 tokens of a sequence each and a
 // prompt of 2000 took 20.3 us in plain order, 15.8 so, 18.3 with the KV heads' work-groups spread over the XCDs.
 constexpr uint32_t kXcds = 8;
-template <typename T, int D, int WAVES>
+template <typename T, int D, int WAVES, bool MORE>
 __global__ void __launch_bounds__(64 * WAVES) paged_append_kernel(const PagedAppendArgs p) {
   __shared__ uint32_t red[WAVES > 1 ? WAVES - 1 : 1][D / 16][16];
   const uint32_t xcd = blockIdx.x % kXcds, of_xcd = blockIdx.x / kXcds, turn = of_xcd / p.n_kv_heads;
   const int kvh = of_xcd - turn * p.n_kv_heads, at = turn * kXcds + (xcd + (turn * 0x9e3779b1u >> 29)) % kXcds;
-  if (at < p.key_chunks) keys_and_bounds<T, D, WAVES>(p, at * p.chunk, kvh, red);
-  else queries_and_values<T, D>(p, (at - p.key_chunks) * (WAVES * 1024 / D), kvh);
+  if (at < p.key_chunks) keys_and_bounds<T, D, WAVES, MORE>(p, at * p.chunk, kvh, red);
+  else queries_and_values<T, D, MORE>(p, (at - p.key_chunks) * (WAVES * 1024 / D), kvh);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool MORE>
 static void launch_paged_append_for(PagedAppendArgs a, hipStream_t stream) {
   // Tokens of a work-group of keys: few, so that short runs do not queue up in one, but no fewer than make some thousand work-groups (prompts of 700 to 21000 tokens,
   // 32/8 heads of 128: 205 us, with 1 everywhere some 600; 200 sequences of a token, padded to 256: 14, with a page everywhere 109; 64 of a token and a prompt of 2000: 18, 122)
@@ -314,18 +358,24 @@ static void launch_paged_append_for(PagedAppendArgs a, hipStream_t stream) {
   const int waves = a.starts == nullptr ? 1 : (int)(page_size * (D / 16) / 64), w = waves <= 1 ? 1 : waves == 2 ? 2 : 4;
   const uint32_t chunks = a.key_chunks + (a.n_tokens + w * 1024 / D - 1) / (w * 1024 / D);
   const dim3 grid((chunks + kXcds - 1) / kXcds * kXcds * a.n_kv_heads);
-  if (w == 1) hipLaunchKernelGGL((paged_append_kernel<T, D, 1>), grid, dim3(64), 0, stream, a);
-  else if (w == 2) hipLaunchKernelGGL((paged_append_kernel<T, D, 2>), grid, dim3(128), 0, stream, a);
-  else hipLaunchKernelGGL((paged_append_kernel<T, D, 4>), grid, dim3(256), 0, stream, a);
+  if (w == 1) hipLaunchKernelGGL((paged_append_kernel<T, D, 1, MORE>), grid, dim3(64), 0, stream, a);
+  else if (w == 2) hipLaunchKernelGGL((paged_append_kernel<T, D, 2, MORE>), grid, dim3(128), 0, stream, a);
+  else hipLaunchKernelGGL((paged_append_kernel<T, D, 4, MORE>), grid, dim3(256), 0, stream, a);
+}
+
+template <typename T, int D>
+static void launch_paged_append_of(const PagedAppendArgs& a, hipStream_t stream) {
+  if (a.q_norm != nullptr || a.k_norm != nullptr || a.k_out != nullptr || a.positions != nullptr || a.weights != nullptr) launch_paged_append_for<T, D, true>(a, stream);
+  else launch_paged_append_for<T, D, false>(a, stream);
 }
 
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t stream) {
   if (a.head_dim == 128) {
-    if (a.dtype == 0) launch_paged_append_for<Bf16, 128>(a, stream);
-    else launch_paged_append_for<F16, 128>(a, stream);
+    if (a.dtype == 0) launch_paged_append_of<Bf16, 128>(a, stream);
+    else launch_paged_append_of<F16, 128>(a, stream);
   } else {
-    if (a.dtype == 0) launch_paged_append_for<Bf16, 64>(a, stream);
-    else launch_paged_append_for<F16, 64>(a, stream);
+    if (a.dtype == 0) launch_paged_append_of<Bf16, 64>(a, stream);
+    else launch_paged_append_of<F16, 64>(a, stream);
   }
   return hipGetLastError();
 }

@@ -279,6 +279,12 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
  * q, k, v, q_out: [n_tokens, heads, head_dim] with strides of token and head (_st, _sh).  Two tokens for one place, or of two sequences for one page, give one or a
  * mixture of both.
  *
+ * aa_paged_append_more: the same with what `more` asks for, each member of which may be NULL.  q_norm, k_norm [head_dim] of the cache's type: a head x of queries and
+ * keys is x * rsqrt(mean(x^2) + norm_eps) * weight before it is rotated, in float32 with one rounding after both (norm_eps from 0 to 1; both, or k_norm alone where there are no queries).  k_out [n_tokens,
+ * n_kv_heads, head_dim], which may be k: the keys as they are stored, in the tokens' order.  positions int32 [batch]: what a sequence's last token has as position is positions[b] - 1 instead of lengths[b] -
+ * 1, for caches that have given up keys; sequences of fewer positions than keys are left out.  These need cos and sin.  weights float32 [n_pages, n_kv_heads,
+ * page_size]: 0 is stored for each new key.
+ *
  * aa_paged_decode_fwd: out[b, h] = softmax(q[b, h] . keys * sm_scale) values over the keys 0 .. lengths[b] - 1 of sequence b; a sequence of none gives 0,
  * one whose scores are all minus infinity NaN, as the quotient has it.
  * q, out: [batch, n_q_heads, head_dim] with strides of sequence and head; out may be q.  sm_scale is positive and below 2.3e38.
@@ -324,7 +330,18 @@ typedef struct {
   float sm_scale;
 } aa_paged_step;
 
+/* What aa_paged_append_more is given beside the tokens (likewise). */
+typedef struct {
+  const void* q_norm;
+  const void* k_norm;
+  void* k_out; int64_t ko_st, ko_sh;
+  const int32_t* positions;
+  float* weights;
+  float norm_eps;
+} aa_paged_more;
+
 int aa_paged_append(const aa_paged_cache* cache, const aa_paged_tokens* tokens, void* stream);
+int aa_paged_append_more(const aa_paged_cache* cache, const aa_paged_tokens* tokens, const aa_paged_more* more, void* stream);
 size_t aa_paged_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages);
 int aa_paged_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, void* stream);
 size_t aa_paged_sparse_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_chosen);
