@@ -75,6 +75,10 @@ _SIGNATURES = {
     "aa_paged_append_more": (c_int, [c_void_p, c_char_p, c_char_p, c_void_p]),
     "aa_paged_decode_workspace_bytes": (c_size_t, [c_int] * 6),
     "aa_paged_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p]),
+    "aa_paged_weighing_workspace_bytes": (c_size_t, [c_int] * 6),
+    "aa_paged_weighing_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p, c_int, c_void_p]),
+    "aa_paged_shared_workspace_bytes": (c_size_t, [c_int] * 6),
+    "aa_paged_shared_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p, c_void_p, c_int, c_void_p]),
     "aa_paged_sparse_workspace_bytes": (c_size_t, [c_int] * 7),
     "aa_paged_sparse_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p]),
     # the operator's sizes, then n_rows, n_keys, causal_offset

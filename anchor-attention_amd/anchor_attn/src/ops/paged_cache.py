@@ -319,6 +319,59 @@ def paged_decode_attention(cache: PagedCache, q: torch.Tensor, page_table: torch
     return out
 
 
+def _whole(name, value):
+    """A whole number that is given as any kind of number."""
+    try:
+        n = int(value)
+    except (TypeError, ValueError, OverflowError):
+        n = None
+    if n is None or n != value:
+        _refuse(f"{name} must be a whole number, not {value}")
+    return n
+
+
+def paged_weighing_decode_attention(cache: PagedCache, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, n_first: int = 0,
+                                    sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_decode_attention` that also counts how much attention each key has had: to ``cache.weights`` of key ``j`` of a sequence and KV head, from the
+    ``n_first``-th key on, is added the sum over the heads of its group of ``softmax(q K^T sm_scale)[j]`` (NaN where the output is), in a fixed order.
+    Two sequences must not share pages behind their first ``n_first`` keys.  Scratch: 4 bytes for each query head and key that the table has room for."""
+    out, tensors, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
+    weights = cache._weighed()
+    if not weights:
+        _refuse("the weights of keys are counted in a cache that has them")
+    n_first = _whole("n_first", n_first)
+    if not 0 <= n_first < 1 << 31:
+        _refuse(f"n_first must be from 0 to 2^31 - 1, not {n_first}")
+    if sizes[0]:
+        lib = _hip.lib()
+        nbytes = lib.aa_paged_weighing_workspace_bytes(*sizes, cache.n_kv_heads, cache.head_dim, cache.page_size, most)
+        ws = lengths.new_empty((nbytes >> 2,))
+        cache._launch(lib.aa_paged_weighing_decode_fwd, _hip.PAGED_STEP.pack(*tensors, ws.data_ptr(), nbytes, 0, *sizes, most, 0, 0, 0, scale), weights, n_first)
+    return out
+
+
+def paged_shared_decode_attention(cache: PagedCache, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, shared_pages: torch.Tensor,
+                                  groups: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_decode_attention` of sequences that begin with the same pages, which are read once for all of them.  Sequences ``groups[g]`` to
+    ``groups[g + 1] - 1`` (``groups`` int32 ``[n_groups + 1]``, ascending; None: all sequences are one group) have the same first ``shared_pages[g]`` pages (int32 ``[n_groups]``) in their rows of
+    the table; those of the first one's row are read.  The first and last groups need not begin and end the batch: sequences in none, and those of fewer keys than their group's
+    shared pages hold, are attended to by themselves.  Sequences append to pages of their own: only whole pages are shared."""
+    out, tensors, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
+    shared_ptr = _indices(shared_pages, "shared_pages", cache, 1)
+    n_groups = shared_pages.shape[0]
+    if not 0 < n_groups <= 65535:
+        _refuse(f"{n_groups} groups are not supported (1 to 65535)")
+    if groups is None and n_groups != 1:
+        _refuse(f"{n_groups} groups of sequences need to be told where they begin")
+    groups_ptr = 0 if groups is None else _indices(groups, "groups", cache, 1, n_groups + 1)
+    if sizes[0]:
+        lib = _hip.lib()
+        nbytes = lib.aa_paged_shared_workspace_bytes(*sizes, cache.n_kv_heads, cache.head_dim, cache.page_size, most)
+        ws = lengths.new_empty((nbytes >> 2,))
+        cache._launch(lib.aa_paged_shared_decode_fwd, _hip.PAGED_STEP.pack(*tensors, ws.data_ptr(), nbytes, 0, *sizes, most, 0, 0, 0, scale), shared_ptr, groups_ptr, n_groups)
+    return out
+
+
 def paged_sparse_decode_attention(cache: PagedCache, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, n_pages: int, n_first: int = 1,
                                   n_last: int = 1, sm_scale: Optional[float] = None,
                                   out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:

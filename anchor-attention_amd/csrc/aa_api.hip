@@ -1019,7 +1019,8 @@ static int paged_decode_args(const char* who, PagedDecodeArgs& a, const aa_paged
   }
   a = {(const uint16_t*)t->q, t->q_sb, t->q_sh, (uint16_t*)t->out, t->o_sb, t->o_sh, (const uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn,
        (const uint16_t*)cache->values, cache->vp_sp, cache->vp_sh, cache->vp_sn, t->page_table, t->pt_sb, 0, t->lengths, t->batch, t->n_q_heads,
-       cache->n_kv_heads, cache->head_dim, cache->n_pages, log2_of(cache->page_size), t->max_pages, 0, t->sm_scale, nullptr, nullptr, nullptr, cache->dtype};
+       cache->n_kv_heads, cache->head_dim, cache->n_pages, log2_of(cache->page_size), t->max_pages, 0, t->sm_scale, nullptr, nullptr, nullptr, cache->dtype,
+       nullptr, nullptr, nullptr, 0, nullptr, nullptr, nullptr};
   return AA_OK;
 }
 
@@ -1031,6 +1032,93 @@ int aa_paged_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* t, voi
   const size_t needed = paged_decode_scratch(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, log2_of(cache->page_size), t->max_pages).total;
   if ((rc = paged_decode_args(who, a, cache, t, needed))) return rc;
   give_scratch(a, static_cast<char*>(t->workspace), t->max_pages);
+  return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
+}
+
+// A step's scratch, the decode kernel's last
+struct WeighScratch {
+  size_t scores, totals, decode, total;
+};
+static WeighScratch carve_weigh(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
+  WeighScratch w;
+  const size_t rows = (size_t)batch * n_q_heads;
+  w.scores = 0;
+  w.totals = align256(rows * max_pages * page_size * 4);
+  w.decode = w.totals + align256(rows * 8);
+  w.total = w.decode + paged_decode_scratch(batch, n_q_heads, n_kv_heads, head_dim, log2_of(page_size), max_pages).total;
+  return w;
+}
+
+size_t aa_paged_weighing_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
+  if (check_paged("aa_paged_weighing_workspace_bytes", batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages)) return 0;
+  return carve_weigh(batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages).total;
+}
+
+int aa_paged_weighing_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* t, float* weights, int n_first, void* stream) {
+  const char* who = "aa_paged_weighing_decode_fwd";
+  PagedDecodeArgs a;
+  int rc;
+  if ((rc = check_given(t, who, "step")) || (rc = check_cache(who, cache, t->batch, t->n_q_heads, t->max_pages, t->page_table, t->lengths)) ||
+      (rc = check_ptr(weights, who, "weights")))
+    return rc;
+  if (n_first < 0) {
+    set_error("%s: n_first must not be negative (got %d)", who, n_first);
+    return AA_EBADARG;
+  }
+  const WeighScratch w = carve_weigh(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages);
+  if ((rc = paged_decode_args(who, a, cache, t, w.total))) return rc;
+  char* ws = static_cast<char*>(t->workspace);
+  a.scores = (float*)(ws + w.scores);
+  a.totals = (float*)(ws + w.totals);
+  a.weights = weights;
+  a.n_first = n_first;
+  give_scratch(a, ws + w.decode, t->max_pages);
+  return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
+}
+
+struct SharedScratch {
+  size_t skips, prefix, stats, parts, decode, total;
+};
+static SharedScratch carve_shared(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
+  SharedScratch w;
+  const size_t rows = (size_t)batch * n_q_heads;
+  w.skips = 0;
+  w.prefix = align256((size_t)batch * 4);
+  w.stats = w.prefix + align256(rows * head_dim * 4);
+  w.parts = w.stats + align256(rows * 8);
+  w.decode = w.parts + align256(paged_prefix_scratch(batch, n_q_heads, n_kv_heads, head_dim).total);
+  w.total = w.decode + paged_decode_scratch(batch, n_q_heads, n_kv_heads, head_dim, log2_of(page_size), max_pages).total;
+  return w;
+}
+
+size_t aa_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
+  if (n_q_heads == 0 || check_paged("aa_paged_shared_workspace_bytes", batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages)) return 0;
+  return carve_shared(batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages).total;
+}
+
+int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* t, const int32_t* shared_pages, const int32_t* groups, int n_groups, void* stream) {
+  const char* who = "aa_paged_shared_decode_fwd";
+  PagedDecodeArgs a;
+  int rc;
+  if ((rc = check_given(t, who, "step")) || (rc = check_cache(who, cache, t->batch, t->n_q_heads, t->max_pages, t->page_table, t->lengths)) ||
+      (rc = check_words(shared_pages, who, "shared_pages")) || (n_groups != 1 && (rc = check_given(groups, who, "groups"))) ||
+      (groups != nullptr && (rc = check_words(groups, who, "groups"))))
+    return rc;
+  if (n_groups <= 0 || n_groups > 65535) {
+    set_error("%s: %d groups are not supported (1 to 65535)", who, n_groups);
+    return n_groups <= 0 ? AA_EBADARG : AA_EUNSUPPORTED;
+  }
+  const SharedScratch w = carve_shared(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages);
+  if ((rc = paged_decode_args(who, a, cache, t, w.total))) return rc;
+  char* ws = static_cast<char*>(t->workspace);
+  a.skips = (int32_t*)(ws + w.skips);
+  a.prefix = (float*)(ws + w.prefix);
+  a.prefix_stats = (float*)(ws + w.stats);
+  const PagedScratch s = paged_prefix_scratch(a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim);
+  char* parts = ws + w.parts;
+  const PagedPrefixArgs x = {a, shared_pages, groups, n_groups, (int32_t*)(parts + s.headers), (float*)(parts + s.stats), (float*)(parts + s.parts)};
+  if ((rc = check_launch(launch_paged_prefix(x, (hipStream_t)stream), who))) return rc;
+  give_scratch(a, ws + w.decode, t->max_pages);
   return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
 }
 

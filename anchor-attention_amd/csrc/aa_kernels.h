@@ -170,12 +170,26 @@ struct PagedDecodeArgs {
   // scratch (paged_decode_scratch), all or none: what the parts of cut units are, their maxima and sums, their accumulators
   int32_t* headers; float* part_stats; float* parts;
   int dtype;
+  // keys' weights (all or none): scores [batch, n_q_heads, max_pages * page size] and maxima and sums [batch, n_q_heads, 2], both scratch, and the weights [n_pages, n_kv_heads, page size], but
+  // for the first n_first keys
+  float* scores; float* totals; float* weights; int n_first;
+  // a shared prefix (all or none): its pages [batch], its accumulators [batch, n_q_heads, head_dim] and maxima and sums [batch, n_q_heads, 2], written by launch_paged_prefix
+  int32_t* skips; float* prefix; float* prefix_stats;
 };
 struct PagedScratch {
   size_t headers, stats, parts, total;  // offsets in bytes
 };
 PagedScratch paged_decode_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_log, int max_pages);
 hipError_t launch_paged_decode(const PagedDecodeArgs& a, hipStream_t stream);
+
+// The prefixes that groups of sequences share: their states, as PagedDecodeArgs has them.
+struct PagedPrefixArgs {
+  PagedDecodeArgs step;  // (its own scratch is not used)
+  const int32_t* shared_pages; const int32_t* groups; int n_groups;  // groups NULL: one, the whole batch
+  int32_t* headers; float* part_stats; float* parts;  // scratch (paged_prefix_scratch)
+};
+PagedScratch paged_prefix_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim);
+hipError_t launch_paged_prefix(const PagedPrefixArgs& a, hipStream_t stream);
 
 constexpr int paged_score_pitch(int max_pages) { return (max_pages + 3) & ~3; }
 struct PagedSelectArgs {

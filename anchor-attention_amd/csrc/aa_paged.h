@@ -1,4 +1,5 @@
-// What the kernels over a cache in pages share: how they read tables and lengths, which come from device memory and are not trusted.
+// What the kernels over a cache in pages share: how they read tables and lengths, which come from device memory and are not trusted, and what attention over tiles of
+// keys is made of.
 #pragma once
 #include "aa_common.h"
 
@@ -52,6 +53,47 @@ __device__ __forceinline__ void unpack8(const uint4 raw, float (&x)[8]) {
 template <typename T>
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return uint4{T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7])};
+}
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <typename T> __device__ __forceinline__ floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c);
+template <> __device__ __forceinline__ floatx4 mfma16<Bf16>(u32x4 a, u32x4 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&a), *reinterpret_cast<const bf16x8*>(&b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ floatx4 mfma16<F16>(u32x4 a, u32x4 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const f16x8*>(&a), *reinterpret_cast<const f16x8*>(&b), c, 0, 0, 0);
+}
+
+// max and sum over the lanes 16, 32 and 48 away, which hold the other keys of a column
+__device__ __forceinline__ float max_over_quarters(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return max_with_other_half(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_over_quarters(const float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t w = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+  const auto s = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+// f over all lanes of a wave
+template <typename F>
+__device__ __forceinline__ float over_wave(const float x, const float none, F f) {
+  const uint32_t all = up_to(__float_as_uint(x), __float_as_uint(none),
+                             [&](const uint32_t a, const uint32_t b) { return __float_as_uint(f(__uint_as_float(a), __uint_as_float(b))); });
+  return __uint_as_float(__builtin_amdgcn_readlane(all, 63));
+}
+
+// Rows of a page behind a wave-uniform address: a lane's loads then have an offset of 32 bits, and the address is scalar arithmetic.  Rows behind the last key are out
+// of range, so that nothing is fetched for them (1000 sequences of 1 to 200 keys, 32/8 heads of 128, 56.7 -> 47.2 us).
+typedef __amdgpu_buffer_rsrc_t Rows;
+__device__ __forceinline__ Rows rows_at(const uint16_t* base, const int bytes) {
+  const uint64_t u = (uint64_t)base;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)hi << 32 | lo), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
 }  // namespace aa

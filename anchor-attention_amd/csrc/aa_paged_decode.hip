@@ -27,9 +27,6 @@
 
 namespace aa {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
 constexpr int kCols = 16;       // columns of a unit: heads of the group
 constexpr int kTile = 32;       // keys of a tile
 // What a unit costs beside its tiles, in tiles.  (128 sequences of 20 to 1200 keys, 32/8 heads of 64: 0 28.5 us, 3 21.7, 6 23.1; 32 of 500 to 16000, 32/8 of 128:
@@ -54,44 +51,6 @@ constexpr int kPerLane = 4, kPerLaneLog = 2;
 // read: 4 22.2 us, 8 22.2, 16 24.4.)
 constexpr int kLeast = 8;
 
-template <typename T> __device__ __forceinline__ floatx4 mfma16(u32x4 a, u32x4 b, floatx4 c);
-template <> __device__ __forceinline__ floatx4 mfma16<Bf16>(u32x4 a, u32x4 b, floatx4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&a), *reinterpret_cast<const bf16x8*>(&b), c, 0, 0, 0);
-}
-template <> __device__ __forceinline__ floatx4 mfma16<F16>(u32x4 a, u32x4 b, floatx4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const f16x8*>(&a), *reinterpret_cast<const f16x8*>(&b), c, 0, 0, 0);
-}
-
-// max and sum over the lanes 16, 32 and 48 away, which hold the other keys of a column
-__device__ __forceinline__ float max_over_quarters(float v) {
-  const uint32_t u = __float_as_uint(v);
-  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  return max_with_other_half(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-__device__ __forceinline__ float sum_over_quarters(const float v) {
-  const uint32_t u = __float_as_uint(v);
-  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const uint32_t w = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-  const auto s = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
-}
-// f over all lanes of a wave
-template <typename F>
-__device__ __forceinline__ float over_wave(const float x, const float none, F f) {
-  const uint32_t all = up_to(__float_as_uint(x), __float_as_uint(none),
-                             [&](const uint32_t a, const uint32_t b) { return __float_as_uint(f(__uint_as_float(a), __uint_as_float(b))); });
-  return __uint_as_float(__builtin_amdgcn_readlane(all, 63));
-}
-
-// Rows of a page behind a wave-uniform address: a lane's loads then have an offset of 32 bits, and the address is scalar arithmetic.  Rows behind the last key are out
-// of range, so that nothing is fetched for them (1000 sequences of 1 to 200 keys, 32/8 heads of 128, 56.7 -> 47.2 us).
-typedef __amdgpu_buffer_rsrc_t Rows;
-__device__ __forceinline__ Rows rows_at(const uint16_t* base, const int bytes) {
-  const uint64_t u = (uint64_t)base;
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
-  return __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)hi << 32 | lo), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
-}
-
 // Place: an integer that counts the tiles of all units
 template <typename Place>
 struct PagedPlace {       // of a tile, among all
@@ -100,9 +59,14 @@ struct PagedPlace {       // of a tile, among all
   Place start;            // the unit's beginning
 };
 
-// keys that are read of a sequence
-__device__ __forceinline__ int keys_of(const PagedDecodeArgs& p, const int length) {
+// kWeigh: the scores and each head's maximum and sum are kept for paged_weigh_kernel; kShared: the first pages of a sequence have been read for its group, whose states are there
+enum DecodeMode { kPlain, kWeigh, kShared };
+
+// keys that are read of sequence b
+template <DecodeMode MODE>
+__device__ __forceinline__ int keys_of(const PagedDecodeArgs& p, const int b, const int length) {
   const int n = min(max(length, 0), p.max_pages << p.page_log);
+  if (MODE == kShared) return n - (((const_i32*)p.skips)[b] << p.page_log);
   return p.n_chosen ? n - (max(0, pages_of(n, p.page_log) - p.n_chosen) << p.page_log) : n;
 }
 __device__ __forceinline__ int tiles_of(const int keys) { return max(1, (keys + kTile - 1) / kTile); }  // (a sequence of none has to be written too)
@@ -117,7 +81,32 @@ __device__ __forceinline__ uint32_t small_quotient(const uint32_t n, const uint3
   return q;
 }
 
-template <typename T, int D, int WAVES, typename Place>
+// What is known of a head over its group's prefix, joined to a part of four channels, or of all that a lane has (x[j][r] channel N * r + j from d on)
+template <int D, int N>
+__device__ __forceinline__ void add_prefix(const PagedDecodeArgs& p, const int b, const int head, const int d, const float scale, float& m, float& l, floatx4 (&x)[N]) {
+  const int64_t row = (int64_t)b * p.n_q_heads + head;
+  const float m0 = p.prefix_stats[2 * row], l0 = p.prefix_stats[2 * row + 1], m1 = fmaxf(m, m0);
+  const float w = m == -INFINITY ? 0.f : fast_exp2((m - m1) * scale), w0 = m0 == -INFINITY ? 0.f : fast_exp2((m0 - m1) * scale);
+  m = m1;
+  l = w * l + w0 * l0;
+  const float* from = p.prefix + row * D + d;
+  if constexpr (N == 1) {
+    const floatx4 y = *reinterpret_cast<const floatx4*>(from);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[0][e] = w * x[0][e] + w0 * y[e];
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        const floatx4 y = *reinterpret_cast<const floatx4*>(from + N * r + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[j + e][r] = w * x[j + e][r] + w0 * y[e];
+      }
+  }
+}
+
+template <typename T, int D, int WAVES, typename Place, DecodeMode MODE>
 __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const PagedDecodeArgs p) {
   constexpr int kKS = D / 32;      // MFMAs of a score
   constexpr int kDV = D / 16;      // channels of V that a lane loads
@@ -144,7 +133,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     for (int j = 0; j < kPerLane; ++j) {
       if (j > 0 && per_log == 0) break;
       const int b = i + (lane << per_log) + j;
-      keys[j] = b < p.batch ? keys_of(p, p.lengths[b]) : 0;
+      keys[j] = b < p.batch ? keys_of<MODE>(p, b, p.lengths[b]) : 0;
       own += b < p.batch ? tiles_of(keys[j]) + kOver : 0;
     }
     sum = sums_up_to(own);
@@ -250,6 +239,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     u.length = f.length;
     u.last_page = max(0, (u.length - 1) >> p.page_log);
     u.table = (const_i32*)(p.table + f.b * p.t_sb + u.kvh * p.t_sh);
+    if (MODE == kShared) u.table += min(((const_i32*)p.skips)[f.b], p.max_pages - 1);  // (of a sequence without keys of its own no page is read)
     u.k_head = u.kvh * p.kp_sh;
     u.v_head = u.kvh * p.vp_sh;
     return u;
@@ -326,7 +316,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       if (++f2.unit == units) {
         f2.unit = 0;
         ++f2.b;
-        f2.length = p.batch <= kScan ? keys_at(keys0, f2.b) : keys_of(p, ((const_i32*)p.lengths)[f2.b]);
+        f2.length = p.batch <= kScan ? keys_at(keys0, f2.b) : keys_of<MODE>(p, f2.b, ((const_i32*)p.lengths)[f2.b]);
         f2.n_tiles = tiles_of(f2.length);
       }
       u2 = unit_of(f2);
@@ -424,6 +414,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       __builtin_amdgcn_sched_barrier(0);
       load_k(x, o);
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (MODE == kWeigh) {
+        const int room = p.max_pages << p.page_log;
+        float* to = p.scores + ((int64_t)f.b * p.n_q_heads + head0 + c16) * room + kTile * t + 4 * g;
+        if (c16 < n_cols) {
+          *reinterpret_cast<floatx4*>(to) = s[0];
+          if (kTile * t + 16 < room) *reinterpret_cast<floatx4*>(to + 16) = s[1];
+        }
+      }
       u32x4 prob, rest;
       probabilities(s, t, prob, rest, false);
       add_values(x, t, prob, rest, false);
@@ -456,7 +454,15 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
 
     const bool from_start = f.tile == 0, to_end = last == f.n_tiles;
     if (from_start && to_end) {
-      const float inv = length == 0 ? 0.f : 1.f / l_run;  // (no keys: 0; keys whose scores are all minus infinity: 0 / 0, as a soft-max has it)
+      bool none = length == 0;
+      if constexpr (MODE == kShared) {
+        if (((const_i32*)p.skips)[f.b] > 0) {
+          none = false;
+          add_prefix<D, kDV>(p, f.b, head0 + min(c16, n_cols - 1), kDV * 4 * g, scale, m_run, l_run, acc);
+        }
+      }
+      if (MODE == kWeigh && g == 0 && c16 < n_cols) *reinterpret_cast<floatx2*>(p.totals + 2 * ((int64_t)f.b * p.n_q_heads + head0 + c16)) = floatx2{m_run, l_run};
+      const float inv = none ? 0.f : 1.f / l_run;  // (no keys: 0; keys whose scores are all minus infinity: 0 / 0, as a soft-max has it)
       if (c16 < n_cols) {
         uint16_t* op = p.out + f.b * p.o_sb + (int64_t)(head0 + c16) * p.o_sh + kDV * 4 * g;
 #pragma unroll
@@ -537,6 +543,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
         for (int e = 0; e < 4; ++e) x[e] += weight * xs[w][e];
       }
       if (begins && ends) {
+        if constexpr (MODE == kShared) {
+          floatx4 y[1] = {x};
+          if (((const_i32*)p.skips)[info.y] > 0) add_prefix<D, 1>(p, info.y, head0 + col, d, scale, m, l, y);
+          x = y[0];
+        }
+        if (MODE == kWeigh && d == 0) *reinterpret_cast<floatx2*>(p.totals + 2 * ((int64_t)info.y * p.n_q_heads + head0 + col)) = floatx2{m, l};
         const float inv = 1.f / l;  // (a unit that is cut has keys)
         uint16_t* op = p.out + info.y * p.o_sb + (int64_t)(head0 + col) * p.o_sh + d;
         *reinterpret_cast<u32x2*>(op) = u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
@@ -560,7 +572,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
 // Joins the parts of a column whose unit begins in share blockIdx.x and ends in another: the weights first, then groups of D / 4 lanes add up
 // every so many parts.  Few bytes; the launch and three loads one after the other take 3 to 5 us, which a step pays whether or not a unit was cut, since the
 // host does not know the lengths.
-template <typename T, int D>
+template <typename T, int D, DecodeMode MODE>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArgs p) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
   __shared__ float weight[256], red[2][4];
@@ -611,6 +623,12 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArg
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[e] += sums[i][tid][e];
     l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    if constexpr (MODE == kShared) {
+      floatx4 y[1] = {sum};
+      if (((const_i32*)p.skips)[header.y] > 0) add_prefix<D, 1>(p, header.y, header.z + col, 4 * tid, scale, m, l, y);
+      sum = y[0];
+    }
+    if (MODE == kWeigh && tid == 0) *reinterpret_cast<floatx2*>(p.totals + 2 * ((int64_t)header.y * p.n_q_heads + header.z + col)) = floatx2{m, l};
     const float inv = 1.f / l;
     uint16_t* op = p.out + header.y * p.o_sb + (int64_t)(header.z + col) * p.o_sh + 4 * tid;
     *reinterpret_cast<u32x2*>(op) = u32x2{T::pack(sum[0] * inv, sum[1] * inv), T::pack(sum[2] * inv, sum[3] * inv)};
@@ -629,15 +647,54 @@ PagedScratch paged_decode_scratch(int batch, int n_q_heads, int n_kv_heads, int 
   return s;
 }
 
-template <typename T, int D>
-static void launch_paged_decode_for(const PagedDecodeArgs& a, hipStream_t stream) {
+// Adds to each key's weight what its KV head's queries have given it: the sum over the heads of the group of 2^((score - maximum) * scale) / sum, from the scores that the
+// decode kernel has left.  Bound by reading these once.  A thread has four keys, a work-group 1024, and as many more as it takes for all of a sequence's.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_weigh_kernel(const PagedDecodeArgs p) {
+  const int b = blockIdx.z, kvh = blockIdx.y, group = p.n_q_heads / p.n_kv_heads, room = p.max_pages << p.page_log, n = keys_of<kWeigh>(p, b, p.lengths[b]);
+  const int64_t head0 = (int64_t)b * p.n_q_heads + (int64_t)kvh * group;
+  const float scale = p.sm_scale * kLog2e;
+  for (int i = (blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += gridDim.x * 1024) {
+    const int page = p.table[b * p.t_sb + (i >> p.page_log)];
+    if ((uint32_t)page >= (uint32_t)p.n_pages) continue;  // (what is read in its place is another sequence's)
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < group; ++h) {
+      const floatx4 s = *reinterpret_cast<const floatx4*>(p.scores + (head0 + h) * room + i);
+      const floatx2 total = *reinterpret_cast<const floatx2*>(p.totals + 2 * (head0 + h));
+      const float inv = 1.f / total[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += prob_exp2<T>(s[e] - total[0], scale) * inv;
+    }
+    float* w = p.weights + (((int64_t)page * p.n_kv_heads + kvh) << p.page_log) + (i & ((1 << p.page_log) - 1));
+    floatx4 old = *reinterpret_cast<const floatx4*>(w);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < n && i + e >= p.n_first) old[e] += sum[e];
+    *reinterpret_cast<floatx4*>(w) = old;
+  }
+}
+
+template <typename T, int D, DecodeMode MODE>
+static void launch_paged_decode_as(const PagedDecodeArgs& a, hipStream_t stream) {
   const int group = a.n_q_heads / a.n_kv_heads, cols = group < kCols ? group : kCols, units = a.n_kv_heads * ((group + kCols - 1) / kCols);
   const size_t lds = (size_t)8 * cols * (D + 4) * 4;
   // (places fit 32 bits unless thousands of sequences have tables for a million keys)
   const int64_t most = (int64_t)a.batch * units * (((int64_t)a.max_pages << a.page_log) / kTile + 1 + kOver);
-  if (most < 1ll << 30) hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int>), dim3(kShares), dim3(256), lds, stream, a);
-  else hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int64_t>), dim3(kShares), dim3(256), lds, stream, a);
-  if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3(kShares, cols), dim3(256), 0, stream, a);
+  if (most < 1ll << 30) hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int, MODE>), dim3(kShares), dim3(256), lds, stream, a);
+  else hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int64_t, MODE>), dim3(kShares), dim3(256), lds, stream, a);
+  if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D, MODE>), dim3(kShares, cols), dim3(256), 0, stream, a);
+  if (MODE == kWeigh) {
+    // work-groups of a (sequence, KV head): as many as its table has room for, or fewer where there are thousands in all
+    const int64_t all = (int64_t)a.batch * a.n_kv_heads, room = (((int64_t)a.max_pages << a.page_log) + 1023) / 1024, each = all < 8192 ? 8192 / all : 1;
+    hipLaunchKernelGGL((paged_weigh_kernel<T>), dim3((uint32_t)(room < each ? room : each), a.n_kv_heads, a.batch), dim3(256), 0, stream, a);
+  }
+}
+
+template <typename T, int D>
+static void launch_paged_decode_for(const PagedDecodeArgs& a, hipStream_t stream) {
+  if (a.scores != nullptr) launch_paged_decode_as<T, D, kWeigh>(a, stream);
+  else if (a.skips != nullptr) launch_paged_decode_as<T, D, kShared>(a, stream);
+  else launch_paged_decode_as<T, D, kPlain>(a, stream);
 }
 
 hipError_t launch_paged_decode(const PagedDecodeArgs& a, hipStream_t stream) {

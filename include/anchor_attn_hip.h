@@ -290,6 +290,16 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
  * q, out: [batch, n_q_heads, head_dim] with strides of sequence and head; out may be q.  sm_scale is positive and below 2.3e38.
  * workspace: aa_paged_decode_workspace_bytes() bytes of device scratch, which may be none (contents undefined afterwards).
  *
+ * aa_paged_weighing_decode_fwd: the same, and to the weight of each key j >= n_first of the sequence, weights[page, kv head, row] (float32 [n_pages, n_kv_heads, page_size],
+ * 16-byte aligned), is added sum over the heads of the group of softmax(q . keys * sm_scale)[j]; NaN where the output is.  Nothing is added for a page outside the
+ * pool.  Sequences must not share pages behind their first n_first keys: of two additions one may be lost.  The workspace (aa_paged_weighing_workspace_bytes()) has 4 bytes for
+ * each query head and key that the table has room for.
+ *
+ * aa_paged_shared_decode_fwd: the same as aa_paged_decode_fwd where sequences groups[g] to groups[g + 1] - 1 (groups int32 [n_groups + 1], ascending; sequences before the
+ * first and behind the last group are in none; NULL with one group: all of the batch) have the same first shared_pages[g] pages (int32 [n_groups]), those in the table's row of sequence groups[g]: they are read once for
+ * the group.  Sequences of fewer keys than these pages hold are attended to by themselves.  What groups and shared_pages hold is clamped to the batch and to
+ * [0, max_pages]; where groups do not ascend outputs may be anything.
+ *
  * aa_paged_sparse_decode_fwd: the same over n_chosen pages for each sequence and KV head, or all where the sequence has no more: its first n_first, its last
  * n_last (at least 1) and those of the others whose score is largest, the lower page first among equal ones.  The score is the largest over the heads of the
  * group of sum_d q_d * (q_d >= 0 ? largest_d : smallest_d), which no product of the query with a key of the page exceeds: exact products, a sum in float64
@@ -344,6 +354,10 @@ int aa_paged_append(const aa_paged_cache* cache, const aa_paged_tokens* tokens, 
 int aa_paged_append_more(const aa_paged_cache* cache, const aa_paged_tokens* tokens, const aa_paged_more* more, void* stream);
 size_t aa_paged_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages);
 int aa_paged_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, void* stream);
+size_t aa_paged_weighing_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages);
+int aa_paged_weighing_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, float* weights, int n_first, void* stream);
+size_t aa_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages);
+int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, const int32_t* shared_pages, const int32_t* groups, int n_groups, void* stream);
 size_t aa_paged_sparse_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_chosen);
 int aa_paged_sparse_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, void* stream);
 

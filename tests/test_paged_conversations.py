@@ -3,7 +3,10 @@ decode over a shared prefix - against plain float64 implementations, at the leng
 
 Tolerances beside those of tests/test_paged_cache.py (u: half a step of the 16-bit type).
 Norm and rotation: a float32 sum of D squares is off by at most D * 2^-24 of it, its inverse root by half of that and 2^-22, three products by 2^-24 each,
-the rotation by 2^-23 of its products' magnitudes: (D / 2 + 16) * 2^-24 of the magnitudes, and u of the result."""
+the rotation by 2^-23 of its products' magnitudes: (D / 2 + 16) * 2^-24 of the magnitudes, and u of the result.
+Weights: a probability is off by what tests/test_paged_cache.py says of it, 2 * D * 2^-24 * sum |q_d k_d| * scale + 2^-14 of it, a sum over the group's heads in float32 and the addition to
+what was there by 2^-24 of each partial sum."""
+
 import ctypes
 import pathlib
 
@@ -183,4 +186,267 @@ def test_what_appending_refuses_beside():
     cache.weights.data = z(5, 2, 16, dtype=torch.float32)
     with pytest.raises(_hip.AnchorAttnHipError, match="other memory"):
         ops.append_to_pages(**good)
+    torch.cuda.synchronize()
+
+
+# ---- decode that counts attention ------------------------------------------------------------------------------------
+
+LENGTHS = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129, 255, 257, 500, 1023]
+
+
+def _weights_close(got, before, q, s, scale, n_first=0):
+    """The weights of a cache after a step, all of them: what no sequence has a key for is as it was."""
+    want, bound = before.double(), torch.zeros_like(before, dtype=torch.float64)
+    group, page = q.shape[1] // s.hkv, s.page
+    for b, n in enumerate(s.host):
+        if n == 0:
+            continue
+        at = s.table[b, :(n + page - 1) // page].long()
+        for h in range(s.hkv):
+            x, k = q[b, h * group:(h + 1) * group].double(), s.rows(s.cache.keys, b, h)
+            p = (x @ k.T * scale).softmax(-1)
+            relative = 2.0 * s.d * 2.0 ** -24 * (x.abs() @ k.abs().T).amax(-1, keepdim=True) * scale + 2.0 ** -14 + n * 2.0 ** -24
+            for t, add in ((want, p.sum(0)), (bound, (relative * p).sum(0) + (group + 1) * 2.0 ** -24 * p.sum(0))):
+                rows = t[at, h].reshape(-1)
+                rows[n_first:n] += add[n_first:]
+                t[at, h] = rows.view(-1, page)
+    err = (got.double() - want).abs()
+    assert bool((err <= bound + torch.where(bound > 0, 2.0 ** -24 * want.abs(), 0.0)).all()), float((err - bound).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lengths,hq,hkv,d,page,layout,extra", [
+    (LENGTHS, 32, 8, 128, 64, "heads", 0), (LENGTHS, 28, 4, 128, 16, "rows", 3), (LENGTHS, 14, 2, 64, 16, "heads", 100), (LENGTHS, 32, 8, 64, 32, "part", 0),
+    (LENGTHS, 3, 3, 128, 256, "heads", 1), ([700, 1, 33], 17, 1, 128, 128, "rows", 0), ([900, 0], 71, 1, 64, 64, "heads", 0), ([20001], 32, 8, 128, 64, "heads", 0),
+    ([9000, 40, 12345], 28, 4, 64, 16, "heads", 1), ([5], 14, 2, 64, 16, "heads", 0), ([0], 4, 2, 128, 16, "heads", 0), ([700] * 130 + [5000], 8, 2, 64, 64, "heads", 0),
+    ([1] * 300, 14, 2, 64, 16, "heads", 0), ([16], 4, 2, 64, 16, "heads", 0),
+])
+def test_weighing_decode(lengths, hq, hkv, d, page, layout, extra, dtype):
+    s = _Setup(lengths, hkv, d, page, dtype, hq + page, layout, extra=extra)
+    cache, q = _weights_of(s), s.queries(hq)
+    cache.weights.uniform_(0, 3, generator=s.g)
+    before = cache.weights.clone()
+    want = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
+    out = _ops().paged_weighing_decode_attention(cache, q, s.table, s.lengths)
+    assert torch.equal(out, want)  # the same bits
+    _weights_close(cache.weights, before, q, s, d ** -0.5)
+    after = cache.weights.clone()
+    cache.weights.copy_(before)
+    assert _ops().paged_weighing_decode_attention(cache, q, s.table, s.lengths, out=torch.empty_like(q)).equal(want) and torch.equal(cache.weights, after)
+    cache.weights.copy_(before)
+    _ops().paged_weighing_decode_attention(cache, q, s.table, s.lengths, n_first=17, sm_scale=0.02)
+    _weights_close(cache.weights, before, q, s, 0.02, 17)
+
+
+@pytest.mark.gpu
+def test_weighing_scores_that_are_infinite_or_nan():
+    """A key of minus infinity has no weight, a sequence whose scores are all of it or one of which is NaN or plus infinity NaN where its heads are, and no other."""
+    s = _Setup([700, 40, 40, 40, 300], 2, 64, 16, BF16, 9)
+    cache, q = _weights_of(s), s.queries(4, 0.5)
+    q[:, :, 0] = 1.0
+    for b, value in ((0, float("-inf")), (1, float("nan")), (2, float("inf"))):
+        s.cache.keys[s.table[b, 1].long(), 0, 3, 0] = value
+    s.cache.keys[s.table[3, :3].long(), 0, :, 0] = float("-inf")
+    before = cache.weights.clone()
+    out = _ops().paged_weighing_decode_attention(cache, q, s.table, s.lengths)
+    assert [[bool(out[b, 2 * h:2 * h + 2].isnan().all()) for h in range(2)] for b in range(5)] == [[False, False], [True, False], [True, False], [True, False], [False, False]]
+    weights = [[cache.weights[s.table[b, :(n + 15) // 16].long(), h].reshape(-1)[:n] for h in range(2)] for b, n in enumerate(s.host)]
+    assert all(bool(weights[b][0].isnan().all()) for b in (1, 2, 3)) and int(cache.weights.isnan().sum()) == 120
+    assert float(weights[0][0][19]) == 5.0 and bool((weights[0][0][:19] > 5.0).all())
+    # and infinite values have no part in it
+    cache.weights.copy_(before)
+    s.cache.values[s.table[4, 0].long(), 0, 5, 3] = float("inf")
+    again = _ops().paged_weighing_decode_attention(cache, q, s.table, s.lengths)
+    assert bool((again[4, :2, 3] == float("inf")).all()) and torch.equal(weights[4][0], cache.weights[s.table[4, :19].long(), 0].reshape(-1)[:300])
+
+
+@pytest.mark.gpu
+def test_weighing_of_lengths_and_pages_that_do_not_fit():
+    """Lengths above the table are its size; a page outside the pool is read as the nearest one, and nothing is added for it."""
+    s = _Setup([64, 64, 64], 2, 64, 16, BF16, 10)
+    cache, q = _weights_of(s), s.queries(4)
+    s.cache.keys.nan_to_num_(0.5), s.cache.values.nan_to_num_(0.5)
+    s.table[1, 2], s.table[1, 3] = -5, 2 ** 31 - 1
+    lengths = _int32([1000, 64, -3])
+    out = _ops().paged_weighing_decode_attention(cache, q, s.table, lengths)
+    assert torch.equal(out, _ops().paged_decode_attention(s.cache, q, s.table, lengths))
+    at = torch.cat((s.table[0], s.table[1, :2])).long()
+    changed = (cache.weights != 5.0).any(-1).any(-1)
+    assert sorted(changed.nonzero().flatten().tolist()) == sorted(at.tolist())
+
+
+# ---- decode over a shared prefix -----------------------------------------------------------------------------------
+
+def _shared_setup(prefixes, sizes, own, hkv, d, page, dtype, seed, layout="heads", extra=0, alone=()):
+    """Groups of ``sizes`` sequences with ``prefixes`` pages in common and ``own`` keys each, after the sequences ``alone`` of no group."""
+    lengths = list(alone)
+    group_of = [None] * len(alone)
+    for g, n in enumerate(sizes):
+        for _ in range(n):
+            lengths.append(prefixes[g] * page + own[(len(lengths) - len(alone)) % len(own)])
+            group_of.append(g)
+    s = _Setup(lengths, hkv, d, page, dtype, seed, layout, extra=extra)
+    begins = [len(alone)]
+    for n in sizes:
+        begins.append(begins[-1] + n)
+    for b, g in enumerate(group_of):
+        if g is not None:
+            s.table[b, :prefixes[g]] = s.table[begins[g], :prefixes[g]]
+    return s, _int32(prefixes), _int32(begins)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("prefixes,sizes,own,hq,hkv,d,page,layout,extra,alone", [
+    ([3], [5], [1, 40, 300], 32, 8, 128, 64, "heads", 0, []),
+    ([1], [2], [1], 14, 2, 64, 16, "heads", 0, []),
+    ([5], [1], [0], 4, 2, 128, 16, "heads", 0, []),
+    ([7, 0, 33, 2], [6, 3, 17, 1], [3, 0, 130, 16], 28, 4, 128, 16, "rows", 2, [5, 0, 700]),
+    ([40], [70], [17, 1, 0, 90], 28, 4, 128, 32, "part", 0, []),
+    ([9, 13, 1], [40, 1, 30], [33, 64], 32, 8, 64, 256, "heads", 1, [1]),
+    ([300], [9], [20], 71, 1, 64, 16, "heads", 0, []),
+    ([157], [33], [7, 1000], 8, 2, 128, 64, "heads", 0, []),
+    ([313], [3], [2], 8, 2, 128, 64, "rows", 0, [9000]),
+    ([2] * 90, [3] * 90, [5, 1, 20], 4, 1, 64, 32, "heads", 0, [7] * 5),
+    ([1, 4096], [1, 2], [33], 4, 2, 64, 16, "heads", 0, []),
+    ([0, 0, 3], [2, 0, 2], [9], 4, 2, 64, 16, "heads", 0, []),
+])
+def test_shared_decode(prefixes, sizes, own, hq, hkv, d, page, layout, extra, alone, dtype):
+    s, shared, groups = _shared_setup(prefixes, sizes, own, hkv, d, page, dtype, hq + page, layout, extra, alone)
+    q = s.queries(hq)
+    wide = torch.full((len(s.host), hq + 1, d + 8), 7.0, dtype=dtype, device="cuda")
+    out = wide[:, 1:, 8:]
+    assert _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, out=out) is out
+    assert bool((wide[:, 0] == 7.0).all()) and bool((wide[:, :, :8] == 7.0).all())
+    _close(out, q, s, d ** -0.5)
+    again = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, sm_scale=d ** -0.5)
+    assert torch.equal(out, again)  # the same bits
+    _close(_ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, sm_scale=0.3), q, s, 0.3)
+    if len(sizes) == 1 and not alone:
+        assert torch.equal(_ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared), out)
+    assert _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, out=q) is q and torch.equal(q, again)
+
+
+@pytest.mark.gpu
+def test_shared_decode_of_sequences_that_are_shorter_than_the_prefix():
+    """A padded batch and sequences that do not have all of it: what they do not see, an infinite value too, does not reach them."""
+    s, shared, groups = _shared_setup([10, 6], [8, 4], [40], 2, 64, 16, BF16, 3)
+    s.host = [165, 0, 159, 160, 1, 200, 0, 161, 96, 95, 16, 97]
+    s.lengths.copy_(_int32(s.host))
+    s.cache.values.nan_to_num_(1.0), s.cache.keys.nan_to_num_(1.0)
+    q = s.queries(8)
+    got = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    _close(got, q, s, 0.125)
+    s.cache.values[s.table[0, 9].long(), :, 15] = float("inf")  # (key 159)
+    s.cache.keys[s.table[8, 5].long(), :, 15] = float("nan")  # (key 95)
+    bad = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    seen = [b for b, n in enumerate(s.host) if n >= (160 if b < 8 else 96)]
+    assert all(not bool(bad[b].isfinite().any()) if b in seen else torch.equal(bad[b], got[b]) for b in range(12))
+    assert all(bool((bad[b] == float("inf")).all()) for b in seen if b < 8) and all(bool(bad[b].isnan().all()) for b in seen if b >= 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("batch,pages", [(3, 4), (40, 300)])
+def test_shared_decode_with_infinite_values_and_scores(batch, pages, dtype):
+    """In the prefix: an infinite value gives an infinity in its channel and nothing else; keys that are all minus infinity leave the own ones, and the other way round."""
+    s, shared, groups = _shared_setup([pages], [batch], [40], 2, 64, 16, dtype, 8)
+    q = s.queries(8, 0.3)
+    q[:, :, 0] = 1.0
+    want = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    at = s.table[0, 1].long()
+    s.cache.values[at, 0, 3, 5], s.cache.values[at, 0, 4, 6], s.cache.values[at, 0, 9, 7] = float("inf"), float("-inf"), float("nan")
+    got = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    assert bool((got[:, :4, 5] == float("inf")).all()) and bool((got[:, :4, 6] == float("-inf")).all()) and bool(got[:, :4, 7].isnan().all())
+    assert torch.equal(got[:, 4:], want[:, 4:])
+    rest = torch.ones(64, dtype=torch.bool, device="cuda")
+    rest[5:8] = False
+    assert bool(((got[:, :4, rest] - want[:, :4, rest]).abs() <= 2 * U[dtype] * want[:, :4, rest].abs() + 2.0 ** -13).all())
+    # minus infinity: the keys of the prefix for KV head 0, all own keys of sequence 1 for KV head 1, all of sequence 2 for both
+    s.cache.values[at, 0, :, 5:8] = 0.5
+    s.cache.keys[s.table[0, :pages].long(), 0, :, 0] = float("-inf")
+    s.cache.keys[s.table[1, pages:pages + 3].long(), 1, :, 0] = float("-inf")
+    s.cache.keys[s.table[2, pages:pages + 3].long(), 0, :, 0] = float("-inf")
+    got = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    plain = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
+    assert bool(got[2, :4].isnan().all()) and bool(plain[2, :4].isnan().all()) and int(got.isnan().sum()) == 4 * 64
+    near = (got.double() - plain.double()).abs() <= 2 * U[dtype] * plain.abs() + 2.0 ** -12
+    assert bool((near | plain.isnan()).all())
+
+
+@pytest.mark.gpu
+def test_groups_that_do_not_fit():
+    """Begins outside the batch, more pages than the table has, pages outside the pool: everything is clamped, and outside of groups all is as it was."""
+    s, shared, groups = _shared_setup([4], [6], [20], 2, 64, 16, BF16, 4)
+    s.cache.keys.nan_to_num_(0.5), s.cache.values.nan_to_num_(0.5)
+    q = s.queries(4)
+    plain = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
+    for shared_pages, begins in (([2 ** 31 - 1], [0, 6]), ([-5], [0, 6]), ([4], [-7, 2 ** 31 - 1]), ([4, 4], [-9, 2, 100]), ([4], [6, 6]), ([4], [5, 3]), ([4, 4, 4], [2, 2, 2, 4]), ([4], [-3, -1])):
+        got = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, _int32(shared_pages), _int32(begins))
+        assert bool(((got.float() - plain.float()).abs() <= 2 * U[BF16] * plain.float().abs() + 2.0 ** -12).all()), (shared_pages, begins)
+    s.table[0, 1], s.table[0, 2] = -1, 2 ** 31 - 1
+    got = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    s.table[:, 1], s.table[:, 2] = 0, s.cache.n_pages - 1
+    assert torch.equal(got, _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups))
+    # no keys but the prefix, in a table that ends with it
+    s.host = [64] * 6
+    got = _ops().paged_shared_decode_attention(s.cache, q, s.table[:, :4], _int32(s.host), shared, groups)
+    _close(got, q, s, 0.125)
+
+
+STEPS = {"weigh": ("aa_paged_weighing_decode_fwd", {"weights": 4096, "n_first": 0}), "shared": ("aa_paged_shared_decode_fwd", {"shared_pages": 4096, "groups": 4096, "n_groups": 2})}
+
+
+@pytest.mark.parametrize("fn,change,message", [
+    *[(fn, c, m) for fn in STEPS for c, m in EVERY + READ], *[(fn, {"workspace_bytes": 100}, "workspace has 100 bytes") for fn in STEPS], *[(fn, {"workspace": 0}, "workspace is NULL") for fn in STEPS],
+    ("weigh", {"weights": 0}, "weights is NULL"), ("weigh", {"weights": 4100}, "weights must be 16-byte"), ("weigh", {"n_first": -1}, "n_first"),
+    ("shared", {"shared_pages": 0}, "shared_pages is NULL"), ("shared", {"groups": 0}, "groups is NULL"), ("shared", {"groups": 6}, "groups must be 4-byte"), ("shared", {"shared_pages": 5}, "shared_pages must be 4-byte"),
+    ("shared", {"n_groups": 0}, "0 groups"), ("shared", {"n_groups": 65536}, "65536 groups"),
+])
+def test_what_the_c_interface_of_steps_refuses(fn, change, message):
+    """Before anything is launched: the addresses are never read."""
+    from anchor_attn.src.ops import _hip
+    name, more = STEPS[fn]
+    assert set(change) <= {*STEP, *more, *CACHE, "cache", "given"}
+    struct = _hip.PagedCacheStruct(*{**CACHE, **{k: v for k, v in change.items() if k in CACHE}}.values())
+    step = _hip.PAGED_STEP.pack(*{**STEP, **{k: v for k, v in change.items() if k in STEP}}.values())
+    with pytest.raises(_hip.AnchorAttnHipError, match=message):
+        _hip.check(getattr(_hip.lib(), name)(None if "cache" in change else ctypes.addressof(struct), None if "given" in change else step,
+                                             *{**more, **{k: v for k, v in change.items() if k in more}}.values(), None))
+
+
+def test_scratch_of_steps():
+    from anchor_attn.src.ops import _hip
+    lib = _hip.lib()
+    assert lib.aa_paged_weighing_workspace_bytes(0, 8, 2, 128, 16, 8) == 0 == lib.aa_paged_shared_workspace_bytes(2, 0, 2, 128, 16, 8)
+    assert lib.aa_paged_weighing_workspace_bytes(2, 8, 2, 128, 16, 8) >= 2 * 8 * (16 * 8 + 2) * 4
+    assert lib.aa_paged_weighing_workspace_bytes(128, 32, 8, 128, 16, 65536) >= 128 * 32 * (1 << 22)
+    assert lib.aa_paged_shared_workspace_bytes(2, 8, 2, 128, 16, 8) >= 2 * 8 * 130 * 4
+
+
+@pytest.mark.gpu
+def test_what_steps_refuse():
+    from anchor_attn.src.ops import _hip
+    ops = _ops()
+    z = lambda *shape, dtype=BF16: torch.zeros(shape, dtype=dtype, device="cuda")  # noqa: E731
+    cache = ops.PagedCache.empty(5, 2, 16, 64, weights=True)
+    for t in (cache.keys, cache.values, cache.weights):
+        t.zero_()
+    table, lengths, q = z(2, 3, dtype=torch.int32), z(2, dtype=torch.int32), z(2, 4, 64)
+    good = {"cache": cache, "q": q, "page_table": table, "lengths": lengths}
+    one = z(1, dtype=torch.int32)
+    reads = [{"q": z(2, 3, 64)}, {"q": z(3, 4, 64)}, {"q": q.cpu()}, {"q": z(2, 4, 64).requires_grad_()}, {"page_table": table.long()}, {"lengths": lengths.long()}, {"out": z(2, 4, 128)},
+             {"out": z(1, 4, 64).expand(2, 4, 64)}, {"sm_scale": 0.0}, {"sm_scale": float("nan")}, {"cache": None}]
+    for fn, base, changes in ((ops.paged_weighing_decode_attention, good, reads + [{"n_first": -1}, {"n_first": 1.5}, {"n_first": None}, {"n_first": 1 << 31}, {"cache": ops.PagedCache(cache.keys, cache.values)}]),
+                              (ops.paged_shared_decode_attention, {**good, "shared_pages": one, "groups": lengths},
+                               reads + [{"shared_pages": one.long()}, {"shared_pages": z(2, dtype=torch.int32)}, {"shared_pages": one.cpu()}, {"shared_pages": None}, {"shared_pages": z(0, dtype=torch.int32), "groups": one},
+                                        {"groups": one}, {"groups": z(4, dtype=torch.int32)[::2]}, {"shared_pages": z(2, dtype=torch.int32), "groups": None}, {"shared_pages": z(1, 1, dtype=torch.int32)}])):
+        fn(**base)
+        for change in changes:
+            with pytest.raises(_hip.AnchorAttnHipError):
+                fn(**{**base, **change})
+        with pytest.raises(_hip.AnchorAttnHipError, match="traced"):
+            torch.func.vmap(lambda x: fn(**{**base, "q": x}))(q[None])
+        assert fn(**{**base, "q": q[:0], "page_table": table[:0], "lengths": lengths[:0]}).shape == (0, 4, 64)
     torch.cuda.synchronize()
