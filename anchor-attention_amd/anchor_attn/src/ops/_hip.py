@@ -30,6 +30,7 @@ class PagedCacheStruct(ctypes.Structure):
 # ``aa_paged_tokens`` and ``aa_paged_step`` (packed: a call with 26 arguments costs 2.2 us of ctypes' conversions, one with a packed struct 0.5)
 PAGED_TOKENS = struct.Struct("@" + "Pqq" * 4 + "PPqPqPP" + "5i0q")
 PAGED_STEP = struct.Struct("@" + "Pqq" * 2 + "PqPPNP" + "6if0q")
+PAGED_EVICTION = struct.Struct("@PqPPPPPN6i")  # aa_paged_eviction
 PAGED_MORE = struct.Struct("@PPPqqPPf0q")  # aa_paged_more
 
 
@@ -79,6 +80,8 @@ _SIGNATURES = {
     "aa_paged_weighing_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p, c_int, c_void_p]),
     "aa_paged_shared_workspace_bytes": (c_size_t, [c_int] * 6),
     "aa_paged_shared_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "aa_paged_evict_workspace_bytes": (c_size_t, [c_int] * 4),
+    "aa_paged_evict": (c_int, [c_void_p, c_char_p, c_void_p]),
     "aa_paged_sparse_workspace_bytes": (c_size_t, [c_int] * 7),
     "aa_paged_sparse_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p]),
     # the operator's sizes, then n_rows, n_keys, causal_offset

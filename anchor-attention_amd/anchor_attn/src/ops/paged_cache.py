@@ -350,6 +350,37 @@ def paged_weighing_decode_attention(cache: PagedCache, q: torch.Tensor, page_tab
     return out
 
 
+def evict_from_pages(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor, n_keys: int, n_first: int = 0, n_last: int = 1,
+                     above: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cuts sequences of more than ``above`` keys (``n_keys`` if it is not given) down to ``n_keys``, for each KV head its own: the first ``n_first``, the last ``n_last``
+    and, of those between, the ones with the largest ``cache.weights``, the lower place first among equals, NaN as infinity.  They become the
+    sequence's first ``n_keys``, in order; their weights move along, and the bounds of pages that have other keys than before are formed anew.  What keeps its place is not
+    written (pages that sequences share stay as they are if ``n_first`` counts their keys), nor are rows behind the last key.  Returns the sequences' new lengths, int32
+    ``[batch]``, and the places that the keys had, int32 ``[batch, KV heads, n_keys]``, ascending (-1 for sequences of which nothing is given up).  The pages behind the new lengths are the program's again;
+    tokens that are appended afterwards need ``positions``."""
+    _plain(cache)
+    weights = cache._weighed()
+    if not weights:
+        _refuse("keys are given up by their weights, which the cache must have")
+    if not cache._apart:
+        _refuse("keys, values and bounds that share memory cannot be moved")
+    tables, batch, most = cache._tables(page_table, lengths)
+    n_keys, n_first, n_last = _whole("n_keys", n_keys), _whole("n_first", n_first), _whole("n_last", n_last)
+    above = n_keys if above is None else _whole("above", above)
+    if n_first < 0 or n_last < 0 or not 0 < n_keys <= 1 << 20 or n_first + n_last > n_keys or not n_keys <= above < 1 << 31:
+        _refuse(f"{n_keys} keys, the first {n_first} and the last {n_last} among them, of sequences of more than {above} are not supported (1 to 1048576)")
+    if batch * cache.n_kv_heads >= 1 << 24:
+        _refuse(f"{batch} sequences of {cache.n_kv_heads} KV heads are not supported (fewer than 2^24 together)")
+    new_lengths, kept = lengths.new_empty((batch,)), lengths.new_empty((batch, cache.n_kv_heads, n_keys))
+    if batch:
+        lib = _hip.lib()
+        nbytes = lib.aa_paged_evict_workspace_bytes(batch, cache.n_kv_heads, cache.head_dim, n_keys)
+        ws = lengths.new_empty((nbytes >> 2,))
+        cache._launch(lib.aa_paged_evict, _hip.PAGED_EVICTION.pack(*tables, new_lengths.data_ptr(), kept.data_ptr(), weights, ws.data_ptr(), nbytes, batch, most, n_keys,
+                                                                   n_first, n_last, above))
+    return new_lengths, kept
+
+
 def paged_shared_decode_attention(cache: PagedCache, q: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, shared_pages: torch.Tensor,
                                   groups: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`paged_decode_attention` of sequences that begin with the same pages, which are read once for all of them.  Sequences ``groups[g]`` to

@@ -191,6 +191,21 @@ struct PagedPrefixArgs {
 PagedScratch paged_prefix_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim);
 hipError_t launch_paged_prefix(const PagedPrefixArgs& a, hipStream_t stream);
 
+struct PagedEvictArgs {
+  uint16_t* keys; int64_t kp_sp, kp_sh, kp_sn;
+  uint16_t* values; int64_t vp_sp, vp_sh, vp_sn;
+  uint16_t* bounds;  // optional
+  float* weights;
+  const int32_t* table; int64_t t_sb;
+  const int32_t* lengths;
+  int32_t* new_lengths;  // [batch]
+  int32_t* kept;         // [batch, n_kv_heads, n_keys]: places that stay, ascending; -1 where nothing goes
+  uint16_t* rows; float* row_weights;  // scratch: [batch, n_kv_heads, n_keys, 2, head_dim] and [batch, n_kv_heads, n_keys]
+  int batch, n_kv_heads, head_dim, n_pages, page_log, max_pages, n_keys, n_first, n_last, above;
+  int dtype;
+};
+hipError_t launch_paged_evict(const PagedEvictArgs& a, hipStream_t stream);
+
 constexpr int paged_score_pitch(int max_pages) { return (max_pages + 3) & ~3; }
 struct PagedSelectArgs {
   const uint16_t* q; int64_t q_sb, q_sh;

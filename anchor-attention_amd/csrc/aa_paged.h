@@ -16,6 +16,45 @@ __device__ __forceinline__ int pages_of(const int length, const int page_log) { 
 // the nearest page there is
 __device__ __forceinline__ int clamped_page(const int page, const int n_pages) { return min(max(page, 0), n_pages - 1); }
 
+// A score or weight as an unsigned number of the same order; NaN as infinity, -0 as 0.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  x = x != x ? INFINITY : x + 0.f;
+  const uint32_t u = __float_as_uint(x);
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+// Bounds are kept as pairs of 16-bit whole numbers of the same order (-0 below 0, NaN of either sign beyond the infinities), two to an
+// instruction.  There and back:
+__device__ __forceinline__ uint32_t in_order(const uint32_t x) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  const i16x2 signs = *reinterpret_cast<const i16x2*>(&x) >> 15;
+  return x ^ (*reinterpret_cast<const uint32_t*>(&signs) & 0x7fff7fffu);
+}
+__device__ __forceinline__ uint32_t least(const uint32_t a, const uint32_t b) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  const i16x2 m = __builtin_elementwise_min(*reinterpret_cast<const i16x2*>(&a), *reinterpret_cast<const i16x2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t most(const uint32_t a, const uint32_t b) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  const i16x2 m = __builtin_elementwise_max(*reinterpret_cast<const i16x2*>(&a), *reinterpret_cast<const i16x2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+// Back, where both bounds of a channel become NaN if a key was.
+template <typename T>
+__device__ __forceinline__ void bounds_back(uint32_t& lo, uint32_t& hi) {
+  lo = in_order(lo);
+  hi = in_order(hi);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const uint32_t mask = 0x7fffu << (16 * half), most_finite = (uint32_t)T::kExponent << (16 * half);
+    if ((lo & mask) > most_finite || (hi & mask) > most_finite) {
+      lo |= mask;
+      hi |= mask;
+    }
+  }
+}
+
 // One instruction's exchange inside rows of 16 lanes (the lanes are all active); those that receive nothing get `none`.
 constexpr int kDppXor1 = 0xb1, kDppXor2 = 0x4e, kDppHalfMirror = 0x141, kDppRor4 = 0x124, kDppRor8 = 0x128;
 template <int CONTROL, int ROWS = 0xf>

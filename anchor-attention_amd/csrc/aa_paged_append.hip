@@ -73,23 +73,6 @@ __device__ __forceinline__ Rows8 rotated(const Rows8& raw, const Angles& a, cons
   return {pack8<T>(x), pack8<T>(y)};
 }
 
-// Bounds are kept as pairs of 16-bit whole numbers of the same order (-0 below 0, NaN of either sign beyond the infinities), two to an
-// instruction.  There and back:
-__device__ __forceinline__ uint32_t in_order(const uint32_t x) {
-  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
-  const i16x2 signs = *reinterpret_cast<const i16x2*>(&x) >> 15;
-  return x ^ (*reinterpret_cast<const uint32_t*>(&signs) & 0x7fff7fffu);
-}
-__device__ __forceinline__ uint32_t least(const uint32_t a, const uint32_t b) {
-  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
-  const i16x2 m = __builtin_elementwise_min(*reinterpret_cast<const i16x2*>(&a), *reinterpret_cast<const i16x2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&m);
-}
-__device__ __forceinline__ uint32_t most(const uint32_t a, const uint32_t b) {
-  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
-  const i16x2 m = __builtin_elementwise_max(*reinterpret_cast<const i16x2*>(&a), *reinterpret_cast<const i16x2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&m);
-}
 struct Bounds8 {  // of 8 channels of each half
   uint32_t lo[8], hi[8];
   __device__ __forceinline__ void clear() {
@@ -112,22 +95,14 @@ __device__ __forceinline__ void words(const Rows8& x, uint32_t (&w)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) w[j] = in_order(raw[j]);
 }
-// Back, where both bounds become NaN if a key was.
 template <typename T>
 __device__ __forceinline__ void bounds_of(const Bounds8& b, Rows8& lo, Rows8& hi) {
   uint32_t l[8], h[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    l[j] = in_order(b.lo[j]);
-    h[j] = in_order(b.hi[j]);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const uint32_t mask = 0x7fffu << (16 * half), most_finite = (uint32_t)T::kExponent << (16 * half);
-      if ((l[j] & mask) > most_finite || (h[j] & mask) > most_finite) {
-        l[j] |= mask;
-        h[j] |= mask;
-      }
-    }
+    l[j] = b.lo[j];
+    h[j] = b.hi[j];
+    bounds_back<T>(l[j], h[j]);
   }
   lo = {uint4{l[0], l[1], l[2], l[3]}, uint4{l[4], l[5], l[6], l[7]}};
   hi = {uint4{h[0], h[1], h[2], h[3]}, uint4{h[4], h[5], h[6], h[7]}};

@@ -51,14 +51,6 @@ constexpr int kQueryWords = 4096;  // of LDS for a group's queries; those of mor
 
 // A score as an unsigned number of the same order, from 1 to below kEnd - 1; NaN as infinity, -0 as 0.
 constexpr uint32_t kEnd = 0xffffffffu;  // what stands for pages that are taken in any case; 0 stands for no page
-__device__ __forceinline__ uint32_t ordered(float x) {
-  x = x != x ? INFINITY : x + 0.f;
-  const uint32_t u = __float_as_uint(x);
-  return (u >> 31) ? ~u : u | 0x80000000u;
-}
-
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 // Bounds of 8 channels of N pages, and sums of their products with queries in float64.
 //
 // WIDE: products in float64 too.  bf16 has the exponents of float32, in which a product may overflow, or lose bits below 2^-126; those of fp16 do not.  bf16 products are

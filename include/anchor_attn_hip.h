@@ -300,6 +300,13 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
  * the group.  Sequences of fewer keys than these pages hold are attended to by themselves.  What groups and shared_pages hold is clamped to the batch and to
  * [0, max_pages]; where groups do not ascend outputs may be anything.
  *
+ * aa_paged_evict: sequences of more than `above` keys (at least n_keys) are cut down to n_keys keys for each KV head: their first n_first, their last n_last and, of those between,
+ * the ones with the largest weights, the lower place first among equal ones, NaN as infinity.  They become the sequence's first n_keys, in order: keys, values and weights
+ * are moved inside its pages, and the bounds (if the cache has them) of pages whose keys are others than before are formed anew.  What stays in its place
+ * is not written, nor are rows behind the n_keys-th.  new_lengths int32 [batch]: the sequences' keys afterwards (lengths as clamped); it may not be lengths.  kept int32 [batch, n_kv_heads, n_keys]: the places
+ * that the keys had, ascending; -1 for sequences that nothing is taken from.  A page outside the pool is read as the nearest one and not written.  Two sequences must not share
+ * pages that are written.  weights float32 [n_pages, n_kv_heads, page_size], 16-byte aligned; workspace: aa_paged_evict_workspace_bytes() bytes.
+ *
  * aa_paged_sparse_decode_fwd: the same over n_chosen pages for each sequence and KV head, or all where the sequence has no more: its first n_first, its last
  * n_last (at least 1) and those of the others whose score is largest, the lower page first among equal ones.  The score is the largest over the heads of the
  * group of sum_d q_d * (q_d >= 0 ? largest_d : smallest_d), which no product of the query with a key of the page exceeds: exact products, a sum in float64
@@ -350,6 +357,17 @@ typedef struct {
   float norm_eps;
 } aa_paged_more;
 
+/* What aa_paged_evict is given (likewise). */
+typedef struct {
+  const int32_t* page_table; int64_t pt_sb;
+  const int32_t* lengths;
+  int32_t* new_lengths;
+  int32_t* kept;
+  float* weights;
+  void* workspace; size_t workspace_bytes;
+  int batch, max_pages, n_keys, n_first, n_last, above;
+} aa_paged_eviction;
+
 int aa_paged_append(const aa_paged_cache* cache, const aa_paged_tokens* tokens, void* stream);
 int aa_paged_append_more(const aa_paged_cache* cache, const aa_paged_tokens* tokens, const aa_paged_more* more, void* stream);
 size_t aa_paged_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages);
@@ -358,6 +376,8 @@ size_t aa_paged_weighing_workspace_bytes(int batch, int n_q_heads, int n_kv_head
 int aa_paged_weighing_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, float* weights, int n_first, void* stream);
 size_t aa_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages);
 int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, const int32_t* shared_pages, const int32_t* groups, int n_groups, void* stream);
+size_t aa_paged_evict_workspace_bytes(int batch, int n_kv_heads, int head_dim, int n_keys);
+int aa_paged_evict(const aa_paged_cache* cache, const aa_paged_eviction* eviction, void* stream);
 size_t aa_paged_sparse_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_chosen);
 int aa_paged_sparse_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, void* stream);
 

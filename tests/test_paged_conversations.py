@@ -450,3 +450,297 @@ def test_what_steps_refuse():
             torch.func.vmap(lambda x: fn(**{**base, "q": x}))(q[None])
         assert fn(**{**base, "q": q[:0], "page_table": table[:0], "lengths": lengths[:0]}).shape == (0, 4, 64)
     torch.cuda.synchronize()
+
+
+# ---- giving up keys --------------------------------------------------------------------------------------------------
+
+def _kept(weights, n, n_keys, n_first, n_last):
+    """The places by their definition, of a sequence and KV head, sorted on the host."""
+    w = [float("inf") if x != x else x for x in weights.tolist()]
+    best = sorted(range(n_first, n - n_last), key=lambda i: (-w[i], i))[:n_keys - n_first - n_last]
+    return [*range(n_first), *sorted(best), *range(n - n_last, n)]
+
+
+def _evict_and_check(s, cache, n_keys, n_first, n_last, above=None):
+    """All of the cache's tensors and what is returned, bit for bit."""
+    page = s.page
+    want = {x: getattr(cache, x).clone() for x in ("keys", "values", "bounds", "weights")}
+    kept = torch.full((len(s.host), s.hkv, n_keys), -1, dtype=torch.int32)
+    old = {x: t.clone() for x, t in want.items()}
+    for b, n in enumerate(s.host):
+        if n <= (n_keys if above is None else above):
+            continue
+        at = s.table[b, :(n + page - 1) // page].long()
+        for h in range(s.hkv):
+            mine = _kept(old["weights"][at, h].reshape(-1)[:n], n, n_keys, n_first, n_last)
+            kept[b, h] = torch.tensor(mine, dtype=torch.int32)
+            to = at[:(n_keys + page - 1) // page]
+            for x in ("keys", "values", "weights"):
+                rows = want[x][to, h].flatten(0, 1)
+                rows[:n_keys] = old[x][at, h].flatten(0, 1)[torch.tensor(mine, device="cuda")]
+                want[x][to, h] = rows.unflatten(0, (-1, page))
+            changed = next((i for i, x in enumerate(mine) if x != i), n_keys)
+            for i in range(changed // page, (n_keys + page - 1) // page):
+                rows = want["keys"][to[i], h, :min(page, n_keys - i * page)]
+                want["bounds"][to[i], h] = torch.stack((rows.amin(0), rows.amax(0)))
+    lengths, got = _ops().evict_from_pages(cache, s.table, s.lengths, n_keys, n_first, n_last, above)
+    assert got.dtype == lengths.dtype == torch.int32 and torch.equal(got.cpu(), kept)
+    s.host = [n_keys if n > (n_keys if above is None else above) else n for n in s.host]
+    assert lengths.tolist() == s.host
+    for x, t in want.items():
+        mine = getattr(cache, x)
+        assert torch.equal(mine.isnan(), t.isnan()) and torch.equal(mine.nan_to_num(9.0), t.nan_to_num(9.0)), x
+    return lengths
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lengths,hkv,d,page,layout,n_keys,n_first,n_last,above", [
+    (LENGTHS, 8, 128, 64, "heads", 40, 4, 10, None), (LENGTHS, 4, 128, 16, "rows", 16, 0, 0, None), (LENGTHS, 2, 64, 16, "heads", 1, 0, 1, None), (LENGTHS, 2, 64, 32, "part", 33, 0, 1, 64),
+    (LENGTHS, 3, 128, 256, "heads", 300, 17, 30, 301), ([700, 1, 33], 1, 128, 128, "rows", 33, 33, 0, None), ([900, 0], 1, 64, 64, "heads", 700, 100, 600, None),
+    ([20001], 8, 128, 64, "heads", 4096, 4, 500, None), ([9000, 40, 12345], 4, 64, 16, "heads", 8999, 1, 2, None), ([5], 2, 64, 16, "heads", 5, 1, 1, None), ([0], 2, 128, 16, "heads", 3, 0, 0, None),
+    ([130] * 70, 2, 64, 64, "heads", 128, 0, 64, None), ([17], 2, 64, 16, "heads", 1, 0, 0, None), ([70001], 1, 64, 16, "heads", 64000, 0, 1, None), ([1000, 2000], 2, 64, 16, "heads", 100000, 10, 10, None),
+    ([1 << 17], 1, 64, 256, "heads", 1000, 1, 1, None),
+])
+def test_evict(lengths, hkv, d, page, layout, n_keys, n_first, n_last, above, dtype):
+    s = _Setup(lengths, hkv, d, page, dtype, hkv + page, layout, extra=1)
+    cache = _weights_of(s)
+    cache.weights.normal_(generator=s.g).mul_(3).exp_()
+    got = _evict_and_check(s, cache, n_keys, n_first, n_last, above)
+    # once more: nothing is left to give up, or the weights have moved along
+    s.lengths = got
+    _evict_and_check(s, cache, max(1, n_keys // 2), n_first // 2, n_last // 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [50, 3000])
+def test_evict_by_weights_that_are_equal_nan_or_of_any_sign(n):
+    """Equal weights go by place, -0 is 0, NaN is infinity, and negative ones are the smallest."""
+    for seed, values in enumerate(([1.0], [0.0, -0.0, 1e-45], [float("nan"), float("inf"), 1.0, -float("nan")], [-1.0, -float("inf"), 0.0, 1e-38, 2.0], [1.0, 1.0 + 2.0 ** -23, 1.0 + 2.0 ** -22])):
+        s = _Setup([n, n - 7], 2, 64, 16, F16, seed, extra=1)
+        cache = _weights_of(s)
+        cache.weights.copy_(torch.tensor(values, device="cuda")[torch.randint(len(values), cache.weights.shape, generator=s.g, device="cuda")])
+        _evict_and_check(s, cache, n // 2, 3, 5)
+
+
+@pytest.mark.gpu
+def test_bounds_of_moved_keys_that_are_nan_or_infinite():
+    s = _Setup([200], 2, 64, 16, F16, 6)
+    cache = _weights_of(s)
+    cache.weights.uniform_(generator=s.g)
+    at = s.table[0].long()
+    cache.keys[at[11], 0, 3, 5], cache.keys[at[10], 0, 2, 6], cache.keys[at[9], 1, 1, 7], cache.keys[at[8], 1, 1, 8] = float("nan"), float("inf"), float("-inf"), -float("nan")
+    for i, h, r in ((11, 0, 3), (10, 0, 2), (9, 1, 1), (8, 1, 1)):
+        cache.weights[at[i], h, r] = 2.0
+    _evict_and_check(s, cache, 60, 1, 1)
+    seen = torch.cat([cache.bounds[at[i], h].flatten() for i in range(4) for h in range(2)])
+    assert int(seen.isnan().sum()) == 4 and int(seen.isinf().sum()) == 2
+
+
+@pytest.mark.gpu
+def test_evict_without_bounds_and_of_what_does_not_fit():
+    """Lengths above the table are its size; a page outside the pool is read as the nearest one and not written."""
+    s = _Setup([64, 64, 64, 64], 2, 64, 16, BF16, 10)
+    keys, values = s.cache.keys.nan_to_num(0.5), s.cache.values.nan_to_num(0.5)
+    cache = _ops().PagedCache(keys, values, None, torch.rand(keys.shape[:3], generator=s.g, device="cuda"))
+    before = keys.clone(), values.clone(), cache.weights.clone()
+    s.table[1, 0], s.table[2, 3] = -5, 2 ** 31 - 1
+    lengths, kept = _ops().evict_from_pages(cache, s.table, _int32([1000, 64, 64, -3]), 20, 2, 3)
+    assert lengths.tolist() == [20, 20, 20, 0] and bool((kept[3] == -1).all())
+    for b, pages in ((0, s.table[0]), (1, torch.cat((_int32([0]), s.table[1, 1:]))), (2, torch.cat((s.table[2, :3], _int32([cache.n_pages - 1]))))):
+        for h in range(2):
+            mine = _kept(before[2][pages.long(), h].reshape(-1), 64, 20, 2, 3)
+            assert kept[b, h].tolist() == mine
+            for i, x in enumerate(mine):
+                if b == 1 and i < 16:
+                    continue  # (in a page outside the pool)
+                for t, u in ((keys, before[0]), (values, before[1]), (cache.weights, before[2])):
+                    assert torch.equal(t[int(pages[i // 16]), h, i % 16], u[int(pages[x // 16]), h, x % 16])
+    written = {int(x) for x in torch.cat((s.table[0, :2], s.table[1, 1:2], s.table[2, :2]))}
+    for t, u in zip((keys, values, cache.weights), before):
+        assert all(torch.equal(t[i], u[i]) for i in range(cache.n_pages) if i not in written)
+
+
+EVICTION = {"page_table": 4096, "pt_sb": 8, "lengths": 4096, "new_lengths": 4096, "kept": 4096, "weights": 4096, "workspace": 4096, "workspace_bytes": 1 << 40, "batch": 2, "max_pages": 8,
+            "n_keys": 10, "n_first": 2, "n_last": 3, "above": 12}
+
+
+@pytest.mark.parametrize("change,message", [
+    *[(c, m) for c, m in EVERY if not {"q", "q_sh"} & set(c) and m != "must divide"], ({"weights": 0}, "weights is NULL"), ({"weights": 4100}, "weights must be 16-byte"),
+    ({"new_lengths": 0}, "new_lengths is NULL"), ({"kept": 0}, "kept is NULL"), ({"kept": 6}, "kept must be 4-byte"), ({"workspace": 0}, "workspace is NULL"), ({"workspace_bytes": 100}, "workspace has 100 bytes"),
+    ({"n_keys": 0}, "not supported"), ({"n_keys": 4}, "not supported"), ({"n_first": -1}, "not supported"), ({"n_last": -1}, "not supported"), ({"n_first": 8}, "not supported"),
+    ({"n_first": 2 ** 31 - 1, "n_last": 2 ** 31 - 1}, "not supported"), ({"above": 9}, "not supported"), ({"n_keys": (1 << 20) + 1, "above": 1 << 21}, "not supported"),
+    ({"batch": 65535, "n_kv_heads": 512, "kp_sh": 128}, "2\\^24"),
+])
+def test_what_the_c_interface_of_eviction_refuses(change, message):
+    """Before anything is launched: the addresses are never read."""
+    from anchor_attn.src.ops import _hip
+    assert set(change) <= {*EVICTION, *CACHE, "cache", "given"}
+    struct = _hip.PagedCacheStruct(*{**CACHE, **{k: v for k, v in change.items() if k in CACHE}}.values())
+    with pytest.raises(_hip.AnchorAttnHipError, match=message):
+        _hip.check(_hip.lib().aa_paged_evict(None if "cache" in change else ctypes.addressof(struct),
+                                             None if "given" in change else _hip.PAGED_EVICTION.pack(*{**EVICTION, **{k: v for k, v in change.items() if k in EVICTION}}.values()), None))
+
+
+def test_packed_eviction_is_laid_out_as_in_c(tmp_path):
+    from anchor_attn.src.ops import _hip
+    size, at = _sizes_in_c(tmp_path, "sizeof(aa_paged_eviction)", "offsetof(aa_paged_eviction, above)")
+    assert size == _hip.PAGED_EVICTION.size and _hip.PAGED_EVICTION.pack(*range(14))[at] == 13
+    assert _hip.lib().aa_paged_evict_workspace_bytes(2, 3, 128, 10) >= 2 * 3 * 10 * (4 * 128 + 4)
+    assert _hip.lib().aa_paged_evict_workspace_bytes(2, 3, 128, 0) == 0 == _hip.lib().aa_paged_evict_workspace_bytes(2, 3, 96, 8)
+
+
+@pytest.mark.gpu
+def test_what_evicting_refuses():
+    from anchor_attn.src.ops import _hip
+    ops = _ops()
+    cache = ops.PagedCache.empty(5, 2, 16, 64, weights=True)
+    for t in (cache.keys, cache.values, cache.weights, cache.bounds):
+        t.zero_()
+    table, lengths = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    good = {"cache": cache, "page_table": table, "lengths": lengths, "n_keys": 8, "n_first": 2, "n_last": 3, "above": 9}
+    ops.evict_from_pages(**good)
+    twice = torch.zeros(5, 2, 16, 64, dtype=BF16, device="cuda")
+    for change in ({"n_keys": 0}, {"n_keys": 4}, {"n_keys": 7.5}, {"n_keys": None}, {"n_keys": (1 << 20) + 1, "above": None}, {"n_first": -1}, {"n_last": -1}, {"n_first": 6}, {"above": 7}, {"above": 1 << 31},
+                   {"above": 9.5}, {"page_table": table.long()}, {"page_table": table[:1]}, {"lengths": lengths.cpu()}, {"lengths": [0, 0]}, {"cache": ops.PagedCache(cache.keys, cache.values)},
+                   {"cache": ops.PagedCache(twice, twice, None, cache.weights)}, {"cache": 1}):
+        with pytest.raises(_hip.AnchorAttnHipError):
+            ops.evict_from_pages(**{**good, **change})
+    assert ops.evict_from_pages(**{**good, "page_table": table[:0], "lengths": lengths[:0]})[1].shape == (0, 2, 8)
+    cache.weights.data = torch.zeros_like(cache.weights)
+    with pytest.raises(_hip.AnchorAttnHipError, match="other memory"):
+        ops.evict_from_pages(**good)
+
+
+# ---- together --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+def test_conversations_that_share_a_prompt_and_give_up_keys():
+    """A prompt with norms through the prefill operator and into pages that four conversations share, then steps that append, attend over the shared pages, count
+    attention and give up keys behind them; every step against float64 attention over what the cache holds.  The same steps as one captured graph, replayed with eager
+    work between, and two such graphs in turn."""
+    from anchor_attn.src.ops.anchor_attn_v4 import anchor_attn
+    ops = _ops()
+    n, batch, hq, hkv, d, page, steps, keep, above = 2048, 4, 8, 2, 128, 64, 6, 2048 + 40, 2048 + 41
+    g = torch.Generator(device="cuda").manual_seed(21)
+    q, k, v = (torch.randn(n, h, d, generator=g, device="cuda").to(BF16) for h in (hq, hkv, hkv))
+    wq, wk = ((1 + 0.3 * torch.randn(d, generator=g, device="cuda")).to(BF16) for _ in range(2))
+    cos, sin = _tables(4096, d)
+    new = [tuple(torch.randn(batch, h, d, generator=g, device="cuda").to(BF16) for h in (hq, hkv, hkv)) for _ in range(steps)]
+    more = {"q_norm": wq, "k_norm": wk}
+
+    def begin():
+        s = _Setup([n] + [0] * (batch - 1), hkv, d, page, BF16, 22, room=300)
+        own = s.table[:, n // page:n // page + 3].clone()
+        s.table[1:, n // page:n // page + 3] = s.table[1:, :3]
+        s.table[0, n // page:n // page + 3] = own[0]
+        s.table[1:, :n // page] = s.table[0, :n // page]
+        s.cache = _weights_of(s)
+        k_out = torch.empty_like(k)
+        q_out = ops.append_to_pages(s.cache, q, k, v, cos, sin, s.table[:1], _int32([n]), _int32([0, n]), k_out=k_out, **more)
+        assert anchor_attn(q_out.transpose(0, 1)[None], k_out.transpose(0, 1)[None], v.transpose(0, 1)[None], return_computational_ratio=False).shape == (1, hq, n, d)
+        assert bool((s.cache.weights[s.table[0, :n // page].long()] == 0).all())
+        # their own beginnings, of different lengths
+        own = [30, 41, 1, 37]
+        x = [torch.randn(sum(own), h, d, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").to(BF16) for h in (hkv, hkv)]
+        s.host = [n + m for m in own]
+        s.lengths = _int32(s.host)
+        ops.append_to_pages(s.cache, None, *x, cos, sin, s.table, s.lengths, _int32([0, 30, 71, 72, 109]), k_norm=wk)
+        s.positions = s.lengths.clone()
+        return s
+
+    shared = _int32([n // page])
+
+    def step(s, x):
+        s.lengths += 1
+        s.positions += 1
+        rotated = ops.append_to_pages(s.cache, *x, cos, sin, s.table, s.lengths, positions=s.positions, **more)
+        out = ops.paged_shared_decode_attention(s.cache, rotated, s.table, s.lengths, shared)
+        same = ops.paged_weighing_decode_attention(s.cache, rotated, s.table, s.lengths, n_first=n)
+        had = s.lengths.clone()
+        lengths, kept = ops.evict_from_pages(s.cache, s.table, s.lengths, keep, n_first=n, n_last=8, above=above)
+        s.lengths.copy_(lengths)
+        return rotated, out, same, had, kept, lengths
+
+    s, eager = begin(), []
+    prompt = s.cache.keys[s.table[0, :n // page].long()].clone()
+    for i, x in enumerate(new):
+        outs = step(s, x)
+        eager.append([t.clone() for t in outs] + [t.clone() for t in (s.cache.keys, s.cache.values, s.cache.bounds, s.cache.weights)])
+    # (each step once more, looked at before keys are given up)
+    s = begin()
+    gone = 0
+    for i, x in enumerate(new):
+        s.lengths += 1
+        s.positions += 1
+        s.host = s.lengths.tolist()
+        rotated = ops.append_to_pages(s.cache, *x, cos, sin, s.table, s.lengths, positions=s.positions, **more)
+        _near(rotated, x[0], wq, 1e-6, cos[s.positions.long() - 1], sin[s.positions.long() - 1])
+        out = ops.paged_shared_decode_attention(s.cache, rotated, s.table, s.lengths, shared)
+        _close(out, rotated, s, d ** -0.5)
+        before = s.cache.weights.clone()
+        same = ops.paged_weighing_decode_attention(s.cache, rotated, s.table, s.lengths, n_first=n)
+        _close(same, rotated, s, d ** -0.5)
+        _weights_close(s.cache.weights, before, rotated, s, d ** -0.5, n)
+        assert all(torch.equal(a, b) for a, b in zip((rotated, out, same), eager[i]))
+        s.lengths = _evict_and_check(s, s.cache, keep, n, 8, above)
+        gone += int(eager[i][3].sum() - s.lengths.sum())
+        assert torch.equal(s.lengths, eager[i][5]) and torch.equal(s.cache.keys[s.table[0, :n // page].long()], prompt)
+        assert bool((s.cache.weights[s.table[0, :n // page].long()] == 0).all())
+    assert gone >= 8 and int((s.positions - s.lengths).sum()) == gone
+
+    graphs = []
+    for _ in range(2):
+        s, x = begin(), tuple(t.clone() for t in new[0])
+        kept_state = [t.clone() for t in (s.lengths, s.positions, s.cache.keys, s.cache.values, s.cache.bounds, s.cache.weights)]
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(s, x)  # (warm-up; what it changed is set back)
+        torch.cuda.current_stream().wait_stream(side)
+        with torch.cuda.graph(graph):
+            outs = step(s, x)
+        for a, b in zip((s.lengths, s.positions, s.cache.keys, s.cache.values, s.cache.bounds, s.cache.weights), kept_state):
+            a.copy_(b)
+        graphs.append((s, x, graph, outs))
+    for i in range(steps):
+        for s, x, graph, outs in graphs:
+            for a, b in zip(x, new[i]):
+                a.copy_(b)
+            graph.replay()
+        step(begin(), new[0])  # (eager work between the replays)
+        torch.cuda.synchronize()
+        for s, _, _, outs in graphs:
+            for a, b in zip((*outs, s.cache.keys, s.cache.values, s.cache.bounds, s.cache.weights), eager[i]):
+                assert torch.equal(a.nan_to_num(9.0), b.nan_to_num(9.0))
+
+
+@pytest.mark.gpu
+def test_steps_on_two_streams_at_once():
+    """Two caches, each on a stream of its own, without waiting in between: the results of one after the other."""
+    ops = _ops()
+
+    def begin(seed):
+        s, shared, groups = _shared_setup([30, 5], [9, 3], [400, 70, 3], 4, 128, 64, BF16, seed)
+        s.cache = _weights_of(s)
+        s.cache.weights.zero_()
+        return s, s.queries(16), shared, groups
+
+    def work(s, q, shared, groups):
+        out = ops.paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+        # (one sequence of each group, which share nothing)
+        table, lengths = s.table[8:10], s.lengths[8:10]
+        weighed = ops.paged_weighing_decode_attention(s.cache, q[8:10], table, lengths)
+        return (out, weighed, *ops.evict_from_pages(s.cache, table, lengths, 300, 10, 20), s.cache.keys.clone(), s.cache.weights.clone())
+
+    want = [work(*begin(i)) for i in range(2)]
+    mine = [begin(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for x, stream in zip(mine, streams):
+        with torch.cuda.stream(stream):
+            got.append(work(*x))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x.nan_to_num(9.0), y.nan_to_num(9.0)) for x, y in zip(a, b))
