@@ -375,8 +375,8 @@ def evict_from_pages(cache: PagedCache, page_table: torch.Tensor, lengths: torch
     if batch:
         lib = _hip.lib()
         nbytes = lib.aa_paged_evict_workspace_bytes(batch, cache.n_kv_heads, cache.head_dim, n_keys)
-        ws = lengths.new_empty((nbytes >> 2,))
-        cache._launch(lib.aa_paged_evict, _hip.PAGED_EVICTION.pack(*tables, new_lengths.data_ptr(), kept.data_ptr(), weights, ws.data_ptr(), nbytes, batch, most, n_keys,
+        ws = lengths.new_empty((nbytes >> 2,)) if nbytes else None
+        cache._launch(lib.aa_paged_evict, _hip.PAGED_EVICTION.pack(*tables, new_lengths.data_ptr(), kept.data_ptr(), weights, ws.data_ptr() if nbytes else 0, nbytes, batch, most, n_keys,
                                                                    n_first, n_last, above))
     return new_lengths, kept
 

@@ -1127,6 +1127,7 @@ static size_t evict_rows_bytes(int batch, int n_kv_heads, int head_dim, int n_ke
 
 size_t aa_paged_evict_workspace_bytes(int batch, int n_kv_heads, int head_dim, int n_keys) {
   if (n_keys <= 0 || n_keys > 1 << 20 || check_paged("aa_paged_evict_workspace_bytes", batch, 0, n_kv_heads, head_dim, 16, 1)) return 0;
+  if (paged_evict_group_rows(batch, n_kv_heads, head_dim, n_keys) >= n_keys) return 0;
   return evict_rows_bytes(batch, n_kv_heads, head_dim, n_keys) + (size_t)batch * n_kv_heads * n_keys * 4;
 }
 
@@ -1134,8 +1135,7 @@ int aa_paged_evict(const aa_paged_cache* cache, const aa_paged_eviction* t, void
   const char* who = "aa_paged_evict";
   int rc;
   if ((rc = check_given(t, who, "eviction")) || (rc = check_cache(who, cache, t->batch, 0, t->max_pages, t->page_table, t->lengths)) ||
-      (rc = check_ptr(t->weights, who, "weights")) || (rc = check_words(t->new_lengths, who, "new_lengths")) || (rc = check_words(t->kept, who, "kept")) ||
-      (rc = check_ptr(t->workspace, who, "workspace")))
+      (rc = check_ptr(t->weights, who, "weights")) || (rc = check_words(t->new_lengths, who, "new_lengths")) || (rc = check_words(t->kept, who, "kept")))
     return rc;
   if (t->n_keys <= 0 || t->n_first < 0 || t->n_last < 0 || (int64_t)t->n_first + t->n_last > t->n_keys || t->above < t->n_keys) {
     set_error("%s: %d keys, the first %d and the last %d among them, of sequences of more than %d are not supported (at least 1, and no more than these have)", who,
@@ -1147,6 +1147,7 @@ int aa_paged_evict(const aa_paged_cache* cache, const aa_paged_eviction* t, void
     return AA_EUNSUPPORTED;
   }
   const size_t needed = aa_paged_evict_workspace_bytes(t->batch, cache->n_kv_heads, cache->head_dim, t->n_keys);
+  if (needed > 0 && (rc = check_ptr(t->workspace, who, "workspace"))) return rc;
   if (t->workspace_bytes < needed) {
     set_error("%s: workspace has %zu bytes, %zu needed", who, t->workspace_bytes, needed);
     return AA_EBADARG;
@@ -1155,7 +1156,7 @@ int aa_paged_evict(const aa_paged_cache* cache, const aa_paged_eviction* t, void
   const PagedEvictArgs a = {(uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn, (uint16_t*)cache->values, cache->vp_sp, cache->vp_sh, cache->vp_sn,
                             (uint16_t*)cache->bounds, t->weights, t->page_table, t->pt_sb, t->lengths, t->new_lengths, t->kept, (uint16_t*)ws,
                             (float*)(ws + evict_rows_bytes(t->batch, cache->n_kv_heads, cache->head_dim, t->n_keys)), t->batch, cache->n_kv_heads, cache->head_dim,
-                            cache->n_pages, log2_of(cache->page_size), t->max_pages, t->n_keys, t->n_first, t->n_last, t->above, cache->dtype};
+                            cache->n_pages, log2_of(cache->page_size), t->max_pages, t->n_keys, t->n_first, t->n_last, t->above, cache->dtype, 0};
   return check_launch(launch_paged_evict(a, (hipStream_t)stream), who);
 }
 

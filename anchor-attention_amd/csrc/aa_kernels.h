@@ -203,7 +203,9 @@ struct PagedEvictArgs {
   uint16_t* rows; float* row_weights;  // scratch: [batch, n_kv_heads, n_keys, 2, head_dim] and [batch, n_kv_heads, n_keys]
   int batch, n_kv_heads, head_dim, n_pages, page_log, max_pages, n_keys, n_first, n_last, above;
   int dtype;
+  int group_rows;  // set by the launcher
 };
+int paged_evict_group_rows(int batch, int n_kv_heads, int head_dim, int n_keys);  // rows that are moved in turn; scratch is used where these are not all
 hipError_t launch_paged_evict(const PagedEvictArgs& a, hipStream_t stream);
 
 constexpr int paged_score_pitch(int max_pages) { return (max_pages + 3) & ~3; }

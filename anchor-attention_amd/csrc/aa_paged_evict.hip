@@ -1,186 +1,403 @@
 // Giving up the keys of a cache in pages that have had the least attention, on gfx950: which ones stay, and their move to the front of the sequence's pages.
 //
-// Choosing: a work-group for each (sequence, KV head) finds the weight that the wanted number of candidates reaches, by histograms of 8 bits of the weights' order at a time,
-// and then lists the places in order, chunk by chunk, with sums over the work-group.  Integers only: the order in which counts are added does not matter.
-// Moving is bound by reading and writing the rows once.  It is in place, and a row goes to a lower place: rows that lie where others will go (below the n_keys-th) are copied to
-// scratch by a launch of its own first, the others are read where they are, which nothing writes.  A work-group has a page of a KV head, whose bounds it forms.
+// Choosing: a work-group for each (sequence, KV head) finds what the wanted number of weights reaches by histograms of 256 equal ranges of the weights' order, each inside the range
+// of the last one that holds it, as pages are chosen for sparse steps, and lists the places in order by sums over the work-group.  Integers only: the order in which counts are added
+// does not matter.  Weights stay in LDS between the rounds, or are read again where there are more than it holds.
+//
+// Moving is bound by reading and writing the rows once.  It is in place, and rows go to lower places in their order, so a work-group that takes them in turn, each chunk read by all before
+// any of it is written, needs no room beside: no later row lies where an earlier one goes.  A work-group has 64 channels of keys or values, a line of the cache; where that makes too few
+// work-groups, the rows of a (sequence, KV head) are cut into groups, and those that come from another group's places are copied to scratch by a launch of its own first.
+#include <algorithm>
+
 #include "aa_kernels.h"
 #include "aa_paged.h"
 
 namespace aa {
 
-constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
+constexpr int kKeepThreads = 1024, kKeepWaves = kKeepThreads / 64, kKeepStep = 4 * kKeepThreads;
+constexpr int kKeepInLds = 36864;                     // weights that LDS holds
+constexpr int kMostKeys = 1 << 20;
 
-__global__ void __launch_bounds__(kEvictThreads) paged_keep_kernel(const PagedEvictArgs p) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t counts[kEvictWaves][2], found[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = blockIdx.x / p.n_kv_heads, kvh = blockIdx.x % p.n_kv_heads;
+__global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedEvictArgs p) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t stay[];  // the weights, or where there are too many of them, the counts
+  static_assert(kMostKeys / kKeepStep * kKeepWaves * 2 <= kKeepInLds, "the counts take less room");
+  __shared__ __attribute__((aligned(16))) uint32_t bins[4][256];
+  __shared__ uint32_t ranges[2][kKeepWaves];
+  __shared__ uint64_t few_counts[kKeepInLds / kKeepStep * kKeepWaves];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int b = blockIdx.x / p.n_kv_heads, kvh = blockIdx.x - b * p.n_kv_heads;
   const int n = clamped_length(p.lengths, b, p.max_pages, p.page_log);
   int32_t* kept = p.kept + (int64_t)blockIdx.x * p.n_keys;
   if (kvh == 0 && tid == 0) p.new_lengths[b] = n > p.above ? p.n_keys : n;
   if (n <= p.above) {
-    for (int i = tid; i < p.n_keys; i += kEvictThreads) kept[i] = -1;
+    for (int i = tid; i < p.n_keys; i += kKeepThreads) kept[i] = -1;
     return;
   }
+  const bool in_lds = n <= kKeepInLds;
+  uint64_t* counts = in_lds ? few_counts : reinterpret_cast<uint64_t*>(stay);
   const int first = p.n_first, end = n - p.n_last;  // the candidates
-  auto key_at = [&](const int i) {
+  bins[0][tid] = 0u;
+  // weights as numbers of the same order; 0 for what is no candidate
+  auto load = [&](const int i, uint32_t (&x)[4]) {
     const int64_t page = clamped_page(p.table[b * p.t_sb + (i >> p.page_log)], p.n_pages);
-    return ordered(p.weights[((page * p.n_kv_heads + kvh) << p.page_log) + (i & ((1 << p.page_log) - 1))]);
+    const floatx4 w = *reinterpret_cast<const floatx4*>(p.weights + ((page * p.n_kv_heads + kvh) << p.page_log) + (i & ((1 << p.page_log) - 1)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = i + e >= first && i + e < end ? ordered(w[e]) : 0u;
   };
-  uint32_t want = p.n_keys - p.n_first - p.n_last, prefix = 0;  // of them, those of this prefix and not above it
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int i = first + tid; i < end; i += kEvictThreads) {
-      const uint32_t x = key_at(i);
-      if (shift == 24 || x >> (shift + 8) == prefix) atomicAdd(&hist[x >> shift & 255u], 1u);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      uint32_t left = want, bin = 255;
-      while (bin > 0 && hist[bin] < left) left -= hist[bin--];
-      found[0] = bin;
-      found[1] = left;
-    }
-    __syncthreads();
-    prefix = prefix << 8 | found[0];
-    want = found[1];
-  }
-  // larger ones all, `want` of the equal ones
-  for (int i = tid; i < first; i += kEvictThreads) kept[i] = i;
-  for (int i = tid; i < p.n_last; i += kEvictThreads) kept[p.n_keys - p.n_last + i] = end + i;
-  uint32_t above = 0, equal = 0;  // before this chunk
-  for (int i0 = first; i0 < end; i0 += kEvictThreads) {
-    const int i = i0 + tid;
-    const uint32_t x = i < end ? key_at(i) : 0u;
-    const bool gt = i < end && x > prefix, eq = i < end && x == prefix;
-    const uint64_t gts = __ballot(gt), eqs = __ballot(eq);
-    if (lane == 0) {
-      counts[wave][0] = __popcll(gts);
-      counts[wave][1] = __popcll(eqs);
-    }
-    __syncthreads();
-    uint32_t a = above, e = equal;
-    for (int w = 0; w < kEvictWaves; ++w) {
-      if (w == wave) {
-        const uint64_t before = (1ull << lane) - 1;
-        a += __popcll(gts & before);
-        e += __popcll(eqs & before);
-        if (gt || (eq && e < want)) kept[first + a + min(e, want)] = i;
+  const int items = (n + kKeepStep - 1) / kKeepStep;
+  auto each = [&](auto&& f) {  // f(j, numbers): item j of a thread is four keys
+#pragma nounroll
+    for (int j = 0; j < items; ++j) {
+      const int i = kKeepStep * j + 4 * tid;
+      uint32_t x[4] = {0u, 0u, 0u, 0u};
+      if (i < n) {
+        if (in_lds) {
+          const uint4 y = *reinterpret_cast<const uint4*>(stay + i);
+          x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+        } else {
+          load(i, x);
+        }
       }
-      above += counts[w][0];
-      equal += counts[w][1];
-      if (w < wave) {
-        a = above;
-        e = equal;
+      f(j, x);
+    }
+  };
+  uint32_t lo = 0xffffffffu, hi = 0u;
+  auto extend = [&](const uint32_t (&x)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      lo = min(lo, x[e] - 1u);  // (0 becomes the largest; no number is)
+      hi = max(hi, x[e]);
+    }
+  };
+  if (in_lds) {
+#pragma unroll 4
+    for (int i = 4 * tid; i < n; i += kKeepStep) {
+      uint32_t x[4];
+      load(i, x);
+      *reinterpret_cast<uint4*>(stay + i) = uint4{x[0], x[1], x[2], x[3]};
+      extend(x);
+    }
+  } else {
+    each([&](const int, const uint32_t (&x)[4]) { extend(x); });
+  }
+  lo = up_to(lo, 0xffffffffu, [](const uint32_t a, const uint32_t b) { return min(a, b); });
+  hi = up_to(hi, 0u, [](const uint32_t a, const uint32_t b) { return max(a, b); });
+  if (lane == 63) {
+    ranges[0][wave] = lo;
+    ranges[1][wave] = hi;
+  }
+  __syncthreads();  // (the bins are 0 too)
+#pragma unroll
+  for (int w = 0; w < kKeepWaves; ++w) {
+    lo = w == 0 ? ranges[0][0] : min(lo, ranges[0][w]);
+    hi = w == 0 ? ranges[1][0] : max(hi, ranges[1][w]);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo) + 1u;
+  hi = __builtin_amdgcn_readfirstlane(hi);
+  // The wanted-th largest weight lies from lo to hi; all of those above are taken.  A range is 2^32 long at most and the next one a 256th, so four do.
+  int wanted = p.n_keys - p.n_first - p.n_last;
+  if (wanted == 0) lo = hi = 0xffffffffu;  // (none)
+#pragma nounroll
+  for (int round = 0; wanted > 0 && lo < hi; ++round) {
+    const uint32_t span = hi - lo;
+    const int shift = span < 256u ? 0 : 24 - __builtin_clz(span);  // span >> shift < 256
+    uint32_t least_ones = 0;  // (not one by one: weights that nothing has been added to are alike)
+    each([&](const int, const uint32_t (&x)[4]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t d = x[e] - lo;
+        if (d == 0u) ++least_ones;
+        else if (d <= span) atomicAdd(&bins[round][d >> shift], 1u);
       }
-    }
+    });
+    least_ones = (uint32_t)sums_up_to((int)least_ones);
+    if (lane == 63 && least_ones > 0) atomicAdd(&bins[round][0], least_ones);
     __syncthreads();
-  }
-}
-
-// Where row i of a (sequence, KV head) is.
-struct EvictRow {
-  int64_t k, v, w;
-  bool ok;
-};
-__device__ __forceinline__ EvictRow row_at(const PagedEvictArgs& p, const int b, const int kvh, const int i) {
-  const int page = p.table[b * p.t_sb + (i >> p.page_log)], slot = i & ((1 << p.page_log) - 1);
-  const int64_t at = clamped_page(page, p.n_pages);
-  return {at * p.kp_sp + kvh * p.kp_sh + slot * p.kp_sn, at * p.vp_sp + kvh * p.vp_sh + slot * p.vp_sn, ((at * p.n_kv_heads + kvh) << p.page_log) + slot, at == page};
-}
-
-// Rows that move from where others go, to scratch.
-template <int D>
-__global__ void __launch_bounds__(256) paged_save_kernel(const PagedEvictArgs p) {
-  constexpr int kPieces = D / 8, kSide = 256 / kPieces;
-  const int c = threadIdx.x % kPieces, kvh = blockIdx.y, b = blockIdx.z;
-  const int64_t unit = ((int64_t)b * p.n_kv_heads + kvh) * p.n_keys;
-  const int begin = blockIdx.x << p.page_log, end = min(begin + (1 << p.page_log), p.n_keys);
-  for (int i = begin + threadIdx.x / kPieces; i < end; i += kSide) {
-    const int from = p.kept[unit + i];
-    if (from < 0 || from == i || from >= p.n_keys) continue;
-    const EvictRow x = row_at(p, b, kvh, from);
-    uint16_t* to = p.rows + (unit + i) * 2 * D + 8 * c;
-    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(p.keys + x.k + 8 * c);
-    *reinterpret_cast<uint4*>(to + D) = *reinterpret_cast<const uint4*>(p.values + x.v + 8 * c);
-    if (c == 0) p.row_weights[unit + i] = p.weights[x.w];
-  }
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_move_kernel(const PagedEvictArgs p) {
-  constexpr int kPieces = D / 8, kSide = 256 / kPieces;
-  __shared__ uint32_t red[4][kPieces][8];
-  const int tid = threadIdx.x, lane = tid & 63, c = tid % kPieces, kvh = blockIdx.y, b = blockIdx.z;
-  const int64_t unit = ((int64_t)b * p.n_kv_heads + kvh) * p.n_keys;
-  const int begin = blockIdx.x << p.page_log, end = min(begin + (1 << p.page_log), p.n_keys);
-  // (a page stays as it is if its last row does and none is taken from behind that)
-  const int last = p.kept[unit + end - 1];
-  if (last < 0 || (last == end - 1 && end - begin == 1 << p.page_log)) return;
-  uint32_t lo[4] = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu}, hi[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-  for (int i = begin + tid / kPieces; i < end; i += kSide) {
-    const int from = p.kept[unit + i];
-    const EvictRow to = row_at(p, b, kvh, i), x = row_at(p, b, kvh, from);
-    const bool saved = from != i && from < p.n_keys;
-    const uint16_t* rows = p.rows + (unit + i) * 2 * D;
-    const uint4 k = *reinterpret_cast<const uint4*>((saved ? rows : p.keys + x.k) + 8 * c);
-    if (from != i && to.ok) {
-      const uint4 v = *reinterpret_cast<const uint4*>((saved ? rows + D : p.values + x.v) + 8 * c);
-      const float w = saved ? p.row_weights[unit + i] : p.weights[x.w];
-      *reinterpret_cast<uint4*>(p.keys + to.k + 8 * c) = k;
-      *reinterpret_cast<uint4*>(p.values + to.v + 8 * c) = v;
-      if (c == 0) p.weights[to.w] = w;
+    const uint4 bin4 = *reinterpret_cast<const uint4*>(&bins[round][4 * lane]);
+    const int m[4] = {(int)bin4.x, (int)bin4.y, (int)bin4.z, (int)bin4.w};
+    const int own = m[0] + m[1] + m[2] + m[3], sums = sums_up_to(own), all = __builtin_amdgcn_readlane(sums, 63);
+    // the last lane that has `wanted` weights in its bins or behind them, and the last of its bins that has
+    const int at = 63 - __builtin_clzll(__ballot(all - sums + own >= wanted));
+    int above = __builtin_amdgcn_readlane(all - sums, at), in_bin = 0, bin = 4 * at;
+#pragma unroll
+    for (int j = 3; j >= 0; --j) {
+      in_bin = __builtin_amdgcn_readlane(m[j], at);
+      if (above + in_bin >= wanted) {
+        bin += j;
+        break;
+      }
+      above += in_bin;
     }
-    const uint32_t words[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      lo[j] = least(lo[j], in_order(words[j]));
-      hi[j] = most(hi[j], in_order(words[j]));
-    }
+    wanted -= above;  // of this bin
+    lo += (uint32_t)bin << shift;
+    hi = lo + min(hi - lo, (1u << shift) - 1u);
+    if (shift == 0 || wanted == in_bin) break;  // (one number is left, or all of the bin are taken)
   }
-  if (p.bounds == nullptr) return;
+
+  // Weights above hi are taken, and of those from lo to hi the first `wanted`: counted by item and wave, which is the keys' order.
+  auto counts_of = [&](const uint32_t (&x)[4]) {  // of an item, in the upper and the lower half
+    uint32_t packed = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int d = 32; d >= kPieces; d >>= 1) {
-      lo[j] = least(lo[j], __shfl_xor(lo[j], d, 64));
-      hi[j] = most(hi[j], __shfl_xor(hi[j], d, 64));
-    }
-  if (lane < kPieces) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      red[tid >> 6][c][j] = lo[j];
-      red[tid >> 6][c][4 + j] = hi[j];
+    for (int e = 0; e < 4; ++e) packed += (x[e] - lo <= hi - lo ? 0x10000u : 0u) + (x[e] > hi ? 1u : 0u);
+    return packed;
+  };
+  each([&](const int j, const uint32_t (&x)[4]) {
+    const uint32_t all = (uint32_t)sums_up_to((int)counts_of(x));
+    if (lane == 63) counts[kKeepWaves * j + wave] = (uint64_t)(all >> 16) << 32 | (all & 0xffffu);
+  });
+  __syncthreads();
+  if (wave == 0) {  // (sums of all before each)
+    uint32_t so_far_equal = 0, so_far_sure = 0;
+#pragma nounroll
+    for (int i = 0; i < items * kKeepWaves; i += 64) {
+      const uint64_t x = i + lane < items * kKeepWaves ? counts[i + lane] : 0u;
+      const uint32_t equal = (uint32_t)(x >> 32), sure = (uint32_t)x;
+      const uint32_t equals = (uint32_t)sums_up_to((int)equal), sures = (uint32_t)sums_up_to((int)sure);
+      if (i + lane < items * kKeepWaves) counts[i + lane] = (uint64_t)(so_far_equal + equals - equal) << 32 | (so_far_sure + sures - sure);
+      so_far_equal += __builtin_amdgcn_readlane(equals, 63);
+      so_far_sure += __builtin_amdgcn_readlane(sures, 63);
     }
   }
   __syncthreads();
-  const int page = p.table[b * p.t_sb + blockIdx.x];
-  if (tid < kPieces && (uint32_t)page < (uint32_t)p.n_pages) {
+  each([&](const int j, const uint32_t (&x)[4]) {
+    const uint64_t before = counts[kKeepWaves * j + wave];
+    const uint32_t own = counts_of(x), in_wave = (uint32_t)sums_up_to((int)own) - own;
+    int equal_before = (int)(before >> 32) + (int)(in_wave >> 16), sure_before = (int)(uint32_t)before + (int)(in_wave & 0xffffu);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int w = 1; w < 4; ++w) {
-        lo[j] = least(lo[j], red[w][c][j]);
-        hi[j] = most(hi[j], red[w][c][4 + j]);
-      }
-      bounds_back<T>(lo[j], hi[j]);
+    for (int e = 0; e < 4; ++e) {
+      const bool equal = x[e] - lo <= hi - lo, sure = x[e] > hi;
+      if (sure || (equal && equal_before < wanted)) kept[first + sure_before + min(equal_before, wanted)] = kKeepStep * j + 4 * tid + e;
+      equal_before += equal;
+      sure_before += sure;
     }
-    uint16_t* to = p.bounds + ((int64_t)page * p.n_kv_heads + kvh) * 2 * D + 8 * c;
-    *reinterpret_cast<uint4*>(to) = uint4{lo[0], lo[1], lo[2], lo[3]};
-    *reinterpret_cast<uint4*>(to + D) = uint4{hi[0], hi[1], hi[2], hi[3]};
+  });
+  for (int i = tid; i < first; i += kKeepThreads) kept[i] = i;
+  for (int i = tid; i < p.n_last; i += kKeepThreads) kept[p.n_keys - p.n_last + i] = end + i;
+}
+
+// f over the lanes of a wave that have the same piece of 8 rows (lane % 8)
+template <typename F>
+__device__ __forceinline__ uint32_t over_eighths(uint32_t x, F f) {
+  x = f(x, dpp<kDppRor8>(x));
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = f(r[0], r[1]);
+  const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return f(s[0], s[1]);
+}
+
+constexpr int kMoveThreads = 512, kMoveRows = kMoveThreads / 8;  // side by side: 8 lanes a row of 64 channels
+constexpr int kMoveEach = 4, kMoveChunk = kMoveEach * kMoveRows;   // where there are several groups, whose rows are a multiple of it
+
+// A (sequence, KV head) and what of its rows this work-group has: 64 channels of keys or of values.
+struct MoveSlice {
+  int b, kvh;
+  int64_t unit;      // its first entry of p.kept
+  bool values;
+  int channel;
+  __device__ __forceinline__ int64_t row(const PagedEvictArgs& p, const int64_t page, const int slot) const {
+    return (values ? page * p.vp_sp + kvh * p.vp_sh + slot * p.vp_sn : page * p.kp_sp + kvh * p.kp_sh + slot * p.kp_sn) + channel;
+  }
+};
+template <int D>
+__device__ __forceinline__ MoveSlice slice_of(const PagedEvictArgs& p) {
+  constexpr int kSlices = D / 64;
+  MoveSlice s;
+  s.b = blockIdx.x / p.n_kv_heads;
+  s.kvh = blockIdx.x - s.b * p.n_kv_heads;
+  s.unit = (int64_t)blockIdx.x * p.n_keys;
+  s.values = blockIdx.y >= kSlices;
+  s.channel = 64 * (blockIdx.y % kSlices) + 8 * (threadIdx.x & 7);
+  return s;
+}
+
+// Rows that come from other groups' places, to scratch: [unit][row][keys, values][channel], and their weights.
+template <int D>
+__global__ void __launch_bounds__(kMoveThreads) paged_save_kernel(const PagedEvictArgs p) {
+  const MoveSlice s = slice_of<D>(p);
+  const uint16_t* pool = s.values ? p.values : p.keys;
+  const int begin = blockIdx.z * kMoveChunk, end = min(begin + kMoveChunk, p.n_keys);
+  if (p.kept[s.unit + end - 1] <= end - 1) return;  // (none moves, or nothing does)
+  const int group_end = (begin / p.group_rows + 1) * p.group_rows;
+#pragma unroll
+  for (int j = 0; j < kMoveEach; ++j) {
+    const int i = begin + kMoveRows * j + (threadIdx.x >> 3);
+    if (i >= end) break;
+    const int from = p.kept[s.unit + i];
+    if (from < group_end || from >= p.n_keys) continue;
+    const int64_t page = clamped_page(p.table[s.b * p.t_sb + (from >> p.page_log)], p.n_pages);
+    const int slot = from & ((1 << p.page_log) - 1);
+    *reinterpret_cast<uint4*>(p.rows + ((s.unit + i) * 2 + s.values) * D + s.channel) = *reinterpret_cast<const uint4*>(pool + s.row(p, page, slot));
+    if (s.values && s.channel == 0) p.row_weights[s.unit + i] = p.weights[((page * p.n_kv_heads + s.kvh) << p.page_log) + slot];
   }
 }
 
-template <typename T, int D>
-static hipError_t launch_paged_evict_for(const PagedEvictArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL(paged_keep_kernel, dim3(a.batch * a.n_kv_heads), dim3(kEvictThreads), 0, stream, a);
-  if ((int64_t)a.max_pages << a.page_log > a.above) {  // (no sequence is longer than its table)
-    const dim3 grid((a.n_keys + (1 << a.page_log) - 1) >> a.page_log, a.n_kv_heads, a.batch);
-    hipLaunchKernelGGL((paged_save_kernel<D>), grid, dim3(256), 0, stream, a);
-    hipLaunchKernelGGL((paged_move_kernel<T, D>), grid, dim3(256), 0, stream, a);
+// The weights of a group's rows, by a work-group of its own.
+__device__ __forceinline__ void move_weights(const PagedEvictArgs& p, const MoveSlice& s, const int end) {
+  constexpr int kEach = 8;
+  const int32_t* table = p.table + s.b * p.t_sb;
+  for (int begin = blockIdx.z * p.group_rows; begin < end; begin += kEach * kMoveThreads) {
+    int from[kEach], page[kEach], to[kEach];
+    float w[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) from[j] = p.kept[s.unit + min(begin + kMoveThreads * j + (int)threadIdx.x, end - 1)];
+    if (from[0] < 0) return;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      page[j] = table[from[j] >> p.page_log];
+      to[j] = table[min(begin + kMoveThreads * j + (int)threadIdx.x, end - 1) >> p.page_log];
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = min(begin + kMoveThreads * j + (int)threadIdx.x, end - 1);
+      const float* row = p.weights + (((int64_t)clamped_page(page[j], p.n_pages) * p.n_kv_heads + s.kvh) << p.page_log) + (from[j] & ((1 << p.page_log) - 1));
+      w[j] = *(from[j] >= end && from[j] < p.n_keys ? p.row_weights + s.unit + i : row);
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) asm volatile("" : "+v"(w[j]));
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = begin + kMoveThreads * j + threadIdx.x;
+      if (i < end && from[j] != i && (uint32_t)to[j] < (uint32_t)p.n_pages)
+        p.weights[(((int64_t)to[j] * p.n_kv_heads + s.kvh) << p.page_log) + (i & ((1 << p.page_log) - 1))] = w[j];
+    }
   }
+}
+
+// EACH: rows of a thread in a chunk
+template <typename T, int D, int EACH>
+__global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const PagedEvictArgs p) {
+  constexpr int kWaves = kMoveThreads / 64, kChunk = EACH * kMoveRows;
+  static_assert(kChunk % 256 == 0, "a page's rows lie in a chunk");
+  constexpr int kStaged = 4096;                    // rows whose places are in LDS, a multiple of a chunk
+  __shared__ uint4 red[EACH * kWaves][8][2];  // bounds of 8 rows each, in their order
+  __shared__ int2 source[kStaged];                 // the place that a row comes from, and its page
+  __shared__ int target[kStaged / 16];             // the pages that rows go to
+  const MoveSlice s = slice_of<D>(p);
+  uint16_t* pool = s.values ? p.values : p.keys;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, page_size = 1 << p.page_log;
+  const int end = min((int)(blockIdx.z + 1) * p.group_rows, p.n_keys);
+  if (blockIdx.y == D / 32) return move_weights(p, s, end);
+  const int32_t* table = p.table + s.b * p.t_sb;
+  int begin = blockIdx.z * p.group_rows;
+  // what keeps its place is left alone: the chunks whose last row does, and is the last of its page
+  for (; begin < end; begin += kChunk) {
+    const int last = min(begin + kChunk, end) - 1, from = p.kept[s.unit + last];
+    if (from < 0) return;
+    if (from > last || (last + 1) % page_size != 0) break;
+  }
+  const int64_t row_page = s.values ? p.vp_sp : p.kp_sp, row_slot = s.values ? p.vp_sn : p.kp_sn, row_head = s.row(p, 0, 0);
+  struct Chunk {
+    u32x4 x[EACH];
+  };
+  for (; begin < end; begin += kStaged) {
+    const int staged_end = min(begin + kStaged, end);
+    __syncthreads();  // (the last ones have been used)
+#pragma unroll
+    for (int j = 0; j < kStaged / kMoveThreads; ++j) {
+      const int from = p.kept[s.unit + min(begin + kMoveThreads * j + tid, end - 1)];
+      source[kMoveThreads * j + tid] = int2{from, clamped_page(table[from >> p.page_log], p.n_pages)};
+    }
+    if (tid < kStaged / 16) target[tid] = table[min((begin >> p.page_log) + tid, (end - 1) >> p.page_log)];
+    __syncthreads();
+    auto load = [&](Chunk& c, const int at) __attribute__((always_inline)) {  // (behind the last row, that one)
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        const int i = min(at + kMoveRows * j + (tid >> 3), staged_end - 1);
+        const uint64_t both = *reinterpret_cast<const uint64_t*>(&source[i - begin]);
+        const int from = (int)(uint32_t)both, page = (int)(uint32_t)(both >> 32);
+        const int64_t row = page * row_page + (from & (page_size - 1)) * row_slot + row_head, scratch_row = ((s.unit + i) * 2 + s.values) * D + s.channel;
+        const bool saved = from >= end && from < p.n_keys;  // (from another group's places)
+        c.x[j] = *reinterpret_cast<const u32x4*>((saved ? p.rows : pool) + (saved ? scratch_row : row));
+      }
+    };
+    auto store = [&](Chunk& c, const int at) __attribute__((always_inline)) {
+      // all rows of the chunk have been read when one is written
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) asm volatile("" ::"v"(c.x[j]));
+      lds_barrier();
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        const int i = at + kMoveRows * j + (tid >> 3);
+        if (i >= staged_end) continue;
+        const int page = target[(i - begin) >> p.page_log];
+        if (source[i - begin].x != i && (uint32_t)page < (uint32_t)p.n_pages) *reinterpret_cast<u32x4*>(pool + page * row_page + (i & (page_size - 1)) * row_slot + row_head) = c.x[j];
+      }
+      if (s.values || p.bounds == nullptr) return;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        const int i = at + kMoveRows * j + (tid >> 3);
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          lo[e] = i < staged_end ? in_order(c.x[j][e]) : 0x7fff7fffu;
+          hi[e] = i < staged_end ? in_order(c.x[j][e]) : 0x80008000u;
+          lo[e] = over_eighths(lo[e], least);
+          hi[e] = over_eighths(hi[e], most);
+        }
+        if (lane < 8) {
+          red[kWaves * j + wave][lane][0] = uint4{lo[0], lo[1], lo[2], lo[3]};
+          red[kWaves * j + wave][lane][1] = uint4{hi[0], hi[1], hi[2], hi[3]};
+        }
+      }
+      lds_barrier();
+      // eight lanes a page of the chunk
+      const int mine = at + (tid >> 3) * page_size, last = min(mine + page_size, staged_end) - 1;
+      if (mine >= min(at + kChunk, staged_end) || (source[last - begin].x == last && last + 1 == mine + page_size)) return;
+      const int page = target[(mine - begin) >> p.page_log], r0 = (mine - at) >> 3;
+      uint32_t lo[4] = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu}, hi[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+      for (int r = r0; r < r0 + (page_size >> 3); ++r) {
+        const uint4 l = red[r][tid & 7][0], h = red[r][tid & 7][1];
+        const uint32_t ls[4] = {l.x, l.y, l.z, l.w}, hs[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          lo[e] = least(lo[e], ls[e]);
+          hi[e] = most(hi[e], hs[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bounds_back<T>(lo[e], hi[e]);
+      if ((uint32_t)page >= (uint32_t)p.n_pages) return;
+      uint16_t* out = p.bounds + ((int64_t)page * p.n_kv_heads + s.kvh) * 2 * D + s.channel;
+      *reinterpret_cast<uint4*>(out) = uint4{lo[0], lo[1], lo[2], lo[3]};
+      *reinterpret_cast<uint4*>(out + D) = uint4{hi[0], hi[1], hi[2], hi[3]};
+    };
+    // a chunk is requested before the last one is stored: its rows lie behind that one's places
+    Chunk a, c;
+    load(a, begin);
+    for (int at = begin;;) {
+      load(c, at + kChunk);
+      store(a, at);
+      if ((at += kChunk) >= staged_end) break;
+      load(a, at + kChunk);
+      store(c, at);
+      if ((at += kChunk) >= staged_end) break;
+    }
+  }
+}
+
+// Rows of a group: all of them where that makes work-groups enough, or as few as make so many.
+constexpr int kMoveEnough = 256;
+int paged_evict_group_rows(int batch, int n_kv_heads, int head_dim, int n_keys) {
+  const int64_t slices = (int64_t)batch * n_kv_heads * 2 * (head_dim / 64);
+  const int chunks = (n_keys + kMoveChunk - 1) / kMoveChunk;
+  const int64_t groups = std::min<int64_t>((kMoveEnough + slices - 1) / slices, chunks);
+  return (int)((chunks + groups - 1) / groups) * kMoveChunk;
+}
+
+template <typename T, int D>
+static hipError_t launch_paged_evict_for(PagedEvictArgs a, hipStream_t stream) {
+  const int64_t most = (int64_t)a.max_pages << a.page_log;
+  const dim3 units(a.batch * a.n_kv_heads);
+  hipLaunchKernelGGL(paged_keep_kernel, units, dim3(kKeepThreads), 4 * (size_t)std::min<int64_t>(most, kKeepInLds), stream, a);
+  if (most <= a.above) return hipGetLastError();  // (no sequence is longer than its table)
+  a.group_rows = paged_evict_group_rows(a.batch, a.n_kv_heads, D, a.n_keys);
+  const int groups = (a.n_keys + a.group_rows - 1) / a.group_rows;
+  if (groups > 1) hipLaunchKernelGGL((paged_save_kernel<D>), dim3(units.x, D / 32, (a.n_keys + kMoveChunk - 1) / kMoveChunk), dim3(kMoveThreads), 0, stream, a);
+  const dim3 grid(units.x, D / 32 + 1, groups);
+  if (groups > 1) hipLaunchKernelGGL((paged_move_kernel<T, D, kMoveEach>), grid, dim3(kMoveThreads), 0, stream, a);
+  else hipLaunchKernelGGL((paged_move_kernel<T, D, 2 * kMoveEach>), grid, dim3(kMoveThreads), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -305,7 +305,7 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
  * are moved inside its pages, and the bounds (if the cache has them) of pages whose keys are others than before are formed anew.  What stays in its place
  * is not written, nor are rows behind the n_keys-th.  new_lengths int32 [batch]: the sequences' keys afterwards (lengths as clamped); it may not be lengths.  kept int32 [batch, n_kv_heads, n_keys]: the places
  * that the keys had, ascending; -1 for sequences that nothing is taken from.  A page outside the pool is read as the nearest one and not written.  Two sequences must not share
- * pages that are written.  weights float32 [n_pages, n_kv_heads, page_size], 16-byte aligned; workspace: aa_paged_evict_workspace_bytes() bytes.
+ * pages that are written.  weights float32 [n_pages, n_kv_heads, page_size], 16-byte aligned; workspace: aa_paged_evict_workspace_bytes() bytes, which may be none.
  *
  * aa_paged_sparse_decode_fwd: the same over n_chosen pages for each sequence and KV head, or all where the sequence has no more: its first n_first, its last
  * n_last (at least 1) and those of the others whose score is largest, the lower page first among equal ones.  The score is the largest over the heads of the

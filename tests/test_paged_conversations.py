@@ -500,7 +500,8 @@ def _evict_and_check(s, cache, n_keys, n_first, n_last, above=None):
     (LENGTHS, 3, 128, 256, "heads", 300, 17, 30, 301), ([700, 1, 33], 1, 128, 128, "rows", 33, 33, 0, None), ([900, 0], 1, 64, 64, "heads", 700, 100, 600, None),
     ([20001], 8, 128, 64, "heads", 4096, 4, 500, None), ([9000, 40, 12345], 4, 64, 16, "heads", 8999, 1, 2, None), ([5], 2, 64, 16, "heads", 5, 1, 1, None), ([0], 2, 128, 16, "heads", 3, 0, 0, None),
     ([130] * 70, 2, 64, 64, "heads", 128, 0, 64, None), ([17], 2, 64, 16, "heads", 1, 0, 0, None), ([70001], 1, 64, 16, "heads", 64000, 0, 1, None), ([1000, 2000], 2, 64, 16, "heads", 100000, 10, 10, None),
-    ([1 << 17], 1, 64, 256, "heads", 1000, 1, 1, None),
+    ([1 << 17], 1, 64, 256, "heads", 1000, 1, 1, None), ([36864, 36865, 5000], 2, 64, 128, "heads", 3001, 5, 100, None), ([1100, 1500, 900] * 30, 2, 128, 16, "rows", 1000, 0, 500, None),
+    ([5000, 4400, 3999], 2, 128, 32, "heads", 4000, 600, 900, 4001), ([300000], 1, 64, 64, "heads", 150000, 0, 0, None),
 ])
 def test_evict(lengths, hkv, d, page, layout, n_keys, n_first, n_last, above, dtype):
     s = _Setup(lengths, hkv, d, page, dtype, hkv + page, layout, extra=1)
@@ -561,15 +562,15 @@ def test_evict_without_bounds_and_of_what_does_not_fit():
         assert all(torch.equal(t[i], u[i]) for i in range(cache.n_pages) if i not in written)
 
 
-EVICTION = {"page_table": 4096, "pt_sb": 8, "lengths": 4096, "new_lengths": 4096, "kept": 4096, "weights": 4096, "workspace": 4096, "workspace_bytes": 1 << 40, "batch": 2, "max_pages": 8,
-            "n_keys": 10, "n_first": 2, "n_last": 3, "above": 12}
+EVICTION = {"page_table": 4096, "pt_sb": 8, "lengths": 4096, "new_lengths": 4096, "kept": 4096, "weights": 4096, "workspace": 4096, "workspace_bytes": 1 << 40, "batch": 2, "max_pages": 100,
+            "n_keys": 1000, "n_first": 2, "n_last": 3, "above": 1200}
 
 
 @pytest.mark.parametrize("change,message", [
     *[(c, m) for c, m in EVERY if not {"q", "q_sh"} & set(c) and m != "must divide"], ({"weights": 0}, "weights is NULL"), ({"weights": 4100}, "weights must be 16-byte"),
     ({"new_lengths": 0}, "new_lengths is NULL"), ({"kept": 0}, "kept is NULL"), ({"kept": 6}, "kept must be 4-byte"), ({"workspace": 0}, "workspace is NULL"), ({"workspace_bytes": 100}, "workspace has 100 bytes"),
-    ({"n_keys": 0}, "not supported"), ({"n_keys": 4}, "not supported"), ({"n_first": -1}, "not supported"), ({"n_last": -1}, "not supported"), ({"n_first": 8}, "not supported"),
-    ({"n_first": 2 ** 31 - 1, "n_last": 2 ** 31 - 1}, "not supported"), ({"above": 9}, "not supported"), ({"n_keys": (1 << 20) + 1, "above": 1 << 21}, "not supported"),
+    ({"n_keys": 0}, "not supported"), ({"n_keys": 4}, "not supported"), ({"n_first": -1}, "not supported"), ({"n_last": -1}, "not supported"), ({"n_first": 998}, "not supported"),
+    ({"n_first": 2 ** 31 - 1, "n_last": 2 ** 31 - 1}, "not supported"), ({"above": 999}, "not supported"), ({"n_keys": (1 << 20) + 1, "above": 1 << 21}, "not supported"),
     ({"batch": 65535, "n_kv_heads": 512, "kp_sh": 128}, "2\\^24"),
 ])
 def test_what_the_c_interface_of_eviction_refuses(change, message):
@@ -586,7 +587,8 @@ def test_packed_eviction_is_laid_out_as_in_c(tmp_path):
     from anchor_attn.src.ops import _hip
     size, at = _sizes_in_c(tmp_path, "sizeof(aa_paged_eviction)", "offsetof(aa_paged_eviction, above)")
     assert size == _hip.PAGED_EVICTION.size and _hip.PAGED_EVICTION.pack(*range(14))[at] == 13
-    assert _hip.lib().aa_paged_evict_workspace_bytes(2, 3, 128, 10) >= 2 * 3 * 10 * (4 * 128 + 4)
+    assert _hip.lib().aa_paged_evict_workspace_bytes(2, 3, 128, 1000) >= 2 * 3 * 1000 * (4 * 128 + 4)
+    assert _hip.lib().aa_paged_evict_workspace_bytes(2, 3, 128, 200) == 0 == _hip.lib().aa_paged_evict_workspace_bytes(64, 8, 128, 10000)  # (rows are moved in turn)
     assert _hip.lib().aa_paged_evict_workspace_bytes(2, 3, 128, 0) == 0 == _hip.lib().aa_paged_evict_workspace_bytes(2, 3, 96, 8)
 
 
