@@ -78,7 +78,7 @@ _SIGNATURES = {
     "aa_paged_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p]),
     "aa_paged_weighing_workspace_bytes": (c_size_t, [c_int] * 6),
     "aa_paged_weighing_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p, c_int, c_void_p]),
-    "aa_paged_shared_workspace_bytes": (c_size_t, [c_int] * 6),
+    "aa_paged_shared_workspace_bytes": (c_size_t, [c_int] * 7),
     "aa_paged_shared_decode_fwd": (c_int, [c_void_p, c_char_p, c_void_p, c_void_p, c_int, c_void_p]),
     "aa_paged_evict_workspace_bytes": (c_size_t, [c_int] * 4),
     "aa_paged_evict": (c_int, [c_void_p, c_char_p, c_void_p]),

@@ -397,7 +397,7 @@ def paged_shared_decode_attention(cache: PagedCache, q: torch.Tensor, page_table
     groups_ptr = 0 if groups is None else _indices(groups, "groups", cache, 1, n_groups + 1)
     if sizes[0]:
         lib = _hip.lib()
-        nbytes = lib.aa_paged_shared_workspace_bytes(*sizes, cache.n_kv_heads, cache.head_dim, cache.page_size, most)
+        nbytes = lib.aa_paged_shared_workspace_bytes(*sizes, cache.n_kv_heads, cache.head_dim, cache.page_size, most, n_groups)
         ws = lengths.new_empty((nbytes >> 2,))
         cache._launch(lib.aa_paged_shared_decode_fwd, _hip.PAGED_STEP.pack(*tensors, ws.data_ptr(), nbytes, 0, *sizes, most, 0, 0, 0, scale), shared_ptr, groups_ptr, n_groups)
     return out

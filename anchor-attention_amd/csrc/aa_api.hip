@@ -1079,21 +1079,21 @@ int aa_paged_weighing_decode_fwd(const aa_paged_cache* cache, const aa_paged_ste
 struct SharedScratch {
   size_t skips, prefix, stats, parts, decode, total;
 };
-static SharedScratch carve_shared(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
+static SharedScratch carve_shared(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_groups) {
   SharedScratch w;
   const size_t rows = (size_t)batch * n_q_heads;
   w.skips = 0;
   w.prefix = align256((size_t)batch * 4);
   w.stats = w.prefix + align256(rows * head_dim * 4);
   w.parts = w.stats + align256(rows * 8);
-  w.decode = w.parts + align256(paged_prefix_scratch(batch, n_q_heads, n_kv_heads, head_dim).total);
+  w.decode = w.parts + align256(paged_prefix_scratch(batch, n_q_heads, n_kv_heads, head_dim, n_groups).total);
   w.total = w.decode + paged_decode_scratch(batch, n_q_heads, n_kv_heads, head_dim, log2_of(page_size), max_pages).total;
   return w;
 }
 
-size_t aa_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
-  if (n_q_heads == 0 || check_paged("aa_paged_shared_workspace_bytes", batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages)) return 0;
-  return carve_shared(batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages).total;
+size_t aa_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_groups) {
+  if (n_q_heads == 0 || n_groups <= 0 || n_groups > 65535 || check_paged("aa_paged_shared_workspace_bytes", batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages)) return 0;
+  return carve_shared(batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages, n_groups).total;
 }
 
 int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* t, const int32_t* shared_pages, const int32_t* groups, int n_groups, void* stream) {
@@ -1108,13 +1108,13 @@ int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step*
     set_error("%s: %d groups are not supported (1 to 65535)", who, n_groups);
     return n_groups <= 0 ? AA_EBADARG : AA_EUNSUPPORTED;
   }
-  const SharedScratch w = carve_shared(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages);
+  const SharedScratch w = carve_shared(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages, n_groups);
   if ((rc = paged_decode_args(who, a, cache, t, w.total))) return rc;
   char* ws = static_cast<char*>(t->workspace);
   a.skips = (int32_t*)(ws + w.skips);
   a.prefix = (float*)(ws + w.prefix);
   a.prefix_stats = (float*)(ws + w.stats);
-  const PagedScratch s = paged_prefix_scratch(a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim);
+  const PagedScratch s = paged_prefix_scratch(a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim, n_groups);
   char* parts = ws + w.parts;
   const PagedPrefixArgs x = {a, shared_pages, groups, n_groups, (int32_t*)(parts + s.headers), (float*)(parts + s.stats), (float*)(parts + s.parts)};
   if ((rc = check_launch(launch_paged_prefix(x, (hipStream_t)stream), who))) return rc;

@@ -188,7 +188,7 @@ struct PagedPrefixArgs {
   const int32_t* shared_pages; const int32_t* groups; int n_groups;  // groups NULL: one, the whole batch
   int32_t* headers; float* part_stats; float* parts;  // scratch (paged_prefix_scratch)
 };
-PagedScratch paged_prefix_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim);
+PagedScratch paged_prefix_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups);
 hipError_t launch_paged_prefix(const PagedPrefixArgs& a, hipStream_t stream);
 
 struct PagedEvictArgs {

@@ -7,6 +7,8 @@
 // have is joined by paged_prefix_join_kernel in order, so that results do not depend on timing.
 //
 // Inside a wave, as in the decode kernel: S^T = K Q^T straight from memory, P^T in S^T's registers, V turned by v_perm once for all rows, P as two 16-bit numbers.
+#include <type_traits>
+
 #include "aa_kernels.h"
 #include "aa_nonfinite.h"
 #include "aa_paged.h"
@@ -29,20 +31,10 @@ __device__ __forceinline__ PagedGroup group_at(const PagedPrefixArgs& p, const i
   return x;
 }
 
-template <typename T, int D, int BLOCKS>
-__global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(const PagedPrefixArgs all) {
-  constexpr int kKS = D / 32;  // MFMAs of a score
-  constexpr int kDV = D / 16;  // channels of V that a lane loads
-  constexpr int kVW = kDV / 2;
-  constexpr int kRows = 16 * BLOCKS, kPitch = D + 4;
-  extern __shared__ __attribute__((aligned(16))) float states[];  // [wave][row][kPitch]: the accumulator, maximum and sum
+// How many of a sequence's first pages its group's state stands for: those that are shared, if it is as long, or none.
+__device__ __forceinline__ void find_skips(const PagedPrefixArgs& all, const int tid, const int threads) {
   const PagedDecodeArgs& p = all.step;
-  const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int heads = p.n_q_heads / p.n_kv_heads, page_size = 1 << p.page_log;
-
-  // ---- whose prefixes count: sequences that are as long -----------------------------------------------
-  for (int b = blockIdx.x * 256 + tid; b < p.batch; b += kPrefixShares * 256) {
+  for (int b = blockIdx.x * threads + tid; b < p.batch; b += kPrefixShares * threads) {
     int from = 0, to = all.groups == nullptr ? 0 : all.n_groups;  // groups that end at or before b
     while (from < to) {
       const int mid = (from + to) >> 1;
@@ -56,14 +48,34 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
     }
     p.skips[b] = skip;
   }
+}
 
-  // ---- this work-group's share ---------------------------------------------------------------------
-  auto tiles_of = [&](const PagedGroup& x) { return ((x.pages << p.page_log) + kPrefixTile - 1) / kPrefixTile; };
-  auto blocks_of = [&](const PagedGroup& x) { return (x.sequences * heads + kRows - 1) / kRows; };
+// a number that all lanes have, in scalar registers
+__device__ __forceinline__ int64_t uniform(const int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x));
+}
+
+// The share-th of kPrefixShares equal parts of all units' tiles, and the group that it begins in (found by every wave for itself).
+struct PrefixShare {
+  int64_t at, end, share, start;  // from, to; how long a share is; where the group begins
+  int group;
+};
+template <int TILE>
+__device__ __forceinline__ int tiles_of(const PagedDecodeArgs& p, const PagedGroup& x) {
+  return ((x.pages << p.page_log) + TILE - 1) / TILE;
+}
+template <int ROWS>
+__device__ __forceinline__ int blocks_of(const PagedGroup& x, const int heads) {
+  return (x.sequences * heads + ROWS - 1) / ROWS;
+}
+template <int TILE, int ROWS>
+__device__ __forceinline__ PrefixShare share_of(const PagedPrefixArgs& all, const int share, const int least) {
+  const PagedDecodeArgs& p = all.step;
+  const int lane = threadIdx.x & 63, heads = p.n_q_heads / p.n_kv_heads;
   auto extent_of = [&](const int i) {  // of group i's units
     if (i >= all.n_groups) return (int64_t)0;
     const PagedGroup x = group_at(all, i);
-    return (int64_t)tiles_of(x) * blocks_of(x) * p.n_kv_heads;
+    return (int64_t)tiles_of<TILE>(p, x) * blocks_of<ROWS>(x, heads) * p.n_kv_heads;
   };
   auto up_to_lane = [&](int64_t x) {
 #pragma unroll
@@ -73,25 +85,48 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
     }
     return x;
   };
+  PrefixShare r = {0, 0, 0, 0, 0};
   int64_t total = 0;
-  for (int i = 0; i < all.n_groups; i += 64) total += __shfl((long long)up_to_lane(extent_of(i + lane)), 63, 64);
-  const int64_t share = max((total + (kPrefixShares - 1)) >> kPrefixSharesLog, (int64_t)kPrefixLeast);
-  int64_t at = min(share * blockIdx.x, total);
-  const int64_t end = min(at + share, total);
-  int group = 0;
-  int64_t start = 0;  // of the group
-  if (at < end) {
+  if (all.n_groups == 1) total = extent_of(0);
+  else
+    for (int i = 0; i < all.n_groups; i += 64) total += __shfl((long long)up_to_lane(extent_of(i + lane)), 63, 64);
+  r.share = max((total + (kPrefixShares - 1)) >> kPrefixSharesLog, (int64_t)least);
+  r.at = min(r.share * share, total);
+  r.end = min(r.at + r.share, total);
+  if (r.at < r.end && all.n_groups > 1) {
     for (int i = 0; i < all.n_groups; i += 64) {
       const int64_t sum = up_to_lane(extent_of(i + lane));
-      const int in = __popcll(__ballot(start + sum <= at));
+      const int in = __popcll(__ballot(r.start + sum <= r.at));
       if (in < 64) {
-        group = i + in;
-        if (in > 0) start += __shfl((long long)sum, in - 1, 64);
+        r.group = i + in;
+        if (in > 0) r.start += __shfl((long long)sum, in - 1, 64);
         break;
       }
-      start += __shfl((long long)sum, 63, 64);
+      r.start += __shfl((long long)sum, 63, 64);
     }
   }
+  return {uniform(r.at), uniform(r.end), uniform(r.share), uniform(r.start), (int)__builtin_amdgcn_readfirstlane(r.group)};
+}
+
+template <typename T, int D, int BLOCKS>
+__global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(const PagedPrefixArgs all) {
+  constexpr int kKS = D / 32;  // MFMAs of a score
+  constexpr int kDV = D / 16;  // channels of V that a lane loads
+  constexpr int kVW = kDV / 2;
+  constexpr int kRows = 16 * BLOCKS, kPitch = D + 4;
+  extern __shared__ __attribute__((aligned(16))) float states[];  // [wave][row][kPitch]: the accumulator, maximum and sum
+  const PagedDecodeArgs& p = all.step;
+  const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int heads = p.n_q_heads / p.n_kv_heads, page_size = 1 << p.page_log;
+
+  find_skips(all, tid, 64 * kPrefixWaves);
+
+  // ---- this work-group's share ---------------------------------------------------------------------
+  const PrefixShare mine = share_of<kPrefixTile, kRows>(all, blockIdx.x, kPrefixLeast);
+  int64_t at = mine.at, start = mine.start;
+  const int64_t end = mine.end, share = mine.share;
+  int group = mine.group;
   int4* header = reinterpret_cast<int4*>(all.headers) + blockIdx.x;
   if (tid == 0) header->x = 0;
 
@@ -106,7 +141,7 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
     x.first = __builtin_amdgcn_readfirstlane(x.first);
     x.sequences = __builtin_amdgcn_readfirstlane(x.sequences);
     x.pages = __builtin_amdgcn_readfirstlane(x.pages);
-    const int tiles = tiles_of(x), blocks = blocks_of(x), length = x.pages << p.page_log, rows = x.sequences * heads;
+    const int tiles = tiles_of<kPrefixTile>(p, x), blocks = blocks_of<kRows>(x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
     if (at - start >= (int64_t)tiles * blocks * p.n_kv_heads) {  // (the next group, perhaps of nothing)
       start += (int64_t)tiles * blocks * p.n_kv_heads;
       ++group;
@@ -356,14 +391,14 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
   }
 }
 
-// Joins the parts of a unit that begins in share blockIdx.x and ends in another, a row by a wave.
+// Joins the parts of a unit that begins in share blockIdx.y and ends in another, a row by a wave.  (Units begin every so many shares: shares as blockIdx.x were one XCD's.)
 template <int D, int BLOCKS>
 __global__ void __launch_bounds__(256) paged_prefix_join_kernel(const PagedPrefixArgs all) {
   constexpr int kRows = 16 * BLOCKS, kEach = D / 64;
   typedef float floats __attribute__((ext_vector_type(kEach)));
   const PagedDecodeArgs& p = all.step;
-  const int lane = threadIdx.x & 63, r = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int4 header = *reinterpret_cast<const int4*>(all.headers + 4 * blockIdx.x);
+  const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = blockIdx.y;
+  const int4 header = *reinterpret_cast<const int4*>(all.headers + 4 * share);
   const int parts = header.x, heads = p.n_q_heads / p.n_kv_heads;
   if (parts == 0) return;
   const PagedGroup x = group_at(all, header.y);
@@ -371,7 +406,7 @@ __global__ void __launch_bounds__(256) paged_prefix_join_kernel(const PagedPrefi
   if (row >= x.sequences * heads) return;
   const float scale = p.sm_scale * kLog2e;
   // the first part is the second of its share, the others the first of theirs
-  auto part = [&](const int i) { return ((int64_t)2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kRows + r; };
+  auto part = [&](const int i) { return ((int64_t)2 * (share + i) + (i == 0 ? 1 : 0)) * kRows + r; };
   float m = -INFINITY;
   for (int i = lane; i < parts; i += 64) m = fmaxf(m, all.part_stats[2 * part(i)]);
   m = over_wave(m, -INFINITY, [](const float a, const float b) { return fmaxf(a, b); });
@@ -390,34 +425,423 @@ __global__ void __launch_bounds__(256) paged_prefix_join_kernel(const PagedPrefi
   if (lane == 0) *reinterpret_cast<floatx2*>(p.prefix_stats + 2 * to) = floatx2{m, l};
 }
 
-// Rows of a unit, in blocks of 16: as many as a KV head's queries of the batch fill, and their accumulators leave registers for.
-static int prefix_blocks(int batch, int n_q_heads, int n_kv_heads, int head_dim) {
-  const int64_t rows = (int64_t)batch * (n_q_heads / n_kv_heads);
-  return rows <= 16 ? 1 : rows <= 32 || head_dim == 128 ? 2 : 4;
+// ---- many rows ------------------------------------------------------------------------------------
+// 128 rows by a work-group, 32 by a wave, as in the flash kernel: 32 x 32 x 16 MFMAs, S^T = K Q^T with keys from LDS, P^T in S^T's registers, V^T by transposing reads, tiles of 64 keys
+// that the memory system fills, chunks swizzled.  Eight waves are two teams that take the tiles in turn and are never in the same half of a tile: while one multiplies (the last tile's
+// probabilities with its values, the next one's keys with the queries), the other forms probabilities, a barrier between the halves, so that the matrix pipe has one team's work at a time and
+// the vector ALU the other's.  Tiles are requested one tile ahead.
+constexpr int kWideTile = 64, kWideRows = 128, kWideThreads = 512, kWideLeast = 4;
+
+template <int D>
+__device__ __forceinline__ int wide_k_swizzle(const int r) { return D == 128 ? r & 15 : (r & 7) ^ ((r >> 3) & 1); }
+template <int D>
+__device__ __forceinline__ int wide_v_swizzle(const int r) { return D == 128 ? (r & 3) << 2 : (r & 3) << 1; }
+
+// load16_to_lds for an address that vector instructions may have formed: one of memory must not read a scalar register within five wait states of their write, which the
+// compiler, which does not look inside, would not see to
+__device__ __forceinline__ void load16_to_lds_from_any(const char* base, const uint32_t byte_off, const uint32_t lds_dst) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" : : "{m0}"(lds_dst), "v"(byte_off), "s"(base) : "memory");
 }
 
-PagedScratch paged_prefix_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim) {
-  const size_t rows = (size_t)kPrefixShares * 2 * 16 * prefix_blocks(batch, n_q_heads, n_kv_heads, head_dim);
+// a barrier that waits for nothing of its own
+__device__ __forceinline__ void wave_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const PagedPrefixArgs all) {
+  constexpr int kKS = D / 16, kDB = D / 32;        // MFMAs of a score, blocks of 32 channels
+  constexpr int kRowBytes = 2 * D, kTileBytes = kWideTile * kRowBytes;
+  constexpr int kRowsALoad = 1024 / kRowBytes, kLoads = 16 / kRowsALoad;  // rows of a load instruction; loads of a wave's 16 rows
+  constexpr int kFours = 4 * kDB;                  // accumulators of a lane, in fours
+  typedef __attribute__((address_space(3))) const typename T::vec8 lds_vec8;
+  typedef short shortx4 __attribute__((ext_vector_type(4)));
+  typedef short shortx8 __attribute__((ext_vector_type(8)));
+  typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
+  // [team][keys 0, 1, values 0, 1]; at the end the second team's states
+  __shared__ __attribute__((aligned(1024))) char tiles[2][4][kTileBytes];
+  static_assert(sizeof(tiles) >= (size_t)4 * 64 * (4 * kFours + 4) * 4, "a team's states take less room");
+  const PagedDecodeArgs& p = all.step;
+  const int tid = threadIdx.x, lane = tid & 63, c32 = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), team = __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int heads = p.n_q_heads / p.n_kv_heads, page_mask = (1 << p.page_log) - 1;
+  // neighbouring shares, which have neighbouring rows of one KV head, are one XCD's
+  const int share_at = (blockIdx.x % 8) * (kPrefixShares / 8) + blockIdx.x / 8;
+  const PrefixShare mine = share_of<kWideTile, kWideRows>(all, share_at, kWideLeast);
+  int64_t at = mine.at, start = mine.start;
+  const int64_t end = mine.end, share = mine.share;
+  int group = mine.group;
+  int4* header = reinterpret_cast<int4*>(all.headers) + share_at;
+  if (tid == 0) header->x = 0;
+
+  const float scale = p.sm_scale * kLog2e;
+  // where a lane's pieces of 16 rows come from (its chunk, which belongs in its slot), and what it reads of a tile
+  uint32_t k_from[kLoads], v_from[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const int r = kRowsALoad * j + lane / (D / 8), slot = lane % (D / 8);
+    k_from[j] = 2u * (uint32_t)p.kp_sn * r + 16u * (slot ^ wide_k_swizzle<D>(r));
+    v_from[j] = 2u * (uint32_t)p.vp_sn * r + 16u * (slot ^ wide_v_swizzle<D>(r));
+  }
+  const uint32_t my_tiles = lds_addr(tiles[team][0]);
+  // (chunk 2 ks + half of a row: the bits of ks are their own; so are those of the block of channels)
+  const uint32_t k_rd = my_tiles + c32 * kRowBytes + ((half ^ wide_k_swizzle<D>(c32)) << 4);
+  const int r0 = 4 * half + ((lane & 15) >> 2), y0 = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const uint32_t v_rd = my_tiles + 2 * kTileBytes + r0 * kRowBytes + ((y0 ^ wide_v_swizzle<D>(r0)) << 4) + 8 * (lane & 1);
+
+  while (at < end && group < all.n_groups) {
+    PagedGroup x = group_at(all, group);
+    x.first = __builtin_amdgcn_readfirstlane(x.first);
+    x.sequences = __builtin_amdgcn_readfirstlane(x.sequences);
+    x.pages = __builtin_amdgcn_readfirstlane(x.pages);
+    const int n_tiles = tiles_of<kWideTile>(p, x), blocks = blocks_of<kWideRows>(x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
+    if (at - start >= (int64_t)n_tiles * blocks * p.n_kv_heads) {  // (the next group, perhaps of nothing)
+      start += (int64_t)n_tiles * blocks * p.n_kv_heads;
+      ++group;
+      continue;
+    }
+    // a KV head's blocks one after the other
+    const uint32_t unit = (uint32_t)((at - start) / n_tiles), block = unit % (uint32_t)blocks, kvh = unit / (uint32_t)blocks;
+    const int t0 = (int)(at - start - (int64_t)unit * n_tiles), t1 = (int)min((int64_t)n_tiles, t0 + (end - at));
+    const int my_row = min((int)(block * kWideRows) + 32 * wave + c32, rows - 1), sequence = my_row / heads;
+    const int64_t my_head = (int64_t)(x.first + sequence) * p.n_q_heads + (int)kvh * heads + my_row - sequence * heads;
+    typename T::vec8 q[kKS];
+    {
+      const uint16_t* qp = p.q + (int64_t)(x.first + sequence) * p.q_sb + (int64_t)((int)kvh * heads + my_row - sequence * heads) * p.q_sh + 8 * half;
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) q[ks] = *reinterpret_cast<const typename T::vec8*>(qp + 16 * ks);
+    }
+    const const_i32* table = (const_i32*)(p.table + x.first * p.t_sb);
+    const int rounds = (t1 - t0 + 1) / 2, own = (t1 - t0 + 1 - team) / 2;  // tiles t0 + team, t0 + team + 2, ...
+    auto tile_at = [&](const int i) { return t0 + team + 2 * i; };
+    // 16 of a tile's rows are a wave's to request, which lie in one page; rows behind the prefix are zeros
+    auto key_of = [&](const int i) { return kWideTile * tile_at(i) + 16 * wave; };
+    auto page_of = [&](const int i) { return table[min(key_of(min(i, max(own - 1, 0))) >> p.page_log, x.pages - 1)]; };
+    auto request = [&](const int i, const int page_there, const bool values) __attribute__((always_inline)) {
+      const int key = key_of(i);
+      const uint32_t to = my_tiles + ((values ? 2 : 0) + (i & 1)) * kTileBytes + 16 * wave * kRowBytes;
+      if (key < length) {
+        const int64_t page = clamped_page(page_there, p.n_pages);
+        const int slot = key & page_mask;
+        const char* base = (const char*)(values ? p.values + page * p.vp_sp + kvh * p.vp_sh + slot * p.vp_sn : p.keys + page * p.kp_sp + kvh * p.kp_sh + slot * p.kp_sn);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) load16_to_lds_from_any(base, values ? v_from[j] : k_from[j], to + j * 1024);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(to + j * 1024 + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+    };
+    float m_run = -INFINITY, l_run = 0.f;
+    floatx16 acc[kDB], s[2];
+    u32x4 prob[4], rest[4];
+    // What a team multiplies of a round: operand f is of values (two products, with probabilities and their rest) or, from kValues on, of the next tile's keys.  Operands are read from LDS
+    // kAhead ahead of the products that take them, in this order, which the compiler would not keep; the first ones before the barrier.
+    constexpr int kAhead = D == 128 ? 6 : 6, kValues = 4 * kDB, kKeys = 2 * kKS;
+    u32x4 operand[kAhead];
+    auto read = [&](const int i, const int f) __attribute__((always_inline)) {  // of values of tile i, keys of tile i + 1
+      if (f < kValues) {
+        const uint32_t at = ((v_rd + (i & 1) * kTileBytes) ^ ((f % kDB) << 6)) + 16 * (f / kDB) * kRowBytes;
+        const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)(uintptr_t)at);
+        const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)(uintptr_t)(at + 8 * kRowBytes));
+        const shortx8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        operand[f % kAhead] = *reinterpret_cast<const u32x4*>(&both);
+      } else {
+        const int g = f - kValues;
+        operand[f % kAhead] = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(((k_rd + ((i + 1) & 1) * kTileBytes) ^ ((g % kKS) << 5)) + 32 * (g / kKS) * kRowBytes);
+      }
+    };
+    auto multiply_values = [&](const int f, auto exact) __attribute__((always_inline)) {
+      const int st = f / kDB, db = f % kDB;
+      u32x4 v = operand[f % kAhead];
+      acc[db] = T::mfma(*reinterpret_cast<const typename T::vec8*>(&v), *reinterpret_cast<const typename T::vec8*>(&prob[st]), acc[db]);
+      if constexpr (decltype(exact)::value) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t y = v[w];
+          if ((y & T::kExponent) == T::kExponent) v[w] &= 0xffff0000u;
+          if (((y >> 16) & T::kExponent) == T::kExponent) v[w] &= 0xffffu;
+        }
+      }
+      acc[db] = T::mfma(*reinterpret_cast<const typename T::vec8*>(&v), *reinterpret_cast<const typename T::vec8*>(&rest[st]), acc[db]);
+    };
+    auto multiply_keys = [&](const int g) __attribute__((always_inline)) {
+      floatx16 none;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) none[r] = 0.f;
+      s[g / kKS] = T::mfma(*reinterpret_cast<const typename T::vec8*>(&operand[(kValues + g) % kAhead]), q[g % kKS], g % kKS == 0 ? none : s[g / kKS]);
+    };
+    auto probabilities = [&](const int i, auto exact) __attribute__((always_inline)) {
+      const int key0 = kWideTile * tile_at(i);
+      if (key0 + kWideTile > length) {
+#pragma unroll
+        for (int r = 0; r < 32; ++r)
+          if (key0 + 32 * (r >> 4) + 16 * ((r & 15) >> 3) >= length) s[r >> 4][r & 15] = -INFINITY;
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
+      const float m_new = fmaxf(m_run, max_with_other_half(mx));
+      const float m_base = m_new == -INFINITY ? 0.f : m_new;  // (no key of this row's so far)
+      if (__any(m_new > m_run)) {
+        const float alpha = fast_exp2((m_run - m_base) * scale);
+        l_run *= alpha;
+#pragma unroll
+        for (int db = 0; db < kDB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
+        m_run = m_new;
+      }
+      // 2^(s * scale - m * scale): the fused product's second term is the same for all keys, so that its rounding cancels in the quotient
+      const float bias = T::kProbLog2 - m_base * scale;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        const float e0 = fast_exp2(__builtin_fmaf(s[w >> 3][2 * (w & 7)], scale, bias)), e1 = fast_exp2(__builtin_fmaf(s[w >> 3][2 * (w & 7) + 1], scale, bias));
+        l_run += e0 + e1;
+        uint32_t both = T::pack(e0, e1);
+        if constexpr (decltype(exact)::value) {
+          if (e0 > 0.f && (both & 0xffffu) == 0u) both |= 1u;
+          if (e1 > 0.f && (both >> 16) == 0u) both |= 0x10000u;
+        }
+        prob[w >> 2][w & 3] = both;
+        rest[w >> 2][w & 3] = T::pack_rest(e0, e1, both);
+      }
+    };
+    auto run = [&](auto exact) __attribute__((always_inline)) {
+      l_run = 0.f;
+#pragma unroll
+      for (int db = 0; db < kDB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
+      int page1 = page_of(1), page2 = page_of(2);  // of the next tile and the one behind it
+      if (own > 0) {
+        const int page0 = page_of(0);
+        request(0, page0, false);
+        request(0, page0, true);
+        if (own > 1) request(1, page1, false);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) asm volatile("" ::"v"(q[ks]));  // (so that the compiler does not wait for them, and all that was requested since, inside the loop)
+      lds_barrier();
+      if (team == 1) wave_barrier();
+      if (own > 0) {
+#pragma unroll
+        for (int f = 0; f < kAhead; ++f) read(-1, kValues + f);
+      }
+      for (int i = 0; i < own; ++i) {
+        if (i > 0) {
+#pragma unroll
+          for (int f = 0; f < kValues; ++f) {
+            multiply_values(f, exact);
+            read(i - 1, f + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < kKeys; ++g) {
+          multiply_keys(g);
+          if (g + kAhead < kKeys) read(i - 1, kValues + g + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // (keys i and values i - 1 have been read; keys i + 1 and values i, requested a round ago, are there)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        wave_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + 1 < own) request(i + 1, page1, true);
+        if (i + 2 < own) request(i + 2, page2, false);
+        page1 = page2;
+        page2 = page_of(i + 3);
+        probabilities(i, exact);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int f = 0; f < kAhead; ++f) read(i, f);
+        __builtin_amdgcn_sched_barrier(0);
+        wave_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (own > 0) {
+#pragma unroll
+        for (int f = 0; f < kValues; ++f) {
+          multiply_values(f, exact);
+          if (f + kAhead < kValues) read(own - 1, f + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      for (int i = own; i < rounds; ++i) {  // (the second team has one tile less where there is an odd number)
+        wave_barrier();
+        wave_barrier();
+      }
+      lds_barrier();
+      if (team == 0) lds_barrier();
+    };
+    run(std::false_type{});
+    float sum = 0.f;
+#pragma unroll
+    for (int db = 0; db < kDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += acc[db][r];
+    // Infinite values: with two products per key they give NaN.  Once more, relative to the maximum: the rest meets the finite values only and a positive probability
+    // does not round to 0.
+    if (__builtin_expect(__syncthreads_or(is_nan(sum) && !is_nan(l_run)), 0)) run(std::true_type{});
+    {
+      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+      l_run = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+
+    // ---- the teams' states -> the unit's, or a part of it: fours of accumulators, lane by lane, half of them by each team ----
+    floatx4* states = reinterpret_cast<floatx4*>(&tiles[0][0][0]) + wave * kFours * 64;
+    floatx2* stats = reinterpret_cast<floatx2*>(reinterpret_cast<floatx4*>(&tiles[0][0][0]) + 4 * kFours * 64) + wave * 128;
+    auto four = [&](const int f) { return floatx4{acc[f >> 2][4 * (f & 3)], acc[f >> 2][4 * (f & 3) + 1], acc[f >> 2][4 * (f & 3) + 2], acc[f >> 2][4 * (f & 3) + 3]}; };
+    const int64_t part = (2 * share_at + (t0 == 0 ? 1 : 0)) * 4 + wave;
+    const bool whole = t0 == 0 && t1 == n_tiles, there = (int)(block * kWideRows) + 32 * wave + c32 < rows;
+    auto hand_over = [&](auto first) __attribute__((always_inline)) {
+#pragma unroll
+      for (int f = 0; f < kFours / 2; ++f) states[(decltype(first)::value + f) * 64 + lane] = four(decltype(first)::value + f);
+      stats[team * 64 + lane] = floatx2{m_run, l_run};
+    };
+    auto finish = [&](auto first) __attribute__((always_inline)) {
+      const floatx2 other = stats[(1 - team) * 64 + lane];
+      const float m = fmaxf(m_run, other[0]), w = m_run == -INFINITY ? 0.f : fast_exp2((m_run - m) * scale), w2 = other[0] == -INFINITY ? 0.f : fast_exp2((other[0] - m) * scale);
+      const float l = w * l_run + w2 * other[1];
+#pragma unroll
+      for (int g = 0; g < kFours / 2; ++g) {
+        const int f = decltype(first)::value + g;
+        const floatx4 a = four(f), b = states[f * 64 + lane];
+        const floatx4 y = {w * a[0] + w2 * b[0], w * a[1] + w2 * b[1], w * a[2] + w2 * b[2], w * a[3] + w2 * b[3]};
+        if (!whole) *reinterpret_cast<floatx4*>(all.parts + ((part * kFours + f) * 64 + lane) * 4) = y;
+        else if (there) *reinterpret_cast<floatx4*>(p.prefix + my_head * D + 8 * f + 4 * half) = y;
+      }
+      if (decltype(first)::value != 0) return;
+      if (!whole) *reinterpret_cast<floatx2*>(all.part_stats + (part * 64 + lane) * 2) = floatx2{m, l};
+      else if (there && half == 0) *reinterpret_cast<floatx2*>(p.prefix_stats + 2 * my_head) = floatx2{m, l};
+    };
+    std::integral_constant<int, 0> lower;
+    std::integral_constant<int, kFours / 2> upper;
+    if (team == 0) hand_over(upper);
+    else hand_over(lower);
+    __syncthreads();
+    if (team == 0) finish(lower);
+    else finish(upper);
+    if (t0 == 0 && t1 < n_tiles && tid == 0) {  // its other parts are the next work-groups'
+      const int64_t last = start + (int64_t)(unit + 1) * n_tiles - 1;
+      *header = int4{(int)(last / share) - share_at + 1, group, (int)kvh, (int)block};
+    }
+    __syncthreads();
+    at += t1 - t0;
+  }
+  find_skips(all, tid, kWideThreads);
+}
+
+// Joins the parts of a unit that begins in share blockIdx.y and ends in another: a work-group has two fours of 32 rows' accumulators, lane by lane as they were left, and
+// its waves every so many parts.
+template <int D>
+__global__ void __launch_bounds__(512) paged_prefix_wide_join_kernel(const PagedPrefixArgs all) {
+  constexpr int kFours = D / 8, kEach = 2, kJoin = 8;
+  __shared__ floatx4 red[kJoin][kEach][64];
+  __shared__ floatx2 red_stats[kJoin][64];
+  const PagedDecodeArgs& p = all.step;
+  const int lane = threadIdx.x & 63, mine = threadIdx.x >> 6, wave = blockIdx.x % 4, f0 = kEach * (blockIdx.x / 4), share = blockIdx.y;
+  const int4 header = *reinterpret_cast<const int4*>(all.headers + 4 * share);
+  const int parts = header.x, heads = p.n_q_heads / p.n_kv_heads;
+  if (parts == 0) return;
+  const PagedGroup x = group_at(all, header.y);
+  const int row = header.w * kWideRows + 32 * wave + (lane & 31);
+  const float scale = p.sm_scale * kLog2e;
+  // the first part is the second of its share, the others the first of theirs
+  auto part = [&](const int i) { return ((int64_t)2 * (share + i) + (i == 0 ? 1 : 0)) * 4 + wave; };
+  float m = -INFINITY, l = 0.f;
+  floatx4 sum[kEach] = {};
+  constexpr int kSide = 4;  // parts that are read side by side
+  for (int i = mine; i < parts; i += kJoin * kSide) {
+    floatx2 stats[kSide];
+    floatx4 y[kSide][kEach];
+#pragma unroll
+    for (int j = 0; j < kSide; ++j) {
+      const int64_t at = part(min(i + kJoin * j, parts - 1));
+      stats[j] = *reinterpret_cast<const floatx2*>(all.part_stats + (at * 64 + lane) * 2);
+#pragma unroll
+      for (int f = 0; f < kEach; ++f) y[j][f] = *reinterpret_cast<const floatx4*>(all.parts + ((at * kFours + f0 + f) * 64 + lane) * 4);
+    }
+    float m_new = m;
+#pragma unroll
+    for (int j = 0; j < kSide; ++j) m_new = i + kJoin * j < parts ? fmaxf(m_new, stats[j][0]) : m_new;
+    const float old = m == -INFINITY ? 0.f : fast_exp2((m - m_new) * scale);
+    m = m_new;
+    l *= old;
+#pragma unroll
+    for (int f = 0; f < kEach; ++f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[f][e] *= old;
+#pragma unroll
+    for (int j = 0; j < kSide; ++j) {
+      if (i + kJoin * j >= parts) break;
+      const float w = stats[j][0] == -INFINITY ? 0.f : fast_exp2((stats[j][0] - m) * scale);
+      l += w * stats[j][1];
+#pragma unroll
+      for (int f = 0; f < kEach; ++f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[f][e] += w * y[j][f][e];
+    }
+  }
+  red_stats[mine][lane] = floatx2{m, l};
+#pragma unroll
+  for (int f = 0; f < kEach; ++f) red[mine][f][lane] = sum[f];
+  __syncthreads();
+  if (mine >= kEach) return;
+  // a wave for each four
+  m = -INFINITY;
+  l = 0.f;
+  floatx4 total = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < kJoin; ++w) m = fmaxf(m, red_stats[w][lane][0]);
+#pragma unroll
+  for (int w = 0; w < kJoin; ++w) {
+    const float weight = red_stats[w][lane][0] == -INFINITY ? 0.f : fast_exp2((red_stats[w][lane][0] - m) * scale);
+    l += weight * red_stats[w][lane][1];
+    const floatx4 y = red[w][mine][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) total[e] += weight * y[e];
+  }
+  if (row >= x.sequences * heads) return;
+  const int s = row / heads;
+  const int64_t to = (int64_t)(x.first + s) * p.n_q_heads + header.z * heads + row - s * heads;
+  *reinterpret_cast<floatx4*>(p.prefix + to * D + 8 * (f0 + mine) + 4 * (lane >> 5)) = total;
+  if (f0 + mine == 0 && lane < 32) *reinterpret_cast<floatx2*>(p.prefix_stats + 2 * to) = floatx2{m, l};
+}
+
+// Rows of a unit, in blocks of 16: as many as a KV head's queries of a group fill on average, 16 or 32, or more where there are more.
+constexpr int kWide = kWideRows / 16;
+static int prefix_blocks(int batch, int n_q_heads, int n_kv_heads, int n_groups) {
+  const int64_t rows = (int64_t)batch * (n_q_heads / n_kv_heads) / n_groups;
+  return rows <= 16 ? 1 : rows <= 32 ? 2 : kWide;
+}
+
+PagedScratch paged_prefix_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups) {
+  const int blocks = prefix_blocks(batch, n_q_heads, n_kv_heads, n_groups);
+  const size_t rows = (size_t)kPrefixShares * 2 * 16 * blocks;
   PagedScratch s = {0, 0, 0, 0};
   s.stats = (size_t)kPrefixShares * 16;
-  s.parts = s.stats + rows * 8;
+  s.parts = s.stats + rows * (blocks == kWide ? 16 : 8);  // (a row's statistics are there twice, once for each of its lanes)
   s.total = s.parts + rows * head_dim * 4;
   return s;
 }
 
 template <typename T, int D, int BLOCKS>
-static hipError_t launch_paged_prefix_for(const PagedPrefixArgs& a, hipStream_t stream) {
+static void launch_paged_prefix_for(const PagedPrefixArgs& a, hipStream_t stream) {
   constexpr size_t lds = (size_t)kPrefixWaves * 16 * BLOCKS * (D + 4) * 4;
   hipLaunchKernelGGL((paged_prefix_kernel<T, D, BLOCKS>), dim3(kPrefixShares), dim3(64 * kPrefixWaves), lds, stream, a);
-  hipLaunchKernelGGL((paged_prefix_join_kernel<D, BLOCKS>), dim3(kPrefixShares, 4 * BLOCKS), dim3(256), 0, stream, a);
-  return hipGetLastError();
+  hipLaunchKernelGGL((paged_prefix_join_kernel<D, BLOCKS>), dim3(4 * BLOCKS, kPrefixShares), dim3(256), 0, stream, a);
 }
 template <typename T, int D>
 static hipError_t launch_paged_prefix_of(const PagedPrefixArgs& a, hipStream_t stream) {
-  const int blocks = prefix_blocks(a.step.batch, a.step.n_q_heads, a.step.n_kv_heads, D);
-  if (blocks == 1) return launch_paged_prefix_for<T, D, 1>(a, stream);
-  if (blocks == 2) return launch_paged_prefix_for<T, D, 2>(a, stream);
-  return launch_paged_prefix_for<T, D, D == 128 ? 2 : 4>(a, stream);
+  const int blocks = prefix_blocks(a.step.batch, a.step.n_q_heads, a.step.n_kv_heads, a.n_groups);
+  if (blocks == 1) launch_paged_prefix_for<T, D, 1>(a, stream);
+  else if (blocks == 2) launch_paged_prefix_for<T, D, 2>(a, stream);
+  else {
+    hipLaunchKernelGGL((paged_prefix_wide_kernel<T, D>), dim3(kPrefixShares), dim3(kWideThreads), 0, stream, a);
+    hipLaunchKernelGGL((paged_prefix_wide_join_kernel<D>), dim3(D / 4, kPrefixShares), dim3(512), 0, stream, a);
+  }
+  return hipGetLastError();
 }
 hipError_t launch_paged_prefix(const PagedPrefixArgs& a, hipStream_t stream) {
   if (a.step.head_dim == 128) return a.step.dtype == 0 ? launch_paged_prefix_of<Bf16, 128>(a, stream) : launch_paged_prefix_of<F16, 128>(a, stream);

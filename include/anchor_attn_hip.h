@@ -374,7 +374,7 @@ size_t aa_paged_decode_workspace_bytes(int batch, int n_q_heads, int n_kv_heads,
 int aa_paged_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, void* stream);
 size_t aa_paged_weighing_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages);
 int aa_paged_weighing_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, float* weights, int n_first, void* stream);
-size_t aa_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages);
+size_t aa_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_groups);
 int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* step, const int32_t* shared_pages, const int32_t* groups, int n_groups, void* stream);
 size_t aa_paged_evict_workspace_bytes(int batch, int n_kv_heads, int head_dim, int n_keys);
 int aa_paged_evict(const aa_paged_cache* cache, const aa_paged_eviction* eviction, void* stream);

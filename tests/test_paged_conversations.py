@@ -419,10 +419,10 @@ def test_what_the_c_interface_of_steps_refuses(fn, change, message):
 def test_scratch_of_steps():
     from anchor_attn.src.ops import _hip
     lib = _hip.lib()
-    assert lib.aa_paged_weighing_workspace_bytes(0, 8, 2, 128, 16, 8) == 0 == lib.aa_paged_shared_workspace_bytes(2, 0, 2, 128, 16, 8)
+    assert lib.aa_paged_weighing_workspace_bytes(0, 8, 2, 128, 16, 8) == 0 == lib.aa_paged_shared_workspace_bytes(2, 0, 2, 128, 16, 8, 1) == lib.aa_paged_shared_workspace_bytes(2, 8, 2, 128, 16, 8, 0)
     assert lib.aa_paged_weighing_workspace_bytes(2, 8, 2, 128, 16, 8) >= 2 * 8 * (16 * 8 + 2) * 4
     assert lib.aa_paged_weighing_workspace_bytes(128, 32, 8, 128, 16, 65536) >= 128 * 32 * (1 << 22)
-    assert lib.aa_paged_shared_workspace_bytes(2, 8, 2, 128, 16, 8) >= 2 * 8 * 130 * 4
+    assert lib.aa_paged_shared_workspace_bytes(2, 8, 2, 128, 16, 8, 1) >= 2 * 8 * 130 * 4
 
 
 @pytest.mark.gpu
