@@ -569,7 +569,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
   if (!goes_on && tid == 0 && p.headers != nullptr) header->x = 0;
 }
 
-// Joins the parts of a column whose unit begins in share blockIdx.x and ends in another: the weights first, then groups of D / 4 lanes add up
+// Joins the parts of a column whose unit begins in share blockIdx.y and ends in another (units begin every so many shares: shares as blockIdx.x would be one XCD's): the
+// weights first, then groups of D / 4 lanes add up
 // every so many parts.  Few bytes; the launch and three loads one after the other take 3 to 5 us, which a step pays whether or not a unit was cut, since the
 // host does not know the lengths.
 template <typename T, int D, DecodeMode MODE>
@@ -577,13 +578,13 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArg
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
   __shared__ float weight[256], red[2][4];
   __shared__ floatx4 sums[kGroups][kLanes];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = blockIdx.y;
-  const int4 header = *reinterpret_cast<const int4*>(p.headers + 4 * blockIdx.x);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = blockIdx.x, share = blockIdx.y;
+  const int4 header = *reinterpret_cast<const int4*>(p.headers + 4 * share);
   const int parts = header.x;
   if (parts == 0 || col >= header.w) return;
   const float scale = p.sm_scale * kLog2e;
   // the first part is the second of its share, the others the first of theirs
-  auto part = [&](const int i) { return ((int64_t)2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * kCols + col; };
+  auto part = [&](const int i) { return ((int64_t)2 * (share + i) + (i == 0 ? 1 : 0)) * kCols + col; };
   static_assert(kShares <= 256, "a thread has a part's maximum and sum");
   const int gr = tid / kLanes, d4 = tid % kLanes;
   floatx4 early[4];  // (requested with the maxima)
@@ -682,7 +683,7 @@ static void launch_paged_decode_as(const PagedDecodeArgs& a, hipStream_t stream)
   const int64_t most = (int64_t)a.batch * units * (((int64_t)a.max_pages << a.page_log) / kTile + 1 + kOver);
   if (most < 1ll << 30) hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int, MODE>), dim3(kShares), dim3(256), lds, stream, a);
   else hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int64_t, MODE>), dim3(kShares), dim3(256), lds, stream, a);
-  if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D, MODE>), dim3(kShares, cols), dim3(256), 0, stream, a);
+  if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D, MODE>), dim3(cols, kShares), dim3(256), 0, stream, a);
   if (MODE == kWeigh) {
     // work-groups of a (sequence, KV head): as many as its table has room for, or fewer where there are thousands in all
     const int64_t all = (int64_t)a.batch * a.n_kv_heads, room = (((int64_t)a.max_pages << a.page_log) + 1023) / 1024, each = all < 8192 ? 8192 / all : 1;

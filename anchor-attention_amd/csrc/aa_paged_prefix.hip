@@ -16,7 +16,7 @@
 namespace aa {
 
 constexpr int kPrefixTile = 32, kPrefixWaves = 4, kPrefixShares = 256, kPrefixSharesLog = 8;
-constexpr int kPrefixLeast = 8;  // tiles of a share at least
+constexpr int kPrefixLeast = 8, kPrefixOver = 4;  // tiles of a share at least; what a unit costs beside its tiles, in tiles
 
 // A group's sequences and prefix; nothing that memory says is trusted.
 struct PagedGroup {
@@ -68,14 +68,17 @@ template <int ROWS>
 __device__ __forceinline__ int blocks_of(const PagedGroup& x, const int heads) {
   return (x.sequences * heads + ROWS - 1) / ROWS;
 }
-template <int TILE, int ROWS>
+// A unit's extent: its tiles, and before them what its beginning and end cost, in tiles (0 where there are none)
+template <int OVER>
+__device__ __forceinline__ int extent_of(const int tiles) { return tiles > 0 ? tiles + OVER : 0; }
+template <int TILE, int ROWS, int OVER>
 __device__ __forceinline__ PrefixShare share_of(const PagedPrefixArgs& all, const int share, const int least) {
   const PagedDecodeArgs& p = all.step;
   const int lane = threadIdx.x & 63, heads = p.n_q_heads / p.n_kv_heads;
-  auto extent_of = [&](const int i) {  // of group i's units
+  auto extents_of = [&](const int i) {  // of group i's units
     if (i >= all.n_groups) return (int64_t)0;
     const PagedGroup x = group_at(all, i);
-    return (int64_t)tiles_of<TILE>(p, x) * blocks_of<ROWS>(x, heads) * p.n_kv_heads;
+    return (int64_t)extent_of<OVER>(tiles_of<TILE>(p, x)) * blocks_of<ROWS>(x, heads) * p.n_kv_heads;
   };
   auto up_to_lane = [&](int64_t x) {
 #pragma unroll
@@ -87,15 +90,15 @@ __device__ __forceinline__ PrefixShare share_of(const PagedPrefixArgs& all, cons
   };
   PrefixShare r = {0, 0, 0, 0, 0};
   int64_t total = 0;
-  if (all.n_groups == 1) total = extent_of(0);
+  if (all.n_groups == 1) total = extents_of(0);
   else
-    for (int i = 0; i < all.n_groups; i += 64) total += __shfl((long long)up_to_lane(extent_of(i + lane)), 63, 64);
+    for (int i = 0; i < all.n_groups; i += 64) total += __shfl((long long)up_to_lane(extents_of(i + lane)), 63, 64);
   r.share = max((total + (kPrefixShares - 1)) >> kPrefixSharesLog, (int64_t)least);
   r.at = min(r.share * share, total);
   r.end = min(r.at + r.share, total);
   if (r.at < r.end && all.n_groups > 1) {
     for (int i = 0; i < all.n_groups; i += 64) {
-      const int64_t sum = up_to_lane(extent_of(i + lane));
+      const int64_t sum = up_to_lane(extents_of(i + lane));
       const int in = __popcll(__ballot(r.start + sum <= r.at));
       if (in < 64) {
         r.group = i + in;
@@ -123,7 +126,7 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
   find_skips(all, tid, 64 * kPrefixWaves);
 
   // ---- this work-group's share ---------------------------------------------------------------------
-  const PrefixShare mine = share_of<kPrefixTile, kRows>(all, blockIdx.x, kPrefixLeast);
+  const PrefixShare mine = share_of<kPrefixTile, kRows, kPrefixOver>(all, blockIdx.x, kPrefixLeast);
   int64_t at = mine.at, start = mine.start;
   const int64_t end = mine.end, share = mine.share;
   int group = mine.group;
@@ -142,13 +145,16 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
     x.sequences = __builtin_amdgcn_readfirstlane(x.sequences);
     x.pages = __builtin_amdgcn_readfirstlane(x.pages);
     const int tiles = tiles_of<kPrefixTile>(p, x), blocks = blocks_of<kRows>(x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
-    if (at - start >= (int64_t)tiles * blocks * p.n_kv_heads) {  // (the next group, perhaps of nothing)
-      start += (int64_t)tiles * blocks * p.n_kv_heads;
+    const int extent = extent_of<kPrefixOver>(tiles);
+    if (at - start >= (int64_t)extent * blocks * p.n_kv_heads) {  // (the next group, perhaps of nothing)
+      start += (int64_t)extent * blocks * p.n_kv_heads;
       ++group;
       continue;
     }
-    const uint32_t unit = (uint32_t)((at - start) / tiles), block = unit % (uint32_t)blocks, kvh = unit / (uint32_t)blocks;
-    const int t0 = (int)(at - start - (int64_t)unit * tiles), t1 = (int)min((int64_t)tiles, t0 + (end - at));
+    const uint32_t unit = (uint32_t)((at - start) / extent), block = unit % (uint32_t)blocks, kvh = unit / (uint32_t)blocks;
+    const int64_t unit_end = start + (int64_t)(unit + 1) * extent, until = min(end, unit_end);
+    const int t0 = max(tiles - (int)(unit_end - at), 0), t1 = max(tiles - (int)(unit_end - until), 0);
+    if (t1 == 0) break;  // (nothing of it is in this share, which ends)
     const int row0 = block * kRows, n_blocks = min(BLOCKS, (rows - row0 + 15) / 16);
     const int from = t0 + (t1 - t0) * wave / kPrefixWaves, to = t0 + (t1 - t0) * (wave + 1) / kPrefixWaves;
 
@@ -383,11 +389,10 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
       if (d == 0) *reinterpret_cast<floatx2*>(stats + 2 * to_row) = floatx2{m, l};
     }
     if (begins && !ends && tid == 0) {  // its other parts are the next work-groups'
-      const int64_t last = start + (int64_t)(unit + 1) * tiles - 1;
-      *header = int4{(int)(last / share) - (int)blockIdx.x + 1, group, (int)kvh, (int)block};
+      *header = int4{(int)((unit_end - 1) / share) - (int)blockIdx.x + 1, group, (int)kvh, (int)block};
     }
     __syncthreads();
-    at += t1 - t0;
+    at = until;
   }
 }
 
@@ -430,7 +435,7 @@ __global__ void __launch_bounds__(256) paged_prefix_join_kernel(const PagedPrefi
 // that the memory system fills, chunks swizzled.  Eight waves are two teams that take the tiles in turn and are never in the same half of a tile: while one multiplies (the last tile's
 // probabilities with its values, the next one's keys with the queries), the other forms probabilities, a barrier between the halves, so that the matrix pipe has one team's work at a time and
 // the vector ALU the other's.  Tiles are requested one tile ahead.
-constexpr int kWideTile = 64, kWideRows = 128, kWideThreads = 512, kWideLeast = 4;
+constexpr int kWideTile = 64, kWideRows = 128, kWideThreads = 512, kWideLeast = 4, kWideOver = 5;
 
 template <int D>
 __device__ __forceinline__ int wide_k_swizzle(const int r) { return D == 128 ? r & 15 : (r & 7) ^ ((r >> 3) & 1); }
@@ -465,7 +470,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
   const int heads = p.n_q_heads / p.n_kv_heads, page_mask = (1 << p.page_log) - 1;
   // neighbouring shares, which have neighbouring rows of one KV head, are one XCD's
   const int share_at = (blockIdx.x % 8) * (kPrefixShares / 8) + blockIdx.x / 8;
-  const PrefixShare mine = share_of<kWideTile, kWideRows>(all, share_at, kWideLeast);
+  const PrefixShare mine = share_of<kWideTile, kWideRows, kWideOver>(all, share_at, kWideLeast);
   int64_t at = mine.at, start = mine.start;
   const int64_t end = mine.end, share = mine.share;
   int group = mine.group;
@@ -493,14 +498,17 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     x.sequences = __builtin_amdgcn_readfirstlane(x.sequences);
     x.pages = __builtin_amdgcn_readfirstlane(x.pages);
     const int n_tiles = tiles_of<kWideTile>(p, x), blocks = blocks_of<kWideRows>(x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
-    if (at - start >= (int64_t)n_tiles * blocks * p.n_kv_heads) {  // (the next group, perhaps of nothing)
-      start += (int64_t)n_tiles * blocks * p.n_kv_heads;
+    const int extent = extent_of<kWideOver>(n_tiles);
+    if (at - start >= (int64_t)extent * blocks * p.n_kv_heads) {  // (the next group, perhaps of nothing)
+      start += (int64_t)extent * blocks * p.n_kv_heads;
       ++group;
       continue;
     }
     // a KV head's blocks one after the other
-    const uint32_t unit = (uint32_t)((at - start) / n_tiles), block = unit % (uint32_t)blocks, kvh = unit / (uint32_t)blocks;
-    const int t0 = (int)(at - start - (int64_t)unit * n_tiles), t1 = (int)min((int64_t)n_tiles, t0 + (end - at));
+    const uint32_t unit = (uint32_t)((at - start) / extent), block = unit % (uint32_t)blocks, kvh = unit / (uint32_t)blocks;
+    const int64_t unit_end = start + (int64_t)(unit + 1) * extent, until = min(end, unit_end);
+    const int t0 = max(n_tiles - (int)(unit_end - at), 0), t1 = max(n_tiles - (int)(unit_end - until), 0);
+    if (t1 == 0) break;  // (nothing of it is in this share, which ends)
     const int my_row = min((int)(block * kWideRows) + 32 * wave + c32, rows - 1), sequence = my_row / heads;
     const int64_t my_head = (int64_t)(x.first + sequence) * p.n_q_heads + (int)kvh * heads + my_row - sequence * heads;
     typename T::vec8 q[kKS];
@@ -530,10 +538,17 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
     };
-    float m_run = -INFINITY, l_run = 0.f;
-    floatx16 acc[kDB], s[2];
-    u32x4 prob[4], rest[4];
-    // What a team multiplies of a round: operand f is of values (two products, with probabilities and their rest) or, from kValues on, of the next tile's keys.  Operands are read from LDS
+    // (the sums of the probabilities as they were rounded, by products with ones: each of the sixteen is a row's)
+    float m_run = -INFINITY;
+    floatx16 acc[kDB], s[2], sums;
+    typename T::vec8 ones;
+    {
+      const uint32_t two = T::pack(1.f, 1.f);
+      const u32x4 all_ones = {two, two, two, two};
+      ones = *reinterpret_cast<const typename T::vec8*>(&all_ones);
+    }
+    u32x4 prob[4];
+    // What a team multiplies of a round: operand f is of values or, from kValues on, of the next tile's keys.  Operands are read from LDS
     // kAhead ahead of the products that take them, in this order, which the compiler would not keep; the first ones before the barrier.
     constexpr int kAhead = D == 128 ? 6 : 6, kValues = 4 * kDB, kKeys = 2 * kKS;
     u32x4 operand[kAhead];
@@ -549,19 +564,9 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         operand[f % kAhead] = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(((k_rd + ((i + 1) & 1) * kTileBytes) ^ ((g % kKS) << 5)) + 32 * (g / kKS) * kRowBytes);
       }
     };
-    auto multiply_values = [&](const int f, auto exact) __attribute__((always_inline)) {
-      const int st = f / kDB, db = f % kDB;
-      u32x4 v = operand[f % kAhead];
-      acc[db] = T::mfma(*reinterpret_cast<const typename T::vec8*>(&v), *reinterpret_cast<const typename T::vec8*>(&prob[st]), acc[db]);
-      if constexpr (decltype(exact)::value) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t y = v[w];
-          if ((y & T::kExponent) == T::kExponent) v[w] &= 0xffff0000u;
-          if (((y >> 16) & T::kExponent) == T::kExponent) v[w] &= 0xffffu;
-        }
-      }
-      acc[db] = T::mfma(*reinterpret_cast<const typename T::vec8*>(&v), *reinterpret_cast<const typename T::vec8*>(&rest[st]), acc[db]);
+    auto multiply_values = [&](const int f) __attribute__((always_inline)) {
+      acc[f % kDB] = T::mfma(*reinterpret_cast<const typename T::vec8*>(&operand[f % kAhead]), *reinterpret_cast<const typename T::vec8*>(&prob[f / kDB]), acc[f % kDB]);
+      if (f % kDB == kDB - 1) sums = T::mfma(ones, *reinterpret_cast<const typename T::vec8*>(&prob[f / kDB]), sums);
     };
     auto multiply_keys = [&](const int g) __attribute__((always_inline)) {
       floatx16 none;
@@ -583,7 +588,8 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
       const float m_base = m_new == -INFINITY ? 0.f : m_new;  // (no key of this row's so far)
       if (__any(m_new > m_run)) {
         const float alpha = fast_exp2((m_run - m_base) * scale);
-        l_run *= alpha;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sums[r] *= alpha;
 #pragma unroll
         for (int db = 0; db < kDB; ++db)
 #pragma unroll
@@ -595,18 +601,17 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
 #pragma unroll
       for (int w = 0; w < 16; ++w) {
         const float e0 = fast_exp2(__builtin_fmaf(s[w >> 3][2 * (w & 7)], scale, bias)), e1 = fast_exp2(__builtin_fmaf(s[w >> 3][2 * (w & 7) + 1], scale, bias));
-        l_run += e0 + e1;
         uint32_t both = T::pack(e0, e1);
         if constexpr (decltype(exact)::value) {
           if (e0 > 0.f && (both & 0xffffu) == 0u) both |= 1u;
           if (e1 > 0.f && (both >> 16) == 0u) both |= 0x10000u;
         }
         prob[w >> 2][w & 3] = both;
-        rest[w >> 2][w & 3] = T::pack_rest(e0, e1, both);
       }
     };
     auto run = [&](auto exact) __attribute__((always_inline)) {
-      l_run = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sums[r] = 0.f;
 #pragma unroll
       for (int db = 0; db < kDB; ++db)
 #pragma unroll
@@ -631,7 +636,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         if (i > 0) {
 #pragma unroll
           for (int f = 0; f < kValues; ++f) {
-            multiply_values(f, exact);
+            multiply_values(f);
             read(i - 1, f + kAhead);
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -662,7 +667,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
       if (own > 0) {
 #pragma unroll
         for (int f = 0; f < kValues; ++f) {
-          multiply_values(f, exact);
+          multiply_values(f);
           if (f + kAhead < kValues) read(own - 1, f + kAhead);
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -680,13 +685,9 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     for (int db = 0; db < kDB; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum += acc[db][r];
-    // Infinite values: with two products per key they give NaN.  Once more, relative to the maximum: the rest meets the finite values only and a positive probability
-    // does not round to 0.
-    if (__builtin_expect(__syncthreads_or(is_nan(sum) && !is_nan(l_run)), 0)) run(std::true_type{});
-    {
-      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
-      l_run = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
+    // Infinite values meet probabilities that were rounded to 0, or those relative to an earlier maximum.  Once more, relative to the last one: a positive probability does not round to 0.
+    if (__builtin_expect(__syncthreads_or(is_nan(sum) && !is_nan(sums[0])), 0)) run(std::true_type{});
+    const float l_run = sums[0];
 
     // ---- the teams' states -> the unit's, or a part of it: fours of accumulators, lane by lane, half of them by each team ----
     floatx4* states = reinterpret_cast<floatx4*>(&tiles[0][0][0]) + wave * kFours * 64;
@@ -723,11 +724,10 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     if (team == 0) finish(lower);
     else finish(upper);
     if (t0 == 0 && t1 < n_tiles && tid == 0) {  // its other parts are the next work-groups'
-      const int64_t last = start + (int64_t)(unit + 1) * n_tiles - 1;
-      *header = int4{(int)(last / share) - share_at + 1, group, (int)kvh, (int)block};
+      *header = int4{(int)((unit_end - 1) / share) - share_at + 1, group, (int)kvh, (int)block};
     }
     __syncthreads();
-    at += t1 - t0;
+    at = until;
   }
   find_skips(all, tid, kWideThreads);
 }

@@ -5,7 +5,10 @@ Tolerances beside those of tests/test_paged_cache.py (u: half a step of the 16-b
 Norm and rotation: a float32 sum of D squares is off by at most D * 2^-24 of it, its inverse root by half of that and 2^-22, three products by 2^-24 each,
 the rotation by 2^-23 of its products' magnitudes: (D / 2 + 16) * 2^-24 of the magnitudes, and u of the result.
 Weights: a probability is off by what tests/test_paged_cache.py says of it, 2 * D * 2^-24 * sum |q_d k_d| * scale + 2^-14 of it, a sum over the group's heads in float32 and the addition to
-what was there by 2^-24 of each partial sum."""
+what was there by 2^-24 of each partial sum.
+Over a prefix that more than 32 rows share (a group's queries of a KV head's group, on average) probabilities p_i are rounded once, by u of each at most, and their sum l is
+that of the rounded ones: an output o = sum p_i v_i / l is off by sum d_i p_i (v_i - o) / l with |d_i| <= u, at most u (sum p_i |v_i| / l + |o|), 1 % more with
+what is of second order."""
 
 import ctypes
 import pathlib
@@ -296,6 +299,26 @@ def _shared_setup(prefixes, sizes, own, hkv, d, page, dtype, seed, layout="heads
     return s, _int32(prefixes), _int32(begins)
 
 
+def _shared_close(out, q, s, scale, n_groups):
+    """What :func:`_close` asks for, and where more than 32 rows share a prefix the rounding of probabilities."""
+    group = q.shape[1] // s.hkv
+    if q.shape[0] * group // n_groups <= 32:
+        return _close(out, q, s, scale)
+    for b in range(q.shape[0]):
+        for h in range(s.hkv):
+            got = out[b, h * group:(h + 1) * group].double()
+            if s.host[b] == 0:
+                assert bool((got == 0).all())
+                continue
+            k, v, x = s.rows(s.cache.keys, b, h), s.rows(s.cache.values, b, h), q[b, h * group:(h + 1) * group].double()
+            p = (x @ k.T * scale).softmax(-1)
+            want = p @ v
+            relative = 2.0 * s.d * 2.0 ** -24 * (x.abs() @ k.abs().T).amax(-1, keepdim=True) * scale + 2.0 ** -14 + k.shape[0] * 2.0 ** -24 + 1.01 * U[out.dtype]
+            bound = 2.02 * U[out.dtype] * want.abs() + relative * (p @ v.abs()) + 2.0 ** -25
+            err = (got - want).abs()
+            assert bool((err <= bound).all()), (b, h, float((err - bound).max()), float(err.max()))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("prefixes,sizes,own,hq,hkv,d,page,layout,extra,alone", [
@@ -319,10 +342,10 @@ def test_shared_decode(prefixes, sizes, own, hq, hkv, d, page, layout, extra, al
     out = wide[:, 1:, 8:]
     assert _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, out=out) is out
     assert bool((wide[:, 0] == 7.0).all()) and bool((wide[:, :, :8] == 7.0).all())
-    _close(out, q, s, d ** -0.5)
+    _shared_close(out, q, s, d ** -0.5, len(sizes))
     again = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, sm_scale=d ** -0.5)
     assert torch.equal(out, again)  # the same bits
-    _close(_ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, sm_scale=0.3), q, s, 0.3)
+    _shared_close(_ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, sm_scale=0.3), q, s, 0.3, len(sizes))
     if len(sizes) == 1 and not alone:
         assert torch.equal(_ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared), out)
     assert _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, out=q) is q and torch.equal(q, again)
@@ -362,7 +385,9 @@ def test_shared_decode_with_infinite_values_and_scores(batch, pages, dtype):
     assert torch.equal(got[:, 4:], want[:, 4:])
     rest = torch.ones(64, dtype=torch.bool, device="cuda")
     rest[5:8] = False
-    assert bool(((got[:, :4, rest] - want[:, :4, rest]).abs() <= 2 * U[dtype] * want[:, :4, rest].abs() + 2.0 ** -13).all())
+    # (probabilities rounded once may have been so relative to different maxima: values below 4 by 2 u each way)
+    slack = 8 * U[dtype] if batch * 4 > 32 else 0.0
+    assert bool(((got[:, :4, rest] - want[:, :4, rest]).abs() <= 2 * U[dtype] * want[:, :4, rest].abs() + 2.0 ** -13 + slack).all())
     # minus infinity: the keys of the prefix for KV head 0, all own keys of sequence 1 for KV head 1, all of sequence 2 for both
     s.cache.values[at, 0, :, 5:8] = 0.5
     s.cache.keys[s.table[0, :pages].long(), 0, :, 0] = float("-inf")
@@ -371,7 +396,7 @@ def test_shared_decode_with_infinite_values_and_scores(batch, pages, dtype):
     got = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
     plain = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
     assert bool(got[2, :4].isnan().all()) and bool(plain[2, :4].isnan().all()) and int(got.isnan().sum()) == 4 * 64
-    near = (got.double() - plain.double()).abs() <= 2 * U[dtype] * plain.abs() + 2.0 ** -12
+    near = (got.double() - plain.double()).abs() <= 2 * U[dtype] * plain.abs() + 2.0 ** -12 + slack
     assert bool((near | plain.isnan()).all())
 
 
