@@ -5,7 +5,7 @@
 // does not matter.  Weights stay in LDS between the rounds, or are read again where there are more than it holds.
 //
 // Moving is bound by reading and writing the rows once.  It is in place, and rows go to lower places in their order, so a work-group that takes them in turn, each chunk read by all before
-// any of it is written, needs no room beside: no later row lies where an earlier one goes.  A work-group has 64 channels of keys or values, a line of the cache; where that makes too few
+// any of it is written, needs no room beside: no later row lies where an earlier one goes.  A work-group has 32 channels of keys or values; where that makes too few
 // work-groups, the rows of a (sequence, KV head) are cut into groups, and those that come from another group's places are copied to scratch by a launch of its own first.
 #include <algorithm>
 
@@ -21,7 +21,8 @@ constexpr int kMostKeys = 1 << 20;
 __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedEvictArgs p) {
   extern __shared__ __attribute__((aligned(16))) uint32_t stay[];  // the weights, or where there are too many of them, the counts
   static_assert(kMostKeys / kKeepStep * kKeepWaves * 2 <= kKeepInLds, "the counts take less room");
-  __shared__ __attribute__((aligned(16))) uint32_t bins[4][256];
+  constexpr int kCopies = 8;  // of the first round's bins, for every eighth lane: most weights are of few bins, which lanes would wait for
+  __shared__ __attribute__((aligned(16))) uint32_t bins[3 + kCopies][256];  // (the first round's last)
   __shared__ uint32_t ranges[2][kKeepWaves];
   __shared__ uint64_t few_counts[kKeepInLds / kKeepStep * kKeepWaves];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -37,7 +38,7 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedEvi
   const bool in_lds = n <= kKeepInLds;
   uint64_t* counts = in_lds ? few_counts : reinterpret_cast<uint64_t*>(stay);
   const int first = p.n_first, end = n - p.n_last;  // the candidates
-  bins[0][tid] = 0u;
+  for (int i = tid; i < (3 + kCopies) * 256; i += kKeepThreads) bins[0][i] = 0u;
   // weights as numbers of the same order; 0 for what is no candidate
   auto load = [&](const int i, uint32_t (&x)[4]) {
     const int64_t page = clamped_page(p.table[b * p.t_sb + (i >> p.page_log)], p.n_pages);
@@ -102,20 +103,24 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedEvi
   for (int round = 0; wanted > 0 && lo < hi; ++round) {
     const uint32_t span = hi - lo;
     const int shift = span < 256u ? 0 : 24 - __builtin_clz(span);  // span >> shift < 256
+    uint32_t* mine = bins[round == 0 ? 3 + (lane & (kCopies - 1)) : round - 1];
     uint32_t least_ones = 0;  // (not one by one: weights that nothing has been added to are alike)
     each([&](const int, const uint32_t (&x)[4]) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t d = x[e] - lo;
         if (d == 0u) ++least_ones;
-        else if (d <= span) atomicAdd(&bins[round][d >> shift], 1u);
+        else if (d <= span) atomicAdd(&mine[d >> shift], 1u);
       }
     });
     least_ones = (uint32_t)sums_up_to((int)least_ones);
-    if (lane == 63 && least_ones > 0) atomicAdd(&bins[round][0], least_ones);
+    if (lane == 63 && least_ones > 0) atomicAdd(&mine[0], least_ones);
     __syncthreads();
-    const uint4 bin4 = *reinterpret_cast<const uint4*>(&bins[round][4 * lane]);
-    const int m[4] = {(int)bin4.x, (int)bin4.y, (int)bin4.z, (int)bin4.w};
+    int m[4] = {0, 0, 0, 0};
+    for (int c = round == 0 ? 3 : round - 1; c < (round == 0 ? 3 + kCopies : round); ++c) {
+      const uint4 bin4 = *reinterpret_cast<const uint4*>(&bins[c][4 * lane]);
+      m[0] += bin4.x, m[1] += bin4.y, m[2] += bin4.z, m[3] += bin4.w;
+    }
     const int own = m[0] + m[1] + m[2] + m[3], sums = sums_up_to(own), all = __builtin_amdgcn_readlane(sums, 63);
     // the last lane that has `wanted` weights in its bins or behind them, and the last of its bins that has
     const int at = 63 - __builtin_clzll(__ballot(all - sums + own >= wanted));
@@ -176,9 +181,12 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedEvi
   for (int i = tid; i < p.n_last; i += kKeepThreads) kept[p.n_keys - p.n_last + i] = end + i;
 }
 
-// f over the lanes of a wave that have the same piece of 8 rows (lane % 8)
+// A slice: so many channels of a row, 8 by a lane.
+constexpr int kSlice = 32, kPieces = kSlice / 8, kWaveRows = 64 / kPieces;
+// f over the lanes of a wave that have the same piece (lane % kPieces)
 template <typename F>
-__device__ __forceinline__ uint32_t over_eighths(uint32_t x, F f) {
+__device__ __forceinline__ uint32_t over_rows(uint32_t x, F f) {
+  if (kPieces == 4) x = f(x, dpp<kDppRor4>(x));
   x = f(x, dpp<kDppRor8>(x));
   const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
   x = f(r[0], r[1]);
@@ -186,8 +194,8 @@ __device__ __forceinline__ uint32_t over_eighths(uint32_t x, F f) {
   return f(s[0], s[1]);
 }
 
-constexpr int kMoveThreads = 512, kMoveRows = kMoveThreads / 8;  // side by side: 8 lanes a row of 64 channels
-constexpr int kMoveEach = 4, kMoveChunk = kMoveEach * kMoveRows;   // where there are several groups, whose rows are a multiple of it
+constexpr int kMoveThreads = 512, kMoveRows = kMoveThreads / kPieces;  // side by side
+constexpr int kMoveEach = 256 / kMoveRows, kMoveChunk = kMoveEach * kMoveRows;   // where there are several groups, whose rows are a multiple of it
 
 // A (sequence, KV head) and what of its rows this work-group has: 64 channels of keys or of values.
 struct MoveSlice {
@@ -201,13 +209,13 @@ struct MoveSlice {
 };
 template <int D>
 __device__ __forceinline__ MoveSlice slice_of(const PagedEvictArgs& p) {
-  constexpr int kSlices = D / 64;
+  constexpr int kSlices = D / kSlice;
   MoveSlice s;
   s.b = blockIdx.x / p.n_kv_heads;
   s.kvh = blockIdx.x - s.b * p.n_kv_heads;
   s.unit = (int64_t)blockIdx.x * p.n_keys;
   s.values = blockIdx.y >= kSlices;
-  s.channel = 64 * (blockIdx.y % kSlices) + 8 * (threadIdx.x & 7);
+  s.channel = kSlice * (blockIdx.y % kSlices) + 8 * (threadIdx.x % kPieces);
   return s;
 }
 
@@ -221,7 +229,7 @@ __global__ void __launch_bounds__(kMoveThreads) paged_save_kernel(const PagedEvi
   const int group_end = (begin / p.group_rows + 1) * p.group_rows;
 #pragma unroll
   for (int j = 0; j < kMoveEach; ++j) {
-    const int i = begin + kMoveRows * j + (threadIdx.x >> 3);
+    const int i = begin + kMoveRows * j + (int)(threadIdx.x / kPieces);
     if (i >= end) break;
     const int from = p.kept[s.unit + i];
     if (from < group_end || from >= p.n_keys) continue;
@@ -271,14 +279,14 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const PagedEvi
   constexpr int kWaves = kMoveThreads / 64, kChunk = EACH * kMoveRows;
   static_assert(kChunk % 256 == 0, "a page's rows lie in a chunk");
   constexpr int kStaged = 4096;                    // rows whose places are in LDS, a multiple of a chunk
-  __shared__ uint4 red[EACH * kWaves][8][2];  // bounds of 8 rows each, in their order
+  __shared__ uint4 red[EACH * kWaves][kPieces][2];  // bounds of kWaveRows rows each, in their order
   __shared__ int2 source[kStaged];                 // the place that a row comes from, and its page
   __shared__ int target[kStaged / 16];             // the pages that rows go to
   const MoveSlice s = slice_of<D>(p);
   uint16_t* pool = s.values ? p.values : p.keys;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, page_size = 1 << p.page_log;
   const int end = min((int)(blockIdx.z + 1) * p.group_rows, p.n_keys);
-  if (blockIdx.y == D / 32) return move_weights(p, s, end);
+  if (blockIdx.y == 2 * D / kSlice) return move_weights(p, s, end);
   const int32_t* table = p.table + s.b * p.t_sb;
   int begin = blockIdx.z * p.group_rows;
   // what keeps its place is left alone: the chunks whose last row does, and is the last of its page
@@ -304,7 +312,7 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const PagedEvi
     auto load = [&](Chunk& c, const int at) __attribute__((always_inline)) {  // (behind the last row, that one)
 #pragma unroll
       for (int j = 0; j < EACH; ++j) {
-        const int i = min(at + kMoveRows * j + (tid >> 3), staged_end - 1);
+        const int i = min(at + kMoveRows * j + tid / kPieces, staged_end - 1);
         const uint64_t both = *reinterpret_cast<const uint64_t*>(&source[i - begin]);
         const int from = (int)(uint32_t)both, page = (int)(uint32_t)(both >> 32);
         const int64_t row = page * row_page + (from & (page_size - 1)) * row_slot + row_head, scratch_row = ((s.unit + i) * 2 + s.values) * D + s.channel;
@@ -319,7 +327,7 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const PagedEvi
       lds_barrier();
 #pragma unroll
       for (int j = 0; j < EACH; ++j) {
-        const int i = at + kMoveRows * j + (tid >> 3);
+        const int i = at + kMoveRows * j + tid / kPieces;
         if (i >= staged_end) continue;
         const int page = target[(i - begin) >> p.page_log];
         if (source[i - begin].x != i && (uint32_t)page < (uint32_t)p.n_pages) *reinterpret_cast<u32x4*>(pool + page * row_page + (i & (page_size - 1)) * row_slot + row_head) = c.x[j];
@@ -327,28 +335,28 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const PagedEvi
       if (s.values || p.bounds == nullptr) return;
 #pragma unroll
       for (int j = 0; j < EACH; ++j) {
-        const int i = at + kMoveRows * j + (tid >> 3);
+        const int i = at + kMoveRows * j + tid / kPieces;
         uint32_t lo[4], hi[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           lo[e] = i < staged_end ? in_order(c.x[j][e]) : 0x7fff7fffu;
           hi[e] = i < staged_end ? in_order(c.x[j][e]) : 0x80008000u;
-          lo[e] = over_eighths(lo[e], least);
-          hi[e] = over_eighths(hi[e], most);
+          lo[e] = over_rows(lo[e], least);
+          hi[e] = over_rows(hi[e], most);
         }
-        if (lane < 8) {
+        if (lane < kPieces) {
           red[kWaves * j + wave][lane][0] = uint4{lo[0], lo[1], lo[2], lo[3]};
           red[kWaves * j + wave][lane][1] = uint4{hi[0], hi[1], hi[2], hi[3]};
         }
       }
       lds_barrier();
-      // eight lanes a page of the chunk
-      const int mine = at + (tid >> 3) * page_size, last = min(mine + page_size, staged_end) - 1;
+      // kPieces lanes a page of the chunk
+      const int mine = at + tid / kPieces * page_size, last = min(mine + page_size, staged_end) - 1;
       if (mine >= min(at + kChunk, staged_end) || (source[last - begin].x == last && last + 1 == mine + page_size)) return;
-      const int page = target[(mine - begin) >> p.page_log], r0 = (mine - at) >> 3;
+      const int page = target[(mine - begin) >> p.page_log], r0 = (mine - at) / kWaveRows;
       uint32_t lo[4] = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu}, hi[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-      for (int r = r0; r < r0 + (page_size >> 3); ++r) {
-        const uint4 l = red[r][tid & 7][0], h = red[r][tid & 7][1];
+      for (int r = r0; r < r0 + page_size / kWaveRows; ++r) {
+        const uint4 l = red[r][tid % kPieces][0], h = red[r][tid % kPieces][1];
         const uint32_t ls[4] = {l.x, l.y, l.z, l.w}, hs[4] = {h.x, h.y, h.z, h.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -380,7 +388,7 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const PagedEvi
 // Rows of a group: all of them where that makes work-groups enough, or as few as make so many.
 constexpr int kMoveEnough = 256;
 int paged_evict_group_rows(int batch, int n_kv_heads, int head_dim, int n_keys) {
-  const int64_t slices = (int64_t)batch * n_kv_heads * 2 * (head_dim / 64);
+  const int64_t slices = (int64_t)batch * n_kv_heads * 2 * (head_dim / kSlice);
   const int chunks = (n_keys + kMoveChunk - 1) / kMoveChunk;
   const int64_t groups = std::min<int64_t>((kMoveEnough + slices - 1) / slices, chunks);
   return (int)((chunks + groups - 1) / groups) * kMoveChunk;
@@ -394,8 +402,8 @@ static hipError_t launch_paged_evict_for(PagedEvictArgs a, hipStream_t stream) {
   if (most <= a.above) return hipGetLastError();  // (no sequence is longer than its table)
   a.group_rows = paged_evict_group_rows(a.batch, a.n_kv_heads, D, a.n_keys);
   const int groups = (a.n_keys + a.group_rows - 1) / a.group_rows;
-  if (groups > 1) hipLaunchKernelGGL((paged_save_kernel<D>), dim3(units.x, D / 32, (a.n_keys + kMoveChunk - 1) / kMoveChunk), dim3(kMoveThreads), 0, stream, a);
-  const dim3 grid(units.x, D / 32 + 1, groups);
+  if (groups > 1) hipLaunchKernelGGL((paged_save_kernel<D>), dim3(units.x, 2 * D / kSlice, (a.n_keys + kMoveChunk - 1) / kMoveChunk), dim3(kMoveThreads), 0, stream, a);
+  const dim3 grid(units.x, 2 * D / kSlice + 1, groups);
   if (groups > 1) hipLaunchKernelGGL((paged_move_kernel<T, D, kMoveEach>), grid, dim3(kMoveThreads), 0, stream, a);
   else hipLaunchKernelGGL((paged_move_kernel<T, D, 2 * kMoveEach>), grid, dim3(kMoveThreads), 0, stream, a);
   return hipGetLastError();
