@@ -2,7 +2,8 @@
 //
 // Choosing: a work-group for each (sequence, KV head) finds what the wanted number of weights reaches by histograms of 256 equal ranges of the weights' order, each inside the range
 // of the last one that holds it, as pages are chosen for sparse steps, and lists the places in order by sums over the work-group.  Integers only: the order in which counts are added
-// does not matter.  Weights stay in LDS between the rounds, or are read again where there are more than it holds.
+// does not matter.  Weights stay in registers between the rounds, or are read again where there are more than these hold.  (In LDS: 33000 keys 28 us; with one copy of the bins no
+// more.)
 //
 // Moving is bound by reading and writing the rows once.  It is in place, and rows go to lower places in their order, so a work-group that takes them in turn, each chunk read by all before
 // any of it is written, needs no room beside: no later row lies where an earlier one goes.  A work-group has 32 channels of keys or values; where that makes too few
@@ -15,16 +16,16 @@
 namespace aa {
 
 constexpr int kKeepThreads = 1024, kKeepWaves = kKeepThreads / 64, kKeepStep = 4 * kKeepThreads;
-constexpr int kKeepInLds = 36864;                     // weights that LDS holds
+constexpr int kKeepItems = 9, kKeepHeld = kKeepItems * kKeepStep;  // fours of weights that a thread holds
 constexpr int kMostKeys = 1 << 20;
 
+// HELD: no sequence has more keys than a work-group holds
+template <bool HELD>
 __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedEvictArgs p) {
-  extern __shared__ __attribute__((aligned(16))) uint32_t stay[];  // the weights, or where there are too many of them, the counts
-  static_assert(kMostKeys / kKeepStep * kKeepWaves * 2 <= kKeepInLds, "the counts take less room");
   constexpr int kCopies = 8;  // of the first round's bins, for every eighth lane: most weights are of few bins, which lanes would wait for
   __shared__ __attribute__((aligned(16))) uint32_t bins[3 + kCopies][256];  // (the first round's last)
   __shared__ uint32_t ranges[2][kKeepWaves];
-  __shared__ uint64_t few_counts[kKeepInLds / kKeepStep * kKeepWaves];
+  __shared__ uint64_t counts[(HELD ? kKeepItems : kMostKeys / kKeepStep) * kKeepWaves];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / p.n_kv_heads, kvh = blockIdx.x - b * p.n_kv_heads;
@@ -35,8 +36,7 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedEvi
     for (int i = tid; i < p.n_keys; i += kKeepThreads) kept[i] = -1;
     return;
   }
-  const bool in_lds = n <= kKeepInLds;
-  uint64_t* counts = in_lds ? few_counts : reinterpret_cast<uint64_t*>(stay);
+  const bool held = HELD || n <= kKeepHeld;
   const int first = p.n_first, end = n - p.n_last;  // the candidates
   for (int i = tid; i < (3 + kCopies) * 256; i += kKeepThreads) bins[0][i] = 0u;
   // weights as numbers of the same order; 0 for what is no candidate
@@ -47,20 +47,27 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedEvi
     for (int e = 0; e < 4; ++e) x[e] = i + e >= first && i + e < end ? ordered(w[e]) : 0u;
   };
   const int items = (n + kKeepStep - 1) / kKeepStep;
+  uint32_t mine[kKeepItems][4] = {};
+  if (held) {
+#pragma unroll
+    for (int j = 0; j < kKeepItems; ++j)
+      if (kKeepStep * j + 4 * tid < n) load(kKeepStep * j + 4 * tid, mine[j]);
+  }
   auto each = [&](auto&& f) {  // f(j, numbers): item j of a thread is four keys
-#pragma nounroll
-    for (int j = 0; j < items; ++j) {
-      const int i = kKeepStep * j + 4 * tid;
-      uint32_t x[4] = {0u, 0u, 0u, 0u};
-      if (i < n) {
-        if (in_lds) {
-          const uint4 y = *reinterpret_cast<const uint4*>(stay + i);
-          x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
-        } else {
-          load(i, x);
-        }
+    if (held) {
+#pragma unroll
+      for (int j = 0; j < kKeepItems; ++j) {
+        if (j > 0 && j >= items) break;
+        f(j, mine[j]);
       }
-      f(j, x);
+    } else {
+#pragma nounroll
+      for (int j = 0; j < items; ++j) {
+        const int i = kKeepStep * j + 4 * tid;
+        uint32_t x[4] = {0u, 0u, 0u, 0u};
+        if (i < n) load(i, x);
+        f(j, x);
+      }
     }
   };
   uint32_t lo = 0xffffffffu, hi = 0u;
@@ -71,17 +78,7 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedEvi
       hi = max(hi, x[e]);
     }
   };
-  if (in_lds) {
-#pragma unroll 4
-    for (int i = 4 * tid; i < n; i += kKeepStep) {
-      uint32_t x[4];
-      load(i, x);
-      *reinterpret_cast<uint4*>(stay + i) = uint4{x[0], x[1], x[2], x[3]};
-      extend(x);
-    }
-  } else {
-    each([&](const int, const uint32_t (&x)[4]) { extend(x); });
-  }
+  each([&](const int, const uint32_t (&x)[4]) { extend(x); });
   lo = up_to(lo, 0xffffffffu, [](const uint32_t a, const uint32_t b) { return min(a, b); });
   hi = up_to(hi, 0u, [](const uint32_t a, const uint32_t b) { return max(a, b); });
   if (lane == 63) {
@@ -103,18 +100,18 @@ __global__ void __launch_bounds__(kKeepThreads) paged_keep_kernel(const PagedEvi
   for (int round = 0; wanted > 0 && lo < hi; ++round) {
     const uint32_t span = hi - lo;
     const int shift = span < 256u ? 0 : 24 - __builtin_clz(span);  // span >> shift < 256
-    uint32_t* mine = bins[round == 0 ? 3 + (lane & (kCopies - 1)) : round - 1];
+    uint32_t* own_bins = bins[round == 0 ? 3 + (lane & (kCopies - 1)) : round - 1];
     uint32_t least_ones = 0;  // (not one by one: weights that nothing has been added to are alike)
     each([&](const int, const uint32_t (&x)[4]) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t d = x[e] - lo;
         if (d == 0u) ++least_ones;
-        else if (d <= span) atomicAdd(&mine[d >> shift], 1u);
+        else if (d <= span) atomicAdd(&own_bins[d >> shift], 1u);
       }
     });
     least_ones = (uint32_t)sums_up_to((int)least_ones);
-    if (lane == 63 && least_ones > 0) atomicAdd(&mine[0], least_ones);
+    if (lane == 63 && least_ones > 0) atomicAdd(&own_bins[0], least_ones);
     __syncthreads();
     int m[4] = {0, 0, 0, 0};
     for (int c = round == 0 ? 3 : round - 1; c < (round == 0 ? 3 + kCopies : round); ++c) {
@@ -398,7 +395,8 @@ template <typename T, int D>
 static hipError_t launch_paged_evict_for(PagedEvictArgs a, hipStream_t stream) {
   const int64_t most = (int64_t)a.max_pages << a.page_log;
   const dim3 units(a.batch * a.n_kv_heads);
-  hipLaunchKernelGGL(paged_keep_kernel, units, dim3(kKeepThreads), 4 * (size_t)std::min<int64_t>(most, kKeepInLds), stream, a);
+  if (most <= kKeepHeld) hipLaunchKernelGGL(paged_keep_kernel<true>, units, dim3(kKeepThreads), 0, stream, a);
+  else hipLaunchKernelGGL(paged_keep_kernel<false>, units, dim3(kKeepThreads), 0, stream, a);
   if (most <= a.above) return hipGetLastError();  // (no sequence is longer than its table)
   a.group_rows = paged_evict_group_rows(a.batch, a.n_kv_heads, D, a.n_keys);
   const int groups = (a.n_keys + a.group_rows - 1) / a.group_rows;
