@@ -1020,7 +1020,7 @@ static int paged_decode_args(const char* who, PagedDecodeArgs& a, const aa_paged
   a = {(const uint16_t*)t->q, t->q_sb, t->q_sh, (uint16_t*)t->out, t->o_sb, t->o_sh, (const uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn,
        (const uint16_t*)cache->values, cache->vp_sp, cache->vp_sh, cache->vp_sn, t->page_table, t->pt_sb, 0, t->lengths, t->batch, t->n_q_heads,
        cache->n_kv_heads, cache->head_dim, cache->n_pages, log2_of(cache->page_size), t->max_pages, 0, t->sm_scale, nullptr, nullptr, nullptr, cache->dtype,
-       nullptr, nullptr, nullptr, 0, nullptr, nullptr, nullptr};
+       nullptr, nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr};
   return AA_OK;
 }
 
@@ -1037,14 +1037,15 @@ int aa_paged_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* t, voi
 
 // A step's scratch, the decode kernel's last
 struct WeighScratch {
-  size_t scores, totals, decode, total;
+  size_t scores, totals, cuts, decode, total;
 };
 static WeighScratch carve_weigh(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
   WeighScratch w;
   const size_t rows = (size_t)batch * n_q_heads;
   w.scores = 0;
   w.totals = align256(rows * max_pages * page_size * 4);
-  w.decode = w.totals + align256(rows * 8);
+  w.cuts = w.totals + align256(rows * 8);
+  w.decode = w.cuts + align256(rows * 8);  // (no more units than rows)
   w.total = w.decode + paged_decode_scratch(batch, n_q_heads, n_kv_heads, head_dim, log2_of(page_size), max_pages).total;
   return w;
 }
@@ -1070,6 +1071,7 @@ int aa_paged_weighing_decode_fwd(const aa_paged_cache* cache, const aa_paged_ste
   char* ws = static_cast<char*>(t->workspace);
   a.scores = (float*)(ws + w.scores);
   a.totals = (float*)(ws + w.totals);
+  a.cuts = (int32_t*)(ws + w.cuts);
   a.weights = weights;
   a.n_first = n_first;
   give_scratch(a, ws + w.decode, t->max_pages);

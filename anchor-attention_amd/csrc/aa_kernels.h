@@ -173,6 +173,7 @@ struct PagedDecodeArgs {
   // keys' weights (all or none): scores [batch, n_q_heads, max_pages * page size] and maxima and sums [batch, n_q_heads, 2], both scratch, and the weights [n_pages, n_kv_heads, page size], but
   // for the first n_first keys
   float* scores; float* totals; float* weights; int n_first;
+  int32_t* cuts;  // scratch too: [batch, units][2], the first share of a unit that several have, and how many (0: one)
   // a shared prefix (all or none): its pages [batch], its accumulators [batch, n_q_heads, head_dim] and maxima and sums [batch, n_q_heads, 2], written by launch_paged_prefix
   int32_t* skips; float* prefix; float* prefix_stats;
 };

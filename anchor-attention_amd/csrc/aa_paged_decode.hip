@@ -461,7 +461,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
           add_prefix<D, kDV>(p, f.b, head0 + min(c16, n_cols - 1), kDV * 4 * g, scale, m_run, l_run, acc);
         }
       }
-      if (MODE == kWeigh && g == 0 && c16 < n_cols) *reinterpret_cast<floatx2*>(p.totals + 2 * ((int64_t)f.b * p.n_q_heads + head0 + c16)) = floatx2{m_run, l_run};
+      if (MODE == kWeigh) {
+        if (g == 0 && c16 < n_cols) *reinterpret_cast<floatx2*>(p.totals + 2 * ((int64_t)f.b * p.n_q_heads + head0 + c16)) = floatx2{m_run, l_run};
+        if (lane == 0) *reinterpret_cast<int2*>(p.cuts + 2 * ((int64_t)f.b * units + f.unit)) = int2{0, 0};
+      }
       const float inv = none ? 0.f : 1.f / l_run;  // (no keys: 0; keys whose scores are all minus infinity: 0 / 0, as a soft-max has it)
       if (c16 < n_cols) {
         uint16_t* op = p.out + f.b * p.o_sb + (int64_t)(head0 + c16) * p.o_sh + kDV * 4 * g;
@@ -561,6 +564,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
         }
       }
     }
+    if (MODE == kWeigh && begins && tid == 0) {
+      const int kvh = head0 / group, unit = kvh * col_blocks + (head0 - kvh * group) / kCols;
+      *reinterpret_cast<int2*>(p.cuts + 2 * ((int64_t)info.y * units + unit)) = ends ? int2{0, 0} : int2{(int)blockIdx.x, info.w};
+    }
     if (begins && !ends) {  // the unit's other parts are the next work-groups'
       goes_on = true;
       if (tid == 0) *header = int4{info.w, info.y, head0, n_cols};
@@ -574,11 +581,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
 // every so many parts.  Few bytes; the launch and three loads one after the other take 3 to 5 us, which a step pays whether or not a unit was cut, since the
 // host does not know the lengths.
 template <typename T, int D, DecodeMode MODE>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArgs p) {
+__device__ __forceinline__ void combine(const PagedDecodeArgs& p, const int col, const int share) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
   __shared__ float weight[256], red[2][4];
   __shared__ floatx4 sums[kGroups][kLanes];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = blockIdx.x, share = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int4 header = *reinterpret_cast<const int4*>(p.headers + 4 * share);
   const int parts = header.x;
   if (parts == 0 || col >= header.w) return;
@@ -629,11 +636,14 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArg
       if (((const_i32*)p.skips)[header.y] > 0) add_prefix<D, 1>(p, header.y, header.z + col, 4 * tid, scale, m, l, y);
       sum = y[0];
     }
-    if (MODE == kWeigh && tid == 0) *reinterpret_cast<floatx2*>(p.totals + 2 * ((int64_t)header.y * p.n_q_heads + header.z + col)) = floatx2{m, l};
     const float inv = 1.f / l;
     uint16_t* op = p.out + header.y * p.o_sb + (int64_t)(header.z + col) * p.o_sh + 4 * tid;
     *reinterpret_cast<u32x2*>(op) = u32x2{T::pack(sum[0] * inv, sum[1] * inv), T::pack(sum[2] * inv, sum[3] * inv)};
   }
+}
+template <typename T, int D, DecodeMode MODE>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArgs p) {
+  combine<T, D, MODE>(p, blockIdx.x, blockIdx.y);
 }
 
 // Scratch of a step: a header, and two parts of 16 columns, for each share.  None where no unit is cut.
@@ -649,23 +659,73 @@ PagedScratch paged_decode_scratch(int batch, int n_q_heads, int n_kv_heads, int 
 }
 
 // Adds to each key's weight what its KV head's queries have given it: the sum over the heads of the group of 2^((score - maximum) * scale) / sum, from the scores that the
-// decode kernel has left.  Bound by reading these once.  A thread has four keys, a work-group 1024, and as many more as it takes for all of a sequence's.
-template <typename T>
-__global__ void __launch_bounds__(256) paged_weigh_kernel(const PagedDecodeArgs p) {
-  const int b = blockIdx.z, kvh = blockIdx.y, group = p.n_q_heads / p.n_kv_heads, room = p.max_pages << p.page_log, n = keys_of<kWeigh>(p, b, p.lengths[b]);
+// decode kernel has left.  Bound by reading these once.  A thread has four keys, a work-group 1024, and as many more as it takes for all of a sequence's.  The work-groups before these
+// join the parts of cut units, whose maxima and sums are therefore joined here once more, 16 heads at a time, instead of waiting for them.  (As a launch of its own after
+// the join: 16 sequences of 500 to 16000 keys, 32/8 heads of 128, 79 us a step.)
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_weigh_kernel(const PagedDecodeArgs p, const int combiners, const int cols, const int side) {
+  __shared__ floatx2 parts_of[16][kCols], totals[kCols];
+  if ((int)blockIdx.x < combiners) {
+    const int share = blockIdx.x / cols;
+    return combine<T, D, kWeigh>(p, blockIdx.x - share * cols, share);
+  }
+  const int tid = threadIdx.x, at = blockIdx.x - combiners, u = at / side, b = u / p.n_kv_heads, kvh = u - b * p.n_kv_heads;
+  const int group = p.n_q_heads / p.n_kv_heads, col_blocks = (group + kCols - 1) / kCols, room = p.max_pages << p.page_log, n = keys_of<kWeigh>(p, b, p.lengths[b]);
   const int64_t head0 = (int64_t)b * p.n_q_heads + (int64_t)kvh * group;
   const float scale = p.sm_scale * kLog2e;
-  for (int i = (blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += gridDim.x * 1024) {
+  const int first = (at - u * side) * 1024;
+  if (first >= n) return;
+  auto find_totals = [&](const int block) {  // of its heads: maxima, and what probabilities are multiplied by
+    const int2 cut = *reinterpret_cast<const int2*>(p.cuts + 2 * ((int64_t)u * col_blocks + block));
+    const int col = tid & 15, slice = tid >> 4;
+    float m = -INFINITY, l = 0.f;
+    if (cut.y == 0) {
+      if (slice == 0 && kCols * block + col < group) {
+        const floatx2 x = *reinterpret_cast<const floatx2*>(p.totals + 2 * (head0 + kCols * block + col));
+        m = x[0];
+        l = x[1];
+      }
+    } else {
+      for (int i = slice; i < cut.y; i += 16) {
+        const floatx2 x = *reinterpret_cast<const floatx2*>(p.part_stats + 2 * (((int64_t)2 * (cut.x + i) + (i == 0 ? 1 : 0)) * kCols + col));
+        const float m_new = fmaxf(m, x[0]), w = m == -INFINITY ? 0.f : fast_exp2((m - m_new) * scale), w2 = x[0] == -INFINITY ? 0.f : fast_exp2((x[0] - m_new) * scale);
+        l = w * l + w2 * x[1];
+        m = m_new;
+      }
+    }
+    parts_of[slice][col] = floatx2{m, l};
+    __syncthreads();
+    if (tid < kCols) {
+      m = -INFINITY;
+      l = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m = fmaxf(m, parts_of[i][tid][0]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) l += parts_of[i][tid][0] == -INFINITY ? 0.f : fast_exp2((parts_of[i][tid][0] - m) * scale) * parts_of[i][tid][1];
+      totals[tid] = floatx2{m, 1.f / l};  // (of none, and of scores that are all minus infinity, infinity times 0)
+    }
+    __syncthreads();
+  };
+  if (col_blocks == 1) find_totals(0);
+  for (int i0 = first; i0 < n; i0 += side * 1024) {
+    const int i = i0 + 4 * tid;
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int block = 0; block < col_blocks; ++block) {
+      if (col_blocks > 1) find_totals(block);
+      if (i >= n) continue;
+      const int heads = min(kCols, group - kCols * block);
+      const float* from = p.scores + (head0 + kCols * block) * room + i;
+#pragma unroll 4
+      for (int h = 0; h < heads; ++h) {
+        const floatx4 s = *reinterpret_cast<const floatx4*>(from + (int64_t)h * room);
+        const floatx2 total = totals[h];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += prob_exp2<T>(s[e] - total[0], scale) * total[1];
+      }
+    }
+    if (i >= n) continue;
     const int page = p.table[b * p.t_sb + (i >> p.page_log)];
     if ((uint32_t)page >= (uint32_t)p.n_pages) continue;  // (what is read in its place is another sequence's)
-    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int h = 0; h < group; ++h) {
-      const floatx4 s = *reinterpret_cast<const floatx4*>(p.scores + (head0 + h) * room + i);
-      const floatx2 total = *reinterpret_cast<const floatx2*>(p.totals + 2 * (head0 + h));
-      const float inv = 1.f / total[1];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += prob_exp2<T>(s[e] - total[0], scale) * inv;
-    }
     float* w = p.weights + (((int64_t)page * p.n_kv_heads + kvh) << p.page_log) + (i & ((1 << p.page_log) - 1));
     floatx4 old = *reinterpret_cast<const floatx4*>(w);
 #pragma unroll
@@ -683,11 +743,13 @@ static void launch_paged_decode_as(const PagedDecodeArgs& a, hipStream_t stream)
   const int64_t most = (int64_t)a.batch * units * (((int64_t)a.max_pages << a.page_log) / kTile + 1 + kOver);
   if (most < 1ll << 30) hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int, MODE>), dim3(kShares), dim3(256), lds, stream, a);
   else hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int64_t, MODE>), dim3(kShares), dim3(256), lds, stream, a);
-  if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D, MODE>), dim3(cols, kShares), dim3(256), 0, stream, a);
-  if (MODE == kWeigh) {
+  if constexpr (MODE == kWeigh) {
     // work-groups of a (sequence, KV head): as many as its table has room for, or fewer where there are thousands in all
     const int64_t all = (int64_t)a.batch * a.n_kv_heads, room = (((int64_t)a.max_pages << a.page_log) + 1023) / 1024, each = all < 8192 ? 8192 / all : 1;
-    hipLaunchKernelGGL((paged_weigh_kernel<T>), dim3((uint32_t)(room < each ? room : each), a.n_kv_heads, a.batch), dim3(256), 0, stream, a);
+    const int side = (int)(room < each ? room : each), combiners = a.headers != nullptr ? kShares * cols : 0;
+    hipLaunchKernelGGL((paged_weigh_kernel<T, D>), dim3((uint32_t)(combiners + side * all)), dim3(256), 0, stream, a, combiners, cols, side);
+  } else {
+    if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D, MODE>), dim3(cols, kShares), dim3(256), 0, stream, a);
   }
 }
 

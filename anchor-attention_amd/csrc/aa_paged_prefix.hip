@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(256) paged_prefix_join_kernel(const PagedPrefi
 // that the memory system fills, chunks swizzled.  Eight waves are two teams that take the tiles in turn and are never in the same half of a tile: while one multiplies (the last tile's
 // probabilities with its values, the next one's keys with the queries), the other forms probabilities, a barrier between the halves, so that the matrix pipe has one team's work at a time and
 // the vector ALU the other's.  Tiles are requested one tile ahead.
-constexpr int kWideTile = 64, kWideRows = 128, kWideThreads = 512, kWideLeast = 4, kWideOver = 5;
+constexpr int kWideTile = 64, kWideRows = 128, kWideThreads = 512, kWideLeast = 4, kWideOver = 10;
 
 template <int D>
 __device__ __forceinline__ int wide_k_swizzle(const int r) { return D == 128 ? r & 15 : (r & 7) ^ ((r >> 3) & 1); }
