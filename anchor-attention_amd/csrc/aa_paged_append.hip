@@ -27,20 +27,10 @@ __device__ __forceinline__ void store8(uint16_t* p, const int half, const Rows8&
 struct Angles {
   float4 cos[2], sin[2];
 };
-// A norm's weights of these channels, and the norm: x * w / sqrt(mean of the head's x^2 + eps), float32.  A head is D / 16 neighbouring lanes', all of them active.
-struct Norm8 {
-  float first[8], second[8];
-};
-template <typename T>
-__device__ __forceinline__ Norm8 norm_of(const uint16_t* weight, const int c, const int half) {
-  const Rows8 raw = load8(weight + 8 * c, half);
-  Norm8 w;
-  unpack8<T>(raw.first, w.first);
-  unpack8<T>(raw.second, w.second);
-  return w;
-}
-template <int PIECES>
-__device__ __forceinline__ void normalise(float (&x)[8], float (&y)[8], const Norm8& w, const float eps) {
+// A norm: x * w / sqrt(mean of the head's x^2 + eps), float32.  A head is D / 16 neighbouring lanes', all of them active.  Its weights stay as they lie in memory: unpacked, they would
+// leave three waves to a SIMD instead of four.
+template <typename T, int PIECES>
+__device__ __forceinline__ void normalise(float (&x)[8], float (&y)[8], const Rows8& weight, const float eps) {
   float sum = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) sum += x[j] * x[j] + y[j] * y[j];
@@ -48,20 +38,22 @@ __device__ __forceinline__ void normalise(float (&x)[8], float (&y)[8], const No
   sum += __uint_as_float(dpp<kDppXor2>(__float_as_uint(sum)));
   if (PIECES == 8) sum += __uint_as_float(dpp<kDppHalfMirror>(__float_as_uint(sum)));  // (the four lanes of either half have the same sum)
   const float scale = rsqrtf(sum * (1.f / (16 * PIECES)) + eps);
+  float w[8];
+  unpack8<T>(weight.first, w);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    x[j] *= scale * w.first[j];
-    y[j] *= scale * w.second[j];
-  }
+  for (int j = 0; j < 8; ++j) x[j] *= scale * w[j];
+  unpack8<T>(weight.second, w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] *= scale * w[j];
 }
 
 // turned by their angles, after a norm if there is one: float32, one rounding
 template <typename T, int PIECES>
-__device__ __forceinline__ Rows8 rotated(const Rows8& raw, const Angles& a, const Norm8* norm = nullptr, const float eps = 0.f) {
+__device__ __forceinline__ Rows8 rotated(const Rows8& raw, const Angles& a, const Rows8* norm = nullptr, const float eps = 0.f) {
   float x[8], y[8];
   unpack8<T>(raw.first, x);
   unpack8<T>(raw.second, y);
-  if (norm != nullptr) normalise<PIECES>(x, y, *norm, eps);
+  if (norm != nullptr) normalise<T, PIECES>(x, y, *norm, eps);
   const float c[8] = {a.cos[0].x, a.cos[0].y, a.cos[0].z, a.cos[0].w, a.cos[1].x, a.cos[1].y, a.cos[1].z, a.cos[1].w};
   const float s[8] = {a.sin[0].x, a.sin[0].y, a.sin[0].z, a.sin[0].w, a.sin[1].x, a.sin[1].y, a.sin[1].z, a.sin[1].w};
 #pragma unroll
@@ -193,8 +185,8 @@ __device__ __forceinline__ void queries_and_values(const PagedAppendArgs& p, con
   if (group > 0) {
     const Angles a = angles_of(p, x.position + x.shift, c);
     const bool normed = MORE && p.q_norm != nullptr;
-    Norm8 norm;
-    if (normed) norm = norm_of<T>(p.q_norm, c, D / 2);
+    Rows8 norm;
+    if (normed) norm = load8(p.q_norm + 8 * c, D / 2);
     for (int h = 0; h < group; h += 4) {
       Rows8 q[4];
       const uint16_t* src = p.q + t * p.q_st + (int64_t)(kvh * group + h) * p.q_sh + 8 * c;
@@ -220,8 +212,8 @@ __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), page_size = 1 << p.page_log;
   const const_i32 *lengths = (const_i32*)p.lengths, *starts = (const_i32*)p.starts, *table = (const_i32*)p.table;
   const bool normed = MORE && p.k_norm != nullptr;
-  Norm8 norm;
-  if (normed) norm = norm_of<T>(p.k_norm, c, D / 2);
+  Rows8 norm;
+  if (normed) norm = load8(p.k_norm + 8 * c, D / 2);
 
   for (int t = first; t < min(first + p.chunk, p.n_tokens);) {
     int b = t, begin = t, end = t + 1;
@@ -244,7 +236,7 @@ __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const 
     uint16_t* bounds = p.bounds + ((int64_t)x.at * p.n_kv_heads + kvh) * 2 * D + 8 * c;
     Rows8 old[2];
     const bool writes = p.bounds != nullptr && row == 0;  // the bounds, at the end
-    if (writes && x.slot != 0) {
+    if (!MORE && writes && x.slot != 0) {  // (with a norm they would take the registers of a fourth wave)
       old[0] = load8(bounds, D / 2);
       old[1] = load8(bounds + D, D / 2);
     }
@@ -296,6 +288,10 @@ __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const 
     }
     if (writes) {
       if (x.slot != 0) {
+        if (MORE) {
+          old[0] = load8(bounds, D / 2);
+          old[1] = load8(bounds + D, D / 2);
+        }
         uint32_t low[8], high[8];
         words(old[0], low);
         words(old[1], high);
@@ -314,7 +310,7 @@ __device__ __forceinline__ void keys_and_bounds(const PagedAppendArgs& p, const 
 // prompt of 2000 took 20.3 us in plain order, 15.8 so, 18.3 with the KV heads' work-groups spread over the XCDs.
 constexpr uint32_t kXcds = 8;
 template <typename T, int D, int WAVES, bool MORE>
-__global__ void __launch_bounds__(64 * WAVES) paged_append_kernel(const PagedAppendArgs p) {
+__global__ void __launch_bounds__(64 * WAVES, MORE ? 4 : 1) paged_append_kernel(const PagedAppendArgs p) {
   __shared__ uint32_t red[WAVES > 1 ? WAVES - 1 : 1][D / 16][16];
   const uint32_t xcd = blockIdx.x % kXcds, of_xcd = blockIdx.x / kXcds, turn = of_xcd / p.n_kv_heads;
   const int kvh = of_xcd - turn * p.n_kv_heads, at = turn * kXcds + (xcd + (turn * 0x9e3779b1u >> 29)) % kXcds;
