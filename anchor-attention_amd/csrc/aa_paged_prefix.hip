@@ -22,13 +22,19 @@ constexpr int kPrefixLeast = 8, kPrefixOver = 4;  // tiles of a share at least; 
 struct PagedGroup {
   int first, sequences, pages;
 };
-__device__ __forceinline__ PagedGroup group_at(const PagedPrefixArgs& p, const int g) {
+template <typename Words>
+__device__ __forceinline__ PagedGroup group_of(const PagedPrefixArgs& p, const Words* groups, const Words* shared_pages, const int g) {
   PagedGroup x;
-  if (p.groups == nullptr) return {0, p.step.batch, min(max(p.shared_pages[0], 0), p.step.max_pages)};
-  x.first = min(max(p.groups[g], 0), p.step.batch);
-  x.sequences = max(min(max(p.groups[g + 1], 0), p.step.batch) - x.first, 0);
-  x.pages = min(max(p.shared_pages[g], 0), p.step.max_pages);
+  if (p.groups == nullptr) return {0, p.step.batch, min(max(shared_pages[0], 0), p.step.max_pages)};
+  x.first = min(max(groups[g], 0), p.step.batch);
+  x.sequences = max(min(max(groups[g + 1], 0), p.step.batch) - x.first, 0);
+  x.pages = min(max(shared_pages[g], 0), p.step.max_pages);
   return x;
+}
+// of a lane's group, and of one that all lanes have (by scalar loads, which are there sooner)
+__device__ __forceinline__ PagedGroup group_at(const PagedPrefixArgs& p, const int g) { return group_of(p, p.groups, p.shared_pages, g); }
+__device__ __forceinline__ PagedGroup common_group_at(const PagedPrefixArgs& p, const int g) {
+  return group_of(p, (const_i32*)p.groups, (const_i32*)p.shared_pages, __builtin_amdgcn_readfirstlane(g));
 }
 
 // How many of a sequence's first pages its group's state stands for: those that are shared, if it is as long, or none.
@@ -75,11 +81,9 @@ template <int TILE, int ROWS, int OVER>
 __device__ __forceinline__ PrefixShare share_of(const PagedPrefixArgs& all, const int share, const int least) {
   const PagedDecodeArgs& p = all.step;
   const int lane = threadIdx.x & 63, heads = p.n_q_heads / p.n_kv_heads;
-  auto extents_of = [&](const int i) {  // of group i's units
-    if (i >= all.n_groups) return (int64_t)0;
-    const PagedGroup x = group_at(all, i);
-    return (int64_t)extent_of<OVER>(tiles_of<TILE>(p, x)) * blocks_of<ROWS>(x, heads) * p.n_kv_heads;
-  };
+  auto extents_in = [&](const PagedGroup& x) { return (int64_t)extent_of<OVER>(tiles_of<TILE>(p, x)) * blocks_of<ROWS>(x, heads) * p.n_kv_heads; };
+  auto extents_of = [&](const int i) { return i < all.n_groups ? extents_in(group_at(all, i)) : (int64_t)0; };  // of group i's units
+
   auto up_to_lane = [&](int64_t x) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -90,7 +94,7 @@ __device__ __forceinline__ PrefixShare share_of(const PagedPrefixArgs& all, cons
   };
   PrefixShare r = {0, 0, 0, 0, 0};
   int64_t total = 0;
-  if (all.n_groups == 1) total = extents_of(0);
+  if (all.n_groups == 1) total = extents_in(common_group_at(all, 0));
   else
     for (int i = 0; i < all.n_groups; i += 64) total += __shfl((long long)up_to_lane(extents_of(i + lane)), 63, 64);
   r.share = max((total + (kPrefixShares - 1)) >> kPrefixSharesLog, (int64_t)least);
@@ -140,10 +144,7 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
     uint32_t v[8][kVW];
   };
   while (at < end && group < all.n_groups) {
-    PagedGroup x = group_at(all, group);
-    x.first = __builtin_amdgcn_readfirstlane(x.first);
-    x.sequences = __builtin_amdgcn_readfirstlane(x.sequences);
-    x.pages = __builtin_amdgcn_readfirstlane(x.pages);
+    const PagedGroup x = common_group_at(all, group);
     const int tiles = tiles_of<kPrefixTile>(p, x), blocks = blocks_of<kRows>(x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
     const int extent = extent_of<kPrefixOver>(tiles);
     if (at - start >= (int64_t)extent * blocks * p.n_kv_heads) {  // (the next group, perhaps of nothing)
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(256) paged_prefix_join_kernel(const PagedPrefi
   const int4 header = *reinterpret_cast<const int4*>(all.headers + 4 * share);
   const int parts = header.x, heads = p.n_q_heads / p.n_kv_heads;
   if (parts == 0) return;
-  const PagedGroup x = group_at(all, header.y);
+  const PagedGroup x = common_group_at(all, header.y);
   const int row = header.w * kRows + r;
   if (row >= x.sequences * heads) return;
   const float scale = p.sm_scale * kLog2e;
@@ -493,10 +494,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
   const uint32_t v_rd = my_tiles + 2 * kTileBytes + r0 * kRowBytes + ((y0 ^ wide_v_swizzle<D>(r0)) << 4) + 8 * (lane & 1);
 
   while (at < end && group < all.n_groups) {
-    PagedGroup x = group_at(all, group);
-    x.first = __builtin_amdgcn_readfirstlane(x.first);
-    x.sequences = __builtin_amdgcn_readfirstlane(x.sequences);
-    x.pages = __builtin_amdgcn_readfirstlane(x.pages);
+    const PagedGroup x = common_group_at(all, group);
     const int n_tiles = tiles_of<kWideTile>(p, x), blocks = blocks_of<kWideRows>(x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
     const int extent = extent_of<kWideOver>(n_tiles);
     if (at - start >= (int64_t)extent * blocks * p.n_kv_heads) {  // (the next group, perhaps of nothing)
@@ -538,6 +536,9 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
     };
+    // A probability is one 16-bit number, relative to a maximum that may be 2^kRoom below the row's: as precise above 1 as below.  fp16 forms 2^kProbLog2 of it, so that the largest fits and
+    // what falls below its smallest number, 2^-33 of the maximum, is 2^-13 of the sum for a million keys.
+    constexpr float kRoom = 6.f, kProbLog2 = T::kProbLog2 != 0.f ? 9.f : 0.f;
     // (the sums of the probabilities as they were rounded, by products with ones: each of the sixteen is a row's)
     float m_run = -INFINITY;
     floatx16 acc[kDB], s[2], sums;
@@ -581,12 +582,29 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         for (int r = 0; r < 32; ++r)
           if (key0 + 32 * (r >> 4) + 16 * ((r & 15) >> 3) >= length) s[r >> 4][r & 15] = -INFINITY;
       }
-      float mx = s[0][0];
+      // 2^(s * scale - m * scale) with the maximum so far, m, before this tile's is known: only where that is larger by 2^kRoom it is taken up, and they are formed again
+      auto form = [&](const float bias) __attribute__((always_inline)) {
 #pragma unroll
-      for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
-      const float m_new = fmaxf(m_run, max_with_other_half(mx));
-      const float m_base = m_new == -INFINITY ? 0.f : m_new;  // (no key of this row's so far)
-      if (__any(m_new > m_run)) {
+        for (int w = 0; w < 16; ++w) {
+          // (the fused product's second term is the same for all keys, so that its rounding cancels in the quotient)
+          const float e0 = fast_exp2(__builtin_fmaf(s[w >> 3][2 * (w & 7)], scale, bias)), e1 = fast_exp2(__builtin_fmaf(s[w >> 3][2 * (w & 7) + 1], scale, bias));
+          uint32_t both = T::pack(e0, e1);
+          if constexpr (decltype(exact)::value) {
+            if (e0 > 0.f && (both & 0xffffu) == 0u) both |= 1u;
+            if (e1 > 0.f && (both >> 16) == 0u) both |= 0x10000u;
+          }
+          prob[w >> 2][w & 3] = both;
+        }
+      };
+      const float bias = kProbLog2 - (m_run == -INFINITY ? 0.f : m_run) * scale;
+      form(bias);
+      float mx[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+#pragma unroll
+      for (int r = 4; r < 32; ++r) mx[r & 3] = fmaxf(mx[r & 3], s[r >> 4][r & 15]);
+      const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      if (__builtin_expect(__any(m_run == -INFINITY || __builtin_fmaf(m_tile, scale, bias) > kProbLog2 + kRoom), 0)) {
+        const float m_new = fmaxf(m_run, max_with_other_half(m_tile));
+        const float m_base = m_new == -INFINITY ? 0.f : m_new;  // (no key of this row's so far)
         const float alpha = fast_exp2((m_run - m_base) * scale);
 #pragma unroll
         for (int r = 0; r < 16; ++r) sums[r] *= alpha;
@@ -595,18 +613,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
         m_run = m_new;
-      }
-      // 2^(s * scale - m * scale): the fused product's second term is the same for all keys, so that its rounding cancels in the quotient
-      const float bias = T::kProbLog2 - m_base * scale;
-#pragma unroll
-      for (int w = 0; w < 16; ++w) {
-        const float e0 = fast_exp2(__builtin_fmaf(s[w >> 3][2 * (w & 7)], scale, bias)), e1 = fast_exp2(__builtin_fmaf(s[w >> 3][2 * (w & 7) + 1], scale, bias));
-        uint32_t both = T::pack(e0, e1);
-        if constexpr (decltype(exact)::value) {
-          if (e0 > 0.f && (both & 0xffffu) == 0u) both |= 1u;
-          if (e1 > 0.f && (both >> 16) == 0u) both |= 0x10000u;
-        }
-        prob[w >> 2][w & 3] = both;
+        form(kProbLog2 - m_base * scale);
       }
     };
     auto run = [&](auto exact) __attribute__((always_inline)) {
@@ -702,7 +709,9 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     };
     auto finish = [&](auto first) __attribute__((always_inline)) {
       const floatx2 other = stats[(1 - team) * 64 + lane];
-      const float m = fmaxf(m_run, other[0]), w = m_run == -INFINITY ? 0.f : fast_exp2((m_run - m) * scale), w2 = other[0] == -INFINITY ? 0.f : fast_exp2((other[0] - m) * scale);
+      constexpr float kBack = T::kProbLog2 - kProbLog2;  // (the decode kernel's factor)
+      const float m = fmaxf(m_run, other[0]), w = m_run == -INFINITY ? 0.f : fast_exp2((m_run - m) * scale + kBack);
+      const float w2 = other[0] == -INFINITY ? 0.f : fast_exp2((other[0] - m) * scale + kBack);
       const float l = w * l_run + w2 * other[1];
 #pragma unroll
       for (int g = 0; g < kFours / 2; ++g) {
@@ -744,7 +753,7 @@ __global__ void __launch_bounds__(512) paged_prefix_wide_join_kernel(const Paged
   const int4 header = *reinterpret_cast<const int4*>(all.headers + 4 * share);
   const int parts = header.x, heads = p.n_q_heads / p.n_kv_heads;
   if (parts == 0) return;
-  const PagedGroup x = group_at(all, header.y);
+  const PagedGroup x = common_group_at(all, header.y);
   const int row = header.w * kWideRows + 32 * wave + (lane & 31);
   const float scale = p.sm_scale * kLog2e;
   // the first part is the second of its share, the others the first of theirs
