@@ -106,6 +106,31 @@ __device__ __forceinline__ void add_prefix(const PagedDecodeArgs& p, const int b
   }
 }
 
+// What some heads of a group (from head0 on in all of the batch's) give four keys from i on: the sum of 2^((score - maximum) * scale) / sum; total(h): a head's maximum and 1 / sum.
+template <typename T, typename F>
+__device__ __forceinline__ void add_probabilities(const PagedDecodeArgs& p, const int64_t head0, const int heads, const int i, const float scale, floatx4& sum, F total) {
+  const int64_t room = p.max_pages << p.page_log;
+  const float* from = p.scores + head0 * room + i;
+#pragma unroll 4
+  for (int h = 0; h < heads; ++h) {
+    const floatx4 s = *reinterpret_cast<const floatx4*>(from + h * room);
+    const floatx2 t = total(h);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += prob_exp2<T>(s[e] - t[0], scale) * t[1];
+  }
+}
+// ... and into the weights of the first n keys
+__device__ __forceinline__ void add_to_weights(const PagedDecodeArgs& p, const int b, const int kvh, const int i, const int n, const floatx4 sum) {
+  const int page = p.table[b * p.t_sb + (i >> p.page_log)];
+  if ((uint32_t)page >= (uint32_t)p.n_pages) return;  // (what is read in its place is another sequence's)
+  float* w = p.weights + (((int64_t)page * p.n_kv_heads + kvh) << p.page_log) + (i & ((1 << p.page_log) - 1));
+  floatx4 old = *reinterpret_cast<const floatx4*>(w);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (i + e < n && i + e >= p.n_first) old[e] += sum[e];
+  *reinterpret_cast<floatx4*>(w) = old;
+}
+
 template <typename T, int D, int WAVES, typename Place, DecodeMode MODE>
 __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const PagedDecodeArgs p) {
   constexpr int kKS = D / 32;      // MFMAs of a score
@@ -115,12 +140,15 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
   // States of units that a wave has a part of only: [wave][0: the first of its units, which began before; 1: its last, which goes on][column]
   extern __shared__ __attribute__((aligned(16))) float states[];
   __shared__ float stats[WAVES][2][2][kCols];
+  __shared__ floatx2 unit_totals[MODE == kWeigh ? kCols : 1];
   __shared__ int4 parts_of[WAVES][2];  // 0 if there is none, 2 if the unit ends in it; sequence; first head, and columns in the upper half; parts of work-groups
 
   const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = p.n_q_heads / p.n_kv_heads, col_blocks = (group + kCols - 1) / kCols, units = p.n_kv_heads * col_blocks;
   const int most_cols = min(group, kCols);
+  // whether a unit's keys get their weights here: where it is one work-group's, and all of its KV head's
+  const bool weighs = MODE == kWeigh && p.headers == nullptr && col_blocks == 1;
 
   // ---- this wave's share -------------------------------------------------------------------------
   // All units one after the other, each as long as its tiles and kOver.  A lane has kPerLane sequences in a row, a scan 64 lanes' (whose numbers stay if
@@ -461,11 +489,21 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
           add_prefix<D, kDV>(p, f.b, head0 + min(c16, n_cols - 1), kDV * 4 * g, scale, m_run, l_run, acc);
         }
       }
-      if (MODE == kWeigh) {
+      if (MODE == kWeigh && !weighs) {
         if (g == 0 && c16 < n_cols) *reinterpret_cast<floatx2*>(p.totals + 2 * ((int64_t)f.b * p.n_q_heads + head0 + c16)) = floatx2{m_run, l_run};
         if (lane == 0) *reinterpret_cast<int2*>(p.cuts + 2 * ((int64_t)f.b * units + f.unit)) = int2{0, 0};
       }
       const float inv = none ? 0.f : 1.f / l_run;  // (no keys: 0; keys whose scores are all minus infinity: 0 / 0, as a soft-max has it)
+      if (MODE == kWeigh && weighs) {  // (this wave's own scores, which it has stored)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        for (int i = 4 * lane; i < length; i += 256) {
+          floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+          add_probabilities<T>(p, (int64_t)f.b * p.n_q_heads + head0, n_cols, i, scale, sum, [&](const int h) {
+            return floatx2{__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m_run), h)), 1.f / __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l_run), h))};
+          });
+          add_to_weights(p, f.b, u.kvh, i, length, sum);
+        }
+      }
       if (c16 < n_cols) {
         uint16_t* op = p.out + f.b * p.o_sb + (int64_t)(head0 + c16) * p.o_sh + kDV * 4 * g;
 #pragma unroll
@@ -551,7 +589,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
           if (((const_i32*)p.skips)[info.y] > 0) add_prefix<D, 1>(p, info.y, head0 + col, d, scale, m, l, y);
           x = y[0];
         }
-        if (MODE == kWeigh && d == 0) *reinterpret_cast<floatx2*>(p.totals + 2 * ((int64_t)info.y * p.n_q_heads + head0 + col)) = floatx2{m, l};
+        if (MODE == kWeigh && d == 0) {
+          if (weighs) unit_totals[col] = floatx2{m, 1.f / l};
+          else *reinterpret_cast<floatx2*>(p.totals + 2 * ((int64_t)info.y * p.n_q_heads + head0 + col)) = floatx2{m, l};
+        }
         const float inv = 1.f / l;  // (a unit that is cut has keys)
         uint16_t* op = p.out + info.y * p.o_sb + (int64_t)(head0 + col) * p.o_sh + d;
         *reinterpret_cast<u32x2*>(op) = u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
@@ -564,7 +605,16 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
         }
       }
     }
-    if (MODE == kWeigh && begins && tid == 0) {
+    if (MODE == kWeigh && weighs) {
+      __syncthreads();  // (all waves have stored their scores before the parts were joined)
+      const int n = keys_of<MODE>(p, info.y, ((const_i32*)p.lengths)[info.y]);
+      for (int i = 4 * tid; i < n; i += 256 * WAVES) {
+        floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+        add_probabilities<T>(p, (int64_t)info.y * p.n_q_heads + head0, n_cols, i, scale, sum, [&](const int h) { return unit_totals[h]; });
+        add_to_weights(p, info.y, head0 / group, i, n, sum);
+      }
+      __syncthreads();  // (before the next unit's totals)
+    } else if (MODE == kWeigh && begins && tid == 0) {
       const int kvh = head0 / group, unit = kvh * col_blocks + (head0 - kvh * group) / kCols;
       *reinterpret_cast<int2*>(p.cuts + 2 * ((int64_t)info.y * units + unit)) = ends ? int2{0, 0} : int2{(int)blockIdx.x, info.w};
     }
@@ -670,7 +720,7 @@ __global__ void __launch_bounds__(256) paged_weigh_kernel(const PagedDecodeArgs 
     return combine<T, D, kWeigh>(p, blockIdx.x - share * cols, share);
   }
   const int tid = threadIdx.x, at = blockIdx.x - combiners, u = at / side, b = u / p.n_kv_heads, kvh = u - b * p.n_kv_heads;
-  const int group = p.n_q_heads / p.n_kv_heads, col_blocks = (group + kCols - 1) / kCols, room = p.max_pages << p.page_log, n = keys_of<kWeigh>(p, b, p.lengths[b]);
+  const int group = p.n_q_heads / p.n_kv_heads, col_blocks = (group + kCols - 1) / kCols, n = keys_of<kWeigh>(p, b, p.lengths[b]);
   const int64_t head0 = (int64_t)b * p.n_q_heads + (int64_t)kvh * group;
   const float scale = p.sm_scale * kLog2e;
   const int first = (at - u * side) * 1024;
@@ -713,25 +763,9 @@ __global__ void __launch_bounds__(256) paged_weigh_kernel(const PagedDecodeArgs 
     for (int block = 0; block < col_blocks; ++block) {
       if (col_blocks > 1) find_totals(block);
       if (i >= n) continue;
-      const int heads = min(kCols, group - kCols * block);
-      const float* from = p.scores + (head0 + kCols * block) * room + i;
-#pragma unroll 4
-      for (int h = 0; h < heads; ++h) {
-        const floatx4 s = *reinterpret_cast<const floatx4*>(from + (int64_t)h * room);
-        const floatx2 total = totals[h];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += prob_exp2<T>(s[e] - total[0], scale) * total[1];
-      }
+      add_probabilities<T>(p, head0 + kCols * block, min(kCols, group - kCols * block), i, scale, sum, [&](const int h) { return totals[h]; });
     }
-    if (i >= n) continue;
-    const int page = p.table[b * p.t_sb + (i >> p.page_log)];
-    if ((uint32_t)page >= (uint32_t)p.n_pages) continue;  // (what is read in its place is another sequence's)
-    float* w = p.weights + (((int64_t)page * p.n_kv_heads + kvh) << p.page_log) + (i & ((1 << p.page_log) - 1));
-    floatx4 old = *reinterpret_cast<const floatx4*>(w);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (i + e < n && i + e >= p.n_first) old[e] += sum[e];
-    *reinterpret_cast<floatx4*>(w) = old;
+    if (i < n) add_to_weights(p, b, kvh, i, n, sum);
   }
 }
 
@@ -744,6 +778,7 @@ static void launch_paged_decode_as(const PagedDecodeArgs& a, hipStream_t stream)
   if (most < 1ll << 30) hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int, MODE>), dim3(kShares), dim3(256), lds, stream, a);
   else hipLaunchKernelGGL((paged_decode_kernel<T, D, 4, int64_t, MODE>), dim3(kShares), dim3(256), lds, stream, a);
   if constexpr (MODE == kWeigh) {
+    if (a.headers == nullptr && group <= kCols) return;  // (the decode kernel has done it: 600 keys, 14/2 heads of 64, 14.5 -> 12 us)
     // work-groups of a (sequence, KV head): as many as its table has room for, or fewer where there are thousands in all
     const int64_t all = (int64_t)a.batch * a.n_kv_heads, room = (((int64_t)a.max_pages << a.page_log) + 1023) / 1024, each = all < 8192 ? 8192 / all : 1;
     const int side = (int)(room < each ? room : each), combiners = a.headers != nullptr ? kShares * cols : 0;
