@@ -1020,7 +1020,7 @@ static int paged_decode_args(const char* who, PagedDecodeArgs& a, const aa_paged
   a = {(const uint16_t*)t->q, t->q_sb, t->q_sh, (uint16_t*)t->out, t->o_sb, t->o_sh, (const uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn,
        (const uint16_t*)cache->values, cache->vp_sp, cache->vp_sh, cache->vp_sn, t->page_table, t->pt_sb, 0, t->lengths, t->batch, t->n_q_heads,
        cache->n_kv_heads, cache->head_dim, cache->n_pages, log2_of(cache->page_size), t->max_pages, 0, t->sm_scale, nullptr, nullptr, nullptr, cache->dtype,
-       nullptr, nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr};
+       nullptr, nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, nullptr, nullptr};
   return AA_OK;
 }
 
@@ -1079,15 +1079,20 @@ int aa_paged_weighing_decode_fwd(const aa_paged_cache* cache, const aa_paged_ste
 }
 
 struct SharedScratch {
-  size_t skips, prefix, stats, parts, decode, total;
+  size_t skips, firsts, entries, cuts, prefix, stats, own, own_stats, parts, decode, total;
 };
 static SharedScratch carve_shared(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_groups) {
   SharedScratch w;
   const size_t rows = (size_t)batch * n_q_heads;
   w.skips = 0;
-  w.prefix = align256((size_t)batch * 4);
+  w.firsts = align256((size_t)batch * 4);
+  w.entries = w.firsts + align256((size_t)batch * 4);
+  w.cuts = w.entries + align256(rows * 8);
+  w.prefix = w.cuts + align256(rows * 8);  // (no more units than rows)
   w.stats = w.prefix + align256(rows * head_dim * 4);
-  w.parts = w.stats + align256(rows * 8);
+  w.own = w.stats + align256(rows * 8);
+  w.own_stats = w.own + align256(rows * head_dim * 4);
+  w.parts = w.own_stats + align256(rows * 8);
   w.decode = w.parts + align256(paged_prefix_scratch(batch, n_q_heads, n_kv_heads, head_dim, n_groups).total);
   w.total = w.decode + paged_decode_scratch(batch, n_q_heads, n_kv_heads, head_dim, log2_of(page_size), max_pages).total;
   return w;
@@ -1113,12 +1118,23 @@ int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step*
   const SharedScratch w = carve_shared(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages, n_groups);
   if ((rc = paged_decode_args(who, a, cache, t, w.total))) return rc;
   char* ws = static_cast<char*>(t->workspace);
+  if (!paged_prefix_pays(a.batch, a.n_kv_heads, a.head_dim, cache->page_size, t->max_pages)) {
+    give_scratch(a, ws + w.decode, t->max_pages);
+    return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
+  }
   a.skips = (int32_t*)(ws + w.skips);
+  a.firsts = (int32_t*)(ws + w.firsts);
+  a.entries = (int32_t*)(ws + w.entries);
+  a.cuts = (int32_t*)(ws + w.cuts);
   a.prefix = (float*)(ws + w.prefix);
   a.prefix_stats = (float*)(ws + w.stats);
+  a.own = (float*)(ws + w.own);
+  a.own_stats = (float*)(ws + w.own_stats);
   const PagedScratch s = paged_prefix_scratch(a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim, n_groups);
-  char* parts = ws + w.parts;
-  const PagedPrefixArgs x = {a, shared_pages, groups, n_groups, (int32_t*)(parts + s.headers), (float*)(parts + s.stats), (float*)(parts + s.parts)};
+  a.prefix_part_stats = (float*)(ws + w.parts + s.stats);
+  a.prefix_parts = (float*)(ws + w.parts + s.parts);
+  a.prefix_rows = paged_prefix_part_rows(a.batch, a.n_q_heads, a.n_kv_heads, n_groups);
+  const PagedPrefixArgs x = {a, shared_pages, groups, n_groups};
   if ((rc = check_launch(launch_paged_prefix(x, (hipStream_t)stream), who))) return rc;
   give_scratch(a, ws + w.decode, t->max_pages);
   return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);

@@ -59,7 +59,7 @@ struct PagedPlace {       // of a tile, among all
   Place start;            // the unit's beginning
 };
 
-// kWeigh: the scores and each head's maximum and sum are kept for paged_weigh_kernel; kShared: the first pages of a sequence have been read for its group, whose states are there
+// kWeigh: the scores and each head's maximum and sum are kept for paged_weigh_kernel; kShared: the first pages of a sequence have been read for its group, whose states paged_finish_kernel joins with those of the own keys
 enum DecodeMode { kPlain, kWeigh, kShared };
 
 // keys that are read of sequence b
@@ -79,31 +79,6 @@ __device__ __forceinline__ uint32_t small_quotient(const uint32_t n, const uint3
   if (q * d > n) --q;
   else if (n - q * d >= d) ++q;
   return q;
-}
-
-// What is known of a head over its group's prefix, joined to a part of four channels, or of all that a lane has (x[j][r] channel N * r + j from d on)
-template <int D, int N>
-__device__ __forceinline__ void add_prefix(const PagedDecodeArgs& p, const int b, const int head, const int d, const float scale, float& m, float& l, floatx4 (&x)[N]) {
-  const int64_t row = (int64_t)b * p.n_q_heads + head;
-  const float m0 = p.prefix_stats[2 * row], l0 = p.prefix_stats[2 * row + 1], m1 = fmaxf(m, m0);
-  const float w = m == -INFINITY ? 0.f : fast_exp2((m - m1) * scale), w0 = m0 == -INFINITY ? 0.f : fast_exp2((m0 - m1) * scale);
-  m = m1;
-  l = w * l + w0 * l0;
-  const float* from = p.prefix + row * D + d;
-  if constexpr (N == 1) {
-    const floatx4 y = *reinterpret_cast<const floatx4*>(from);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[0][e] = w * x[0][e] + w0 * y[e];
-  } else {
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int j = 0; j < N; j += 4) {
-        const floatx4 y = *reinterpret_cast<const floatx4*>(from + N * r + j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[j + e][r] = w * x[j + e][r] + w0 * y[e];
-      }
-  }
 }
 
 // What some heads of a group (from head0 on in all of the batch's) give four keys from i on: the sum of 2^((score - maximum) * scale) / sum; total(h): a head's maximum and 1 / sum.
@@ -482,18 +457,25 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
 
     const bool from_start = f.tile == 0, to_end = last == f.n_tiles;
     if (from_start && to_end) {
-      bool none = length == 0;
-      if constexpr (MODE == kShared) {
-        if (((const_i32*)p.skips)[f.b] > 0) {
-          none = false;
-          add_prefix<D, kDV>(p, f.b, head0 + min(c16, n_cols - 1), kDV * 4 * g, scale, m_run, l_run, acc);
-        }
-      }
       if (MODE == kWeigh && !weighs) {
         if (g == 0 && c16 < n_cols) *reinterpret_cast<floatx2*>(p.totals + 2 * ((int64_t)f.b * p.n_q_heads + head0 + c16)) = floatx2{m_run, l_run};
         if (lane == 0) *reinterpret_cast<int2*>(p.cuts + 2 * ((int64_t)f.b * units + f.unit)) = int2{0, 0};
       }
-      const float inv = none ? 0.f : 1.f / l_run;  // (no keys: 0; keys whose scores are all minus infinity: 0 / 0, as a soft-max has it)
+      bool joins = false;  // (with the state of the prefix, by paged_finish_kernel)
+      if constexpr (MODE == kShared) {
+        joins = ((const_i32*)p.skips)[f.b] > 0;
+        if (lane == 0) *reinterpret_cast<int2*>(p.cuts + 2 * ((int64_t)f.b * units + f.unit)) = int2{0, 0};
+        if (joins && c16 < n_cols) {
+          const int64_t row = (int64_t)f.b * p.n_q_heads + head0 + c16;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < kDV; j += 4)
+              *reinterpret_cast<floatx4*>(p.own + row * D + kDV * (4 * g + r) + j) = floatx4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
+          if (g == 0) *reinterpret_cast<floatx2*>(p.own_stats + 2 * row) = floatx2{m_run, l_run};
+        }
+      }
+      const float inv = length == 0 ? 0.f : 1.f / l_run;  // (no keys: 0; keys whose scores are all minus infinity: 0 / 0, as a soft-max has it)
       if (MODE == kWeigh && weighs) {  // (this wave's own scores, which it has stored)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         for (int i = 4 * lane; i < length; i += 256) {
@@ -504,7 +486,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
           add_to_weights(p, f.b, u.kvh, i, length, sum);
         }
       }
-      if (c16 < n_cols) {
+      if (c16 < n_cols && !joins) {
         uint16_t* op = p.out + f.b * p.o_sb + (int64_t)(head0 + c16) * p.o_sh + kDV * 4 * g;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -585,9 +567,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       }
       if (begins && ends) {
         if constexpr (MODE == kShared) {
-          floatx4 y[1] = {x};
-          if (((const_i32*)p.skips)[info.y] > 0) add_prefix<D, 1>(p, info.y, head0 + col, d, scale, m, l, y);
-          x = y[0];
+          if (((const_i32*)p.skips)[info.y] > 0) {
+            const int64_t row = (int64_t)info.y * p.n_q_heads + head0 + col;
+            *reinterpret_cast<floatx4*>(p.own + row * D + d) = x;
+            if (d == 0) *reinterpret_cast<floatx2*>(p.own_stats + 2 * row) = floatx2{m, l};
+            continue;
+          }
         }
         if (MODE == kWeigh && d == 0) {
           if (weighs) unit_totals[col] = floatx2{m, 1.f / l};
@@ -614,7 +599,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
         add_to_weights(p, info.y, head0 / group, i, n, sum);
       }
       __syncthreads();  // (before the next unit's totals)
-    } else if (MODE == kWeigh && begins && tid == 0) {
+    } else if (MODE != kPlain && begins && tid == 0) {
       const int kvh = head0 / group, unit = kvh * col_blocks + (head0 - kvh * group) / kCols;
       *reinterpret_cast<int2*>(p.cuts + 2 * ((int64_t)info.y * units + unit)) = ends ? int2{0, 0} : int2{(int)blockIdx.x, info.w};
     }
@@ -681,11 +666,6 @@ __device__ __forceinline__ void combine(const PagedDecodeArgs& p, const int col,
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[e] += sums[i][tid][e];
     l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    if constexpr (MODE == kShared) {
-      floatx4 y[1] = {sum};
-      if (((const_i32*)p.skips)[header.y] > 0) add_prefix<D, 1>(p, header.y, header.z + col, 4 * tid, scale, m, l, y);
-      sum = y[0];
-    }
     const float inv = 1.f / l;
     uint16_t* op = p.out + header.y * p.o_sb + (int64_t)(header.z + col) * p.o_sh + 4 * tid;
     *reinterpret_cast<u32x2*>(op) = u32x2{T::pack(sum[0] * inv, sum[1] * inv), T::pack(sum[2] * inv, sum[3] * inv)};
@@ -694,6 +674,89 @@ __device__ __forceinline__ void combine(const PagedDecodeArgs& p, const int col,
 template <typename T, int D, DecodeMode MODE>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArgs p) {
   combine<T, D, MODE>(p, blockIdx.x, blockIdx.y);
+}
+
+// Joins what is known of a unit's heads over the shared prefix and over the sequence's own keys, each whole or in parts.  256 threads have four channels of a head each; of few heads, every
+// so many of its parts.  Heads lie beside one another in a wave as they do in the parts of many rows, and fours of channels as in the others.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_finish_kernel(const PagedDecodeArgs p) {
+  constexpr int kLanes = D / 4, kHeads = 256 / kLanes, kFours = D / 8;
+  __shared__ floatx4 sums[256];
+  __shared__ floatx2 stats[256];
+  const int group = p.n_q_heads / p.n_kv_heads, col_blocks = (group + kCols - 1) / kCols, units = p.n_kv_heads * col_blocks, tid = threadIdx.x;
+  const int b = blockIdx.x / units, unit = blockIdx.x - b * units, kvh = col_blocks == 1 ? unit : unit / col_blocks;
+  const int head0 = kvh * group + (unit - kvh * col_blocks) * kCols, n_cols = min(kCols, (kvh + 1) * group - head0);
+  const const_i32* cut = (const_i32*)p.cuts + 2 * (int64_t)blockIdx.x;
+  const int skip = ((const_i32*)p.skips)[b], of_group = ((const_i32*)p.firsts)[b], first = cut[0], parts = cut[1];
+  if (skip == 0 && parts == 0) return;  // (the decode kernel's own)
+  int heads_log = 0;
+  while (1 << heads_log < min(n_cols, kHeads)) ++heads_log;
+  const int heads = 1 << heads_log, side = kHeads >> heads_log, d = 4 * ((tid >> heads_log) % kLanes), sub = (tid >> heads_log) / kLanes;
+  const float scale = p.sm_scale * kLog2e;
+  for (int col0 = 0; col0 < n_cols; col0 += heads) {
+    const int col = col0 + (tid & (heads - 1)), head = head0 + min(col, n_cols - 1);
+    const int64_t row = (int64_t)b * p.n_q_heads + head;
+    // (read where they are not there too: sooner than what says so)
+    const floatx2 own_stats = *reinterpret_cast<const floatx2*>(p.own_stats + 2 * row);
+    const floatx4 own = *reinterpret_cast<const floatx4*>(p.own + row * D + d);
+    const bool has = parts == 0 && sub == 0;
+    float m = has ? own_stats[0] : -INFINITY, l = has ? own_stats[1] : 0.f;
+    floatx4 x = {has ? own[0] : 0.f, has ? own[1] : 0.f, has ? own[2] : 0.f, has ? own[3] : 0.f};
+    auto add = [&](const floatx2 s, const floatx4 y) __attribute__((always_inline)) {
+      const float m_new = fmaxf(m, s[0]), w = m == -INFINITY ? 0.f : fast_exp2((m - m_new) * scale), w2 = s[0] == -INFINITY ? 0.f : fast_exp2((s[0] - m_new) * scale);
+      m = m_new;
+      l = w * l + w2 * s[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = w * x[e] + w2 * y[e];
+    };
+    auto add_all = [&](const int n, auto stats_at, auto part_at) __attribute__((always_inline)) {  // a part's statistics and accumulators
+      constexpr int kSide = 8;  // that are read side by side
+      for (int i = sub; i < n; i += side * kSide) {
+        floatx2 s[kSide];
+        floatx4 y[kSide];
+#pragma unroll
+        for (int j = 0; j < kSide; ++j) {
+          const int at = min(i + side * j, n - 1);
+          s[j] = *reinterpret_cast<const floatx2*>(stats_at(at));
+          y[j] = *reinterpret_cast<const floatx4*>(part_at(at));
+        }
+#pragma unroll
+        for (int j = 0; j < kSide; ++j)
+          if (i + side * j < n) add(s[j], y[j]);
+      }
+    };
+    // (the first part of several is the second of its share, the others the first of theirs)
+    if (skip > 0) {
+      const int in_group = (b - of_group) * group + head - kvh * group, row0 = in_group & -p.prefix_rows, s0 = row0 / group, r = in_group - row0;
+      const int2 entry = *reinterpret_cast<const int2*>(p.entries + 2 * ((int64_t)(of_group + s0) * p.n_q_heads + kvh * group + row0 - s0 * group));
+      if (entry.y == 0) {
+        if (sub == 0) add(*reinterpret_cast<const floatx2*>(p.prefix_stats + 2 * row), *reinterpret_cast<const floatx4*>(p.prefix + row * D + d));
+      } else if (p.prefix_rows > 32) {  // four waves' 32 rows, fours of channels lane by lane
+        const int lane = (r & 31) + 32 * (d >> 2 & 1), f = d >> 3;
+        auto at = [&](const int i) { return ((int64_t)2 * (entry.x + i) + (i == 0 ? 1 : 0)) * 4 + (r >> 5); };
+        add_all(entry.y, [&](const int i) { return p.prefix_part_stats + (at(i) * 64 + lane) * 2; }, [&](const int i) { return p.prefix_parts + ((at(i) * kFours + f) * 64 + lane) * 4; });
+      } else {
+        auto at = [&](const int i) { return ((int64_t)2 * (entry.x + i) + (i == 0 ? 1 : 0)) * p.prefix_rows + r; };
+        add_all(entry.y, [&](const int i) { return p.prefix_part_stats + 2 * at(i); }, [&](const int i) { return p.prefix_parts + at(i) * D + d; });
+      }
+    }
+    if (parts > 0) {
+      auto at = [&](const int i) { return ((int64_t)2 * (first + i) + (i == 0 ? 1 : 0)) * kCols + (head - head0); };
+      add_all(parts, [&](const int i) { return p.part_stats + 2 * at(i); }, [&](const int i) { return p.parts + at(i) * D + d; });
+    }
+    if (side > 1) {
+      sums[tid] = x;
+      stats[tid] = floatx2{m, l};
+      __syncthreads();
+      if (sub == 0)
+        for (int i = 1; i < side; ++i) add(stats[tid + i * heads * kLanes], sums[tid + i * heads * kLanes]);
+    }
+    if (sub == 0 && col < n_cols) {
+      const float inv = 1.f / l;
+      *reinterpret_cast<u32x2*>(p.out + b * p.o_sb + (int64_t)head * p.o_sh + d) = u32x2{T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv)};
+    }
+    if (side > 1) __syncthreads();
+  }
 }
 
 // Scratch of a step: a header, and two parts of 16 columns, for each share.  None where no unit is cut.
@@ -783,6 +846,8 @@ static void launch_paged_decode_as(const PagedDecodeArgs& a, hipStream_t stream)
     const int64_t all = (int64_t)a.batch * a.n_kv_heads, room = (((int64_t)a.max_pages << a.page_log) + 1023) / 1024, each = all < 8192 ? 8192 / all : 1;
     const int side = (int)(room < each ? room : each), combiners = a.headers != nullptr ? kShares * cols : 0;
     hipLaunchKernelGGL((paged_weigh_kernel<T, D>), dim3((uint32_t)(combiners + side * all)), dim3(256), 0, stream, a, combiners, cols, side);
+  } else if constexpr (MODE == kShared) {
+    hipLaunchKernelGGL((paged_finish_kernel<T, D>), dim3((uint32_t)((int64_t)a.batch * units)), dim3(256), 0, stream, a);
   } else {
     if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D, MODE>), dim3(cols, kShares), dim3(256), 0, stream, a);
   }

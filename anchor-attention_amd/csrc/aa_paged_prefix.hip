@@ -37,7 +37,7 @@ __device__ __forceinline__ PagedGroup common_group_at(const PagedPrefixArgs& p, 
   return group_of(p, (const_i32*)p.groups, (const_i32*)p.shared_pages, __builtin_amdgcn_readfirstlane(g));
 }
 
-// How many of a sequence's first pages its group's state stands for: those that are shared, if it is as long, or none.
+// How many of a sequence's first pages its group's state stands for: those that are shared, if it is as long, or none; and the group's first sequence.
 __device__ __forceinline__ void find_skips(const PagedPrefixArgs& all, const int tid, const int threads) {
   const PagedDecodeArgs& p = all.step;
   for (int b = blockIdx.x * threads + tid; b < p.batch; b += kPrefixShares * threads) {
@@ -47,13 +47,22 @@ __device__ __forceinline__ void find_skips(const PagedPrefixArgs& all, const int
       if (all.groups[mid + 1] <= b) from = mid + 1;
       else to = mid;
     }
-    int skip = 0;
+    int skip = 0, first = 0;
     if (from < all.n_groups) {
       const PagedGroup x = group_at(all, from);
       if (b >= x.first && b < x.first + x.sequences && clamped_length(p.lengths, b, p.max_pages, p.page_log) >= x.pages << p.page_log) skip = x.pages;
+      first = x.first;
     }
     p.skips[b] = skip;
+    p.firsts[b] = first;
   }
+}
+
+// Where the states of a unit's rows are, by its first row: the share that it begins in and how many have parts of it (0: it is whole)
+template <int ROWS>
+__device__ __forceinline__ void note_unit(const PagedDecodeArgs& p, const int first, const int kvh, const int block, const int heads, const int share, const int parts) {
+  const int row0 = ROWS * block, s = row0 / heads;
+  *reinterpret_cast<int2*>(p.entries + 2 * ((int64_t)(first + s) * p.n_q_heads + kvh * heads + row0 - s * heads)) = int2{share, parts};
 }
 
 // a number that all lanes have, in scalar registers
@@ -134,8 +143,6 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
   int64_t at = mine.at, start = mine.start;
   const int64_t end = mine.end, share = mine.share;
   int group = mine.group;
-  int4* header = reinterpret_cast<int4*>(all.headers) + blockIdx.x;
-  if (tid == 0) header->x = 0;
 
   const float scale = p.sm_scale * kLog2e;
   const uint32_t k_lane = (2u * (c16 * (uint32_t)p.kp_sn + 8 * g)) & 0xfffffu, v_lane = (2u * (4 * g * (uint32_t)p.vp_sn + kDV * c16)) & 0xfffffu;
@@ -144,6 +151,7 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
     uint32_t v[8][kVW];
   };
   while (at < end && group < all.n_groups) {
+    at = uniform(at), start = uniform(start), group = __builtin_amdgcn_readfirstlane(group);  // (which the compiler does not see of what a loop carries)
     const PagedGroup x = common_group_at(all, group);
     const int tiles = tiles_of<kPrefixTile>(p, x), blocks = blocks_of<kRows>(x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
     const int extent = extent_of<kPrefixOver>(tiles);
@@ -383,52 +391,16 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
         stats = p.prefix_stats;
       } else {
         to_row = (int64_t)(2 * blockIdx.x + (begins ? 1 : 0)) * kRows + r;
-        sums = all.parts;
-        stats = all.part_stats;
+        sums = p.prefix_parts;
+        stats = p.prefix_part_stats;
       }
       *reinterpret_cast<floatx4*>(sums + to_row * D + d) = sum;
       if (d == 0) *reinterpret_cast<floatx2*>(stats + 2 * to_row) = floatx2{m, l};
     }
-    if (begins && !ends && tid == 0) {  // its other parts are the next work-groups'
-      *header = int4{(int)((unit_end - 1) / share) - (int)blockIdx.x + 1, group, (int)kvh, (int)block};
-    }
+    if (begins && tid == 0) note_unit<kRows>(p, x.first, (int)kvh, (int)block, heads, blockIdx.x, ends ? 0 : (int)((unit_end - 1) / share) - (int)blockIdx.x + 1);
     __syncthreads();
     at = until;
   }
-}
-
-// Joins the parts of a unit that begins in share blockIdx.y and ends in another, a row by a wave.  (Units begin every so many shares: shares as blockIdx.x were one XCD's.)
-template <int D, int BLOCKS>
-__global__ void __launch_bounds__(256) paged_prefix_join_kernel(const PagedPrefixArgs all) {
-  constexpr int kRows = 16 * BLOCKS, kEach = D / 64;
-  typedef float floats __attribute__((ext_vector_type(kEach)));
-  const PagedDecodeArgs& p = all.step;
-  const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = blockIdx.y;
-  const int4 header = *reinterpret_cast<const int4*>(all.headers + 4 * share);
-  const int parts = header.x, heads = p.n_q_heads / p.n_kv_heads;
-  if (parts == 0) return;
-  const PagedGroup x = common_group_at(all, header.y);
-  const int row = header.w * kRows + r;
-  if (row >= x.sequences * heads) return;
-  const float scale = p.sm_scale * kLog2e;
-  // the first part is the second of its share, the others the first of theirs
-  auto part = [&](const int i) { return ((int64_t)2 * (share + i) + (i == 0 ? 1 : 0)) * kRows + r; };
-  float m = -INFINITY;
-  for (int i = lane; i < parts; i += 64) m = fmaxf(m, all.part_stats[2 * part(i)]);
-  m = over_wave(m, -INFINITY, [](const float a, const float b) { return fmaxf(a, b); });
-  float l = 0.f;
-  floats sum = {};
-  for (int i = 0; i < parts; ++i) {
-    const float mi = all.part_stats[2 * part(i)], w = mi == -INFINITY ? 0.f : fast_exp2((mi - m) * scale);
-    l += w * all.part_stats[2 * part(i) + 1];
-    const floats y = *reinterpret_cast<const floats*>(all.parts + part(i) * D + kEach * lane);
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) sum[e] += w * y[e];
-  }
-  const int s = row / heads;
-  const int64_t to = (int64_t)(x.first + s) * p.n_q_heads + header.z * heads + row - s * heads;
-  *reinterpret_cast<floats*>(p.prefix + to * D + kEach * lane) = sum;
-  if (lane == 0) *reinterpret_cast<floatx2*>(p.prefix_stats + 2 * to) = floatx2{m, l};
 }
 
 // ---- many rows ------------------------------------------------------------------------------------
@@ -475,8 +447,6 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
   int64_t at = mine.at, start = mine.start;
   const int64_t end = mine.end, share = mine.share;
   int group = mine.group;
-  int4* header = reinterpret_cast<int4*>(all.headers) + share_at;
-  if (tid == 0) header->x = 0;
 
   const float scale = p.sm_scale * kLog2e;
   // where a lane's pieces of 16 rows come from (its chunk, which belongs in its slot), and what it reads of a tile
@@ -494,6 +464,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
   const uint32_t v_rd = my_tiles + 2 * kTileBytes + r0 * kRowBytes + ((y0 ^ wide_v_swizzle<D>(r0)) << 4) + 8 * (lane & 1);
 
   while (at < end && group < all.n_groups) {
+    at = uniform(at), start = uniform(start), group = __builtin_amdgcn_readfirstlane(group);  // (which the compiler does not see of what a loop carries)
     const PagedGroup x = common_group_at(all, group);
     const int n_tiles = tiles_of<kWideTile>(p, x), blocks = blocks_of<kWideRows>(x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
     const int extent = extent_of<kWideOver>(n_tiles);
@@ -718,11 +689,11 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         const int f = decltype(first)::value + g;
         const floatx4 a = four(f), b = states[f * 64 + lane];
         const floatx4 y = {w * a[0] + w2 * b[0], w * a[1] + w2 * b[1], w * a[2] + w2 * b[2], w * a[3] + w2 * b[3]};
-        if (!whole) *reinterpret_cast<floatx4*>(all.parts + ((part * kFours + f) * 64 + lane) * 4) = y;
+        if (!whole) *reinterpret_cast<floatx4*>(p.prefix_parts + ((part * kFours + f) * 64 + lane) * 4) = y;
         else if (there) *reinterpret_cast<floatx4*>(p.prefix + my_head * D + 8 * f + 4 * half) = y;
       }
       if (decltype(first)::value != 0) return;
-      if (!whole) *reinterpret_cast<floatx2*>(all.part_stats + (part * 64 + lane) * 2) = floatx2{m, l};
+      if (!whole) *reinterpret_cast<floatx2*>(p.prefix_part_stats + (part * 64 + lane) * 2) = floatx2{m, l};
       else if (there && half == 0) *reinterpret_cast<floatx2*>(p.prefix_stats + 2 * my_head) = floatx2{m, l};
     };
     std::integral_constant<int, 0> lower;
@@ -732,90 +703,11 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     __syncthreads();
     if (team == 0) finish(lower);
     else finish(upper);
-    if (t0 == 0 && t1 < n_tiles && tid == 0) {  // its other parts are the next work-groups'
-      *header = int4{(int)((unit_end - 1) / share) - share_at + 1, group, (int)kvh, (int)block};
-    }
+    if (t0 == 0 && tid == 0) note_unit<kWideRows>(p, x.first, (int)kvh, (int)block, heads, share_at, whole ? 0 : (int)((unit_end - 1) / share) - share_at + 1);
     __syncthreads();
     at = until;
   }
   find_skips(all, tid, kWideThreads);
-}
-
-// Joins the parts of a unit that begins in share blockIdx.y and ends in another: a work-group has two fours of 32 rows' accumulators, lane by lane as they were left, and
-// its waves every so many parts.
-template <int D>
-__global__ void __launch_bounds__(512) paged_prefix_wide_join_kernel(const PagedPrefixArgs all) {
-  constexpr int kFours = D / 8, kEach = 2, kJoin = 8;
-  __shared__ floatx4 red[kJoin][kEach][64];
-  __shared__ floatx2 red_stats[kJoin][64];
-  const PagedDecodeArgs& p = all.step;
-  const int lane = threadIdx.x & 63, mine = threadIdx.x >> 6, wave = blockIdx.x % 4, f0 = kEach * (blockIdx.x / 4), share = blockIdx.y;
-  const int4 header = *reinterpret_cast<const int4*>(all.headers + 4 * share);
-  const int parts = header.x, heads = p.n_q_heads / p.n_kv_heads;
-  if (parts == 0) return;
-  const PagedGroup x = common_group_at(all, header.y);
-  const int row = header.w * kWideRows + 32 * wave + (lane & 31);
-  const float scale = p.sm_scale * kLog2e;
-  // the first part is the second of its share, the others the first of theirs
-  auto part = [&](const int i) { return ((int64_t)2 * (share + i) + (i == 0 ? 1 : 0)) * 4 + wave; };
-  float m = -INFINITY, l = 0.f;
-  floatx4 sum[kEach] = {};
-  constexpr int kSide = 4;  // parts that are read side by side
-  for (int i = mine; i < parts; i += kJoin * kSide) {
-    floatx2 stats[kSide];
-    floatx4 y[kSide][kEach];
-#pragma unroll
-    for (int j = 0; j < kSide; ++j) {
-      const int64_t at = part(min(i + kJoin * j, parts - 1));
-      stats[j] = *reinterpret_cast<const floatx2*>(all.part_stats + (at * 64 + lane) * 2);
-#pragma unroll
-      for (int f = 0; f < kEach; ++f) y[j][f] = *reinterpret_cast<const floatx4*>(all.parts + ((at * kFours + f0 + f) * 64 + lane) * 4);
-    }
-    float m_new = m;
-#pragma unroll
-    for (int j = 0; j < kSide; ++j) m_new = i + kJoin * j < parts ? fmaxf(m_new, stats[j][0]) : m_new;
-    const float old = m == -INFINITY ? 0.f : fast_exp2((m - m_new) * scale);
-    m = m_new;
-    l *= old;
-#pragma unroll
-    for (int f = 0; f < kEach; ++f)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[f][e] *= old;
-#pragma unroll
-    for (int j = 0; j < kSide; ++j) {
-      if (i + kJoin * j >= parts) break;
-      const float w = stats[j][0] == -INFINITY ? 0.f : fast_exp2((stats[j][0] - m) * scale);
-      l += w * stats[j][1];
-#pragma unroll
-      for (int f = 0; f < kEach; ++f)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[f][e] += w * y[j][f][e];
-    }
-  }
-  red_stats[mine][lane] = floatx2{m, l};
-#pragma unroll
-  for (int f = 0; f < kEach; ++f) red[mine][f][lane] = sum[f];
-  __syncthreads();
-  if (mine >= kEach) return;
-  // a wave for each four
-  m = -INFINITY;
-  l = 0.f;
-  floatx4 total = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int w = 0; w < kJoin; ++w) m = fmaxf(m, red_stats[w][lane][0]);
-#pragma unroll
-  for (int w = 0; w < kJoin; ++w) {
-    const float weight = red_stats[w][lane][0] == -INFINITY ? 0.f : fast_exp2((red_stats[w][lane][0] - m) * scale);
-    l += weight * red_stats[w][lane][1];
-    const floatx4 y = red[w][mine][lane];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) total[e] += weight * y[e];
-  }
-  if (row >= x.sequences * heads) return;
-  const int s = row / heads;
-  const int64_t to = (int64_t)(x.first + s) * p.n_q_heads + header.z * heads + row - s * heads;
-  *reinterpret_cast<floatx4*>(p.prefix + to * D + 8 * (f0 + mine) + 4 * (lane >> 5)) = total;
-  if (f0 + mine == 0 && lane < 32) *reinterpret_cast<floatx2*>(p.prefix_stats + 2 * to) = floatx2{m, l};
 }
 
 // Rows of a unit, in blocks of 16: as many as a KV head's queries of a group fill on average, 16 or 32, or more where there are more.
@@ -825,11 +717,22 @@ static int prefix_blocks(int batch, int n_q_heads, int n_kv_heads, int n_groups)
   return rows <= 16 ? 1 : rows <= 32 ? 2 : kWide;
 }
 
+// Where the keys and values of all sequences fit the caches, as much as the table has room for, what sequences share is there after the first one's read, and the steps of the others cost less than
+// two kernels more.  One group, 100 keys of their own, all bytes as if none were shared, time by this path and with every sequence by itself:
+//   14/2 heads of 64: 2 sequences behind 1024 keys (1 MB) 17.3 and 11.0 us, 32 behind 4096 (69 MB) 24.2 and 15.2, 64 behind 8192 (272 MB) 28.7 and 30.7, 64 behind 16384 (540 MB) 30.0 and 51.8
+//   32/8 of 128: 4 behind 1024 (18 MB) 22.4 and 13.6, 8 behind 8192 (272 MB) 30.7 and 27.8, 32 behind 4096 (550 MB) 31.9 and 43.0
+//   28/4 of 128, fp16: 16 behind 8192 (272 MB) 38.9 and 27.5, 32 behind 8192 (543 MB) 35.4 and 45.3
+// The lengths are the device's to know: in a table with room for more, few keys take this path too.
+bool paged_prefix_pays(int batch, int n_kv_heads, int head_dim, int page_size, int max_pages) {
+  return (double)batch * max_pages * page_size * n_kv_heads * head_dim * 4 > 256e6;
+}
+
+int paged_prefix_part_rows(int batch, int n_q_heads, int n_kv_heads, int n_groups) { return 16 * prefix_blocks(batch, n_q_heads, n_kv_heads, n_groups); }
+
 PagedScratch paged_prefix_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups) {
   const int blocks = prefix_blocks(batch, n_q_heads, n_kv_heads, n_groups);
   const size_t rows = (size_t)kPrefixShares * 2 * 16 * blocks;
   PagedScratch s = {0, 0, 0, 0};
-  s.stats = (size_t)kPrefixShares * 16;
   s.parts = s.stats + rows * (blocks == kWide ? 16 : 8);  // (a row's statistics are there twice, once for each of its lanes)
   s.total = s.parts + rows * head_dim * 4;
   return s;
@@ -839,17 +742,13 @@ template <typename T, int D, int BLOCKS>
 static void launch_paged_prefix_for(const PagedPrefixArgs& a, hipStream_t stream) {
   constexpr size_t lds = (size_t)kPrefixWaves * 16 * BLOCKS * (D + 4) * 4;
   hipLaunchKernelGGL((paged_prefix_kernel<T, D, BLOCKS>), dim3(kPrefixShares), dim3(64 * kPrefixWaves), lds, stream, a);
-  hipLaunchKernelGGL((paged_prefix_join_kernel<D, BLOCKS>), dim3(4 * BLOCKS, kPrefixShares), dim3(256), 0, stream, a);
 }
 template <typename T, int D>
 static hipError_t launch_paged_prefix_of(const PagedPrefixArgs& a, hipStream_t stream) {
   const int blocks = prefix_blocks(a.step.batch, a.step.n_q_heads, a.step.n_kv_heads, a.n_groups);
   if (blocks == 1) launch_paged_prefix_for<T, D, 1>(a, stream);
   else if (blocks == 2) launch_paged_prefix_for<T, D, 2>(a, stream);
-  else {
-    hipLaunchKernelGGL((paged_prefix_wide_kernel<T, D>), dim3(kPrefixShares), dim3(kWideThreads), 0, stream, a);
-    hipLaunchKernelGGL((paged_prefix_wide_join_kernel<D>), dim3(D / 4, kPrefixShares), dim3(512), 0, stream, a);
-  }
+  else hipLaunchKernelGGL((paged_prefix_wide_kernel<T, D>), dim3(kPrefixShares), dim3(kWideThreads), 0, stream, a);
   return hipGetLastError();
 }
 hipError_t launch_paged_prefix(const PagedPrefixArgs& a, hipStream_t stream) {

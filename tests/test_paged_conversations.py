@@ -299,6 +299,12 @@ def _shared_setup(prefixes, sizes, own, hkv, d, page, dtype, seed, layout="heads
     return s, _int32(prefixes), _int32(begins)
 
 
+def _roomy(s):
+    """The setup's table with room for so many pages (zeros, which nothing reads) that the kernels for shared pages are what runs, and that the caches do not hold them all."""
+    pages = 300_000_000 // (s.table.shape[0] * s.cache.page_size * s.hkv * s.d * 4) + 1
+    return torch.cat([s.table, torch.zeros(s.table.shape[0], max(pages - s.table.shape[1], 0), dtype=torch.int32, device="cuda")], 1)
+
+
 def _shared_close(out, q, s, scale, n_groups):
     """What :func:`_close` asks for, and where more than 32 rows share a prefix the rounding of probabilities."""
     group = q.shape[1] // s.hkv
@@ -337,18 +343,23 @@ def _shared_close(out, q, s, scale, n_groups):
 ])
 def test_shared_decode(prefixes, sizes, own, hq, hkv, d, page, layout, extra, alone, dtype):
     s, shared, groups = _shared_setup(prefixes, sizes, own, hkv, d, page, dtype, hq + page, layout, extra, alone)
-    q = s.queries(hq)
+    for table in (_roomy(s), s.table):
+        _check_shared_decode(s, table, shared, groups, s.queries(hq), len(sizes) == 1 and not alone)
+
+
+def _check_shared_decode(s, table, shared, groups, q, all_in_one):
+    hq, d, dtype, n_groups = q.shape[1], s.d, q.dtype, len(shared)
     wide = torch.full((len(s.host), hq + 1, d + 8), 7.0, dtype=dtype, device="cuda")
     out = wide[:, 1:, 8:]
-    assert _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, out=out) is out
+    assert _ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, shared, groups, out=out) is out
     assert bool((wide[:, 0] == 7.0).all()) and bool((wide[:, :, :8] == 7.0).all())
-    _shared_close(out, q, s, d ** -0.5, len(sizes))
-    again = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, sm_scale=d ** -0.5)
+    _shared_close(out, q, s, d ** -0.5, n_groups)
+    again = _ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, shared, groups, sm_scale=d ** -0.5)
     assert torch.equal(out, again)  # the same bits
-    _shared_close(_ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, sm_scale=0.3), q, s, 0.3, len(sizes))
-    if len(sizes) == 1 and not alone:
-        assert torch.equal(_ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared), out)
-    assert _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups, out=q) is q and torch.equal(q, again)
+    _shared_close(_ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, shared, groups, sm_scale=0.3), q, s, 0.3, n_groups)
+    if all_in_one:
+        assert torch.equal(_ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, shared), out)
+    assert _ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, shared, groups, out=q) is q and torch.equal(q, again)
 
 
 @pytest.mark.gpu
@@ -359,11 +370,11 @@ def test_shared_decode_of_sequences_that_are_shorter_than_the_prefix():
     s.lengths.copy_(_int32(s.host))
     s.cache.values.nan_to_num_(1.0), s.cache.keys.nan_to_num_(1.0)
     q = s.queries(8)
-    got = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    got = _ops().paged_shared_decode_attention(s.cache, q, _roomy(s), s.lengths, shared, groups)
     _close(got, q, s, 0.125)
     s.cache.values[s.table[0, 9].long(), :, 15] = float("inf")  # (key 159)
     s.cache.keys[s.table[8, 5].long(), :, 15] = float("nan")  # (key 95)
-    bad = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    bad = _ops().paged_shared_decode_attention(s.cache, q, _roomy(s), s.lengths, shared, groups)
     seen = [b for b, n in enumerate(s.host) if n >= (160 if b < 8 else 96)]
     assert all(not bool(bad[b].isfinite().any()) if b in seen else torch.equal(bad[b], got[b]) for b in range(12))
     assert all(bool((bad[b] == float("inf")).all()) for b in seen if b < 8) and all(bool(bad[b].isnan().all()) for b in seen if b >= 8)
@@ -377,10 +388,10 @@ def test_shared_decode_with_infinite_values_and_scores(batch, pages, dtype):
     s, shared, groups = _shared_setup([pages], [batch], [40], 2, 64, 16, dtype, 8)
     q = s.queries(8, 0.3)
     q[:, :, 0] = 1.0
-    want = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    want = _ops().paged_shared_decode_attention(s.cache, q, _roomy(s), s.lengths, shared, groups)
     at = s.table[0, 1].long()
     s.cache.values[at, 0, 3, 5], s.cache.values[at, 0, 4, 6], s.cache.values[at, 0, 9, 7] = float("inf"), float("-inf"), float("nan")
-    got = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    got = _ops().paged_shared_decode_attention(s.cache, q, _roomy(s), s.lengths, shared, groups)
     assert bool((got[:, :4, 5] == float("inf")).all()) and bool((got[:, :4, 6] == float("-inf")).all()) and bool(got[:, :4, 7].isnan().all())
     assert torch.equal(got[:, 4:], want[:, 4:])
     rest = torch.ones(64, dtype=torch.bool, device="cuda")
@@ -393,7 +404,7 @@ def test_shared_decode_with_infinite_values_and_scores(batch, pages, dtype):
     s.cache.keys[s.table[0, :pages].long(), 0, :, 0] = float("-inf")
     s.cache.keys[s.table[1, pages:pages + 3].long(), 1, :, 0] = float("-inf")
     s.cache.keys[s.table[2, pages:pages + 3].long(), 0, :, 0] = float("-inf")
-    got = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    got = _ops().paged_shared_decode_attention(s.cache, q, _roomy(s), s.lengths, shared, groups)
     plain = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
     assert bool(got[2, :4].isnan().all()) and bool(plain[2, :4].isnan().all()) and int(got.isnan().sum()) == 4 * 64
     near = (got.double() - plain.double()).abs() <= 2 * U[dtype] * plain.abs() + 2.0 ** -12 + slack
@@ -408,15 +419,17 @@ def test_groups_that_do_not_fit():
     q = s.queries(4)
     plain = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
     for shared_pages, begins in (([2 ** 31 - 1], [0, 6]), ([-5], [0, 6]), ([4], [-7, 2 ** 31 - 1]), ([4, 4], [-9, 2, 100]), ([4], [6, 6]), ([4], [5, 3]), ([4, 4, 4], [2, 2, 2, 4]), ([4], [-3, -1])):
-        got = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, _int32(shared_pages), _int32(begins))
+        got = _ops().paged_shared_decode_attention(s.cache, q, _roomy(s), s.lengths, _int32(shared_pages), _int32(begins))
         assert bool(((got.float() - plain.float()).abs() <= 2 * U[BF16] * plain.float().abs() + 2.0 ** -12).all()), (shared_pages, begins)
     s.table[0, 1], s.table[0, 2] = -1, 2 ** 31 - 1
-    got = _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+    got = _ops().paged_shared_decode_attention(s.cache, q, _roomy(s), s.lengths, shared, groups)
     s.table[:, 1], s.table[:, 2] = 0, s.cache.n_pages - 1
-    assert torch.equal(got, _ops().paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups))
+    assert torch.equal(got, _ops().paged_shared_decode_attention(s.cache, q, _roomy(s), s.lengths, shared, groups))
     # no keys but the prefix, in a table that ends with it
     s.host = [64] * 6
     got = _ops().paged_shared_decode_attention(s.cache, q, s.table[:, :4], _int32(s.host), shared, groups)
+    _close(got, q, s, 0.125)
+    got = _ops().paged_shared_decode_attention(s.cache, q, _roomy(s), _int32(s.host), shared, groups)
     _close(got, q, s, 0.125)
 
 
@@ -673,7 +686,7 @@ def test_conversations_that_share_a_prompt_and_give_up_keys():
         s.host = [n + m for m in own]
         s.lengths = _int32(s.host)
         ops.append_to_pages(s.cache, None, *x, cos, sin, s.table, s.lengths, _int32([0, 30, 71, 72, 109]), k_norm=wk)
-        s.positions = s.lengths.clone()
+        s.positions, s.roomy = s.lengths.clone(), _roomy(s)
         return s
 
     shared = _int32([n // page])
@@ -682,7 +695,7 @@ def test_conversations_that_share_a_prompt_and_give_up_keys():
         s.lengths += 1
         s.positions += 1
         rotated = ops.append_to_pages(s.cache, *x, cos, sin, s.table, s.lengths, positions=s.positions, **more)
-        out = ops.paged_shared_decode_attention(s.cache, rotated, s.table, s.lengths, shared)
+        out = ops.paged_shared_decode_attention(s.cache, rotated, s.roomy, s.lengths, shared)
         same = ops.paged_weighing_decode_attention(s.cache, rotated, s.table, s.lengths, n_first=n)
         had = s.lengths.clone()
         lengths, kept = ops.evict_from_pages(s.cache, s.table, s.lengths, keep, n_first=n, n_last=8, above=above)
@@ -703,7 +716,7 @@ def test_conversations_that_share_a_prompt_and_give_up_keys():
         s.host = s.lengths.tolist()
         rotated = ops.append_to_pages(s.cache, *x, cos, sin, s.table, s.lengths, positions=s.positions, **more)
         _near(rotated, x[0], wq, 1e-6, cos[s.positions.long() - 1], sin[s.positions.long() - 1])
-        out = ops.paged_shared_decode_attention(s.cache, rotated, s.table, s.lengths, shared)
+        out = ops.paged_shared_decode_attention(s.cache, rotated, s.roomy, s.lengths, shared)
         _close(out, rotated, s, d ** -0.5)
         before = s.cache.weights.clone()
         same = ops.paged_weighing_decode_attention(s.cache, rotated, s.table, s.lengths, n_first=n)
@@ -751,10 +764,11 @@ def test_steps_on_two_streams_at_once():
         s, shared, groups = _shared_setup([30, 5], [9, 3], [400, 70, 3], 4, 128, 64, BF16, seed)
         s.cache = _weights_of(s)
         s.cache.weights.zero_()
+        s.roomy = _roomy(s)
         return s, s.queries(16), shared, groups
 
     def work(s, q, shared, groups):
-        out = ops.paged_shared_decode_attention(s.cache, q, s.table, s.lengths, shared, groups)
+        out = ops.paged_shared_decode_attention(s.cache, q, s.roomy, s.lengths, shared, groups)
         # (one sequence of each group, which share nothing)
         table, lengths = s.table[8:10], s.lengths[8:10]
         weighed = ops.paged_weighing_decode_attention(s.cache, q[8:10], table, lengths)
