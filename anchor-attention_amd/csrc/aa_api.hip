@@ -1133,7 +1133,7 @@ int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step*
   const PagedScratch s = paged_prefix_scratch(a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim, n_groups);
   a.prefix_part_stats = (float*)(ws + w.parts + s.stats);
   a.prefix_parts = (float*)(ws + w.parts + s.parts);
-  a.prefix_rows = paged_prefix_part_rows(a.batch, a.n_q_heads, a.n_kv_heads, n_groups);
+  a.prefix_rows = paged_prefix_part_rows(a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim, n_groups);
   const PagedPrefixArgs x = {a, shared_pages, groups, n_groups};
   if ((rc = check_launch(launch_paged_prefix(x, (hipStream_t)stream), who))) return rc;
   give_scratch(a, ws + w.decode, t->max_pages);

@@ -192,7 +192,7 @@ struct PagedPrefixArgs {
   const int32_t* shared_pages; const int32_t* groups; int n_groups;  // groups NULL: one, the whole batch
 };
 bool paged_prefix_pays(int batch, int n_kv_heads, int head_dim, int page_size, int max_pages);  // (by how much a batch may read: else every sequence reads the prefix for itself)
-int paged_prefix_part_rows(int batch, int n_q_heads, int n_kv_heads, int n_groups);  // rows of a part: row by row up to 32, else as paged_prefix_wide_kernel leaves them
+int paged_prefix_part_rows(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups);  // rows of a part: 16, row by row, or 128 as paged_prefix_wide_kernel leaves them
 PagedScratch paged_prefix_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups);
 hipError_t launch_paged_prefix(const PagedPrefixArgs& a, hipStream_t stream);
 

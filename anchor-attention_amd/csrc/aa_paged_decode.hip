@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(256) paged_finish_kernel(const PagedDecodeArgs
       const int2 entry = *reinterpret_cast<const int2*>(p.entries + 2 * ((int64_t)(of_group + s0) * p.n_q_heads + kvh * group + row0 - s0 * group));
       if (entry.y == 0) {
         if (sub == 0) add(*reinterpret_cast<const floatx2*>(p.prefix_stats + 2 * row), *reinterpret_cast<const floatx4*>(p.prefix + row * D + d));
-      } else if (p.prefix_rows > 32) {  // four waves' 32 rows, fours of channels lane by lane
+      } else if (p.prefix_rows != 16) {  // four waves' 32 rows, fours of channels lane by lane
         const int lane = (r & 31) + 32 * (d >> 2 & 1), f = d >> 3;
         auto at = [&](const int i) { return ((int64_t)2 * (entry.x + i) + (i == 0 ? 1 : 0)) * 4 + (r >> 5); };
         add_all(entry.y, [&](const int i) { return p.prefix_part_stats + (at(i) * 64 + lane) * 2; }, [&](const int i) { return p.prefix_parts + ((at(i) * kFours + f) * 64 + lane) * 4; });

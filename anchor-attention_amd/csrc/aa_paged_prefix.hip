@@ -1,12 +1,14 @@
-// Attention of one new token per sequence over the first pages of its group's sequences, which all of them share, on gfx950: the state (maximum, sum,
-// accumulator) of each head over the prefix, which the decode kernel joins with the sequence's own keys.
+// Attention of one new token per sequence over the first pages of its group's sequences, which all of them share, on gfx950: of each head over the prefix the largest score m, the sum l of
+// 2^((score - m) * scale) and the accumulator of these times the values.  The decode kernel has the same of the sequence's own keys, and paged_finish_kernel joins them:
+//   o = (w a + w' a') / (w l + w' l'),  w = 2^((m - max(m, m')) * scale).
 //
-// The heads of a KV head's queries, of all sequences of the group, are rows of one product, so that keys and values are read once for 16 * BLOCKS of them.  A unit is a
-// (group, KV head, 16 * BLOCKS rows); its keys come in tiles of 32.  The tiles of all units, one after the other, are cut into equal shares, one for each of a
-// fixed number of work-groups; inside a share a unit's tiles are its four waves', each with accumulators of its own, joined through LDS.  A unit that several shares
-// have is joined by paged_prefix_join_kernel in order, so that results do not depend on timing.
+// The heads of a KV head's queries, of all sequences of the group, are rows of one product, so that keys and values are read once for 16 or 128 of them (unit_rows).  A unit is a
+// (group, KV head, rows); its keys come in tiles of 32 or 64.  The tiles of all units, one after the other, are cut into equal shares, one for each of a fixed number of
+// work-groups.  A unit that several shares have is joined in their order, so that results do not depend on timing.
 //
-// Inside a wave, as in the decode kernel: S^T = K Q^T straight from memory, P^T in S^T's registers, V turned by v_perm once for all rows, P as two 16-bit numbers.
+// Of 16 rows a share's tiles are its four waves', each with accumulators of its own, joined through LDS: inside a wave, as in the decode kernel, S^T = K Q^T straight from memory, P^T in
+// S^T's registers, V turned by v_perm, P as two 16-bit numbers.  It is bound by the latency of its loads: 8192 keys of 8 KV heads of 128 (34 MB) in 8.4 us beside 19 us of the rest.
+// Of 128 rows: below.
 #include <type_traits>
 
 #include "aa_kernels.h"
@@ -124,13 +126,13 @@ __device__ __forceinline__ PrefixShare share_of(const PagedPrefixArgs& all, cons
   return {uniform(r.at), uniform(r.end), uniform(r.share), uniform(r.start), (int)__builtin_amdgcn_readfirstlane(r.group)};
 }
 
-template <typename T, int D, int BLOCKS>
+template <typename T, int D>
 __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(const PagedPrefixArgs all) {
   constexpr int kKS = D / 32;  // MFMAs of a score
   constexpr int kDV = D / 16;  // channels of V that a lane loads
   constexpr int kVW = kDV / 2;
-  constexpr int kRows = 16 * BLOCKS, kPitch = D + 4;
-  extern __shared__ __attribute__((aligned(16))) float states[];  // [wave][row][kPitch]: the accumulator, maximum and sum
+  constexpr int kRows = 16, kPitch = D + 4;
+  __shared__ __attribute__((aligned(16))) float states[kPrefixWaves * kRows * kPitch];  // [wave][row][kPitch]: the accumulator, maximum and sum
   const PagedDecodeArgs& p = all.step;
   const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -164,16 +166,15 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
     const int64_t unit_end = start + (int64_t)(unit + 1) * extent, until = min(end, unit_end);
     const int t0 = max(tiles - (int)(unit_end - at), 0), t1 = max(tiles - (int)(unit_end - until), 0);
     if (t1 == 0) break;  // (nothing of it is in this share, which ends)
-    const int row0 = block * kRows, n_blocks = min(BLOCKS, (rows - row0 + 15) / 16);
+    const int row0 = block * kRows;
     const int from = t0 + (t1 - t0) * wave / kPrefixWaves, to = t0 + (t1 - t0) * (wave + 1) / kPrefixWaves;
 
-    u32x4 q[BLOCKS][kKS];
-#pragma unroll
-    for (int c = 0; c < BLOCKS; ++c) {
-      const int row = min(row0 + 16 * c + c16, rows - 1), s = row / heads;
+    u32x4 q[kKS];
+    {
+      const int row = min(row0 + c16, rows - 1), s = row / heads;
       const uint16_t* qp = p.q + (int64_t)(x.first + s) * p.q_sb + (int64_t)((int)kvh * heads + row - s * heads) * p.q_sh + 8 * g;
 #pragma unroll
-      for (int s = 0; s < kKS; ++s) q[c][s] = *reinterpret_cast<const u32x4*>(qp + 32 * s);
+      for (int s = 0; s < kKS; ++s) q[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s);
     }
     const const_i32* table = (const_i32*)(p.table + x.first * p.t_sb);
     struct Spot {
@@ -211,34 +212,25 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
         }
       }
     };
-    float m_run[BLOCKS], l_run[BLOCKS];
-    floatx4 acc[BLOCKS][kDV];
+    float m_run = -INFINITY, l_run;
+    floatx4 acc[kDV];
     auto clear = [&]() __attribute__((always_inline)) {
+      l_run = 0.f;
 #pragma unroll
-      for (int c = 0; c < BLOCKS; ++c) {
-        l_run[c] = 0.f;
-#pragma unroll
-        for (int j = 0; j < kDV; ++j) acc[c][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-      }
+      for (int j = 0; j < kDV; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
     };
     clear();
-#pragma unroll
-    for (int c = 0; c < BLOCKS; ++c) m_run[c] = -INFINITY;
 
     // (the last tile of a prefix of 16 * odd keys has no second half)
     auto seen = [&](const int t, const int i) __attribute__((always_inline)) { return kPrefixTile * t + 16 * (i >> 2) < length; };
-    auto scores = [&](const Tile& y, floatx4 (&s)[BLOCKS][2]) __attribute__((always_inline)) {
+    auto scores = [&](const Tile& y, floatx4 (&s)[2]) __attribute__((always_inline)) {
+      s[0] = s[1] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < BLOCKS; ++c) {
-        if (c > 0 && c >= n_blocks) break;
-        s[c][0] = s[c][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < kKS; ++i)
 #pragma unroll
-        for (int i = 0; i < kKS; ++i)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) s[c][half] = mfma16<T>(y.k[half][i], q[c][i], s[c][half]);
-      }
+        for (int half = 0; half < 2; ++half) s[half] = mfma16<T>(y.k[half][i], q[i], s[half]);
     };
-    auto probabilities = [&](floatx4 (&s)[2], const int t, const int c, u32x4& prob, u32x4& rest, const bool exact) __attribute__((always_inline)) {
+    auto probabilities = [&](floatx4 (&s)[2], const int t, u32x4& prob, u32x4& rest, const bool exact) __attribute__((always_inline)) {
       if (kPrefixTile * (t + 1) > length) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = seen(t, i) ? s[i >> 2][i & 3] : -INFINITY;
@@ -246,21 +238,21 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
       float mx = s[0][0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
-      const float m_new = fmaxf(m_run[c], max_over_quarters(mx));
+      const float m_new = fmaxf(m_run, max_over_quarters(mx));
       const float m_base = m_new == -INFINITY ? 0.f : m_new;
-      if (__any(m_new > m_run[c])) {
-        const float alpha = fast_exp2((m_run[c] - m_base) * scale);
-        l_run[c] *= alpha;
+      if (__any(m_new > m_run)) {
+        const float alpha = fast_exp2((m_run - m_base) * scale);
+        l_run *= alpha;
 #pragma unroll
         for (int j = 0; j < kDV; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[c][j][r] *= alpha;
-        m_run[c] = m_new;
+          for (int r = 0; r < 4; ++r) acc[j][r] *= alpha;
+        m_run = m_new;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float e0 = prob_exp2<T>(s[i >> 1][2 * (i & 1)] - m_base, scale), e1 = prob_exp2<T>(s[i >> 1][2 * (i & 1) + 1] - m_base, scale);
-        l_run[c] += e0 + e1;
+        l_run += e0 + e1;
         uint32_t w = T::pack(e0, e1);
         if (exact) {
           if (e0 > 0.f && (w & 0xffffu) == 0u) w |= 1u;
@@ -270,7 +262,7 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
         rest[i] = T::pack_rest(e0, e1, w);
       }
     };
-    auto add_values = [&](Tile& y, const int t, const u32x4 (&prob)[BLOCKS], const u32x4 (&rest)[BLOCKS], const bool exact) __attribute__((always_inline)) {
+    auto add_values = [&](Tile& y, const int t, const u32x4& prob, const u32x4& rest, const bool exact) __attribute__((always_inline)) {
 #pragma unroll
       for (int w = 0; w < kVW; ++w)
 #pragma unroll
@@ -285,12 +277,8 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
               if (((v[i] >> 16) & T::kExponent) == T::kExponent) finite[i] &= 0xffffu;
             }
           }
-#pragma unroll
-          for (int c = 0; c < BLOCKS; ++c) {
-            if (c > 0 && c >= n_blocks) break;
-            acc[c][2 * w + odd] = mfma16<T>(v, prob[c], acc[c][2 * w + odd]);
-            acc[c][2 * w + odd] = mfma16<T>(finite, rest[c], acc[c][2 * w + odd]);
-          }
+          acc[2 * w + odd] = mfma16<T>(v, prob, acc[2 * w + odd]);
+          acc[2 * w + odd] = mfma16<T>(finite, rest, acc[2 * w + odd]);
         }
     };
 
@@ -303,31 +291,22 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
     }
     for (int t = from; t < to; ++t) {
       const Spot o = spot(min(t + 1, to - 1));
-      floatx4 s[BLOCKS][2];
+      floatx4 s[2];
       scores(y, s);
       __builtin_amdgcn_sched_barrier(0);
       load_k(y, o);
       __builtin_amdgcn_sched_barrier(0);
-      u32x4 prob[BLOCKS], rest[BLOCKS];
-#pragma unroll
-      for (int c = 0; c < BLOCKS; ++c) {
-        if (c > 0 && c >= n_blocks) break;
-        probabilities(s[c], t, c, prob[c], rest[c], false);
-      }
+      u32x4 prob, rest;
+      probabilities(s, t, prob, rest, false);
       add_values(y, t, prob, rest, false);
       __builtin_amdgcn_sched_barrier(0);
       load_v(y, o);
     }
-    bool again = false;
+    l_run = sum_over_quarters(l_run);
+    float sum = 0.f;
 #pragma unroll
-    for (int c = 0; c < BLOCKS; ++c) {
-      l_run[c] = sum_over_quarters(l_run[c]);
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < kDV; ++j) sum += (acc[c][j][0] + acc[c][j][1]) + (acc[c][j][2] + acc[c][j][3]);
-      again |= is_nan(sum) && !is_nan(l_run[c]);
-    }
-    if (__builtin_expect(__any(again), 0)) {
+    for (int j = 0; j < kDV; ++j) sum += (acc[j][0] + acc[j][1]) + (acc[j][2] + acc[j][3]);
+    if (__builtin_expect(__any(is_nan(sum) && !is_nan(l_run)), 0)) {
       // Infinite values: with two products per key they give NaN.  Once more, relative to the maximum: the rest meets the finite values only and a positive
       // probability does not round to 0.
       clear();
@@ -336,35 +315,28 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
         const Spot o = spot(t);
         load_k(z, o);
         load_v(z, o);
-        floatx4 s[BLOCKS][2];
+        floatx4 s[2];
+        u32x4 prob, rest;
         scores(z, s);
-        u32x4 prob[BLOCKS], rest[BLOCKS];
-#pragma unroll
-        for (int c = 0; c < BLOCKS; ++c) {
-          if (c > 0 && c >= n_blocks) break;
-          probabilities(s[c], t, c, prob[c], rest[c], true);
-        }
+        probabilities(s, t, prob, rest, true);
         add_values(z, t, prob, rest, true);
       }
-#pragma unroll
-      for (int c = 0; c < BLOCKS; ++c) l_run[c] = sum_over_quarters(l_run[c]);
+      l_run = sum_over_quarters(l_run);
     }
 
     // ---- the waves' states -> the unit's, or a part of it -----------------------------------------------
-#pragma unroll
-    for (int c = 0; c < BLOCKS; ++c) {
-      if (c > 0 && c >= n_blocks) break;
-      float* to_lds = states + (wave * kRows + 16 * c + c16) * kPitch;
+    {
+      float* to_lds = states + (wave * kRows + c16) * kPitch;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int j = 0; j < kDV; j += 4)
-          *reinterpret_cast<floatx4*>(to_lds + kDV * (4 * g + r) + j) = floatx4{acc[c][j][r], acc[c][j + 1][r], acc[c][j + 2][r], acc[c][j + 3][r]};
-      if (g == 0) *reinterpret_cast<floatx2*>(to_lds + D) = floatx2{m_run[c], l_run[c]};
+          *reinterpret_cast<floatx4*>(to_lds + kDV * (4 * g + r) + j) = floatx4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
+      if (g == 0) *reinterpret_cast<floatx2*>(to_lds + D) = floatx2{m_run, l_run};
     }
     __syncthreads();
     const bool begins = t0 == 0, ends = t1 == tiles;
-    for (int i = tid; i < 16 * n_blocks * (D / 4); i += 64 * kPrefixWaves) {
+    for (int i = tid; i < kRows * (D / 4); i += 64 * kPrefixWaves) {
       const int r = i / (D / 4), d = 4 * (i % (D / 4)), row = row0 + r;
       if (row >= rows) break;  // (rows ascend)
       float m = -INFINITY, l = 0.f, ms[kPrefixWaves];
@@ -710,11 +682,16 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
   find_skips(all, tid, kWideThreads);
 }
 
-// Rows of a unit, in blocks of 16: as many as a KV head's queries of a group fill on average, 16 or 32, or more where there are more.
-constexpr int kWide = kWideRows / 16;
-static int prefix_blocks(int batch, int n_q_heads, int n_kv_heads, int n_groups) {
+// Rows of a unit, by how many rows of a KV head a group has on average: 16, whose keys need no turn through LDS, or 128, which share what they read.  Up to 16 rows 16 cost less, between 16 and
+// 32 with heads of 64 too, where products are cheap next to what a work-group begins and ends with.  A step of one group, 100 keys of their own, 16 and 128 rows to a unit:
+//   32/8 heads of 128: 4 sequences (16 rows) behind 8192 keys 27.2 and 31.2 us, behind 32768 41.0 and 43.7; 8 (32 rows) 30.1 and 31.5, 57.0 and 44.1; 16 (64 rows) 33.4 and 31.5, 90.7 and 45.3
+//   28/4 of 128: 2 (14 rows) 28.2 and 33.0, 41.1 and 42.5; 3 (21 rows) 29.4 and 33.3, 44.0 and 42.6; 6 (42 rows) 28.6 and 34.7, 51.5 and 43.8
+//   32/8 of 64: 4 (16 rows) 22.0 and 24.1, 29.0 and 31.8; 8 (32 rows) 24.1 and 24.2, 34.6 and 32.2; 16 (64 rows) 26.2 and 24.7, 46.6 and 32.4
+//   14/2 of 64: 4 (28 rows) 22.6 and 25.9, 29.4 and 32.9; 8 (56 rows) 23.8 and 26.1, 30.5 and 33.6; 16 (112 rows) 25.4 and 26.5, 36.7 and 35.2
+// (32 rows in two blocks of 16 gave 30.9 and 44.0 with 32/8 heads of 128, 24.6 and 34.1 with 32/8 of 64: nothing that one of the two does not.)
+static int unit_rows(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups) {
   const int64_t rows = (int64_t)batch * (n_q_heads / n_kv_heads) / n_groups;
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : kWide;
+  return rows <= (head_dim == 64 ? 32 : 16) ? 16 : kWideRows;
 }
 
 // Where the keys and values of all sequences fit the caches, as much as the table has room for, what sequences share is there after the first one's read, and the steps of the others cost less than
@@ -727,27 +704,21 @@ bool paged_prefix_pays(int batch, int n_kv_heads, int head_dim, int page_size, i
   return (double)batch * max_pages * page_size * n_kv_heads * head_dim * 4 > 256e6;
 }
 
-int paged_prefix_part_rows(int batch, int n_q_heads, int n_kv_heads, int n_groups) { return 16 * prefix_blocks(batch, n_q_heads, n_kv_heads, n_groups); }
+int paged_prefix_part_rows(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups) { return unit_rows(batch, n_q_heads, n_kv_heads, head_dim, n_groups); }
 
 PagedScratch paged_prefix_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups) {
-  const int blocks = prefix_blocks(batch, n_q_heads, n_kv_heads, n_groups);
-  const size_t rows = (size_t)kPrefixShares * 2 * 16 * blocks;
+  const int each = unit_rows(batch, n_q_heads, n_kv_heads, head_dim, n_groups);
+  const size_t rows = (size_t)kPrefixShares * 2 * each;
   PagedScratch s = {0, 0, 0, 0};
-  s.parts = s.stats + rows * (blocks == kWide ? 16 : 8);  // (a row's statistics are there twice, once for each of its lanes)
+  s.parts = s.stats + rows * (each == kWideRows ? 16 : 8);  // (a row's statistics are there twice, once for each of its lanes)
   s.total = s.parts + rows * head_dim * 4;
   return s;
 }
 
-template <typename T, int D, int BLOCKS>
-static void launch_paged_prefix_for(const PagedPrefixArgs& a, hipStream_t stream) {
-  constexpr size_t lds = (size_t)kPrefixWaves * 16 * BLOCKS * (D + 4) * 4;
-  hipLaunchKernelGGL((paged_prefix_kernel<T, D, BLOCKS>), dim3(kPrefixShares), dim3(64 * kPrefixWaves), lds, stream, a);
-}
 template <typename T, int D>
 static hipError_t launch_paged_prefix_of(const PagedPrefixArgs& a, hipStream_t stream) {
-  const int blocks = prefix_blocks(a.step.batch, a.step.n_q_heads, a.step.n_kv_heads, a.n_groups);
-  if (blocks == 1) launch_paged_prefix_for<T, D, 1>(a, stream);
-  else if (blocks == 2) launch_paged_prefix_for<T, D, 2>(a, stream);
+  if (unit_rows(a.step.batch, a.step.n_q_heads, a.step.n_kv_heads, D, a.n_groups) != kWideRows)
+    hipLaunchKernelGGL((paged_prefix_kernel<T, D>), dim3(kPrefixShares), dim3(64 * kPrefixWaves), 0, stream, a);
   else hipLaunchKernelGGL((paged_prefix_wide_kernel<T, D>), dim3(kPrefixShares), dim3(kWideThreads), 0, stream, a);
   return hipGetLastError();
 }

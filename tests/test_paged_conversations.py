@@ -306,9 +306,9 @@ def _roomy(s):
 
 
 def _shared_close(out, q, s, scale, n_groups):
-    """What :func:`_close` asks for, and where more than 32 rows share a prefix the rounding of probabilities."""
+    """What :func:`_close` asks for, and where more than 16 rows (32 with heads of 64) share a prefix the rounding of probabilities."""
     group = q.shape[1] // s.hkv
-    if q.shape[0] * group // n_groups <= 32:
+    if q.shape[0] * group // n_groups <= (32 if s.d == 64 else 16):
         return _close(out, q, s, scale)
     for b in range(q.shape[0]):
         for h in range(s.hkv):
