@@ -194,7 +194,7 @@ __device__ __forceinline__ uint32_t over_rows(uint32_t x, F f) {
 constexpr int kMoveThreads = 512, kMoveRows = kMoveThreads / kPieces;  // side by side
 constexpr int kMoveEach = 256 / kMoveRows, kMoveChunk = kMoveEach * kMoveRows;   // where there are several groups, whose rows are a multiple of it
 
-// A (sequence, KV head) and what of its rows this work-group has: 64 channels of keys or of values.
+// A (sequence, KV head) and what of its rows this work-group has: a slice of keys or of values.
 struct MoveSlice {
   int b, kvh;
   int64_t unit;      // its first entry of p.kept
@@ -382,12 +382,15 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const PagedEvi
   }
 }
 
-// Rows of a group: all of them where that makes work-groups enough, or as few as make so many.
-constexpr int kMoveEnough = 256;
+// Rows of a group: all of them where that makes work-groups enough, one for each compute unit, or as few as make four times that (256 rows at least).  A step that gives up 64 keys of 4160, in turn
+// and in groups: 1 sequence with 8 KV heads of 128 (64 slices) 39.5 and 25.4 us, 2 (128) 41.4 and 31.1 (36.7 with groups for 256), 4 (256) 44.0 and 45.9, 8 (512) 49.4 and 62.2; of
+// heads of 64: 1 39.1 and 21.2, 4 (128) 41.5 and 33.5, 8 (256) 43.6 and 44.9.  232 keys of 33000: 1 with 8 of 128 256 and 99, 2 273 and 174, 4 338 and 314, 8 439 and 540.
+constexpr int kMoveEnough = 256, kMoveSpread = 1024;
 int paged_evict_group_rows(int batch, int n_kv_heads, int head_dim, int n_keys) {
   const int64_t slices = (int64_t)batch * n_kv_heads * 2 * (head_dim / kSlice);
   const int chunks = (n_keys + kMoveChunk - 1) / kMoveChunk;
-  const int64_t groups = std::min<int64_t>((kMoveEnough + slices - 1) / slices, chunks);
+  if (slices >= kMoveEnough) return chunks * kMoveChunk;
+  const int64_t groups = std::min<int64_t>((kMoveSpread + slices - 1) / slices, chunks);
   return (int)((chunks + groups - 1) / groups) * kMoveChunk;
 }
 
