@@ -8,7 +8,9 @@
 // of few KV heads or large pages had too few work-groups: 6001 tokens, 14/2 heads of 64, pages of 64 48 us, of 256 47; 21 and 18 so.)
 //
 // Measured: a token of each of 96 sequences, 28/4 heads of 128, bf16 4.5 us, the launch and a chain of three loads; a prompt of 6001, 32/8 of 64, fp16 16.0 us, 4.8
-// TB/s; six prompts of 700 to 21000 tokens, 32/8 of 128, bf16 205 us, 5.1 TB/s, where a copy reaches 5.2.
+// TB/s; six prompts of 700 to 21000 tokens, 32/8 of 128, bf16 205 us, 5.1 TB/s, where a copy reaches 5.2.  With norms (MORE), which need a head's squares summed over its lanes before its
+// first product and its weights beside its angles: the same prompt 18.6 us a step, six prompts of 28/4 of 128 169 us, 4.9 TB/s, a token 4.7 us.  Norms in a launch of their own would read and
+// write queries and keys once more.
 #include "aa_kernels.h"
 #include "aa_paged.h"
 

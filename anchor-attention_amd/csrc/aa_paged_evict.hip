@@ -8,6 +8,9 @@
 // Moving is bound by reading and writing the rows once.  It is in place, and rows go to lower places in their order, so a work-group that takes them in turn, each chunk read by all before
 // any of it is written, needs no room beside: no later row lies where an earlier one goes.  A work-group has 32 channels of keys or values; where that makes too few
 // work-groups, the rows of a (sequence, KV head) are cut into groups, and those that come from another group's places are copied to scratch by a launch of its own first.
+//
+// Measured: 8 sequences of 3000 to 33000 keys down to 4096, 8 KV heads of 128, 92 us a step: choosing 25.4, as long as one work-group takes for the longest, moving 53.7, 4.4
+// TB/s; one of 4160 keys, 8 of 64, 21 us: choosing 8.4, saving 3.5, moving 9.0, chains of loads all three.  (Slices of 64 channels: moving 60.)
 #include <algorithm>
 
 #include "aa_kernels.h"
