@@ -1170,6 +1170,11 @@ int aa_paged_evict(const aa_paged_cache* cache, const aa_paged_eviction* t, void
     set_error("%s: workspace has %zu bytes, %zu needed", who, t->workspace_bytes, needed);
     return AA_EBADARG;
   }
+  const int64_t between = ((intptr_t)t->new_lengths - (intptr_t)t->lengths) / 4;
+  if (between > -t->batch && between < t->batch) {  // (which is read until the last key has been moved)
+    set_error("%s: new_lengths and lengths share memory", who);
+    return AA_EBADARG;
+  }
   char* ws = static_cast<char*>(t->workspace);
   const PagedEvictArgs a = {(uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn, (uint16_t*)cache->values, cache->vp_sp, cache->vp_sh, cache->vp_sn,
                             (uint16_t*)cache->bounds, t->weights, t->page_table, t->pt_sb, t->lengths, t->new_lengths, t->kept, (uint16_t*)ws,

@@ -102,6 +102,26 @@ def test_append_with_norms(before, new, gone, hq, hkv, d, page, layout, padding,
 
 
 @pytest.mark.gpu
+def test_a_cache_with_weights_is_copied_and_appended_to_without_angles():
+    """Copies have weights of their own; keys that are rotated already set theirs to 0 and nobody else's; what the cache holds is what was given."""
+    import copy
+    s = _Setup([20, 0, 33], 2, 64, 16, BF16, 31)
+    s.cache = _weights_of(s)
+    s.cache.weights.fill_(3.0)
+    other = copy.deepcopy(s.cache)
+    assert torch.equal(other.weights, s.cache.weights) and other.weights.data_ptr() != s.cache.weights.data_ptr()
+    k, v = (torch.randn(7, 2, 64, device="cuda").to(BF16) for _ in range(2))
+    _ops().append_to_pages(other, None, k, v, None, None, s.table, s.lengths, _int32([0, 4, 4, 7]))
+    new = [(0, 16 + i, i) for i in range(4)] + [(2, 30 + i, 4 + i) for i in range(3)]
+    want = torch.full_like(other.weights, 3.0)
+    for b, place, t in new:
+        page = int(s.table[b, place // 16])
+        want[page, :, place % 16] = 0.0
+        assert torch.equal(other.keys[page, :, place % 16], k[t]) and torch.equal(other.values[page, :, place % 16], v[t])
+    assert torch.equal(other.weights, want) and bool((s.cache.weights == 3.0).all())
+
+
+@pytest.mark.gpu
 def test_positions_that_angles_do_not_reach():
     """Tokens behind the angles are left out, and all of a sequence that has had fewer positions than it has keys."""
     ops = _ops()
@@ -340,6 +360,10 @@ def _shared_close(out, q, s, scale, n_groups):
     ([2] * 90, [3] * 90, [5, 1, 20], 4, 1, 64, 32, "heads", 0, [7] * 5),
     ([1, 4096], [1, 2], [33], 4, 2, 64, 16, "heads", 0, []),
     ([0, 0, 3], [2, 0, 2], [9], 4, 2, 64, 16, "heads", 0, []),
+    ([3, 2, 5] * 40, [2, 0, 1] * 40, [9, 0], 4, 2, 64, 16, "heads", 0, [3]),
+    ([70], [32], [20, 0, 3], 32, 8, 128, 64, "heads", 0, []),
+    ([70], [33], [20, 0, 3], 32, 8, 128, 64, "heads", 0, [5]),
+    ([1], [300], [1], 1, 1, 128, 256, "heads", 0, []),
 ])
 def test_shared_decode(prefixes, sizes, own, hq, hkv, d, page, layout, extra, alone, dtype):
     s, shared, groups = _shared_setup(prefixes, sizes, own, hkv, d, page, dtype, hq + page, layout, extra, alone)
@@ -600,7 +624,7 @@ def test_evict_without_bounds_and_of_what_does_not_fit():
         assert all(torch.equal(t[i], u[i]) for i in range(cache.n_pages) if i not in written)
 
 
-EVICTION = {"page_table": 4096, "pt_sb": 8, "lengths": 4096, "new_lengths": 4096, "kept": 4096, "weights": 4096, "workspace": 4096, "workspace_bytes": 1 << 40, "batch": 2, "max_pages": 100,
+EVICTION = {"page_table": 4096, "pt_sb": 8, "lengths": 4096, "new_lengths": 8192, "kept": 4096, "weights": 4096, "workspace": 4096, "workspace_bytes": 1 << 40, "batch": 2, "max_pages": 100,
             "n_keys": 1000, "n_first": 2, "n_last": 3, "above": 1200}
 
 
@@ -609,7 +633,7 @@ EVICTION = {"page_table": 4096, "pt_sb": 8, "lengths": 4096, "new_lengths": 4096
     ({"new_lengths": 0}, "new_lengths is NULL"), ({"kept": 0}, "kept is NULL"), ({"kept": 6}, "kept must be 4-byte"), ({"workspace": 0}, "workspace is NULL"), ({"workspace_bytes": 100}, "workspace has 100 bytes"),
     ({"n_keys": 0}, "not supported"), ({"n_keys": 4}, "not supported"), ({"n_first": -1}, "not supported"), ({"n_last": -1}, "not supported"), ({"n_first": 998}, "not supported"),
     ({"n_first": 2 ** 31 - 1, "n_last": 2 ** 31 - 1}, "not supported"), ({"above": 999}, "not supported"), ({"n_keys": (1 << 20) + 1, "above": 1 << 21}, "not supported"),
-    ({"batch": 65535, "n_kv_heads": 512, "kp_sh": 128}, "2\\^24"),
+    ({"batch": 65535, "n_kv_heads": 512, "kp_sh": 128}, "2\\^24"), ({"new_lengths": 4096}, "share memory"), ({"new_lengths": 4092}, "share memory"),
 ])
 def test_what_the_c_interface_of_eviction_refuses(change, message):
     """Before anything is launched: the addresses are never read."""
