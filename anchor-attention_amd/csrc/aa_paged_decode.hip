@@ -680,15 +680,20 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArg
 // so many of its parts.  Heads lie beside one another in a wave as they do in the parts of many rows, and fours of channels as in the others.  Bound by the latency of what it
 // reads, each thing known by the one before (cut, unit, parts): 32 sequences behind 32768 keys, 32/8 heads of 128 (256 work-groups of 32 parts) 8.6 us, of the step's 60.  (The prefix joined
 // by a launch of its own, before the decode kernel, which read its state: 61.3 a step.  A head's channels side by side in a wave: 9.7 us.)
+// A line of many rows' parts has heads of two sequences, which should be one XCD's: neighbours are where an XCD's share is consecutive, or, of 8 units a sequence, where each has its own
+// (128 sequences, 28/4 heads of 128, in plain order 47.8 us a step, so 46.2; 32, 32/8 of 128, 59.4 and 59.7).
+constexpr int kXcds = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_finish_kernel(const PagedDecodeArgs p) {
   constexpr int kLanes = D / 4, kHeads = 256 / kLanes, kFours = D / 8;
   __shared__ floatx4 sums[256];
   __shared__ floatx2 stats[256];
   const int group = p.n_q_heads / p.n_kv_heads, col_blocks = (group + kCols - 1) / kCols, units = p.n_kv_heads * col_blocks, tid = threadIdx.x;
-  const int b = blockIdx.x / units, unit = blockIdx.x - b * units, kvh = col_blocks == 1 ? unit : unit / col_blocks;
+  const int at = units % kXcds == 0 ? blockIdx.x : blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+  const int b = at / units, unit = at - b * units, kvh = col_blocks == 1 ? unit : unit / col_blocks;
+  if (b >= p.batch) return;
   const int head0 = kvh * group + (unit - kvh * col_blocks) * kCols, n_cols = min(kCols, (kvh + 1) * group - head0);
-  const const_i32* cut = (const_i32*)p.cuts + 2 * (int64_t)blockIdx.x;
+  const const_i32* cut = (const_i32*)p.cuts + 2 * ((int64_t)b * units + unit);
   const int skip = ((const_i32*)p.skips)[b], of_group = ((const_i32*)p.firsts)[b], first = cut[0], parts = cut[1];
   if (skip == 0 && parts == 0) return;  // (the decode kernel's own)
   int heads_log = 0;
@@ -850,7 +855,7 @@ static void launch_paged_decode_as(const PagedDecodeArgs& a, hipStream_t stream)
     const int side = (int)(room < each ? room : each), combiners = a.headers != nullptr ? kShares * cols : 0;
     hipLaunchKernelGGL((paged_weigh_kernel<T, D>), dim3((uint32_t)(combiners + side * all)), dim3(256), 0, stream, a, combiners, cols, side);
   } else if constexpr (MODE == kShared) {
-    hipLaunchKernelGGL((paged_finish_kernel<T, D>), dim3((uint32_t)((int64_t)a.batch * units)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((paged_finish_kernel<T, D>), dim3(((uint32_t)((int64_t)a.batch * units) + kXcds - 1) / kXcds * kXcds), dim3(256), 0, stream, a);
   } else {
     if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D, MODE>), dim3(cols, kShares), dim3(256), 0, stream, a);
   }
