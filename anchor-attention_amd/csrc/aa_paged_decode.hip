@@ -99,12 +99,17 @@ __device__ __forceinline__ void add_to_weights(const PagedDecodeArgs& p, const i
   const int page = p.table[b * p.t_sb + (i >> p.page_log)];
   if ((uint32_t)page >= (uint32_t)p.n_pages) return;  // (what is read in its place is another sequence's)
   float* w = p.weights + (((int64_t)page * p.n_kv_heads + kvh) << p.page_log) + (i & ((1 << p.page_log) - 1));
-  floatx4 old = *reinterpret_cast<const floatx4*>(w);
+  const floatx4 old = *reinterpret_cast<const floatx4*>(w);
+  if (i >= p.n_first && i + 3 < n) {
+    *reinterpret_cast<floatx4*>(w) = floatx4{old[0] + sum[0], old[1] + sum[1], old[2] + sum[2], old[3] + sum[3]};
+    return;
+  }
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (i + e < n && i + e >= p.n_first) old[e] += sum[e];
-  *reinterpret_cast<floatx4*>(w) = old;
+  for (int e = 0; e < 4; ++e)  // (what is not this sequence's to count is not written, not even as it was)
+    if (i + e < n && i + e >= p.n_first) w[e] = old[e] + sum[e];
 }
+// the first four keys of n that has any to count
+__device__ __forceinline__ int first_counted(const PagedDecodeArgs& p, const int n) { return min(p.n_first, n) & ~3; }
 
 template <typename T, int D, int WAVES, typename Place, DecodeMode MODE>
 __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const PagedDecodeArgs p) {
@@ -420,7 +425,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       if constexpr (MODE == kWeigh) {
         const int room = p.max_pages << p.page_log;
         float* to = p.scores + ((int64_t)f.b * p.n_q_heads + head0 + c16) * room + kTile * t + 4 * g;
-        if (c16 < n_cols) {
+        if (c16 < n_cols && kTile * (t + 1) > p.n_first) {
           *reinterpret_cast<floatx4*>(to) = s[0];
           if (kTile * t + 16 < room) *reinterpret_cast<floatx4*>(to + 16) = s[1];
         }
@@ -478,7 +483,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       const float inv = length == 0 ? 0.f : 1.f / l_run;  // (no keys: 0; keys whose scores are all minus infinity: 0 / 0, as a soft-max has it)
       if (MODE == kWeigh && weighs) {  // (this wave's own scores, which it has stored)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        for (int i = 4 * lane; i < length; i += 256) {
+        for (int i = first_counted(p, length) + 4 * lane; i < length; i += 256) {
           floatx4 sum = {0.f, 0.f, 0.f, 0.f};
           add_probabilities<T>(p, (int64_t)f.b * p.n_q_heads + head0, n_cols, i, scale, sum, [&](const int h) {
             return floatx2{__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m_run), h)), 1.f / __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l_run), h))};
@@ -593,7 +598,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     if (MODE == kWeigh && weighs) {
       __syncthreads();  // (all waves have stored their scores before the parts were joined)
       const int n = keys_of<MODE>(p, info.y, ((const_i32*)p.lengths)[info.y]);
-      for (int i = 4 * tid; i < n; i += 256 * WAVES) {
+      for (int i = first_counted(p, n) + 4 * tid; i < n; i += 256 * WAVES) {
         floatx4 sum = {0.f, 0.f, 0.f, 0.f};
         add_probabilities<T>(p, (int64_t)info.y * p.n_q_heads + head0, n_cols, i, scale, sum, [&](const int h) { return unit_totals[h]; });
         add_to_weights(p, info.y, head0 / group, i, n, sum);
@@ -794,7 +799,7 @@ __global__ void __launch_bounds__(256) paged_weigh_kernel(const PagedDecodeArgs 
   const int group = p.n_q_heads / p.n_kv_heads, col_blocks = (group + kCols - 1) / kCols, n = keys_of<kWeigh>(p, b, p.lengths[b]);
   const int64_t head0 = (int64_t)b * p.n_q_heads + (int64_t)kvh * group;
   const float scale = p.sm_scale * kLog2e;
-  const int first = (at - u * side) * 1024;
+  const int first = first_counted(p, n) + (at - u * side) * 1024;
   if (first >= n) return;
   auto find_totals = [&](const int block) {  // of its heads: maxima, and what probabilities are multiplied by
     const int2 cut = *reinterpret_cast<const int2*>(p.cuts + 2 * ((int64_t)u * col_blocks + block));

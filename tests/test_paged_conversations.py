@@ -263,6 +263,54 @@ def test_weighing_decode(lengths, hq, hkv, d, page, layout, extra, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n_first", [1, 3, 4, 15, 33, 1023, 1025, 4999, 5000, 5001, 2 ** 31 - 1])
+@pytest.mark.parametrize("lengths", [[5000], [700, 5000, 0, 3]])
+def test_weighing_from_some_key_on(lengths, n_first):
+    """Keys before n_first and rows behind the last key keep their weights; one short table and one whose steps are cut and joined."""
+    s = _Setup(lengths, 2, 64, 16, BF16, 9, extra=1)
+    s.cache = _weights_of(s)
+    q, before = s.queries(8), s.cache.weights.clone()
+    out = _ops().paged_weighing_decode_attention(s.cache, q, s.table, s.lengths, n_first=n_first)
+    _close(out, q, s, 0.125)
+    _weights_close(s.cache.weights, before, q, s, 0.125, n_first)
+    short = min(lengths[0], 700)
+    s.host = [short] + [0] * (len(lengths) - 1)
+    before = s.cache.weights.clone()
+    out = _ops().paged_weighing_decode_attention(s.cache, q, s.table[:, :44], _int32(s.host), n_first=n_first)
+    _close(out, q, s, 0.125)
+    _weights_close(s.cache.weights, before, q, s, 0.125, n_first)
+
+
+@pytest.mark.gpu
+def test_pages_far_into_a_large_pool():
+    """Pages whose keys lie more than 2^32 bytes into the pool: every operator, the same bits as of the same pages in a small one."""
+    ops = _ops()
+    s = _Setup([300, 170, 300], 8, 128, 64, BF16, 12, room=10)
+    s.table[1, :2] = s.table[0, :2]
+    s.table[s.table < 0] = 0
+    s.cache = _weights_of(s)
+    far = 34000 - s.cache.n_pages
+    big = ops.PagedCache.empty(34000, 8, 64, 128, weights=True)
+    assert big.keys[far:].data_ptr() - big.keys.data_ptr() > 1 << 32
+    for a, b in ((big.keys, s.cache.keys), (big.values, s.cache.values), (big.bounds, s.cache.bounds), (big.weights, s.cache.weights)):
+        a[far:] = b
+    wq, wk = (1 + torch.randn(128, device="cuda") / 4).to(BF16), (1 + torch.randn(128, device="cuda") / 4).to(BF16)
+    cos, sin = _tables(400, 128)
+    q, k, v = (torch.randn(3, h, 128, device="cuda").to(BF16) for h in (32, 8, 8))
+    results = []
+    for cache, table in ((s.cache, s.table), (big, (s.table.long() + far).clamp(max=33999).int())):
+        lengths, roomy = s.lengths + 1, _roomy(s)
+        roomy[:, :table.shape[1]] = table
+        rotated = ops.append_to_pages(cache, q, k, v, cos, sin, table, lengths, q_norm=wq, k_norm=wk, positions=lengths + 3)
+        shared = ops.paged_shared_decode_attention(cache, rotated, roomy, lengths, _int32([2]), _int32([0, 2]))
+        counted = ops.paged_weighing_decode_attention(cache, rotated, table, lengths, n_first=128)
+        new, kept = ops.evict_from_pages(cache, table, lengths, 160, n_first=128, n_last=4)
+        here = slice(far if cache is big else 0, None)
+        results.append([rotated, shared, counted, new, kept, *(t[here].nan_to_num(9.0) for t in (cache.keys, cache.values, cache.bounds, cache.weights))])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.gpu
 def test_weighing_scores_that_are_infinite_or_nan():
     """A key of minus infinity has no weight, a sequence whose scores are all of it or one of which is NaN or plus infinity NaN where its heads are, and no other."""
     s = _Setup([700, 40, 40, 40, 300], 2, 64, 16, BF16, 9)
