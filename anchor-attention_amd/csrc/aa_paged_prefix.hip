@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     u32x4 prob[4];
     // What a team multiplies of a round: operand f is of values or, from kValues on, of the next tile's keys.  Operands are read from LDS
     // kAhead ahead of the products that take them, in this order, which the compiler would not keep; the first ones before the barrier.
-    constexpr int kAhead = D == 128 ? 6 : 6, kValues = 4 * kDB, kKeys = 2 * kKS;
+    constexpr int kAhead = 6, kValues = 4 * kDB, kKeys = 2 * kKS;
     u32x4 operand[kAhead];
     auto read = [&](const int i, const int f) __attribute__((always_inline)) {  // of values of tile i, keys of tile i + 1
       if (f < kValues) {
