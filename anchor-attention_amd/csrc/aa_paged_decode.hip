@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
   // States of units that a wave has a part of only: [wave][0: the first of its units, which began before; 1: its last, which goes on][column]
   extern __shared__ __attribute__((aligned(16))) float states[];
   __shared__ float stats[WAVES][2][2][kCols];
-  __shared__ floatx2 unit_totals[MODE == kWeigh ? kCols : 1];
+  __shared__ floatx2 unit_totals[MODE == kWeigh ? kCols : 1], wave_totals[MODE == kWeigh ? WAVES : 1][kCols];
   __shared__ int4 parts_of[WAVES][2];  // 0 if there is none, 2 if the unit ends in it; sequence; first head, and columns in the upper half; parts of work-groups
 
   const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
@@ -482,12 +482,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
       }
       const float inv = length == 0 ? 0.f : 1.f / l_run;  // (no keys: 0; keys whose scores are all minus infinity: 0 / 0, as a soft-max has it)
       if (MODE == kWeigh && weighs) {  // (this wave's own scores, which it has stored)
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (g == 0) wave_totals[wave][c16] = floatx2{m_run, 1.f / l_run};
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         for (int i = first_counted(p, length) + 4 * lane; i < length; i += 256) {
           floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-          add_probabilities<T>(p, (int64_t)f.b * p.n_q_heads + head0, n_cols, i, scale, sum, [&](const int h) {
-            return floatx2{__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m_run), h)), 1.f / __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l_run), h))};
-          });
+          add_probabilities<T>(p, (int64_t)f.b * p.n_q_heads + head0, n_cols, i, scale, sum, [&](const int h) { return wave_totals[wave][h]; });
           add_to_weights(p, f.b, u.kvh, i, length, sum);
         }
       }
