@@ -609,17 +609,17 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_decode_kernel(const Paged
     }
     if (begins && !ends) {  // the unit's other parts are the next work-groups'
       goes_on = true;
-      if (tid == 0) *header = int4{info.w, info.y, head0, n_cols};
+      if (MODE != kShared && tid == 0) *header = int4{info.w, info.y, head0, n_cols};
     }
   }
-  if (!goes_on && tid == 0 && p.headers != nullptr) header->x = 0;
+  if (MODE != kShared && !goes_on && tid == 0 && p.headers != nullptr) header->x = 0;
 }
 
 // Joins the parts of a column whose unit begins in share blockIdx.y and ends in another (units begin every so many shares: shares as blockIdx.x would be one XCD's): the
 // weights first, then groups of D / 4 lanes add up
 // every so many parts.  Few bytes; the launch and three loads one after the other take 3 to 5 us, which a step pays whether or not a unit was cut, since the
 // host does not know the lengths.
-template <typename T, int D, DecodeMode MODE>
+template <typename T, int D>
 __device__ __forceinline__ void combine(const PagedDecodeArgs& p, const int col, const int share) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
   __shared__ float weight[256], red[2][4];
@@ -675,9 +675,9 @@ __device__ __forceinline__ void combine(const PagedDecodeArgs& p, const int col,
     *reinterpret_cast<u32x2*>(op) = u32x2{T::pack(sum[0] * inv, sum[1] * inv), T::pack(sum[2] * inv, sum[3] * inv)};
   }
 }
-template <typename T, int D, DecodeMode MODE>
+template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArgs p) {
-  combine<T, D, MODE>(p, blockIdx.x, blockIdx.y);
+  combine<T, D>(p, blockIdx.x, blockIdx.y);
 }
 
 // Joins what is known of a unit's heads over the shared prefix and over the sequence's own keys, each whole or in parts.  256 threads have four channels of a head each; of few heads, every
@@ -792,7 +792,7 @@ __global__ void __launch_bounds__(256) paged_weigh_kernel(const PagedDecodeArgs 
   __shared__ floatx2 parts_of[16][kCols], totals[kCols];
   if ((int)blockIdx.x < combiners) {
     const int share = blockIdx.x / cols;
-    return combine<T, D, kWeigh>(p, blockIdx.x - share * cols, share);
+    return combine<T, D>(p, blockIdx.x - share * cols, share);
   }
   const int tid = threadIdx.x, at = blockIdx.x - combiners, u = at / side, b = u / p.n_kv_heads, kvh = u - b * p.n_kv_heads;
   const int group = p.n_q_heads / p.n_kv_heads, col_blocks = (group + kCols - 1) / kCols, n = keys_of<kWeigh>(p, b, p.lengths[b]);
@@ -861,7 +861,7 @@ static void launch_paged_decode_as(const PagedDecodeArgs& a, hipStream_t stream)
   } else if constexpr (MODE == kShared) {
     hipLaunchKernelGGL((paged_finish_kernel<T, D>), dim3(((uint32_t)((int64_t)a.batch * units) + kXcds - 1) / kXcds * kXcds), dim3(256), 0, stream, a);
   } else {
-    if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D, MODE>), dim3(cols, kShares), dim3(256), 0, stream, a);
+    if (a.headers != nullptr) hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3(cols, kShares), dim3(256), 0, stream, a);
   }
 }
 
