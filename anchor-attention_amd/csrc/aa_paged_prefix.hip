@@ -384,8 +384,9 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
 //
 // Measured: 32 sequences behind 32768 keys, 32/8 heads of 128, bf16 30.1 us, 134 MB at 4.5 TB/s and 17 GFLOP; 128 behind 8000, 28/4 of 128, fp16 26.8 us, 548 TFLOP/s at the 1.5 to 1.6 GHz
 // that matrix work leaves this card.  A half of a tile that multiplies takes 1300 to 1800 cycles, of which 1152 are products, one that forms probabilities 1500.
-// (Probabilities as two 16-bit numbers: 1.48 us a tile instead of 1.05.  Their sums by vector additions: 5 % more.  A maximum known before the probabilities are formed: 49.2 us a step of 128
-// instead of 48.4.  Extents, kWideOver, that count 0, 5, 16 and 24 tiles beside a unit's own: 53.5, 51.8, 49.5 and 50 us instead of 48.3.)
+// A probability enters as two 16-bit numbers, its rounding and the rest, as in the decode kernel, so that a step has the same precision however many sequences share its pages.  It costs
+// half as many products again; the listed sizes of perf/more_operators.py take 59.1, 50.7 and 66.6 us a step, 53.1, 46.6 and 60.3 with the rounding alone.  (Sums by products with ones, a
+// product more for each of the two: 59.6, 51.0, 68.5.)
 constexpr int kWideTile = 64, kWideRows = 128, kWideThreads = 512, kWideLeast = 4, kWideOver = 10;
 
 template <int D>
@@ -485,22 +486,15 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
     };
-    // A probability is one 16-bit number, relative to a maximum that may be 2^kRoom below the row's: as precise above 1 as below.  fp16 forms 2^kProbLog2 of it, so that the largest fits and
-    // what falls below its smallest number, 2^-33 of the maximum, is 2^-13 of the sum for a million keys.
-    constexpr float kRoom = 6.f, kProbLog2 = T::kProbLog2 != 0.f ? 9.f : 0.f;
-    // (the sums of the probabilities as they were rounded, by products with ones: each of the sixteen is a row's)
-    float m_run = -INFINITY;
-    floatx16 acc[kDB], s[2], sums;
-    typename T::vec8 ones;
-    {
-      const uint32_t two = T::pack(1.f, 1.f);
-      const u32x4 all_ones = {two, two, two, two};
-      ones = *reinterpret_cast<const typename T::vec8*>(&all_ones);
-    }
-    u32x4 prob[4];
+    // A probability is two 16-bit numbers, as in the decode kernel, relative to a maximum that may be 2^kRoom below the row's: as precise above 1 as below, and of fp16, which has
+    // 2^kProbLog2 of it, 2^15.9 at most fits.
+    constexpr float kRoom = T::kProbLog2 != 0.f ? 0.9f : 6.f, kProbLog2 = T::kProbLog2;
+    float m_run = -INFINITY, l_run;  // (until the end a lane's sum is of its half of the keys)
+    floatx16 acc[kDB], s[2];
+    u32x4 prob[4], rest[4];
     // What a team multiplies of a round: operand f is of values or, from kValues on, of the next tile's keys.  Operands are read from LDS
     // kAhead ahead of the products that take them, in this order, which the compiler would not keep; the first ones before the barrier.
-    constexpr int kAhead = 6, kValues = 4 * kDB, kKeys = 2 * kKS;
+    constexpr int kAhead = 4, kValues = 4 * kDB, kKeys = 2 * kKS;
     u32x4 operand[kAhead];
     auto read = [&](const int i, const int f) __attribute__((always_inline)) {  // of values of tile i, keys of tile i + 1
       if (f < kValues) {
@@ -514,9 +508,18 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         operand[f % kAhead] = *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(((k_rd + ((i + 1) & 1) * kTileBytes) ^ ((g % kKS) << 5)) + 32 * (g / kKS) * kRowBytes);
       }
     };
-    auto multiply_values = [&](const int f) __attribute__((always_inline)) {
-      acc[f % kDB] = T::mfma(*reinterpret_cast<const typename T::vec8*>(&operand[f % kAhead]), *reinterpret_cast<const typename T::vec8*>(&prob[f / kDB]), acc[f % kDB]);
-      if (f % kDB == kDB - 1) sums = T::mfma(ones, *reinterpret_cast<const typename T::vec8*>(&prob[f / kDB]), sums);
+    auto multiply_values = [&](const int f, auto exact) __attribute__((always_inline)) {
+      u32x4 finite = operand[f % kAhead];
+      if constexpr (decltype(exact)::value) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if ((finite[i] & T::kExponent) == T::kExponent) finite[i] &= 0xffff0000u;
+          if (((finite[i] >> 16) & T::kExponent) == T::kExponent) finite[i] &= 0xffffu;
+        }
+      }
+      const auto p1 = *reinterpret_cast<const typename T::vec8*>(&prob[f / kDB]), p2 = *reinterpret_cast<const typename T::vec8*>(&rest[f / kDB]);
+      acc[f % kDB] = T::mfma(*reinterpret_cast<const typename T::vec8*>(&operand[f % kAhead]), p1, acc[f % kDB]);
+      acc[f % kDB] = T::mfma(*reinterpret_cast<const typename T::vec8*>(&finite), p2, acc[f % kDB]);
     };
     auto multiply_keys = [&](const int g) __attribute__((always_inline)) {
       floatx16 none;
@@ -533,6 +536,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
       }
       // 2^(s * scale - m * scale) with the maximum so far, m, before this tile's is known: only where that is larger by 2^kRoom it is taken up, and they are formed again
       auto form = [&](const float bias) __attribute__((always_inline)) {
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 16; ++w) {
           // (the fused product's second term is the same for all keys, so that its rounding cancels in the quotient)
@@ -543,10 +547,14 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
             if (e1 > 0.f && (both >> 16) == 0u) both |= 0x10000u;
           }
           prob[w >> 2][w & 3] = both;
+          rest[w >> 2][w & 3] = T::pack_rest(e0, e1, both);
+          sum[0] += e0;
+          sum[1] += e1;
         }
+        return sum[0] + sum[1];
       };
       const float bias = kProbLog2 - (m_run == -INFINITY ? 0.f : m_run) * scale;
-      form(bias);
+      float sum = form(bias);
       float mx[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
 #pragma unroll
       for (int r = 4; r < 32; ++r) mx[r & 3] = fmaxf(mx[r & 3], s[r >> 4][r & 15]);
@@ -555,19 +563,18 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         const float m_new = fmaxf(m_run, max_with_other_half(m_tile));
         const float m_base = m_new == -INFINITY ? 0.f : m_new;  // (no key of this row's so far)
         const float alpha = fast_exp2((m_run - m_base) * scale);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sums[r] *= alpha;
+        l_run *= alpha;
 #pragma unroll
         for (int db = 0; db < kDB; ++db)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
         m_run = m_new;
-        form(kProbLog2 - m_base * scale);
+        sum = form(kProbLog2 - m_base * scale);
       }
+      l_run += sum;
     };
     auto run = [&](auto exact) __attribute__((always_inline)) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sums[r] = 0.f;
+      l_run = 0.f;
 #pragma unroll
       for (int db = 0; db < kDB; ++db)
 #pragma unroll
@@ -592,7 +599,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         if (i > 0) {
 #pragma unroll
           for (int f = 0; f < kValues; ++f) {
-            multiply_values(f);
+            multiply_values(f, exact);
             read(i - 1, f + kAhead);
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -623,7 +630,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
       if (own > 0) {
 #pragma unroll
         for (int f = 0; f < kValues; ++f) {
-          multiply_values(f);
+          multiply_values(f, exact);
           if (f + kAhead < kValues) read(own - 1, f + kAhead);
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -634,6 +641,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
       }
       lds_barrier();
       if (team == 0) lds_barrier();
+      l_run += xor32(l_run);
     };
     run(std::false_type{});
     float sum = 0.f;
@@ -641,9 +649,8 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     for (int db = 0; db < kDB; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum += acc[db][r];
-    // Infinite values meet probabilities that were rounded to 0, or those relative to an earlier maximum.  Once more, relative to the last one: a positive probability does not round to 0.
-    if (__builtin_expect(__syncthreads_or(is_nan(sum) && !is_nan(sums[0])), 0)) run(std::true_type{});
-    const float l_run = sums[0];
+    // Infinite values: with two products per key they give NaN.  Once more, relative to the last maximum: the rest meets the finite values only and a positive probability does not round to 0.
+    if (__builtin_expect(__syncthreads_or(is_nan(sum) && !is_nan(l_run)), 0)) run(std::true_type{});
 
     // ---- the teams' states -> the unit's, or a part of it: fours of accumulators, lane by lane, half of them by each team ----
     floatx4* states = reinterpret_cast<floatx4*>(&tiles[0][0][0]) + wave * kFours * 64;
@@ -658,9 +665,8 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     };
     auto finish = [&](auto first) __attribute__((always_inline)) {
       const floatx2 other = stats[(1 - team) * 64 + lane];
-      constexpr float kBack = T::kProbLog2 - kProbLog2;  // (the decode kernel's factor)
-      const float m = fmaxf(m_run, other[0]), w = m_run == -INFINITY ? 0.f : fast_exp2((m_run - m) * scale + kBack);
-      const float w2 = other[0] == -INFINITY ? 0.f : fast_exp2((other[0] - m) * scale + kBack);
+      const float m = fmaxf(m_run, other[0]), w = m_run == -INFINITY ? 0.f : fast_exp2((m_run - m) * scale);
+      const float w2 = other[0] == -INFINITY ? 0.f : fast_exp2((other[0] - m) * scale);
       const float l = w * l_run + w2 * other[1];
 #pragma unroll
       for (int g = 0; g < kFours / 2; ++g) {

@@ -1,0 +1,46 @@
+"""Decode over a shared prefix in tables with room for gigabytes, where the kernels for shared pages run: whatever the number of sequences that share, the tolerances are those of
+a plain step, as tests/test_paged_cache.py derives them (a probability is kept as two 16-bit numbers)."""
+import pytest
+import torch
+
+from test_paged_cache import BF16, F16, _close, _ops, _Setup
+from test_paged_conversations import _int32, _shared_setup
+
+
+def _wide_table(s, keys_and_values=1_000_000_000):
+    """The setup's table with room for so many bytes of keys and values (zeros, which nothing reads), or for 2^20 keys a sequence."""
+    pages = min(keys_and_values // (s.table.shape[0] * s.cache.page_size * s.hkv * s.d * 4) + 1, (1 << 20) // s.cache.page_size)
+    return torch.cat([s.table, torch.zeros(s.table.shape[0], max(pages - s.table.shape[1], 0), dtype=torch.int32, device="cuda")], 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("prefixes,sizes,own,hq,hkv,d,page,layout,alone", [
+    ([40], [70], [17, 1, 0, 90], 28, 4, 128, 32, "part", []),
+    ([9, 13, 1], [40, 1, 30], [33, 64], 32, 8, 64, 256, "heads", [1]),
+    ([157], [33], [7, 1000], 8, 2, 128, 64, "heads", []),
+    ([70], [33], [20, 0, 3], 32, 8, 128, 64, "rows", [5]),
+    ([600], [9], [20], 71, 1, 64, 16, "heads", []),
+    ([313], [3], [2], 8, 2, 128, 64, "rows", [900]),
+])
+def test_shared_steps_are_as_precise_as_plain_ones(prefixes, sizes, own, hq, hkv, d, page, layout, alone, dtype):
+    s, shared, groups = _shared_setup(prefixes, sizes, own, hkv, d, page, dtype, hq + page, layout, 0, alone)
+    table, q = _wide_table(s), s.queries(hq)
+    for scale in (d ** -0.5, 0.3, 0.004):
+        _close(_ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, shared, groups, sm_scale=scale), q, s, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("batch,hq,hkv,d", [(40, 8, 2, 128), (40, 8, 2, 64), (2, 8, 2, 128)])
+def test_many_equal_keys_far_below_a_sink(batch, hq, hkv, d, dtype):
+    """A key of 16 to 20 nats more than the 4096 others, whose values are zeros: the output is what these have together.  (At 20 nats a probability of fp16, kept as 2^15 times itself on a
+    grid of 2^-24, is off by 2^-11.1 of it, which the rounding of scores, of up to 20, and of sums over 4096 keys covers.)"""
+    s, shared, groups = _shared_setup([64], [batch], [1], hkv, d, 64, dtype, 7)
+    s.cache.keys.zero_()
+    s.cache.values.fill_(64.0)
+    first = s.table[0, 0].long()
+    s.cache.keys[first, :, 0, 0], s.cache.values[first, :, 0] = 16.0, 0.0
+    q = torch.zeros(batch, hq, d, dtype=dtype, device="cuda")
+    q[:, :, 0] = torch.linspace(1.0, 1.25, batch * hq, device="cuda").view(batch, hq).to(dtype)
+    _close(_ops().paged_shared_decode_attention(s.cache, q, _wide_table(s), s.lengths, shared, groups, sm_scale=1.0), q, s, 1.0)
