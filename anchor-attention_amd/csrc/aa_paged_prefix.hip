@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
 // that matrix work leaves this card.  A half of a tile that multiplies takes 1300 to 1800 cycles, of which 1152 are products, one that forms probabilities 1500.
 // A probability enters as two 16-bit numbers, its rounding and the rest, as in the decode kernel, so that a step has the same precision however many sequences share its pages.  It costs
 // half as many products again; the listed sizes of perf/more_operators.py take 59.1, 50.7 and 66.6 us a step, 53.1, 46.6 and 60.3 with the rounding alone.  (Sums by products with ones, a
-// product more for each of the two: 59.6, 51.0, 68.5.)
+// product more for each of the two: 59.6, 51.0, 68.5.  Exponents as the decode kernel has them, (score - m) * scale, at all scores: 58.7, 50.6 and 68.3 instead of 58.0, 50.2 and 66.8.)
 constexpr int kWideTile = 64, kWideRows = 128, kWideThreads = 512, kWideLeast = 4, kWideOver = 10;
 
 template <int D>
@@ -486,9 +486,6 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
     };
-    // A probability is two 16-bit numbers, as in the decode kernel, relative to a maximum that may be 2^kRoom below the row's: as precise above 1 as below, and of fp16, which has
-    // 2^kProbLog2 of it, 2^15.9 at most fits.
-    constexpr float kRoom = T::kProbLog2 != 0.f ? 0.9f : 6.f, kProbLog2 = T::kProbLog2;
     float m_run = -INFINITY, l_run;  // (until the end a lane's sum is of its half of the keys)
     floatx16 acc[kDB], s[2];
     u32x4 prob[4], rest[4];
@@ -534,13 +531,28 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
         for (int r = 0; r < 32; ++r)
           if (key0 + 32 * (r >> 4) + 16 * ((r & 15) >> 3) >= length) s[r >> 4][r & 15] = -INFINITY;
       }
-      // 2^(s * scale - m * scale) with the maximum so far, m, before this tile's is known: only where that is larger by 2^kRoom it is taken up, and they are formed again
-      auto form = [&](const float bias) __attribute__((always_inline)) {
+      float mx[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+#pragma unroll
+      for (int r = 4; r < 32; ++r) mx[r & 3] = fmaxf(mx[r & 3], s[r >> 4][r & 15]);
+      const float m_new = fmaxf(m_run, max_with_other_half(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))));
+      const float m_base = m_new == -INFINITY ? 0.f : m_new;  // (no key of this row's so far)
+      if (__any(m_new > m_run)) {
+        const float alpha = fast_exp2((m_run - m_base) * scale);
+        l_run *= alpha;
+#pragma unroll
+        for (int db = 0; db < kDB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
+        m_run = m_new;
+      }
+      auto form = [&](auto near) __attribute__((always_inline)) {
+        const float bias = T::kProbLog2 - m_base * scale;
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 16; ++w) {
-          // (the fused product's second term is the same for all keys, so that its rounding cancels in the quotient)
-          const float e0 = fast_exp2(__builtin_fmaf(s[w >> 3][2 * (w & 7)], scale, bias)), e1 = fast_exp2(__builtin_fmaf(s[w >> 3][2 * (w & 7) + 1], scale, bias));
+          const float s0 = s[w >> 3][2 * (w & 7)], s1 = s[w >> 3][2 * (w & 7) + 1];
+          const float e0 = decltype(near)::value ? fast_exp2(__builtin_fmaf(s0, scale, bias)) : prob_exp2<T>(s0 - m_base, scale);
+          const float e1 = decltype(near)::value ? fast_exp2(__builtin_fmaf(s1, scale, bias)) : prob_exp2<T>(s1 - m_base, scale);
           uint32_t both = T::pack(e0, e1);
           if constexpr (decltype(exact)::value) {
             if (e0 > 0.f && (both & 0xffffu) == 0u) both |= 1u;
@@ -551,27 +563,11 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
           sum[0] += e0;
           sum[1] += e1;
         }
-        return sum[0] + sum[1];
+        l_run += sum[0] + sum[1];
       };
-      const float bias = kProbLog2 - (m_run == -INFINITY ? 0.f : m_run) * scale;
-      float sum = form(bias);
-      float mx[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
-#pragma unroll
-      for (int r = 4; r < 32; ++r) mx[r & 3] = fmaxf(mx[r & 3], s[r >> 4][r & 15]);
-      const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      if (__builtin_expect(__any(m_run == -INFINITY || __builtin_fmaf(m_tile, scale, bias) > kProbLog2 + kRoom), 0)) {
-        const float m_new = fmaxf(m_run, max_with_other_half(m_tile));
-        const float m_base = m_new == -INFINITY ? 0.f : m_new;  // (no key of this row's so far)
-        const float alpha = fast_exp2((m_run - m_base) * scale);
-        l_run *= alpha;
-#pragma unroll
-        for (int db = 0; db < kDB; ++db)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
-        m_run = m_new;
-        sum = form(kProbLog2 - m_base * scale);
-      }
-      l_run += sum;
+      // One fused operation a key, where the rounding of m * scale, which is in every probability as long as m is the maximum, is 2^-17 at most; elsewhere it would reach whole powers of two
+      if (__builtin_expect(__any(!(fabsf(m_base * scale) < 256.f)), 0)) form(std::false_type{});
+      else form(std::true_type{});
     };
     auto run = [&](auto exact) __attribute__((always_inline)) {
       l_run = 0.f;

@@ -44,3 +44,28 @@ def test_many_equal_keys_far_below_a_sink(batch, hq, hkv, d, dtype):
     q = torch.zeros(batch, hq, d, dtype=dtype, device="cuda")
     q[:, :, 0] = torch.linspace(1.0, 1.25, batch * hq, device="cuda").view(batch, hq).to(dtype)
     _close(_ops().paged_shared_decode_attention(s.cache, q, _wide_table(s), s.lengths, shared, groups, sm_scale=1.0), q, s, 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("times,scale", [(1, 30.0), (1, 1e3), (1, 1e6), (1, 1e7), (1, 1e9), (1, 1e20), (1, 1e29), (2.0 ** 9, 1.0), (2.0 ** 9, 1e6)])
+@pytest.mark.parametrize("batch,hq,hkv,d", [(40, 8, 2, 128), (40, 8, 2, 64), (2, 8, 2, 128)])
+def test_scores_far_apart(batch, hq, hkv, d, times, scale, dtype):
+    """Products of whole numbers, which float32 has exactly, with scales that leave no probability between 0 and those of the largest scores (e^-30 is below 2^-40): the output is the mean of
+    these keys' values, off by its own rounding, and by 2^-24 of what was added up for each sum, weight and quotient."""
+    s, shared, groups = _shared_setup([70], [batch], [1, 30, 100], hkv, d, 16, dtype, 11)
+    for t in (s.cache.keys, s.cache.values):
+        t.copy_(torch.randint(-4, 5, t.shape, generator=s.g, device="cuda"))
+    s.cache.keys.mul_(times)
+    q = (times * torch.randint(-4, 5, (batch, hq, d), generator=s.g, device="cuda")).to(dtype)
+    out = _ops().paged_shared_decode_attention(s.cache, q, _wide_table(s), s.lengths, shared, groups, sm_scale=scale)
+    u, group = torch.finfo(dtype).eps / 2, hq // hkv
+    for b in range(batch):
+        for h in range(hkv):
+            got = out[b, h * group:(h + 1) * group].double()
+            scores = q[b, h * group:(h + 1) * group].double() @ s.rows(s.cache.keys, b, h).T
+            best, v = (scores == scores.amax(-1, keepdim=True)).double(), s.rows(s.cache.values, b, h)
+            want = best @ v / best.sum(-1, keepdim=True)
+            assert bool(((got - want).abs() <= 1.001 * u * want.abs() + 2.0 ** -20 * v.abs().max()).all()), (b, h)
+    if scale > 30:  # (e^-30 is a number that can be the whole of an output, and sums have orders of their own)
+        assert torch.equal(out, _ops().paged_decode_attention(s.cache, q, s.table, s.lengths, sm_scale=scale))
