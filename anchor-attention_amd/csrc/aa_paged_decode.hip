@@ -826,7 +826,10 @@ __global__ void __launch_bounds__(256) paged_weigh_kernel(const PagedDecodeArgs 
 #pragma unroll
       for (int i = 0; i < 16; ++i) m = fmaxf(m, parts_of[i][tid][0]);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) l += parts_of[i][tid][0] == -INFINITY ? 0.f : fast_exp2((parts_of[i][tid][0] - m) * scale) * parts_of[i][tid][1];
+      for (int i = 0; i < 16; ++i) {  // (the sum of a part whose scores are all NaN, which has no maximum, is NaN and stays so)
+        const floatx2 x = parts_of[i][tid];
+        l += (x[0] == -INFINITY ? 0.f : fast_exp2((x[0] - m) * scale)) * x[1];
+      }
       totals[tid] = floatx2{m, 1.f / l};  // (of none, and of scores that are all minus infinity, infinity times 0)
     }
     __syncthreads();
