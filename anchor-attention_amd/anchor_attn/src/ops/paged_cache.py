@@ -369,8 +369,8 @@ def evict_from_pages(cache: PagedCache, page_table: torch.Tensor, lengths: torch
     above = n_keys if above is None else _whole("above", above)
     if n_first < 0 or n_last < 0 or not 0 < n_keys <= 1 << 20 or n_first + n_last > n_keys or not n_keys <= above < 1 << 31:
         _refuse(f"{n_keys} keys, the first {n_first} and the last {n_last} among them, of sequences of more than {above} are not supported (1 to 1048576)")
-    if batch * cache.n_kv_heads >= 1 << 24:
-        _refuse(f"{batch} sequences of {cache.n_kv_heads} KV heads are not supported (fewer than 2^24 together)")
+    if batch * cache.n_kv_heads >= 1 << 22:
+        _refuse(f"{batch} sequences of {cache.n_kv_heads} KV heads are not supported (fewer than 2^22 together)")
     new_lengths, kept = lengths.new_empty((batch,)), lengths.new_empty((batch, cache.n_kv_heads, n_keys))
     if batch:
         lib = _hip.lib()

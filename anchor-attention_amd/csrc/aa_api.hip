@@ -1066,6 +1066,10 @@ int aa_paged_weighing_decode_fwd(const aa_paged_cache* cache, const aa_paged_ste
     set_error("%s: n_first must not be negative (got %d)", who, n_first);
     return AA_EBADARG;
   }
+  if ((int64_t)t->batch * cache->n_kv_heads >= (1 << 24) - 4096) {  // (a launch has fewer than 2^24 work-groups of 256, of which 4096 join parts)
+    set_error("%s: %d sequences of %d KV heads are not supported (fewer than 2^24 - 4096 together)", who, t->batch, cache->n_kv_heads);
+    return AA_EUNSUPPORTED;
+  }
   const WeighScratch w = carve_weigh(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages);
   if ((rc = paged_decode_args(who, a, cache, t, w.total))) return rc;
   char* ws = static_cast<char*>(t->workspace);
@@ -1115,6 +1119,10 @@ int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step*
     set_error("%s: %d groups are not supported (1 to 65535)", who, n_groups);
     return n_groups <= 0 ? AA_EBADARG : AA_EUNSUPPORTED;
   }
+  if ((int64_t)t->batch * t->n_q_heads > (1 << 24) - 8) {  // (a launch has fewer than 2^24 work-groups of 256, and a multiple of 8)
+    set_error("%s: %d sequences of %d query heads are not supported (at most 2^24 - 8 together)", who, t->batch, t->n_q_heads);
+    return AA_EUNSUPPORTED;
+  }
   const SharedScratch w = carve_shared(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages, n_groups);
   if ((rc = paged_decode_args(who, a, cache, t, w.total))) return rc;
   char* ws = static_cast<char*>(t->workspace);
@@ -1160,8 +1168,9 @@ int aa_paged_evict(const aa_paged_cache* cache, const aa_paged_eviction* t, void
               t->n_keys, t->n_first, t->n_last, t->above);
     return AA_EBADARG;
   }
-  if (t->n_keys > 1 << 20 || (int64_t)t->batch * cache->n_kv_heads >= 1 << 24) {
-    set_error("%s: %d keys of %d sequences and %d KV heads are not supported (at most 1048576, fewer than 2^24 together)", who, t->n_keys, t->batch, cache->n_kv_heads);
+  if (t->n_keys > 1 << 20 || (int64_t)t->batch * cache->n_kv_heads >= 1 << 22) {  // (a launch has fewer than 2^32 threads, and each of these 1024)
+    set_error("%s: %d keys of %d sequences and %d KV heads are not supported (at most 1048576, fewer than 2^22 together: a launch has fewer than 2^24 work-groups of 256)", who,
+              t->n_keys, t->batch, cache->n_kv_heads);
     return AA_EUNSUPPORTED;
   }
   const size_t needed = aa_paged_evict_workspace_bytes(t->batch, cache->n_kv_heads, cache->head_dim, t->n_keys);
