@@ -1020,7 +1020,7 @@ static int paged_decode_args(const char* who, PagedDecodeArgs& a, const aa_paged
   a = {(const uint16_t*)t->q, t->q_sb, t->q_sh, (uint16_t*)t->out, t->o_sb, t->o_sh, (const uint16_t*)cache->keys, cache->kp_sp, cache->kp_sh, cache->kp_sn,
        (const uint16_t*)cache->values, cache->vp_sp, cache->vp_sh, cache->vp_sn, t->page_table, t->pt_sb, 0, t->lengths, t->batch, t->n_q_heads,
        cache->n_kv_heads, cache->head_dim, cache->n_pages, log2_of(cache->page_size), t->max_pages, 0, t->sm_scale, nullptr, nullptr, nullptr, cache->dtype,
-       nullptr, nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, nullptr, nullptr};
+       nullptr, nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
   return AA_OK;
 }
 
@@ -1083,13 +1083,14 @@ int aa_paged_weighing_decode_fwd(const aa_paged_cache* cache, const aa_paged_ste
 }
 
 struct SharedScratch {
-  size_t skips, firsts, entries, cuts, prefix, stats, own, own_stats, parts, decode, total;
+  size_t prefix_rows, skips, firsts, entries, cuts, prefix, stats, own, own_stats, parts, decode, total;
 };
-static SharedScratch carve_shared(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_groups) {
+static SharedScratch carve_shared(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages) {
   SharedScratch w;
   const size_t rows = (size_t)batch * n_q_heads;
-  w.skips = 0;
-  w.firsts = align256((size_t)batch * 4);
+  w.prefix_rows = 0;
+  w.skips = align256(4);
+  w.firsts = w.skips + align256((size_t)batch * 4);
   w.entries = w.firsts + align256((size_t)batch * 4);
   w.cuts = w.entries + align256(rows * 8);
   w.prefix = w.cuts + align256(rows * 8);  // (no more units than rows)
@@ -1097,14 +1098,14 @@ static SharedScratch carve_shared(int batch, int n_q_heads, int n_kv_heads, int 
   w.own = w.stats + align256(rows * 8);
   w.own_stats = w.own + align256(rows * head_dim * 4);
   w.parts = w.own_stats + align256(rows * 8);
-  w.decode = w.parts + align256(paged_prefix_scratch(batch, n_q_heads, n_kv_heads, head_dim, n_groups).total);
+  w.decode = w.parts + align256(paged_prefix_scratch(head_dim).total);
   w.total = w.decode + paged_decode_scratch(batch, n_q_heads, n_kv_heads, head_dim, log2_of(page_size), max_pages).total;
   return w;
 }
 
 size_t aa_paged_shared_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int n_groups) {
   if (n_q_heads == 0 || n_groups <= 0 || n_groups > 65535 || check_paged("aa_paged_shared_workspace_bytes", batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages)) return 0;
-  return carve_shared(batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages, n_groups).total;
+  return carve_shared(batch, n_q_heads, n_kv_heads, head_dim, page_size, max_pages).total;
 }
 
 int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step* t, const int32_t* shared_pages, const int32_t* groups, int n_groups, void* stream) {
@@ -1123,13 +1124,14 @@ int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step*
     set_error("%s: %d sequences of %d query heads are not supported (at most 2^24 - 8 together)", who, t->batch, t->n_q_heads);
     return AA_EUNSUPPORTED;
   }
-  const SharedScratch w = carve_shared(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages, n_groups);
+  const SharedScratch w = carve_shared(t->batch, t->n_q_heads, cache->n_kv_heads, cache->head_dim, cache->page_size, t->max_pages);
   if ((rc = paged_decode_args(who, a, cache, t, w.total))) return rc;
   char* ws = static_cast<char*>(t->workspace);
   if (!paged_prefix_pays(a.batch, a.n_kv_heads, a.head_dim, cache->page_size, t->max_pages)) {
     give_scratch(a, ws + w.decode, t->max_pages);
     return check_launch(launch_paged_decode(a, (hipStream_t)stream), who);
   }
+  a.prefix_rows = (int32_t*)(ws + w.prefix_rows);
   a.skips = (int32_t*)(ws + w.skips);
   a.firsts = (int32_t*)(ws + w.firsts);
   a.entries = (int32_t*)(ws + w.entries);
@@ -1138,10 +1140,9 @@ int aa_paged_shared_decode_fwd(const aa_paged_cache* cache, const aa_paged_step*
   a.prefix_stats = (float*)(ws + w.stats);
   a.own = (float*)(ws + w.own);
   a.own_stats = (float*)(ws + w.own_stats);
-  const PagedScratch s = paged_prefix_scratch(a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim, n_groups);
+  const PagedScratch s = paged_prefix_scratch(a.head_dim);
   a.prefix_part_stats = (float*)(ws + w.parts + s.stats);
   a.prefix_parts = (float*)(ws + w.parts + s.parts);
-  a.prefix_rows = paged_prefix_part_rows(a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim, n_groups);
   const PagedPrefixArgs x = {a, shared_pages, groups, n_groups};
   if ((rc = check_launch(launch_paged_prefix(x, (hipStream_t)stream), who))) return rc;
   give_scratch(a, ws + w.decode, t->max_pages);

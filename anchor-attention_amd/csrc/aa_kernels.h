@@ -176,8 +176,8 @@ struct PagedDecodeArgs {
   int32_t* cuts;  // scratch too, and for shared prefixes: [batch, units][2], the first share of a unit that several have, and how many (0: one)
   // a shared prefix (all or none), all scratch.  Written by launch_paged_prefix: its pages and its group's first sequence [batch]; a unit's first share and how many have parts of it (0:
   // it is whole), at its first row [batch, n_q_heads, 2]; whole units' accumulators [batch, n_q_heads, head_dim] and maxima and sums [batch, n_q_heads, 2], and the parts of the others,
-  // of prefix_rows rows.  Written by the decode kernel: accumulators, maxima and sums of a sequence's own keys
-  int32_t* skips; int32_t* firsts; int32_t* entries; float* prefix; float* prefix_stats; float* prefix_parts; float* prefix_part_stats; int prefix_rows;
+  // of *prefix_rows rows: 16, row by row, or 128 as many_rows leaves them.  Written by the decode kernel: accumulators, maxima and sums of a sequence's own keys
+  int32_t* skips; int32_t* firsts; int32_t* entries; float* prefix; float* prefix_stats; float* prefix_parts; float* prefix_part_stats; int32_t* prefix_rows;
   float* own; float* own_stats;
 };
 struct PagedScratch {
@@ -192,8 +192,7 @@ struct PagedPrefixArgs {
   const int32_t* shared_pages; const int32_t* groups; int n_groups;  // groups NULL: one, the whole batch
 };
 bool paged_prefix_pays(int batch, int n_kv_heads, int head_dim, int page_size, int max_pages);  // (by how much a batch may read: else every sequence reads the prefix for itself)
-int paged_prefix_part_rows(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups);  // rows of a part: 16, row by row, or 128 as paged_prefix_wide_kernel leaves them
-PagedScratch paged_prefix_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups);
+PagedScratch paged_prefix_scratch(int head_dim);
 hipError_t launch_paged_prefix(const PagedPrefixArgs& a, hipStream_t stream);
 
 struct PagedEvictArgs {

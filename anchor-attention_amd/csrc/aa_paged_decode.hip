@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(256) paged_finish_kernel(const PagedDecodeArgs
   if (b >= p.batch) return;
   const int head0 = kvh * group + (unit - kvh * col_blocks) * kCols, n_cols = min(kCols, (kvh + 1) * group - head0);
   const const_i32* cut = (const_i32*)p.cuts + 2 * ((int64_t)b * units + unit);
-  const int skip = ((const_i32*)p.skips)[b], of_group = ((const_i32*)p.firsts)[b], first = cut[0], parts = cut[1];
+  const int skip = ((const_i32*)p.skips)[b], of_group = ((const_i32*)p.firsts)[b], first = cut[0], parts = cut[1], prefix_rows = *(const_i32*)p.prefix_rows;
   if (skip == 0 && parts == 0) return;  // (the decode kernel's own)
   int heads_log = 0;
   while (1 << heads_log < min(n_cols, kHeads)) ++heads_log;
@@ -738,16 +738,16 @@ __global__ void __launch_bounds__(256) paged_finish_kernel(const PagedDecodeArgs
     };
     // (the first part of several is the second of its share, the others the first of theirs)
     if (skip > 0) {
-      const int in_group = (b - of_group) * group + head - kvh * group, row0 = in_group & -p.prefix_rows, s0 = row0 / group, r = in_group - row0;
+      const int in_group = (b - of_group) * group + head - kvh * group, row0 = in_group & -prefix_rows, s0 = row0 / group, r = in_group - row0;
       const int2 entry = *reinterpret_cast<const int2*>(p.entries + 2 * ((int64_t)(of_group + s0) * p.n_q_heads + kvh * group + row0 - s0 * group));
       if (entry.y == 0) {
         if (sub == 0) add(*reinterpret_cast<const floatx2*>(p.prefix_stats + 2 * row), *reinterpret_cast<const floatx4*>(p.prefix + row * D + d));
-      } else if (p.prefix_rows != 16) {  // four waves' 32 rows, fours of channels lane by lane
+      } else if (prefix_rows != 16) {  // four waves' 32 rows, fours of channels lane by lane
         const int lane = (r & 31) + 32 * (d >> 2 & 1), f = d >> 3;
         auto at = [&](const int i) { return ((int64_t)2 * (entry.x + i) + (i == 0 ? 1 : 0)) * 4 + (r >> 5); };
         add_all(entry.y, [&](const int i) { return p.prefix_part_stats + (at(i) * 64 + lane) * 2; }, [&](const int i) { return p.prefix_parts + ((at(i) * kFours + f) * 64 + lane) * 4; });
       } else {
-        auto at = [&](const int i) { return ((int64_t)2 * (entry.x + i) + (i == 0 ? 1 : 0)) * p.prefix_rows + r; };
+        auto at = [&](const int i) { return ((int64_t)2 * (entry.x + i) + (i == 0 ? 1 : 0)) * 16 + r; };
         add_all(entry.y, [&](const int i) { return p.prefix_part_stats + 2 * at(i); }, [&](const int i) { return p.prefix_parts + at(i) * D + d; });
       }
     }

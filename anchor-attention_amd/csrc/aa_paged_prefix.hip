@@ -2,11 +2,11 @@
 // 2^((score - m) * scale) and the accumulator of these times the values.  The decode kernel has the same of the sequence's own keys, and paged_finish_kernel joins them:
 //   o = (w a + w' a') / (w l + w' l'),  w = 2^((m - max(m, m')) * scale).
 //
-// The heads of a KV head's queries, of all sequences of the group, are rows of one product, so that keys and values are read once for 16 or 128 of them (unit_rows).  A unit is a
+// The heads of a KV head's queries, of all sequences of the group, are rows of one product, so that keys and values are read once for 16 or 128 of them (takes_many).  A unit is a
 // (group, KV head, rows); its keys come in tiles of 32 or 64.  The tiles of all units, one after the other, are cut into equal shares, one for each of a fixed number of
 // work-groups.  A unit that several shares have is joined in their order, so that results do not depend on timing.
 //
-// Of 16 rows a share's tiles are its four waves', each with accumulators of its own, joined through LDS: inside a wave, as in the decode kernel, S^T = K Q^T straight from memory, P^T in
+// Of 16 rows a share's tiles are its eight waves', each with accumulators of its own, joined through LDS: inside a wave, as in the decode kernel, S^T = K Q^T straight from memory, P^T in
 // S^T's registers, V turned by v_perm, P as two 16-bit numbers.  It is bound by memory: 4 sequences behind 32768 keys, 32/8 heads of 128 (134 MB), in 25.7 us, the rate of a copy;
 // behind 8192 in 11.9.
 // Of 128 rows: below.
@@ -18,8 +18,12 @@
 
 namespace aa {
 
-constexpr int kPrefixTile = 32, kPrefixWaves = 4, kPrefixShares = 256, kPrefixSharesLog = 8;
-constexpr int kPrefixLeast = 8, kPrefixOver = 4;  // tiles of a share at least; what a unit costs beside its tiles, in tiles
+constexpr int kPrefixShares = 256, kPrefixSharesLog = 8, kPrefixWaves = 8, kPrefixThreads = 64 * kPrefixWaves;
+// How the work is cut: keys of a tile and rows of a unit; tiles of a share at least; what a unit costs beside its tiles, in tiles
+struct PrefixForm {
+  int tile, rows, least, over;
+};
+constexpr PrefixForm kFew = {32, 16, 8, 4}, kMany = {64, 128, 4, 10};
 
 // A group's sequences and prefix; nothing that memory says is trusted.
 struct PagedGroup {
@@ -27,11 +31,12 @@ struct PagedGroup {
 };
 template <typename Words>
 __device__ __forceinline__ PagedGroup group_of(const PagedPrefixArgs& p, const Words* groups, const Words* shared_pages, const int g) {
-  PagedGroup x;
-  if (p.groups == nullptr) return {0, p.step.batch, min(max(shared_pages[0], 0), p.step.max_pages)};
-  x.first = min(max(groups[g], 0), p.step.batch);
-  x.sequences = max(min(max(groups[g + 1], 0), p.step.batch) - x.first, 0);
-  x.pages = min(max(shared_pages[g], 0), p.step.max_pages);
+  PagedGroup x = {0, p.step.batch, 0};
+  if (p.groups != nullptr) {
+    x.first = min(max(groups[g], 0), p.step.batch);
+    x.sequences = max(min(max(groups[g + 1], 0), p.step.batch) - x.first, 0);
+  }
+  x.pages = x.sequences > 1 ? min(max(shared_pages[g], 0), p.step.max_pages) : 0;  // (one alone shares nothing)
   return x;
 }
 // of a lane's group, and of one that all lanes have (by scalar loads, which are there sooner)
@@ -73,48 +78,64 @@ __device__ __forceinline__ int64_t uniform(const int64_t x) {
   return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x));
 }
 
-// The share-th of kPrefixShares equal parts of all units' tiles, and the group that it begins in (found by every wave for itself).
+__device__ __forceinline__ int tiles_of(const PagedDecodeArgs& p, const PrefixForm& form, const PagedGroup& x) {
+  return ((x.pages << p.page_log) + form.tile - 1) / form.tile;
+}
+__device__ __forceinline__ int blocks_of(const PrefixForm& form, const PagedGroup& x, const int heads) {
+  return (x.sequences * heads + form.rows - 1) / form.rows;
+}
+// A unit's extent: its tiles, and before them what its beginning and end cost, in tiles (0 where there are none)
+__device__ __forceinline__ int extent_of(const PrefixForm& form, const int tiles) { return tiles > 0 ? tiles + form.over : 0; }
+// ... of all of a group's units
+__device__ __forceinline__ int64_t extents_in(const PagedDecodeArgs& p, const PrefixForm& form, const PagedGroup& x) {
+  return (int64_t)extent_of(form, tiles_of(p, form, x)) * blocks_of(form, x, p.n_q_heads / p.n_kv_heads) * p.n_kv_heads;
+}
+// the group of the lane's number from i on, one of nothing where there is none
+__device__ __forceinline__ PagedGroup lane_group_at(const PagedPrefixArgs& all, const int i) {
+  const int g = i + (int)(threadIdx.x & 63);
+  return g < all.n_groups ? group_at(all, g) : PagedGroup{0, 0, 0};
+}
+__device__ __forceinline__ int64_t up_to_lane(int64_t x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up((long long)x, d, 64);
+    x += lane >= d ? y : 0;
+  }
+  return x;
+}
+// All units' extents in either form, found by every wave for itself; `mine`, the group of the lane's number.
+struct PrefixTotals {
+  int64_t few, many;
+};
+__device__ __forceinline__ PrefixTotals totals_of(const PagedPrefixArgs& all, const PagedGroup& mine) {
+  PrefixTotals t = {0, 0};
+  if (all.n_groups == 1) {
+    const PagedGroup x = common_group_at(all, 0);
+    return {extents_in(all.step, kFew, x), extents_in(all.step, kMany, x)};
+  }
+  for (int i = 0; i < all.n_groups; i += 64) {
+    const PagedGroup x = i == 0 ? mine : lane_group_at(all, i);
+    t.few += __shfl((long long)up_to_lane(extents_in(all.step, kFew, x)), 63, 64);
+    t.many += __shfl((long long)up_to_lane(extents_in(all.step, kMany, x)), 63, 64);
+  }
+  return {uniform(t.few), uniform(t.many)};
+}
+__device__ __forceinline__ int64_t length_of_share(const PrefixForm& form, const int64_t total) {
+  return max((total + (kPrefixShares - 1)) >> kPrefixSharesLog, (int64_t)form.least);
+}
+// The share-th of kPrefixShares equal parts of all units' extents, and the group that it begins in.
 struct PrefixShare {
   int64_t at, end, share, start;  // from, to; how long a share is; where the group begins
   int group;
 };
-template <int TILE>
-__device__ __forceinline__ int tiles_of(const PagedDecodeArgs& p, const PagedGroup& x) {
-  return ((x.pages << p.page_log) + TILE - 1) / TILE;
-}
-template <int ROWS>
-__device__ __forceinline__ int blocks_of(const PagedGroup& x, const int heads) {
-  return (x.sequences * heads + ROWS - 1) / ROWS;
-}
-// A unit's extent: its tiles, and before them what its beginning and end cost, in tiles (0 where there are none)
-template <int OVER>
-__device__ __forceinline__ int extent_of(const int tiles) { return tiles > 0 ? tiles + OVER : 0; }
-template <int TILE, int ROWS, int OVER>
-__device__ __forceinline__ PrefixShare share_of(const PagedPrefixArgs& all, const int share, const int least) {
-  const PagedDecodeArgs& p = all.step;
-  const int lane = threadIdx.x & 63, heads = p.n_q_heads / p.n_kv_heads;
-  auto extents_in = [&](const PagedGroup& x) { return (int64_t)extent_of<OVER>(tiles_of<TILE>(p, x)) * blocks_of<ROWS>(x, heads) * p.n_kv_heads; };
-  auto extents_of = [&](const int i) { return i < all.n_groups ? extents_in(group_at(all, i)) : (int64_t)0; };  // of group i's units
-
-  auto up_to_lane = [&](int64_t x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t y = __shfl_up((long long)x, d, 64);
-      x += lane >= d ? y : 0;
-    }
-    return x;
-  };
-  PrefixShare r = {0, 0, 0, 0, 0};
-  int64_t total = 0;
-  if (all.n_groups == 1) total = extents_in(common_group_at(all, 0));
-  else
-    for (int i = 0; i < all.n_groups; i += 64) total += __shfl((long long)up_to_lane(extents_of(i + lane)), 63, 64);
-  r.share = max((total + (kPrefixShares - 1)) >> kPrefixSharesLog, (int64_t)least);
+__device__ __forceinline__ PrefixShare share_of(const PagedPrefixArgs& all, const PrefixForm& form, const int64_t total, const PagedGroup& mine, const int share) {
+  PrefixShare r = {0, 0, length_of_share(form, total), 0, 0};
   r.at = min(r.share * share, total);
   r.end = min(r.at + r.share, total);
   if (r.at < r.end && all.n_groups > 1) {
     for (int i = 0; i < all.n_groups; i += 64) {
-      const int64_t sum = up_to_lane(extents_of(i + lane));
+      const int64_t sum = up_to_lane(extents_in(all.step, form, i == 0 ? mine : lane_group_at(all, i)));
       const int in = __popcll(__ballot(r.start + sum <= r.at));
       if (in < 64) {
         r.group = i + in;
@@ -127,22 +148,20 @@ __device__ __forceinline__ PrefixShare share_of(const PagedPrefixArgs& all, cons
   return {uniform(r.at), uniform(r.end), uniform(r.share), uniform(r.start), (int)__builtin_amdgcn_readfirstlane(r.group)};
 }
 
+// `states`: [wave][row][kPitch] floats of LDS, the accumulator, maximum and sum
 template <typename T, int D>
-__global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(const PagedPrefixArgs all) {
+__device__ __forceinline__ void few_rows(const PagedPrefixArgs& all, const int64_t total, const PagedGroup& lanes, float* states) {
   constexpr int kKS = D / 32;  // MFMAs of a score
   constexpr int kDV = D / 16;  // channels of V that a lane loads
   constexpr int kVW = kDV / 2;
-  constexpr int kRows = 16, kPitch = D + 4;
-  __shared__ __attribute__((aligned(16))) float states[kPrefixWaves * kRows * kPitch];  // [wave][row][kPitch]: the accumulator, maximum and sum
+  constexpr int kRows = kFew.rows, kTile = kFew.tile, kPitch = D + 4;
   const PagedDecodeArgs& p = all.step;
   const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int heads = p.n_q_heads / p.n_kv_heads, page_size = 1 << p.page_log;
 
-  find_skips(all, tid, 64 * kPrefixWaves);
-
   // ---- this work-group's share ---------------------------------------------------------------------
-  const PrefixShare mine = share_of<kPrefixTile, kRows, kPrefixOver>(all, blockIdx.x, kPrefixLeast);
+  const PrefixShare mine = share_of(all, kFew, total, lanes, blockIdx.x);
   int64_t at = mine.at, start = mine.start;
   const int64_t end = mine.end, share = mine.share;
   int group = mine.group;
@@ -156,8 +175,8 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
   while (at < end && group < all.n_groups) {
     at = uniform(at), start = uniform(start), group = __builtin_amdgcn_readfirstlane(group);  // (which the compiler does not see of what a loop carries)
     const PagedGroup x = common_group_at(all, group);
-    const int tiles = tiles_of<kPrefixTile>(p, x), blocks = blocks_of<kRows>(x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
-    const int extent = extent_of<kPrefixOver>(tiles);
+    const int tiles = tiles_of(p, kFew, x), blocks = blocks_of(kFew, x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
+    const int extent = extent_of(kFew, tiles);
     if (at - start >= (int64_t)extent * blocks * p.n_kv_heads) {  // (the next group, perhaps of nothing)
       start += (int64_t)extent * blocks * p.n_kv_heads;
       ++group;
@@ -186,7 +205,7 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
       Spot o;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int key = kPrefixTile * t + 16 * half, row = key & (page_size - 1);
+        const int key = kTile * t + 16 * half, row = key & (page_size - 1);
         const int64_t page = clamped_page(table[min(key >> p.page_log, x.pages - 1)], p.n_pages);
         o.k[half] = page * p.kp_sp + row * p.kp_sn + kvh * p.kp_sh;
         o.v[half] = page * p.vp_sp + row * p.vp_sn + kvh * p.vp_sh;
@@ -223,7 +242,7 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
     clear();
 
     // (the last tile of a prefix of 16 * odd keys has no second half)
-    auto seen = [&](const int t, const int i) __attribute__((always_inline)) { return kPrefixTile * t + 16 * (i >> 2) < length; };
+    auto seen = [&](const int t, const int i) __attribute__((always_inline)) { return kTile * t + 16 * (i >> 2) < length; };
     auto scores = [&](const Tile& y, floatx4 (&s)[2]) __attribute__((always_inline)) {
       s[0] = s[1] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -232,7 +251,7 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
         for (int half = 0; half < 2; ++half) s[half] = mfma16<T>(y.k[half][i], q[i], s[half]);
     };
     auto probabilities = [&](floatx4 (&s)[2], const int t, u32x4& prob, u32x4& rest, const bool exact) __attribute__((always_inline)) {
-      if (kPrefixTile * (t + 1) > length) {
+      if (kTile * (t + 1) > length) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = seen(t, i) ? s[i >> 2][i & 3] : -INFINITY;
       }
@@ -337,7 +356,7 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
     }
     __syncthreads();
     const bool begins = t0 == 0, ends = t1 == tiles;
-    for (int i = tid; i < kRows * (D / 4); i += 64 * kPrefixWaves) {
+    for (int i = tid; i < kRows * (D / 4); i += kPrefixThreads) {
       const int r = i / (D / 4), d = 4 * (i % (D / 4)), row = row0 + r;
       if (row >= rows) break;  // (rows ascend)
       float m = -INFINITY, l = 0.f, ms[kPrefixWaves];
@@ -387,7 +406,6 @@ __global__ void __launch_bounds__(64 * kPrefixWaves, 1) paged_prefix_kernel(cons
 // A probability enters as two 16-bit numbers, its rounding and the rest, as in the decode kernel, so that a step has the same precision however many sequences share its pages.  It costs
 // half as many products again; the listed sizes of perf/more_operators.py take 59.1, 50.7 and 66.6 us a step, 53.1, 46.6 and 60.3 with the rounding alone.  (Sums by products with ones, a
 // product more for each of the two: 59.6, 51.0, 68.5.  Exponents as the decode kernel has them, (score - m) * scale, at all scores: 58.7, 50.6 and 68.3 instead of 58.0, 50.2 and 66.8.)
-constexpr int kWideTile = 64, kWideRows = 128, kWideThreads = 512, kWideLeast = 4, kWideOver = 10;
 
 template <int D>
 __device__ __forceinline__ int wide_k_swizzle(const int r) { return D == 128 ? r & 15 : (r & 7) ^ ((r >> 3) & 1); }
@@ -403,26 +421,26 @@ __device__ __forceinline__ void load16_to_lds_from_any(const char* base, const u
 // a barrier that waits for nothing of its own
 __device__ __forceinline__ void wave_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
+// `tiles`: kManyLds<D> bytes of LDS, on a 1024-byte boundary: [team][keys 0, 1, values 0, 1]; at the end the second team's states
+template <int D> constexpr int kManyLds = 2 * 4 * kMany.tile * 2 * D;
 template <typename T, int D>
-__global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const PagedPrefixArgs all) {
+__device__ __forceinline__ void many_rows(const PagedPrefixArgs& all, const int64_t total, const PagedGroup& lanes, char* tiles) {
   constexpr int kKS = D / 16, kDB = D / 32;        // MFMAs of a score, blocks of 32 channels
-  constexpr int kRowBytes = 2 * D, kTileBytes = kWideTile * kRowBytes;
+  constexpr int kRowBytes = 2 * D, kTileBytes = kMany.tile * kRowBytes;
   constexpr int kRowsALoad = 1024 / kRowBytes, kLoads = 16 / kRowsALoad;  // rows of a load instruction; loads of a wave's 16 rows
   constexpr int kFours = 4 * kDB;                  // accumulators of a lane, in fours
   typedef __attribute__((address_space(3))) const typename T::vec8 lds_vec8;
   typedef short shortx4 __attribute__((ext_vector_type(4)));
   typedef short shortx8 __attribute__((ext_vector_type(8)));
   typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
-  // [team][keys 0, 1, values 0, 1]; at the end the second team's states
-  __shared__ __attribute__((aligned(1024))) char tiles[2][4][kTileBytes];
-  static_assert(sizeof(tiles) >= (size_t)4 * 64 * (4 * kFours + 4) * 4, "a team's states take less room");
+  static_assert(kManyLds<D> >= 4 * 64 * (4 * kFours + 4) * 4, "a team's states take less room");
   const PagedDecodeArgs& p = all.step;
   const int tid = threadIdx.x, lane = tid & 63, c32 = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), team = __builtin_amdgcn_readfirstlane(tid >> 8);
   const int heads = p.n_q_heads / p.n_kv_heads, page_mask = (1 << p.page_log) - 1;
   // neighbouring shares, which have neighbouring rows of one KV head, are one XCD's
   const int share_at = (blockIdx.x % 8) * (kPrefixShares / 8) + blockIdx.x / 8;
-  const PrefixShare mine = share_of<kWideTile, kWideRows, kWideOver>(all, share_at, kWideLeast);
+  const PrefixShare mine = share_of(all, kMany, total, lanes, share_at);
   int64_t at = mine.at, start = mine.start;
   const int64_t end = mine.end, share = mine.share;
   int group = mine.group;
@@ -436,7 +454,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     k_from[j] = 2u * (uint32_t)p.kp_sn * r + 16u * (slot ^ wide_k_swizzle<D>(r));
     v_from[j] = 2u * (uint32_t)p.vp_sn * r + 16u * (slot ^ wide_v_swizzle<D>(r));
   }
-  const uint32_t my_tiles = lds_addr(tiles[team][0]);
+  const uint32_t my_tiles = lds_addr(tiles) + team * 4 * kTileBytes;
   // (chunk 2 ks + half of a row: the bits of ks are their own; so are those of the block of channels)
   const uint32_t k_rd = my_tiles + c32 * kRowBytes + ((half ^ wide_k_swizzle<D>(c32)) << 4);
   const int r0 = 4 * half + ((lane & 15) >> 2), y0 = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
@@ -445,8 +463,8 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
   while (at < end && group < all.n_groups) {
     at = uniform(at), start = uniform(start), group = __builtin_amdgcn_readfirstlane(group);  // (which the compiler does not see of what a loop carries)
     const PagedGroup x = common_group_at(all, group);
-    const int n_tiles = tiles_of<kWideTile>(p, x), blocks = blocks_of<kWideRows>(x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
-    const int extent = extent_of<kWideOver>(n_tiles);
+    const int n_tiles = tiles_of(p, kMany, x), blocks = blocks_of(kMany, x, heads), length = x.pages << p.page_log, rows = x.sequences * heads;
+    const int extent = extent_of(kMany, n_tiles);
     if (at - start >= (int64_t)extent * blocks * p.n_kv_heads) {  // (the next group, perhaps of nothing)
       start += (int64_t)extent * blocks * p.n_kv_heads;
       ++group;
@@ -457,7 +475,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     const int64_t unit_end = start + (int64_t)(unit + 1) * extent, until = min(end, unit_end);
     const int t0 = max(n_tiles - (int)(unit_end - at), 0), t1 = max(n_tiles - (int)(unit_end - until), 0);
     if (t1 == 0) break;  // (nothing of it is in this share, which ends)
-    const int my_row = min((int)(block * kWideRows) + 32 * wave + c32, rows - 1), sequence = my_row / heads;
+    const int my_row = min((int)(block * kMany.rows) + 32 * wave + c32, rows - 1), sequence = my_row / heads;
     const int64_t my_head = (int64_t)(x.first + sequence) * p.n_q_heads + (int)kvh * heads + my_row - sequence * heads;
     typename T::vec8 q[kKS];
     {
@@ -469,7 +487,7 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     const int rounds = (t1 - t0 + 1) / 2, own = (t1 - t0 + 1 - team) / 2;  // tiles t0 + team, t0 + team + 2, ...
     auto tile_at = [&](const int i) { return t0 + team + 2 * i; };
     // 16 of a tile's rows are a wave's to request, which lie in one page; rows behind the prefix are zeros
-    auto key_of = [&](const int i) { return kWideTile * tile_at(i) + 16 * wave; };
+    auto key_of = [&](const int i) { return kMany.tile * tile_at(i) + 16 * wave; };
     auto page_of = [&](const int i) { return table[min(key_of(min(i, max(own - 1, 0))) >> p.page_log, x.pages - 1)]; };
     auto request = [&](const int i, const int page_there, const bool values) __attribute__((always_inline)) {
       const int key = key_of(i);
@@ -525,8 +543,8 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
       s[g / kKS] = T::mfma(*reinterpret_cast<const typename T::vec8*>(&operand[(kValues + g) % kAhead]), q[g % kKS], g % kKS == 0 ? none : s[g / kKS]);
     };
     auto probabilities = [&](const int i, auto exact) __attribute__((always_inline)) {
-      const int key0 = kWideTile * tile_at(i);
-      if (key0 + kWideTile > length) {
+      const int key0 = kMany.tile * tile_at(i);
+      if (key0 + kMany.tile > length) {
 #pragma unroll
         for (int r = 0; r < 32; ++r)
           if (key0 + 32 * (r >> 4) + 16 * ((r & 15) >> 3) >= length) s[r >> 4][r & 15] = -INFINITY;
@@ -649,11 +667,11 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     if (__builtin_expect(__syncthreads_or(is_nan(sum) && !is_nan(l_run)), 0)) run(std::true_type{});
 
     // ---- the teams' states -> the unit's, or a part of it: fours of accumulators, lane by lane, half of them by each team ----
-    floatx4* states = reinterpret_cast<floatx4*>(&tiles[0][0][0]) + wave * kFours * 64;
-    floatx2* stats = reinterpret_cast<floatx2*>(reinterpret_cast<floatx4*>(&tiles[0][0][0]) + 4 * kFours * 64) + wave * 128;
+    floatx4* states = reinterpret_cast<floatx4*>(tiles) + wave * kFours * 64;
+    floatx2* stats = reinterpret_cast<floatx2*>(reinterpret_cast<floatx4*>(tiles) + 4 * kFours * 64) + wave * 128;
     auto four = [&](const int f) { return floatx4{acc[f >> 2][4 * (f & 3)], acc[f >> 2][4 * (f & 3) + 1], acc[f >> 2][4 * (f & 3) + 2], acc[f >> 2][4 * (f & 3) + 3]}; };
     const int64_t part = (2 * share_at + (t0 == 0 ? 1 : 0)) * 4 + wave;
-    const bool whole = t0 == 0 && t1 == n_tiles, there = (int)(block * kWideRows) + 32 * wave + c32 < rows;
+    const bool whole = t0 == 0 && t1 == n_tiles, there = (int)(block * kMany.rows) + 32 * wave + c32 < rows;
     auto hand_over = [&](auto first) __attribute__((always_inline)) {
 #pragma unroll
       for (int f = 0; f < kFours / 2; ++f) states[(decltype(first)::value + f) * 64 + lane] = four(decltype(first)::value + f);
@@ -683,23 +701,37 @@ __global__ void __launch_bounds__(kWideThreads) paged_prefix_wide_kernel(const P
     __syncthreads();
     if (team == 0) finish(lower);
     else finish(upper);
-    if (t0 == 0 && tid == 0) note_unit<kWideRows>(p, x.first, (int)kvh, (int)block, heads, share_at, whole ? 0 : (int)((unit_end - 1) / share) - share_at + 1);
+    if (t0 == 0 && tid == 0) note_unit<kMany.rows>(p, x.first, (int)kvh, (int)block, heads, share_at, whole ? 0 : (int)((unit_end - 1) / share) - share_at + 1);
     __syncthreads();
     at = until;
   }
-  find_skips(all, tid, kWideThreads);
 }
 
-// Rows of a unit, by how many rows of a KV head a group has on average: 16, whose keys need no turn through LDS, or 128, which share what they read.  Up to 16 rows 16 cost less, between 16 and
-// 32 with heads of 64 too, where products are cheap next to what a work-group begins and ends with.  A step of one group, 100 keys of their own, 16 and 128 rows to a unit:
-//   32/8 heads of 128: 4 sequences (16 rows) behind 8192 keys 27.2 and 31.2 us, behind 32768 41.0 and 43.7; 8 (32 rows) 30.1 and 31.5, 57.0 and 44.1; 16 (64 rows) 33.4 and 31.5, 90.7 and 45.3
-//   28/4 of 128: 2 (14 rows) 28.2 and 33.0, 41.1 and 42.5; 3 (21 rows) 29.4 and 33.3, 44.0 and 42.6; 6 (42 rows) 28.6 and 34.7, 51.5 and 43.8
-//   32/8 of 64: 4 (16 rows) 22.0 and 24.1, 29.0 and 31.8; 8 (32 rows) 24.1 and 24.2, 34.6 and 32.2; 16 (64 rows) 26.2 and 24.7, 46.6 and 32.4
-//   14/2 of 64: 4 (28 rows) 22.6 and 25.9, 29.4 and 32.9; 8 (56 rows) 23.8 and 26.1, 30.5 and 33.6; 16 (112 rows) 25.4 and 26.5, 36.7 and 35.2
-// (32 rows in two blocks of 16 gave 30.9 and 44.0 with 32/8 heads of 128, 24.6 and 34.1 with 32/8 of 64: nothing that one of the two does not.)
-static int unit_rows(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups) {
-  const int64_t rows = (int64_t)batch * (n_q_heads / n_kv_heads) / n_groups;
-  return rows <= (head_dim == 64 ? 32 : 16) ? 16 : kWideRows;
+// Which form the launch takes, by all units' extents in either: an extent of few rows takes about 0.6 us of its work-group, one of many 1.5, and many rows' parts some 8 us more to begin, join
+// and read again.  The groups are looked at as they are; their number and the batch, all that the host knows, say little of groups of which many are empty, as where a captured step has room for more, or one
+// is large and the others are small: 128 sequences, 28/4 heads of 128, behind 8000 keys in one group of 64 that could be take 112 us a step with few rows to a unit and 49 with many, 32, 32/8 of 128,
+// behind 32768 in one of 200 100 and 56.  A step of one group, bf16, 100 keys of their own, few and many rows, behind 8192 keys and behind 32768 (* where the rule takes the slower one):
+//   32/8 heads of 128: 4 sequences (16 rows) 27.6 and 33.6 us, 42.3 and 48.2; 8 (32 rows) 31.8 and 33.6, 58.5 and 48.1; 12 (48 rows) 37.2 and 33.9, 77.4 and 49.2
+//   28/4 of 128: 3 (21 rows) 30.6 and 36.1, 44.5 and 46.2; 6 (42 rows) 29.7 and 36.3, 53.2 and 47.0; 16 (112 rows) 40.8 and 38.0, 87.9 and 47.8
+//   32/8 of 64: 4 (16 rows) 22.6 and 25.7, 30.8 and 35.8; 8 (32 rows) 25.1 and 25.5, 38.8 and 35.9; 16 (64 rows) 28.6 and 26.0, 55.5 and 36.0
+//   14/2 of 64: 4 (28 rows) 23.2 and 27.0, 29.4 and 34.6; 16 (112 rows) 25.9 and 27.2, 34.5 and 36.5 *; 32 (224 rows) 28.9 and 27.9, 52.5 and 35.5
+//   128 sequences behind 1024 keys: 32/8 of 128 36.3 and 38.5 *, 28/4 of 128 38.6 and 33.2, 32/8 of 64 27.3 and 27.8 *
+__device__ __forceinline__ bool takes_many(const PrefixTotals& t) {
+  const int64_t few = max(t.few, (int64_t)kFew.least * kPrefixShares), many = max(t.many, (int64_t)kMany.least * kPrefixShares);
+  return 2 * few > 5 * many + 26 * kPrefixShares;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPrefixThreads) paged_prefix_kernel(const PagedPrefixArgs all) {
+  constexpr int kFewLds = kPrefixWaves * kFew.rows * (D + 4) * 4;
+  __shared__ __attribute__((aligned(1024))) char lds[kManyLds<D> > kFewLds ? kManyLds<D> : kFewLds];
+  find_skips(all, threadIdx.x, kPrefixThreads);
+  const PagedGroup lanes = all.n_groups == 1 ? PagedGroup{0, 0, 0} : lane_group_at(all, 0);
+  const PrefixTotals totals = totals_of(all, lanes);
+  const bool many = takes_many(totals);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *all.step.prefix_rows = many ? kMany.rows : kFew.rows;
+  if (many) many_rows<T, D>(all, totals.many, lanes, lds);
+  else few_rows<T, D>(all, totals.few, lanes, reinterpret_cast<float*>(lds));
 }
 
 // Where the keys and values of all sequences fit the caches, as much as the table has room for, what sequences share is there after the first one's read, and the steps of the others cost less than
@@ -712,22 +744,17 @@ bool paged_prefix_pays(int batch, int n_kv_heads, int head_dim, int page_size, i
   return (double)batch * max_pages * page_size * n_kv_heads * head_dim * 4 > 256e6;
 }
 
-int paged_prefix_part_rows(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups) { return unit_rows(batch, n_q_heads, n_kv_heads, head_dim, n_groups); }
-
-PagedScratch paged_prefix_scratch(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_groups) {
-  const int each = unit_rows(batch, n_q_heads, n_kv_heads, head_dim, n_groups);
-  const size_t rows = (size_t)kPrefixShares * 2 * each;
+PagedScratch paged_prefix_scratch(int head_dim) {
+  constexpr size_t kRows = (size_t)kPrefixShares * 2 * kMany.rows;
   PagedScratch s = {0, 0, 0, 0};
-  s.parts = s.stats + rows * (each == kWideRows ? 16 : 8);  // (a row's statistics are there twice, once for each of its lanes)
-  s.total = s.parts + rows * head_dim * 4;
+  s.parts = s.stats + kRows * 16;  // (a row's statistics are there twice, once for each of its lanes)
+  s.total = s.parts + kRows * head_dim * 4;
   return s;
 }
 
 template <typename T, int D>
 static hipError_t launch_paged_prefix_of(const PagedPrefixArgs& a, hipStream_t stream) {
-  if (unit_rows(a.step.batch, a.step.n_q_heads, a.step.n_kv_heads, D, a.n_groups) != kWideRows)
-    hipLaunchKernelGGL((paged_prefix_kernel<T, D>), dim3(kPrefixShares), dim3(64 * kPrefixWaves), 0, stream, a);
-  else hipLaunchKernelGGL((paged_prefix_wide_kernel<T, D>), dim3(kPrefixShares), dim3(kWideThreads), 0, stream, a);
+  hipLaunchKernelGGL((paged_prefix_kernel<T, D>), dim3(kPrefixShares), dim3(kPrefixThreads), 0, stream, a);
   return hipGetLastError();
 }
 hipError_t launch_paged_prefix(const PagedPrefixArgs& a, hipStream_t stream) {

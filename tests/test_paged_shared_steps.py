@@ -69,3 +69,30 @@ def test_scores_far_apart(batch, hq, hkv, d, times, scale, dtype):
             assert bool(((got - want).abs() <= 1.001 * u * want.abs() + 2.0 ** -20 * v.abs().max()).all()), (b, h)
     if scale > 30:  # (e^-30 is a number that can be the whole of an output, and sums have orders of their own)
         assert torch.equal(out, _ops().paged_decode_attention(s.cache, q, s.table, s.lengths, sm_scale=scale))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("prefix,batch,hq,hkv,d,page", [(125, 128, 28, 4, 128, 64), (250, 32, 32, 8, 128, 128), (300, 100, 32, 8, 64, 64), (20, 9, 14, 2, 64, 16)])
+def test_empty_groups_change_nothing(prefix, batch, hq, hkv, d, page, dtype):
+    """A captured step has room for more groups than there are: the same bits as without it."""
+    s, shared, groups = _shared_setup([prefix], [batch], [3, 70, 1], hkv, d, page, dtype, 5)
+    table, q = _wide_table(s), s.queries(hq)
+    want = _ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, shared)
+    _close(want, q, s, d ** -0.5)
+    for before, behind in ((0, 0), (0, 63), (1, 0), (70, 200)):
+        pages, begins = _int32([5] * before + [prefix] + [9] * behind), _int32([0] * before + [0, batch] + [batch] * behind)
+        assert torch.equal(_ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, pages, begins), want), (before, behind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("prefixes,sizes,hq,hkv,d", [
+    ([200] + [3] * 40, [90] + [2] * 40, 32, 8, 64), ([2] * 70 + [100], [1] * 70 + [64], 32, 8, 128), ([100] * 3, [1] * 3, 28, 4, 128), ([400, 1, 400], [40, 1, 2], 28, 4, 128),
+    ([50, 7] * 33, [1, 3] * 33, 14, 2, 64),
+])
+def test_groups_of_very_different_sizes(prefixes, sizes, hq, hkv, d, dtype):
+    """A large group beside many small ones, and groups of one sequence, which share with nobody."""
+    s, shared, groups = _shared_setup(prefixes, sizes, [40, 0, 1], hkv, d, 16, dtype, 6)
+    table, q = _wide_table(s), s.queries(hq)
+    _close(_ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, shared, groups), q, s, d ** -0.5)
