@@ -386,7 +386,7 @@ def paged_shared_decode_attention(cache: PagedCache, q: torch.Tensor, page_table
     """:func:`paged_decode_attention` of sequences that begin with the same pages, which are read once for all of them.  Sequences ``groups[g]`` to
     ``groups[g + 1] - 1`` (``groups`` int32 ``[n_groups + 1]``, ascending; None: all sequences are one group) have the same first ``shared_pages[g]`` pages (int32 ``[n_groups]``) in their rows of
     the table; any of these rows may be what is read.  The first and last groups need not begin and end the batch: sequences in none, and those of fewer keys than their group's
-    shared pages hold, are attended to by themselves.  Sequences append to pages of their own: only whole pages are shared.  A batch whose table has room for 256 MB of keys and values at most reads the shared pages once for each sequence, which is
+    shared pages hold, are attended to by themselves.  Sequences append to pages of their own: only whole pages are shared.  A batch whose table has room for 256 MB of keys and values at most (340 with heads of 128) reads the shared pages once for each sequence, which is
     less time, since they stay in the caches."""
     out, tensors, sizes, most, scale = _decode_args(cache, q, page_table, lengths, sm_scale, out)
     shared_ptr = _indices(shared_pages, "shared_pages", cache, 1)

@@ -1098,7 +1098,7 @@ static SharedScratch carve_shared(int batch, int n_q_heads, int n_kv_heads, int 
   w.own = w.stats + align256(rows * 8);
   w.own_stats = w.own + align256(rows * head_dim * 4);
   w.parts = w.own_stats + align256(rows * 8);
-  w.decode = w.parts + align256(paged_prefix_scratch(head_dim).total);
+  w.decode = w.parts + (paged_prefix_pays(batch, n_kv_heads, head_dim, page_size, max_pages) ? align256(paged_prefix_scratch(head_dim).total) : 0);
   w.total = w.decode + paged_decode_scratch(batch, n_q_heads, n_kv_heads, head_dim, log2_of(page_size), max_pages).total;
   return w;
 }

@@ -736,12 +736,14 @@ __global__ void __launch_bounds__(kPrefixThreads) paged_prefix_kernel(const Page
 
 // Where the keys and values of all sequences fit the caches, as much as the table has room for, what sequences share is there after the first one's read, and the steps of the others cost less than
 // two kernels more.  One group, 100 keys of their own, all bytes as if none were shared, time by this path and with every sequence by itself:
-//   14/2 heads of 64: 2 sequences behind 1024 keys (1 MB) 17.3 and 11.0 us, 32 behind 4096 (69 MB) 24.2 and 15.2, 64 behind 8192 (272 MB) 28.7 and 30.7, 64 behind 16384 (540 MB) 30.0 and 51.8
-//   32/8 of 128: 4 behind 1024 (18 MB) 22.4 and 13.6, 8 behind 8192 (272 MB) 30.7 and 27.8, 32 behind 4096 (550 MB) 31.9 and 43.0
-//   28/4 of 128, fp16: 16 behind 8192 (272 MB) 38.9 and 27.5, 32 behind 8192 (543 MB) 35.4 and 45.3
-// The lengths are the device's to know: in a table with room for more, few keys take this path too.
+//   32/8 heads of 64: 64 sequences behind 1024 keys (151 MB) 23.0 and 19.3 us, 12 behind 8192 (204 MB) 25.6 and 25.8, 32 behind 4096 (277 MB) 25.5 and 29.2, 16 behind 8192 (273 MB) 26.0 and 31.2
+//   14/2 of 64: 32 behind 8192 (136 MB) 27.9 and 20.4, 64 behind 8192 (273 MB) 29.5 and 31.2, 32 behind 16384 (271 MB) 32.3 and 30.5 *, 16 behind 32768 (269 MB) 36.5 and 30.2 *, 64 behind 16384 (541 MB) 32.8 and 52.1
+//   32/8 of 128: 16 behind 4096 (277 MB) 30.2 and 28.0, 8 behind 8192 (273 MB) 31.8 and 28.0, 2 behind 32768 (269 MB) 41.8 and 44.7 *, 64 behind 1024 (302 MB) 29.6 and 28.9, 12 behind 8192 (409 MB)
+//     33.9 and 36.6, 6 behind 16384 (406 MB) 39.4 and 63.0
+//   28/4 of 128: 16 behind 8192 (273 MB) 38.0 and 28.3, 128 behind 1024 (302 MB) 33.2 and 30.0, 12 behind 16384 (406 MB) 41.9 and 63.3, 16 behind 16384 (541 MB) 42.0 and 45.5
+// (* where the rule takes the slower one.)  The lengths are the device's to know: in a table with room for more, few keys take this path too.
 bool paged_prefix_pays(int batch, int n_kv_heads, int head_dim, int page_size, int max_pages) {
-  return (double)batch * max_pages * page_size * n_kv_heads * head_dim * 4 > 256e6;
+  return batch > 1 && (double)batch * max_pages * page_size * n_kv_heads * head_dim * 4 > (head_dim == 64 ? 256e6 : 340e6);
 }
 
 PagedScratch paged_prefix_scratch(int head_dim) {

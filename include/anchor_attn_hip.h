@@ -297,7 +297,7 @@ int aa_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sn, const void*
  *
  * aa_paged_shared_decode_fwd: the same as aa_paged_decode_fwd where sequences groups[g] to groups[g + 1] - 1 (groups int32 [n_groups + 1], ascending; sequences before the
  * first and behind the last group are in none; NULL with one group: all of the batch) have the same first shared_pages[g] pages (int32 [n_groups]), in any of their rows of the table: they are read once for
- * the group, from the first one's row, or, where the table has room for 256 MB of keys and values at most, by every sequence from its own, which is less time.  Sequences of fewer keys than these pages hold are attended to by themselves.  What groups and shared_pages hold is clamped to the batch and to
+ * the group, from the first one's row, or, where the table has room for 256 MB of keys and values at most (340 with a head dimension of 128), by every sequence from its own, which is less time.  Sequences of fewer keys than these pages hold are attended to by themselves.  What groups and shared_pages hold is clamped to the batch and to
  * [0, max_pages]; where groups do not ascend outputs may be anything.
  *
  * aa_paged_evict: sequences of more than `above` keys (at least n_keys) are cut down to n_keys keys for each KV head: their first n_first, their last n_last and, of those between,

@@ -3,7 +3,8 @@ a plain step, as tests/test_paged_cache.py derives them (a probability is kept a
 import pytest
 import torch
 
-from test_paged_cache import BF16, F16, _close, _ops, _Setup
+import test_paged_conversations as conversations
+from test_paged_cache import BF16, F16, _close, _ops
 from test_paged_conversations import _int32, _shared_setup
 
 
@@ -96,3 +97,70 @@ def test_groups_of_very_different_sizes(prefixes, sizes, hq, hkv, d, dtype):
     s, shared, groups = _shared_setup(prefixes, sizes, [40, 0, 1], hkv, d, 16, dtype, 6)
     table, q = _wide_table(s), s.queries(hq)
     _close(_ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, shared, groups), q, s, d ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,hq,hkv,d,megabytes", [(16, 28, 4, 128, 272), (8, 32, 8, 128, 273), (6, 28, 4, 128, 335), (12, 14, 2, 64, 250), (1, 8, 2, 128, 1000), (1, 14, 2, 64, 500)])
+def test_batches_that_the_caches_hold_are_plain_steps(batch, hq, hkv, d, megabytes):
+    """The same bits as a plain step's, where room for all keys and values is below what makes sharing less time, or there is nobody to share with."""
+    s, shared, groups = _shared_setup([40], [batch], [30, 1], hkv, d, 64, BF16, 3)
+    pages = min(megabytes * 10 ** 6 // (batch * 64 * hkv * d * 4), (1 << 20) // 64)
+    table = torch.cat([s.table, torch.zeros(batch, pages - s.table.shape[1], dtype=torch.int32, device="cuda")], 1)
+    q = s.queries(hq)
+    want = _ops().paged_decode_attention(s.cache, q, table, s.lengths)
+    _close(want, q, s, d ** -0.5)
+    assert torch.equal(_ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, shared, groups), want)
+
+
+def test_scratch_of_what_is_not_shared():
+    """Parts of 256 work-groups, 35 MB with heads of 128, are there for the tables that may be shared only."""
+    from anchor_attn.src.ops import _hip
+    scratch = _hip.lib().aa_paged_shared_workspace_bytes
+    assert scratch(2, 8, 2, 128, 16, 8, 1) < 1 << 20 and scratch(1, 8, 2, 128, 16, 65536, 1) < 10 << 20 and scratch(8, 32, 8, 128, 64, 128, 3) < 10 << 20
+    assert scratch(12, 32, 8, 128, 64, 130, 3) > 30 << 20 and scratch(64, 14, 2, 64, 16, 1 << 12, 1) > 15 << 20
+
+
+_SHARED = next(m for m in conversations.test_shared_decode.pytestmark if m.args[0].startswith("prefixes"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize(*_SHARED.args)
+def test_shared_decode_in_wide_tables(prefixes, sizes, own, hq, hkv, d, page, layout, extra, alone, dtype):
+    s, shared, groups = _shared_setup(prefixes, sizes, own, hkv, d, page, dtype, hq + page + 1, layout, extra, alone)
+    conversations._check_shared_decode(s, _wide_table(s), shared, groups, s.queries(hq), len(sizes) == 1 and not alone)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prefixes,sizes,hq,hkv,d,page", [([60, 9], [40, 3], 32, 8, 128, 64), ([300, 0, 40], [3, 1, 2], 14, 2, 64, 16)])
+def test_captured_steps_on_two_streams(prefixes, sizes, hq, hkv, d, page):
+    """Two captured steps whose groups, pages and lengths change between the replays, on a stream each and at once: the bits of eager steps."""
+    ops, sets = _ops(), []
+    for seed in range(2):
+        s, shared, groups = _shared_setup(prefixes, sizes, [40, 0, 700], hkv, d, page, BF16, seed)
+        s.cache.keys.nan_to_num_(0.5), s.cache.values.nan_to_num_(0.5)
+        table, q, stream = _wide_table(s), s.queries(hq), torch.cuda.Stream()
+        wants = []
+        for pages, begins, fewer in ((shared, groups, 0), (shared // 2, groups, 3), (shared, torch.zeros_like(groups), 7), (shared * 0, groups, 0), (shared, groups, 100000)):
+            lengths = (s.lengths - fewer).clamp(min=0)
+            wants.append((pages.clone(), begins.clone(), lengths, ops.paged_shared_decode_attention(s.cache, q, table, lengths, pages, begins)))
+        pages, begins, lengths = shared.clone(), groups.clone(), s.lengths.clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream):
+            ops.paged_shared_decode_attention(s.cache, q, table, lengths, pages, begins)
+            stream.synchronize()
+            with torch.cuda.graph(graph, stream=stream):
+                out = ops.paged_shared_decode_attention(s.cache, q, table, lengths, pages, begins)
+        torch.cuda.synchronize()
+        # (a graph holds no reference to what it reads: the cache, the table and the queries live as long)
+        sets.append((graph, stream, out, (pages, begins, lengths), wants, (s, table, q)))
+    for i in [0, 1, 2, 3, 4, 0, 2, 1]:
+        for graph, stream, _, given, wants, _ in sets:
+            with torch.cuda.stream(stream):
+                for x, y in zip(given, wants[i]):
+                    x.copy_(y)
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, _, out, _, wants, _ in sets:
+            assert torch.equal(out, wants[i][3]), i
