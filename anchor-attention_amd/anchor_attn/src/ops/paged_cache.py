@@ -210,7 +210,7 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
     ``x / sqrt(mean(x^2) + norm_eps) * weight``, in float32 with one rounding after both.  ``positions`` int32 ``[batch]``: how many positions a sequence has had, where
     that is more than its keys (:func:`evict_from_pages`): its last token is rotated by ``positions[b] - 1``; a sequence of fewer positions than keys is left out.
     ``k_out`` ``[tokens, KV heads, D]``, which may be ``k``: the keys as they are stored, for the prompt's own attention.  The weights of new keys, in a cache that keeps them, become 0."""
-    _plain(cache, q, k, v, cos, sin, out, q_norm, k_norm, k_out)
+    _plain(cache, q, k, v, cos, sin, out)
     if not cache._apart:
         _refuse("keys, values and bounds that share memory cannot be appended to (parts of one tensor that lie between each other need the same strides)")
     k_args, (n, _, _) = _rows(k, "k", cache, cache.n_kv_heads)
@@ -245,9 +245,9 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
             if shape[0] != n:
                 _refuse(f"q has {shape[0]} tokens, k {n}")
             q_args = (*q_rows, *_out_rows(out, shape, cache)) if out is not None else (*q_rows, *_new_rows(out := torch.empty_like(q)))
-    weights = cache._weighed()
     more = None
-    if weights or not (q_norm is k_norm is positions is k_out is None):
+    if cache._weights or q_norm is not None or k_norm is not None or positions is not None or k_out is not None:  # (a step without any does no more than look)
+        _plain(cache, q_norm, k_norm, k_out)
         if cos is None and not (k_norm is positions is k_out is None):
             _refuse("norms, positions and rotated keys need cos and sin")
         if (q_norm is None) != (k_norm is None or q is None):
@@ -260,11 +260,13 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
         if not 0 <= eps <= 1:
             _refuse(f"norm_eps must be from 0 to 1, not {norm_eps}")
         more = _hip.PAGED_MORE.pack(*norms, *((0, 0, 0) if k_out is None else _out_rows(k_out, k.shape, cache, "k_out")),
-                                    0 if positions is None else _indices(positions, "positions", cache, 1, batch), weights, eps)
-    if n and batch and more is not None:
-        cache._launch(_hip.lib().aa_paged_append_more, _hip.PAGED_TOKENS.pack(*q_args, *k_args, *v_args, *angles, *tables, starts_ptr, n_positions, batch, n, heads, most), more)
-    elif n and batch:
-        cache._launch(_hip.lib().aa_paged_append, _hip.PAGED_TOKENS.pack(*q_args, *k_args, *v_args, *angles, *tables, starts_ptr, n_positions, batch, n, heads, most))
+                                    0 if positions is None else _indices(positions, "positions", cache, 1, batch), cache._weighed(), eps)
+    if n and batch:
+        tokens = _hip.PAGED_TOKENS.pack(*q_args, *k_args, *v_args, *angles, *tables, starts_ptr, n_positions, batch, n, heads, most)
+        if more is None:
+            cache._launch(_hip.lib().aa_paged_append, tokens)
+        else:
+            cache._launch(_hip.lib().aa_paged_append_more, tokens, more)
     return out
 
 
