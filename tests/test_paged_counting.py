@@ -27,3 +27,17 @@ def test_parts_whose_scores_are_all_nan(n, d, dtype):
         assert bool(s.cache.weights[at, 0].reshape(-1)[33:n].isnan().all()) and int(s.cache.weights.isnan().sum()) == n - 33, tile
         s.cache.weights[at, 0] = counted[at, 0]
         assert torch.equal(s.cache.weights, counted), tile
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lengths,hq,hkv,d", [([20001, 5], 71, 1, 64), ([3000, 9000, 0], 40, 2, 128), ([2500], 17, 1, 128)])
+def test_groups_of_more_heads_than_a_unit_where_units_are_cut(lengths, hq, hkv, d, dtype):
+    """Each block of 16 heads of a KV head has parts of its own, in groups that no power of two divides."""
+    s = _Setup(lengths, hkv, d, 32, dtype, hq, extra=3)
+    s.cache = _weights_of(s)
+    s.cache.weights.uniform_(0, 2, generator=s.g)
+    q, before = s.queries(hq), s.cache.weights.clone()
+    out = _ops().paged_weighing_decode_attention(s.cache, q, s.table, s.lengths, n_first=100)
+    assert torch.equal(out, _ops().paged_decode_attention(s.cache, q, s.table, s.lengths))
+    _weights_close(s.cache.weights, before, q, s, d ** -0.5, 100)

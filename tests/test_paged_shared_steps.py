@@ -23,6 +23,8 @@ def _wide_table(s, keys_and_values=1_000_000_000):
     ([70], [33], [20, 0, 3], 32, 8, 128, 64, "rows", [5]),
     ([600], [9], [20], 71, 1, 64, 16, "heads", []),
     ([313], [3], [2], 8, 2, 128, 64, "rows", [900]),
+    ([30], [5], [5000, 20], 71, 1, 64, 16, "heads", [3000]),
+    ([40], [4], [0, 9000], 40, 2, 128, 32, "heads", []),
 ])
 def test_shared_steps_are_as_precise_as_plain_ones(prefixes, sizes, own, hq, hkv, d, page, layout, alone, dtype):
     s, shared, groups = _shared_setup(prefixes, sizes, own, hkv, d, page, dtype, hq + page, layout, 0, alone)
@@ -164,3 +166,18 @@ def test_captured_steps_on_two_streams(prefixes, sizes, hq, hkv, d, page):
         torch.cuda.synchronize()
         for _, _, out, _, wants, _ in sets:
             assert torch.equal(out, wants[i][3]), i
+
+
+@pytest.mark.gpu
+def test_thousands_of_sequences_in_tables_for_a_million_keys():
+    """Places that count more tiles than 32 bits have: the bits of a table for half as many keys."""
+    batch, hq, hkv, d, page = 4096, 16, 8, 64, 256
+    s, shared, groups = _shared_setup([5, 0, 2], [3000, 96, 1000], [3, 0, 40], hkv, d, page, BF16, 2)
+    q, results = s.queries(hq), []
+    for keys in (1 << 19, 1 << 20):
+        table = torch.zeros(batch, keys // page, dtype=torch.int32, device="cuda")
+        table[:, :s.table.shape[1]] = s.table
+        results.append(_ops().paged_shared_decode_attention(s.cache, q, table, s.lengths, shared, groups))
+    assert torch.equal(*results)
+    plain = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
+    assert bool(((plain.float() - results[0].float()).abs() <= 2 ** -7 * plain.float().abs() + 2 ** -12).all())
