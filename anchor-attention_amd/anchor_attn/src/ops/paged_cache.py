@@ -180,12 +180,16 @@ def _plain(cache, *tensors):
     if not _called_plainly():
         _refuse("these operators cannot be traced, compiled, vmapped or watched by a mode")
     if torch.is_grad_enabled():
-        try:
-            for t in tensors:
-                if t is not None and t.requires_grad:
-                    _refuse("these operators have no gradients: detach their inputs or call them under torch.no_grad()")
-        except AttributeError:
-            pass  # (what is no tensor is refused where its type is looked at)
+        _without_gradients(*tensors)
+
+
+def _without_gradients(*tensors):
+    try:
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _refuse("these operators have no gradients: detach their inputs or call them under torch.no_grad()")
+    except AttributeError:
+        pass  # (what is no tensor is refused where its type is looked at)
 
 
 def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cos: Optional[torch.Tensor],
@@ -247,7 +251,8 @@ def append_to_pages(cache: PagedCache, q: Optional[torch.Tensor], k: torch.Tenso
             q_args = (*q_rows, *_out_rows(out, shape, cache)) if out is not None else (*q_rows, *_new_rows(out := torch.empty_like(q)))
     more = None
     if cache._weights or q_norm is not None or k_norm is not None or positions is not None or k_out is not None:  # (a step without any does no more than look)
-        _plain(cache, q_norm, k_norm, k_out)
+        if torch.is_grad_enabled():
+            _without_gradients(q_norm, k_norm, k_out)
         if cos is None and not (k_norm is positions is k_out is None):
             _refuse("norms, positions and rotated keys need cos and sin")
         if (q_norm is None) != (k_norm is None or q is None):
