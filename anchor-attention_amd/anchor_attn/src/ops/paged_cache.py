@@ -360,7 +360,7 @@ def paged_weighing_decode_attention(cache: PagedCache, q: torch.Tensor, page_tab
 def evict_from_pages(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor, n_keys: int, n_first: int = 0, n_last: int = 1,
                      above: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Cuts sequences of more than ``above`` keys (``n_keys`` if it is not given) down to ``n_keys``, for each KV head its own: the first ``n_first``, the last ``n_last``
-    and, of those between, the ones with the largest ``cache.weights``, the lower place first among equals, NaN as infinity.  They become the
+    and, of those between, the ones with the largest ``cache.weights``, the lower place first among equals (as all keys are that no step has counted, a prompt's at first), NaN as infinity.  They become the
     sequence's first ``n_keys``, in order; their weights move along, and the bounds of pages that have other keys than before are formed anew.  What keeps its place is not
     written (pages that sequences share stay as they are if ``n_first`` counts their keys), nor are rows behind the last key.  Returns the sequences' new lengths, int32
     ``[batch]``, and the places that the keys had, int32 ``[batch, KV heads, n_keys]``, ascending (-1 for sequences of which nothing is given up).  The pages behind the new lengths are the program's again;

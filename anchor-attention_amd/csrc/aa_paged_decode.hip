@@ -682,10 +682,10 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const PagedDecodeArg
 
 // Joins what is known of a unit's heads over the shared prefix and over the sequence's own keys, each whole or in parts.  256 threads have four channels of a head each; of few heads, every
 // so many of its parts.  Heads lie beside one another in a wave as they do in the parts of many rows, and fours of channels as in the others.  Bound by the latency of what it
-// reads, each thing known by the one before (cut, unit, parts): 32 sequences behind 32768 keys, 32/8 heads of 128 (256 work-groups of 32 parts) 8.6 us, of the step's 60.  (The prefix joined
+// reads, each thing known by the one before (cut, unit, parts): 32 sequences behind 32768 keys, 32/8 heads of 128 (256 work-groups of 32 parts) 9.0 us, of the step's 65.  (The prefix joined
 // by a launch of its own, before the decode kernel, which read its state: 61.3 a step.  A head's channels side by side in a wave: 9.7 us.)
 // A line of many rows' parts has heads of two sequences, which should be one XCD's: neighbours are where an XCD's share is consecutive, or, of 8 units a sequence, where each has its own
-// (128 sequences, 28/4 heads of 128, in plain order 47.8 us a step, so 46.2; 32, 32/8 of 128, 59.4 and 59.7).
+// (128 sequences, 28/4 heads of 128, in plain order 51.8 us a step, so 50.0).
 constexpr int kXcds = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_finish_kernel(const PagedDecodeArgs p) {

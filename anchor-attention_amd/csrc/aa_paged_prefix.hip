@@ -7,8 +7,8 @@
 // work-groups.  A unit that several shares have is joined in their order, so that results do not depend on timing.
 //
 // Of 16 rows a share's tiles are its eight waves', each with accumulators of its own, joined through LDS: inside a wave, as in the decode kernel, S^T = K Q^T straight from memory, P^T in
-// S^T's registers, V turned by v_perm, P as two 16-bit numbers.  It is bound by memory: 4 sequences behind 32768 keys, 32/8 heads of 128 (134 MB), in 25.7 us, the rate of a copy;
-// behind 8192 in 11.9.
+// S^T's registers, V turned by v_perm, P as two 16-bit numbers.  It is bound by memory: 4 sequences behind 32768 keys, 32/8 heads of 128 (134 MB), in 26.8 us, near the rate of a copy;
+// behind 8192 in 13.0.
 // Of 128 rows: below.
 #include <type_traits>
 
@@ -401,11 +401,13 @@ __device__ __forceinline__ void few_rows(const PagedPrefixArgs& all, const int64
 // probabilities with its values, the next one's keys with the queries), the other forms probabilities, a barrier between the halves, so that the matrix pipe has one team's work at a time and
 // the vector ALU the other's.  Tiles are requested one tile ahead.
 //
-// Measured: 32 sequences behind 32768 keys, 32/8 heads of 128, bf16 30.1 us, 134 MB at 4.5 TB/s and 17 GFLOP; 128 behind 8000, 28/4 of 128, fp16 26.8 us, 548 TFLOP/s at the 1.5 to 1.6 GHz
-// that matrix work leaves this card.  A half of a tile that multiplies takes 1300 to 1800 cycles, of which 1152 are products, one that forms probabilities 1500.
+// Measured: 32 sequences behind 32768 keys, 32/8 heads of 128, bf16 37.5 us, 134 MB at 3.6 TB/s; 128 behind 8000, 28/4 of 128, fp16 31.5 us, 467 TFLOP/s with each product counted once; 200 in
+// groups of 2 to 76 behind 600 to 24000, 32/8 of 64, bf16 40.8.  A tile's products are 1536 cycles of a wave's; the matrix pipe is busy in 39 % of the cycles of the second (a share has 14 tiles, and begins
+// and ends as long as ten take).
 // A probability enters as two 16-bit numbers, its rounding and the rest, as in the decode kernel, so that a step has the same precision however many sequences share its pages.  It costs
-// half as many products again; the listed sizes of perf/more_operators.py take 59.1, 50.7 and 66.6 us a step, 53.1, 46.6 and 60.3 with the rounding alone.  (Sums by products with ones, a
-// product more for each of the two: 59.6, 51.0, 68.5.  Exponents as the decode kernel has them, (score - m) * scale, at all scores: 58.7, 50.6 and 68.3 instead of 58.0, 50.2 and 66.8.)
+// half as many products again: these three take 58.0, 50.1 and 66.8 us a step, 53.1, 46.6 and 60.3 with the rounding alone.  (Sums by products with ones, a product more for each of
+// the two: 59.6, 51.0, 68.5.  Exponents as the decode kernel has them, (score - m) * scale, at all scores: 58.7, 50.6 and 68.3.  kMany.over, what a unit counts beside its tiles, 0, 5, 16 and 24 instead of
+// 10: 58.9, 59.4, 59.3 and 59.2 instead of 59.3, 56.9, 53.8, 52.8 and 53.0 instead of 51.5, 75.1, 65.6, 67.4 and 69.9 instead of 67.2.)
 
 template <int D>
 __device__ __forceinline__ int wide_k_swizzle(const int r) { return D == 128 ? r & 15 : (r & 7) ^ ((r >> 3) & 1); }

@@ -49,8 +49,9 @@ constexpr int kMostPages = 1 << 16;
 constexpr int kListed = 1024;      // the chosen pages up to that many pass through LDS
 constexpr int kQueryWords = 4096;  // of LDS for a group's queries; those of more heads are read from memory
 
-// A score as an unsigned number of the same order, from 1 to below kEnd - 1; NaN as infinity, -0 as 0.
+// Scores are compared as ordered() numbers them, from 1 to below kEnd - 1.
 constexpr uint32_t kEnd = 0xffffffffu;  // what stands for pages that are taken in any case; 0 stands for no page
+
 // Bounds of 8 channels of N pages, and sums of their products with queries in float64.
 //
 // WIDE: products in float64 too.  bf16 has the exponents of float32, in which a product may overflow, or lose bits below 2^-126; those of fp16 do not.  bf16 products are
