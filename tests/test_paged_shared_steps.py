@@ -181,3 +181,33 @@ def test_thousands_of_sequences_in_tables_for_a_million_keys():
     assert torch.equal(*results)
     plain = _ops().paged_decode_attention(s.cache, q, s.table, s.lengths)
     assert bool(((plain.float() - results[0].float()).abs() <= 2 ** -7 * plain.float().abs() + 2 ** -12).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("batch,hq,hkv,d,pages", [(40, 8, 2, 128, 70), (40, 8, 2, 64, 71), (3, 8, 2, 128, 33), (90, 28, 4, 128, 9)])
+def test_infinite_values_of_shared_keys(batch, hq, hkv, d, pages, dtype):
+    """Keys far below the largest (some 50 nats, where float32 has their probabilities) whose values are infinite or NaN: these channels are what 64 bits give, and the others are as close as ever."""
+    s, shared, groups = _shared_setup([pages], [batch], [20, 0], hkv, d, 16, dtype, 13)
+    s.cache.keys.mul_(0.3)
+    s.cache.keys[s.table[0, 2].long(), :, 5] *= 2.0
+    q = s.queries(hq, 1.0)
+    q[:, :, 0] = 6.0
+    s.cache.keys[s.table[0, 1].long(), :, :, 0] = -6.0
+    for slot, channel, value in ((1, 3, float("inf")), (7, 4, float("-inf")), (9, 5, float("nan")), (2, 6, float("inf")), (3, 6, float("-inf"))):
+        s.cache.values[s.table[0, 1].long(), 0, slot, channel] = value
+    out = _ops().paged_shared_decode_attention(s.cache, q, _wide_table(s), s.lengths, shared, groups, sm_scale=1.0)
+    u, group = torch.finfo(dtype).eps / 2, hq // hkv
+    for b in range(batch):
+        for h in range(hkv):
+            got, x = out[b, h * group:(h + 1) * group].double(), q[b, h * group:(h + 1) * group].double()
+            k, v = s.rows(s.cache.keys, b, h), s.rows(s.cache.values, b, h)
+            p = (x @ k.T).softmax(-1)
+            bad = ~v.isfinite().all(0)
+            assert int(bad.sum()) == (4 if h == 0 else 0) and bool((p[:, 16:32] > 2.0 ** -100).all())
+            if h == 0:
+                assert bool((got[:, 3] == float("inf")).all()) and bool((got[:, 4] == float("-inf")).all()) and bool(got[:, 5:7].isnan().all())
+            v = v.nan_to_num(0.0, 0.0, 0.0)
+            want, magnitude = p @ v, (x.abs() @ k.abs().T).amax(-1, keepdim=True)
+            bound = 1.001 * u * want.abs() + (2.0 * d * 2.0 ** -24 * magnitude + 2.0 ** -14 + u * u + k.shape[0] * 2.0 ** -24) * (p @ v.abs()) + 2.0 ** -25
+            assert bool(((got - want).abs() <= bound)[:, ~bad].all()), (b, h, float(((got - want).abs() - bound)[:, ~bad].max()))
